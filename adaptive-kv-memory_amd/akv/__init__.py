@@ -11,6 +11,17 @@ from .drop_in import AKVCache, AKVLayer, _PRESETS, recommend_preset, select_demo
 from .fused_attention import fused_int4_decode_attention, mixed_precision_decode_attention
 from .importance import ImportanceConfig, ImportanceScorer, ScoringStrategy
 from .packed_layout import PackedKVArena, PackedKVConfig, PagedKVCache
+from .paged_packed import (
+    PackedPagedCache,
+    PagedBatch,
+    PagedPool,
+    compact_pages,
+    copy_pages,
+    paged_append,
+    paged_attention,
+    paged_importance,
+    paged_read,
+)
 from .production_cache import ProductionCache, ProductionCacheConfig
 from .quantizer import KVQuantizer, QuantConfig, QuantizedTensor
 from .triton_kernels import fused_decode_attention, fused_quantize_evict
@@ -34,5 +45,7 @@ __all__ = [
     "KVQuantizer", "QuantConfig", "QuantizedTensor",
     "fused_decode_attention", "fused_quantize_evict",
     "HAS_TRITON", "fused_importance_update", "fused_mixed_precision_attention", "fused_quantized_attention",
+    "PackedPagedCache", "PagedBatch", "PagedPool", "compact_pages", "copy_pages", "paged_append", "paged_attention",
+    "paged_importance", "paged_read",
     "WarmTier", "decode_attention", "dequantize", "prefill_attention", "quantize_kv",
 ]

@@ -142,6 +142,57 @@ class KiviSide(ctypes.Structure):
     ]
 
 
+class PagedPool(ctypes.Structure):
+    _fields_ = [
+        ("data", _vp), ("n_pages", _i64), ("num_layers", _i32), ("heads", _i32), ("D", _i32), ("page_size", _i32),
+        ("group_size", _i32), ("_pad0", _i32),
+    ]
+
+
+class PagedBatch(ctypes.Structure):
+    _fields_ = [
+        ("page_table", _vp), ("kv_lens", _vp), ("q_starts", _vp), ("table_stride", _i64), ("n_tokens", _i64),
+        ("n_seqs", _i32), ("table_width", _i32), ("max_q", _i32), ("_pad0", _i32),
+    ]
+
+
+class PagedRowsArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _i32), ("layer", _i32), ("dtype", _i32), ("_pad0", _i32),
+        ("pool", PagedPool), ("batch", PagedBatch),
+        ("k", _vp), ("v", _vp), ("k_t", _i64), ("k_h", _i64), ("v_t", _i64), ("v_h", _i64),
+    ]
+
+
+class PagedAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _i32), ("layer", _i32), ("Hq", _i32), ("q_dtype", _i32), ("causal", _i32),
+        ("sm_scale", ctypes.c_float),
+        ("pool", PagedPool), ("batch", PagedBatch),
+        ("q", _vp), ("q_t", _i64), ("q_h", _i64), ("out", _vp), ("lse", _vp),
+        ("workspace", _vp), ("workspace_bytes", _i64),
+    ]
+
+
+class PagedImportanceArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _i32), ("layer", _i32), ("Hq", _i32), ("q_dtype", _i32), ("causal", _i32), ("q_window", _i32),
+        ("sm_scale", ctypes.c_float), ("decay", ctypes.c_float),
+        ("pool", PagedPool), ("batch", PagedBatch),
+        ("q", _vp), ("q_t", _i64), ("q_h", _i64), ("lse", _vp), ("scores", _vp), ("out", _vp),
+        ("n_scores", _i64), ("score_stride", _i64), ("out_stride", _i64),
+    ]
+
+
+class PagedCompactArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _i32), ("n_seqs", _i32), ("pool", PagedPool),
+        ("src_table", _vp), ("dst_table", _vp), ("src_stride", _i64), ("dst_stride", _i64),
+        ("src_width", _i32), ("dst_width", _i32), ("keep", _vp), ("n_keep", _vp),
+        ("keep_stride", _i64), ("max_keep", _i64),
+    ]
+
+
 EXPORTS = (
     "akv_abi_version", "akv_last_error", "akv_struct_size",
     "akv_decode_workspace_bytes", "akv_decode_counter_bytes", "akv_decode_attn", "akv_decode_attn_noalloc",
@@ -152,8 +203,11 @@ EXPORTS = (
     "akv_prefill_workspace_bytes", "akv_prefill_attn", "akv_select_demote", "akv_stream_read",
     "akv_rows_move", "akv_promote_select", "akv_kivi_append",
     "akv_timeline_words", "akv_timeline_fetch", "akv_timeline_clear",
+    "akv_paged_append", "akv_paged_read", "akv_paged_attn_workspace_bytes", "akv_paged_attn",
+    "akv_paged_importance", "akv_paged_copy", "akv_paged_compact",
 )
-STRUCTS = (WarmDesc, DecodeArgs, QuantArgs, DequantArgs, ImportanceArgs, PrefillArgs, RowsJob, KiviSide)
+STRUCTS = (WarmDesc, DecodeArgs, QuantArgs, DequantArgs, ImportanceArgs, PrefillArgs, RowsJob, KiviSide,
+           PagedPool, PagedBatch, PagedRowsArgs, PagedAttnArgs, PagedImportanceArgs, PagedCompactArgs)
 
 _lib: Optional[ctypes.CDLL] = None
 
@@ -220,6 +274,14 @@ def load() -> ctypes.CDLL:
     lib.akv_timeline_fetch.argtypes = [_vp, _i64]
     lib.akv_timeline_clear.restype = ctypes.c_int
     lib.akv_timeline_clear.argtypes = [_vp]
+    for name, args in (("akv_paged_append", PagedRowsArgs), ("akv_paged_read", PagedRowsArgs), ("akv_paged_attn", PagedAttnArgs),
+                       ("akv_paged_importance", PagedImportanceArgs), ("akv_paged_compact", PagedCompactArgs)):
+        getattr(lib, name).restype = ctypes.c_int
+        getattr(lib, name).argtypes = [ctypes.POINTER(args), _vp]
+    lib.akv_paged_attn_workspace_bytes.restype = _i64
+    lib.akv_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttnArgs)]
+    lib.akv_paged_copy.restype = ctypes.c_int
+    lib.akv_paged_copy.argtypes = [ctypes.POINTER(PagedPool), _vp, _vp, _i64, _vp]
     if lib.akv_abi_version() != ABI_VERSION:
         raise RuntimeError(f"{LIB_PATH} has ABI {lib.akv_abi_version()}, expected {ABI_VERSION}")
     for i, st in enumerate(STRUCTS):

@@ -11,6 +11,7 @@
 #include "kivi.h"
 #include "prefill.h"
 #include "misc.h"
+#include "paged.h"
 #include "quant.h"
 #include "rows.h"
 
@@ -313,6 +314,12 @@ int64_t akv_struct_size(int32_t which) {
         case 5: return (int64_t)sizeof(akv_prefill_args);
         case 6: return (int64_t)sizeof(akv_rows_job);
         case 7: return (int64_t)sizeof(akv_kivi_side);
+        case 8: return (int64_t)sizeof(akv_paged_pool);
+        case 9: return (int64_t)sizeof(akv_paged_batch);
+        case 10: return (int64_t)sizeof(akv_paged_rows_args);
+        case 11: return (int64_t)sizeof(akv_paged_attn_args);
+        case 12: return (int64_t)sizeof(akv_paged_importance_args);
+        case 13: return (int64_t)sizeof(akv_paged_compact_args);
         default: return -1;
     }
 }
@@ -911,6 +918,208 @@ int akv_promote_select(const float *scores, const float *previous, float *proxy,
     if (!scores || !out || (previous && !proxy)) return fail(AKV_E_INVALID, "null pointer");
     hipError_t e = akv::promote_launch(scores, previous, proxy, n, decay, fresh, threshold, cap, out, (hipStream_t)stream);
     if (e != hipSuccess) return hip_fail(e, "promote launch");
+    return ok();
+}
+
+// ------------------------------------------------------------------ paged 4-bit cache
+
+static int check_paged_pool(const akv_paged_pool &p) {
+    if (p.D != 64 && p.D != 128) return fail(AKV_E_UNSUPPORTED, "head_dim 64 or 128, got %d", p.D);
+    if ((p.group_size != 32 && p.group_size != 64 && p.group_size != 128) || p.group_size > p.D)
+        return fail(AKV_E_UNSUPPORTED, "group_size 32, 64 or 128 and at most head_dim, got %d", p.group_size);
+    if (p.page_size < 16 || p.page_size > 256 || !pow2(p.page_size))
+        return fail(AKV_E_UNSUPPORTED, "page_size a power of two from 16 to 256, got %d", p.page_size);
+    if (p.heads < 1 || p.heads > 65535 || p.num_layers < 1 || p.num_layers > 65535 || p.n_pages < 0 ||
+        p.n_pages >= ((int64_t)1 << 31))
+        return fail(AKV_E_SHAPE, "bad pool sizes");
+    if (p.n_pages > 0 && !p.data) return fail(AKV_E_INVALID, "the pool's data is NULL");
+    if (!aligned16(p.data)) return fail(AKV_E_ALIGN, "the pool must be 16-byte aligned");
+    return AKV_OK;
+}
+
+static int64_t paged_page_bytes(const akv_paged_pool &p) {
+    return (int64_t)p.heads * (p.page_size / 16) * akv::paged_tile_bytes(p.D, p.D / p.group_size);
+}
+
+static bool aligned4(const void *p) { return ((uintptr_t)p & 3u) == 0; }
+
+// The pool and batch of a call as the kernels see them.
+static int paged_views(int32_t abi, int32_t layer, const akv_paged_pool &p, const akv_paged_batch &b, akv::PagedView *v,
+                       akv::PagedSeqs *s) {
+    if (abi != AKV_ABI_VERSION) return fail(AKV_E_ABI, "ABI mismatch");
+    const int rc = check_paged_pool(p);
+    if (rc != AKV_OK) return rc;
+    if (layer < 0 || layer >= p.num_layers) return fail(AKV_E_SHAPE, "layer %d of %d", layer, p.num_layers);
+    if (b.n_seqs < 0 || b.n_seqs > 65535) return fail(AKV_E_SHAPE, "0 to 65535 sequences");
+    if (b.table_width < 0 || (b.n_seqs > 1 && b.table_stride < b.table_width)) return fail(AKV_E_SHAPE, "bad page table");
+    if (b.n_tokens < 0 || b.n_tokens >= ((int64_t)1 << 31) || b.max_q < 0) return fail(AKV_E_SHAPE, "bad row counts");
+    if ((int64_t)b.table_width * p.page_size >= ((int64_t)1 << 31)) return fail(AKV_E_SHAPE, "sequences of 2^31 tokens or more");
+    if (b.n_seqs > 0 && (!b.kv_lens || !b.q_starts || (b.table_width > 0 && !b.page_table)))
+        return fail(AKV_E_INVALID, "null pointer in the batch");
+    if (!aligned4(b.page_table) || !aligned4(b.kv_lens) || !aligned4(b.q_starts))
+        return fail(AKV_E_ALIGN, "the batch's arrays must be 4-byte aligned");
+    int log_tpp = 0;
+    while ((16 << log_tpp) < p.page_size) ++log_tpp;
+    const int64_t page = paged_page_bytes(p);
+    *v = akv::PagedView{(unsigned char *)p.data + layer * p.n_pages * page, page, (uint32_t)p.n_pages, p.heads, log_tpp};
+    *s = akv::PagedSeqs{b.page_table, b.kv_lens, b.q_starts, b.table_stride, b.n_tokens, b.n_seqs, b.table_width, b.max_q};
+    return AKV_OK;
+}
+
+static int paged_rows_params(const akv_paged_rows_args *a, akv::PagedRowsParams *p) {
+    if (!a) return fail(AKV_E_INVALID, "args is NULL");
+    const int rc = paged_views(a->abi_version, a->layer, a->pool, a->batch, &p->pool, &p->seqs);
+    if (rc != AKV_OK) return rc;
+    if (a->dtype < 0 || a->dtype > 2) return fail(AKV_E_DTYPE, "float16, bfloat16 or float32 rows");
+    if (a->batch.n_tokens > 0 && (!a->k || !a->v)) return fail(AKV_E_INVALID, "k and v are required");
+    if (!aligned16(a->k) || !aligned16(a->v) || ((a->k_t | a->k_h | a->v_t | a->v_h) & 15))
+        return fail(AKV_E_ALIGN, "rows must be 16-byte aligned");
+    p->D = a->pool.D; p->ng = a->pool.D / a->pool.group_size; p->dt = a->dtype;
+    p->k = (unsigned char *)a->k; p->v = (unsigned char *)a->v;
+    p->k_t = a->k_t; p->k_h = a->k_h; p->v_t = a->v_t; p->v_h = a->v_h;
+    return AKV_OK;
+}
+
+int akv_paged_append(const akv_paged_rows_args *a, void *stream) {
+    akv::PagedRowsParams p{};
+    const int rc = paged_rows_params(a, &p);
+    if (rc != AKV_OK) return rc;
+    hipError_t e = akv::paged_append_launch(p, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "paged append launch");
+    return ok();
+}
+
+int akv_paged_read(const akv_paged_rows_args *a, void *stream) {
+    akv::PagedRowsParams p{};
+    const int rc = paged_rows_params(a, &p);
+    if (rc != AKV_OK) return rc;
+    hipError_t e = akv::paged_read_launch(p, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "paged read launch");
+    return ok();
+}
+
+int akv_paged_copy(const akv_paged_pool *pool, const int32_t *src, const int32_t *dst, int64_t n, void *stream) {
+    if (!pool) return fail(AKV_E_INVALID, "pool is NULL");
+    const int rc = check_paged_pool(*pool);
+    if (rc != AKV_OK) return rc;
+    if (n < 0 || n > pool->n_pages) return fail(AKV_E_SHAPE, "%lld pairs in a pool of %lld pages", (long long)n, (long long)pool->n_pages);
+    if (n > 0 && (!src || !dst)) return fail(AKV_E_INVALID, "src and dst are required");
+    if (!aligned4(src) || !aligned4(dst)) return fail(AKV_E_ALIGN, "src and dst must be 4-byte aligned");
+    const akv::PagedCopyParams p{(unsigned char *)pool->data, paged_page_bytes(*pool), pool->n_pages, n, pool->num_layers, src, dst};
+    hipError_t e = akv::paged_copy_launch(p, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "paged copy launch");
+    return ok();
+}
+
+int akv_paged_compact(const akv_paged_compact_args *a, void *stream) {
+    if (!a) return fail(AKV_E_INVALID, "args is NULL");
+    if (a->abi_version != AKV_ABI_VERSION) return fail(AKV_E_ABI, "ABI mismatch");
+    const int rc = check_paged_pool(a->pool);
+    if (rc != AKV_OK) return rc;
+    if (a->n_seqs < 0 || a->n_seqs > 65535) return fail(AKV_E_SHAPE, "0 to 65535 sequences");
+    if (a->src_width < 0 || a->dst_width < 0 || a->max_keep < 0 || a->max_keep >= ((int64_t)1 << 31) ||
+        (a->n_seqs > 1 && (a->src_stride < a->src_width || a->dst_stride < a->dst_width || a->keep_stride < a->max_keep)))
+        return fail(AKV_E_SHAPE, "bad tables");
+    if ((int64_t)a->src_width * a->pool.page_size >= ((int64_t)1 << 31) ||
+        (int64_t)a->dst_width * a->pool.page_size >= ((int64_t)1 << 31))
+        return fail(AKV_E_SHAPE, "sequences of 2^31 tokens or more");
+    if (a->n_seqs > 0 && a->max_keep > 0 &&
+        (!a->keep || !a->n_keep || (a->src_width > 0 && !a->src_table) || (a->dst_width > 0 && !a->dst_table)))
+        return fail(AKV_E_INVALID, "null pointer");
+    if (!aligned4(a->src_table) || !aligned4(a->dst_table) || !aligned4(a->keep) || !aligned4(a->n_keep))
+        return fail(AKV_E_ALIGN, "tables and lists must be 4-byte aligned");
+    int log_tpp = 0;
+    while ((16 << log_tpp) < a->pool.page_size) ++log_tpp;
+    const int64_t page = paged_page_bytes(a->pool);
+    akv::PagedCompactParams p{};
+    p.pool = akv::PagedView{(unsigned char *)a->pool.data, page, (uint32_t)a->pool.n_pages, a->pool.heads, log_tpp};
+    p.layer_bytes = page * a->pool.n_pages;
+    p.layers = a->pool.num_layers; p.D = a->pool.D; p.ng = a->pool.D / a->pool.group_size; p.n_seqs = a->n_seqs;
+    p.src_table = a->src_table; p.dst_table = a->dst_table;
+    p.src_stride = a->src_stride; p.dst_stride = a->dst_stride;
+    p.src_width = a->src_width; p.dst_width = a->dst_width;
+    p.keep = a->keep; p.n_keep = a->n_keep; p.keep_stride = a->keep_stride; p.max_keep = a->max_keep;
+    hipError_t e = akv::paged_compact_launch(p, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "paged compact launch");
+    return ok();
+}
+
+// Shared by the attention and the importance.
+static int check_paged_queries(int32_t Hq, int32_t dt, float sm_scale, const akv_paged_pool &pool, const akv_paged_batch &b,
+                               const void *q, int64_t q_t, int64_t q_h) {
+    if (dt != AKV_DT_F16 && dt != AKV_DT_BF16) return fail(AKV_E_DTYPE, "float16 or bfloat16 queries");
+    if (Hq < 1 || Hq % pool.heads) return fail(AKV_E_SHAPE, "%d query heads on %d cached heads", Hq, pool.heads);
+    if (!(sm_scale > 0.0f) || !std::isfinite(sm_scale)) return fail(AKV_E_INVALID, "sm_scale must be positive");
+    if (b.n_tokens > 0 && !q) return fail(AKV_E_INVALID, "q is required");
+    if (!aligned16(q) || ((q_t | q_h) & 15)) return fail(AKV_E_ALIGN, "query rows must be 16-byte aligned");
+    if ((int64_t)b.max_q * (Hq / pool.heads) >= ((int64_t)1 << 27)) return fail(AKV_E_SHAPE, "too many rows a sequence");
+    // units of 32 tokens x heads x chunks of 16 rows are counted in 31 bits
+    const int64_t units = ((int64_t)b.table_width * pool.page_size + 31) / 32 + 1;
+    const int64_t chunks = ((int64_t)b.max_q * (Hq / pool.heads) + 15) / 16 + 1;
+    if ((double)units * b.n_seqs * pool.heads * chunks >= 1073741824.0) return fail(AKV_E_SHAPE, "too much for one call");
+    return AKV_OK;
+}
+
+static int paged_attn_params(const akv_paged_attn_args *a, akv::PagedAttnParams *p, int64_t *bytes) {
+    if (!a) return fail(AKV_E_INVALID, "args is NULL");
+    int rc = paged_views(a->abi_version, a->layer, a->pool, a->batch, &p->pool, &p->seqs);
+    if (rc != AKV_OK) return rc;
+    rc = check_paged_queries(a->Hq, a->q_dtype, a->sm_scale, a->pool, a->batch, a->q, a->q_t, a->q_h);
+    if (rc != AKV_OK) return rc;
+    p->D = a->pool.D; p->ng = a->pool.D / a->pool.group_size;
+    p->Hq = a->Hq; p->g = a->Hq / a->pool.heads;
+    p->q_bf16 = a->q_dtype == AKV_DT_BF16; p->causal = a->causal != 0;
+    p->scale_log2 = a->sm_scale * 1.4426950408889634f;
+    p->q = (const unsigned char *)a->q; p->q_t = a->q_t; p->q_h = a->q_h;
+    p->out = a->out; p->lse = a->lse; p->part = (float *)a->workspace;
+    *bytes = akv::paged_attn_plan(p);
+    return AKV_OK;
+}
+
+int64_t akv_paged_attn_workspace_bytes(const akv_paged_attn_args *a) {
+    akv::PagedAttnParams p{};
+    int64_t bytes;
+    return paged_attn_params(a, &p, &bytes) == AKV_OK ? bytes : -1;
+}
+
+int akv_paged_attn(const akv_paged_attn_args *a, void *stream) {
+    akv::PagedAttnParams p{};
+    int64_t bytes;
+    const int rc = paged_attn_params(a, &p, &bytes);
+    if (rc != AKV_OK) return rc;
+    if (a->batch.n_tokens == 0) return ok();
+    if (!a->out) return fail(AKV_E_INVALID, "out is required");
+    if (!aligned16(a->out) || !aligned4(a->lse)) return fail(AKV_E_ALIGN, "out must be 16-byte aligned");
+    if (!a->workspace || a->workspace_bytes < bytes) return fail(AKV_E_WORKSPACE, "workspace of %lld bytes needed", (long long)bytes);
+    if (!aligned16(a->workspace)) return fail(AKV_E_ALIGN, "workspace must be 16-byte aligned");
+    hipError_t e = akv::paged_attn_launch(p, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "paged attention launch");
+    return ok();
+}
+
+int akv_paged_importance(const akv_paged_importance_args *a, void *stream) {
+    if (!a) return fail(AKV_E_INVALID, "args is NULL");
+    akv::PagedImportanceParams p{};
+    int rc = paged_views(a->abi_version, a->layer, a->pool, a->batch, &p.pool, &p.seqs);
+    if (rc != AKV_OK) return rc;
+    rc = check_paged_queries(a->Hq, a->q_dtype, a->sm_scale, a->pool, a->batch, a->q, a->q_t, a->q_h);
+    if (rc != AKV_OK) return rc;
+    if (a->q_window < 0) return fail(AKV_E_SHAPE, "q_window must be >= 0");
+    if (a->n_scores < 0 || a->n_scores >= ((int64_t)1 << 31) ||
+        (a->batch.n_seqs > 1 && (a->score_stride < a->n_scores || a->out_stride < a->n_scores)))
+        return fail(AKV_E_SHAPE, "bad score rows");
+    if (a->batch.n_seqs == 0 || a->n_scores == 0) return ok();
+    if (!a->scores || !a->out || (a->batch.n_tokens > 0 && !a->lse)) return fail(AKV_E_INVALID, "scores, out and lse are required");
+    if (!aligned4(a->scores) || !aligned4(a->out) || !aligned4(a->lse)) return fail(AKV_E_ALIGN, "float32 rows must be 4-byte aligned");
+    p.D = a->pool.D; p.ng = a->pool.D / a->pool.group_size;
+    p.Hq = a->Hq; p.g = a->Hq / a->pool.heads;
+    p.q_bf16 = a->q_dtype == AKV_DT_BF16; p.causal = a->causal != 0; p.q_window = a->q_window;
+    p.scale_log2 = a->sm_scale * 1.4426950408889634f; p.decay = a->decay;
+    p.q = (const unsigned char *)a->q; p.q_t = a->q_t; p.q_h = a->q_h;
+    p.lse = a->lse; p.scores = a->scores; p.out = a->out;
+    p.n_scores = a->n_scores; p.score_stride = a->score_stride; p.out_stride = a->out_stride;
+    hipError_t e = akv::paged_importance_launch(p, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "paged importance launch");
     return ok();
 }
 

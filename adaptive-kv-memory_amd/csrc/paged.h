@@ -1,0 +1,111 @@
+// Parameter blocks and device views of the paged 4-bit cache (akv_paged_* of akv_hip.h).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "akv_hip.h"
+
+namespace akv {
+
+constexpr int kTileTok = 16;   // tokens of a tile
+constexpr int kUnitTok = 32;   // tokens a wave of the attention takes at a time: two tiles
+
+__host__ __device__ constexpr int paged_tile_bytes(int D, int ng) { return 16 * D + 128 * ng; }
+
+// One layer of a pool as a kernel sees it.
+struct PagedView {
+    unsigned char *base;       // the layer's first page
+    int64_t page_bytes;        // every head of a page
+    uint32_t n_pages;
+    int heads, log_tpp;        // log2 of the tiles a page has of one head
+};
+
+struct PagedSeqs {
+    const int32_t *table, *kv_lens, *q_starts;
+    int64_t table_stride, n_tokens;
+    int n_seqs, width, max_q;
+};
+
+struct PagedRowsParams {
+    PagedView pool;
+    PagedSeqs seqs;
+    int D, ng, dt;
+    unsigned char *k, *v;
+    int64_t k_t, k_h, v_t, v_h;
+};
+
+struct PagedAttnParams {
+    PagedView pool;
+    PagedSeqs seqs;
+    int D, ng, Hq, g;          // g = Hq / heads
+    int q_bf16, causal;
+    float scale_log2;          // sm_scale * log2(e)
+    const unsigned char *q;
+    int64_t q_t, q_h;
+    void *out;
+    float *lse;
+    float *part;               // partial states of items that several workgroups share
+    int groups;                // workgroups of the launch
+    int rows;                  // most rows of an item
+};
+
+struct PagedImportanceParams {
+    PagedView pool;
+    PagedSeqs seqs;
+    int D, ng, Hq, g;
+    int q_bf16, causal, q_window;
+    float scale_log2, decay;
+    const unsigned char *q;
+    int64_t q_t, q_h;
+    const float *lse, *scores;
+    float *out;
+    int64_t n_scores, score_stride, out_stride;
+};
+
+struct PagedCopyParams {
+    unsigned char *data;
+    int64_t page_bytes, n_pages, n;
+    int layers;
+    const int32_t *src, *dst;
+};
+
+struct PagedCompactParams {
+    PagedView pool;            // layer 0
+    int64_t layer_bytes;
+    int layers, D, ng, n_seqs;
+    const int32_t *src_table, *dst_table;
+    int64_t src_stride, dst_stride;
+    int src_width, dst_width;
+    const int32_t *keep, *n_keep;
+    int64_t keep_stride, max_keep;
+};
+
+hipError_t paged_append_launch(const PagedRowsParams &p, hipStream_t s);
+hipError_t paged_read_launch(const PagedRowsParams &p, hipStream_t s);
+hipError_t paged_copy_launch(const PagedCopyParams &p, hipStream_t s);
+hipError_t paged_compact_launch(const PagedCompactParams &p, hipStream_t s);
+// Sets p.groups and p.rows; the workspace bytes.
+int64_t paged_attn_plan(PagedAttnParams *p);
+hipError_t paged_attn_launch(const PagedAttnParams &p, hipStream_t s);
+hipError_t paged_importance_launch(const PagedImportanceParams &p, hipStream_t s);
+
+#ifdef __HIPCC__
+// Rows [begin, begin + n) of sequence s in the call's tensors, and its cached tokens.
+struct SeqRows {
+    int begin, n;
+    int64_t kv;
+};
+__device__ __forceinline__ SeqRows seq_rows(const PagedSeqs &q, int s, int log_page) {
+    const int64_t lim = q.n_tokens;
+    int64_t a = q.q_starts[s], b = q.q_starts[s + 1];
+    a = a < 0 ? 0 : a > lim ? lim : a;
+    b = b < a ? a : b > lim ? lim : b;
+    const int64_t cap = (int64_t)q.width << log_page;
+    int64_t kv = q.kv_lens[s];
+    kv = kv < 0 ? 0 : kv > cap ? cap : kv;
+    return {(int)a, (int)(b - a), kv};
+}
+#endif
+
+}  // namespace akv

@@ -1,0 +1,455 @@
+// The paged 4-bit cache's data movement: append (quantize into slots), read (values out of
+// slots), copies of whole pages and the compaction of sequences to the tokens that stay.
+// All of it is bound by memory; the tile layout is written out in akv_hip.h.
+#include "akv_common.h"
+#include "fastdiv.h"
+#include "paged.h"
+
+namespace akv {
+namespace {
+
+constexpr float kTop = 61440.0f;  // appended values are clamped to this: 15 * scale + zero stays below 65504
+
+// float64 -> float16, rounded once: the float32 between is rounded towards zero and its last
+// bit set if anything was cut off, so that the second rounding sees on which side of a tie
+// the value lies.
+__device__ __forceinline__ _Float16 round16(double d) {
+    float f = (float)d;
+    uint32_t u = __builtin_bit_cast(uint32_t, f);
+    if ((double)f != d) {
+        if (__builtin_fabs((double)f) > __builtin_fabs(d)) --u;
+        u |= 1u;
+    }
+    return (_Float16)__builtin_bit_cast(float, u);
+}
+
+// (x - z) / s rounded to the nearest whole number, ties to even, as exact arithmetic has it.
+// The float32 quotient is within 8e-6 of the true one (below 16, four roundings); where that
+// leaves the side of a border open float64 decides.
+__device__ __forceinline__ uint32_t code_of(float x, float z, float s, float inv) {
+    const float r = (x - z) * inv;
+    float c = __builtin_rintf(r);
+    if (__builtin_fabsf(__builtin_fabsf(r - c) - 0.5f) < 2e-5f)
+        c = (float)__builtin_rint(((double)x - (double)z) / (double)s);
+    return (uint32_t)__builtin_fminf(__builtin_fmaxf(c, 0.0f), 15.0f);
+}
+
+// Sequence of each lane's token t: the number of sequences that end at or before it.
+__device__ __forceinline__ int seq_of(const PagedSeqs &q, int t, bool live) {
+    const int lane = threadIdx.x & 63;
+    const int first = __builtin_amdgcn_readfirstlane(t);
+    const int last = __builtin_amdgcn_readlane(t, 63);
+    int n = 0;
+    for (int s0 = 0; s0 < q.n_seqs; s0 += 64) {
+        const int end = s0 + lane < q.n_seqs ? q.q_starts[s0 + lane + 1] : 0x7fffffff;
+        for (int tt = first; tt <= last; ++tt) {
+            const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(end <= tt));
+            if (tt == t) n += c;
+        }
+    }
+    return live && n < q.n_seqs ? n : -1;
+}
+
+// The tile and the token within it of a row of the call, or null.
+__device__ __forceinline__ unsigned char *slot_of(const PagedRowsParams &p, int t, int h, bool live, int tile_bytes,
+                                                  int *tok) {
+    const int s = seq_of(p.seqs, t, live);
+    if (s < 0) return nullptr;
+    const int log_page = p.pool.log_tpp + 4;
+    const SeqRows r = seq_rows(p.seqs, s, log_page);
+    const int64_t pos = r.kv - r.n + (t - r.begin);
+    if (t < r.begin || t >= r.begin + r.n || pos < 0) return nullptr;
+    const uint32_t page = (uint32_t)p.seqs.table[s * p.seqs.table_stride + (pos >> log_page)];
+    if (page >= p.pool.n_pages) return nullptr;
+    const int tile = (int)(pos >> 4) & ((1 << p.pool.log_tpp) - 1);
+    *tok = (int)(pos & 15);
+    return p.pool.base + page * p.pool.page_bytes + (((int64_t)h << p.pool.log_tpp) + tile) * tile_bytes;
+}
+
+template <int DT>
+__device__ __forceinline__ void load8(const unsigned char *p, float *x) {
+    if constexpr (DT == AKV_DT_F32) {
+        const f4 a = ((const f4 *)p)[0], b = ((const f4 *)p)[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+    } else {
+        const u4 a = *(const u4 *)p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t w = a[i];
+            if constexpr (DT == AKV_DT_F16) {
+                const h2 v = as_h2(w);
+                x[2 * i] = (float)v[0], x[2 * i + 1] = (float)v[1];
+            } else {
+                x[2 * i] = __builtin_bit_cast(float, w << 16);
+                x[2 * i + 1] = __builtin_bit_cast(float, w & 0xffff0000u);
+            }
+        }
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ void store8(unsigned char *p, const float *x) {
+    if constexpr (DT == AKV_DT_F32) {
+        ((f4 *)p)[0] = (f4){x[0], x[1], x[2], x[3]};
+        ((f4 *)p)[1] = (f4){x[4], x[5], x[6], x[7]};
+    } else {
+        u4 a;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (DT == AKV_DT_F16) a[i] = as_u32((h2){(_Float16)x[2 * i], (_Float16)x[2 * i + 1]});
+            else a[i] = f32_to_bf16_rne(x[2 * i]) | ((uint32_t)f32_to_bf16_rne(x[2 * i + 1]) << 16);
+        }
+        *(u4 *)p = a;
+    }
+}
+
+// Bytes (g of d[0], g of d[1], ...) of up to four dwords.
+__device__ __forceinline__ uint32_t byte_of(uint32_t d, int g) { return (d >> (8 * g)) & 255u; }
+
+// Byte offset in a tile of the 16-bit piece (quad, row, pair, half, parity) of the V codes.
+template <int D>
+__device__ __forceinline__ int v_piece(int tok, int r, int h) {
+    return 8 * D + (((tok >> 2) * 16 + r) * 2 + ((tok >> 1) & 1)) * (D / 16) + h * 4 + (tok & 1) * 2;
+}
+template <int D>
+__device__ __forceinline__ int v_meta(int tok, int grp, int ng) {
+    return 16 * D + 64 * ng + (((tok >> 2) * ng + grp) * 4 + (tok & 3)) * 2;
+}
+
+}  // namespace
+
+// A lane holds 8 channels 32 g + 8 i .. of one side of one (token, head); D / 8 lanes a side,
+// both sides next to each other.  Group minima and maxima by shuffles.  A V row's bytes are
+// dealt to 16 places of its tile, so four lanes (i of every g) transpose their 4 x 4 bytes
+// and store 16-bit pieces.  Bound by memory for prompts and by latency for a decode step.
+template <int D, int DT>
+__global__ __launch_bounds__(256) void paged_append_kernel(const PagedRowsParams p) {
+    constexpr int LN = D / 8;  // lanes a side
+    const int64_t gl = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t pair = gl / (2 * LN);
+    const int side = (int)(gl / LN) & 1, b = (int)gl & (LN - 1), g = b >> 2, i = b & 3;
+    const int64_t n_pairs = p.seqs.n_tokens * p.pool.heads;
+    const bool live = pair < n_pairs;
+    const int64_t pc = live ? pair : n_pairs - 1;
+    const int t = (int)(pc / p.pool.heads), h = (int)(pc % p.pool.heads);
+    int tok = 0;
+    const int ng = p.ng, tile_bytes = paged_tile_bytes(D, ng);
+    unsigned char *tile = slot_of(p, t, h, live, tile_bytes, &tok);
+    const unsigned char *src = side ? p.v + t * p.v_t + h * p.v_h : p.k + t * p.k_t + h * p.k_h;
+    float x[8];
+    load8<DT>(src + b * (DT == AKV_DT_F32 ? 32 : 16), x);
+    float lo = kTop, hi = -kTop;
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        bad |= !(__builtin_fabsf(x[e]) < INFINITY);
+        x[e] = __builtin_fminf(__builtin_fmaxf(x[e], -kTop), kTop);
+        lo = __builtin_fminf(lo, x[e]);
+        hi = __builtin_fmaxf(hi, x[e]);
+    }
+    const int gl_lanes = LN / ng;  // lanes of a group: 4, 8 or 16
+    int any = bad;
+    for (int m = 1; m < gl_lanes; m <<= 1) {
+        lo = __builtin_fminf(lo, __shfl_xor(lo, m));
+        hi = __builtin_fmaxf(hi, __shfl_xor(hi, m));
+        any |= __shfl_xor(any, m);
+    }
+    const _Float16 s16 = round16(((double)hi - (double)lo) / 15.0), z16 = (_Float16)lo;
+    const float s = (float)s16, z = (float)z16;
+    const bool flat = s == 0.0f || any;
+    const float inv = 1.0f / s;
+    uint32_t c[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c[e] = flat ? 0u : code_of(x[e], z, s, inv);
+    const uint16_t sb = any ? 0x7e00 : __builtin_bit_cast(uint16_t, s16);
+    const uint16_t zb = any ? 0x7e00 : __builtin_bit_cast(uint16_t, z16);
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w |= c[e] << (4 * e);
+    uint32_t d[4];
+#pragma unroll
+    for (int q = 0; q < D / 32; ++q) d[q] = __shfl(w, (threadIdx.x & 63 & ~(LN - 1)) + 4 * q + i);
+    if (!tile) return;
+    const int grp = g * 32 / (D / ng);
+    const bool lead = b % gl_lanes == 0;
+    if (side == 0) {
+        *(uint32_t *)(tile + tok * (D / 2) + (i * (D / 32) + g) * 4) = w;
+        if (lead) *(uint32_t *)(tile + 16 * D + (tok * ng + grp) * 4) = sb | ((uint32_t)zb << 16);
+    } else {
+        if constexpr (D == 128) {
+            const int r = 4 * i + g;
+            *(uint16_t *)(tile + v_piece<D>(tok, r, 0)) = byte_of(d[0], g) | (byte_of(d[1], g) << 8);
+            *(uint16_t *)(tile + v_piece<D>(tok, r, 1)) = byte_of(d[2], g) | (byte_of(d[3], g) << 8);
+        } else {
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                const int k = 2 * g + m;
+                *(uint16_t *)(tile + v_piece<D>(tok, 4 * i + k, 0)) = byte_of(d[0], k) | (byte_of(d[1], k) << 8);
+            }
+        }
+        if (lead) {
+            *(uint16_t *)(tile + v_meta<D>(tok, grp, ng)) = sb;
+            *(uint16_t *)(tile + v_meta<D>(tok, grp, ng) + 32 * ng) = zb;
+        }
+    }
+}
+
+// The append's lanes, the other way round.
+template <int D, int DT>
+__global__ __launch_bounds__(256) void paged_read_kernel(const PagedRowsParams p) {
+    constexpr int LN = D / 8;
+    const int64_t gl = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t pair = gl / (2 * LN);
+    const int side = (int)(gl / LN) & 1, b = (int)gl & (LN - 1), g = b >> 2, i = b & 3;
+    const int64_t n_pairs = p.seqs.n_tokens * p.pool.heads;
+    const bool live = pair < n_pairs;
+    const int64_t pc = live ? pair : n_pairs - 1;
+    const int t = (int)(pc / p.pool.heads), h = (int)(pc % p.pool.heads);
+    int tok = 0;
+    const int ng = p.ng, tile_bytes = paged_tile_bytes(D, ng);
+    const unsigned char *tile = slot_of(p, t, h, live, tile_bytes, &tok);
+    const int grp = g * 32 / (D / ng);
+    uint32_t w = 0;
+    uint16_t sb = 0, zb = 0;
+    if (tile) {
+        if (side == 0) {
+            w = *(const uint32_t *)(tile + tok * (D / 2) + (i * (D / 32) + g) * 4);
+            const uint32_t m = *(const uint32_t *)(tile + 16 * D + (tok * ng + grp) * 4);
+            sb = (uint16_t)m, zb = (uint16_t)(m >> 16);
+        } else {
+            // bytes g of row r = 4 i + g (D = 128) or of rows 4 i + 2 g, + 1 (D = 64)
+            if constexpr (D == 128)
+                w = *(const uint16_t *)(tile + v_piece<D>(tok, 4 * i + g, 0)) |
+                    ((uint32_t)*(const uint16_t *)(tile + v_piece<D>(tok, 4 * i + g, 1)) << 16);
+            else
+                w = *(const uint16_t *)(tile + v_piece<D>(tok, 4 * i + 2 * g, 0)) |
+                    ((uint32_t)*(const uint16_t *)(tile + v_piece<D>(tok, 4 * i + 2 * g + 1, 0)) << 16);
+            sb = *(const uint16_t *)(tile + v_meta<D>(tok, grp, ng));
+            zb = *(const uint16_t *)(tile + v_meta<D>(tok, grp, ng) + 32 * ng);
+        }
+    }
+    uint32_t d[4];
+#pragma unroll
+    for (int q = 0; q < D / 32; ++q) d[q] = __shfl(w, (threadIdx.x & 63 & ~(LN - 1)) + 4 * q + i);
+    if (side == 1) {
+        if constexpr (D == 128)  // row 4 i + q has this lane's group in byte g
+            w = byte_of(d[0], g) | (byte_of(d[1], g) << 8) | (byte_of(d[2], g) << 16) | (byte_of(d[3], g) << 24);
+        else                     // rows 4 i + 2 q, + 1 of lane q: this lane's group in bytes g and 2 + g
+            w = byte_of(d[0], g) | (byte_of(d[0], 2 + g) << 8) | (byte_of(d[1], g) << 16) | (byte_of(d[1], 2 + g) << 24);
+    }
+    if (!live) return;
+    const float s = (float)__builtin_bit_cast(_Float16, sb), z = (float)__builtin_bit_cast(_Float16, zb);
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = __builtin_fmaf((float)((w >> (4 * e)) & 15u), s, z);
+    unsigned char *dst = side ? p.v + t * p.v_t + h * p.v_h : p.k + t * p.k_t + h * p.k_h;
+    store8<DT>(dst + b * (DT == AKV_DT_F32 ? 32 : 16), x);
+}
+
+// 16-byte pieces of the pages of all pairs and layers, four a thread; bound by memory.
+__global__ __launch_bounds__(256) void paged_copy_kernel(const PagedCopyParams p) {
+    const int64_t per = p.page_bytes >> 4;  // pieces a page
+    const int64_t total = per * p.n * p.layers;
+    u4 v[4];
+    u4 *to[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int64_t u = ((int64_t)blockIdx.x * 4 + k) * 256 + threadIdx.x;
+        to[k] = nullptr;
+        if (u < total) {
+            const int64_t page = u / per, off = u - page * per;
+            const int64_t layer = page / p.n, i = page - layer * p.n;
+            const uint32_t a = (uint32_t)p.src[i], b = (uint32_t)p.dst[i];
+            if (a < p.n_pages && b < p.n_pages && a != b) {
+                unsigned char *base = p.data + layer * p.n_pages * p.page_bytes;
+                v[k] = ((const u4 *)(base + a * p.page_bytes))[off];
+                to[k] = (u4 *)(base + b * p.page_bytes) + off;
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (to[k]) *to[k] = v[k];
+}
+
+// One wave a tile of the destination: its 16 rows come from up to 16 tiles.  Lane (row t of
+// the tile, i) of the K codes, lane (quad a, row r) of the V codes as they are stored; whole
+// tiles leave in 16-byte stores, the last one of a sequence row by row.
+template <int D, int NG>
+__global__ __launch_bounds__(256) void paged_compact_kernel(const PagedCompactParams p) {
+    constexpr int TB = paged_tile_bytes(D, NG), VW = D / 64;  // dwords a token pair of a V row
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int H = p.pool.heads;
+    // z: layer, y: sequence, x: (tile of the longest row, head), heads next to each other
+    const int layer = blockIdx.z, s = blockIdx.y;
+    const int64_t x = (int64_t)blockIdx.x * 4 + wave;
+    const int64_t tile_no = x / H;
+    const int h = (int)(x - tile_no * H);
+    const int log_page = p.pool.log_tpp + 4;
+    int64_t n = p.n_keep[s];
+    const int64_t cap = (int64_t)p.dst_width << log_page;
+    n = n > p.max_keep ? p.max_keep : n;
+    n = n > cap ? cap : n;
+    const int64_t j0 = tile_no * 16;
+    if (j0 >= n) return;
+    unsigned char *base = p.pool.base + layer * p.layer_bytes;
+    const uint32_t dpage = (uint32_t)p.dst_table[s * p.dst_stride + (j0 >> log_page)];
+    if (dpage >= p.pool.n_pages) return;
+    const int in_page = (1 << p.pool.log_tpp) - 1;
+    unsigned char *dst = base + dpage * p.pool.page_bytes +
+                         (((int64_t)h << p.pool.log_tpp) + ((int)tile_no & in_page)) * TB;
+    // lane & 15: a row of the tile; its place in the source as a byte offset, -1 if it has none
+    const int row = lane & 15;
+    int64_t from = -1;
+    if (j0 + row < n) {
+        const int64_t pos = p.keep[s * p.keep_stride + j0 + row];
+        if (pos >= 0 && pos < ((int64_t)p.src_width << log_page)) {
+            const uint32_t page = (uint32_t)p.src_table[s * p.src_stride + (pos >> log_page)];
+            if (page < p.pool.n_pages)
+                from = (page * p.pool.page_bytes + (((int64_t)h << p.pool.log_tpp) + ((int)(pos >> 4) & in_page)) * TB) * 16 +
+                       (pos & 15);
+        }
+    }
+    const bool whole = __builtin_amdgcn_ballot_w64(from >= 0) == ~0ull;
+    auto tile_of = [&](int t) { return base + (__shfl(from, t) >> 4); };
+    auto tok_of = [&](int t) { return (int)(__shfl(from, t) & 15); };
+    // every lane takes part in the shuffles; rows without a source read the tile they would go to
+    if (from < 0) from = (int64_t)(dst - base) * 16 + row;
+    const bool mine = !(from >= 0 && (base + (from >> 4)) == dst && (from & 15) == row);  // not in its place already
+    if (!__builtin_amdgcn_ballot_w64(mine)) return;
+    const int kt = lane >> 2, ki = lane & 3;  // K codes: token, quarter row
+    const unsigned char *ksrc = tile_of(kt) + tok_of(kt) * (D / 2) + ki * (D / 8);
+    const int a = lane >> 4, r = lane & 15;
+    const unsigned char *vsrc[4];
+    int par[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int tk = tok_of(4 * a + j);
+        vsrc[j] = tile_of(4 * a + j) + 8 * D + (((tk >> 2) * 16 + r) * 2 + ((tk >> 1) & 1)) * (D / 16);
+        par[j] = (tk & 1) * 16;
+    }
+    // meta: lane (token mt, group mg), NG groups a token
+    const int mt = (lane / NG) & 15, mg = lane % NG;
+    const unsigned char *mtile = tile_of(mt);
+    const int mtok = tok_of(mt);
+    const uint32_t km = *(const uint32_t *)(mtile + 16 * D + (mtok * NG + mg) * 4);
+    const unsigned char *vm = mtile + 16 * D + 64 * NG + (((mtok >> 2) * NG + mg) * 4 + (mtok & 3)) * 2;
+    const uint16_t vs = *(const uint16_t *)vm, vz = *(const uint16_t *)(vm + 32 * NG);
+    uint32_t kc[D / 32];
+    uint32_t vq[4][VW];
+    if constexpr (D == 128) {
+        const u4 x4 = *(const u4 *)ksrc;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) kc[e] = x4[e];
+    } else {
+        const u2 x2 = *(const u2 *)ksrc;
+        kc[0] = x2[0], kc[1] = x2[1];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (VW == 2) {
+            const u2 x2 = *(const u2 *)vsrc[j];
+            vq[j][0] = x2[0] >> par[j], vq[j][1] = x2[1] >> par[j];
+        } else {
+            vq[j][0] = *(const uint32_t *)vsrc[j] >> par[j];
+        }
+    }
+    const bool meta_lane = lane < 16 * NG;
+    if (whole) {
+        if constexpr (D == 128) {
+            *(u4 *)(dst + lane * 16) = (u4){kc[0], kc[1], kc[2], kc[3]};
+            u4 o;
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) o[2 * q + w] = (vq[2 * q][w] & 0xffffu) | (vq[2 * q + 1][w] << 16);
+            *(u4 *)(dst + 8 * D + lane * 16) = o;
+        } else {
+            *(u2 *)(dst + lane * 8) = (u2){kc[0], kc[1]};
+            *(u2 *)(dst + 8 * D + lane * 8) = (u2){(vq[0][0] & 0xffffu) | (vq[1][0] << 16), (vq[2][0] & 0xffffu) | (vq[3][0] << 16)};
+        }
+    } else {
+        const uint64_t ok = __builtin_amdgcn_ballot_w64(mine);  // lanes 0-15: the rows to write
+        if ((ok >> kt) & 1) {
+            if constexpr (D == 128) *(u4 *)(dst + lane * 16) = (u4){kc[0], kc[1], kc[2], kc[3]};
+            else *(u2 *)(dst + lane * 8) = (u2){kc[0], kc[1]};
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if ((ok >> (4 * a + j)) & 1) {
+#pragma unroll
+                for (int w = 0; w < VW; ++w)
+                    *(uint16_t *)(dst + 8 * D + ((a * 16 + r) * 2 + (j >> 1)) * (D / 16) + w * 4 + (j & 1) * 2) = (uint16_t)vq[j][w];
+            }
+        if (!((ok >> mt) & 1)) return;
+    }
+    if (meta_lane) {
+        *(uint32_t *)(dst + 16 * D + (mt * NG + mg) * 4) = km;
+        unsigned char *o = dst + 16 * D + 64 * NG + (((mt >> 2) * NG + mg) * 4 + (mt & 3)) * 2;
+        *(uint16_t *)o = vs;
+        *(uint16_t *)(o + 32 * NG) = vz;
+    }
+}
+
+namespace {
+
+template <template <int, int> class K>
+hipError_t rows_launch(const PagedRowsParams &p, hipStream_t s) {
+    const int64_t lanes = p.seqs.n_tokens * p.pool.heads * (p.D / 4);
+    if (lanes == 0 || p.seqs.n_seqs == 0) return hipSuccess;
+    const int64_t blocks = (lanes + 255) / 256;
+    if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+    auto go = [&](auto kern) { kern<<<dim3((unsigned)blocks), dim3(256), 0, s>>>(p); };
+    if (p.D == 128) {
+        if (p.dt == AKV_DT_F16) go(K<128, AKV_DT_F16>::fn);
+        else if (p.dt == AKV_DT_BF16) go(K<128, AKV_DT_BF16>::fn);
+        else go(K<128, AKV_DT_F32>::fn);
+    } else {
+        if (p.dt == AKV_DT_F16) go(K<64, AKV_DT_F16>::fn);
+        else if (p.dt == AKV_DT_BF16) go(K<64, AKV_DT_BF16>::fn);
+        else go(K<64, AKV_DT_F32>::fn);
+    }
+    return hipGetLastError();
+}
+template <int D, int DT>
+struct AppendK {
+    static constexpr auto fn = paged_append_kernel<D, DT>;
+};
+template <int D, int DT>
+struct ReadK {
+    static constexpr auto fn = paged_read_kernel<D, DT>;
+};
+
+}  // namespace
+
+hipError_t paged_append_launch(const PagedRowsParams &p, hipStream_t s) { return rows_launch<AppendK>(p, s); }
+hipError_t paged_read_launch(const PagedRowsParams &p, hipStream_t s) { return rows_launch<ReadK>(p, s); }
+
+hipError_t paged_copy_launch(const PagedCopyParams &p, hipStream_t s) {
+    const int64_t pieces = (p.page_bytes >> 4) * p.n * p.layers;
+    if (pieces == 0) return hipSuccess;
+    const int64_t blocks = (pieces + 1023) / 1024;
+    if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+    paged_copy_kernel<<<dim3((unsigned)blocks), dim3(256), 0, s>>>(p);
+    return hipGetLastError();
+}
+
+hipError_t paged_compact_launch(const PagedCompactParams &p, hipStream_t s) {
+    const int64_t tiles = (p.max_keep + 15) / 16;
+    if (tiles == 0 || p.n_seqs == 0 || p.layers == 0) return hipSuccess;
+    const int64_t bx = (tiles * p.pool.heads + 3) / 4;
+    if (bx > 0x7fffffff) return hipErrorInvalidConfiguration;
+    const dim3 grid((unsigned)bx, (unsigned)p.n_seqs, (unsigned)p.layers), block(256);
+    if (p.D == 128) {
+        if (p.ng == 4) paged_compact_kernel<128, 4><<<grid, block, 0, s>>>(p);
+        else if (p.ng == 2) paged_compact_kernel<128, 2><<<grid, block, 0, s>>>(p);
+        else paged_compact_kernel<128, 1><<<grid, block, 0, s>>>(p);
+    } else {
+        if (p.ng == 2) paged_compact_kernel<64, 2><<<grid, block, 0, s>>>(p);
+        else paged_compact_kernel<64, 1><<<grid, block, 0, s>>>(p);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace akv

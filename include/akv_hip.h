@@ -343,7 +343,9 @@ int akv_abi_version(void);
 const char *akv_last_error(void);
 /* sizeof of the args structs, for bindings that mirror them (ctypes, cgo):
  * 0 akv_warm_desc, 1 akv_decode_args, 2 akv_quant_args, 3 akv_dequant_args,
- * 4 akv_importance_args, 5 akv_prefill_args, 6 akv_rows_job, 7 akv_kivi_side; -1 for an unknown id. */
+ * 4 akv_importance_args, 5 akv_prefill_args, 6 akv_rows_job, 7 akv_kivi_side, 8 akv_paged_pool,
+ * 9 akv_paged_batch, 10 akv_paged_rows_args, 11 akv_paged_attn_args, 12 akv_paged_importance_args,
+ * 13 akv_paged_compact_args; -1 for an unknown id. */
 int64_t akv_struct_size(int32_t which);
 /* A measurement helper with no counterpart in the reference: reads `bytes` (a multiple of
  * 16, 16-byte aligned) once with 16-byte non-temporal loads, as fast as a read-once kernel
@@ -424,6 +426,135 @@ int akv_kivi_append(const akv_kivi_side *sides, int32_t n_sides, int32_t B, int3
  * are above it. */
 int akv_promote_select(const float *scores, const float *previous, float *proxy, int64_t n, float decay, float fresh,
                        float threshold, int64_t cap, int64_t *out, void *stream);
+
+/* ------------------------------------------------------------- paged 4-bit cache */
+
+/* A pool of 4-bit pages: data [num_layers][n_pages][heads][page_size / 16][tile] bytes.  A
+ * page holds page_size token slots of every head; a tile is 16 of them of one head, in
+ * 16 D + 128 NG bytes with NG = D / group_size (integer codes c, values c * scale + zero):
+ *   K codes 8 D bytes:  nibble n of dword (t, i, g), the low one first, is channel
+ *                       32 g + 8 i + n of token t (t < 16, i < 4, g < D / 32);
+ *   V codes 8 D bytes:  nibble b of byte (a, r, p, h, e, l) is channel 32 (2 h + l) + 2 r + b
+ *                       of token 4 a + 2 p + e (a < 4, r < 16, h < D / 64; p, e, l, b < 2);
+ *   K meta 64 NG bytes: float16 (scale, zero) of (t, channel group);
+ *   V meta 64 NG bytes: float16 scales (a, channel group, p, e), then the zeros alike. */
+typedef struct akv_paged_pool {
+    void *data;            /* 16-byte aligned */
+    int64_t n_pages;
+    int32_t num_layers, heads;
+    int32_t D;             /* 64 or 128 */
+    int32_t page_size;     /* a power of two, 16 to 256 */
+    int32_t group_size;    /* 32, 64 or 128, at most D */
+    int32_t _pad0;
+} akv_paged_pool;
+
+/* Sequences of a call.  Sequence s has kv_lens[s] cached tokens, token j of it in slot
+ * j % page_size of page page_table[s][j / page_size]; its q_starts[s + 1] - q_starts[s] newest
+ * ones are this call's, rows q_starts[s].. of the call's (n_tokens, heads, D) tensors.  The
+ * arrays are device memory (4-byte aligned) and are read when the work runs, so a captured
+ * call follows them.  q_starts ascends from 0; lengths past the table count as its end, and
+ * slots on pages outside the pool are not written and hold no token. */
+typedef struct akv_paged_batch {
+    const int32_t *page_table; /* [n_seqs] rows of table_width entries, table_stride apart */
+    const int32_t *kv_lens;    /* [n_seqs] */
+    const int32_t *q_starts;   /* [n_seqs + 1] */
+    int64_t table_stride;
+    int64_t n_tokens;
+    int32_t n_seqs, table_width;
+    int32_t max_q;         /* no sequence has more rows than this in the call */
+    int32_t _pad0;
+} akv_paged_batch;
+
+typedef struct akv_paged_rows_args {
+    int32_t abi_version;
+    int32_t layer;
+    int32_t dtype;         /* AKV_DT_* of k and v */
+    int32_t _pad0;
+    akv_paged_pool pool;
+    akv_paged_batch batch;
+    void *k, *v;           /* (n_tokens, heads, D), channels contiguous */
+    int64_t k_t, k_h, v_t, v_h; /* byte strides of token and head, multiples of 16 */
+} akv_paged_rows_args;
+
+/* Quantize the call's rows into their slots.  Per token, head and group of channels, over
+ * the values clamped to +-61440: scale = (max - min) / 15 and zero = min, each rounded to
+ * float16 once; code = (x - zero) / scale rounded to the nearest, ties to even, within
+ * 0..15 (0 where scale is 0).  A group that holds a value that is not finite gets NaN for
+ * both, and reads back as NaN. */
+int akv_paged_append(const akv_paged_rows_args *args, void *stream);
+/* The values of the call's rows as the cache holds them (code * scale + zero, rounded to
+ * dtype) into k and v; rows without a slot become 0. */
+int akv_paged_read(const akv_paged_rows_args *args, void *stream);
+
+typedef struct akv_paged_attn_args {
+    int32_t abi_version;
+    int32_t layer;
+    int32_t Hq;            /* a multiple of the pool's heads */
+    int32_t q_dtype;       /* AKV_DT_F16 or AKV_DT_BF16 */
+    int32_t causal;        /* 1: row i of m sees tokens 0 .. kv_len - m + i; 0: every token */
+    float sm_scale;        /* > 0 */
+    akv_paged_pool pool;
+    akv_paged_batch batch;
+    const void *q;         /* (n_tokens, Hq, D), channels contiguous */
+    int64_t q_t, q_h;      /* byte strides of token and head, multiples of 16 */
+    void *out;             /* (n_tokens, Hq, D) contiguous, q dtype */
+    float *lse;            /* optional (n_tokens, Hq): log sum exp(sm_scale q.k) */
+    void *workspace;       /* akv_paged_attn_workspace_bytes() bytes, no initial value needed */
+    int64_t workspace_bytes;
+} akv_paged_attn_args;
+
+/* Attention of the call's rows over their sequences' cached tokens; query head h reads
+ * cached head h / (Hq / heads).  Rows that see no token: 0, and -inf in lse.  Calls that
+ * share a workspace must not overlap. */
+int64_t akv_paged_attn_workspace_bytes(const akv_paged_attn_args *args);
+int akv_paged_attn(const akv_paged_attn_args *args, void *stream);
+
+typedef struct akv_paged_importance_args {
+    int32_t abi_version;
+    int32_t layer;
+    int32_t Hq;
+    int32_t q_dtype;       /* AKV_DT_F16 or AKV_DT_BF16 */
+    int32_t causal;
+    int32_t q_window;      /* > 0: only a sequence's last q_window rows count */
+    float sm_scale, decay;
+    akv_paged_pool pool;
+    akv_paged_batch batch;
+    const void *q;
+    int64_t q_t, q_h;
+    const float *lse;      /* (n_tokens, Hq) of akv_paged_attn */
+    const float *scores;   /* [n_seqs] rows of n_scores, score_stride apart */
+    float *out;            /* likewise, out_stride apart; may be scores */
+    int64_t n_scores, score_stride, out_stride;
+} akv_paged_importance_args;
+
+/* out[s][j] = scores[s][j] * decay + sum over rows of the mean over heads of
+ * exp(sm_scale q.k_j - lse), for the first min(kv_len, n_scores) tokens of every sequence that
+ * has rows in the call; other entries are copied (left alone where out is scores). */
+int akv_paged_importance(const akv_paged_importance_args *args, void *stream);
+
+/* Page dst[i] of every layer becomes a copy of page src[i], i < n (n int32 each on the
+ * device).  No page may be written twice, or both read and written; pairs with a page
+ * outside the pool are skipped. */
+int akv_paged_copy(const akv_paged_pool *pool, const int32_t *src, const int32_t *dst, int64_t n, void *stream);
+
+typedef struct akv_paged_compact_args {
+    int32_t abi_version;
+    int32_t n_seqs;
+    akv_paged_pool pool;
+    const int32_t *src_table, *dst_table; /* [n_seqs] rows */
+    int64_t src_stride, dst_stride;
+    int32_t src_width, dst_width;
+    const int32_t *keep;   /* [n_seqs] rows of max_keep positions, keep_stride apart */
+    const int32_t *n_keep; /* [n_seqs] */
+    int64_t keep_stride;
+    int64_t max_keep;
+} akv_paged_compact_args;
+
+/* Token j of sequence s on its dst_table becomes token keep[s][j] on its src_table, j <
+ * min(n_keep[s], max_keep), in every layer and head.  No slot that is read may be written,
+ * except tokens that stay in their slot.  Slots behind the last token keep what they hold;
+ * tokens whose position or page is out of range are skipped. */
+int akv_paged_compact(const akv_paged_compact_args *args, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,223 @@
+"""The paged 4-bit cache's books and refusals, on the host."""
+import ctypes
+import random
+
+import numpy as np
+import pytest
+import torch
+
+import paged_ref as ref
+
+
+@pytest.mark.parametrize("D,G", [(128, 32), (128, 64), (128, 128), (64, 32), (64, 64)])
+def test_every_byte_of_a_tile_has_one_use(D, G):
+    seen = np.zeros((ref.tile_bytes(D, G), 2), int)
+    for at, sh, sa, za in ref.places(D, G):
+        np.add.at(seen, (at.ravel(), sh.ravel() // 4), 1)
+        for x in (sa, sa + 1, za, za + 1):
+            np.add.at(seen, (x.ravel(), 0), 1)
+            np.add.at(seen, (x.ravel(), 1), 1)
+    assert (seen == 1).all()
+
+
+def _whole(book):
+    """Every page is free once or held by exactly as many sequences as it counts."""
+    held = {}
+    for pages in book.pages.values():
+        for p in pages:
+            held[p] = held.get(p, 0) + 1
+    assert len(set(book.free)) == len(book.free) and not set(book.free) & set(held)
+    assert len(book.free) + len(held) == len(book.refs)
+    assert all(book.refs[p] == held.get(p, 0) for p in range(len(book.refs)))
+    for s, pages in book.pages.items():
+        assert len(pages) == -(-book.lens[s] // book.page_size)
+
+
+def test_ledger_copy_on_write():
+    from akv.paged_packed import PageLedger
+    book = PageLedger(10, 16)
+    a = book.add()
+    assert book.extend([a], [20]) == []
+    b, c = book.fork(a), book.fork(a)
+    last = book.pages[a][1]
+    copies = book.extend([a, b, c], [1, 1, 0])
+    # a and b get pages of their own; c, which does not write, keeps the old one
+    assert [x for x, _ in copies] == [last, last] and book.pages[c][1] == last
+    assert len({book.pages[s][1] for s in (a, b, c)}) == 3 and len({book.pages[s][0] for s in (a, b, c)}) == 1
+    assert book.extend([c], [1]) == []       # alone on it now
+    _whole(book)
+    d = book.fork(a)
+    book.crop(d, 16)                          # at a page's end: nothing shared is written
+    assert book.extend([d], [1]) == []
+    e = book.fork(d)
+    assert [x for x, _ in book.extend([d, e], [1, 1])] == [book.pages[e][1]]  # the second one writes in place
+    _whole(book)
+
+
+def test_ledger_refuses_whole():
+    from akv.paged_packed import PageLedger
+    book = PageLedger(4, 16)
+    a, b = book.add(), book.add()
+    book.extend([a, b], [17, 1])
+    before = (list(book.free), dict(book.lens), [list(p) for p in book.pages.values()])
+    for seqs, n, err in (([a, b], [16, 32], RuntimeError), ([a, a], [1, 1], ValueError), ([9], [1], ValueError),
+                         ([a], [-1], ValueError), ([a, b], [1], ValueError)):
+        with pytest.raises(err):
+            book.extend(seqs, n)
+    with pytest.raises(ValueError):
+        book.plan_compaction([a], [18])
+    c = book.fork(a)
+    book.extend([b], [15])
+    with pytest.raises(RuntimeError):
+        book.plan_compaction([a], [17])      # one free page, and the old ones are shared
+    book.remove(c)
+    book.crop(b, 1)
+    assert before == (list(book.free), dict(book.lens), [list(p) for p in book.pages.values()])
+    _whole(book)
+
+
+def test_ledger_at_random():
+    from akv.paged_packed import PageLedger
+    rng = random.Random(3)
+    book = PageLedger(60, 16)
+    for _ in range(3000):
+        live = list(book.pages)
+        op = rng.choice(["add", "fork", "extend", "extend", "crop", "remove", "compact"])
+        if op == "add" or not live:
+            book.add()
+        elif op == "fork":
+            book.fork(rng.choice(live))
+        elif op == "remove" and len(live) > 6:
+            book.remove(rng.choice(live))
+        elif op == "crop":
+            s = rng.choice(live)
+            n = rng.randint(-50, 80)
+            want = max(0, min(n if n >= 0 else n + book.lens[s], book.lens[s]))
+            book.crop(s, n)
+            assert book.lens[s] == want
+        else:
+            some = rng.sample(live, rng.randint(1, min(4, len(live))))
+            try:
+                if op == "extend":
+                    n = [rng.randint(0, 40) for _ in some]
+                    old = [book.lens[s] for s in some]
+                    copies = book.extend(some, n)
+                    assert len({b for _, b in copies}) == len(copies) and not {a for a, _ in copies} & {b for _, b in copies}
+                    assert [book.lens[s] for s in some] == [a + b for a, b in zip(old, n)]
+                    for s, o, c in zip(some, old, n):
+                        assert all(book.refs[p] == 1 for p in book.pages[s][o // 16:]) or c == 0
+                else:
+                    n = [rng.randint(0, book.lens[s]) for s in some]
+                    groups = book.plan_compaction(some, n)
+                    assert sorted(i for g in groups for i in g) == list(range(len(some)))
+                    for g in groups:
+                        moved = [book.replace(some[i], n[i]) for i in g]
+                        assert not {p for a, _ in moved for p in a} & {p for _, b in moved for p in b}
+                        for a, _ in moved:
+                            book._drop(a)
+            except RuntimeError:
+                pass
+        _whole(book)
+
+
+# ------------------------------------------------------------------ refusals
+
+
+def _pool(nat, **kw):
+    d = dict(data=4096, n_pages=4, num_layers=2, heads=2, D=128, page_size=16, group_size=32)
+    d.update(kw)
+    return nat.PagedPool(**d)
+
+
+def _batch(nat, **kw):
+    d = dict(page_table=4096, kv_lens=4096, q_starts=4096, table_stride=4, n_tokens=3, n_seqs=2, table_width=4, max_q=2)
+    d.update(kw)
+    return nat.PagedBatch(**d)
+
+
+POOLS = [(dict(D=96), "E_UNSUPPORTED"), (dict(group_size=16), "E_UNSUPPORTED"), (dict(D=64, group_size=128), "E_UNSUPPORTED"),
+         (dict(page_size=8), "E_UNSUPPORTED"), (dict(page_size=48), "E_UNSUPPORTED"), (dict(page_size=512), "E_UNSUPPORTED"),
+         (dict(heads=0), "E_SHAPE"), (dict(num_layers=0), "E_SHAPE"), (dict(n_pages=-1), "E_SHAPE"),
+         (dict(data=0), "E_INVALID"), (dict(data=8), "E_ALIGN")]
+BATCHES = [(dict(n_seqs=-1), "E_SHAPE"), (dict(n_seqs=65536), "E_SHAPE"), (dict(table_stride=3), "E_SHAPE"),
+           (dict(table_width=-1), "E_SHAPE"), (dict(n_tokens=-1), "E_SHAPE"), (dict(max_q=-1), "E_SHAPE"),
+           (dict(table_width=2 ** 27, table_stride=2 ** 27), "E_SHAPE"), (dict(kv_lens=0), "E_INVALID"),
+           (dict(q_starts=0), "E_INVALID"), (dict(page_table=0), "E_INVALID"), (dict(kv_lens=4098), "E_ALIGN")]
+
+
+@pytest.mark.parametrize("call", ["rows", "attn", "importance"])
+def test_c_refusals(call):
+    from akv import _native as nat
+    lib = nat.load()
+
+    def run(pool=None, batch=None, **kw):
+        common = dict(abi_version=nat.ABI_VERSION, layer=0, pool=_pool(nat, **(pool or {})), batch=_batch(nat, **(batch or {})))
+        if call == "rows":
+            a = nat.PagedRowsArgs(**{**common, "dtype": 0, "k": 4096, "v": 4096, "k_t": 512, "k_h": 256, "v_t": 512, "v_h": 256, **kw})
+            return lib.akv_paged_append(ctypes.byref(a), None), lib.akv_paged_read(ctypes.byref(a), None)
+        q = dict(Hq=4, q_dtype=0, causal=1, sm_scale=0.1, q=4096, q_t=1024, q_h=256, out=4096, lse=4096)
+        if call == "attn":
+            a = nat.PagedAttnArgs(**{**common, **q, "workspace": 4096, "workspace_bytes": 64, **kw})
+            rc = lib.akv_paged_attn(ctypes.byref(a), None)
+            if rc in (nat.AKV_E_SHAPE, nat.AKV_E_DTYPE, nat.AKV_E_UNSUPPORTED, nat.AKV_E_ABI):
+                assert lib.akv_paged_attn_workspace_bytes(ctypes.byref(a)) == -1
+            return (rc,)
+        a = nat.PagedImportanceArgs(**{**common, **q, "q_window": 0, "decay": 0.9, "scores": 4096, "n_scores": 10,
+                                       "score_stride": 10, "out_stride": 10, **kw})
+        return (lib.akv_paged_importance(ctypes.byref(a), None),)
+
+    code = lambda name: getattr(nat, "AKV_" + name)  # noqa: E731
+    for kw, want in POOLS:
+        assert set(run(pool=kw)) == {code(want)}, (kw, lib.akv_last_error())
+    for kw, want in BATCHES:
+        assert set(run(batch=kw)) == {code(want)}, (kw, lib.akv_last_error())
+    own = [(dict(abi_version=4), "E_ABI"), (dict(layer=2), "E_SHAPE"), (dict(layer=-1), "E_SHAPE")]
+    if call == "rows":
+        own += [(dict(dtype=3), "E_DTYPE"), (dict(k=0), "E_INVALID"), (dict(v=4100), "E_ALIGN"), (dict(k_t=520), "E_ALIGN")]
+    else:
+        own += [(dict(q_dtype=2), "E_DTYPE"), (dict(Hq=3), "E_SHAPE"), (dict(Hq=0), "E_SHAPE"), (dict(sm_scale=0.0), "E_INVALID"),
+                (dict(sm_scale=float("nan")), "E_INVALID"), (dict(sm_scale=float("inf")), "E_INVALID"), (dict(q=0), "E_INVALID"),
+                (dict(q=4100), "E_ALIGN"), (dict(q_h=260), "E_ALIGN"), (dict(out=0), "E_INVALID"), (dict(lse=4097), "E_ALIGN")]
+    if call == "attn":
+        own += [(dict(workspace=0), "E_WORKSPACE"), (dict(workspace_bytes=63), "E_WORKSPACE"), (dict(out=4100), "E_ALIGN")]
+    if call == "importance":
+        own += [(dict(q_window=-1), "E_SHAPE"), (dict(score_stride=9), "E_SHAPE"), (dict(n_scores=-1), "E_SHAPE"),
+                (dict(lse=0), "E_INVALID"), (dict(scores=0), "E_INVALID"), (dict(out=4098), "E_ALIGN")]
+    for kw, want in own:
+        assert set(run(**kw)) == {code(want)}, (kw, lib.akv_last_error())
+
+
+def test_c_refusals_of_moves():
+    from akv import _native as nat
+    lib = nat.load()
+    for kw, want in POOLS:
+        p = _pool(nat, **kw)
+        assert lib.akv_paged_copy(ctypes.byref(p), 4096, 4096, 1, None) == getattr(nat, "AKV_" + want), kw
+    p = _pool(nat)
+    assert lib.akv_paged_copy(None, None, None, 0, None) == nat.AKV_E_INVALID
+    for n, a, b, want in ((5, 4096, 4096, nat.AKV_E_SHAPE), (-1, 4096, 4096, nat.AKV_E_SHAPE), (1, None, 4096, nat.AKV_E_INVALID),
+                          (1, 4096, 4098, nat.AKV_E_ALIGN), (0, None, None, nat.AKV_OK)):
+        assert lib.akv_paged_copy(ctypes.byref(p), a, b, n, None) == want
+    base = dict(abi_version=nat.ABI_VERSION, n_seqs=2, pool=p, src_table=4096, dst_table=4096, src_stride=4, dst_stride=4,
+                src_width=4, dst_width=4, keep=4096, n_keep=4096, keep_stride=9, max_keep=9)
+    for kw, want in ((dict(abi_version=3), nat.AKV_E_ABI), (dict(n_seqs=-1), nat.AKV_E_SHAPE), (dict(src_stride=3), nat.AKV_E_SHAPE),
+                     (dict(keep_stride=8), nat.AKV_E_SHAPE), (dict(dst_width=2 ** 27, dst_stride=2 ** 27), nat.AKV_E_SHAPE),
+                     (dict(keep=0), nat.AKV_E_INVALID), (dict(n_keep=0), nat.AKV_E_INVALID), (dict(src_table=0), nat.AKV_E_INVALID),
+                     (dict(dst_table=4097), nat.AKV_E_ALIGN)):
+        a = nat.PagedCompactArgs(**{**base, **kw})
+        assert lib.akv_paged_compact(ctypes.byref(a), None) == want, kw
+    assert lib.akv_paged_compact(None, None) == nat.AKV_E_INVALID
+
+
+def test_host_tensors_are_refused():
+    import akv
+    with pytest.raises(RuntimeError, match="CPU"):
+        akv.PagedPool.empty(1, 4, 2, 128, device="cpu")
+    with pytest.raises(RuntimeError, match="CPU"):
+        akv.PagedBatch(torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), 0, 0)
+    with pytest.raises(RuntimeError):
+        akv.PackedPagedCache(1, 2, 128, device="cpu")
+    with pytest.raises(ValueError):
+        akv.PagedPool(torch.zeros(1, 2, 3, 4, 5, dtype=torch.uint8), 128)
+    with pytest.raises(NotImplementedError):
+        akv.PagedPool.empty(1, 4, 2, 128, page_size=40)
