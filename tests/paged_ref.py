@@ -29,7 +29,7 @@ def places(D, G):
 
 def quantize(x, G):
     """(..., D) float64 -> codes (..., D) uint8, scale and zero (..., NG) float16."""
-    xg = x.reshape(*x.shape[:-1], -1, G)
+    xg = x.reshape(*x.shape[:-1], x.shape[-1] // G, G)
     bad = ~np.isfinite(xg).all(-1)
     xg = np.clip(np.where(np.isfinite(xg), xg, 0.0), -TOP, TOP)
     lo, hi = xg.min(-1), xg.max(-1)
