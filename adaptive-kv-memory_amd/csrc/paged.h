@@ -45,7 +45,8 @@ struct PagedAttnParams {
     int64_t q_t, q_h;
     void *out;
     float *lse;
-    float *part;               // partial states of items that several workgroups share
+    float *part;               // the workspace; in the kernels, partial states of items that several workgroups share
+    int *sums;                 // first units of the sequences
     int groups;                // workgroups of the launch
     int rows;                  // most rows of an item
 };
@@ -61,6 +62,7 @@ struct PagedImportanceParams {
     const float *lse, *scores;
     float *out;
     int64_t n_scores, score_stride, out_stride;
+    int head_split;            // waves that share a run of tokens, each with its heads
 };
 
 struct PagedCopyParams {

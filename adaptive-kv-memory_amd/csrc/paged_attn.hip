@@ -7,9 +7,10 @@
 // MFMA; the operand for the query takes the 1/16, its rows are scaled to a maximum in
 // [2^13, 2^14), and the factor 2^24 leaves with the softmax scale.  Scores are thus exact to
 // float32 rounding, whatever the cache's widths.  Values: o = sum of p (c s + z) is the product
-// of the codes with p s (float16, rounded once more than p) plus sum of p z, one more MFMA row
-// per channel group.  Softmax state: running maximum and sum per row in float32.
+// of the codes with p s plus sum of p z, one more MFMA row per channel group; p and p s enter as two
+// float16 each.  Softmax state: running maximum and sum per row in float32.
 #include <algorithm>
+#include <type_traits>
 
 #include "akv_common.h"
 #include "paged.h"
@@ -19,6 +20,7 @@ namespace {
 
 constexpr float kMinMax = -0x1p126f;  // a finite start of the running maximum: a row that sees nothing stays at p = 0
 constexpr int kThreads = 256, kWaves = 4, kRows = 16;
+constexpr int kImpTiles = 4;          // tiles of a wave's run in the importance
 constexpr int kMaxGroups = 512;       // two workgroups a compute unit
 
 __device__ __forceinline__ float xmax(float x) {
@@ -44,23 +46,36 @@ struct Query {
     float kx;       // score -> log2 domain
 };
 
-template <int D, int NG>
-__device__ __forceinline__ void load_query(Query<D, NG> &Q, const unsigned char *row, bool bf16, float scale_log2) {
-    constexpr int NS = D / 32;
+template <int D>
+__device__ __forceinline__ void load_row(u4 (&w)[D / 32], const unsigned char *row) {
     const int grp = (threadIdx.x >> 4) & 3;
+#pragma unroll
+    for (int g = 0; g < D / 32; ++g) w[g] = *(const u4 *)(row + (32 * g + 8 * grp) * 2);
+}
+
+template <int D, int NG>
+__device__ __forceinline__ void make_query(Query<D, NG> &Q, const u4 (&w)[D / 32], bool bf16, float scale_log2) {
+    constexpr int NS = D / 32;
     float x[NS][8];
     float top = 0.0f;
+    if (bf16) {
 #pragma unroll
-    for (int g = 0; g < NS; ++g) {
-        const u4 w = *(const u4 *)(row + (32 * g + 8 * grp) * 2);
+        for (int g = 0; g < NS; ++g)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t v = w[i];
-            x[g][2 * i] = bf16 ? __builtin_bit_cast(float, v << 16) : lo_f(v);
-            x[g][2 * i + 1] = bf16 ? __builtin_bit_cast(float, v & 0xffff0000u) : hi_f(v);
-            top = __builtin_fmaxf(top, __builtin_fmaxf(__builtin_fabsf(x[g][2 * i]), __builtin_fabsf(x[g][2 * i + 1])));
-        }
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t v = w[g][i >> 1];
+                x[g][i] = __builtin_bit_cast(float, i & 1 ? v & 0xffff0000u : v << 16);
+            }
+    } else {
+#pragma unroll
+        for (int g = 0; g < NS; ++g)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[g][i] = i & 1 ? hi_f(w[g][i >> 1]) : lo_f(w[g][i >> 1]);
     }
+#pragma unroll
+    for (int g = 0; g < NS; ++g)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = __builtin_fmaxf(top, __builtin_fabsf(x[g][i]));
     top = xmax(top);
     const int ex = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 14;  // top = f 2^ex, f in [1/2, 1)
 #pragma unroll
@@ -110,34 +125,46 @@ __device__ __forceinline__ f4 tile_scores(const Query<D, NG> &Q, const uint32_t 
     return s;
 }
 
-// Units of a sequence: 32 cached tokens of one head for one chunk of 16 rows.
+// The work of a sequence, in units: 32 cached tokens of one head for one chunk of 16 rows.  An
+// item (one head and chunk) counts kSetup units more than it has, the time until its first
+// tiles are there: without them the runs of short sequences took twice as long as the others
+// (a step of 24 sequences of 33 to 65536 tokens: 113 us without, 76 with).
+constexpr int kSetup = 2;
 struct SeqWork {
     SeqRows r;
-    int rows, chunks, units;  // rows = query tokens * g; units of one (head, chunk)
+    int rows, chunks, units, cost;  // rows = query tokens * g; units of one (head, chunk), and what it counts
 };
-__device__ __forceinline__ SeqWork seq_work(const PagedAttnParams &p, int s) {
+__device__ __forceinline__ SeqWork seq_work(const PagedAttnParams &p, const SeqRows &r) {
     SeqWork w;
-    w.r = seq_rows(p.seqs, s, p.pool.log_tpp + 4);
-    const int n = min(w.r.n, p.seqs.max_q);
-    w.rows = n * p.g;
+    w.r = r;
+    w.rows = min(r.n, p.seqs.max_q) * p.g;
     w.chunks = (w.rows + kRows - 1) / kRows;
-    w.units = max(1, (int)((w.r.kv + kUnitTok - 1) / kUnitTok));
+    w.units = max(1, (int)((r.kv + kUnitTok - 1) / kUnitTok));
+    w.cost = w.units + kSetup;
     return w;
 }
-__device__ __forceinline__ int seq_total(const PagedAttnParams &p, int s) {
-    const SeqWork w = seq_work(p, s);
-    return w.chunks * w.units * p.pool.heads;
-}
+__device__ __forceinline__ int seq_total(const PagedAttnParams &p, const SeqWork &w) { return w.chunks * w.cost * p.pool.heads; }
 
-// Exclusive sums of the sequences' units: entry i is that of the first sequence of thread i
-// (runs of `per` sequences), entry 256 the total.
-__device__ __forceinline__ void scan_seqs(const PagedAttnParams &p, int *pre, int per) {
-    __shared__ int wave_sum[kWaves];
+// Where the sequences' units lie: pre[i] is the first unit of sequence i * per, pre[256] the
+// total; up to 256 sequences their rows are kept too.
+struct Scan {
+    int pre[257];
+    int wave_sum[kWaves];
+    int begin[kThreads], n[kThreads], kv[kThreads];
+};
+__device__ __forceinline__ SeqRows scanned_rows(const PagedAttnParams &p, const Scan &sc, int s) {
+    return p.seqs.n_seqs <= kThreads ? SeqRows{sc.begin[s], sc.n[s], sc.kv[s]} : seq_rows(p.seqs, s, p.pool.log_tpp + 4);
+}
+__device__ __forceinline__ void scan_seqs(const PagedAttnParams &p, Scan &sc, int per) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     int mine = 0;
     for (int i = 0; i < per; ++i) {
         const int s = t * per + i;
-        if (s < p.seqs.n_seqs) mine += seq_total(p, s);
+        if (s < p.seqs.n_seqs) {
+            const SeqRows r = seq_rows(p.seqs, s, p.pool.log_tpp + 4);
+            mine += seq_total(p, seq_work(p, r));
+            if (per == 1) sc.begin[t] = r.begin, sc.n[t] = r.n, sc.kv[t] = (int)r.kv;
+        }
     }
     int inc = mine;
 #pragma unroll
@@ -145,12 +172,12 @@ __device__ __forceinline__ void scan_seqs(const PagedAttnParams &p, int *pre, in
         const int o = __shfl_up(inc, d);
         if (lane >= d) inc += o;
     }
-    if (lane == 63) wave_sum[wave] = inc;
+    if (lane == 63) sc.wave_sum[wave] = inc;
     __syncthreads();
     int before = 0;
-    for (int w = 0; w < wave; ++w) before += wave_sum[w];
-    pre[t] = before + inc - mine;
-    if (t == 255) pre[256] = before + inc;
+    for (int w = 0; w < wave; ++w) before += sc.wave_sum[w];
+    sc.pre[t] = before + inc - mine;
+    if (t == kThreads - 1) sc.pre[kThreads] = before + inc;
     __syncthreads();
 }
 
@@ -191,7 +218,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
     constexpr int NS = D / 32, NB = D / 16, TB = paged_tile_bytes(D, NG), EROW = D + 4;
     constexpr int MW = NG == 4 ? 2 : 1;          // meta dwords a lane loads of a tile
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ int pre[257];
+    __shared__ Scan sc;
     __shared__ int e_seq[2 * kWaves], e_item[2 * kWaves], e_flags[2 * kWaves];  // flags: 1 used, 2 starts, 4 ends
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
@@ -200,10 +227,14 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
     uint32_t *meta = (uint32_t *)(smem + 2 * kWaves * p.rows * EROW * 4) + wave * 2 * 32 * NG;
     if (lane < 2) e_flags[2 * wave + lane] = 0;
 
-    const int per = (p.seqs.n_seqs + 255) / 256;
-    scan_seqs(p, pre, per);
-    const int total = pre[256];
+    const int per = (p.seqs.n_seqs + kThreads - 1) / kThreads;
+    scan_seqs(p, sc, per);
+    const int total = sc.pre[kThreads];
     const int share = share_of(total, p.groups);
+    if (blockIdx.x == 0) {  // for the merge
+        p.sums[threadIdx.x] = sc.pre[threadIdx.x];
+        if (threadIdx.x == 0) p.sums[kThreads] = total;
+    }
     int x = (int)min((int64_t)(blockIdx.x * kWaves + wave) * share, (int64_t)total);
     const int x_end = min(x + share, total);
 
@@ -213,20 +244,24 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
     if (x < x_end) {
         int k = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) k += __builtin_popcountll(__builtin_amdgcn_ballot_w64(pre[64 * i + lane] <= x));
+        for (int i = 0; i < 4; ++i) k += __builtin_popcountll(__builtin_amdgcn_ballot_w64(sc.pre[64 * i + lane] <= x));
         s = (k - 1) * per;
-        off = x - __builtin_amdgcn_readfirstlane(pre[k - 1]);
+        off = x - sc.pre[k - 1];
         for (;;) {
-            w = seq_work(p, s);
-            const int n = w.chunks * w.units * p.pool.heads;
+            w = seq_work(p, scanned_rows(p, sc, s));
+            const int n = seq_total(p, w);
             if (off < n) break;
             off -= n;
             ++s;
         }
     }
     while (x < x_end) {
-        const int item = off / w.units, j0 = off - item * w.units;
-        const int j1 = min(w.units, j0 + (x_end - x));
+        const int item = off / w.cost, c0 = off - item * w.cost;
+        const int c1 = min(w.cost, c0 + (x_end - x));
+        const int j0 = max(0, c0 - kSetup), j1 = max(0, c1 - kSetup);
+        x += c1 - c0;
+        off += c1 - c0;
+        if (j1 == 0) break;  // no unit of the item is in the run, and the run ends
         const int h = item / w.chunks, row0 = (item - h * w.chunks) * kRows;
         const int rows = min(kRows, w.rows - row0);
 
@@ -237,14 +272,15 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
         const int see = (int)(p.causal ? max(old + qt, (int64_t)0) : kv);
         const int see_all = (int)(p.causal ? max(old + row0 / p.g, (int64_t)0) : kv);
         const int see_any = (int)(p.causal ? max(old + (row0 + rows - 1) / p.g, (int64_t)0) : kv);
-        Query<D, NG> Q;
-        load_query<D, NG>(Q, p.q + (w.r.begin + qt) * p.q_t + (h * p.g + row % p.g) * p.q_h, p.q_bf16, p.scale_log2);
+        u4 qw[NS];
+        load_row<D>(qw, p.q + (w.r.begin + qt) * p.q_t + (h * p.g + row % p.g) * p.q_h);
 
         const int32_t *table = p.seqs.table + s * p.seqs.table_stride;
         const int jn = min(j1, (see_any + kUnitTok - 1) / kUnitTok);
         const int log_tpp = p.pool.log_tpp;
         int pb = (2 * j0) >> log_tpp;
         int pid = pb + lane < p.seqs.width ? table[pb + lane] : -1;
+        asm volatile("" : "+v"(pid));
 
         struct Unit {
             uint32_t kc[2][NS], vc[2][NS], m[2][MW];
@@ -258,6 +294,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
                 if (pi - pb >= 64) {
                     pb = pi;
                     pid = pb + lane < p.seqs.width ? table[pb + lane] : -1;
+                    asm volatile("" : "+v"(pid));  // waited for here: not by every unit, behind its tiles' loads
                 }
                 uint32_t page = (uint32_t)__builtin_amdgcn_readlane(pid, pi - pb);
                 const int left = (int)(kv - 16 * (int64_t)t);
@@ -288,9 +325,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
 #pragma unroll
         for (int b = 0; b < NB; ++b) acc[b] = (f4){0.f, 0.f, 0.f, 0.f};
 
-        auto consume = [&](Unit &u, int j) {
-            const bool clean = kUnitTok * (j + 1) <= see_all && u.nv[0] == 16 && u.nv[1] == 16;
-            if (!clean) {  // V meta of slots without a token: whatever is there becomes 0
+        auto work = [&](const Query<D, NG> &Q, Unit &u, int j, auto is_clean) {
+            constexpr bool clean = decltype(is_clean)::value;
+            if constexpr (!clean) {  // V meta of slots without a token: whatever is there becomes 0
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -312,7 +349,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 sc[i] = tile_scores<D, NG>(Q, u.kc[i], meta + i * 32 * NG) * Q.kx;
-                if (!clean)
+                if constexpr (!clean)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int in = 4 * grp + e;
@@ -337,19 +374,28 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
 #pragma unroll
             for (int e = 0; e < 8; ++e) pr[e] = __builtin_amdgcn_exp2f(sc[e >> 2][e & 3] + bias);
             l += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
-            h2 ph[4];
+            // p, and p s below, as two float16 that add up to it: one alone would cost float16
+            // outputs half a step (measured 3.5e-4 of the output's norm; 2.1e-4 is its own rounding)
+            h2 ph[4], pl[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) ph[q] = (h2){(_Float16)pr[2 * q], (_Float16)pr[2 * q + 1]};
+            for (int q = 0; q < 4; ++q) {
+                ph[q] = (h2){(_Float16)pr[2 * q], (_Float16)pr[2 * q + 1]};
+                pl[q] = (h2){(_Float16)(pr[2 * q] - (float)ph[q][0]), (_Float16)(pr[2 * q + 1] - (float)ph[q][1])};
+            }
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                u4 pw;
+                u4 pw, rw;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const u2 sv = *(const u2 *)(meta + i * 32 * NG + 16 * NG + (grp * NG + g) * 2);
-                    pw[2 * i] = as_u32(ph[2 * i] * as_h2(sv[0]));
-                    pw[2 * i + 1] = as_u32(ph[2 * i + 1] * as_h2(sv[1]));
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const h2 sc2 = as_h2(sv[q]), t2 = ph[2 * i + q] * sc2;
+                        pw[2 * i + q] = as_u32(t2);
+                        rw[2 * i + q] = as_u32(__builtin_elementwise_fma(pl[2 * i + q], sc2, __builtin_elementwise_fma(ph[2 * i + q], sc2, -t2)));
+                    }
                 }
-                const h8 pg = __builtin_bit_cast(h8, pw);
+                const h8 pg = __builtin_bit_cast(h8, pw), rg = __builtin_bit_cast(h8, rw);
                 // the group's blocks of 16 channels: block 4 h + 2 l + b is nibble 2 l + b of half h
 #pragma unroll
                 for (int b = g * (NB / NG); b < (g + 1) * (NB / NG); ++b) {
@@ -361,6 +407,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
                         a[q] = (n >= 2 ? v >> 8 : v) & (n & 1 ? 0x00F000F0u : 0x000F000Fu);
                     }
                     acc[b] = mfma_k32(__builtin_bit_cast(h8, a), pg, acc[b]);
+                    acc[b] = mfma_k32(__builtin_bit_cast(h8, a), rg, acc[b]);
                 }
             }
             u4 za = {0u, 0u, 0u, 0u};
@@ -370,25 +417,37 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
                 za = (u4){a[0], a[1], b[0], b[1]};
             }
             accz = mfma_k32(__builtin_bit_cast(h8, za), __builtin_bit_cast(h8, (u4){as_u32(ph[0]), as_u32(ph[1]), as_u32(ph[2]), as_u32(ph[3])}), accz);
+            accz = mfma_k32(__builtin_bit_cast(h8, za), __builtin_bit_cast(h8, (u4){as_u32(pl[0]), as_u32(pl[1]), as_u32(pl[2]), as_u32(pl[3])}), accz);
         };
 
-        if (j0 < jn) load(U[0], j0);
-        if (j0 + 1 < jn) load(U[1], j0 + 1);
-        for (int j = j0; j < jn; j += 2) {
-            consume(U[0], j);
-            if (j + 2 < jn) load(U[0], j + 2);
-            if (j + 1 < jn) {
-                consume(U[1], j + 1);
-                if (j + 3 < jn) load(U[1], j + 3);
-            }
+        auto consume = [&](const Query<D, NG> &Q, Unit &u, int j) {
+            if (kUnitTok * (j + 1) <= see_all && u.nv[0] == 16 && u.nv[1] == 16) work(Q, u, j, std::true_type{});
+            else work(Q, u, j, std::false_type{});
+        };
+
+        // Both buffers are always loaded (the last unit again at the end), so that a unit waits
+        // for its own loads and never for those behind it.
+        if (j0 < jn) {
+            load(U[0], j0);
+            load(U[1], min(j0 + 1, jn - 1));
         }
+        Query<D, NG> Q;
+        make_query<D, NG>(Q, qw, p.q_bf16, p.scale_log2);
+        int j = j0;
+        for (; j + 1 < jn; j += 2) {
+            consume(Q, U[0], j);
+            load(U[0], min(j + 2, jn - 1));
+            consume(Q, U[1], j + 1);
+            load(U[1], min(j + 3, jn - 1));
+        }
+        if (j < jn) consume(Q, U[0], j);
 
         // the segment's state in true units: 2^24 of the codes (2^20 where they lay a nibble higher), zeros
         l = xsum(l);
         float z[NG];
 #pragma unroll
         for (int g = 0; g < NG; ++g) z[g] = __shfl(accz[g], col);
-        const bool starts = j0 == 0, ends = j1 == w.units;
+        const bool starts = j0 == 0, ends = c1 == w.cost;
         const int slot = 2 * wave + (ends ? 0 : 1);
         float *er = entries + (slot * p.rows + col) * EROW;
 #pragma unroll
@@ -418,10 +477,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
             }
         }
 
-        x += j1 - j0;
-        off += j1 - j0;
-        if (x < x_end && off == w.chunks * w.units * p.pool.heads) {
-            do w = seq_work(p, ++s);
+        if (x < x_end && off == seq_total(p, w)) {
+            do w = seq_work(p, scanned_rows(p, sc, ++s));
             while (w.chunks == 0);
             off = 0;
         }
@@ -457,7 +514,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
         }
         if (!last) continue;
         if (began && (f & 4)) {
-            const SeqWork sw = seq_work(p, e_seq[e]);
+            const SeqWork sw = seq_work(p, scanned_rows(p, sc, e_seq[e]));
             const int it = e_item[e], h = it / sw.chunks, row = (it - h * sw.chunks) * kRows + row_t;
             if (row_t < kRows && row < sw.rows && row_t < p.rows) {
                 if constexpr (D == 128) {
@@ -478,151 +535,217 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
     }
 }
 
-// Items that several workgroups share: one workgroup an item joins their partial states in order.
+// Items that several workgroups share: one workgroup an item.  Sixteen threads a row; where an
+// item has fewer than 16 rows the others take partial states of their own, joined through LDS
+// in a fixed order.  Bound by latency: the states of an item are loaded at once, eight a thread.
 template <int D>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnParams p) {
-    constexpr int EROW = D + 4;
-    __shared__ int pre[257];
-    const int per = (p.seqs.n_seqs + 255) / 256;
-    scan_seqs(p, pre, per);
-    const int share = share_of(pre[256], p.groups) * kWaves;  // units a workgroup has
+    constexpr int EROW = D + 4, CH = D / 16, B = 8;
+    __shared__ float so[kThreads][CH + 1], sm[16], sl[16];
+    const int per = (p.seqs.n_seqs + kThreads - 1) / kThreads;
     const int s = blockIdx.y, k = s / per;
-    int at = pre[k];
-    for (int i = k * per; i < s; ++i) at += seq_total(p, i);
-    const SeqWork w = seq_work(p, s);
+    int at = p.sums[k];
+    const int share = share_of(p.sums[kThreads], p.groups) * kWaves;  // units a workgroup has
+    const SeqWork w = seq_work(p, seq_rows(p.seqs, s, p.pool.log_tpp + 4));
+    for (int i = k * per; i < s; ++i) at += seq_total(p, seq_work(p, seq_rows(p.seqs, i, p.pool.log_tpp + 4)));
+    int rp = 1;
+    while (rp < p.rows) rp <<= 1;
+    const int t16 = threadIdx.x >> 4, row_t = t16 & (rp - 1), sp = t16 / rp, ps = 16 / rp, ch = (threadIdx.x & 15) * CH;
     for (int item = blockIdx.x; item < w.chunks * p.pool.heads; item += gridDim.x) {
-        const int first = at + item * w.units;
-        const int g0 = first / share, g1 = (first + w.units - 1) / share;
+        const int first = at + item * w.cost;
+        const int g0 = (first + kSetup) / share, g1 = (first + w.cost - 1) / share;
         if (g0 == g1) continue;
-        const int row_t = threadIdx.x >> 4, ch = (threadIdx.x & 15) * (D / 16);
         const int h = item / w.chunks, row = (item - h * w.chunks) * kRows + row_t;
-        if (row_t >= p.rows || row >= w.rows) continue;
-        float o[8];
+        const bool live = row_t < p.rows && row < w.rows;
+        float o[CH];
         float M = kMinMax, L = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = 0.f;
-        for (int g = g0; g <= g1; ++g) {
-            const float *pr = p.part + ((int64_t)(2 * g + (g == g0 ? 1 : 0)) * p.rows + row_t) * EROW;
-            const float m = pr[D], l = pr[D + 1];
-            const float mn = __builtin_fmaxf(M, m);
-            const float a = __builtin_amdgcn_exp2f(M - mn), b = __builtin_amdgcn_exp2f(m - mn);
+        for (int i = 0; i < CH; ++i) o[i] = 0.f;
+        for (int g = g0 + sp; g <= g1 && live; g += B * ps) {
+            f4 v[B][CH / 4];
+            f2 ml[B];
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) o[i] = __builtin_fmaf(pr[ch + i], b, o[i] * a);
-            L = __builtin_fmaf(l, b, L * a);
+            for (int i = 0; i < B; ++i) {
+                const int gi = min(g + i * ps, g1);
+                const float *pr = p.part + ((int64_t)(2 * gi + (gi == g0 ? 1 : 0)) * p.rows + row_t) * EROW;
+#pragma unroll
+                for (int c = 0; c < CH / 4; ++c) v[i][c] = ((const f4 *)(pr + ch))[c];
+                ml[i] = *(const f2 *)(pr + D);
+            }
+            float mn = M;
+#pragma unroll
+            for (int i = 0; i < B; ++i) mn = __builtin_fmaxf(mn, ml[i][0]);
+            const float a = __builtin_amdgcn_exp2f(M - mn);
+            L *= a;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) o[c] *= a;
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                const float b = g + i * ps <= g1 ? __builtin_amdgcn_exp2f(ml[i][0] - mn) : 0.f;
+                L = __builtin_fmaf(ml[i][1], b, L);
+#pragma unroll
+                for (int c = 0; c < CH; ++c) o[c] = __builtin_fmaf(v[i][c >> 2][c & 3], b, o[c]);
+            }
             M = mn;
         }
-        if constexpr (D == 128) {
-            write_row(p, w.r, h, row, ch, o, M, L);
-        } else {
-            float o8[8];
+        if (ps > 1) {
+            __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o8[i] = o[i], o8[4 + i] = __shfl_down(o[i], 1);
-            if (!(threadIdx.x & 1)) write_row(p, w.r, h, row, ch, o8, M, L);
+            for (int c = 0; c < CH; ++c) so[threadIdx.x][c] = o[c];
+            if (ch == 0) sm[t16] = M, sl[t16] = L;
+            __syncthreads();
+            if (sp == 0)
+                for (int q = 1; q < ps; ++q) {
+                    const float m = sm[q * rp + row_t], mn = __builtin_fmaxf(M, m);
+                    const float a = __builtin_amdgcn_exp2f(M - mn), b = __builtin_amdgcn_exp2f(m - mn);
+                    L = __builtin_fmaf(sl[q * rp + row_t], b, L * a);
+#pragma unroll
+                    for (int c = 0; c < CH; ++c) o[c] = __builtin_fmaf(so[threadIdx.x + 16 * q * rp][c], b, o[c] * a);
+                    M = mn;
+                }
         }
+        if (sp != 0 || !live) continue;
+        float o8[8];
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            o8[i] = o[i];
+            if constexpr (CH == 4) o8[4 + i] = __shfl_down(o[i], 1);
+        }
+        if (CH == 8 || !(threadIdx.x & 1)) write_row(p, w.r, h, row, ch, o8, M, L);
     }
 }
 
-// The importance: a workgroup takes 64 tokens of a sequence, its waves the heads in turn; the
-// sum over rows stays in registers and is joined over heads in a fixed order.  Bound by the K
-// half of the cache.
+// The importance.  A wave takes 64 tokens of a sequence and some of its heads (the heads are
+// split over the waves of a workgroup, at most four ways), the next head's keys in flight; the
+// sums over rows stay in registers, lane by lane of a row, until the end, and are joined in a
+// fixed order.  Bound by the K half of the cache.
 template <int D, int NG>
-__global__ __launch_bounds__(kThreads) void paged_importance_kernel(const PagedImportanceParams p) {
-    constexpr int NS = D / 32, TB = paged_tile_bytes(D, NG), NT = 4;
-    __shared__ __align__(16) uint32_t smeta[kWaves][NT * 16 * NG];
+__global__ __launch_bounds__(kThreads, 2) void paged_importance_kernel(const PagedImportanceParams p) {
+    constexpr int NS = D / 32, TB = paged_tile_bytes(D, NG), NT = kImpTiles, MT = 16 * NG;
+    constexpr uint32_t ALL = (1u << NT) - 1;
+    __shared__ __align__(16) uint32_t smeta[kWaves][NT * MT];
     __shared__ float sums[kWaves][NT * 16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
     const int k_at = (4 * col + grp) * (D / 8);  // K codes of token col, quarter grp
-    const int s = blockIdx.y;
+    const int s = blockIdx.y, hs = p.head_split, h0 = wave & (hs - 1);
+    const int blocks = kWaves / hs;              // runs of NT tiles a workgroup has
     const SeqRows r = seq_rows(p.seqs, s, p.pool.log_tpp + 4);
-    const int64_t tok0 = (int64_t)blockIdx.x * (NT * 16);
+    const int64_t tok0 = ((int64_t)blockIdx.x * blocks + wave / hs) * (NT * 16);
     const int n = min(r.n, p.seqs.max_q);
     const int64_t kv = n > 0 ? min(r.kv, p.n_scores) : 0;  // tokens whose score changes
     const int first = p.q_window > 0 && p.q_window < n ? n - p.q_window : 0;
     const int rows = (n - first) * p.g;
-    float sum[NT][4];
+    float sum[NT * 4];
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum[i][e] = 0.f;
+    for (int i = 0; i < NT * 4; ++i) sum[i] = 0.f;
     uint32_t *meta = smeta[wave];
     if (tok0 < kv) {
-        const int log_tpp = p.pool.log_tpp;
+        const int log_tpp = p.pool.log_tpp, in_page = (1 << log_tpp) - 1;
         const int32_t *table = p.seqs.table + s * p.seqs.table_stride;
-        int64_t at[NT];   // the tiles' places for head 0
-        int nv[NT];
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            const int64_t t = (tok0 >> 4) + i;
-            const int64_t left = r.kv - 16 * t;
-            uint32_t page = left > 0 ? (uint32_t)table[t >> log_tpp] : 0xffffffffu;
-            nv[i] = page < p.pool.n_pages ? (int)min(left, (int64_t)16) : 0;
-            if (page >= p.pool.n_pages) page = 0;
-            at[i] = (int64_t)page * p.pool.page_bytes + (t & ((1 << log_tpp) - 1)) * TB;
-        }
-        for (int h = wave; h < p.pool.heads; h += kWaves) {
-            uint32_t kc[NT][NS];
-            __builtin_amdgcn_wave_barrier();
+        const int t0 = (int)(tok0 >> 4);
+        // lane i < NT: the page of tile i; tiles past the end or outside the pool read page 0 and count nothing
+        const bool there = lane < NT && 16 * (int64_t)(t0 + lane) < r.kv;
+        uint32_t page = there ? (uint32_t)table[(t0 + lane) >> log_tpp] : 0xffffffffu;
+        const uint32_t have = (uint32_t)__builtin_amdgcn_ballot_w64(page < p.pool.n_pages);
+        if (page >= p.pool.n_pages) page = 0;
+        struct Keys {
+            uint32_t kc[NT][NS], m[NT];
+        } K[2];
+        auto load = [&](Keys &k, int h) {
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
-                const unsigned char *tile = p.pool.base + at[i] + ((int64_t)h << log_tpp) * TB;
+                const unsigned char *tile = p.pool.base + (int64_t)(uint32_t)__builtin_amdgcn_readlane(page, i) * p.pool.page_bytes +
+                                            (int64_t)((h << log_tpp) + ((t0 + i) & in_page)) * TB;
                 if constexpr (D == 128) {
                     const u4 a = *(const u4 *)(tile + k_at);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) kc[i][e] = a[e];
+                    for (int e = 0; e < 4; ++e) k.kc[i][e] = a[e];
                 } else {
                     const u2 a = *(const u2 *)(tile + k_at);
-                    kc[i][0] = a[0], kc[i][1] = a[1];
+                    k.kc[i][0] = a[0], k.kc[i][1] = a[1];
                 }
-                meta[i * 16 * NG + (lane & (16 * NG - 1))] = *(const uint32_t *)(tile + 16 * D + (lane & (16 * NG - 1)) * 4);
+                k.m[i] = *(const uint32_t *)(tile + 16 * D + (lane & (MT - 1)) * 4);
             }
+        };
+        auto consume = [&](Keys &k, int h) {
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < NT; ++i) meta[i * MT + (lane & (MT - 1))] = k.m[i];
             __builtin_amdgcn_wave_barrier();
             for (int row0 = 0; row0 < rows; row0 += kRows) {
-                const int row = min(row0 + col, rows - 1);
+                const bool live = row0 + col < rows;
+                const int row = live ? row0 + col : rows - 1;
                 const int qt = first + row / p.g;
                 const int64_t t = r.begin + qt;
                 const int head = h * p.g + row % p.g;
+                u4 qw[NS];
+                load_row<D>(qw, p.q + t * p.q_t + head * p.q_h);
+                const float lse2 = p.lse[t * p.Hq + head] * 1.4426950408889634f;
                 Query<D, NG> Q;
-                load_query<D, NG>(Q, p.q + t * p.q_t + head * p.q_h, p.q_bf16, p.scale_log2);
-                const float lse2 = row0 + col < rows ? p.lse[t * p.Hq + head] * 1.4426950408889634f : INFINITY;
-                const int64_t see = p.causal ? r.kv - r.n + qt + 1 : r.kv;
+                make_query<D, NG>(Q, qw, p.q_bf16, p.scale_log2);
+                const float bias = live ? -lse2 : -INFINITY;
+                const int see = p.causal ? (int)max(r.kv - r.n + qt + 1, (int64_t)0) : (int)r.kv;
+                const bool clean = have == ALL && __builtin_amdgcn_ballot_w64(tok0 + NT * 16 <= see) == ~0ull;
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
-                    const f4 sc = tile_scores<D, NG>(Q, kc[i], meta + i * 16 * NG);
+                    const f4 x = tile_scores<D, NG>(Q, k.kc[i], meta + i * MT);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int in = 4 * grp + e;
-                        const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], Q.kx, -lse2));
-                        if (tok0 + 16 * i + in < see && in < nv[i]) sum[i][e] += row0 + col < rows ? pr : 0.f;
+                        float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], Q.kx, bias));
+                        if (!clean) pr = tok0 + 16 * i + 4 * grp + e < see && (have >> i & 1) && live ? pr : 0.f;
+                        sum[4 * i + e] += pr;
                     }
+                    __builtin_amdgcn_sched_barrier(0);  // one tile's meta in registers at a time
                 }
             }
+        };
+        const int last = h0 + (p.pool.heads - 1 - h0) / hs * hs;
+        load(K[0], h0);
+        load(K[1], min(h0 + hs, last));
+        int h = h0;
+        for (; h + hs <= last; h += 2 * hs) {
+            consume(K[0], h);
+            load(K[0], min(h + 2 * hs, last));
+            consume(K[1], h + hs);
+            load(K[1], min(h + 3 * hs, last));
         }
+        if (h <= last) consume(K[0], h);
     }
+    // over the 16 rows: each step halves what a lane holds; lane col ends with its NT / 4 sums of the quad's
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+    for (int d = 8, c = NT * 2; d > 0; d >>= 1, c >>= 1)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float v = sum[i][e];
-#pragma unroll
-            for (int d = 1; d < 16; d <<= 1) v += __shfl_xor(v, d);
-            if (col == 0) sums[wave][16 * i + 4 * grp + e] = v;
+        for (int i = 0; i < c; ++i) {
+            const bool up = col & d;
+            const float mine = up ? sum[i + c] : sum[i], other = up ? sum[i] : sum[i + c];
+            sum[i] = mine + __shfl_xor(other, d);
         }
+#pragma unroll
+    for (int i = 0; i < NT / 4; ++i) {
+        const int v = NT / 4 * col + i;  // tile v / 4, token 4 grp + v % 4 of it
+        sums[wave][16 * (v >> 2) + 4 * grp + (v & 3)] = sum[i];
+    }
     __syncthreads();
-    const int64_t j = tok0 + threadIdx.x;
-    if (threadIdx.x < NT * 16 && j < p.n_scores) {
+    for (int i = threadIdx.x; i < blocks * NT * 16; i += kThreads) {
+        const int64_t j = (int64_t)blockIdx.x * blocks * (NT * 16) + i;
+        if (j >= p.n_scores) break;
+        const int b = i / (NT * 16);
         const float *old = p.scores + s * p.score_stride + j;
         float *out = p.out + s * p.out_stride + j;
-        float v = 0.f;
-#pragma unroll
-        for (int q = 0; q < kWaves; ++q) v += sums[q][threadIdx.x];
-        if (j < kv) *out = __builtin_fmaf(*old, p.decay, v / (float)p.Hq);
-        else if (out != old) *out = *old;
+        if (j < kv) {
+            float v = 0.f;
+            for (int q = 0; q < hs; ++q) v += sums[b * hs + q][i & (NT * 16 - 1)];
+            *out = __builtin_fmaf(*old, p.decay, v / (float)p.Hq);
+        } else if (out != old) {
+            *out = *old;
+        }
     }
 }
 
 namespace {
 int attn_lds(const PagedAttnParams &p) { return 2 * kWaves * p.rows * (p.D + 4) * 4 + kWaves * 2 * 128 * p.ng; }
+constexpr int64_t kSumsBytes = 2048;  // Scan::pre at the start of the workspace
 }  // namespace
 
 int64_t paged_attn_plan(PagedAttnParams *p) {
@@ -631,13 +754,15 @@ int64_t paged_attn_plan(PagedAttnParams *p) {
     const int64_t units = std::max<int64_t>(1, (((int64_t)p->seqs.width << (p->pool.log_tpp + 4)) + kUnitTok - 1) / kUnitTok);
     const int64_t most = units * p->seqs.n_seqs * p->pool.heads * std::max<int64_t>(1, (r + kRows - 1) / kRows);
     p->groups = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxGroups, (most + kWaves - 1) / kWaves));
-    return (int64_t)p->groups * 2 * p->rows * (p->D + 4) * 4;
+    return kSumsBytes + (int64_t)p->groups * 2 * p->rows * (p->D + 4) * 4;
 }
 
 hipError_t paged_attn_launch(const PagedAttnParams &p0, hipStream_t st) {
     PagedAttnParams p = p0;
     if (p.seqs.n_seqs == 0 || p.seqs.max_q == 0) return hipSuccess;
     if (p.pool.n_pages == 0) p.seqs.width = 0;
+    p.sums = (int *)p.part;
+    p.part += kSumsBytes / 4;
     const size_t lds = attn_lds(p);
     auto go = [&](auto kern) {
         if (lds > 48 * 1024) (void)hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -663,7 +788,9 @@ hipError_t paged_attn_launch(const PagedAttnParams &p0, hipStream_t st) {
 hipError_t paged_importance_launch(const PagedImportanceParams &p0, hipStream_t st) {
     PagedImportanceParams p = p0;
     if (p.pool.n_pages == 0) p.seqs.width = 0;
-    const dim3 grid((unsigned)((p.n_scores + 63) / 64), p.seqs.n_seqs), block(kThreads);
+    p.head_split = p.pool.heads >= 4 ? 4 : p.pool.heads >= 2 ? 2 : 1;
+    const int64_t tokens = kImpTiles * 16 * (kWaves / p.head_split);
+    const dim3 grid((unsigned)((p.n_scores + tokens - 1) / tokens), p.seqs.n_seqs), block(kThreads);
     if (p.D == 128) {
         if (p.ng == 4) paged_importance_kernel<128, 4><<<grid, block, 0, st>>>(p);
         else if (p.ng == 2) paged_importance_kernel<128, 2><<<grid, block, 0, st>>>(p);
