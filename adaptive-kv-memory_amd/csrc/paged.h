@@ -10,6 +10,10 @@ namespace akv {
 
 constexpr int kTileTok = 16;   // tokens of a tile
 constexpr int kUnitTok = 32;   // tokens a wave of the attention takes at a time: two tiles
+constexpr int kRows = 16;      // query rows (tokens x heads of a group) that a wave takes
+// Sequences of more rows a cached head go to the tile kernel: a chunk of 16 rows costs a compute
+// unit 0.6 us for 64 tokens, a tile of up to 256 rows 3 us.
+constexpr int kFewRows = 80;
 
 __host__ __device__ constexpr int paged_tile_bytes(int D, int ng) { return 16 * D + 128 * ng; }
 
@@ -46,8 +50,10 @@ struct PagedAttnParams {
     void *out;
     float *lse;
     float *part;               // the workspace; in the kernels, partial states of items that several workgroups share
+    float *tile_part;          // the same of the tile kernel
     int *sums;                 // first units of the sequences
-    int groups;                // workgroups of the launch
+    int groups, tile_groups;   // workgroups of the two kernels
+    int few_rows;              // the tile kernel takes sequences of more rows
     int rows;                  // most rows of an item
 };
 
@@ -87,9 +93,11 @@ hipError_t paged_append_launch(const PagedRowsParams &p, hipStream_t s);
 hipError_t paged_read_launch(const PagedRowsParams &p, hipStream_t s);
 hipError_t paged_copy_launch(const PagedCopyParams &p, hipStream_t s);
 hipError_t paged_compact_launch(const PagedCompactParams &p, hipStream_t s);
-// Sets p.groups and p.rows; the workspace bytes.
+// Sets the launch's sizes and the parts of the workspace; its bytes.
 int64_t paged_attn_plan(PagedAttnParams *p);
 hipError_t paged_attn_launch(const PagedAttnParams &p, hipStream_t s);
+int64_t paged_tile_plan(PagedAttnParams *p);
+hipError_t paged_tile_launch(const PagedAttnParams &p, hipStream_t s);
 hipError_t paged_importance_launch(const PagedImportanceParams &p, hipStream_t s);
 
 #ifdef __HIPCC__

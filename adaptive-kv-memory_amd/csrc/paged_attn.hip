@@ -14,12 +14,12 @@
 
 #include "akv_common.h"
 #include "paged.h"
+#include "paged_device.h"
 
 namespace akv {
 namespace {
 
-constexpr float kMinMax = -0x1p126f;  // a finite start of the running maximum: a row that sees nothing stays at p = 0
-constexpr int kThreads = 256, kWaves = 4, kRows = 16;
+constexpr int kThreads = 256, kWaves = 4;
 constexpr int kImpTiles = 4;          // tiles of a wave's run in the importance
 constexpr int kMaxGroups = 512;       // two workgroups a compute unit
 
@@ -138,7 +138,7 @@ __device__ __forceinline__ SeqWork seq_work(const PagedAttnParams &p, const SeqR
     SeqWork w;
     w.r = r;
     w.rows = min(r.n, p.seqs.max_q) * p.g;
-    w.chunks = (w.rows + kRows - 1) / kRows;
+    w.chunks = w.rows <= kFewRows ? (w.rows + kRows - 1) / kRows : 0;  // more rows are paged_tile_kernel's
     w.units = max(1, (int)((r.kv + kUnitTok - 1) / kUnitTok));
     w.cost = w.units + kSetup;
     return w;
@@ -191,16 +191,12 @@ __device__ __forceinline__ void write_row(const PagedAttnParams &p, const SeqRow
                                           float m, float l) {
     const int64_t t = r.begin + row / p.g;
     const int head = h * p.g + row % p.g;
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    const float inv = row_inverse(l);
     u4 w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float a = o[2 * i] * inv, b = o[2 * i + 1] * inv;
-        w[i] = p.q_bf16 ? f32_to_bf16_rne(a) | ((uint32_t)f32_to_bf16_rne(b) << 16) : as_u32((h2){(_Float16)a, (_Float16)b});
-    }
+    for (int i = 0; i < 4; ++i) w[i] = to_pair(p.q_bf16, o[2 * i] * inv, o[2 * i + 1] * inv);
     *(u4 *)((unsigned char *)p.out + ((t * p.Hq + head) * p.D + ch) * 2) = w;
-    // p carries a factor 4
-    if (p.lse && ch == 0) p.lse[t * p.Hq + head] = l > 0.0f || l != l ? 0.69314718055994531f * (m + (__builtin_log2f(l) - 2.0f)) : -INFINITY;
+    if (p.lse && ch == 0) p.lse[t * p.Hq + head] = row_lse(m, l, 2.0f);  // p is held times 4
 }
 
 }  // namespace
@@ -746,21 +742,35 @@ __global__ __launch_bounds__(kThreads, 2) void paged_importance_kernel(const Pag
 namespace {
 int attn_lds(const PagedAttnParams &p) { return 2 * kWaves * p.rows * (p.D + 4) * 4 + kWaves * 2 * 128 * p.ng; }
 constexpr int64_t kSumsBytes = 2048;  // Scan::pre at the start of the workspace
+static_assert((kThreads + 1) * 4 <= kSumsBytes, "the sums fit");
 }  // namespace
+
+// Most chunks of 16 rows that a sequence of few rows has.
+static int few_chunks(const PagedAttnParams &p) {
+    return (int)((std::min<int64_t>((int64_t)p.seqs.max_q * p.g, kFewRows) + kRows - 1) / kRows);
+}
 
 int64_t paged_attn_plan(PagedAttnParams *p) {
     const int64_t r = (int64_t)p->seqs.max_q * p->g;
     p->rows = (int)std::max<int64_t>(1, std::min<int64_t>(kRows, r));
     const int64_t units = std::max<int64_t>(1, (((int64_t)p->seqs.width << (p->pool.log_tpp + 4)) + kUnitTok - 1) / kUnitTok);
-    const int64_t most = units * p->seqs.n_seqs * p->pool.heads * std::max<int64_t>(1, (r + kRows - 1) / kRows);
+    const int64_t most = (units + kSetup) * p->seqs.n_seqs * p->pool.heads * few_chunks(*p);
     p->groups = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxGroups, (most + kWaves - 1) / kWaves));
-    return kSumsBytes + (int64_t)p->groups * 2 * p->rows * (p->D + 4) * 4;
+    // where every sequence has the most rows there is none of few, and if there is the tiles take it
+    if (r > kFewRows && p->seqs.n_tokens == (int64_t)p->seqs.n_seqs * p->seqs.max_q) p->groups = 0;
+    const int64_t own = p->groups ? kSumsBytes + (int64_t)p->groups * 2 * p->rows * (p->D + 4) * 4 : 0;
+    p->tile_part = p->part + own / 4;
+    return own + paged_tile_plan(p);
 }
 
 hipError_t paged_attn_launch(const PagedAttnParams &p0, hipStream_t st) {
     PagedAttnParams p = p0;
     if (p.seqs.n_seqs == 0 || p.seqs.max_q == 0) return hipSuccess;
     if (p.pool.n_pages == 0) p.seqs.width = 0;
+    if (p.tile_groups) {
+        const hipError_t e = paged_tile_launch(p, st);
+        if (e != hipSuccess || !p.groups) return e;
+    }
     p.sums = (int *)p.part;
     p.part += kSumsBytes / 4;
     const size_t lds = attn_lds(p);
@@ -778,8 +788,7 @@ hipError_t paged_attn_launch(const PagedAttnParams &p0, hipStream_t st) {
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const int64_t items = ((int64_t)p.seqs.max_q * p.g + kRows - 1) / kRows * p.pool.heads;
-    const dim3 grid((unsigned)std::min<int64_t>(items, 1024), p.seqs.n_seqs);
+    const dim3 grid(p.pool.heads * few_chunks(p), p.seqs.n_seqs);
     if (p.D == 128) paged_merge_kernel<128><<<grid, dim3(kThreads), 0, st>>>(p);
     else paged_merge_kernel<64><<<grid, dim3(kThreads), 0, st>>>(p);
     return hipGetLastError();

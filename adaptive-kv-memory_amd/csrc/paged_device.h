@@ -1,0 +1,23 @@
+// Device helpers shared by the attention kernels over the paged 4-bit cache.
+#pragma once
+
+#include "akv_common.h"
+#include "paged.h"
+
+namespace akv {
+namespace {
+
+constexpr float kMinMax = -0x1p126f;  // a finite start of the running maximum: a row that sees nothing stays at p = 0
+
+// 1 / sum of a row's p; 0 for a row that sees nothing (and NaN stays).
+__device__ __forceinline__ float row_inverse(float l) { return l > 0.0f || l != l ? 1.0f / l : 0.0f; }
+// log of the sum of exp, from the maximum (log2 domain) and the sum of p times 2^bias.
+__device__ __forceinline__ float row_lse(float m, float l, float bias) {
+    return l > 0.0f || l != l ? 0.69314718055994531f * (m + (__builtin_log2f(l) - bias)) : -INFINITY;
+}
+__device__ __forceinline__ uint32_t to_pair(bool bf16, float a, float b) {
+    return bf16 ? f32_to_bf16_rne(a) | ((uint32_t)f32_to_bf16_rne(b) << 16) : as_u32((h2){(_Float16)a, (_Float16)b});
+}
+
+}  // namespace
+}  // namespace akv

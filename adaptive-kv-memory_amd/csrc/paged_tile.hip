@@ -1,0 +1,605 @@
+// Attention over the paged 4-bit cache for chunks of a prompt: many query rows a sequence.
+// Bound by the matrix cores and the softmax around them.
+//
+// A workgroup of W waves takes 32 W rows (query token, head of the group) of one sequence and
+// cached head, each wave 32 of them as the columns of 32x32x16 MFMAs, and walks the cache in
+// steps of 64 tokens, two buffers in LDS: while the MFMAs read one step, the next step's tiles
+// are in flight to registers, one wave a tile and side, and are then dequantized into the
+// other buffer, once for all rows.  Keys and values become float16 c s + z, p is rounded to
+// float16 too (a float16 output is off by about 3e-4 of its norm, where its own rounding is
+// 2e-4); scores, running maximum and sum are float32.  Where the rows' log-sums are asked for,
+// which are float32, keys enter as two float16 that add up to them (TWO: 1.06 ms where one
+// takes 0.84, chunks of 65 to 512 tokens on 64 heads after 2k to 32k).
+//   K  [64 tokens][D / 8 chunks] of 16 bytes, chunk c at place c ^ (token & 7) of its row;
+//   V  the PV operand: [tile][32 channels][lane] of 16 bytes, tokens 4 hi + 0..3, 8 + 4 hi + 0..3.
+// S^T = K Q^T leaves a lane with 16 scores of its row for every 32 tokens, which are the PV
+// operand's tokens in order, so p goes from registers to the second product.
+//
+// The rows' tiles of all sequences and heads form one list whose entries count the tokens they
+// see; it is cut into equal runs, one a workgroup.  Entries that several share leave partial
+// states for paged_tile_merge_kernel.
+#include <algorithm>
+
+#include "akv_common.h"
+#include "paged.h"
+#include "paged_device.h"
+
+namespace akv {
+namespace {
+
+constexpr int kStep = 64;               // tokens a step
+constexpr int kSetupTok = 2 * kStep;    // what an entry's start counts
+constexpr float kLag = 8.0f;            // log2 units the running maximum may lag behind
+constexpr float kPBias = 7.0f;          // p is held times 2^7
+
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+struct TileSeq {
+    SeqRows r;
+    int rows, tiles;
+    int64_t a, b;                       // entry t counts a + b t
+    __device__ __forceinline__ int64_t cost(int t) const { return a + b * t; }
+    __device__ __forceinline__ int64_t before(int64_t t) const { return a * t + b * (t * (t - 1) / 2); }
+};
+template <int R>
+__device__ __forceinline__ TileSeq tile_seq(const PagedAttnParams &p, int s) {
+    TileSeq q;
+    q.r = seq_rows(p.seqs, s, p.pool.log_tpp + 4);
+    q.rows = min(q.r.n, p.seqs.max_q) * p.g;
+    q.tiles = q.rows > p.few_rows ? (q.rows + R - 1) / R : 0;
+    const int64_t old = max(q.r.kv - q.r.n, (int64_t)0);
+    q.a = (int64_t)p.g * ((p.causal ? old : q.r.kv) + kSetupTok) + R;
+    q.b = p.causal ? R : 0;
+    return q;
+}
+// Tokens that row `row` sees.
+__device__ __forceinline__ int sees(const PagedAttnParams &p, const TileSeq &q, int row) {
+    return p.causal ? (int)max(q.r.kv - q.r.n + row / p.g + 1, (int64_t)0) : (int)q.r.kv;
+}
+template <int R>
+__device__ __forceinline__ int steps_of(const PagedAttnParams &p, const TileSeq &q, int t) {
+    return max(1, (sees(p, q, min((t + 1) * R, q.rows) - 1) + kStep - 1) / kStep);
+}
+
+template <int R>
+__device__ __forceinline__ void scan_tiles(const PagedAttnParams &p, int64_t *pre, int64_t *wave_sum, int per) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    int64_t mine = 0;
+    for (int i = 0; i < per; ++i) {
+        const int s = t * per + i;
+        if (s < p.seqs.n_seqs) {
+            const TileSeq q = tile_seq<R>(p, s);
+            mine += q.before(q.tiles) * p.pool.heads;
+        }
+    }
+    int64_t inc = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int64_t o = __shfl_up(inc, d);
+        if (lane >= d) inc += o;
+    }
+    if (lane == 63) wave_sum[wave] = inc;
+    __syncthreads();
+    int64_t before = 0;
+    for (int w = 0; w < wave; ++w) before += wave_sum[w];
+    pre[t] = before + inc - mine;
+    if (t == (int)blockDim.x - 1) pre[blockDim.x] = before + inc;
+    __syncthreads();
+}
+
+__device__ __forceinline__ int64_t tile_share(const PagedAttnParams &p, int64_t total) {
+    return max((total + p.tile_groups - 1) / p.tile_groups, (int64_t)4 * kStep * p.g);
+}
+
+__device__ __forceinline__ h2 magic_sub(uint32_t bits, float m) {
+    const h2 mm = {(_Float16)m, (_Float16)m};
+    return as_h2(bits) - mm;
+}
+// The four pairs of a dword of codes (nibbles n and n + 4 of it) as c s + z.
+__device__ __forceinline__ void dequant8(uint32_t w, h2 s, h2 z, uint32_t *o) {
+    const uint32_t v = w >> 8;
+    o[0] = as_u32(__builtin_elementwise_fma(magic_sub((w & 0x000F000Fu) | 0x64006400u, 1024.f), s, z));
+    o[1] = as_u32(__builtin_elementwise_fma(magic_sub((w & 0x00F000F0u) | 0x54005400u, 64.f), s, z));
+    o[2] = as_u32(__builtin_elementwise_fma(magic_sub((v & 0x000F000Fu) | 0x64006400u, 1024.f), s, z));
+    o[3] = as_u32(__builtin_elementwise_fma(magic_sub((v & 0x00F000F0u) | 0x54005400u, 64.f), s, z));
+}
+
+// The same as two float16 that add up to c s + z (to 2^-22 of it).
+__device__ __forceinline__ void dequant8_two(uint32_t w, h2 s, h2 z, uint32_t *o, uint32_t *lo) {
+    const uint32_t v = w >> 8;
+    const h2 c[4] = {magic_sub((w & 0x000F000Fu) | 0x64006400u, 1024.f), magic_sub((w & 0x00F000F0u) | 0x54005400u, 64.f),
+                     magic_sub((v & 0x000F000Fu) | 0x64006400u, 1024.f), magic_sub((v & 0x00F000F0u) | 0x54005400u, 64.f)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float a = __builtin_fmaf((float)c[i][0], (float)s[0], (float)z[0]);
+        const float b = __builtin_fmaf((float)c[i][1], (float)s[1], (float)z[1]);
+        const h2 hi = {(_Float16)a, (_Float16)b};
+        o[i] = as_u32(hi);
+        lo[i] = as_u32((h2){(_Float16)(a - (float)hi[0]), (_Float16)(b - (float)hi[1])});
+    }
+}
+
+// One tile of K or V on its way from memory to LDS.
+template <int D, int NG, bool TWO>
+struct KLoad {
+    uint32_t c[D / 32], m[NG];
+    __device__ __forceinline__ void load(const unsigned char *tile, int lane) {
+        if constexpr (D == 128) {
+            const u4 a = *(const u4 *)(tile + lane * 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[e] = a[e];
+        } else {
+            const u2 a = *(const u2 *)(tile + lane * 8);
+            c[0] = a[0], c[1] = a[1];
+        }
+        const unsigned char *mt = tile + 16 * D + (lane >> 2) * NG * 4;
+        if constexpr (NG == 4) {
+            const u4 a = *(const u4 *)mt;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m[e] = a[e];
+        } else if constexpr (NG == 2) {
+            const u2 a = *(const u2 *)mt;
+            m[0] = a[0], m[1] = a[1];
+        } else {
+            m[0] = *(const uint32_t *)mt;
+        }
+    }
+    // lane (token lane / 4, i = lane % 4): chunk 4 g + i
+    __device__ __forceinline__ void stage(unsigned char *kt, int tile, int lane) const {
+        const int tok = 16 * tile + (lane >> 2), i = lane & 3;
+#pragma unroll
+        for (int g = 0; g < D / 32; ++g) {
+            const uint32_t w = m[g * NG / (D / 32)];
+            const h2 s = as_h2((w & 0xffffu) | (w << 16)), z = as_h2((w >> 16) | (w & 0xffff0000u));
+            uint32_t o[4], r[4];
+            if constexpr (TWO) dequant8_two(c[g], s, z, o, r);
+            else dequant8(c[g], s, z, o);
+            u4 *d = (u4 *)(kt + tok * (2 * D) + (((4 * g + i) ^ (tok & 7)) << 4));
+            *d = (u4){o[0], o[1], o[2], o[3]};
+            if constexpr (TWO) d[kStep * 2 * D / 16] = (u4){r[0], r[1], r[2], r[3]};
+        }
+    }
+};
+template <int D, int NG>
+struct VLoad {
+    static constexpr int NL = NG == 4 ? 2 : 1;  // groups a lane's channels lie in
+    uint32_t c[2][2], s[2][2 * NL], z[2][2 * NL];  // [quad a, a + 2][pair ..]
+    __device__ __forceinline__ void load(const unsigned char *tile, int lane) {
+        const int r = lane & 15, a = (lane >> 4) & 1, h = lane >> 5;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int aq = a + 2 * q;
+            if constexpr (D == 128) {
+                const u4 x = *(const u4 *)(tile + 8 * D + (aq * 16 + r) * 16);
+                c[q][0] = h ? x[1] : x[0];
+                c[q][1] = h ? x[3] : x[2];
+            } else {
+                const u2 x = *(const u2 *)(tile + 8 * D + (aq * 16 + r) * 8);
+                c[q][0] = x[0], c[q][1] = x[1];
+            }
+            // meta dwords (quad, group, pair)
+            const int g0 = NG == 4 ? 2 * h : NG == 2 ? h : 0;
+            const unsigned char *mt = tile + 16 * D + 64 * NG + (aq * NG + g0) * 8;
+            if constexpr (NL == 2) {
+                const u4 x = *(const u4 *)mt, y = *(const u4 *)(mt + 32 * NG);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[q][e] = x[e], z[q][e] = y[e];
+            } else {
+                const u2 x = *(const u2 *)mt, y = *(const u2 *)(mt + 32 * NG);
+                s[q][0] = x[0], s[q][1] = x[1], z[q][0] = y[0], z[q][1] = y[1];
+            }
+        }
+    }
+    __device__ __forceinline__ void mask(int nv, int lane) {  // slots without a token become 0
+        const int a = (lane >> 4) & 1;
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int e = 0; e < 2 * NL; ++e) {
+                const int tok = 4 * (a + 2 * q) + 2 * (e & 1);
+                const uint32_t k = (tok < nv ? 0xffffu : 0u) | (tok + 1 < nv ? 0xffff0000u : 0u);
+                s[q][e] &= k;
+                z[q][e] &= k;
+            }
+    }
+    // lane (row r of the codes, quads a and a + 2, h): the 16 bytes of channels 32 (2 h + l) + 2 r + b
+    __device__ __forceinline__ void stage(unsigned char *vt, int tile, int lane) const {
+        const int r = lane & 15, a = (lane >> 4) & 1, h = lane >> 5;
+        unsigned char *at = vt + (tile * (D / 32) * 64 + a * 32 + 2 * r) * 16;
+        if constexpr (D == 128) {
+#pragma unroll
+            for (int l = 0; l < 2; ++l) {
+                u4 o[2];
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int pr = 0; pr < 2; ++pr) {
+                        const uint32_t w = l ? c[q][pr] >> 8 : c[q][pr];
+                        const h2 sv = as_h2(s[q][(NL == 2 ? 2 * l : 0) + pr]), zv = as_h2(z[q][(NL == 2 ? 2 * l : 0) + pr]);
+                        o[0][2 * q + pr] = as_u32(__builtin_elementwise_fma(magic_sub((w & 0x000F000Fu) | 0x64006400u, 1024.f), sv, zv));
+                        o[1][2 * q + pr] = as_u32(__builtin_elementwise_fma(magic_sub((w & 0x00F000F0u) | 0x54005400u, 64.f), sv, zv));
+                    }
+                u4 *d = (u4 *)(at + (2 * h + l) * 1024);
+                d[0] = o[0], d[1] = o[1];
+            }
+        } else {  // h says which l of the two
+            u4 o[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int pr = 0; pr < 2; ++pr) {
+                    const uint32_t w = c[q][pr] >> (8 * h);
+                    const h2 sv = as_h2(s[q][pr]), zv = as_h2(z[q][pr]);
+                    o[0][2 * q + pr] = as_u32(__builtin_elementwise_fma(magic_sub((w & 0x000F000Fu) | 0x64006400u, 1024.f), sv, zv));
+                    o[1][2 * q + pr] = as_u32(__builtin_elementwise_fma(magic_sub((w & 0x00F000F0u) | 0x54005400u, 64.f), sv, zv));
+                }
+            u4 *d = (u4 *)(at + h * 1024);
+            d[0] = o[0], d[1] = o[1];
+        }
+    }
+};
+
+}  // namespace
+
+template <int D, int NG, int W, bool TWO>
+__global__ __launch_bounds__(64 * W, 2) void paged_tile_kernel(const PagedAttnParams p) {
+    constexpr int R = 32 * W, NB = D / 32, TB = paged_tile_bytes(D, NG), EROW = D + 4;
+    constexpr int KT = (TWO ? 2 : 1) * kStep * 2 * D, BUF = KT + kStep * 2 * D;
+    extern __shared__ __align__(16) unsigned char smem[];
+    int64_t *pre = (int64_t *)smem, *wave_sum = pre + 64 * W + 1;  // before the first step only
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, hi = lane >> 5;
+
+    const int per = (p.seqs.n_seqs + 64 * W - 1) / (64 * W);
+    scan_tiles<R>(p, pre, wave_sum, per);
+    const int64_t total = pre[64 * W];
+    const int64_t share = tile_share(p, total);
+    if (blockIdx.x == 0) {  // for the merge
+        int64_t *sums = (int64_t *)p.sums;
+        sums[threadIdx.x] = pre[threadIdx.x];
+        if (threadIdx.x == 0) sums[64 * W] = total;
+    }
+    int64_t x = min((int64_t)blockIdx.x * share, total);
+    const int64_t x_end = min(x + share, total);
+    if (x >= x_end) return;
+    int at = 0;  // the last sum at or below x
+    for (int step = 32 * W; step > 0; step >>= 1)
+        if (pre[at + step] <= x) at += step;
+    int s = at * per;
+    int64_t off = x - pre[at];
+    __syncthreads();  // pre is done with
+    TileSeq q = tile_seq<R>(p, s);
+    while (off >= q.before(q.tiles) * p.pool.heads) {
+        off -= q.before(q.tiles) * p.pool.heads;
+        q = tile_seq<R>(p, ++s);
+    }
+
+    while (x < x_end) {
+        const int64_t head_cost = q.before(q.tiles);
+        const int h = __builtin_amdgcn_readfirstlane((int)(off / head_cost));
+        const int64_t in_head = off - h * head_cost;
+        int t = 0;
+        for (int step = 1 << (31 - __builtin_clz(q.tiles)); step > 0; step >>= 1)
+            if (t + step < q.tiles && q.before(t + step) <= in_head) t += step;
+        t = __builtin_amdgcn_readfirstlane(t);
+        const int64_t c0 = in_head - q.before(t), cost = q.cost(t);
+        const int64_t c1 = min(cost, c0 + (x_end - x));
+        const int n_steps = steps_of<R>(p, q, t);
+        const int f0 = __builtin_amdgcn_readfirstlane((int)(c0 * n_steps / cost));
+        const int f1 = __builtin_amdgcn_readfirstlane((int)(c1 * n_steps / cost));
+        x += c1 - c0;
+        off += c1 - c0;
+        if (f0 < f1) {
+            const int row0 = t * R + 32 * wave;
+            const int row = min(row0 + col, q.rows - 1);
+            const int head = h * p.g + row % p.g;
+            const bool idle = row0 >= q.rows;
+            const int see = sees(p, q, row);
+            const int see_all = idle ? 0 : sees(p, q, row0), see_any = idle ? 0 : sees(p, q, min(row0 + 31, q.rows - 1));
+            const int kv = (int)q.r.kv;
+
+            // ---- a wave's tile of a step: K for waves 0-3, V for waves 4-7; both where there are only four
+            const int32_t *table = p.seqs.table + s * p.seqs.table_stride;
+            const int log_tpp = p.pool.log_tpp, tl = wave & 3;
+            int pb = (4 * f0) >> log_tpp;
+            int pid = pb + lane < p.seqs.width ? table[pb + lane] : -1;
+            asm volatile("" : "+v"(pid));
+            KLoad<D, NG, TWO> kl;
+            VLoad<D, NG> vl;
+            int nv = 0;         // tokens of the wave's tile of the step that was loaded last
+            uint32_t have = 0;  // and which of the step's four tiles have a page
+            auto load = [&](int step) {
+                if (((4 * step + 3) >> log_tpp) - pb >= 64) {
+                    pb = (4 * step) >> log_tpp;
+                    pid = pb + lane < p.seqs.width ? table[pb + lane] : -1;
+                    asm volatile("" : "+v"(pid));
+                }
+                have = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    have |= ((uint32_t)__builtin_amdgcn_readlane(pid, ((4 * step + i) >> log_tpp) - pb) < p.pool.n_pages ? 1u : 0u) << i;
+                uint32_t page = (uint32_t)__builtin_amdgcn_readlane(pid, ((4 * step + tl) >> log_tpp) - pb);
+                nv = page < p.pool.n_pages ? min(max(kv - 16 * (4 * step + tl), 0), 16) : 0;
+                if (page >= p.pool.n_pages) page = 0;  // read, and masked
+                const unsigned char *tile = p.pool.base + (int64_t)page * p.pool.page_bytes +
+                                            (int64_t)((h << log_tpp) + ((4 * step + tl) & ((1 << log_tpp) - 1))) * TB;
+                if (W == 4 || wave < 4) kl.load(tile, lane);
+                if (W == 4 || wave >= 4) vl.load(tile, lane);
+            };
+            auto stage = [&](unsigned char *buf) {
+                if (W == 4 || wave < 4) kl.stage(buf, tl, lane);
+                if (W == 4 || wave >= 4) {
+                    if (nv < 16) vl.mask(nv, lane);
+                    vl.stage(buf + KT, tl, lane);
+                }
+            };
+            // a tile of rows that see nothing has a step without loads
+            const int f2 = min(f1, (sees(p, q, min((t + 1) * R, q.rows) - 1) + kStep - 1) / kStep);
+            if (f0 < f2) load(f0);
+
+            // ---- the query operand: chunk c = 2 st + hi, channels 8 c + (0, 4, 1, 5, 2, 6, 3, 7)
+            h8 qop[D / 16];
+            float kx;
+            {
+                const unsigned char *qr = p.q + (q.r.begin + row / p.g) * p.q_t + head * p.q_h;
+                u4 w[D / 16];
+#pragma unroll
+                for (int st = 0; st < D / 16; ++st) w[st] = *(const u4 *)(qr + (2 * st + hi) * 16);
+                float top = 0.0f;
+                float y[D / 16][8];
+                if (p.q_bf16) {
+#pragma unroll
+                    for (int st = 0; st < D / 16; ++st)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            y[st][i] = __builtin_bit_cast(float, i & 1 ? w[st][i >> 1] & 0xffff0000u : w[st][i >> 1] << 16);
+                } else {
+#pragma unroll
+                    for (int st = 0; st < D / 16; ++st)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) y[st][i] = (float)as_h2(w[st][i >> 1])[i & 1];
+                }
+#pragma unroll
+                for (int st = 0; st < D / 16; ++st)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) top = __builtin_fmaxf(top, __builtin_fabsf(y[st][i]));
+                top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+                const int ex = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 0;  // the row's maximum goes to [1/2, 1)
+#pragma unroll
+                for (int st = 0; st < D / 16; ++st) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[st][i] = __builtin_ldexpf(y[st][i], -ex);
+                    qop[st] = (h8){(_Float16)y[st][0], (_Float16)y[st][4], (_Float16)y[st][1], (_Float16)y[st][5],
+                                   (_Float16)y[st][2], (_Float16)y[st][6], (_Float16)y[st][3], (_Float16)y[st][7]};
+                }
+                kx = __builtin_ldexpf(p.scale_log2, ex);
+            }
+
+            float mx = kMinMax, l = 0.0f;
+            f16v acc[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[b][i] = 0.0f;
+
+            if (f0 < f2) stage(smem);
+            __syncthreads();
+            for (int step = f0; step < f2; ++step) {
+                const unsigned char *buf = smem + ((step - f0) & 1) * BUF;
+                const uint32_t here = have;
+                if (step + 1 < f2) load(step + 1);
+                if (kStep * step < see_any) {
+                    f16v sc[2];
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) sc[b][i] = 0.0f;
+#pragma unroll
+                        for (int st = 0; st < D / 16; ++st) {
+                            const h8 *a = (const h8 *)(buf + (32 * b + col) * (2 * D) + (((2 * st + hi) ^ (col & 7)) << 4));
+                            sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], qop[st], sc[b], 0, 0, 0);
+                            if constexpr (TWO) sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[kStep * 2 * D / 16], qop[st], sc[b], 0, 0, 0);
+                        }
+                    }
+                    const bool clean = kStep * (step + 1) <= see_all && here == 15u;
+                    if (!clean) {
+#pragma unroll
+                        for (int b = 0; b < 2; ++b)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const int tok = 32 * b + 8 * (i >> 2) + 4 * hi + (i & 3);
+                                if (kStep * step + tok >= see || !(here >> (tok >> 4) & 1)) sc[b][i] = -INFINITY;
+                            }
+                    }
+                    float top = sc[0][0];
+#pragma unroll
+                    for (int i = 1; i < 32; ++i) top = __builtin_fmaxf(top, sc[i >> 4][i & 15]);
+                    top *= kx;
+                    if (__builtin_amdgcn_ballot_w64(top > mx + kLag)) {
+                        const float mn = __builtin_fmaxf(mx, __builtin_fmaxf(top, __shfl_xor(top, 32)));
+                        const float alpha = __builtin_amdgcn_exp2f(mx - mn);
+                        l *= alpha;
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) acc[b] *= alpha;
+                        mx = mn;
+                    }
+                    const float bias = kPBias - mx;
+#pragma unroll
+                    for (int tile = 0; tile < 4; ++tile) {
+                        float pr[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            pr[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[tile >> 1][8 * (tile & 1) + i], kx, bias));
+                        l += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
+                        const h8 pop = {(_Float16)pr[0], (_Float16)pr[1], (_Float16)pr[2], (_Float16)pr[3],
+                                        (_Float16)pr[4], (_Float16)pr[5], (_Float16)pr[6], (_Float16)pr[7]};
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) {
+                            const h8 a = *(const h8 *)(buf + KT + ((tile * NB + b) * 64 + lane) * 16);
+                            acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pop, acc[b], 0, 0, 0);
+                        }
+                    }
+                }
+                if (step + 1 < f2) stage(smem + ((step + 1 - f0) & 1) * BUF);
+                __syncthreads();
+            }
+
+            l += __shfl_xor(l, 32);
+            if (row0 + col < q.rows) {
+                if (f0 == 0 && f1 == n_steps) {
+                    const int64_t o = (q.r.begin + row / p.g) * p.Hq + head;
+                    const float inv = row_inverse(l);
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float v[4] = {acc[b][4 * i] * inv, acc[b][4 * i + 1] * inv, acc[b][4 * i + 2] * inv, acc[b][4 * i + 3] * inv};
+                            *(u2 *)((unsigned char *)p.out + (o * D + 32 * b + 8 * i + 4 * hi) * 2) =
+                                (u2){to_pair(p.q_bf16, v[0], v[1]), to_pair(p.q_bf16, v[2], v[3])};
+                        }
+                    if (p.lse && hi == 0) p.lse[o] = row_lse(mx, l, kPBias);
+                } else {
+                    float *pr = p.tile_part + ((int64_t)(2 * blockIdx.x + (f0 == 0 ? 1 : 0)) * R + 32 * wave + col) * EROW;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            *(f4 *)(pr + 32 * b + 8 * i + 4 * hi) = (f4){acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]};
+                    if (hi == 0) pr[D] = mx, pr[D + 1] = l;
+                }
+            }
+        }
+        if (x < x_end && off >= head_cost * p.pool.heads) {
+            do q = tile_seq<R>(p, ++s);
+            while (q.tiles == 0);
+            off = 0;
+        }
+    }
+}
+
+// Entries that several workgroups share: 16 rows of one a workgroup, joined in order.
+template <int D, int W>
+__global__ __launch_bounds__(256) void paged_tile_merge_kernel(const PagedAttnParams p) {
+    constexpr int R = 32 * W, EROW = D + 4, CH = D / 16, B = 4;
+    const int64_t *sums = (const int64_t *)p.sums;
+    const int per = (p.seqs.n_seqs + 64 * W - 1) / (64 * W);
+    const int s = blockIdx.y, k = s / per;
+    int64_t at = sums[k];
+    const int64_t share = tile_share(p, sums[64 * W]);
+    const TileSeq q = tile_seq<R>(p, s);
+    for (int i = k * per; i < s; ++i) {
+        const TileSeq o = tile_seq<R>(p, i);
+        at += o.before(o.tiles) * p.pool.heads;
+    }
+    constexpr int G16 = R / 16;
+    const int64_t blocks = (int64_t)q.tiles * p.pool.heads * G16;
+    for (int64_t blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
+        const int g16 = (int)(blk % G16), item = (int)(blk / G16);
+        const int h = item / q.tiles, t = item - h * q.tiles;
+        const int in = 16 * g16 + (threadIdx.x >> 4), ch = (threadIdx.x & 15) * CH;
+        const int row = t * R + in;
+        if (row >= q.rows) continue;
+        const int64_t u0 = at + h * q.before(q.tiles) + q.before(t), cost = q.cost(t);
+        const int n_steps = steps_of<R>(p, q, t);
+        const int64_t g0 = u0 / share, g1 = (u0 + cost - 1) / share;
+        if (g0 == g1) continue;
+        float o[CH];
+        float M = kMinMax, L = 0.f;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) o[i] = 0.f;
+        bool whole = false;
+        for (int64_t g = g0; g <= g1 && !whole; g += B) {
+            f4 v[B][CH / 4];
+            f2 ml[B];
+            bool use[B];
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                const int64_t gi = min(g + i, g1);
+                const int64_t c0 = max(gi * share - u0, (int64_t)0), c1 = min((gi + 1) * share - u0, cost);
+                const int f0 = (int)(c0 * n_steps / cost), f1 = (int)(c1 * n_steps / cost);
+                use[i] = f0 < f1 && g + i <= g1;
+                whole |= f0 == 0 && f1 == n_steps;
+                const float *pr = p.tile_part + ((2 * gi + (f0 == 0 ? 1 : 0)) * R + in) * EROW;
+#pragma unroll
+                for (int c = 0; c < CH / 4; ++c) v[i][c] = use[i] ? ((const f4 *)(pr + ch))[c] : (f4){0.f, 0.f, 0.f, 0.f};
+                ml[i] = use[i] ? *(const f2 *)(pr + D) : (f2){kMinMax, 0.f};
+            }
+            float mn = M;
+#pragma unroll
+            for (int i = 0; i < B; ++i) mn = __builtin_fmaxf(mn, ml[i][0]);
+            const float a = __builtin_amdgcn_exp2f(M - mn);
+            L *= a;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) o[c] *= a;
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                const float b = __builtin_amdgcn_exp2f(ml[i][0] - mn);
+                L = __builtin_fmaf(ml[i][1], b, L);
+#pragma unroll
+                for (int c = 0; c < CH; ++c) o[c] = __builtin_fmaf(v[i][c >> 2][c & 3], b, o[c]);
+            }
+            M = mn;
+        }
+        if (whole) continue;  // one workgroup had every step of it, and wrote
+        const int head = h * p.g + row % p.g;
+        const int64_t ro = (q.r.begin + row / p.g) * p.Hq + head;
+        const float inv = row_inverse(L);
+#pragma unroll
+        for (int c = 0; c < CH / 4; ++c)
+            *(u2 *)((unsigned char *)p.out + (ro * D + ch + 4 * c) * 2) =
+                (u2){to_pair(p.q_bf16, o[4 * c] * inv, o[4 * c + 1] * inv), to_pair(p.q_bf16, o[4 * c + 2] * inv, o[4 * c + 3] * inv)};
+        if (p.lse && ch == 0) p.lse[ro] = row_lse(M, L, kPBias);
+    }
+}
+
+namespace {
+constexpr int kTileWaves = 8, kTileGroups = 256;  // one workgroup a compute unit
+constexpr int64_t kTileSums = 8192;               // scan_tiles' sums at the start of the workspace
+static_assert((64 * kTileWaves + 1) * 8 <= kTileSums, "the sums fit");
+
+template <int D, int NG, bool TWO>
+hipError_t tile_go_as(const PagedAttnParams &p, hipStream_t st) {
+    constexpr int W = kTileWaves;
+    constexpr int LDS = 2 * (TWO ? 3 : 2) * kStep * 2 * D;
+    static_assert((64 * W + 1 + W) * 8 <= LDS, "the sums fit the buffers");
+    auto kern = paged_tile_kernel<D, NG, W, TWO>;
+    if (LDS > 48 * 1024) (void)hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    kern<<<dim3(p.tile_groups), dim3(64 * W), LDS, st>>>(p);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    const int64_t blocks = ((int64_t)p.seqs.max_q * p.g + 32 * W - 1) / (32 * W) * p.pool.heads * (2 * W);
+    paged_tile_merge_kernel<D, W><<<dim3((unsigned)std::min<int64_t>(blocks, 2048), p.seqs.n_seqs), dim3(256), 0, st>>>(p);
+    return hipGetLastError();
+}
+template <int D, int NG>
+hipError_t tile_go(const PagedAttnParams &p, hipStream_t st) {
+    return p.lse ? tile_go_as<D, NG, true>(p, st) : tile_go_as<D, NG, false>(p, st);
+}
+}  // namespace
+
+int64_t paged_tile_plan(PagedAttnParams *p) {
+    const int64_t rows = (int64_t)p->seqs.max_q * p->g;
+    p->tile_groups = 0;
+    if (rows <= kFewRows) return 0;
+    p->few_rows = p->groups ? kFewRows : 0;
+    // steps that there can be: a workgroup has four at least
+    const int64_t steps = std::max<int64_t>(1, (((int64_t)p->seqs.width << (p->pool.log_tpp + 4)) + kStep - 1) / kStep);
+    const int64_t items = (rows + 32 * kTileWaves - 1) / (32 * kTileWaves) * p->pool.heads * p->seqs.n_seqs;
+    p->tile_groups = (int)std::max<int64_t>(1, std::min<int64_t>(kTileGroups, items * steps));
+    return kTileSums + (int64_t)p->tile_groups * 2 * 32 * kTileWaves * (p->D + 4) * 4;
+}
+
+hipError_t paged_tile_launch(const PagedAttnParams &p0, hipStream_t st) {
+    PagedAttnParams p = p0;
+    p.sums = (int *)p.tile_part;
+    p.tile_part += kTileSums / 4;
+    if (p.D == 128) {
+        if (p.ng == 4) return tile_go<128, 4>(p, st);
+        if (p.ng == 2) return tile_go<128, 2>(p, st);
+        return tile_go<128, 1>(p, st);
+    }
+    if (p.ng == 2) return tile_go<64, 2>(p, st);
+    return tile_go<64, 1>(p, st);
+}
+
+}  // namespace akv

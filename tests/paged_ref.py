@@ -86,14 +86,15 @@ class Pool:
         return [a + b for a, b in self.parts(layer, table, pos)]
 
 
-def attention(q, kp, vp, scale, seen, half):
+def attention(q, kp, vp, scale, seen, half, rounded=False):
     """One sequence: q (m, Hq, D), parts of its cached keys and values (n, H, D), row i sees the
     first seen[i] tokens.  Returns out, lse and how far each may be off: `half` is half a step
     of the output's type.
 
     The scores are exact but for float32 sums (at most 64 roundings of terms that add up to
     `mass`); p and p * scale are rounded to float16 (2^-11 each, or 2^-25 absolute below its
-    normal range, p times 4 and codes up to 15)."""
+    normal range, p times 4 and codes up to 15).  `rounded`: the keys are rounded to float16 too,
+    half a step (2^-11) of each, which moves a score by 2^-11 of the terms |q||k| that it sums."""
     m, Hq, D = q.shape
     n, H = kp[0].shape[:2]
     out, lse = np.zeros((m, Hq, D)), np.full((m, Hq), -np.inf)
@@ -107,6 +108,8 @@ def attention(q, kp, vp, scale, seen, half):
             x = scale * ((kc + kz) @ q[i, h])
             mass = scale * ((np.abs(kc) + np.abs(kz)) @ np.abs(q[i, h])).max()
             d = 64 * 2.0 ** -24 * mass
+            if rounded:
+                d += 2.0 ** -11 * scale * (np.abs(kc + kz) @ np.abs(q[i, h])).max()
             e = np.exp(x - x.max())
             l = e.sum()
             p = e / l

@@ -149,7 +149,11 @@ def _check_attention(w, Hq, dt, causal, layer=0, seed=9, big=1.0):
     scale = w.D ** -0.5 / big
     out, lse = akv.paged_attention(q, w.pool, w.batch, layer, sm_scale=scale, causal=causal, return_lse=True)
     only = akv.paged_attention(q, w.pool, w.batch, layer, sm_scale=scale, causal=causal)
-    assert out.dtype == q.dtype and torch.equal(only, out)
+    # chunks of many rows round the keys where no log-sums are asked for
+    many = [m * Hq // w.H > 80 for m in w.q]
+    assert out.dtype == only.dtype == q.dtype
+    for s in range(len(w.q)):
+        assert many[s] or torch.equal(only[w.rows(s)], out[w.rows(s)])
     half = torch.finfo(q.dtype).eps / 2
     worst = 0.0
     for s, (n, m) in enumerate(zip(w.kv, w.q)):
@@ -167,6 +171,10 @@ def _check_attention(w, Hq, dt, causal, layer=0, seed=9, big=1.0):
         assert (np.abs(go - eo) <= bo).all(), f"sequence {s}: {(np.abs(go - eo) / np.maximum(bo, 1e-30)).max():.2f} of the bound"
         assert (np.abs(gl[ok] - el[ok]) <= bl[ok]).all(), f"sequence {s}: lse off by {np.abs(gl[ok] - el[ok]).max():.2e}"
         worst = max(worst, float((np.abs(go - eo) / np.maximum(bo, 1e-30)).max()))
+        if many[s]:
+            go = only[r].double().cpu().numpy()
+            _, _, bo, _ = ref.attention(q[r].double().cpu().numpy(), kp, vp, scale, seen, half, rounded=True)
+            assert (np.abs(go - eo) <= bo).all(), f"sequence {s}: {(np.abs(go - eo) / np.maximum(bo, 1e-30)).max():.2f} of the bound"
     print(f"  worst share of the bound {worst:.2f}")
     return q, lse
 
