@@ -274,14 +274,14 @@ def load() -> ctypes.CDLL:
     lib.akv_timeline_fetch.argtypes = [_vp, _i64]
     lib.akv_timeline_clear.restype = ctypes.c_int
     lib.akv_timeline_clear.argtypes = [_vp]
-    for name, args in (("akv_paged_append", PagedRowsArgs), ("akv_paged_read", PagedRowsArgs), ("akv_paged_attn", PagedAttnArgs),
-                       ("akv_paged_importance", PagedImportanceArgs), ("akv_paged_compact", PagedCompactArgs)):
+    # their structs as addresses: callers pack them as bytes or fill the mirrors
+    for name in ("akv_paged_append", "akv_paged_read", "akv_paged_attn", "akv_paged_importance", "akv_paged_compact"):
         getattr(lib, name).restype = ctypes.c_int
-        getattr(lib, name).argtypes = [ctypes.POINTER(args), _vp]
+        getattr(lib, name).argtypes = [_vp, _vp]
     lib.akv_paged_attn_workspace_bytes.restype = _i64
-    lib.akv_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttnArgs)]
+    lib.akv_paged_attn_workspace_bytes.argtypes = [_vp]
     lib.akv_paged_copy.restype = ctypes.c_int
-    lib.akv_paged_copy.argtypes = [ctypes.POINTER(PagedPool), _vp, _vp, _i64, _vp]
+    lib.akv_paged_copy.argtypes = [_vp, _vp, _vp, _i64, _vp]
     if lib.akv_abi_version() != ABI_VERSION:
         raise RuntimeError(f"{LIB_PATH} has ABI {lib.akv_abi_version()}, expected {ABI_VERSION}")
     for i, st in enumerate(STRUCTS):

@@ -20,7 +20,7 @@ no gradient.  The tile layout is written out in include/akv_hip.h."""
 from __future__ import annotations
 
 import ctypes
-from contextlib import nullcontext
+import struct
 from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
@@ -28,12 +28,29 @@ import torch
 from . import _native as nat
 
 _QUERY = (torch.float16, torch.bfloat16)
-_byref = ctypes.byref
+_stream, _current = torch._C._cuda_getCurrentRawStream, torch.cuda.current_device
+
+# the args structs, packed in one call (a ctypes structure with its nested ones costs five times
+# that, which a decode step's calls would feel)
+_POOL, _BATCH = ctypes.sizeof(nat.PagedPool), ctypes.sizeof(nat.PagedBatch)
+_ROWS = struct.Struct(f"@4i{_POOL}s{_BATCH}s6q")
+_ATTN = struct.Struct(f"@5if{_POOL}s{_BATCH}s7q")
+_IMPORTANCE = struct.Struct(f"@6i2f{_POOL}s{_BATCH}s9q")
+_COMPACT = struct.Struct(f"@2i{_POOL}s4q2i4q")
+for _s, _c in ((_ROWS, nat.PagedRowsArgs), (_ATTN, nat.PagedAttnArgs), (_IMPORTANCE, nat.PagedImportanceArgs),
+               (_COMPACT, nat.PagedCompactArgs)):
+    assert _s.size == ctypes.sizeof(_c), _c
 
 
-def _device(t: torch.Tensor):
-    """The context in which a tensor's device is the current one."""
-    return nullcontext() if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _call(index: int, what: str, fn, *args) -> None:
+    """fn(*args, stream): on the current stream of the device, which is made the current one."""
+    if index == _current():
+        rc = fn(*args, _stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _stream(index))
+    if rc:
+        nat.check(rc, what)
 
 
 def _check_device(pool: "PagedPool", *tensors) -> None:
@@ -48,7 +65,8 @@ def _int32(name: str, t: torch.Tensor, dims: int) -> torch.Tensor:
     """An int32 tensor of ``dims`` dimensions, its last one consecutive."""
     if t.dim() != dims or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be an int32 tensor of {dims} dimension{'s' if dims > 1 else ''}")
-    t = t.to(torch.int32)
+    if t.dtype != torch.int32:
+        t = t.to(torch.int32)
     return t if t.numel() == 0 or t.stride(-1) == 1 else t.contiguous()
 
 
@@ -70,10 +88,10 @@ class PagedPool:
         self.num_layers, self.num_pages, self.heads = data.shape[:3]
         self.page_size = 16 * data.shape[3]
         self._index = data.get_device()
-        self._c = nat.PagedPool(data.data_ptr(), self.num_pages, self.num_layers, self.heads, head_dim, self.page_size,
-                                group_size, 0)
+        self._c = bytes(nat.PagedPool(data.data_ptr(), self.num_pages, self.num_layers, self.heads, head_dim,
+                                      self.page_size, group_size, 0))
         # every refusal of a pool's shape is the library's
-        nat.check(nat.load().akv_paged_copy(_byref(self._c), None, None, 0, None), "PagedPool")
+        nat.check(nat.load().akv_paged_copy(self._c, None, None, 0, None), "PagedPool")
 
     @classmethod
     def empty(cls, num_layers: int, num_pages: int, heads: int, head_dim: int, page_size: int = 16,
@@ -114,8 +132,9 @@ class PagedBatch:
         self._index = self.page_table.get_device()
         if self.kv_lens.get_device() != self._index or self.q_starts.get_device() != self._index:
             raise ValueError("a batch's tensors live on one device")
-        self._c = nat.PagedBatch(self.page_table.data_ptr(), self.kv_lens.data_ptr(), self.q_starts.data_ptr(),
-                                 self.page_table.stride(0), self.n_tokens, S, W, self.max_q, 0)
+        self._c = bytes(nat.PagedBatch(self.page_table.data_ptr(), self.kv_lens.data_ptr(), self.q_starts.data_ptr(),
+                                       self.page_table.stride(0), self.n_tokens, S, W, self.max_q, 0))
+        self._workspace: dict = {}  # bytes an attention call needs, by the sizes they depend on
 
 
 def _rows(x: torch.Tensor, name: str, T: int, H: int, D: int) -> torch.Tensor:
@@ -129,10 +148,12 @@ def _rows(x: torch.Tensor, name: str, T: int, H: int, D: int) -> torch.Tensor:
     return x
 
 
-def _rows_args(pool: PagedPool, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, layer: int) -> nat.PagedRowsArgs:
+def _rows_args(pool: PagedPool, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, layer: int) -> bytes:
     e = k.element_size()
-    return nat.PagedRowsArgs(nat.ABI_VERSION, layer, nat.dtype_code(k.dtype), 0, pool._c, batch._c, k.data_ptr(),
-                             v.data_ptr(), k.stride(0) * e, k.stride(1) * e, v.stride(0) * e, v.stride(1) * e)
+    kt, kh, _ = k.stride()
+    vt, vh, _ = v.stride()
+    return _ROWS.pack(nat.ABI_VERSION, layer, nat.dtype_code(k.dtype), 0, pool._c, batch._c, k.data_ptr(), v.data_ptr(),
+                      kt * e, kh * e, vt * e, vh * e)
 
 
 def paged_append(pool: PagedPool, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, layer: int = 0) -> None:
@@ -144,13 +165,11 @@ def paged_append(pool: PagedPool, batch: PagedBatch, k: torch.Tensor, v: torch.T
     arithmetic.  Values past +-61440 are clamped; a group with a value that is not finite reads
     back as NaN."""
     T, H, D = batch.n_tokens, pool.heads, pool.head_dim
-    nat.require_device(k, v)
     _check_device(pool, k, v, batch.page_table)
     if k.dtype != v.dtype:
         raise TypeError(f"k is {k.dtype} and v {v.dtype}")
     k, v = _rows(k, "k", T, H, D), _rows(v, "v", T, H, D)
-    with _device(k):
-        nat.check(nat.load().akv_paged_append(_byref(_rows_args(pool, batch, k, v, layer)), nat.stream_of(k)), "paged_append")
+    _call(pool._index, "paged_append", nat.load().akv_paged_append, _rows_args(pool, batch, k, v, layer))
 
 
 def paged_read(pool: PagedPool, batch: PagedBatch, layer: int = 0,
@@ -159,13 +178,11 @@ def paged_read(pool: PagedPool, batch: PagedBatch, layer: int = 0,
     _check_device(pool, batch.page_table)
     nat.dtype_code(dtype)
     k, v = torch.empty(2, batch.n_tokens, pool.heads, pool.head_dim, dtype=dtype, device=pool.data.device).unbind(0)
-    with _device(k):
-        nat.check(nat.load().akv_paged_read(_byref(_rows_args(pool, batch, k, v, layer)), nat.stream_of(k)), "paged_read")
+    _call(pool._index, "paged_read", nat.load().akv_paged_read, _rows_args(pool, batch, k, v, layer))
     return k, v
 
 
 def _queries(q: torch.Tensor, pool: PagedPool, batch: PagedBatch) -> torch.Tensor:
-    nat.require_device(q)
     _check_device(pool, q, batch.page_table)
     if q.dtype not in _QUERY:
         raise TypeError("paged attention takes float16 or bfloat16 queries")
@@ -186,17 +203,19 @@ def paged_attention(q: torch.Tensor, pool: PagedPool, batch: PagedBatch, layer: 
     lib = nat.load()
     out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
     lse = torch.empty(T, Hq, dtype=torch.float32, device=q.device) if return_lse else None
-    a = nat.PagedAttnArgs(nat.ABI_VERSION, layer, Hq, nat.dtype_code(q.dtype), int(causal),
-                          nat.default_sm_scale(D) if sm_scale is None else float(sm_scale), pool._c, batch._c,
-                          q.data_ptr(), q.stride(0) * 2, q.stride(1) * 2, out.data_ptr(),
-                          None if lse is None else lse.data_ptr(), None, 0)
-    ref = _byref(a)
-    need = lib.akv_paged_attn_workspace_bytes(ref)
-    if need > 0:
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), need
-    with _device(q):
-        nat.check(lib.akv_paged_attn(ref, nat.stream_of(q)), "paged_attention")
+    qt, qh, _ = q.stride()
+    head = (nat.ABI_VERSION, layer, Hq, nat.dtype_code(q.dtype), int(causal),
+            nat.default_sm_scale(D) if sm_scale is None else float(sm_scale), pool._c, batch._c, q.data_ptr(), qt * 2, qh * 2,
+            out.data_ptr(), 0 if lse is None else lse.data_ptr())
+    key = (D, pool.group_size, pool.heads, pool.page_size, Hq)
+    need = batch._workspace.get(key)
+    if need is None:
+        need = lib.akv_paged_attn_workspace_bytes(_ATTN.pack(*head, 0, 0))
+        if need >= 0:
+            batch._workspace[key] = need
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+    _call(pool._index, "paged_attention", lib.akv_paged_attn,
+          _ATTN.pack(*head, 0, 0) if ws is None else _ATTN.pack(*head, ws.data_ptr(), need))
     return out if lse is None else (out, lse)
 
 
@@ -220,27 +239,25 @@ def paged_importance(q: torch.Tensor, lse: torch.Tensor, pool: PagedPool, batch:
             raise ValueError(f"scores must be ({batch.n_seqs}, tokens) float32")
         if t.shape[1] > 1 and t.stride(1) != 1:
             raise ValueError("a sequence's scores must be consecutive")
-    lse = lse.contiguous()
-    a = nat.PagedImportanceArgs(nat.ABI_VERSION, layer, Hq, nat.dtype_code(q.dtype), int(causal), int(q_window),
-                                nat.default_sm_scale(D) if sm_scale is None else float(sm_scale), float(decay), pool._c,
-                                batch._c, q.data_ptr(), q.stride(0) * 2, q.stride(1) * 2, lse.data_ptr(),
-                                scores.data_ptr(), dst.data_ptr(), scores.shape[1], scores.stride(0), dst.stride(0))
-    with _device(q):
-        nat.check(nat.load().akv_paged_importance(_byref(a), nat.stream_of(q)), "paged_importance")
+    if not lse.is_contiguous():
+        lse = lse.contiguous()
+    qt, qh, _ = q.stride()
+    args = _IMPORTANCE.pack(nat.ABI_VERSION, layer, Hq, nat.dtype_code(q.dtype), int(causal), int(q_window),
+                            nat.default_sm_scale(D) if sm_scale is None else float(sm_scale), float(decay), pool._c,
+                            batch._c, q.data_ptr(), qt * 2, qh * 2, lse.data_ptr(), scores.data_ptr(), dst.data_ptr(),
+                            scores.shape[1], scores.stride(0), dst.stride(0))
+    _call(pool._index, "paged_importance", nat.load().akv_paged_importance, args)
     return dst
 
 
 def copy_pages(pool: PagedPool, src: torch.Tensor, dst: torch.Tensor) -> None:
     """Page dst[i] of every layer becomes a copy of page src[i].  int32 tensors on the pool's
     device; no page may be written twice, or both read and written."""
-    nat.require_device(src, dst)
-    src, dst = _int32("src", src, 1), _int32("dst", dst, 1)
     _check_device(pool, src, dst)
+    src, dst = _int32("src", src, 1), _int32("dst", dst, 1)
     if src.shape != dst.shape:
         raise ValueError("src and dst must be of one length")
-    with _device(src):
-        nat.check(nat.load().akv_paged_copy(_byref(pool._c), src.data_ptr(), dst.data_ptr(), src.shape[0], nat.stream_of(src)),
-                  "copy_pages")
+    _call(pool._index, "copy_pages", nat.load().akv_paged_copy, pool._c, src.data_ptr(), dst.data_ptr(), src.shape[0])
 
 
 def compact_pages(pool: PagedPool, src_table: torch.Tensor, dst_table: torch.Tensor, keep: torch.Tensor,
@@ -250,18 +267,16 @@ def compact_pages(pool: PagedPool, src_table: torch.Tensor, dst_table: torch.Ten
 
     keep (S, K) and n_keep (S,) int32.  No slot that is read may be written, except tokens that
     stay where they are.  Slots behind the last token keep what they hold."""
-    nat.require_device(src_table, dst_table, keep, n_keep)
-    src_table, dst_table, keep = (_int32(n, t, 2) for n, t in (("src_table", src_table), ("dst_table", dst_table), ("keep", keep)))
-    n_keep = _int32("n_keep", n_keep, 1)
     _check_device(pool, src_table, dst_table, keep, n_keep)
+    src_table, dst_table = _int32("src_table", src_table, 2), _int32("dst_table", dst_table, 2)
+    keep, n_keep = _int32("keep", keep, 2), _int32("n_keep", n_keep, 1)
     S = n_keep.shape[0]
     if src_table.shape[0] != S or dst_table.shape[0] != S or keep.shape[0] != S:
         raise ValueError(f"{S} sequences take {S} rows of src_table, dst_table and keep")
-    a = nat.PagedCompactArgs(nat.ABI_VERSION, S, pool._c, src_table.data_ptr(), dst_table.data_ptr(), src_table.stride(0),
-                             dst_table.stride(0), src_table.shape[1], dst_table.shape[1], keep.data_ptr(), n_keep.data_ptr(),
-                             keep.stride(0), keep.shape[1])
-    with _device(keep):
-        nat.check(nat.load().akv_paged_compact(_byref(a), nat.stream_of(keep)), "compact_pages")
+    args = _COMPACT.pack(nat.ABI_VERSION, S, pool._c, src_table.data_ptr(), dst_table.data_ptr(), src_table.stride(0),
+                         dst_table.stride(0), src_table.shape[1], dst_table.shape[1], keep.data_ptr(), n_keep.data_ptr(),
+                         keep.stride(0), keep.shape[1])
+    _call(pool._index, "compact_pages", nat.load().akv_paged_compact, args)
 
 
 class PageLedger:

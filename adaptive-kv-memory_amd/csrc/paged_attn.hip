@@ -480,53 +480,52 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
         }
     }
 
-    // join what the runs left: entries of one item are neighbours
+    // join what the runs left: entries of one item are neighbours, the last of them ends the
+    // item or the workgroup's run
     __syncthreads();
-    const int row_t = threadIdx.x >> 4, ch = (threadIdx.x & 15) * (D / 16);
-    float o[8];
-    float M = 0.f, L = 0.f;
-    bool open = false, began = false;
+    const int flags = lane < 2 * kWaves ? e_flags[lane] : 0;
+    uint32_t used = (uint32_t)__builtin_amdgcn_ballot_w64(flags & 1);
+    const uint32_t starts = (uint32_t)__builtin_amdgcn_ballot_w64(flags & 2), ends = (uint32_t)__builtin_amdgcn_ballot_w64(flags & 4);
+    constexpr int CH = D / 16;
+    const int row_t = threadIdx.x >> 4, ch = (threadIdx.x & 15) * CH;
+    if (row_t >= p.rows) return;
+    while (used) {
+        const uint32_t first = used & -used;
+        float o[CH];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = 0.f;
-    for (int e = 0; e < 2 * kWaves; ++e) {
-        const int f = e_flags[e];
-        if (!(f & 1)) continue;
-        if (!open) began = f & 2;
-        if (row_t < p.rows) {
+        for (int i = 0; i < CH; ++i) o[i] = 0.f;
+        float M = kMinMax, L = 0.f;
+        int e;
+        do {
+            e = __builtin_ctz(used);
+            used &= used - 1;
             const float *er = entries + (e * p.rows + row_t) * EROW;
-            const float m = er[D], le = er[D + 1];
-            const float mn = open ? __builtin_fmaxf(M, m) : m;
-            const float a = open ? __builtin_amdgcn_exp2f(M - mn) : 0.f, b = __builtin_amdgcn_exp2f(m - mn);
+            const f2 ml = *(const f2 *)(er + D);
+            const float mn = __builtin_fmaxf(M, ml[0]);
+            const float a = __builtin_amdgcn_exp2f(M - mn), b = __builtin_amdgcn_exp2f(ml[0] - mn);
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) o[i] = open ? __builtin_fmaf(er[ch + i], b, o[i] * a) : er[ch + i];
-            L = open ? __builtin_fmaf(le, b, L * a) : le;
+            for (int i = 0; i < CH; ++i) o[i] = __builtin_fmaf(er[ch + i], b, o[i] * a);
+            L = __builtin_fmaf(ml[1], b, L * a);
             M = mn;
-        }
-        open = !(f & 4);
-        bool last = !open;
-        if (open) {  // nothing more of it in this workgroup?
-            last = true;
-            for (int e2 = e + 1; e2 < 2 * kWaves; ++e2) last &= !(e_flags[e2] & 1);
-        }
-        if (!last) continue;
-        if (began && (f & 4)) {
+        } while (!(ends >> e & 1) && used);
+        const bool began = starts & first;
+        if (began && (ends >> e & 1)) {
             const SeqWork sw = seq_work(p, scanned_rows(p, sc, e_seq[e]));
             const int it = e_item[e], h = it / sw.chunks, row = (it - h * sw.chunks) * kRows + row_t;
-            if (row_t < kRows && row < sw.rows && row_t < p.rows) {
-                if constexpr (D == 128) {
-                    write_row(p, sw.r, h, row, ch, o, M, L);
-                } else {  // 4 channels a thread: pairs of threads write together
-                    float o8[8];
+            if (row < sw.rows) {
+                float o8[8];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) o8[i] = o[i], o8[4 + i] = __shfl_down(o[i], 1);
-                    if (!(threadIdx.x & 1)) write_row(p, sw.r, h, row, ch, o8, M, L);
+                for (int i = 0; i < CH; ++i) {
+                    o8[i] = o[i];
+                    if constexpr (CH == 4) o8[4 + i] = __shfl_down(o[i], 1);  // pairs of threads write together
                 }
+                if (CH == 8 || !(threadIdx.x & 1)) write_row(p, sw.r, h, row, ch, o8, M, L);
             }
-        } else if (row_t < p.rows) {
+        } else {
             float *pr = p.part + ((int64_t)(2 * blockIdx.x + (began ? 1 : 0)) * p.rows + row_t) * EROW;
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) pr[ch + i] = o[i];
-            if (ch == 0) pr[D] = M, pr[D + 1] = L;
+            for (int i = 0; i < CH; i += 4) *(f4 *)(pr + ch + i) = (f4){o[i], o[i + 1], o[i + 2], o[i + 3]};
+            if (ch == 0) *(f2 *)(pr + D) = (f2){M, L};
         }
     }
 }
