@@ -971,6 +971,7 @@ static int paged_rows_params(const akv_paged_rows_args *a, akv::PagedRowsParams 
     const int rc = paged_views(a->abi_version, a->layer, a->pool, a->batch, &p->pool, &p->seqs);
     if (rc != AKV_OK) return rc;
     if (a->dtype < 0 || a->dtype > 2) return fail(AKV_E_DTYPE, "float16, bfloat16 or float32 rows");
+    if (a->batch.n_tokens * a->pool.heads >= ((int64_t)1 << 31)) return fail(AKV_E_SHAPE, "2^31 rows or more");
     if (a->batch.n_tokens > 0 && (!a->k || !a->v)) return fail(AKV_E_INVALID, "k and v are required");
     if (!aligned16(a->k) || !aligned16(a->v) || ((a->k_t | a->k_h | a->v_t | a->v_h) & 15))
         return fail(AKV_E_ALIGN, "rows must be 16-byte aligned");

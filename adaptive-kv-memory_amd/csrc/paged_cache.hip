@@ -23,15 +23,57 @@ __device__ __forceinline__ _Float16 round16(double d) {
     return (_Float16)__builtin_bit_cast(float, u);
 }
 
-// (x - z) / s rounded to the nearest whole number, ties to even, as exact arithmetic has it.
-// The float32 quotient is within 8e-6 of the true one (below 16, four roundings); where that
-// leaves the side of a border open float64 decides.
-__device__ __forceinline__ uint32_t code_of(float x, float z, float s, float inv) {
-    const float r = (x - z) * inv;
-    float c = __builtin_rintf(r);
-    if (__builtin_fabsf(__builtin_fabsf(r - c) - 0.5f) < 2e-5f)
-        c = (float)__builtin_rint(((double)x - (double)z) / (double)s);
-    return (uint32_t)__builtin_fminf(__builtin_fmaxf(c, 0.0f), 15.0f);
+// (hi - lo) / 15 as exact arithmetic rounds it to float16.  The float32 quotient is within four
+// of its units of the true one; float64 decides where a float16 tie may lie between them, and
+// below float16's normal range, where ties lie elsewhere.
+__device__ __forceinline__ _Float16 scale_of(float hi, float lo) {
+    const float f = (hi - lo) * (1.0f / 15.0f);
+    const uint32_t from_tie = (__builtin_bit_cast(uint32_t, f) + 0x1000u + 4u) & 0x1fffu;
+    // (asked of the whole wave: the compiler would compute both sides always)
+    if (__builtin_amdgcn_ballot_w64(from_tie <= 8u || f < 0x1p-14f)) return round16(((double)hi - (double)lo) / 15.0);
+    return (_Float16)f;
+}
+
+// Codes of eight values: (x - z) / s rounded to the nearest whole number, ties to even, as
+// exact arithmetic has it, within 0..15.  The float32 quotient is within 8e-6 of the true one
+// (below 16, four roundings); where that leaves the side of a border open float64 decides.
+// Nibble e of the result is value e.
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float z, float s) {
+    const float inv = __builtin_amdgcn_rcpf(s);
+    float c[8], far = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float r = (x[e] - z) * inv;
+        c[e] = __builtin_rintf(r);
+        far = __builtin_fmaxf(far, __builtin_fabsf(r - c[e]));
+    }
+    if (__builtin_amdgcn_ballot_w64(far > 0.5f - 2e-5f))
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c[e] = (float)__builtin_rint(((double)x[e] - (double)z) / (double)s);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c[e] = __builtin_amdgcn_fmed3f(c[e], 0.0f, 15.0f);
+    // four digits to the base 16 are exact in float32
+    const float a = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]);
+    const float b = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(c[7], 16.f, c[6]), 16.f, c[5]), 16.f, c[4]);
+    return (uint32_t)a | ((uint32_t)b << 16);
+}
+
+// x combined with that of the lanes of its group of LANES: quads, half rows, rows, by DPP.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+template <bool MAX>
+__device__ __forceinline__ float pick(float a, float b) {  // NaN stays
+    return MAX ? __builtin_elementwise_maximum(a, b) : __builtin_elementwise_minimum(a, b);
+}
+template <bool MAX>
+__device__ __forceinline__ float over_group(float x, int lanes) {
+    x = pick<MAX>(x, dpp<0xB1>(x));                  // neighbours
+    x = pick<MAX>(x, dpp<0x4E>(x));                  // pairs of a quad
+    if (lanes >= 8) x = pick<MAX>(x, dpp<0x141>(x)); // quads of a half row (mirrored: a quad's lanes agree)
+    if (lanes >= 16) x = pick<MAX>(x, dpp<0x140>(x));
+    return x;
 }
 
 // Sequence of each lane's token t: the number of sequences that end at or before it.
@@ -50,20 +92,25 @@ __device__ __forceinline__ int seq_of(const PagedSeqs &q, int t, bool live) {
     return live && n < q.n_seqs ? n : -1;
 }
 
-// The tile and the token within it of a row of the call, or null.
-__device__ __forceinline__ unsigned char *slot_of(const PagedRowsParams &p, int t, int h, bool live, int tile_bytes,
-                                                  int *tok) {
+// Where the rows of token t lie: the tile of head 0, the next head's distance, the token in it.
+struct Slot {
+    unsigned char *page;  // null: the token has no slot
+    int64_t head_bytes;
+    int tok;
+};
+__device__ __forceinline__ Slot slot_of(const PagedRowsParams &p, int t, bool live) {
+    const int tile_bytes = paged_tile_bytes(p.D, p.ng), log_page = p.pool.log_tpp + 4;
+    Slot at{nullptr, (int64_t)tile_bytes << p.pool.log_tpp, 0};
     const int s = seq_of(p.seqs, t, live);
-    if (s < 0) return nullptr;
-    const int log_page = p.pool.log_tpp + 4;
+    if (s < 0) return at;
     const SeqRows r = seq_rows(p.seqs, s, log_page);
     const int64_t pos = r.kv - r.n + (t - r.begin);
-    if (t < r.begin || t >= r.begin + r.n || pos < 0) return nullptr;
+    if (t < r.begin || t >= r.begin + r.n || pos < 0) return at;
     const uint32_t page = (uint32_t)p.seqs.table[s * p.seqs.table_stride + (pos >> log_page)];
-    if (page >= p.pool.n_pages) return nullptr;
-    const int tile = (int)(pos >> 4) & ((1 << p.pool.log_tpp) - 1);
-    *tok = (int)(pos & 15);
-    return p.pool.base + page * p.pool.page_bytes + (((int64_t)h << p.pool.log_tpp) + tile) * tile_bytes;
+    if (page >= p.pool.n_pages) return at;
+    at.page = p.pool.base + page * p.pool.page_bytes + (int64_t)((int)(pos >> 4) & ((1 << p.pool.log_tpp) - 1)) * tile_bytes;
+    at.tok = (int)(pos & 15);
+    return at;
 }
 
 template <int DT>
@@ -119,132 +166,147 @@ __device__ __forceinline__ int v_meta(int tok, int grp, int ng) {
 
 }  // namespace
 
-// A lane holds 8 channels 32 g + 8 i .. of one side of one (token, head); D / 8 lanes a side,
-// both sides next to each other.  Group minima and maxima by shuffles.  A V row's bytes are
-// dealt to 16 places of its tile, so four lanes (i of every g) transpose their 4 x 4 bytes
-// and store 16-bit pieces.  Bound by memory for prompts and by latency for a decode step.
-template <int D, int DT>
+// Append and read.  A lane holds 8 channels 32 g + 8 i .. of one side of one (token, head); D / 8
+// lanes a side, both sides next to each other, IT such sets of rows a wave: rows of one token
+// look their slot up once.  Group minima and maxima by DPP.  A V row's bytes are dealt to 16
+// places of its tile, so four lanes (i of every g) transpose their 4 x 4 bytes and move 16-bit
+// pieces.  Bound by memory for prompts (IT = 4) and by latency for a decode step (IT = 1).
+template <int D, int DT, int IT>
 __global__ __launch_bounds__(256) void paged_append_kernel(const PagedRowsParams p) {
-    constexpr int LN = D / 8;  // lanes a side
-    const int64_t gl = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t pair = gl / (2 * LN);
-    const int side = (int)(gl / LN) & 1, b = (int)gl & (LN - 1), g = b >> 2, i = b & 3;
-    const int64_t n_pairs = p.seqs.n_tokens * p.pool.heads;
-    const bool live = pair < n_pairs;
-    const int64_t pc = live ? pair : n_pairs - 1;
-    const int t = (int)(pc / p.pool.heads), h = (int)(pc % p.pool.heads);
-    int tok = 0;
-    const int ng = p.ng, tile_bytes = paged_tile_bytes(D, ng);
-    unsigned char *tile = slot_of(p, t, h, live, tile_bytes, &tok);
-    const unsigned char *src = side ? p.v + t * p.v_t + h * p.v_h : p.k + t * p.k_t + h * p.k_h;
-    float x[8];
-    load8<DT>(src + b * (DT == AKV_DT_F32 ? 32 : 16), x);
-    float lo = kTop, hi = -kTop;
-    bool bad = false;
+    constexpr int LN = D / 8, PW = 32 / LN;  // lanes a side, rows of a wave's set
+    const uint32_t lane = threadIdx.x & 63, H = p.pool.heads, n_pairs = (uint32_t)p.seqs.n_tokens * H;
+    const uint32_t first = (blockIdx.x * 4 + (threadIdx.x >> 6)) * (PW * IT);
+    if (first >= n_pairs) return;
+    const int side = (lane / LN) & 1, b = lane & (LN - 1), g = b >> 2, i = b & 3;
+    uint32_t pair = first + lane / (2 * LN);
+    uint32_t t = pair / H, h = pair - t * H;
+    const int ng = p.ng, grp = g * 32 / (D / ng), lanes = LN / ng;
+    const unsigned char *src = side ? p.v : p.k;
+    const int64_t st = side ? p.v_t : p.k_t, sh = side ? p.v_h : p.k_h;
+    float x[IT][8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        bad |= !(__builtin_fabsf(x[e]) < INFINITY);
-        x[e] = __builtin_fminf(__builtin_fmaxf(x[e], -kTop), kTop);
-        lo = __builtin_fminf(lo, x[e]);
-        hi = __builtin_fmaxf(hi, x[e]);
+    for (int it = 0; it < IT; ++it) {
+        uint32_t tt = t, hh = h + it * PW;
+        while (hh >= H) hh -= H, ++tt;
+        if (pair + it * PW >= n_pairs) tt = t, hh = h;
+        if (pair < n_pairs) load8<DT>(src + tt * st + hh * sh + b * (DT == AKV_DT_F32 ? 32 : 16), x[it]);
     }
-    const int gl_lanes = LN / ng;  // lanes of a group: 4, 8 or 16
-    int any = bad;
-    for (int m = 1; m < gl_lanes; m <<= 1) {
-        lo = __builtin_fminf(lo, __shfl_xor(lo, m));
-        hi = __builtin_fmaxf(hi, __shfl_xor(hi, m));
-        any |= __shfl_xor(any, m);
-    }
-    const _Float16 s16 = round16(((double)hi - (double)lo) / 15.0), z16 = (_Float16)lo;
-    const float s = (float)s16, z = (float)z16;
-    const bool flat = s == 0.0f || any;
-    const float inv = 1.0f / s;
-    uint32_t c[8];
+    Slot at = slot_of(p, t, pair < n_pairs);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) c[e] = flat ? 0u : code_of(x[e], z, s, inv);
-    const uint16_t sb = any ? 0x7e00 : __builtin_bit_cast(uint16_t, s16);
-    const uint16_t zb = any ? 0x7e00 : __builtin_bit_cast(uint16_t, z16);
-    uint32_t w = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w |= c[e] << (4 * e);
-    uint32_t d[4];
-#pragma unroll
-    for (int q = 0; q < D / 32; ++q) d[q] = __shfl(w, (threadIdx.x & 63 & ~(LN - 1)) + 4 * q + i);
-    if (!tile) return;
-    const int grp = g * 32 / (D / ng);
-    const bool lead = b % gl_lanes == 0;
-    if (side == 0) {
-        *(uint32_t *)(tile + tok * (D / 2) + (i * (D / 32) + g) * 4) = w;
-        if (lead) *(uint32_t *)(tile + 16 * D + (tok * ng + grp) * 4) = sb | ((uint32_t)zb << 16);
-    } else {
-        if constexpr (D == 128) {
-            const int r = 4 * i + g;
-            *(uint16_t *)(tile + v_piece<D>(tok, r, 0)) = byte_of(d[0], g) | (byte_of(d[1], g) << 8);
-            *(uint16_t *)(tile + v_piece<D>(tok, r, 1)) = byte_of(d[2], g) | (byte_of(d[3], g) << 8);
-        } else {
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                const int k = 2 * g + m;
-                *(uint16_t *)(tile + v_piece<D>(tok, 4 * i + k, 0)) = byte_of(d[0], k) | (byte_of(d[1], k) << 8);
-            }
+    for (int it = 0; it < IT; ++it) {
+        if (it > 0) {
+            const uint32_t was = t;
+            pair += PW;
+            h += PW;
+            while (h >= H) h -= H, ++t;
+            if (__builtin_amdgcn_ballot_w64(t != was)) at = slot_of(p, t, pair < n_pairs);
         }
-        if (lead) {
-            *(uint16_t *)(tile + v_meta<D>(tok, grp, ng)) = sb;
-            *(uint16_t *)(tile + v_meta<D>(tok, grp, ng) + 32 * ng) = zb;
+        float lo = pick<false>(pick<false>(pick<false>(x[it][0], x[it][1]), pick<false>(x[it][2], x[it][3])),
+                               pick<false>(pick<false>(x[it][4], x[it][5]), pick<false>(x[it][6], x[it][7])));
+        float hi = pick<true>(pick<true>(pick<true>(x[it][0], x[it][1]), pick<true>(x[it][2], x[it][3])),
+                              pick<true>(pick<true>(x[it][4], x[it][5]), pick<true>(x[it][6], x[it][7])));
+        lo = over_group<false>(lo, lanes);
+        hi = over_group<true>(hi, lanes);
+        const bool bad = !(__builtin_fabsf(lo) < INFINITY && __builtin_fabsf(hi) < INFINITY);
+        // values past the clamp get the end's code by themselves
+        lo = __builtin_amdgcn_fmed3f(lo, -kTop, kTop);
+        hi = __builtin_amdgcn_fmed3f(hi, -kTop, kTop);
+        const _Float16 s16 = scale_of(hi, lo), z16 = (_Float16)lo;
+        const float s = (float)s16, z = (float)z16;
+        const uint32_t w = s == 0.0f || bad ? 0u : codes_of(x[it], z, s);
+        const uint32_t sb = bad ? 0x7e00u : __builtin_bit_cast(uint16_t, s16);
+        const uint32_t zb = bad ? 0x7e00u : __builtin_bit_cast(uint16_t, z16);
+        uint32_t d[4];
+#pragma unroll
+        for (int q = 0; q < D / 32; ++q) d[q] = __shfl(w, (lane & ~(LN - 1)) + 4 * q + i);
+        if (!at.page) continue;
+        unsigned char *tile = at.page + h * at.head_bytes;
+        const int tok = at.tok;
+        const bool lead = b % lanes == 0;
+        if (side == 0) {
+            *(uint32_t *)(tile + tok * (D / 2) + (i * (D / 32) + g) * 4) = w;
+            if (lead) *(uint32_t *)(tile + 16 * D + (tok * ng + grp) * 4) = sb | (zb << 16);
+        } else {
+            if constexpr (D == 128) {
+                const int r = 4 * i + g;
+                *(uint16_t *)(tile + v_piece<D>(tok, r, 0)) = byte_of(d[0], g) | (byte_of(d[1], g) << 8);
+                *(uint16_t *)(tile + v_piece<D>(tok, r, 1)) = byte_of(d[2], g) | (byte_of(d[3], g) << 8);
+            } else {
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    const int k = 2 * g + m;
+                    *(uint16_t *)(tile + v_piece<D>(tok, 4 * i + k, 0)) = byte_of(d[0], k) | (byte_of(d[1], k) << 8);
+                }
+            }
+            if (lead) {
+                *(uint16_t *)(tile + v_meta<D>(tok, grp, ng)) = sb;
+                *(uint16_t *)(tile + v_meta<D>(tok, grp, ng) + 32 * ng) = zb;
+            }
         }
     }
 }
 
-// The append's lanes, the other way round.
-template <int D, int DT>
+template <int D, int DT, int IT>
 __global__ __launch_bounds__(256) void paged_read_kernel(const PagedRowsParams p) {
-    constexpr int LN = D / 8;
-    const int64_t gl = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t pair = gl / (2 * LN);
-    const int side = (int)(gl / LN) & 1, b = (int)gl & (LN - 1), g = b >> 2, i = b & 3;
-    const int64_t n_pairs = p.seqs.n_tokens * p.pool.heads;
-    const bool live = pair < n_pairs;
-    const int64_t pc = live ? pair : n_pairs - 1;
-    const int t = (int)(pc / p.pool.heads), h = (int)(pc % p.pool.heads);
-    int tok = 0;
-    const int ng = p.ng, tile_bytes = paged_tile_bytes(D, ng);
-    const unsigned char *tile = slot_of(p, t, h, live, tile_bytes, &tok);
-    const int grp = g * 32 / (D / ng);
-    uint32_t w = 0;
-    uint16_t sb = 0, zb = 0;
-    if (tile) {
-        if (side == 0) {
-            w = *(const uint32_t *)(tile + tok * (D / 2) + (i * (D / 32) + g) * 4);
-            const uint32_t m = *(const uint32_t *)(tile + 16 * D + (tok * ng + grp) * 4);
-            sb = (uint16_t)m, zb = (uint16_t)(m >> 16);
-        } else {
-            // bytes g of row r = 4 i + g (D = 128) or of rows 4 i + 2 g, + 1 (D = 64)
-            if constexpr (D == 128)
-                w = *(const uint16_t *)(tile + v_piece<D>(tok, 4 * i + g, 0)) |
-                    ((uint32_t)*(const uint16_t *)(tile + v_piece<D>(tok, 4 * i + g, 1)) << 16);
-            else
-                w = *(const uint16_t *)(tile + v_piece<D>(tok, 4 * i + 2 * g, 0)) |
-                    ((uint32_t)*(const uint16_t *)(tile + v_piece<D>(tok, 4 * i + 2 * g + 1, 0)) << 16);
-            sb = *(const uint16_t *)(tile + v_meta<D>(tok, grp, ng));
-            zb = *(const uint16_t *)(tile + v_meta<D>(tok, grp, ng) + 32 * ng);
+    constexpr int LN = D / 8, PW = 32 / LN;
+    const uint32_t lane = threadIdx.x & 63, H = p.pool.heads, n_pairs = (uint32_t)p.seqs.n_tokens * H;
+    const uint32_t first = (blockIdx.x * 4 + (threadIdx.x >> 6)) * (PW * IT);
+    if (first >= n_pairs) return;
+    const int side = (lane / LN) & 1, b = lane & (LN - 1), g = b >> 2, i = b & 3;
+    uint32_t pair = first + lane / (2 * LN);
+    uint32_t t = pair / H, h = pair - t * H;
+    const int ng = p.ng, grp = g * 32 / (D / ng);
+    unsigned char *dst = side ? p.v : p.k;
+    const int64_t st = side ? p.v_t : p.k_t, sh = side ? p.v_h : p.k_h;
+    Slot at = slot_of(p, t, pair < n_pairs);
+    uint32_t w[IT], sz[IT], row_t[IT], row_h[IT];
+#pragma unroll
+    for (int it = 0; it < IT; ++it) {
+        if (it > 0) {
+            const uint32_t was = t;
+            pair += PW;
+            h += PW;
+            while (h >= H) h -= H, ++t;
+            if (__builtin_amdgcn_ballot_w64(t != was)) at = slot_of(p, t, pair < n_pairs);
+        }
+        row_t[it] = t;
+        row_h[it] = h;
+        w[it] = sz[it] = 0;
+        if (at.page) {
+            const unsigned char *tile = at.page + h * at.head_bytes;
+            const int tok = at.tok;
+            if (side == 0) {
+                w[it] = *(const uint32_t *)(tile + tok * (D / 2) + (i * (D / 32) + g) * 4);
+                sz[it] = *(const uint32_t *)(tile + 16 * D + (tok * ng + grp) * 4);
+            } else {
+                // bytes g of row r = 4 i + g (D = 128) or of rows 4 i + 2 g, + 1 (D = 64)
+                const int r = D == 128 ? 4 * i + g : 4 * i + 2 * g;
+                w[it] = *(const uint16_t *)(tile + v_piece<D>(tok, r, 0)) |
+                        ((uint32_t)*(const uint16_t *)(tile + (D == 128 ? v_piece<D>(tok, r, 1) : v_piece<D>(tok, r + 1, 0))) << 16);
+                sz[it] = *(const uint16_t *)(tile + v_meta<D>(tok, grp, ng)) |
+                         ((uint32_t)*(const uint16_t *)(tile + v_meta<D>(tok, grp, ng) + 32 * ng) << 16);
+            }
         }
     }
-    uint32_t d[4];
+    pair -= (IT - 1) * PW;
 #pragma unroll
-    for (int q = 0; q < D / 32; ++q) d[q] = __shfl(w, (threadIdx.x & 63 & ~(LN - 1)) + 4 * q + i);
-    if (side == 1) {
-        if constexpr (D == 128)  // row 4 i + q has this lane's group in byte g
-            w = byte_of(d[0], g) | (byte_of(d[1], g) << 8) | (byte_of(d[2], g) << 16) | (byte_of(d[3], g) << 24);
-        else                     // rows 4 i + 2 q, + 1 of lane q: this lane's group in bytes g and 2 + g
-            w = byte_of(d[0], g) | (byte_of(d[0], 2 + g) << 8) | (byte_of(d[1], g) << 16) | (byte_of(d[1], 2 + g) << 24);
+    for (int it = 0; it < IT; ++it) {
+        uint32_t d[4], c = w[it];
+#pragma unroll
+        for (int q = 0; q < D / 32; ++q) d[q] = __shfl(c, (lane & ~(LN - 1)) + 4 * q + i);
+        if (side == 1) {
+            if constexpr (D == 128)  // row 4 i + q has this lane's group in byte g
+                c = byte_of(d[0], g) | (byte_of(d[1], g) << 8) | (byte_of(d[2], g) << 16) | (byte_of(d[3], g) << 24);
+            else                     // rows 4 i + 2 q, + 1 of lane q: this lane's group in bytes g and 2 + g
+                c = byte_of(d[0], g) | (byte_of(d[0], 2 + g) << 8) | (byte_of(d[1], g) << 16) | (byte_of(d[1], 2 + g) << 24);
+        }
+        const float s = (float)as_h2(sz[it])[0], z = (float)as_h2(sz[it])[1];
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = __builtin_fmaf((float)((c >> (4 * e)) & 15u), s, z);
+        if (pair + it * PW < n_pairs)
+            store8<DT>(dst + row_t[it] * st + row_h[it] * sh + b * (DT == AKV_DT_F32 ? 32 : 16), x);
     }
-    if (!live) return;
-    const float s = (float)__builtin_bit_cast(_Float16, sb), z = (float)__builtin_bit_cast(_Float16, zb);
-    float x[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = __builtin_fmaf((float)((w >> (4 * e)) & 15u), s, z);
-    unsigned char *dst = side ? p.v + t * p.v_t + h * p.v_h : p.k + t * p.k_t + h * p.k_h;
-    store8<DT>(dst + b * (DT == AKV_DT_F32 ? 32 : 16), x);
 }
 
 // 16-byte pieces of the pages of all pairs and layers, four a thread; bound by memory.
@@ -394,31 +456,40 @@ __global__ __launch_bounds__(256) void paged_compact_kernel(const PagedCompactPa
 
 namespace {
 
-template <template <int, int> class K>
+// Rows of the smallest call whose waves take four sets each (fewer rows leave compute units
+// idle: 384 rows, a decode step of 48 sequences, ROWS_ONE us at one set and ROWS_FOUR at four).
+constexpr int64_t kManyRows = 8192;
+
+template <template <int, int, int> class K>
 hipError_t rows_launch(const PagedRowsParams &p, hipStream_t s) {
-    const int64_t lanes = p.seqs.n_tokens * p.pool.heads * (p.D / 4);
-    if (lanes == 0 || p.seqs.n_seqs == 0) return hipSuccess;
-    const int64_t blocks = (lanes + 255) / 256;
-    if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
-    auto go = [&](auto kern) { kern<<<dim3((unsigned)blocks), dim3(256), 0, s>>>(p); };
+    const int64_t rows = p.seqs.n_tokens * p.pool.heads;
+    if (rows == 0 || p.seqs.n_seqs == 0) return hipSuccess;
+    if (rows >= (int64_t)1 << 31) return hipErrorInvalidConfiguration;
+    const bool many = rows >= kManyRows;
+    const int64_t wave_rows = (256 / p.D) * (many ? 4 : 1);
+    const unsigned blocks = (unsigned)((rows + 4 * wave_rows - 1) / (4 * wave_rows));
+    auto go = [&](auto one, auto four) {
+        if (many) four<<<dim3(blocks), dim3(256), 0, s>>>(p);
+        else one<<<dim3(blocks), dim3(256), 0, s>>>(p);
+    };
     if (p.D == 128) {
-        if (p.dt == AKV_DT_F16) go(K<128, AKV_DT_F16>::fn);
-        else if (p.dt == AKV_DT_BF16) go(K<128, AKV_DT_BF16>::fn);
-        else go(K<128, AKV_DT_F32>::fn);
+        if (p.dt == AKV_DT_F16) go(K<128, AKV_DT_F16, 1>::fn, K<128, AKV_DT_F16, 4>::fn);
+        else if (p.dt == AKV_DT_BF16) go(K<128, AKV_DT_BF16, 1>::fn, K<128, AKV_DT_BF16, 4>::fn);
+        else go(K<128, AKV_DT_F32, 1>::fn, K<128, AKV_DT_F32, 4>::fn);
     } else {
-        if (p.dt == AKV_DT_F16) go(K<64, AKV_DT_F16>::fn);
-        else if (p.dt == AKV_DT_BF16) go(K<64, AKV_DT_BF16>::fn);
-        else go(K<64, AKV_DT_F32>::fn);
+        if (p.dt == AKV_DT_F16) go(K<64, AKV_DT_F16, 1>::fn, K<64, AKV_DT_F16, 4>::fn);
+        else if (p.dt == AKV_DT_BF16) go(K<64, AKV_DT_BF16, 1>::fn, K<64, AKV_DT_BF16, 4>::fn);
+        else go(K<64, AKV_DT_F32, 1>::fn, K<64, AKV_DT_F32, 4>::fn);
     }
     return hipGetLastError();
 }
-template <int D, int DT>
+template <int D, int DT, int IT>
 struct AppendK {
-    static constexpr auto fn = paged_append_kernel<D, DT>;
+    static constexpr auto fn = paged_append_kernel<D, DT, IT>;
 };
-template <int D, int DT>
+template <int D, int DT, int IT>
 struct ReadK {
-    static constexpr auto fn = paged_read_kernel<D, DT>;
+    static constexpr auto fn = paged_read_kernel<D, DT, IT>;
 };
 
 }  // namespace

@@ -90,6 +90,28 @@ def test_append_and_read(D, G, P, kv, q, dt):
                 assert (d <= np.abs(e) * (torch.finfo(out).eps / 2 + 2.0 ** -24) + 2.0 ** -25).all()
 
 
+@pytest.mark.parametrize("dt", ["fp16", "fp32"])
+@pytest.mark.parametrize("D,G,P,H", [(128, 32, 16, 3), (64, 32, 64, 8), (128, 64, 32, 1)])
+def test_append_and_read_of_many_rows(D, G, P, H, dt):
+    """Prompts: waves take several sets of rows, of one token or of several."""
+    import akv
+    T = 9001 // H
+    announce(f"paged append of {T} tokens, D={D} G={G} P={P} H={H} {dt}")
+    q = [T // 3, 0, T - T // 3 - 5, 5]
+    kv = [q[0], 9, q[2] + 21, 5]
+    w = World(D, G, P, H, kv, q)
+    k, v = _x((w.T, H, D), 3, dt, outliers=True), _x((w.T, H, D), 4, dt)
+    akv.paged_append(w.pool, w.batch, k, v)
+    for s in range(len(kv)):
+        r = w.rows(s)
+        w.ref.write(0, w.table[s], np.arange(kv[s] - q[s], kv[s]), *(x[r].double().cpu().numpy() for x in (k, v)))
+    w.same_pool()
+    got = akv.paged_read(w.pool, w.batch, dtype=torch.float32)
+    for s in range(len(kv)):
+        for g, e in zip(got, w.ref.read(0, w.table[s], np.arange(kv[s] - q[s], kv[s]))):
+            assert (np.abs(g[w.rows(s)].double().cpu().numpy() - e) <= np.abs(e) * 2.0 ** -24 + 2.0 ** -25).all()
+
+
 @pytest.mark.parametrize("dt", list(DT))
 @pytest.mark.parametrize("D,G,P", FORMS[:4:3])
 def test_append_odd_values(D, G, P, dt):
