@@ -976,6 +976,7 @@ static int paged_rows_params(const akv_paged_rows_args *a, akv::PagedRowsParams 
     if (!aligned16(a->k) || !aligned16(a->v) || ((a->k_t | a->k_h | a->v_t | a->v_h) & 15))
         return fail(AKV_E_ALIGN, "rows must be 16-byte aligned");
     p->D = a->pool.D; p->ng = a->pool.D / a->pool.group_size; p->dt = a->dtype;
+    p->log_lanes = a->pool.group_size == 32 ? 2 : a->pool.group_size == 64 ? 3 : 4;
     p->k = (unsigned char *)a->k; p->v = (unsigned char *)a->v;
     p->k_t = a->k_t; p->k_h = a->k_h; p->v_t = a->v_t; p->v_h = a->v_h;
     return AKV_OK;

@@ -35,6 +35,7 @@ struct PagedRowsParams {
     PagedView pool;
     PagedSeqs seqs;
     int D, ng, dt;
+    int log_lanes;             // log2 of a group's lanes, eight channels each
     unsigned char *k, *v;
     int64_t k_t, k_h, v_t, v_h;
 };

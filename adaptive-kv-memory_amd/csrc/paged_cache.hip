@@ -58,7 +58,7 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float z, float
     return (uint32_t)a | ((uint32_t)b << 16);
 }
 
-// x combined with that of the lanes of its group of LANES: quads, half rows, rows, by DPP.
+// x combined with that of the lanes of its group (4, 8 or 16 of them) by DPP.
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
@@ -68,11 +68,11 @@ __device__ __forceinline__ float pick(float a, float b) {  // NaN stays
     return MAX ? __builtin_elementwise_maximum(a, b) : __builtin_elementwise_minimum(a, b);
 }
 template <bool MAX>
-__device__ __forceinline__ float over_group(float x, int lanes) {
+__device__ __forceinline__ float over_group(float x, int log_lanes) {
     x = pick<MAX>(x, dpp<0xB1>(x));                  // neighbours
     x = pick<MAX>(x, dpp<0x4E>(x));                  // pairs of a quad
-    if (lanes >= 8) x = pick<MAX>(x, dpp<0x141>(x)); // quads of a half row (mirrored: a quad's lanes agree)
-    if (lanes >= 16) x = pick<MAX>(x, dpp<0x140>(x));
+    if (log_lanes >= 3) x = pick<MAX>(x, dpp<0x141>(x)); // quads of a half row (mirrored: a quad's lanes agree)
+    if (log_lanes >= 4) x = pick<MAX>(x, dpp<0x140>(x));
     return x;
 }
 
@@ -114,26 +114,28 @@ __device__ __forceinline__ Slot slot_of(const PagedRowsParams &p, int t, bool li
 }
 
 template <int DT>
-__device__ __forceinline__ void load8(const unsigned char *p, float *x) {
-    if constexpr (DT == AKV_DT_F32) {
-        const f4 a = ((const f4 *)p)[0], b = ((const f4 *)p)[1];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
-    } else {
-        const u4 a = *(const u4 *)p;
+struct Raw8 {  // eight values as they come
+    u4 a, b;
+    __device__ __forceinline__ void load(const unsigned char *p) {
+        a = *(const u4 *)p;
+        if constexpr (DT == AKV_DT_F32) b = ((const u4 *)p)[1];
+    }
+    __device__ __forceinline__ void to(float (&x)[8]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t w = a[i];
-            if constexpr (DT == AKV_DT_F16) {
-                const h2 v = as_h2(w);
-                x[2 * i] = (float)v[0], x[2 * i + 1] = (float)v[1];
+            if constexpr (DT == AKV_DT_F32) {
+                x[i] = __builtin_bit_cast(float, w);
+                x[4 + i] = __builtin_bit_cast(float, (uint32_t)b[i]);
+            } else if constexpr (DT == AKV_DT_F16) {
+                x[2 * i] = (float)as_h2(w)[0], x[2 * i + 1] = (float)as_h2(w)[1];
             } else {
                 x[2 * i] = __builtin_bit_cast(float, w << 16);
                 x[2 * i + 1] = __builtin_bit_cast(float, w & 0xffff0000u);
             }
         }
     }
-}
+};
 
 template <int DT>
 __device__ __forceinline__ void store8(unsigned char *p, const float *x) {
@@ -180,18 +182,20 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedRowsParams
     const int side = (lane / LN) & 1, b = lane & (LN - 1), g = b >> 2, i = b & 3;
     uint32_t pair = first + lane / (2 * LN);
     uint32_t t = pair / H, h = pair - t * H;
-    const int ng = p.ng, grp = g * 32 / (D / ng), lanes = LN / ng;
-    const unsigned char *src = side ? p.v : p.k;
+    const int ng = p.ng, ll = p.log_lanes, grp = b >> ll;
+    const unsigned char *src = (side ? p.v : p.k) + b * (DT == AKV_DT_F32 ? 32 : 16);
     const int64_t st = side ? p.v_t : p.k_t, sh = side ? p.v_h : p.k_h;
-    float x[IT][8];
+    // the slot first: loads return in order, and its three would wait behind the rows
+    Slot at = slot_of(p, t, pair < n_pairs);
+    Raw8<DT> raw[IT];
+    uint32_t tt = t, hh = h;
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
-        uint32_t tt = t, hh = h + it * PW;
+        const bool live = pair + it * PW < n_pairs;  // others read the last row
+        raw[it].load(src + (live ? tt : (uint32_t)p.seqs.n_tokens - 1) * st + (live ? hh : H - 1) * sh);
+        hh += PW;
         while (hh >= H) hh -= H, ++tt;
-        if (pair + it * PW >= n_pairs) tt = t, hh = h;
-        if (pair < n_pairs) load8<DT>(src + tt * st + hh * sh + b * (DT == AKV_DT_F32 ? 32 : 16), x[it]);
     }
-    Slot at = slot_of(p, t, pair < n_pairs);
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
         if (it > 0) {
@@ -201,19 +205,21 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedRowsParams
             while (h >= H) h -= H, ++t;
             if (__builtin_amdgcn_ballot_w64(t != was)) at = slot_of(p, t, pair < n_pairs);
         }
-        float lo = pick<false>(pick<false>(pick<false>(x[it][0], x[it][1]), pick<false>(x[it][2], x[it][3])),
-                               pick<false>(pick<false>(x[it][4], x[it][5]), pick<false>(x[it][6], x[it][7])));
-        float hi = pick<true>(pick<true>(pick<true>(x[it][0], x[it][1]), pick<true>(x[it][2], x[it][3])),
-                              pick<true>(pick<true>(x[it][4], x[it][5]), pick<true>(x[it][6], x[it][7])));
-        lo = over_group<false>(lo, lanes);
-        hi = over_group<true>(hi, lanes);
+        float x[8];
+        raw[it].to(x);
+        float lo = pick<false>(pick<false>(pick<false>(x[0], x[1]), pick<false>(x[2], x[3])),
+                               pick<false>(pick<false>(x[4], x[5]), pick<false>(x[6], x[7])));
+        float hi = pick<true>(pick<true>(pick<true>(x[0], x[1]), pick<true>(x[2], x[3])),
+                              pick<true>(pick<true>(x[4], x[5]), pick<true>(x[6], x[7])));
+        lo = over_group<false>(lo, ll);
+        hi = over_group<true>(hi, ll);
         const bool bad = !(__builtin_fabsf(lo) < INFINITY && __builtin_fabsf(hi) < INFINITY);
         // values past the clamp get the end's code by themselves
         lo = __builtin_amdgcn_fmed3f(lo, -kTop, kTop);
         hi = __builtin_amdgcn_fmed3f(hi, -kTop, kTop);
         const _Float16 s16 = scale_of(hi, lo), z16 = (_Float16)lo;
         const float s = (float)s16, z = (float)z16;
-        const uint32_t w = s == 0.0f || bad ? 0u : codes_of(x[it], z, s);
+        const uint32_t w = s == 0.0f || bad ? 0u : codes_of(x, z, s);
         const uint32_t sb = bad ? 0x7e00u : __builtin_bit_cast(uint16_t, s16);
         const uint32_t zb = bad ? 0x7e00u : __builtin_bit_cast(uint16_t, z16);
         uint32_t d[4];
@@ -222,7 +228,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedRowsParams
         if (!at.page) continue;
         unsigned char *tile = at.page + h * at.head_bytes;
         const int tok = at.tok;
-        const bool lead = b % lanes == 0;
+        const bool lead = (b & ((1 << ll) - 1)) == 0;
         if (side == 0) {
             *(uint32_t *)(tile + tok * (D / 2) + (i * (D / 32) + g) * 4) = w;
             if (lead) *(uint32_t *)(tile + 16 * D + (tok * ng + grp) * 4) = sb | (zb << 16);
@@ -255,7 +261,7 @@ __global__ __launch_bounds__(256) void paged_read_kernel(const PagedRowsParams p
     const int side = (lane / LN) & 1, b = lane & (LN - 1), g = b >> 2, i = b & 3;
     uint32_t pair = first + lane / (2 * LN);
     uint32_t t = pair / H, h = pair - t * H;
-    const int ng = p.ng, grp = g * 32 / (D / ng);
+    const int ng = p.ng, grp = b >> p.log_lanes;
     unsigned char *dst = side ? p.v : p.k;
     const int64_t st = side ? p.v_t : p.k_t, sh = side ? p.v_h : p.k_h;
     Slot at = slot_of(p, t, pair < n_pairs);
@@ -457,7 +463,7 @@ __global__ __launch_bounds__(256) void paged_compact_kernel(const PagedCompactPa
 namespace {
 
 // Rows of the smallest call whose waves take four sets each (fewer rows leave compute units
-// idle: 384 rows, a decode step of 48 sequences, ROWS_ONE us at one set and ROWS_FOUR at four).
+// idle: 384 rows, a decode step of 48 sequences, are appended and read in 6.7 us at one set and 10.8 at four).
 constexpr int64_t kManyRows = 8192;
 
 template <template <int, int, int> class K>
