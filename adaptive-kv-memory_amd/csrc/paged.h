@@ -104,9 +104,12 @@ hipError_t paged_importance_launch(const PagedImportanceParams &p, hipStream_t s
 #ifdef __HIPCC__
 // Rows [begin, begin + n) of sequence s in the call's tensors, and its cached tokens.
 struct SeqRows {
-    int begin, n;
-    int64_t kv;
+    int begin, n, kv;
 };
+// The same of a sequence that is one for the whole wave, in scalar registers.
+__device__ __forceinline__ SeqRows wave_uniform(const SeqRows &r) {
+    return {__builtin_amdgcn_readfirstlane(r.begin), __builtin_amdgcn_readfirstlane(r.n), __builtin_amdgcn_readfirstlane(r.kv)};
+}
 __device__ __forceinline__ SeqRows seq_rows(const PagedSeqs &q, int s, int log_page) {
     const int64_t lim = q.n_tokens;
     int64_t a = q.q_starts[s], b = q.q_starts[s + 1];
@@ -115,7 +118,7 @@ __device__ __forceinline__ SeqRows seq_rows(const PagedSeqs &q, int s, int log_p
     const int64_t cap = (int64_t)q.width << log_page;
     int64_t kv = q.kv_lens[s];
     kv = kv < 0 ? 0 : kv > cap ? cap : kv;
-    return {(int)a, (int)(b - a), kv};
+    return {(int)a, (int)(b - a), (int)kv};
 }
 #endif
 

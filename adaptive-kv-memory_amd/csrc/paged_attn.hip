@@ -139,7 +139,7 @@ __device__ __forceinline__ SeqWork seq_work(const PagedAttnParams &p, const SeqR
     w.r = r;
     w.rows = min(r.n, p.seqs.max_q) * p.g;
     w.chunks = w.rows <= kFewRows ? (w.rows + kRows - 1) / kRows : 0;  // more rows are paged_tile_kernel's
-    w.units = max(1, (int)((r.kv + kUnitTok - 1) / kUnitTok));
+    w.units = max(1, (r.kv + (kUnitTok - 1)) / kUnitTok);
     w.cost = w.units + kSetup;
     return w;
 }
@@ -163,7 +163,7 @@ __device__ __forceinline__ void scan_seqs(const PagedAttnParams &p, Scan &sc, in
         if (s < p.seqs.n_seqs) {
             const SeqRows r = seq_rows(p.seqs, s, p.pool.log_tpp + 4);
             mine += seq_total(p, seq_work(p, r));
-            if (per == 1) sc.begin[t] = r.begin, sc.n[t] = r.n, sc.kv[t] = (int)r.kv;
+            if (per == 1) sc.begin[t] = r.begin, sc.n[t] = r.n, sc.kv[t] = r.kv;
         }
     }
     int inc = mine;
@@ -225,7 +225,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
 
     const int per = (p.seqs.n_seqs + kThreads - 1) / kThreads;
     scan_seqs(p, sc, per);
-    const int total = sc.pre[kThreads];
+    const int total = __builtin_amdgcn_readfirstlane(sc.pre[kThreads]);
     const int share = share_of(total, p.groups);
     if (blockIdx.x == 0) {  // for the merge
         p.sums[threadIdx.x] = sc.pre[threadIdx.x];
@@ -242,9 +242,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
 #pragma unroll
         for (int i = 0; i < 4; ++i) k += __builtin_popcountll(__builtin_amdgcn_ballot_w64(sc.pre[64 * i + lane] <= x));
         s = (k - 1) * per;
-        off = x - sc.pre[k - 1];
+        off = x - __builtin_amdgcn_readfirstlane(sc.pre[k - 1]);
         for (;;) {
-            w = seq_work(p, scanned_rows(p, sc, s));
+            w = seq_work(p, wave_uniform(scanned_rows(p, sc, s)));
             const int n = seq_total(p, w);
             if (off < n) break;
             off -= n;
@@ -263,11 +263,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
 
         const int row = row0 + min(col, rows - 1);
         const int qt = row / p.g;
-        const int64_t kv = w.r.kv;
-        const int64_t old = p.causal ? kv - w.r.n + 1 : kv;  // cached tokens the call's first row sees
-        const int see = (int)(p.causal ? max(old + qt, (int64_t)0) : kv);
-        const int see_all = (int)(p.causal ? max(old + row0 / p.g, (int64_t)0) : kv);
-        const int see_any = (int)(p.causal ? max(old + (row0 + rows - 1) / p.g, (int64_t)0) : kv);
+        const int kv = w.r.kv;
+        const int old = kv - w.r.n + 1;  // cached tokens the call's first row sees
+        const int see = p.causal ? max(old + qt, 0) : kv;
+        const int see_all = p.causal ? max(old + row0 / p.g, 0) : kv;
+        const int see_any = p.causal ? max(old + (row0 + rows - 1) / p.g, 0) : kv;
         u4 qw[NS];
         load_row<D>(qw, p.q + (w.r.begin + qt) * p.q_t + (h * p.g + row % p.g) * p.q_h);
 
@@ -293,7 +293,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
                     asm volatile("" : "+v"(pid));  // waited for here: not by every unit, behind its tiles' loads
                 }
                 uint32_t page = (uint32_t)__builtin_amdgcn_readlane(pid, pi - pb);
-                const int left = (int)(kv - 16 * (int64_t)t);
+                const int left = kv - 16 * t;
                 u.nv[i] = page < p.pool.n_pages ? min(left, 16) : 0;
                 if (page >= p.pool.n_pages) page = 0;  // read, and masked
                 const unsigned char *tile = p.pool.base + (int64_t)page * p.pool.page_bytes +
@@ -474,7 +474,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
         }
 
         if (x < x_end && off == seq_total(p, w)) {
-            do w = seq_work(p, scanned_rows(p, sc, ++s));
+            do w = seq_work(p, wave_uniform(scanned_rows(p, sc, ++s)));
             while (w.chunks == 0);
             off = 0;
         }
@@ -625,10 +625,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_importance_kernel(const Pag
     const int k_at = (4 * col + grp) * (D / 8);  // K codes of token col, quarter grp
     const int s = blockIdx.y, hs = p.head_split, h0 = wave & (hs - 1);
     const int blocks = kWaves / hs;              // runs of NT tiles a workgroup has
-    const SeqRows r = seq_rows(p.seqs, s, p.pool.log_tpp + 4);
+    const SeqRows r = wave_uniform(seq_rows(p.seqs, s, p.pool.log_tpp + 4));
     const int64_t tok0 = ((int64_t)blockIdx.x * blocks + wave / hs) * (NT * 16);
     const int n = min(r.n, p.seqs.max_q);
-    const int64_t kv = n > 0 ? min(r.kv, p.n_scores) : 0;  // tokens whose score changes
+    const int64_t kv = n > 0 ? min((int64_t)r.kv, p.n_scores) : 0;  // tokens whose score changes
     const int first = p.q_window > 0 && p.q_window < n ? n - p.q_window : 0;
     const int rows = (n - first) * p.g;
     float sum[NT * 4];
@@ -680,7 +680,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_importance_kernel(const Pag
                 Query<D, NG> Q;
                 make_query<D, NG>(Q, qw, p.q_bf16, p.scale_log2);
                 const float bias = live ? -lse2 : -INFINITY;
-                const int see = p.causal ? (int)max(r.kv - r.n + qt + 1, (int64_t)0) : (int)r.kv;
+                const int see = p.causal ? max(r.kv - r.n + qt + 1, 0) : r.kv;
                 const bool clean = have == ALL && __builtin_amdgcn_ballot_w64(tok0 + NT * 16 <= see) == ~0ull;
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {

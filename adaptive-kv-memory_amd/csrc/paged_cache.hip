@@ -104,7 +104,7 @@ __device__ __forceinline__ Slot slot_of(const PagedRowsParams &p, int t, bool li
     const int s = seq_of(p.seqs, t, live);
     if (s < 0) return at;
     const SeqRows r = seq_rows(p.seqs, s, log_page);
-    const int64_t pos = r.kv - r.n + (t - r.begin);
+    const int64_t pos = (int64_t)r.kv - r.n + (t - r.begin);
     if (t < r.begin || t >= r.begin + r.n || pos < 0) return at;
     const uint32_t page = (uint32_t)p.seqs.table[s * p.seqs.table_stride + (pos >> log_page)];
     if (page >= p.pool.n_pages) return at;

@@ -19,6 +19,7 @@
 // see; it is cut into equal runs, one a workgroup.  Entries that several share leave partial
 // states for paged_tile_merge_kernel.
 #include <algorithm>
+#include <type_traits>
 
 #include "akv_common.h"
 #include "paged.h"
@@ -27,7 +28,8 @@
 namespace akv {
 namespace {
 
-constexpr int kStep = 64;               // tokens a step
+constexpr int kStep = 64;               // tokens a step: a tile for each wave of a group
+constexpr int kTileWaves = 8;
 constexpr int kSetupTok = 2 * kStep;    // what an entry's start counts
 constexpr float kLag = 8.0f;            // log2 units the running maximum may lag behind
 constexpr float kPBias = 7.0f;          // p is held times 2^7
@@ -42,23 +44,28 @@ struct TileSeq {
     __device__ __forceinline__ int64_t before(int64_t t) const { return a * t + b * (t * (t - 1) / 2); }
 };
 template <int R>
-__device__ __forceinline__ TileSeq tile_seq(const PagedAttnParams &p, int s) {
+__device__ __forceinline__ TileSeq tile_seq(const PagedAttnParams &p, int s, bool uniform = true) {
     TileSeq q;
     q.r = seq_rows(p.seqs, s, p.pool.log_tpp + 4);
+    if (uniform) q.r = wave_uniform(q.r);
     q.rows = min(q.r.n, p.seqs.max_q) * p.g;
     q.tiles = q.rows > p.few_rows ? (q.rows + R - 1) / R : 0;
-    const int64_t old = max(q.r.kv - q.r.n, (int64_t)0);
+    const int64_t old = max(q.r.kv - q.r.n, 0);
     q.a = (int64_t)p.g * ((p.causal ? old : q.r.kv) + kSetupTok) + R;
     q.b = p.causal ? R : 0;
     return q;
 }
 // Tokens that row `row` sees.
 __device__ __forceinline__ int sees(const PagedAttnParams &p, const TileSeq &q, int row) {
-    return p.causal ? (int)max(q.r.kv - q.r.n + row / p.g + 1, (int64_t)0) : (int)q.r.kv;
+    return p.causal ? max(q.r.kv - q.r.n + row / p.g + 1, 0) : q.r.kv;
 }
 template <int R>
 __device__ __forceinline__ int steps_of(const PagedAttnParams &p, const TileSeq &q, int t) {
     return max(1, (sees(p, q, min((t + 1) * R, q.rows) - 1) + kStep - 1) / kStep);
+}
+
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+    return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
 }
 
 template <int R>
@@ -68,7 +75,7 @@ __device__ __forceinline__ void scan_tiles(const PagedAttnParams &p, int64_t *pr
     for (int i = 0; i < per; ++i) {
         const int s = t * per + i;
         if (s < p.seqs.n_seqs) {
-            const TileSeq q = tile_seq<R>(p, s);
+            const TileSeq q = tile_seq<R>(p, s, false);
             mine += q.before(q.tiles) * p.pool.heads;
         }
     }
@@ -119,30 +126,47 @@ __device__ __forceinline__ void dequant8_two(uint32_t w, h2 s, h2 z, uint32_t *o
     }
 }
 
-// One tile of K or V on its way from memory to LDS.
+// N products of operands in LDS, AHEAD of them loaded before the first, one more behind each:
+// read(i) loads operand i, mul(i, a) takes it.  (Left to itself the compiler loads an operand,
+// waits and multiplies, 32 times a step.)
+constexpr int kAhead = 4;
+template <int N, typename Read, typename Mul>
+__device__ __forceinline__ void products(Read read, Mul mul) {
+    h8 a[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) a[i] = read(i);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        mul(i, a[i % kAhead]);
+        if (i + kAhead < N) a[i % kAhead] = read(i + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// One tile of K or V on its way from memory to LDS.  What a load brings stays as it is until it
+// is staged: any use before would wait for it.
+template <int N>
+struct Words {  // N dwords of one load: 4, 2 or 1
+    typedef uint32_t vec __attribute__((ext_vector_type(N)));
+    vec v;
+    __device__ __forceinline__ void load(const unsigned char *p) { v = *(const vec *)p; }
+    __device__ __forceinline__ uint32_t operator[](int i) const { return v[i]; }
+};
+template <>
+struct Words<1> {
+    uint32_t v;
+    __device__ __forceinline__ void load(const unsigned char *p) { v = *(const uint32_t *)p; }
+    __device__ __forceinline__ uint32_t operator[](int) const { return v; }
+};
+
 template <int D, int NG, bool TWO>
 struct KLoad {
-    uint32_t c[D / 32], m[NG];
+    Words<D / 32> c;
+    Words<NG> m;
     __device__ __forceinline__ void load(const unsigned char *tile, int lane) {
-        if constexpr (D == 128) {
-            const u4 a = *(const u4 *)(tile + lane * 16);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) c[e] = a[e];
-        } else {
-            const u2 a = *(const u2 *)(tile + lane * 8);
-            c[0] = a[0], c[1] = a[1];
-        }
-        const unsigned char *mt = tile + 16 * D + (lane >> 2) * NG * 4;
-        if constexpr (NG == 4) {
-            const u4 a = *(const u4 *)mt;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) m[e] = a[e];
-        } else if constexpr (NG == 2) {
-            const u2 a = *(const u2 *)mt;
-            m[0] = a[0], m[1] = a[1];
-        } else {
-            m[0] = *(const uint32_t *)mt;
-        }
+        c.load(tile + lane * (D / 8));
+        m.load(tile + 16 * D + (lane >> 2) * NG * 4);
     }
     // lane (token lane / 4, i = lane % 4): chunk 4 g + i
     __device__ __forceinline__ void stage(unsigned char *kt, int tile, int lane) const {
@@ -163,77 +187,58 @@ struct KLoad {
 template <int D, int NG>
 struct VLoad {
     static constexpr int NL = NG == 4 ? 2 : 1;  // groups a lane's channels lie in
-    uint32_t c[2][2], s[2][2 * NL], z[2][2 * NL];  // [quad a, a + 2][pair ..]
+    Words<D / 32> c[2];                         // (quad a, a + 2): pairs (p, h) of row r
+    Words<2 * NL> s[2], z[2];                   // the same quads' meta pairs (group, p)
     __device__ __forceinline__ void load(const unsigned char *tile, int lane) {
         const int r = lane & 15, a = (lane >> 4) & 1, h = lane >> 5;
+        const int g0 = NG == 4 ? 2 * h : NG == 2 ? h : 0;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             const int aq = a + 2 * q;
-            if constexpr (D == 128) {
-                const u4 x = *(const u4 *)(tile + 8 * D + (aq * 16 + r) * 16);
-                c[q][0] = h ? x[1] : x[0];
-                c[q][1] = h ? x[3] : x[2];
-            } else {
-                const u2 x = *(const u2 *)(tile + 8 * D + (aq * 16 + r) * 8);
-                c[q][0] = x[0], c[q][1] = x[1];
-            }
-            // meta dwords (quad, group, pair)
-            const int g0 = NG == 4 ? 2 * h : NG == 2 ? h : 0;
+            c[q].load(tile + 8 * D + (aq * 16 + r) * (D / 8));
             const unsigned char *mt = tile + 16 * D + 64 * NG + (aq * NG + g0) * 8;
-            if constexpr (NL == 2) {
-                const u4 x = *(const u4 *)mt, y = *(const u4 *)(mt + 32 * NG);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[q][e] = x[e], z[q][e] = y[e];
-            } else {
-                const u2 x = *(const u2 *)mt, y = *(const u2 *)(mt + 32 * NG);
-                s[q][0] = x[0], s[q][1] = x[1], z[q][0] = y[0], z[q][1] = y[1];
-            }
+            s[q].load(mt);
+            z[q].load(mt + 32 * NG);
         }
     }
-    __device__ __forceinline__ void mask(int nv, int lane) {  // slots without a token become 0
-        const int a = (lane >> 4) & 1;
+    // lane (row r of the codes, quads a and a + 2, h): the 16 bytes of channels 32 (2 h + l) + 2 r + b;
+    // at D = 64 h says which l of the two.  Slots from token nv on become 0.
+    __device__ __forceinline__ void stage(unsigned char *vt, int tile, int lane, int nv) const {
+        constexpr int L = D / 64;
+        const int r = lane & 15, a = (lane >> 4) & 1, h = lane >> 5;
+        uint32_t keep[2][2] = {{~0u, ~0u}, {~0u, ~0u}};
+        if (nv < 16) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int pr = 0; pr < 2; ++pr) {
+                    const int tok = 4 * (a + 2 * q) + 2 * pr;
+                    keep[q][pr] = (tok < nv ? 0xffffu : 0u) | (tok + 1 < nv ? 0xffff0000u : 0u);
+                }
+        }
+        uint32_t w[2][2];
 #pragma unroll
         for (int q = 0; q < 2; ++q)
 #pragma unroll
-            for (int e = 0; e < 2 * NL; ++e) {
-                const int tok = 4 * (a + 2 * q) + 2 * (e & 1);
-                const uint32_t k = (tok < nv ? 0xffffu : 0u) | (tok + 1 < nv ? 0xffff0000u : 0u);
-                s[q][e] &= k;
-                z[q][e] &= k;
+            for (int pr = 0; pr < 2; ++pr) {
+                if constexpr (D == 128) w[q][pr] = h ? c[q][2 * pr + 1] : c[q][2 * pr];
+                else w[q][pr] = c[q][pr] >> (8 * h);
             }
-    }
-    // lane (row r of the codes, quads a and a + 2, h): the 16 bytes of channels 32 (2 h + l) + 2 r + b
-    __device__ __forceinline__ void stage(unsigned char *vt, int tile, int lane) const {
-        const int r = lane & 15, a = (lane >> 4) & 1, h = lane >> 5;
-        unsigned char *at = vt + (tile * (D / 32) * 64 + a * 32 + 2 * r) * 16;
-        if constexpr (D == 128) {
+        unsigned char *at = vt + (tile * (D / 32) * 64 + a * 32 + 2 * r) * 16 + h * (L * 1024);
 #pragma unroll
-            for (int l = 0; l < 2; ++l) {
-                u4 o[2];
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
-#pragma unroll
-                    for (int pr = 0; pr < 2; ++pr) {
-                        const uint32_t w = l ? c[q][pr] >> 8 : c[q][pr];
-                        const h2 sv = as_h2(s[q][(NL == 2 ? 2 * l : 0) + pr]), zv = as_h2(z[q][(NL == 2 ? 2 * l : 0) + pr]);
-                        o[0][2 * q + pr] = as_u32(__builtin_elementwise_fma(magic_sub((w & 0x000F000Fu) | 0x64006400u, 1024.f), sv, zv));
-                        o[1][2 * q + pr] = as_u32(__builtin_elementwise_fma(magic_sub((w & 0x00F000F0u) | 0x54005400u, 64.f), sv, zv));
-                    }
-                u4 *d = (u4 *)(at + (2 * h + l) * 1024);
-                d[0] = o[0], d[1] = o[1];
-            }
-        } else {  // h says which l of the two
+        for (int l = 0; l < L; ++l) {
             u4 o[2];
 #pragma unroll
             for (int q = 0; q < 2; ++q)
 #pragma unroll
                 for (int pr = 0; pr < 2; ++pr) {
-                    const uint32_t w = c[q][pr] >> (8 * h);
-                    const h2 sv = as_h2(s[q][pr]), zv = as_h2(z[q][pr]);
-                    o[0][2 * q + pr] = as_u32(__builtin_elementwise_fma(magic_sub((w & 0x000F000Fu) | 0x64006400u, 1024.f), sv, zv));
-                    o[1][2 * q + pr] = as_u32(__builtin_elementwise_fma(magic_sub((w & 0x00F000F0u) | 0x54005400u, 64.f), sv, zv));
+                    const uint32_t v = w[q][pr] >> (8 * l);
+                    const int mi = (NL == 2 ? 2 * l : 0) + pr;
+                    const h2 sv = as_h2(s[q][mi] & keep[q][pr]), zv = as_h2(z[q][mi] & keep[q][pr]);
+                    o[0][2 * q + pr] = as_u32(__builtin_elementwise_fma(magic_sub((v & 0x000F000Fu) | 0x64006400u, 1024.f), sv, zv));
+                    o[1][2 * q + pr] = as_u32(__builtin_elementwise_fma(magic_sub((v & 0x00F000F0u) | 0x54005400u, 64.f), sv, zv));
                 }
-            u4 *d = (u4 *)(at + h * 1024);
+            u4 *d = (u4 *)(at + l * 1024);
             d[0] = o[0], d[1] = o[1];
         }
     }
@@ -242,7 +247,7 @@ struct VLoad {
 }  // namespace
 
 template <int D, int NG, int W, bool TWO>
-__global__ __launch_bounds__(64 * W, 2) void paged_tile_kernel(const PagedAttnParams p) {
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_tile_kernel(const PagedAttnParams p) {
     constexpr int R = 32 * W, NB = D / 32, TB = paged_tile_bytes(D, NG), EROW = D + 4;
     constexpr int KT = (TWO ? 2 : 1) * kStep * 2 * D, BUF = KT + kStep * 2 * D;
     extern __shared__ __align__(16) unsigned char smem[];
@@ -252,7 +257,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_tile_kernel(const PagedAttnPa
 
     const int per = (p.seqs.n_seqs + 64 * W - 1) / (64 * W);
     scan_tiles<R>(p, pre, wave_sum, per);
-    const int64_t total = pre[64 * W];
+    const int64_t total = uniform64(pre[64 * W]);
     const int64_t share = tile_share(p, total);
     if (blockIdx.x == 0) {  // for the merge
         int64_t *sums = (int64_t *)p.sums;
@@ -265,8 +270,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_tile_kernel(const PagedAttnPa
     int at = 0;  // the last sum at or below x
     for (int step = 32 * W; step > 0; step >>= 1)
         if (pre[at + step] <= x) at += step;
-    int s = at * per;
-    int64_t off = x - pre[at];
+    int s = __builtin_amdgcn_readfirstlane(at * per);
+    int64_t off = uniform64(x - pre[at]);
     __syncthreads();  // pre is done with
     TileSeq q = tile_seq<R>(p, s);
     while (off >= q.before(q.tiles) * p.pool.heads) {
@@ -296,85 +301,10 @@ __global__ __launch_bounds__(64 * W, 2) void paged_tile_kernel(const PagedAttnPa
             const bool idle = row0 >= q.rows;
             const int see = sees(p, q, row);
             const int see_all = idle ? 0 : sees(p, q, row0), see_any = idle ? 0 : sees(p, q, min(row0 + 31, q.rows - 1));
-            const int kv = (int)q.r.kv;
 
-            // ---- a wave's tile of a step: K for waves 0-3, V for waves 4-7; both where there are only four
-            const int32_t *table = p.seqs.table + s * p.seqs.table_stride;
-            const int log_tpp = p.pool.log_tpp, tl = wave & 3;
-            int pb = (4 * f0) >> log_tpp;
-            int pid = pb + lane < p.seqs.width ? table[pb + lane] : -1;
-            asm volatile("" : "+v"(pid));
-            KLoad<D, NG, TWO> kl;
-            VLoad<D, NG> vl;
-            int nv = 0;         // tokens of the wave's tile of the step that was loaded last
-            uint32_t have = 0;  // and which of the step's four tiles have a page
-            auto load = [&](int step) {
-                if (((4 * step + 3) >> log_tpp) - pb >= 64) {
-                    pb = (4 * step) >> log_tpp;
-                    pid = pb + lane < p.seqs.width ? table[pb + lane] : -1;
-                    asm volatile("" : "+v"(pid));
-                }
-                have = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    have |= ((uint32_t)__builtin_amdgcn_readlane(pid, ((4 * step + i) >> log_tpp) - pb) < p.pool.n_pages ? 1u : 0u) << i;
-                uint32_t page = (uint32_t)__builtin_amdgcn_readlane(pid, ((4 * step + tl) >> log_tpp) - pb);
-                nv = page < p.pool.n_pages ? min(max(kv - 16 * (4 * step + tl), 0), 16) : 0;
-                if (page >= p.pool.n_pages) page = 0;  // read, and masked
-                const unsigned char *tile = p.pool.base + (int64_t)page * p.pool.page_bytes +
-                                            (int64_t)((h << log_tpp) + ((4 * step + tl) & ((1 << log_tpp) - 1))) * TB;
-                if (W == 4 || wave < 4) kl.load(tile, lane);
-                if (W == 4 || wave >= 4) vl.load(tile, lane);
-            };
-            auto stage = [&](unsigned char *buf) {
-                if (W == 4 || wave < 4) kl.stage(buf, tl, lane);
-                if (W == 4 || wave >= 4) {
-                    if (nv < 16) vl.mask(nv, lane);
-                    vl.stage(buf + KT, tl, lane);
-                }
-            };
-            // a tile of rows that see nothing has a step without loads
+            // steps that have tokens: a tile of rows that see nothing has none
             const int f2 = min(f1, (sees(p, q, min((t + 1) * R, q.rows) - 1) + kStep - 1) / kStep);
-            if (f0 < f2) load(f0);
-
-            // ---- the query operand: chunk c = 2 st + hi, channels 8 c + (0, 4, 1, 5, 2, 6, 3, 7)
-            h8 qop[D / 16];
-            float kx;
-            {
-                const unsigned char *qr = p.q + (q.r.begin + row / p.g) * p.q_t + head * p.q_h;
-                u4 w[D / 16];
-#pragma unroll
-                for (int st = 0; st < D / 16; ++st) w[st] = *(const u4 *)(qr + (2 * st + hi) * 16);
-                float top = 0.0f;
-                float y[D / 16][8];
-                if (p.q_bf16) {
-#pragma unroll
-                    for (int st = 0; st < D / 16; ++st)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            y[st][i] = __builtin_bit_cast(float, i & 1 ? w[st][i >> 1] & 0xffff0000u : w[st][i >> 1] << 16);
-                } else {
-#pragma unroll
-                    for (int st = 0; st < D / 16; ++st)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) y[st][i] = (float)as_h2(w[st][i >> 1])[i & 1];
-                }
-#pragma unroll
-                for (int st = 0; st < D / 16; ++st)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) top = __builtin_fmaxf(top, __builtin_fabsf(y[st][i]));
-                top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-                const int ex = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 0;  // the row's maximum goes to [1/2, 1)
-#pragma unroll
-                for (int st = 0; st < D / 16; ++st) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) y[st][i] = __builtin_ldexpf(y[st][i], -ex);
-                    qop[st] = (h8){(_Float16)y[st][0], (_Float16)y[st][4], (_Float16)y[st][1], (_Float16)y[st][5],
-                                   (_Float16)y[st][2], (_Float16)y[st][6], (_Float16)y[st][3], (_Float16)y[st][7]};
-                }
-                kx = __builtin_ldexpf(p.scale_log2, ex);
-            }
-
+            const int32_t *table = p.seqs.table + s * p.seqs.table_stride;
             float mx = kMinMax, l = 0.0f;
             f16v acc[NB];
 #pragma unroll
@@ -382,27 +312,102 @@ __global__ __launch_bounds__(64 * W, 2) void paged_tile_kernel(const PagedAttnPa
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[b][i] = 0.0f;
 
-            if (f0 < f2) stage(smem);
-            __syncthreads();
-            for (int step = f0; step < f2; ++step) {
-                const unsigned char *buf = smem + ((step - f0) & 1) * BUF;
-                const uint32_t here = have;
-                if (step + 1 < f2) load(step + 1);
-                if (kStep * step < see_any) {
-                    f16v sc[2];
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) sc[b][i] = 0.0f;
-#pragma unroll
-                        for (int st = 0; st < D / 16; ++st) {
-                            const h8 *a = (const h8 *)(buf + (32 * b + col) * (2 * D) + (((2 * st + hi) ^ (col & 7)) << 4));
-                            sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], qop[st], sc[b], 0, 0, 0);
-                            if constexpr (TWO) sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[kStep * 2 * D / 16], qop[st], sc[b], 0, 0, 0);
-                        }
+
+            // Waves 0-3 stage K, waves 4-7 V, a tile each, and run half a step behind: one group's
+            // products meet the other's softmax and staging on each SIMD (PONG_A ms without the
+            // offset, PONG_B with it, on the chunks above).  Slots between barriers, t a step:
+            //   2 t      K group's products (t), V group's softmax (t - 1)
+            //   2 t + 1  K group's softmax (t), V group's products (t)
+            // where products (t) are P V of step t - 1 and Q K of step t.  K (t + 1) is staged after
+            // the K group's softmax (t), V (t + 1) after the V group's, each into the buffer whose
+            // last reader was a slot before.  Each group has its own copy of the loop, and its loads
+            // are not conditional (the last step's again at the end): registers that a branch may or
+            // may not load are copied behind it, which waits for the load.
+            auto walk = [&](auto is_late) {
+                constexpr bool late = decltype(is_late)::value;
+                const int log_tpp = p.pool.log_tpp, tl = wave & 3;
+                int pb = (4 * f0) >> log_tpp;
+                int pid = pb + lane < p.seqs.width ? table[pb + lane] : -1;
+                asm volatile("" : "+v"(pid));
+                std::conditional_t<late, VLoad<D, NG>, KLoad<D, NG, TWO>> raw;
+                int nv = 0;         // tokens of the wave's tile of the step that was loaded last
+                uint32_t have = 0;  // and which of the step's four tiles have a page
+                auto load = [&](int step) {
+                    if (((4 * step + 3) >> log_tpp) - pb >= 64) {
+                        pb = (4 * step) >> log_tpp;
+                        pid = pb + lane < p.seqs.width ? table[pb + lane] : -1;
+                        asm volatile("" : "+v"(pid));
                     }
-                    const bool clean = kStep * (step + 1) <= see_all && here == 15u;
-                    if (!clean) {
+                    have = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        have |= ((uint32_t)__builtin_amdgcn_readlane(pid, ((4 * step + i) >> log_tpp) - pb) < p.pool.n_pages ? 1u : 0u) << i;
+                    uint32_t page = (uint32_t)__builtin_amdgcn_readlane(pid, ((4 * step + tl) >> log_tpp) - pb);
+                    nv = page < p.pool.n_pages ? min(max(q.r.kv - 16 * (4 * step + tl), 0), 16) : 0;
+                    if (page >= p.pool.n_pages) page = 0;  // read, and masked
+                    raw.load(p.pool.base + (int64_t)page * p.pool.page_bytes +
+                                 (int64_t)((h << log_tpp) + ((4 * step + tl) & ((1 << log_tpp) - 1))) * TB, lane);
+                };
+                auto stage = [&](unsigned char *buf) {
+                    if constexpr (late) raw.stage(buf + KT, tl, lane, nv);
+                    else raw.stage(buf, tl, lane);
+                };
+                load(f0);
+
+                // ---- the query operand: chunk c = 2 st + hi, channels 8 c + (0, 4, 1, 5, 2, 6, 3, 7)
+                h8 qop[D / 16];
+                float kx;
+                {
+                    const unsigned char *qr = p.q + (q.r.begin + row / p.g) * p.q_t + head * p.q_h;
+                    u4 w[D / 16];
+#pragma unroll
+                    for (int st = 0; st < D / 16; ++st) w[st] = *(const u4 *)(qr + (2 * st + hi) * 16);
+                    float top = 0.0f;
+                    float y[D / 16][8];
+                    if (p.q_bf16) {
+#pragma unroll
+                        for (int st = 0; st < D / 16; ++st)
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                y[st][i] = __builtin_bit_cast(float, i & 1 ? w[st][i >> 1] & 0xffff0000u : w[st][i >> 1] << 16);
+                    } else {
+#pragma unroll
+                        for (int st = 0; st < D / 16; ++st)
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) y[st][i] = (float)as_h2(w[st][i >> 1])[i & 1];
+                    }
+#pragma unroll
+                    for (int st = 0; st < D / 16; ++st)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) top = __builtin_fmaxf(top, __builtin_fabsf(y[st][i]));
+                    top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+                    const int ex = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 0;  // the row's maximum goes to [1/2, 1)
+#pragma unroll
+                    for (int st = 0; st < D / 16; ++st) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) y[st][i] = __builtin_ldexpf(y[st][i], -ex);
+                        qop[st] = (h8){(_Float16)y[st][0], (_Float16)y[st][4], (_Float16)y[st][1], (_Float16)y[st][5],
+                                       (_Float16)y[st][2], (_Float16)y[st][6], (_Float16)y[st][3], (_Float16)y[st][7]};
+                    }
+                    kx = __builtin_ldexpf(p.scale_log2, ex);
+                }
+
+
+                f16v sc[2];
+                h8 pop[4];
+                auto scores = [&](const unsigned char *buf) {  // operand: (chunk pair, half of K, 32 tokens)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sc[i >> 4][i & 15] = 0.0f;
+                    constexpr int PARTS = TWO ? 2 : 1;
+                    products<PARTS * 2 * (D / 16)>(
+                        [&](int i) {
+                            const int st = i / (2 * PARTS), part = i / 2 % PARTS, b = i & 1;
+                            return *(const h8 *)(buf + part * (kStep * 2 * D) + (32 * b + col) * (2 * D) + (((2 * st + hi) ^ (col & 7)) << 4));
+                        },
+                        [&](int i, h8 a) { sc[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qop[i / (2 * PARTS)], sc[i & 1], 0, 0, 0); });
+                };
+                auto softmax = [&](int step, uint32_t here) {
+                    if (kStep * (step + 1) > see_all || here != 15u) {
 #pragma unroll
                         for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -431,17 +436,37 @@ __global__ __launch_bounds__(64 * W, 2) void paged_tile_kernel(const PagedAttnPa
                         for (int i = 0; i < 8; ++i)
                             pr[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[tile >> 1][8 * (tile & 1) + i], kx, bias));
                         l += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
-                        const h8 pop = {(_Float16)pr[0], (_Float16)pr[1], (_Float16)pr[2], (_Float16)pr[3],
-                                        (_Float16)pr[4], (_Float16)pr[5], (_Float16)pr[6], (_Float16)pr[7]};
-#pragma unroll
-                        for (int b = 0; b < NB; ++b) {
-                            const h8 a = *(const h8 *)(buf + KT + ((tile * NB + b) * 64 + lane) * 16);
-                            acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pop, acc[b], 0, 0, 0);
-                        }
+                        pop[tile] = (h8){(_Float16)pr[0], (_Float16)pr[1], (_Float16)pr[2], (_Float16)pr[3],
+                                         (_Float16)pr[4], (_Float16)pr[5], (_Float16)pr[6], (_Float16)pr[7]};
                     }
-                }
-                if (step + 1 < f2) stage(smem + ((step + 1 - f0) & 1) * BUF);
+                };
+                auto outputs = [&](const unsigned char *buf) {
+                    products<4 * NB>([&](int i) { return *(const h8 *)(buf + KT + (i * 64 + lane) * 16); },
+                                     [&](int i, h8 a) { acc[i % NB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pop[i / NB], acc[i % NB], 0, 0, 0); });
+                };
+
+                stage(smem);
                 __syncthreads();
+                if (late) __syncthreads();
+                for (int step = f0; step < f2; ++step) {
+                    unsigned char *buf = smem + ((step - f0) & 1) * BUF, *other = smem + ((step - f0 + 1) & 1) * BUF;
+                    const uint32_t here = have;
+                    const bool seen = kStep * step < see_any;
+                    load(min(step + 1, f2 - 1));
+                    if (step > f0 && kStep * (step - 1) < see_any) outputs(other);
+                    if (seen) scores(buf);
+                    __syncthreads();
+                    if (seen) softmax(step, here);
+                    if (step + 1 < f2) stage(other);
+                    __syncthreads();
+                }
+                if (!late) __syncthreads();
+                if (kStep * (f2 - 1) < see_any) outputs(smem + ((f2 - 1 - f0) & 1) * BUF);
+                __syncthreads();
+            };
+            if (f0 < f2) {
+                if (wave < W / 2) walk(std::false_type{});
+                else walk(std::true_type{});
             }
 
             l += __shfl_xor(l, 32);
@@ -553,7 +578,7 @@ __global__ __launch_bounds__(256) void paged_tile_merge_kernel(const PagedAttnPa
 }
 
 namespace {
-constexpr int kTileWaves = 8, kTileGroups = 256;  // one workgroup a compute unit
+constexpr int kTileGroups = 256;  // one workgroup a compute unit
 constexpr int64_t kTileSums = 8192;               // scan_tiles' sums at the start of the workspace
 static_assert((64 * kTileWaves + 1) * 8 <= kTileSums, "the sums fit");
 
