@@ -98,24 +98,36 @@ __device__ __forceinline__ int64_t tile_share(const PagedAttnParams &p, int64_t 
     return max((total + p.tile_groups - 1) / p.tile_groups, (int64_t)4 * kStep * p.g);
 }
 
-__device__ __forceinline__ h2 magic_sub(uint32_t bits, float m) {
-    const h2 mm = {(_Float16)m, (_Float16)m};
-    return as_h2(bits) - mm;
-}
+// Masks of the two nibbles of a byte in both halves of a dword, in registers (so that mask and
+// exponent are one v_and_or_b32), and a pair of codes as float16: under the exponent of 1024
+// the low nibble reads as 1024 + c, under that of 64 the high one as 64 + c.
+struct Nibbles {
+    uint32_t lo, hi;
+    __device__ __forceinline__ void init() {
+        lo = 0x000F000Fu;
+        hi = 0x00F000F0u;
+        asm volatile("" : "+v"(lo), "+v"(hi));
+    }
+    __device__ __forceinline__ h2 low(uint32_t w) const {
+        return as_h2((w & lo) | 0x64006400u) - (h2){(_Float16)1024.f, (_Float16)1024.f};
+    }
+    __device__ __forceinline__ h2 high(uint32_t w) const {
+        return as_h2((w & hi) | 0x54005400u) - (h2){(_Float16)64.f, (_Float16)64.f};
+    }
+};
 // The four pairs of a dword of codes (nibbles n and n + 4 of it) as c s + z.
-__device__ __forceinline__ void dequant8(uint32_t w, h2 s, h2 z, uint32_t *o) {
+__device__ __forceinline__ void dequant8(const Nibbles &nb, uint32_t w, h2 s, h2 z, uint32_t *o) {
     const uint32_t v = w >> 8;
-    o[0] = as_u32(__builtin_elementwise_fma(magic_sub((w & 0x000F000Fu) | 0x64006400u, 1024.f), s, z));
-    o[1] = as_u32(__builtin_elementwise_fma(magic_sub((w & 0x00F000F0u) | 0x54005400u, 64.f), s, z));
-    o[2] = as_u32(__builtin_elementwise_fma(magic_sub((v & 0x000F000Fu) | 0x64006400u, 1024.f), s, z));
-    o[3] = as_u32(__builtin_elementwise_fma(magic_sub((v & 0x00F000F0u) | 0x54005400u, 64.f), s, z));
+    o[0] = as_u32(__builtin_elementwise_fma(nb.low(w), s, z));
+    o[1] = as_u32(__builtin_elementwise_fma(nb.high(w), s, z));
+    o[2] = as_u32(__builtin_elementwise_fma(nb.low(v), s, z));
+    o[3] = as_u32(__builtin_elementwise_fma(nb.high(v), s, z));
 }
 
 // The same as two float16 that add up to c s + z (to 2^-22 of it).
-__device__ __forceinline__ void dequant8_two(uint32_t w, h2 s, h2 z, uint32_t *o, uint32_t *lo) {
+__device__ __forceinline__ void dequant8_two(const Nibbles &nb, uint32_t w, h2 s, h2 z, uint32_t *o, uint32_t *lo) {
     const uint32_t v = w >> 8;
-    const h2 c[4] = {magic_sub((w & 0x000F000Fu) | 0x64006400u, 1024.f), magic_sub((w & 0x00F000F0u) | 0x54005400u, 64.f),
-                     magic_sub((v & 0x000F000Fu) | 0x64006400u, 1024.f), magic_sub((v & 0x00F000F0u) | 0x54005400u, 64.f)};
+    const h2 c[4] = {nb.low(w), nb.high(w), nb.low(v), nb.high(v)};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float a = __builtin_fmaf((float)c[i][0], (float)s[0], (float)z[0]);
@@ -169,15 +181,15 @@ struct KLoad {
         m.load(tile + 16 * D + (lane >> 2) * NG * 4);
     }
     // lane (token lane / 4, i = lane % 4): chunk 4 g + i
-    __device__ __forceinline__ void stage(unsigned char *kt, int tile, int lane) const {
+    __device__ __forceinline__ void stage(unsigned char *kt, int tile, int lane, const Nibbles &nb) const {
         const int tok = 16 * tile + (lane >> 2), i = lane & 3;
 #pragma unroll
         for (int g = 0; g < D / 32; ++g) {
             const uint32_t w = m[g * NG / (D / 32)];
             const h2 s = as_h2((w & 0xffffu) | (w << 16)), z = as_h2((w >> 16) | (w & 0xffff0000u));
             uint32_t o[4], r[4];
-            if constexpr (TWO) dequant8_two(c[g], s, z, o, r);
-            else dequant8(c[g], s, z, o);
+            if constexpr (TWO) dequant8_two(nb, c[g], s, z, o, r);
+            else dequant8(nb, c[g], s, z, o);
             u4 *d = (u4 *)(kt + tok * (2 * D) + (((4 * g + i) ^ (tok & 7)) << 4));
             *d = (u4){o[0], o[1], o[2], o[3]};
             if constexpr (TWO) d[kStep * 2 * D / 16] = (u4){r[0], r[1], r[2], r[3]};
@@ -203,7 +215,7 @@ struct VLoad {
     }
     // lane (row r of the codes, quads a and a + 2, h): the 16 bytes of channels 32 (2 h + l) + 2 r + b;
     // at D = 64 h says which l of the two.  Slots from token nv on become 0.
-    __device__ __forceinline__ void stage(unsigned char *vt, int tile, int lane, int nv) const {
+    __device__ __forceinline__ void stage(unsigned char *vt, int tile, int lane, const Nibbles &nb, int nv) const {
         constexpr int L = D / 64;
         const int r = lane & 15, a = (lane >> 4) & 1, h = lane >> 5;
         uint32_t keep[2][2] = {{~0u, ~0u}, {~0u, ~0u}};
@@ -235,8 +247,8 @@ struct VLoad {
                     const uint32_t v = w[q][pr] >> (8 * l);
                     const int mi = (NL == 2 ? 2 * l : 0) + pr;
                     const h2 sv = as_h2(s[q][mi] & keep[q][pr]), zv = as_h2(z[q][mi] & keep[q][pr]);
-                    o[0][2 * q + pr] = as_u32(__builtin_elementwise_fma(magic_sub((v & 0x000F000Fu) | 0x64006400u, 1024.f), sv, zv));
-                    o[1][2 * q + pr] = as_u32(__builtin_elementwise_fma(magic_sub((v & 0x00F000F0u) | 0x54005400u, 64.f), sv, zv));
+                    o[0][2 * q + pr] = as_u32(__builtin_elementwise_fma(nb.low(v), sv, zv));
+                    o[1][2 * q + pr] = as_u32(__builtin_elementwise_fma(nb.high(v), sv, zv));
                 }
             u4 *d = (u4 *)(at + l * 1024);
             d[0] = o[0], d[1] = o[1];
@@ -330,6 +342,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
                 int pid = pb + lane < p.seqs.width ? table[pb + lane] : -1;
                 asm volatile("" : "+v"(pid));
                 std::conditional_t<late, VLoad<D, NG>, KLoad<D, NG, TWO>> raw;
+                Nibbles nb;
+                nb.init();
                 int nv = 0;         // tokens of the wave's tile of the step that was loaded last
                 uint32_t have = 0;  // and which of the step's four tiles have a page
                 auto load = [&](int step) {
@@ -349,8 +363,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
                                  (int64_t)((h << log_tpp) + ((4 * step + tl) & ((1 << log_tpp) - 1))) * TB, lane);
                 };
                 auto stage = [&](unsigned char *buf) {
-                    if constexpr (late) raw.stage(buf + KT, tl, lane, nv);
-                    else raw.stage(buf, tl, lane);
+                    if constexpr (late) raw.stage(buf + KT, tl, lane, nb, nv);
+                    else raw.stage(buf, tl, lane, nb);
                 };
                 load(f0);
 
@@ -435,9 +449,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
                             pr[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[tile >> 1][8 * (tile & 1) + i], kx, bias));
-                        l += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
                         pop[tile] = (h8){(_Float16)pr[0], (_Float16)pr[1], (_Float16)pr[2], (_Float16)pr[3],
                                          (_Float16)pr[4], (_Float16)pr[5], (_Float16)pr[6], (_Float16)pr[7]};
+                        l += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
                     }
                 };
                 auto outputs = [&](const unsigned char *buf) {
@@ -446,18 +460,20 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
                 };
 
                 stage(smem);
+                uint32_t here = have;
+                load(min(f0 + 1, f2 - 1));
                 __syncthreads();
                 if (late) __syncthreads();
                 for (int step = f0; step < f2; ++step) {
                     unsigned char *buf = smem + ((step - f0) & 1) * BUF, *other = smem + ((step - f0 + 1) & 1) * BUF;
-                    const uint32_t here = have;
                     const bool seen = kStep * step < see_any;
-                    load(min(step + 1, f2 - 1));
                     if (step > f0 && kStep * (step - 1) < see_any) outputs(other);
                     if (seen) scores(buf);
                     __syncthreads();
                     if (seen) softmax(step, here);
                     if (step + 1 < f2) stage(other);
+                    here = have;
+                    load(min(step + 2, f2 - 1));  // a whole step until it is staged
                     __syncthreads();
                 }
                 if (!late) __syncthreads();
