@@ -10,8 +10,10 @@
 // 2e-4); scores, running maximum and sum are float32.  Where the rows' log-sums are asked for,
 // which are float32, keys enter as two float16 that add up to them (TWO: 1.06 ms where one
 // takes 0.84, chunks of 65 to 512 tokens on 64 heads after 2k to 32k).
-//   K  [64 tokens][D / 8 chunks] of 16 bytes, chunk c at place c ^ (token & 7) of its row;
-//   V  the PV operand: [tile][32 channels][lane] of 16 bytes, tokens 4 hi + 0..3, 8 + 4 hi + 0..3.
+//   K  [64 tokens][D / 8 chunks] of 16 bytes, chunk c at place c ^ turn(token) of its row;
+//   V  the PV operand: [tile][32 channels][lane] of 16 bytes, tokens 4 hi + 0..3, 8 + 4 hi + 0..3;
+//      row 16 b + r of its MFMA is channel 2 r + b of the 32.
+// Both keep the eight lanes that LDS serves at a time on different banks, written and read.
 // S^T = K Q^T leaves a lane with 16 scores of its row for every 32 tokens, which are the PV
 // operand's tokens in order, so p goes from registers to the second product.
 //
@@ -97,6 +99,10 @@ __device__ __forceinline__ void scan_tiles(const PagedAttnParams &p, int64_t *pr
 __device__ __forceinline__ int64_t tile_share(const PagedAttnParams &p, int64_t total) {
     return max((total + p.tile_groups - 1) / p.tile_groups, (int64_t)4 * kStep * p.g);
 }
+
+// Neighbouring tokens, whose chunks are written together, differ in bit 2, and any eight in a row
+// in all three.
+__device__ __forceinline__ int turn(int token) { return (token & 1) << 2 | (token & 2) | (token >> 2 & 1); }
 
 // Masks of the two nibbles of a byte in both halves of a dword, in registers (so that mask and
 // exponent are one v_and_or_b32), and a pair of codes as float16: under the exponent of 1024
@@ -190,7 +196,7 @@ struct KLoad {
             uint32_t o[4], r[4];
             if constexpr (TWO) dequant8_two(nb, c[g], s, z, o, r);
             else dequant8(nb, c[g], s, z, o);
-            u4 *d = (u4 *)(kt + tok * (2 * D) + (((4 * g + i) ^ (tok & 7)) << 4));
+            u4 *d = (u4 *)(kt + tok * (2 * D) + (((4 * g + i) ^ turn(tok)) << 4));
             *d = (u4){o[0], o[1], o[2], o[3]};
             if constexpr (TWO) d[kStep * 2 * D / 16] = (u4){r[0], r[1], r[2], r[3]};
         }
@@ -236,7 +242,7 @@ struct VLoad {
                 if constexpr (D == 128) w[q][pr] = h ? c[q][2 * pr + 1] : c[q][2 * pr];
                 else w[q][pr] = c[q][pr] >> (8 * h);
             }
-        unsigned char *at = vt + (tile * (D / 32) * 64 + a * 32 + 2 * r) * 16 + h * (L * 1024);
+        unsigned char *at = vt + (tile * (D / 32) * 64 + a * 32 + r) * 16 + h * (L * 1024);
 #pragma unroll
         for (int l = 0; l < L; ++l) {
             u4 o[2];
@@ -251,7 +257,7 @@ struct VLoad {
                     o[1][2 * q + pr] = as_u32(__builtin_elementwise_fma(nb.high(v), sv, zv));
                 }
             u4 *d = (u4 *)(at + l * 1024);
-            d[0] = o[0], d[1] = o[1];
+            d[0] = o[0], d[16] = o[1];
         }
     }
 };
@@ -416,7 +422,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
                     products<PARTS * 2 * (D / 16)>(
                         [&](int i) {
                             const int st = i / (2 * PARTS), part = i / 2 % PARTS, b = i & 1;
-                            return *(const h8 *)(buf + part * (kStep * 2 * D) + (32 * b + col) * (2 * D) + (((2 * st + hi) ^ (col & 7)) << 4));
+                            return *(const h8 *)(buf + part * (kStep * 2 * D) + (32 * b + col) * (2 * D) + (((2 * st + hi) ^ turn(col)) << 4));
                         },
                         [&](int i, h8 a) { sc[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qop[i / (2 * PARTS)], sc[i & 1], 0, 0, 0); });
                 };
@@ -493,10 +499,11 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float v[4] = {acc[b][4 * i] * inv, acc[b][4 * i + 1] * inv, acc[b][4 * i + 2] * inv, acc[b][4 * i + 3] * inv};
-                            *(u2 *)((unsigned char *)p.out + (o * D + 32 * b + 8 * i + 4 * hi) * 2) =
-                                (u2){to_pair(p.q_bf16, v[0], v[1]), to_pair(p.q_bf16, v[2], v[3])};
+                        for (int k = 0; k < 2; ++k) {  // channels 32 b + 16 k + 8 hi ..: pairs of rows r, 16 + r
+                            u4 v;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) v[j] = to_pair(p.q_bf16, acc[b][4 * k + j] * inv, acc[b][8 + 4 * k + j] * inv);
+                            *(u4 *)((unsigned char *)p.out + (o * D + 32 * b + 16 * k + 8 * hi) * 2) = v;
                         }
                     if (p.lse && hi == 0) p.lse[o] = row_lse(mx, l, kPBias);
                 } else {
@@ -504,8 +511,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            *(f4 *)(pr + 32 * b + 8 * i + 4 * hi) = (f4){acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]};
+                        for (int k = 0; k < 4; ++k)
+                            *(f4 *)(pr + 32 * b + 16 * (k >> 1) + 8 * hi + 4 * (k & 1)) =
+                                (f4){acc[b][4 * (k >> 1) + 2 * (k & 1)], acc[b][8 + 4 * (k >> 1) + 2 * (k & 1)],
+                                     acc[b][4 * (k >> 1) + 2 * (k & 1) + 1], acc[b][8 + 4 * (k >> 1) + 2 * (k & 1) + 1]};
                     if (hi == 0) pr[D] = mx, pr[D + 1] = l;
                 }
             }
