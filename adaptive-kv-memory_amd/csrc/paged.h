@@ -12,8 +12,10 @@ constexpr int kTileTok = 16;   // tokens of a tile
 constexpr int kUnitTok = 32;   // tokens a wave of the attention takes at a time: two tiles
 constexpr int kRows = 16;      // query rows (tokens x heads of a group) that a wave takes
 // Sequences of more rows a cached head go to the tile kernel: a chunk of 16 rows costs a compute
-// unit 0.6 us for 64 tokens, a tile of up to 256 rows 3 us.
-constexpr int kFewRows = 80;
+// unit 0.6 us for 64 tokens, a tile of up to 256 rows 2 us.  Chunks against a tile, us: 16
+// sequences of 8192 tokens, 48, 64 and 80 rows: 108, 132, 157 against 122, 118, 121; 64 of 1024:
+// 63, 66, 91 against 80, 81, 83; one of 32768: 39, 45, 50 against 56, 55, 59.
+constexpr int kFewRows = 64;
 
 __host__ __device__ constexpr int paged_tile_bytes(int D, int ng) { return 16 * D + 128 * ng; }
 

@@ -2,7 +2,6 @@
 // slots), copies of whole pages and the compaction of sequences to the tokens that stay.
 // All of it is bound by memory; the tile layout is written out in akv_hip.h.
 #include "akv_common.h"
-#include "fastdiv.h"
 #include "paged.h"
 
 namespace akv {

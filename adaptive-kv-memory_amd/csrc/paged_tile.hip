@@ -8,8 +8,8 @@
 // other buffer, once for all rows.  Keys and values become float16 c s + z, p is rounded to
 // float16 too (a float16 output is off by about 3e-4 of its norm, where its own rounding is
 // 2e-4); scores, running maximum and sum are float32.  Where the rows' log-sums are asked for,
-// which are float32, keys enter as two float16 that add up to them (TWO: 1.06 ms where one
-// takes 0.84, chunks of 65 to 512 tokens on 64 heads after 2k to 32k).
+// which are float32, keys enter as two float16 that add up to them (TWO: 1.63 ms where one
+// takes 1.29, eight chunks of 512 tokens on 64 heads over 8 after 8k).
 //   K  [64 tokens][D / 8 chunks] of 16 bytes, chunk c at place c ^ turn(token) of its row;
 //   V  the PV operand: [tile][32 channels][lane] of 16 bytes, tokens 4 hi + 0..3, 8 + 4 hi + 0..3;
 //      row 16 b + r of its MFMA is channel 2 r + b of the 32.
@@ -168,13 +168,13 @@ template <int N>
 struct Words {  // N dwords of one load: 4, 2 or 1
     typedef uint32_t vec __attribute__((ext_vector_type(N)));
     vec v;
-    __device__ __forceinline__ void load(const unsigned char *p) { v = *(const vec *)p; }
+    __device__ __forceinline__ void load(const unsigned char *tile, uint32_t at) { v = *(const vec *)(tile + at); }
     __device__ __forceinline__ uint32_t operator[](int i) const { return v[i]; }
 };
 template <>
 struct Words<1> {
     uint32_t v;
-    __device__ __forceinline__ void load(const unsigned char *p) { v = *(const uint32_t *)p; }
+    __device__ __forceinline__ void load(const unsigned char *tile, uint32_t at) { v = *(const uint32_t *)(tile + at); }
     __device__ __forceinline__ uint32_t operator[](int) const { return v; }
 };
 
@@ -183,8 +183,8 @@ struct KLoad {
     Words<D / 32> c;
     Words<NG> m;
     __device__ __forceinline__ void load(const unsigned char *tile, int lane) {
-        c.load(tile + lane * (D / 8));
-        m.load(tile + 16 * D + (lane >> 2) * NG * 4);
+        c.load(tile, (uint32_t)lane * (D / 8));
+        m.load(tile + 16 * D, (uint32_t)(lane >> 2) * (NG * 4));
     }
     // lane (token lane / 4, i = lane % 4): chunk 4 g + i
     __device__ __forceinline__ void stage(unsigned char *kt, int tile, int lane, const Nibbles &nb) const {
@@ -208,15 +208,13 @@ struct VLoad {
     Words<D / 32> c[2];                         // (quad a, a + 2): pairs (p, h) of row r
     Words<2 * NL> s[2], z[2];                   // the same quads' meta pairs (group, p)
     __device__ __forceinline__ void load(const unsigned char *tile, int lane) {
-        const int r = lane & 15, a = (lane >> 4) & 1, h = lane >> 5;
-        const int g0 = NG == 4 ? 2 * h : NG == 2 ? h : 0;
+        const uint32_t r = lane & 15, a = (lane >> 4) & 1, h = lane >> 5;
+        const uint32_t code = (a * 16 + r) * (D / 8), meta = (a * NG + (NG == 4 ? 2 * h : NG == 2 ? h : 0)) * 8;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-            const int aq = a + 2 * q;
-            c[q].load(tile + 8 * D + (aq * 16 + r) * (D / 8));
-            const unsigned char *mt = tile + 16 * D + 64 * NG + (aq * NG + g0) * 8;
-            s[q].load(mt);
-            z[q].load(mt + 32 * NG);
+            c[q].load(tile + 8 * D + q * 4 * D, code);
+            s[q].load(tile + 16 * D + 64 * NG + q * 16 * NG, meta);
+            z[q].load(tile + 16 * D + 96 * NG + q * 16 * NG, meta);
         }
     }
     // lane (row r of the codes, quads a and a + 2, h): the 16 bytes of channels 32 (2 h + l) + 2 r + b;
@@ -330,10 +328,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[b][i] = 0.0f;
 
-
             // Waves 0-3 stage K, waves 4-7 V, a tile each, and run half a step behind: one group's
-            // products meet the other's softmax and staging on each SIMD (PONG_A ms without the
-            // offset, PONG_B with it, on the chunks above).  Slots between barriers, t a step:
+            // products meet the other's softmax and staging on each SIMD (0.80 ms without the
+            // offset, 0.74 with it, chunks of 65 to 512 tokens on 64 heads after 2k to 32k).
+            // Slots between barriers, t a step:
             //   2 t      K group's products (t), V group's softmax (t - 1)
             //   2 t + 1  K group's softmax (t), V group's products (t)
             // where products (t) are P V of step t - 1 and Q K of step t.  K (t + 1) is staged after
@@ -344,29 +342,42 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
             auto walk = [&](auto is_late) {
                 constexpr bool late = decltype(is_late)::value;
                 const int log_tpp = p.pool.log_tpp, tl = wave & 3;
-                int pb = (4 * f0) >> log_tpp;
-                int pid = pb + lane < p.seqs.width ? table[pb + lane] : -1;
-                asm volatile("" : "+v"(pid));
+                // lane i: the address of this head's tiles in the page at entry pb + i of the table
+                // (of page 0 where that is no page of the pool), and which entries are pages
+                int pb;
+                uint32_t page_lo, page_hi;
+                uint64_t valid;
+                auto pages = [&](int step) {
+                    pb = (4 * step) >> log_tpp;
+                    uint32_t id = pb + lane < p.seqs.width ? (uint32_t)table[pb + lane] : ~0u;
+                    valid = __builtin_amdgcn_ballot_w64(id < p.pool.n_pages);
+                    if (id >= p.pool.n_pages) id = 0;
+                    const uint64_t at = (uint64_t)p.pool.base + id * (uint64_t)p.pool.page_bytes + ((uint64_t)(h * TB) << log_tpp);
+                    page_lo = (uint32_t)at;
+                    page_hi = (uint32_t)(at >> 32);
+                };
+                pages(f0);
                 std::conditional_t<late, VLoad<D, NG>, KLoad<D, NG, TWO>> raw;
                 Nibbles nb;
                 nb.init();
                 int nv = 0;         // tokens of the wave's tile of the step that was loaded last
                 uint32_t have = 0;  // and which of the step's four tiles have a page
                 auto load = [&](int step) {
-                    if (((4 * step + 3) >> log_tpp) - pb >= 64) {
-                        pb = (4 * step) >> log_tpp;
-                        pid = pb + lane < p.seqs.width ? table[pb + lane] : -1;
-                        asm volatile("" : "+v"(pid));
-                    }
-                    have = 0;
+                    const int t0 = 4 * step, mine = t0 + tl, last = (t0 + 3) >> log_tpp;
+                    if (last - pb >= 64) pages(step);
+                    const int e0 = (t0 >> log_tpp) - pb, e1 = (mine >> log_tpp) - pb;
+                    const uint32_t all = (2u << (last - pb - e0)) - 1;
+                    have = 15;
+                    if (((uint32_t)(valid >> e0) & all) != all) {
+                        have = 0;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        have |= ((uint32_t)__builtin_amdgcn_readlane(pid, ((4 * step + i) >> log_tpp) - pb) < p.pool.n_pages ? 1u : 0u) << i;
-                    uint32_t page = (uint32_t)__builtin_amdgcn_readlane(pid, ((4 * step + tl) >> log_tpp) - pb);
-                    nv = page < p.pool.n_pages ? min(max(q.r.kv - 16 * (4 * step + tl), 0), 16) : 0;
-                    if (page >= p.pool.n_pages) page = 0;  // read, and masked
-                    raw.load(p.pool.base + (int64_t)page * p.pool.page_bytes +
-                                 (int64_t)((h << log_tpp) + ((4 * step + tl) & ((1 << log_tpp) - 1))) * TB, lane);
+                        for (int i = 0; i < 4; ++i) have |= (uint32_t)(valid >> (((t0 + i) >> log_tpp) - pb) & 1) << i;
+                    }
+                    nv = have >> tl & 1 ? min(max(q.r.kv - 16 * mine, 0), 16) : 0;
+                    const uint64_t at = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane(page_hi, e1) << 32 |
+                                         (uint32_t)__builtin_amdgcn_readlane(page_lo, e1)) +
+                                        (uint32_t)((mine & ((1 << log_tpp) - 1)) * TB);
+                    raw.load((const unsigned char *)at, lane);
                 };
                 auto stage = [&](unsigned char *buf) {
                     if constexpr (late) raw.stage(buf + KT, tl, lane, nb, nv);
@@ -411,7 +422,6 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
                     }
                     kx = __builtin_ldexpf(p.scale_log2, ex);
                 }
-
 
                 f16v sc[2];
                 h8 pop[4];
@@ -466,20 +476,18 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
                 };
 
                 stage(smem);
-                uint32_t here = have;
-                load(min(f0 + 1, f2 - 1));
                 __syncthreads();
                 if (late) __syncthreads();
                 for (int step = f0; step < f2; ++step) {
                     unsigned char *buf = smem + ((step - f0) & 1) * BUF, *other = smem + ((step - f0 + 1) & 1) * BUF;
+                    const uint32_t here = have;
                     const bool seen = kStep * step < see_any;
+                    load(min(step + 1, f2 - 1));
                     if (step > f0 && kStep * (step - 1) < see_any) outputs(other);
                     if (seen) scores(buf);
                     __syncthreads();
                     if (seen) softmax(step, here);
                     if (step + 1 < f2) stage(other);
-                    here = have;
-                    load(min(step + 2, f2 - 1));  // a whole step until it is staged
                     __syncthreads();
                 }
                 if (!late) __syncthreads();
@@ -527,78 +535,95 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     }
 }
 
-// Entries that several workgroups share: 16 rows of one a workgroup, joined in order.
+constexpr int kMergeRows = 64;
+// Entries that several workgroups share, joined in order: kMergeRows rows of the entry that holds
+// the start of a run, a workgroup, by the first start in it.  Bound by the states' bytes and the search's latency (255
+// starts, 69 MB at D = 128: 18 us; 16 rows a workgroup 24, 32 rows 20).
 template <int D, int W>
 __global__ __launch_bounds__(256) void paged_tile_merge_kernel(const PagedAttnParams p) {
-    constexpr int R = 32 * W, EROW = D + 4, CH = D / 16, B = 4;
+    constexpr int R = 32 * W, EROW = D + 4, CH = D / 16, B = 2, J = kMergeRows / 16;
+    static_assert(64 * W % 256 == 0, "whole rounds of sums");
     const int64_t *sums = (const int64_t *)p.sums;
+    const int64_t total = sums[64 * W], share = tile_share(p, total);
+    const int64_t x = (blockIdx.x + 1) * share;
+    if (x >= total) return;
+    int at = -1;  // the last sum at or below x
+    for (int i = threadIdx.x; i < 64 * W; i += 256) at += __syncthreads_count(sums[i] <= x);
     const int per = (p.seqs.n_seqs + 64 * W - 1) / (64 * W);
-    const int s = blockIdx.y, k = s / per;
-    int64_t at = sums[k];
-    const int64_t share = tile_share(p, sums[64 * W]);
-    const TileSeq q = tile_seq<R>(p, s);
-    for (int i = k * per; i < s; ++i) {
-        const TileSeq o = tile_seq<R>(p, i);
-        at += o.before(o.tiles) * p.pool.heads;
+    int s = at * per;
+    int64_t off = x - sums[at];
+    TileSeq q = tile_seq<R>(p, s);
+    while (off >= q.before(q.tiles) * p.pool.heads) {
+        off -= q.before(q.tiles) * p.pool.heads;
+        q = tile_seq<R>(p, ++s);
     }
-    constexpr int G16 = R / 16;
-    const int64_t blocks = (int64_t)q.tiles * p.pool.heads * G16;
-    for (int64_t blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
-        const int g16 = (int)(blk % G16), item = (int)(blk / G16);
-        const int h = item / q.tiles, t = item - h * q.tiles;
-        const int in = 16 * g16 + (threadIdx.x >> 4), ch = (threadIdx.x & 15) * CH;
-        const int row = t * R + in;
-        if (row >= q.rows) continue;
-        const int64_t u0 = at + h * q.before(q.tiles) + q.before(t), cost = q.cost(t);
-        const int n_steps = steps_of<R>(p, q, t);
-        const int64_t g0 = u0 / share, g1 = (u0 + cost - 1) / share;
-        if (g0 == g1) continue;
-        float o[CH];
-        float M = kMinMax, L = 0.f;
+    const int h = (int)(off / q.before(q.tiles));
+    const int64_t in_head = off - h * q.before(q.tiles);
+    int t = 0;
+    for (int step = 1 << (31 - __builtin_clz(q.tiles)); step > 0; step >>= 1)
+        if (t + step < q.tiles && q.before(t + step) <= in_head) t += step;
+    const int64_t u0 = x - (in_head - q.before(t)), cost = q.cost(t);
+    const int64_t g0 = u0 / share, g1 = (u0 + cost - 1) / share;
+    const int in = kMergeRows * blockIdx.y + (threadIdx.x >> 4), ch = (threadIdx.x & 15) * CH;
+    const int row0 = t * R + in;
+    if (g0 != blockIdx.x || row0 >= q.rows) return;
+    const int n_steps = steps_of<R>(p, q, t);
+    float o[J][CH];
+    float M[J], L[J];
 #pragma unroll
-        for (int i = 0; i < CH; ++i) o[i] = 0.f;
-        bool whole = false;
-        for (int64_t g = g0; g <= g1 && !whole; g += B) {
-            f4 v[B][CH / 4];
-            f2 ml[B];
-            bool use[B];
+    for (int j = 0; j < J; ++j) {
+        M[j] = kMinMax, L[j] = 0.f;
 #pragma unroll
-            for (int i = 0; i < B; ++i) {
-                const int64_t gi = min(g + i, g1);
-                const int64_t c0 = max(gi * share - u0, (int64_t)0), c1 = min((gi + 1) * share - u0, cost);
-                const int f0 = (int)(c0 * n_steps / cost), f1 = (int)(c1 * n_steps / cost);
-                use[i] = f0 < f1 && g + i <= g1;
-                whole |= f0 == 0 && f1 == n_steps;
-                const float *pr = p.tile_part + ((2 * gi + (f0 == 0 ? 1 : 0)) * R + in) * EROW;
+        for (int c = 0; c < CH; ++c) o[j][c] = 0.f;
+    }
+    int f1 = 0;  // steps before run g
+    for (int64_t g = g0; g <= g1; g += B) {
+        f4 v[B][J][CH / 4];
+        f2 ml[B][J];
 #pragma unroll
-                for (int c = 0; c < CH / 4; ++c) v[i][c] = use[i] ? ((const f4 *)(pr + ch))[c] : (f4){0.f, 0.f, 0.f, 0.f};
-                ml[i] = use[i] ? *(const f2 *)(pr + D) : (f2){kMinMax, 0.f};
+        for (int i = 0; i < B; ++i) {
+            const int f0 = f1;
+            f1 = g + i < g1 ? (int)(((g + i + 1) * share - u0) * n_steps / cost) : n_steps;
+            if (f0 == 0 && f1 == n_steps) return;  // one workgroup had every step of it, and wrote
+            const float *pr = p.tile_part + ((2 * (g + i) + (f0 == 0 ? 1 : 0)) * R + in) * EROW;
+#pragma unroll
+            for (int j = 0; j < J; ++j) {  // rows past the last are of the tile too
+#pragma unroll
+                for (int c = 0; c < CH / 4; ++c) v[i][j][c] = f0 < f1 ? ((const f4 *)(pr + 16 * j * EROW + ch))[c] : (f4){0.f, 0.f, 0.f, 0.f};
+                ml[i][j] = f0 < f1 ? *(const f2 *)(pr + 16 * j * EROW + D) : (f2){kMinMax, 0.f};
             }
-            float mn = M;
-#pragma unroll
-            for (int i = 0; i < B; ++i) mn = __builtin_fmaxf(mn, ml[i][0]);
-            const float a = __builtin_amdgcn_exp2f(M - mn);
-            L *= a;
-#pragma unroll
-            for (int c = 0; c < CH; ++c) o[c] *= a;
-#pragma unroll
-            for (int i = 0; i < B; ++i) {
-                const float b = __builtin_amdgcn_exp2f(ml[i][0] - mn);
-                L = __builtin_fmaf(ml[i][1], b, L);
-#pragma unroll
-                for (int c = 0; c < CH; ++c) o[c] = __builtin_fmaf(v[i][c >> 2][c & 3], b, o[c]);
-            }
-            M = mn;
         }
-        if (whole) continue;  // one workgroup had every step of it, and wrote
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            float mn = M[j];
+#pragma unroll
+            for (int i = 0; i < B; ++i) mn = __builtin_fmaxf(mn, ml[i][j][0]);
+            const float a = __builtin_amdgcn_exp2f(M[j] - mn);
+            L[j] *= a;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) o[j][c] *= a;
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                const float b = __builtin_amdgcn_exp2f(ml[i][j][0] - mn);
+                L[j] = __builtin_fmaf(ml[i][j][1], b, L[j]);
+#pragma unroll
+                for (int c = 0; c < CH; ++c) o[j][c] = __builtin_fmaf(v[i][j][c >> 2][c & 3], b, o[j][c]);
+            }
+            M[j] = mn;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const int row = row0 + 16 * j;
+        if (row >= q.rows) break;
         const int head = h * p.g + row % p.g;
         const int64_t ro = (q.r.begin + row / p.g) * p.Hq + head;
-        const float inv = row_inverse(L);
+        const float inv = row_inverse(L[j]);
 #pragma unroll
         for (int c = 0; c < CH / 4; ++c)
             *(u2 *)((unsigned char *)p.out + (ro * D + ch + 4 * c) * 2) =
-                (u2){to_pair(p.q_bf16, o[4 * c] * inv, o[4 * c + 1] * inv), to_pair(p.q_bf16, o[4 * c + 2] * inv, o[4 * c + 3] * inv)};
-        if (p.lse && ch == 0) p.lse[ro] = row_lse(M, L, kPBias);
+                (u2){to_pair(p.q_bf16, o[j][4 * c] * inv, o[j][4 * c + 1] * inv), to_pair(p.q_bf16, o[j][4 * c + 2] * inv, o[j][4 * c + 3] * inv)};
+        if (p.lse && ch == 0) p.lse[ro] = row_lse(M[j], L[j], kPBias);
     }
 }
 
@@ -617,8 +642,8 @@ hipError_t tile_go_as(const PagedAttnParams &p, hipStream_t st) {
     kern<<<dim3(p.tile_groups), dim3(64 * W), LDS, st>>>(p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const int64_t blocks = ((int64_t)p.seqs.max_q * p.g + 32 * W - 1) / (32 * W) * p.pool.heads * (2 * W);
-    paged_tile_merge_kernel<D, W><<<dim3((unsigned)std::min<int64_t>(blocks, 2048), p.seqs.n_seqs), dim3(256), 0, st>>>(p);
+    if (p.tile_groups == 1) return hipSuccess;
+    paged_tile_merge_kernel<D, W><<<dim3(p.tile_groups - 1, 32 * W / kMergeRows), dim3(256), 0, st>>>(p);
     return hipGetLastError();
 }
 template <int D, int NG>
