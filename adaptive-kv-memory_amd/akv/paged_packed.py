@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
+from operator import index
 from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
@@ -62,12 +63,13 @@ def _check_device(pool: "PagedPool", *tensors) -> None:
 
 
 def _int32(name: str, t: torch.Tensor, dims: int) -> torch.Tensor:
-    """An int32 tensor of ``dims`` dimensions, its last one consecutive."""
+    """An int32 tensor of ``dims`` dimensions, its last one consecutive and its rows apart."""
     if t.dim() != dims or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be an int32 tensor of {dims} dimension{'s' if dims > 1 else ''}")
     if t.dtype != torch.int32:
         t = t.to(torch.int32)
-    return t if t.numel() == 0 or t.stride(-1) == 1 else t.contiguous()
+    plain = t.numel() == 0 or (t.stride(-1) == 1 and (dims == 1 or t.shape[0] == 1 or t.stride(0) >= t.shape[1]))
+    return t if plain else t.contiguous()
 
 
 class PagedPool:
@@ -114,7 +116,8 @@ class PagedBatch:
     ``page_table[s, j // page_size]``.  kv_lens (S,) int32: cached tokens, those of this call
     among them.  q_starts (S + 1,) int32: sequence s owns rows ``q_starts[s]`` to
     ``q_starts[s + 1]`` of the call's (n_tokens, heads, head_dim) tensors; they are its newest
-    tokens.  n_tokens: the rows; max_q: no sequence has more of them.
+    tokens.  n_tokens: the rows; max_q: no sequence has more of them.  What calls return for rows
+    that are no sequence's (those of a padded batch) is not defined.
 
     The tensors are kept, not copied (other integer types and orders are): what they hold when
     the work runs counts.  n_tokens and max_q are fixed."""
@@ -344,6 +347,7 @@ class PageLedger:
         """Slots for ``counts`` more tokens; (from, to) of the shared pages that get written and
         have to be copied first.  Raises, and changes nothing, when the pages do not suffice."""
         self._known(seqs)
+        counts = [index(c) for c in counts]
         if len(counts) != len(seqs) or any(c < 0 for c in counts):
             raise ValueError("one count of new tokens, at least 0, for each sequence")
         need, left = 0, {}
@@ -406,7 +410,7 @@ class PackedPagedCache:
     A step: ``batch = cache.extend(seqs, counts)`` makes room (and copies the shared pages that
     will be written), then per layer ``append`` and ``attention``.  ``fork`` shares a sequence's
     pages; ``compact`` keeps chosen tokens; ``crop`` drops the last ones; ``remove`` frees.
-    Operations that raise leave the cache as it was.  Calls go to the current stream."""
+    Calls that are refused leave the cache as it was.  Work goes to the current stream."""
 
     def __init__(self, num_layers: int, num_heads: int, head_dim: int, page_size: int = 16, max_pages: int = 4096,
                  group_size: int = 32, device="cuda"):
@@ -458,7 +462,7 @@ class PackedPagedCache:
 
     def extend(self, seqs: Sequence[int], counts: Union[int, Sequence[int]] = 1) -> PagedBatch:
         """Room for ``counts`` new tokens of each sequence: the batch whose rows they are."""
-        counts = [counts] * len(seqs) if isinstance(counts, int) else list(counts)
+        counts = [counts] * len(seqs) if isinstance(counts, int) else [index(c) for c in counts]
         copies = self._book.extend(seqs, counts)
         if copies:
             copy_pages(self.pool, *self._upload([a for a, _ in copies], [b for _, b in copies]))

@@ -1055,10 +1055,14 @@ static int check_paged_queries(int32_t Hq, int32_t dt, float sm_scale, const akv
     if (b.n_tokens > 0 && !q) return fail(AKV_E_INVALID, "q is required");
     if (!aligned16(q) || ((q_t | q_h) & 15)) return fail(AKV_E_ALIGN, "query rows must be 16-byte aligned");
     if ((int64_t)b.max_q * (Hq / pool.heads) >= ((int64_t)1 << 27)) return fail(AKV_E_SHAPE, "too many rows a sequence");
-    // units of 32 tokens, and a few for an item, x heads x chunks of 16 rows are counted in 31 bits
-    const int64_t units = ((int64_t)b.table_width * pool.page_size + 31) / 32 + 4;
-    const int64_t chunks = ((int64_t)b.max_q * (Hq / pool.heads) + 15) / 16 + 1;
-    if ((double)units * b.n_seqs * pool.heads * chunks >= 1073741824.0) return fail(AKV_E_SHAPE, "too much for one call");
+    // units of 32 tokens, and a few for an item, x heads x chunks of 16 rows are counted in 31
+    // bits; the tile kernel's tokens x rows, and its steps of a tile's share, in 63
+    const double cap = (double)b.table_width * pool.page_size, rows = (double)b.max_q * (Hq / pool.heads);
+    const double few = std::min(rows, (double)akv::kFewRows);
+    if ((cap / 32 + 4) * b.n_seqs * pool.heads * (few / 16 + 1) >= 0x1p30) return fail(AKV_E_SHAPE, "too much for one call");
+    const double tile = (Hq / pool.heads) * (cap + 256) + rows + 256, tiles = rows / 256 + 1;
+    if (tile * (cap / 64 + 2) >= 0x1p62 || tile * tiles * pool.heads * b.n_seqs >= 0x1p62)
+        return fail(AKV_E_SHAPE, "too much for one call");
     return AKV_OK;
 }
 

@@ -317,6 +317,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
         };
 
         float mx = kMinMax, l = 0.0f;
+        uint32_t poisoned = 0;  // groups of channels in which the row sees a value that is not finite
         f4 acc[NB], accz = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int b = 0; b < NB; ++b) acc[b] = (f4){0.f, 0.f, 0.f, 0.f};
@@ -330,7 +331,19 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
                     for (int q = 0; q < MW; ++q) {
                         const int d = (lane & (32 * NG / MW - 1)) * MW + q - 16 * NG;
                         const int tok = ((d & (8 * NG - 1)) / (2 * NG)) * 4 + (d & 1) * 2;
-                        if (d >= 0) u.m[i][q] &= (tok < u.nv[i] ? 0xffffu : 0u) | (tok + 1 < u.nv[i] ? 0xffff0000u : 0u);
+                        const uint32_t keep = (tok < u.nv[i] ? 0xffffu : 0u) | (tok + 1 < u.nv[i] ? 0xffff0000u : 0u);
+                        // values that are not finite would reach rows that do not see them as 0 * NaN:
+                        // they become 0 too, and the rows that see them NaN in the end
+                        const uint32_t bad = d >= 0 ? not_finite(u.m[i][q]) & keep : 0u;
+                        if (d >= 0) u.m[i][q] &= keep & ~bad;
+                        const int group = (d >> 1) & (NG - 1);
+                        for (uint64_t left = __builtin_amdgcn_ballot_w64(bad != 0); left; left &= left - 1) {
+                            const int from = __builtin_ctzll(left);
+                            const int at = kUnitTok * j + 16 * i + __builtin_amdgcn_readlane(tok, from);
+                            const int of = __builtin_amdgcn_readlane(group, from);
+                            const uint32_t what = __builtin_amdgcn_readlane(bad, from);
+                            if ((at < see && (what & 0xffffu)) || (at + 1 < see && what >> 16)) poisoned |= 1u << of;
+                        }
                     }
             }
             __builtin_amdgcn_wave_barrier();
@@ -442,7 +455,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
         l = xsum(l);
         float z[NG];
 #pragma unroll
-        for (int g = 0; g < NG; ++g) z[g] = __shfl(accz[g], col);
+        for (int g = 0; g < NG; ++g) {
+            const float v = __shfl(accz[g], col);
+            z[g] = poisoned >> g & 1 ? NAN : v;
+        }
         const bool starts = j0 == 0, ends = c1 == w.cost;
         const int slot = 2 * wave + (ends ? 0 : 1);
         float *er = entries + (slot * p.rows + col) * EROW;

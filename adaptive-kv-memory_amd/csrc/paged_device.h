@@ -15,6 +15,10 @@ __device__ __forceinline__ float row_inverse(float l) { return l > 0.0f || l != 
 __device__ __forceinline__ float row_lse(float m, float l, float bias) {
     return l > 0.0f || l != l ? 0.69314718055994531f * (m + (__builtin_log2f(l) - bias)) : -INFINITY;
 }
+// The halves of a pair of float16 that are not finite, as a mask.
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    return ((w & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) | ((w & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u);
+}
 __device__ __forceinline__ uint32_t to_pair(bool bf16, float a, float b) {
     return bf16 ? f32_to_bf16_rne(a) | ((uint32_t)f32_to_bf16_rne(b) << 16) : as_u32((h2){(_Float16)a, (_Float16)b});
 }

@@ -217,6 +217,45 @@ struct VLoad {
             z[q].load(tile + 16 * D + 96 * NG + q * 16 * NG, meta);
         }
     }
+    // Where rows see different tokens, values that are not finite would reach those that do not
+    // see them as 0 * NaN.  They become 0 in the lane's part of the staged tile, and word (h, a)
+    // of the tile's four says which, for `poison`: bit 16 half + 4 l + 2 q + pr.
+    static __device__ __forceinline__ void hide(unsigned char *vt, uint32_t *bad, int tile, int lane) {
+        constexpr int L = D / 64;
+        asm volatile("" : "+v"(lane));  // or what comes of it is kept in registers through the whole loop
+        const int r = lane & 15, a = (lane >> 4) & 1, h = lane >> 5;
+        unsigned char *at = vt + (tile * (D / 32) * 64 + a * 32 + r) * 16 + h * (L * 1024);
+        uint32_t w = 0;
+#pragma unroll
+        for (int l = 0; l < L; ++l) {
+            u4 *d = (u4 *)(at + l * 1024);
+            u4 x = d[0], y = d[16];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t b = not_finite(x[i]);
+                x[i] &= ~b, y[i] &= ~b;  // of one group, so both or none
+                w |= (b & 0x10001u) << (4 * l + i);
+            }
+            d[0] = x, d[16] = y;
+        }
+        if (r == 0) bad[2 * h + a] = w;
+    }
+    // What `hide` left of a step, for a row that sees its first `see` tokens: the groups whose
+    // values are not finite.
+    static __device__ __forceinline__ uint32_t poison(const uint32_t *bad, int lane, int see) {
+        asm volatile("" : "+v"(lane));
+        const uint32_t mine = bad[lane & 15];
+        uint32_t groups = 0;
+        for (uint64_t left = __builtin_amdgcn_ballot_w64(mine != 0) & 0xffffu; left; left &= left - 1) {
+            const int from = __builtin_ctzll(left), a = from & 1, h = from >> 1 & 1;
+            for (uint32_t w = __builtin_amdgcn_readlane(mine, from); w; w &= w - 1) {
+                const int bit = __builtin_ctz(w), half = bit >> 4, l = bit >> 2 & 1, q = bit >> 1 & 1, pr = bit & 1;
+                const int tok = 16 * (from >> 2) + 4 * (a + 2 * q) + 2 * pr + half;
+                if (tok < see) groups |= 1u << ((D == 128 ? 2 * h + l : h) / (D / 32 / NG));
+            }
+        }
+        return groups;
+    }
     // lane (row r of the codes, quads a and a + 2, h): the 16 bytes of channels 32 (2 h + l) + 2 r + b;
     // at D = 64 h says which l of the two.  Slots from token nv on become 0.
     __device__ __forceinline__ void stage(unsigned char *vt, int tile, int lane, const Nibbles &nb, int nv) const {
@@ -322,6 +361,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
             const int f2 = min(f1, (sees(p, q, min((t + 1) * R, q.rows) - 1) + kStep - 1) / kStep);
             const int32_t *table = p.seqs.table + s * p.seqs.table_stride;
             float mx = kMinMax, l = 0.0f;
+            uint32_t poisoned = 0;  // groups of channels in which the row sees a value that is not finite
             f16v acc[NB];
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -379,9 +419,15 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
                                         (uint32_t)((mine & ((1 << log_tpp) - 1)) * TB);
                     raw.load((const unsigned char *)at, lane);
                 };
-                auto stage = [&](unsigned char *buf) {
-                    if constexpr (late) raw.stage(buf + KT, tl, lane, nb, nv);
-                    else raw.stage(buf, tl, lane, nb);
+                const int all_see = sees(p, q, t * R);
+                auto apart = [&](int step) { return kStep * (step + 1) > all_see; };  // rows see different tokens of it
+                auto stage = [&](unsigned char *buf, int step) {
+                    if constexpr (late) {
+                        raw.stage(buf + KT, tl, lane, nb, nv);
+                        if (apart(step)) raw.hide(buf + KT, (uint32_t *)(smem + 2 * BUF) + 16 * ((step - f0) & 1) + 4 * tl, tl, lane);
+                    } else {
+                        raw.stage(buf, tl, lane, nb);
+                    }
                 };
                 load(f0);
 
@@ -446,6 +492,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
                                 if (kStep * step + tok >= see || !(here >> (tok >> 4) & 1)) sc[b][i] = -INFINITY;
                             }
                     }
+                    if (apart(step))
+                        poisoned |= VLoad<D, NG>::poison((uint32_t *)(smem + 2 * BUF) + 16 * ((step - f0) & 1), lane, see - kStep * step);
                     float top = sc[0][0];
 #pragma unroll
                     for (int i = 1; i < 32; ++i) top = __builtin_fmaxf(top, sc[i >> 4][i & 15]);
@@ -475,7 +523,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
                                      [&](int i, h8 a) { acc[i % NB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pop[i / NB], acc[i % NB], 0, 0, 0); });
                 };
 
-                stage(smem);
+                stage(smem, f0);
                 __syncthreads();
                 if (late) __syncthreads();
                 for (int step = f0; step < f2; ++step) {
@@ -487,7 +535,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
                     if (seen) scores(buf);
                     __syncthreads();
                     if (seen) softmax(step, here);
-                    if (step + 1 < f2) stage(other);
+                    if (step + 1 < f2) stage(other, step + 1);
                     __syncthreads();
                 }
                 if (!late) __syncthreads();
@@ -500,6 +548,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
             }
 
             l += __shfl_xor(l, 32);
+            if (__builtin_amdgcn_ballot_w64(poisoned != 0))
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+                    if (poisoned >> (b / (NB / NG)) & 1) acc[b] += NAN;
             if (row0 + col < q.rows) {
                 if (f0 == 0 && f1 == n_steps) {
                     const int64_t o = (q.r.begin + row / p.g) * p.Hq + head;
@@ -635,7 +687,7 @@ static_assert((64 * kTileWaves + 1) * 8 <= kTileSums, "the sums fit");
 template <int D, int NG, bool TWO>
 hipError_t tile_go_as(const PagedAttnParams &p, hipStream_t st) {
     constexpr int W = kTileWaves;
-    constexpr int LDS = 2 * (TWO ? 3 : 2) * kStep * 2 * D;
+    constexpr int LDS = 2 * (TWO ? 3 : 2) * kStep * 2 * D + 2 * 16 * 4;  // two buffers, and what `hide` writes of each
     static_assert((64 * W + 1 + W) * 8 <= LDS, "the sums fit the buffers");
     auto kern = paged_tile_kernel<D, NG, W, TWO>;
     if (LDS > 48 * 1024) (void)hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);

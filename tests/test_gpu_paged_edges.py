@@ -1,0 +1,201 @@
+"""Calls of the paged 4-bit cache that a program makes seldom: values that are not finite next
+to rows that do not see them, batches on both sides of a choice of kernel, calls that overlap,
+calls that are replayed, tables of other orders, lists that name a token twice."""
+import numpy as np
+import pytest
+import torch
+
+import paged_ref as ref
+from gpu_util import announce
+from test_gpu_paged import DT, FORMS, World, _check_attention, _x
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("D,G,P", FORMS)
+@pytest.mark.parametrize("Hq,kv,m", [(8, 70, 6), (8, 500, 16), (8, 300, 90), (2, 3001, 200), (2, 150, 150)])
+def test_rows_do_not_feel_what_they_do_not_see(Hq, kv, m, D, G, P):
+    """Tokens with NaN values or keys among a chunk's own: the rows before them come out bit for
+    bit as if they were finite, the rows behind them NaN where the token's group reaches."""
+    import akv
+    announce(f"paged attention Hq={Hq} D={D} G={G} kv={kv} rows={m}, NaN in tokens that some rows see")
+    w = World(D, G, P, 2, [kv, 40], [m, 1])
+    w.fill()
+    g = Hq // 2
+    first, second, last = m // 3, m // 2, m - 1  # rows of the sequence: their own tokens
+    for dt in ("fp16", "bf16"):
+        k, v, q = (_x((w.T, h, D), i, dt) for i, h in ((1, 2), (2, 2), (3, Hq)))
+        akv.paged_append(w.pool, w.batch, k, v)
+        plain = [akv.paged_attention(q, w.pool, w.batch), *akv.paged_attention(q, w.pool, w.batch, return_lse=True)]
+        v[first, 1, D - 1] = float("nan")   # the last group of head 1
+        v[second, 0, 3] = float("inf")      # the first of head 0
+        k[last, 0, 0] = float("nan")
+        akv.paged_append(w.pool, w.batch, k, v)
+        got = [akv.paged_attention(q, w.pool, w.batch), *akv.paged_attention(q, w.pool, w.batch, return_lse=True)]
+        for a, b in zip(plain, got):
+            nan = torch.zeros_like(a, dtype=torch.bool)
+            nan[last:m, :g] = True          # a key that is NaN: everything of the rows that see it
+            if a.dim() == 3:
+                nan[first:m, g:, D - G:] = True
+                nan[second:m, :g, :G] = True
+            assert bool(b[nan].isnan().all())
+            assert torch.equal(a[~nan], b[~nan])
+
+
+@pytest.mark.parametrize("Hq,H,q", [(1, 1, [64, 65, 1, 66]), (8, 1, [8, 9, 0, 10]), (7, 1, [9, 10, 9]), (6, 2, [21, 22, 40])])
+def test_rows_on_both_sides_of_the_kernels(Hq, H, q):
+    """Sequences just below and above the rows from which on the tile kernel takes them, in one batch."""
+    announce(f"paged attention Hq={Hq} H={H} rows {q}")
+    w = World(128, 32, 16, H, [m + 130 for m in q], q)
+    w.fill()
+    for dt in ("fp16", "bf16"):
+        _check_attention(w, Hq, dt, True)
+
+
+def test_many_chunks():
+    """More chunks than the tile kernel's scan has threads, and runs of sequences without any."""
+    announce("paged attention, 700 sequences, every third a chunk of 70 rows")
+    q = [70 if i % 3 == 0 else (1 if i < 400 else 0) for i in range(700)]
+    kv = [m + i % 17 for i, m in enumerate(q)]
+    w = World(64, 32, 16, 1, kv, q)
+    w.fill()
+    _check_attention(w, 1, "fp16", True)
+
+
+def test_a_long_chunk_over_many_pages():
+    """Page tables longer than the entries a wave holds at a time, and runs that start inside."""
+    announce("paged attention, one chunk after 5000 tokens on 16-token pages")
+    w = World(64, 64, 16, 1, [5077], [77])
+    w.fill()
+    for dt in ("fp16", "bf16"):
+        _check_attention(w, 1, dt, True)
+        _check_attention(w, 1, dt, False)
+
+
+def test_one_batch_on_two_streams_at_once():
+    import akv
+    announce("paged attention, one batch on two streams")
+    w = World(128, 32, 16, 2, [700, 900, 80], [40, 1, 5])
+    w.fill()
+    qs = [_x((w.T, 8, 128), i, "bf16") for i in range(2)]
+    scores = torch.rand(3, 900, device="cuda")
+    alone = [akv.paged_attention(q, w.pool, w.batch, return_lse=True) for q in qs]
+    imps = [akv.paged_importance(q, a[1], w.pool, w.batch, scores, out=torch.empty_like(scores)) for q, a in zip(qs, alone)]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    both = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                o, l = akv.paged_attention(qs[i], w.pool, w.batch, return_lse=True)
+                both[i].append((o, l, akv.paged_importance(qs[i], l, w.pool, w.batch, scores, out=torch.empty_like(scores))))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o, l, imp in both[i]:
+            assert torch.equal(o, alone[i][0]) and torch.equal(l, alone[i][1]) and torch.equal(imp, imps[i])
+
+
+def test_replayed_chunks_follow_lengths_tables_and_rows():
+    """Two captured chunk calls, replayed in turns with eager work between, after the lengths, the
+    rows and the tables on the device have changed."""
+    import akv
+    announce("paged attention and importance of chunks, captured and replayed")
+    w = World(128, 32, 16, 2, [400, 900, 70], [30, 60, 2])
+    w.fill()
+    q = _x((w.T, 8, 128), 4)
+    scores = torch.rand(3, 900, device="cuda")
+
+    def work():
+        o, l = akv.paged_attention(q, w.pool, w.batch, return_lse=True)
+        return o, l, akv.paged_importance(q, l, w.pool, w.batch, scores, out=torch.empty_like(scores))
+    work()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = work()
+        graphs.append((graph, out))
+    for turn, (kv, starts) in enumerate([([400, 900, 70], [0, 30, 90, 92]), ([31, 64, 0], [0, 30, 90, 92]),
+                                         ([300, 899, 60], [0, 60, 61, 92]), ([300, 899, 60], [0, 0, 60, 60]),
+                                         ([400, 900, 70], [0, 30, 90, 92])]):
+        w.batch.kv_lens.copy_(torch.tensor(kv, dtype=torch.int32))
+        w.batch.q_starts.copy_(torch.tensor(starts, dtype=torch.int32))
+        if turn == 2:
+            w.batch.page_table[[0, 1]] = w.batch.page_table[[1, 0]]
+        want = work()
+        for graph, out in graphs:
+            for t in out:
+                t.fill_(7.0)
+            graph.replay()
+            torch.cuda.synchronize()
+            n = starts[-1]
+            assert torch.equal(out[0][:n], want[0][:n]) and torch.equal(out[1][:n], want[1][:n]) and torch.equal(out[2], want[2])
+            assert bool((out[0][n:] == 7.0).all()) and bool((out[1][n:] == 7.0).all())  # rows behind the last sequence's
+
+
+def test_tables_and_lists_of_other_kinds():
+    """int64, transposed, sliced and broadcast tables, and rows of other strides, say the same."""
+    import akv
+    announce("paged calls with tables and rows of other strides")
+    w = World(128, 64, 32, 2, [200, 200, 200], [3, 3, 3])
+    w.fill()
+    b = w.batch
+    b.page_table[:] = b.page_table[0]  # the three share their pages (read only)
+    q = _x((w.T, 8, 128), 1)
+    want = akv.paged_attention(q, w.pool, b)
+    wide = torch.full((3, 20), -1, dtype=torch.int32, device="cuda")
+    wide[:, 3:3 + b.page_table.shape[1]] = b.page_table
+    lens = torch.stack([b.kv_lens, b.kv_lens * 0], 1)[:, 0]
+    for table in (b.page_table.long(), b.page_table.t().contiguous().t(), wide[:, 3:3 + b.page_table.shape[1]],
+                  b.page_table[:1].expand(3, -1)):
+        other = akv.PagedBatch(table, lens, b.q_starts.long(), w.T, 3)
+        assert torch.equal(akv.paged_attention(q, w.pool, other), want)
+    for x in (_x((8, w.T, 128), 1).transpose(0, 1), _x((w.T, 8, 256), 1)[..., 100:228], _x((128, w.T, 8), 1).permute(1, 2, 0),
+              _x((1, 8, 128), 1).expand(w.T, 8, 128), _x((w.T, 1, 128), 1).expand(w.T, 8, 128)):
+        assert torch.equal(akv.paged_attention(x, w.pool, b), akv.paged_attention(x.contiguous(), w.pool, b))
+
+
+def test_compact_lists_that_name_a_token_often():
+    """keep may name a token twice, out of order, or none: what it says is moved."""
+    import akv
+    announce("paged compact, tokens named twice, lists of other kinds")
+    w = World(128, 32, 16, 2, [50, 33], [1, 1], spare=12, layers=2)
+    for layer in range(2):
+        w.fill(seed=layer, layer=layer)
+    dst = torch.from_numpy(w.spare[:8].reshape(2, 4).copy()).cuda()
+    keep = [[7] * 5 + [49, 0, 49, 3] * 6 + [2], [32, 31, 30] * 7]
+    rows = torch.full((2, 40), -1, dtype=torch.int64, device="cuda")
+    for s, k in enumerate(keep):
+        rows[s, :len(k)] = torch.tensor(k)
+    akv.compact_pages(w.pool, w.batch.page_table, dst, rows, torch.tensor([len(k) for k in keep], device="cuda"))
+    full = akv.PagedBatch(dst, torch.tensor([len(k) for k in keep], dtype=torch.int32, device="cuda"),
+                          torch.tensor([0, len(keep[0]), len(keep[0]) + len(keep[1])], dtype=torch.int32, device="cuda"),
+                          sum(map(len, keep)), max(map(len, keep)))
+    for layer in range(2):
+        k, v = akv.paged_read(w.pool, full, layer, torch.float32)
+        at = 0
+        for s, idx in enumerate(keep):
+            ek, ev = w.ref.read(layer, w.table[s], np.array(idx))
+            # c s + z in float32: one rounding of the sum, 2^-24 of it and of its parts
+            for x, e in ((k, ek), (v, ev)):
+                x = x[at:at + len(idx)].double().cpu().numpy()
+                assert (np.abs(x - e) <= np.abs(e) * 2.0 ** -23 + 2.0 ** -30).all()
+            at += len(idx)
+
+
+def test_a_prompt_of_more_rows_than_a_decode_call_may_count():
+    """131072 tokens' rows in one call are no decode work: only their own sequence's size counts.
+    (A few cached tokens and one head of them: the rows are padding past the sequence.)"""
+    import akv
+    announce("paged attention, a batch that allows 131072 rows a sequence")
+    w = World(64, 64, 256, 1, [300], [5])
+    w.fill()
+    T = 131072
+    table = torch.full((1, 512), -1, dtype=torch.int32, device="cuda")
+    table[:, :w.batch.page_table.shape[1]] = w.batch.page_table
+    big = akv.PagedBatch(table, w.batch.kv_lens, w.batch.q_starts, T, T)
+    q = torch.zeros(T, 64, 64, dtype=torch.float16, device="cuda")
+    q[:5] = _x((5, 64, 64), 2)
+    out = akv.paged_attention(q, w.pool, big)
+    # 5 rows x 64 heads are a chunk's rows in both calls
+    assert torch.equal(out[:5], akv.paged_attention(q[:5].contiguous(), w.pool, w.batch))
