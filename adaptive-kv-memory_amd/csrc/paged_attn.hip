@@ -53,46 +53,67 @@ __device__ __forceinline__ void load_row(u4 (&w)[D / 32], const unsigned char *r
     for (int g = 0; g < D / 32; ++g) w[g] = *(const u4 *)(row + (32 * g + 8 * grp) * 2);
 }
 
+// The row's maximum goes to [2^13, 2^14); channels that meet a code in the high nibble of its byte
+// are held divided by 16.
 template <int D, int NG>
 __device__ __forceinline__ void make_query(Query<D, NG> &Q, const u4 (&w)[D / 32], bool bf16, float scale_log2) {
     constexpr int NS = D / 32;
-    float x[NS][8];
-    float top = 0.0f;
+    int ex;  // top = f 2^ex, f in [1/2, 1)
     if (bf16) {
+        float x[NS][8];
+        float top = 0.0f;
 #pragma unroll
         for (int g = 0; g < NS; ++g)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const uint32_t v = w[g][i >> 1];
                 x[g][i] = __builtin_bit_cast(float, i & 1 ? v & 0xffff0000u : v << 16);
+                top = __builtin_fmaxf(top, __builtin_fabsf(x[g][i]));
             }
-    } else {
+        top = xmax(top);
+        ex = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 14;
+#pragma unroll
+        for (int g = 0; g < NS; ++g) {
+            float y[8];
+#pragma unroll
+            for (int n = 0; n < 8; ++n) y[n] = __builtin_ldexpf(x[g][n], (n & 1 ? 10 : 14) - ex);
+            Q.op[g] = (h8){(_Float16)y[0], (_Float16)y[4], (_Float16)y[1], (_Float16)y[5],
+                           (_Float16)y[2], (_Float16)y[6], (_Float16)y[3], (_Float16)y[7]};
+        }
+    } else {  // in float16 throughout: powers of two
+        typedef uint16_t s2 __attribute__((ext_vector_type(2)));
+        s2 most = {0, 0};
 #pragma unroll
         for (int g = 0; g < NS; ++g)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[g][i] = i & 1 ? hi_f(w[g][i >> 1]) : lo_f(w[g][i >> 1]);
-    }
+            for (int i = 0; i < 4; ++i)
+                most = __builtin_elementwise_max(most, __builtin_bit_cast(s2, (uint32_t)w[g][i] & 0x7fff7fffu));
+        const float top = xmax((float)__builtin_bit_cast(_Float16, most[0] > most[1] ? most[0] : most[1]));
+        // at most 2^30, in two steps (float16's largest is 2^15): then every step of the input is a whole number
+        ex = max(top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 14, -16);
+        const int e1 = min(14 - ex, 15);
+        const _Float16 a = (_Float16)__builtin_ldexpf(1.0f, e1), c = (_Float16)__builtin_ldexpf(1.0f, 14 - ex - e1);
+        const _Float16 d = (_Float16)__builtin_ldexpf(1.0f, 10 - ex - e1);
 #pragma unroll
-    for (int g = 0; g < NS; ++g)
+        for (int g = 0; g < NS; ++g) {
+            u4 y;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = __builtin_fmaxf(top, __builtin_fabsf(x[g][i]));
-    top = xmax(top);
-    const int ex = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 14;  // top = f 2^ex, f in [1/2, 1)
-#pragma unroll
-    for (int g = 0; g < NG; ++g) Q.sum[g] = 0.0f;
-#pragma unroll
-    for (int g = 0; g < NS; ++g) {
-        float y[8];
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            y[n] = __builtin_ldexpf(x[g][n], 14 - ex);
-            Q.sum[g * NG / NS] += y[n];
+            for (int n = 0; n < 4; ++n) {  // channels n and n + 4
+                const uint32_t at = (n & 1) ? 0x07060302u : 0x05040100u;
+                const h2 v = as_h2(__builtin_amdgcn_perm((uint32_t)w[g][2 + (n >> 1)], (uint32_t)w[g][n >> 1], at));
+                y[n] = as_u32(v * (h2){a, a} * (n & 1 ? (h2){d, d} : (h2){c, c}));
+            }
+            Q.op[g] = __builtin_bit_cast(h8, y);
         }
-        Q.op[g] = (h8){(_Float16)y[0], (_Float16)y[4], (_Float16)(y[1] * 0.0625f), (_Float16)(y[5] * 0.0625f),
-                       (_Float16)y[2], (_Float16)y[6], (_Float16)(y[3] * 0.0625f), (_Float16)(y[7] * 0.0625f)};
     }
+    const h8 ones = {1, 1, 16, 16, 1, 1, 16, 16};
 #pragma unroll
-    for (int g = 0; g < NG; ++g) Q.sum[g] = xsum(Q.sum[g]) * 0x1p-24f;
+    for (int g = 0; g < NG; ++g) {
+        f4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < NS / NG; ++st) c = mfma_k32(ones, Q.op[g * (NS / NG) + st], c);
+        Q.sum[g] = c[0] * 0x1p-24f;
+    }
     Q.kx = __builtin_ldexpf(scale_log2, ex + 10);
 }
 
