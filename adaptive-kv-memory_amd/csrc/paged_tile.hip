@@ -206,17 +206,16 @@ template <int D, int NG>
 struct VLoad {
     static constexpr int NL = NG == 4 ? 2 : 1;  // groups a lane's channels lie in
     Words<D / 32> c[2];                         // (quad a, a + 2): pairs (p, h) of row r
-    Words<2 * NL> s[2], z[2];                   // the same quads' meta pairs (group, p)
+    Words<1> m;                                 // a dword of the tile's meta
     __device__ __forceinline__ void load(const unsigned char *tile, int lane) {
-        const uint32_t r = lane & 15, a = (lane >> 4) & 1, h = lane >> 5;
-        const uint32_t code = (a * 16 + r) * (D / 8), meta = (a * NG + (NG == 4 ? 2 * h : NG == 2 ? h : 0)) * 8;
+        m.load(tile + 16 * D + 64 * NG, (uint32_t)(lane & (16 * NG - 1)) * 4);
+        const uint32_t r = lane & 15, a = (lane >> 4) & 1;
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            c[q].load(tile + 8 * D + q * 4 * D, code);
-            s[q].load(tile + 16 * D + 64 * NG + q * 16 * NG, meta);
-            z[q].load(tile + 16 * D + 96 * NG + q * 16 * NG, meta);
-        }
+        for (int q = 0; q < 2; ++q) c[q].load(tile + 8 * D + q * 4 * D, (a * 16 + r) * (D / 8));
     }
+    // The meta goes through LDS: a lane needs up to 16 dwords of it, which read from memory took
+    // four loads more and 16 registers through the products (500 of a step's 4700 cycles).
+    __device__ __forceinline__ void post(uint32_t *meta, int lane) const { meta[lane & (16 * NG - 1)] = m[0]; }
     // Where rows see different tokens, values that are not finite would reach those that do not
     // see them as 0 * NaN.  They become 0 in the lane's part of the staged tile, and word (h, a)
     // of the tile's four says which, for `poison`: bit 16 half + 4 l + 2 q + pr.
@@ -258,9 +257,18 @@ struct VLoad {
     }
     // lane (row r of the codes, quads a and a + 2, h): the 16 bytes of channels 32 (2 h + l) + 2 r + b;
     // at D = 64 h says which l of the two.  Slots from token nv on become 0.
-    __device__ __forceinline__ void stage(unsigned char *vt, int tile, int lane, const Nibbles &nb, int nv) const {
+    __device__ __forceinline__ void stage(unsigned char *vt, const uint32_t *meta, int tile, int lane, const Nibbles &nb, int nv) const {
         constexpr int L = D / 64;
         const int r = lane & 15, a = (lane >> 4) & 1, h = lane >> 5;
+        uint32_t s[2][2 * NL], z[2][2 * NL];    // the quads' pairs (group, p)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            typedef uint32_t vec __attribute__((ext_vector_type(2 * NL)));
+            const uint32_t at = ((a + 2 * q) * NG + (NG == 4 ? 2 * h : NG == 2 ? h : 0)) * 2;
+            const vec sv = *(const vec *)(meta + at), zv = *(const vec *)(meta + 8 * NG + at);
+#pragma unroll
+            for (int i = 0; i < 2 * NL; ++i) s[q][i] = sv[i], z[q][i] = zv[i];
+        }
         uint32_t keep[2][2] = {{~0u, ~0u}, {~0u, ~0u}};
         if (nv < 16) {
 #pragma unroll
@@ -421,9 +429,13 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
                 };
                 const int all_see = sees(p, q, t * R);
                 auto apart = [&](int step) { return kStep * (step + 1) > all_see; };  // rows see different tokens of it
+                uint32_t *meta = (uint32_t *)(smem + 2 * BUF) + 2 * 16 + 16 * NG * tl;
+                auto post = [&] {
+                    if constexpr (late) raw.post(meta, lane);
+                };
                 auto stage = [&](unsigned char *buf, int step) {
                     if constexpr (late) {
-                        raw.stage(buf + KT, tl, lane, nb, nv);
+                        raw.stage(buf + KT, meta, tl, lane, nb, nv);
                         if (apart(step)) raw.hide(buf + KT, (uint32_t *)(smem + 2 * BUF) + 16 * ((step - f0) & 1) + 4 * tl, tl, lane);
                     } else {
                         raw.stage(buf, tl, lane, nb);
@@ -523,6 +535,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
                                      [&](int i, h8 a) { acc[i % NB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pop[i / NB], acc[i % NB], 0, 0, 0); });
                 };
 
+                post();
                 stage(smem, f0);
                 __syncthreads();
                 if (late) __syncthreads();
@@ -533,6 +546,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
                     load(min(step + 1, f2 - 1));
                     if (step > f0 && kStep * (step - 1) < see_any) outputs(other);
                     if (seen) scores(buf);
+                    post();
                     __syncthreads();
                     if (seen) softmax(step, here);
                     if (step + 1 < f2) stage(other, step + 1);
@@ -687,7 +701,7 @@ static_assert((64 * kTileWaves + 1) * 8 <= kTileSums, "the sums fit");
 template <int D, int NG, bool TWO>
 hipError_t tile_go_as(const PagedAttnParams &p, hipStream_t st) {
     constexpr int W = kTileWaves;
-    constexpr int LDS = 2 * (TWO ? 3 : 2) * kStep * 2 * D + 2 * 16 * 4;  // two buffers, and what `hide` writes of each
+    constexpr int LDS = 2 * (TWO ? 3 : 2) * kStep * 2 * D + (2 * 16 + 4 * 16 * NG) * 4;  // two buffers, what `hide` writes of each, V meta
     static_assert((64 * W + 1 + W) * 8 <= LDS, "the sums fit the buffers");
     auto kern = paged_tile_kernel<D, NG, W, TWO>;
     if (LDS > 48 * 1024) (void)hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
