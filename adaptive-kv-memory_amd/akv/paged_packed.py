@@ -374,6 +374,18 @@ class PageLedger:
             self.lens[s] = n + c
         return copies
 
+    def undo_extend(self, seqs: Sequence[int], counts: Sequence[int], copies: Sequence[Tuple[int, int]]) -> None:
+        """Back to before an ``extend`` whose work could not be launched."""
+        for s, c in zip(seqs, counts):
+            self.crop(s, self.lens[s] - c)
+        back = {new: old for old, new in copies}
+        for s in seqs:
+            pages = self.pages[s]
+            if pages and pages[-1] in back:
+                new, pages[-1] = pages[-1], back[pages[-1]]
+                self.refs[pages[-1]] += 1
+                self._drop([new])
+
     def plan_compaction(self, seqs: Sequence[int], counts: Sequence[int]) -> List[List[int]]:
         """Indices of ``seqs`` in groups whose new pages are free at their turn (each group's
         old pages are given back before the next).  Raises when one does not fit."""
@@ -403,6 +415,10 @@ class PageLedger:
         self.pages[seq], self.lens[seq] = new, count
         return old, new
 
+    def undo_replace(self, seq: int, old: List[int], length: int) -> None:
+        self._drop(self.pages[seq])
+        self.pages[seq], self.lens[seq] = old, length
+
 
 class PackedPagedCache:
     """Sequences of one model in a pool of 4-bit pages, shared by all its layers.
@@ -410,7 +426,8 @@ class PackedPagedCache:
     A step: ``batch = cache.extend(seqs, counts)`` makes room (and copies the shared pages that
     will be written), then per layer ``append`` and ``attention``.  ``fork`` shares a sequence's
     pages; ``compact`` keeps chosen tokens; ``crop`` drops the last ones; ``remove`` frees.
-    Calls that are refused leave the cache as it was.  Work goes to the current stream."""
+    Calls that raise leave the cache as it was (a compaction in turns, the turns that are done).
+    Work goes to the current stream."""
 
     def __init__(self, num_layers: int, num_heads: int, head_dim: int, page_size: int = 16, max_pages: int = 4096,
                  group_size: int = 32, device="cuda"):
@@ -464,9 +481,14 @@ class PackedPagedCache:
         """Room for ``counts`` new tokens of each sequence: the batch whose rows they are."""
         counts = [counts] * len(seqs) if isinstance(counts, int) else [index(c) for c in counts]
         copies = self._book.extend(seqs, counts)
-        if copies:
-            copy_pages(self.pool, *self._upload([a for a, _ in copies], [b for _, b in copies]))
-        return self._batch(seqs, counts)
+        try:
+            batch = self._batch(seqs, counts)
+            if copies:
+                copy_pages(self.pool, *self._upload([a for a, _ in copies], [b for _, b in copies]))
+        except BaseException:
+            self._book.undo_extend(seqs, counts, copies)
+            raise
+        return batch
 
     # ---- a layer's work
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, batch: PagedBatch) -> None:
@@ -500,11 +522,17 @@ class PackedPagedCache:
         _check_device(self.pool, *keep)
         book = self._book
         for group in book.plan_compaction(seqs, counts):
+            lens = [book.lens[seqs[i]] for i in group]
             moved = [book.replace(seqs[i], counts[i]) for i in group]
-            old, wo = self._table([a for a, _ in moved])
-            new, wn = self._table([b for _, b in moved])
-            t_old, t_new, n = self._upload(old, new, [counts[i] for i in group])
-            rows = torch.nn.utils.rnn.pad_sequence([keep[i].to(torch.int32) for i in group], batch_first=True)
-            compact_pages(self.pool, t_old.view(len(group), wo), t_new.view(len(group), wn), rows, n)
+            try:
+                old, wo = self._table([a for a, _ in moved])
+                new, wn = self._table([b for _, b in moved])
+                t_old, t_new, n = self._upload(old, new, [counts[i] for i in group])
+                rows = torch.nn.utils.rnn.pad_sequence([keep[i].to(torch.int32) for i in group], batch_first=True)
+                compact_pages(self.pool, t_old.view(len(group), wo), t_new.view(len(group), wn), rows, n)
+            except BaseException:
+                for i, (a, _), n in zip(group, moved, lens):
+                    book.undo_replace(seqs[i], a, n)
+                raise
             for a, _ in moved:
                 book._drop(a)

@@ -199,3 +199,82 @@ def test_a_prompt_of_more_rows_than_a_decode_call_may_count():
     out = akv.paged_attention(q, w.pool, big)
     # 5 rows x 64 heads are a chunk's rows in both calls
     assert torch.equal(out[:5], akv.paged_attention(q[:5].contiguous(), w.pool, w.batch))
+
+
+def test_a_cache_whose_work_fails_is_as_it_was(monkeypatch):
+    """Uploads and launches that fail inside extend and compact: pages, lengths and contents stay."""
+    import akv
+    from akv import paged_packed
+    announce("paged cache, work that fails inside a call")
+    cache = akv.PackedPagedCache(2, 2, 64, max_pages=12)
+    a = cache.add_sequence()
+    batch = cache.extend([a], 40)
+    for layer in range(2):
+        cache.append(layer, _x((40, 2, 64), layer), _x((40, 2, 64), layer + 2), batch)
+    b, = cache.fork(a)
+
+    def state():
+        return ([cache.get_seq_length(s) for s in (a, b)], cache.num_free_pages,
+                [t for s in (a, b) for layer in range(2) for t in cache.get_kv(layer, s)])
+
+    def same(x, y):
+        return x[:2] == y[:2] and all(torch.equal(s, t) for s, t in zip(x[2], y[2]))
+    before = state()
+    keep = [torch.arange(0, 40, 3, device="cuda"), torch.arange(5, device="cuda")]
+
+    def fail(*args, **kw):
+        raise torch.OutOfMemoryError("no room")
+    for name in ("copy_pages", "compact_pages"):
+        monkeypatch.setattr(paged_packed, name, fail)
+    for _ in range(20):  # more often than there are pages
+        with pytest.raises(torch.OutOfMemoryError):
+            cache.extend([a, b], [1, 30])
+        with pytest.raises(torch.OutOfMemoryError):
+            cache.compact([a, b], keep)
+    monkeypatch.undo()
+    monkeypatch.setattr(cache, "_upload", fail)
+    for _ in range(20):
+        with pytest.raises(torch.OutOfMemoryError):
+            cache.extend([b], [30])
+        with pytest.raises(torch.OutOfMemoryError):
+            cache.compact([b], keep[1:])
+    monkeypatch.undo()
+    assert same(state(), before)
+    cache.compact([a, b], keep)
+    got = state()
+    for i in range(4):  # keys and values of both layers of a
+        assert torch.equal(got[2][i], before[2][i][:, ::3]) and torch.equal(got[2][4 + i], before[2][i][:, :5])
+
+
+def test_pages_past_32_bits_of_bytes():
+    """A pool of 5 GiB: sequences on its last pages answer as those on a small pool's."""
+    import akv
+    announce("paged cache, pages 4 GiB into a pool")
+    H, D, n = 8, 128, 262144
+    if torch.cuda.mem_get_info()[0] < 8 << 30:
+        pytest.skip("needs 8 GiB")
+    w = World(D, 32, 16, H, [100, 333], [100, 60], spare=30)
+    big = akv.PagedPool.empty(1, n, H, D, 16, 32)
+    assert big.nbytes() == 5 << 30
+    shift = n - w.ref.data.shape[1]
+    far = akv.PagedBatch(torch.where(w.batch.page_table < 0, w.batch.page_table, w.batch.page_table + shift), w.batch.kv_lens,
+                         w.batch.q_starts, w.T, 100)
+    w.fill()
+    big.data[:, shift:].copy_(w.pool.data)
+    k, v, q = _x((w.T, H, D), 1), _x((w.T, H, D), 2), _x((w.T, 16, D), 3, "bf16")
+    one = q[[0, 100]].contiguous()
+    spare = torch.from_numpy(w.spare[:20].copy()).cuda()
+    dst = spare[:14].view(2, 7)
+    keep = torch.arange(100, device="cuda", dtype=torch.int32).repeat(2, 1).flip(1)
+    res = []
+    for pool, batch, off in ((w.pool, w.batch, 0), (big, far, shift)):
+        akv.paged_append(pool, batch, k, v)
+        o, l = akv.paged_attention(q, pool, batch, return_lse=True)
+        ones = akv.PagedBatch(batch.page_table, batch.kv_lens, torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda"), 2, 1)
+        o1, l1 = akv.paged_attention(one, pool, ones, return_lse=True)
+        imp = akv.paged_importance(one, l1, pool, ones, torch.zeros(2, 333, device="cuda"))
+        akv.copy_pages(pool, batch.page_table[1, :6], spare[14:20] + off)
+        akv.compact_pages(pool, batch.page_table, dst + off, keep, torch.tensor([100, 90], device="cuda"))
+        res.append([o, l, o1, l1, imp, *akv.paged_read(pool, batch)])
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+    assert torch.equal(big.data[:, shift:], w.pool.data) and not bool(big.data[:, :shift:997].any())

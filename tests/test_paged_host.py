@@ -76,6 +76,31 @@ def test_ledger_refuses_whole():
     _whole(book)
 
 
+def test_ledger_undoes_what_was_not_launched():
+    """An extend or a replacement that is undone leaves pages, counts and lengths as they were."""
+    from akv.paged_packed import PageLedger
+    book = PageLedger(20, 16)
+    a = book.add()
+    book.extend([a], [40])
+    b, c = book.fork(a), book.add()
+    book.extend([c], [16])
+    state = lambda: ({s: list(p) for s, p in book.pages.items()}, dict(book.lens), list(book.refs), sorted(book.free))  # noqa: E731
+    before = state()
+    for counts in ([1, 1, 1], [30, 0, 5], [0, 9, 0], [0, 0, 0], [8, 8, 100]):
+        copies = book.extend([b, a, c], counts)
+        assert len(copies) == (1 if counts[0] or counts[1] else 0)
+        book.undo_extend([b, a, c], counts, copies)
+        assert state() == before
+        _whole(book)
+    for s, n in ((a, 3), (b, 40), (c, 0)):
+        length = book.lens[s]
+        old, _ = book.replace(s, n)
+        book.undo_replace(s, old, length)
+        assert state() == before
+        _whole(book)
+
+
+
 def test_ledger_at_random():
     from akv.paged_packed import PageLedger
     rng = random.Random(3)
