@@ -16,6 +16,11 @@ constexpr int kRows = 16;      // query rows (tokens x heads of a group) that a 
 // sequences of 8192 tokens, 48, 64 and 80 rows: 108, 132, 157 against 122, 118, 121; 64 of 1024:
 // 63, 66, 91 against 80, 81, 83; one of 32768: 39, 45, 50 against 56, 55, 59.
 constexpr int kFewRows = 64;
+// The same for the importance, by the rows that a call's sequences may have.  16 rows a wave
+// against 128 a workgroup, us: two sequences of 12000 tokens and 8 heads, 128, 256 and 2048 rows: 40,
+// 72, 502 against 38, 60, 362 (in bfloat16 33 against 37 at 128); one of 2000: 28, 50, 412 against
+// 25, 40, 229.
+constexpr int kFewWindowRows = 128;
 
 __host__ __device__ constexpr int paged_tile_bytes(int D, int ng) { return 16 * D + 128 * ng; }
 
@@ -102,6 +107,7 @@ hipError_t paged_attn_launch(const PagedAttnParams &p, hipStream_t s);
 int64_t paged_tile_plan(PagedAttnParams *p);
 hipError_t paged_tile_launch(const PagedAttnParams &p, hipStream_t s);
 hipError_t paged_importance_launch(const PagedImportanceParams &p, hipStream_t s);
+hipError_t paged_importance_tile_launch(const PagedImportanceParams &p, hipStream_t s);
 
 #ifdef __HIPCC__
 // Rows [begin, begin + n) of sequence s in the call's tensors, and its cached tokens.

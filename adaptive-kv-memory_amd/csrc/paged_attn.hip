@@ -842,6 +842,8 @@ hipError_t paged_attn_launch(const PagedAttnParams &p0, hipStream_t st) {
 hipError_t paged_importance_launch(const PagedImportanceParams &p0, hipStream_t st) {
     PagedImportanceParams p = p0;
     if (p.pool.n_pages == 0) p.seqs.width = 0;
+    const int64_t window = p.q_window > 0 ? std::min(p.q_window, p.seqs.max_q) : p.seqs.max_q;
+    if (window * p.g > kFewWindowRows) return paged_importance_tile_launch(p, st);
     p.head_split = p.pool.heads >= 4 ? 4 : p.pool.heads >= 2 ? 2 : 1;
     const int64_t tokens = kImpTiles * 16 * (kWaves / p.head_split);
     const dim3 grid((unsigned)((p.n_scores + tokens - 1) / tokens), p.seqs.n_seqs), block(kThreads);

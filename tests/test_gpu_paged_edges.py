@@ -42,6 +42,71 @@ def test_rows_do_not_feel_what_they_do_not_see(Hq, kv, m, D, G, P):
             assert torch.equal(a[~nan], b[~nan])
 
 
+@pytest.mark.parametrize("D,G,P", FORMS)
+@pytest.mark.parametrize("Hq,H,kv,q,win", [
+    (8, 2, [200, 70, 5], [40, 1, 5], 0), (3, 3, [1, 300, 0, 131], [1, 260, 0, 129], 0), (16, 2, [500, 65], [30, 17], 20),
+    (64, 1, [100, 64, 63], [3, 2, 1], 0),
+])
+def test_importance_of_chunks(Hq, H, kv, q, win, D, G, P):
+    """More rows than the wave kernel takes, ragged beside sequences of few and of none."""
+    import akv
+    announce(f"paged importance of chunks Hq={Hq} H={H} D={D} G={G} P={P} kv={kv} q={q} window={win}")
+    w = World(D, G, P, H, kv, q)
+    w.fill()
+    for dt, causal in (("fp16", True), ("bf16", False), ("bf16", True)):
+        x, lse = _check_attention(w, Hq, dt, causal)
+        for N in (max(kv) + 7, max(kv) // 2):
+            scores = torch.rand(len(kv), N + 3, device="cuda")[:, 1:N + 1]
+            old = scores.double().cpu().numpy()
+            out = torch.full((len(kv), N), -5.0, device="cuda")
+            akv.paged_importance(x, lse, w.pool, w.batch, scores, decay=0.75, q_window=win, causal=causal, out=out)
+            for s, (n, m) in enumerate(zip(kv, q)):
+                got = out[s].double().cpu().numpy()
+                at = min(n, N) if m else 0
+                assert np.array_equal(got[at:], old[s, at:])
+                if not at:
+                    continue
+                first = max(0, m - win) if win else 0
+                r = slice(w.starts[s] + first, w.starts[s + 1])
+                seen = np.arange(n - m + first, n) + 1 if causal else np.full(m - first, n)
+                kp, _ = w.ref.parts(0, w.table[s], np.arange(n))
+                e, d = ref.importance(x[r].double().cpu().numpy(), kp, D ** -0.5, seen, lse[r].double().cpu().numpy())
+                # keys as two float16 add up to them to 2^-22, which the bound's 64 roundings of 2^-24 hold
+                exp = 0.75 * old[s, :at] + e[:at]
+                assert (np.abs(got[:at] - exp) <= d[:at] + 2.0 ** -22 * (np.abs(exp) + old[s, :at])).all()
+            again = torch.full((len(kv), N), 3.0, device="cuda")
+            akv.paged_importance(x, lse, w.pool, w.batch, scores, decay=0.75, q_window=win, causal=causal, out=again)
+            assert torch.equal(out, again)
+            akv.paged_importance(x, lse, w.pool, w.batch, scores, decay=0.75, q_window=win, causal=causal)
+            assert torch.equal(out, scores)
+
+
+def test_importance_of_chunks_over_odd_pages():
+    """Table entries outside the pool and keys that are not finite count for no row that does not see them."""
+    import akv
+    announce("paged importance of chunks, pages outside the pool, NaN keys")
+    w = World(128, 32, 16, 2, [300], [150])
+    w.fill()
+    q = _x((150, 4, 128), 1)
+    k, v = _x((150, 2, 128), 2), _x((150, 2, 128), 3)
+    k[140, 0, 7] = float("nan")  # token 290: the last ten rows of heads 0 and 1 see it
+    akv.paged_append(w.pool, w.batch, k, v)
+    w.batch.page_table[0, 2] = 10 ** 6
+    w.batch.page_table[0, 7] = -1
+    zero = torch.zeros(1, 300, device="cuda")
+    _, lse = akv.paged_attention(q, w.pool, w.batch, return_lse=True)
+    assert bool(lse[140:, :2].isnan().all()) and bool(lse[:140].isfinite().all()) and bool(lse[:, 2:].isfinite().all())
+    got = akv.paged_importance(q[:140].contiguous(), lse[:140].contiguous(), w.pool, akv.PagedBatch(
+        w.batch.page_table, torch.tensor([290], device="cuda"), torch.tensor([0, 140], device="cuda"), 140, 140), zero, out=torch.empty_like(zero))
+    assert bool(got.isfinite().all()) and not bool(got[0, 32:48].any()) and not bool(got[0, 112:128].any())
+    assert bool((got[0, :32] > 0).all()) and not bool(got[0, 290:].any())
+    # every row's weights add up to 1: the two calls' scores are off by at most 64 roundings of 2^-24 of
+    # the terms they sum each, which are below 30
+    assert abs(float(got.double().sum()) - 140.0) < 140 * 2.0 ** -12
+    got = akv.paged_importance(q, lse, w.pool, w.batch, zero, out=torch.empty_like(zero))
+    assert bool(got[0, :32].isnan().all()) and not bool(got[0, 32:48].any()) and not bool(got[0, 112:128].any())
+
+
 @pytest.mark.parametrize("Hq,H,q", [(1, 1, [64, 65, 1, 66]), (8, 1, [8, 9, 0, 10]), (7, 1, [9, 10, 9]), (6, 2, [21, 22, 40])])
 def test_rows_on_both_sides_of_the_kernels(Hq, H, q):
     """Sequences just below and above the rows from which on the tile kernel takes them, in one batch."""
