@@ -234,7 +234,7 @@ __device__ __forceinline__ void write_row(const PagedAttnParams &p, const SeqRow
 // workgroup's runs are joined through LDS, items that several workgroups share leave partial
 // states for paged_merge_kernel.  A wave loads its tiles straight to registers, two units
 // ahead; the meta of a tile goes through LDS, where each lane reads its tokens'.
-template <int D, int NG>
+template <int D, int NG, bool TWO>
 __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAttnParams p) {
     constexpr int NS = D / 32, NB = D / 16, TB = paged_tile_bytes(D, NG), EROW = D + 4;
     constexpr int MW = NG == 4 ? 2 : 1;          // meta dwords a lane loads of a tile
@@ -408,13 +408,14 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
 #pragma unroll
             for (int e = 0; e < 8; ++e) pr[e] = __builtin_amdgcn_exp2f(sc[e >> 2][e & 3] + bias);
             l += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
-            // p, and p s below, as two float16 that add up to it: one alone would cost float16
-            // outputs half a step (measured 3.5e-4 of the output's norm; 2.1e-4 is its own rounding)
+            // float16 outputs: p, and p s below, as two float16 that add up to it: one alone would cost
+            // them half a step (measured 3.5e-4 of the output's norm; 2.1e-4 is its own rounding).
+            // Beside bfloat16's own 1.7e-3 one is as good.
             h2 ph[4], pl[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 ph[q] = (h2){(_Float16)pr[2 * q], (_Float16)pr[2 * q + 1]};
-                pl[q] = (h2){(_Float16)(pr[2 * q] - (float)ph[q][0]), (_Float16)(pr[2 * q + 1] - (float)ph[q][1])};
+                if constexpr (TWO) pl[q] = (h2){(_Float16)(pr[2 * q] - (float)ph[q][0]), (_Float16)(pr[2 * q + 1] - (float)ph[q][1])};
             }
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
@@ -426,10 +427,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
                     for (int q = 0; q < 2; ++q) {
                         const h2 sc2 = as_h2(sv[q]), t2 = ph[2 * i + q] * sc2;
                         pw[2 * i + q] = as_u32(t2);
-                        rw[2 * i + q] = as_u32(__builtin_elementwise_fma(pl[2 * i + q], sc2, __builtin_elementwise_fma(ph[2 * i + q], sc2, -t2)));
+                        if constexpr (TWO)
+                            rw[2 * i + q] = as_u32(__builtin_elementwise_fma(pl[2 * i + q], sc2, __builtin_elementwise_fma(ph[2 * i + q], sc2, -t2)));
                     }
                 }
-                const h8 pg = __builtin_bit_cast(h8, pw), rg = __builtin_bit_cast(h8, rw);
                 // the group's blocks of 16 channels: block 4 h + 2 l + b is nibble 2 l + b of half h
 #pragma unroll
                 for (int b = g * (NB / NG); b < (g + 1) * (NB / NG); ++b) {
@@ -440,8 +441,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
                         const uint32_t v = u.vc[q >> 1][(q & 1) * (NB / 4) + h4];
                         a[q] = (n >= 2 ? v >> 8 : v) & (n & 1 ? 0x00F000F0u : 0x000F000Fu);
                     }
-                    acc[b] = mfma_k32(__builtin_bit_cast(h8, a), pg, acc[b]);
-                    acc[b] = mfma_k32(__builtin_bit_cast(h8, a), rg, acc[b]);
+                    acc[b] = mfma_k32(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, pw), acc[b]);
+                    if constexpr (TWO) acc[b] = mfma_k32(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, rw), acc[b]);
                 }
             }
             u4 za = {0u, 0u, 0u, 0u};
@@ -451,7 +452,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
                 za = (u4){a[0], a[1], b[0], b[1]};
             }
             accz = mfma_k32(__builtin_bit_cast(h8, za), __builtin_bit_cast(h8, (u4){as_u32(ph[0]), as_u32(ph[1]), as_u32(ph[2]), as_u32(ph[3])}), accz);
-            accz = mfma_k32(__builtin_bit_cast(h8, za), __builtin_bit_cast(h8, (u4){as_u32(pl[0]), as_u32(pl[1]), as_u32(pl[2]), as_u32(pl[3])}), accz);
+            if constexpr (TWO) accz = mfma_k32(__builtin_bit_cast(h8, za), __builtin_bit_cast(h8, (u4){as_u32(pl[0]), as_u32(pl[1]), as_u32(pl[2]), as_u32(pl[3])}), accz);
         };
 
         auto consume = [&](const Query<D, NG> &Q, Unit &u, int j) {
@@ -823,14 +824,19 @@ hipError_t paged_attn_launch(const PagedAttnParams &p0, hipStream_t st) {
         if (lds > 48 * 1024) (void)hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         kern<<<dim3(p.groups), dim3(kThreads), lds, st>>>(p);
     };
-    if (p.D == 128) {
-        if (p.ng == 4) go(paged_decode_kernel<128, 4>);
-        else if (p.ng == 2) go(paged_decode_kernel<128, 2>);
-        else go(paged_decode_kernel<128, 1>);
-    } else {
-        if (p.ng == 2) go(paged_decode_kernel<64, 2>);
-        else go(paged_decode_kernel<64, 1>);
-    }
+    auto by_form = [&](auto two) {
+        constexpr bool TWO = decltype(two)::value;
+        if (p.D == 128) {
+            if (p.ng == 4) go(paged_decode_kernel<128, 4, TWO>);
+            else if (p.ng == 2) go(paged_decode_kernel<128, 2, TWO>);
+            else go(paged_decode_kernel<128, 1, TWO>);
+        } else {
+            if (p.ng == 2) go(paged_decode_kernel<64, 2, TWO>);
+            else go(paged_decode_kernel<64, 1, TWO>);
+        }
+    };
+    if (p.q_bf16) by_form(std::false_type{});
+    else by_form(std::true_type{});
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const dim3 grid(p.pool.heads * few_chunks(p), p.seqs.n_seqs);
