@@ -223,9 +223,10 @@ __device__ __forceinline__ void write_row(const PagedAttnParams &p, const SeqRow
 }  // namespace
 
 // Single tokens and a few drafted ones.  Bound by the cache's bytes and, nearly as much, by issue:
-// 340 vector instructions and 26 MFMAs for 32 tokens of a head, two waves a SIMD.  24 sequences
-// of 33 to 65536 tokens, 32 heads over 8 (299 MB): 62 us, 4.8 TB/s, and 5 us of merge; 20 rows
-// of nine sequences of 1001 to 9001 tokens: 18 us and 5.6 us; one row of 517 tokens, whose time
+// 270 vector instructions and 17 MFMAs for 32 tokens of a head (340 and 26 where p is two
+// float16), two waves a SIMD.  24 sequences of 33 to 65536 tokens, 32 heads over 8, bfloat16 (299
+// MB): 57.5 us, 5.2 TB/s, and 5 us of merge; 20 rows of nine sequences of 1001 to 9001 tokens,
+// float16: 18 us and 5.6 us; one row of 517 tokens, whose time
 // is the chain of loads from lengths to tiles: 6.2 us and 3.4 us.
 //
 // The units of all sequences, heads and chunks form one list, cut into equal runs, one a wave:
