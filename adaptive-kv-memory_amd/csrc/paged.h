@@ -77,6 +77,7 @@ struct PagedImportanceParams {
     float *out;
     int64_t n_scores, score_stride, out_stride;
     int head_split;            // waves that share a run of tokens, each with its heads
+    int head_lds, blocks;      // most heads of a wave; runs of a wave (a decode step's)
 };
 
 struct PagedCopyParams {

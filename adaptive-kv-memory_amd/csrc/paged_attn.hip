@@ -21,6 +21,10 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kImpTiles = 4;          // tiles of a wave's run in the importance
+constexpr int kImpBlocks = 4;         // most runs of a wave in a decode step's
+constexpr int kImpHeads = 3;          // most heads of a wave there
+// LDS of one head's query operand of 16 rows, its groups' sums, factor and log-sum.
+__host__ __device__ constexpr int paged_query_bytes(int D, int ng) { return 32 * D + 64 * (ng + 2); }
 constexpr int kMaxGroups = 512;       // two workgroups a compute unit: what registers allow at head_dim 128
 
 __device__ __forceinline__ float xmax(float x) {
@@ -760,9 +764,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_importance_kernel(const Pag
     for (int d = 8, c = NT * 2; d > 0; d >>= 1, c >>= 1)
 #pragma unroll
         for (int i = 0; i < c; ++i) {
-            const bool up = col & d;
-            const float mine = up ? sum[i + c] : sum[i], other = up ? sum[i] : sum[i + c];
-            sum[i] = mine + __shfl_xor(other, d);
+            float a = sum[i], b = sum[i + c];
+            asm("" : "+v"(a), "+v"(b));  // or a choice of values becomes one of indexes, 16 selects long
+            sum[i] = (col & d ? b : a) + __shfl_xor(col & d ? a : b, d);
         }
 #pragma unroll
     for (int i = 0; i < NT / 4; ++i) {
@@ -779,6 +783,176 @@ __global__ __launch_bounds__(kThreads, 2) void paged_importance_kernel(const Pag
         if (j < kv) {
             float v = 0.f;
             for (int q = 0; q < hs; ++q) v += sums[b * hs + q][i & (NT * 16 - 1)];
+            *out = __builtin_fmaf(*old, p.decay, v / (float)p.Hq);
+        } else if (out != old) {
+            *out = *old;
+        }
+    }
+}
+
+// The importance of a large decode step: at most 16 rows a head, few heads.  As above, but a wave makes
+// its heads' query operands once, in LDS, and takes p.blocks runs of 64 tokens, whose pages it looks up
+// at once, the next (run, head)'s keys in flight.  Bound by issue and memory, nearly even: one row of 24
+// sequences of 16000 tokens, 32 heads over 8 (246 MB of keys): 62 us, 4.0 TB/s, where the kernel above
+// takes 103; of 16 of 31744, 8 over 2: 29 against 42.  Lengths far apart keep less of the card
+// busy (eight of 1000 to 31744: 12.4 against 11.6).
+template <int D, int NG>
+__global__ __launch_bounds__(kThreads, 2) void paged_importance_step_kernel(const PagedImportanceParams p) {
+    constexpr int NS = D / 32, TB = paged_tile_bytes(D, NG), NT = kImpTiles, MT = 16 * NG;
+    constexpr uint32_t ALL = (1u << NT) - 1;
+    __shared__ __align__(16) uint32_t smeta[kWaves][NT * MT];
+    __shared__ float sums[kWaves][kImpBlocks * NT * 16];
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, grp = lane >> 4;
+    const int k_at = (4 * col + grp) * (D / 8);  // K codes of token col, quarter grp
+    const int s = blockIdx.y, hs = p.head_split, h0 = wave & (hs - 1), nh = (p.pool.heads - 1 - h0) / hs + 1;
+    const int runs = kWaves / hs, run_tok = p.blocks * NT * 16;
+    const SeqRows r = wave_uniform(seq_rows(p.seqs, s, p.pool.log_tpp + 4));
+    const int64_t tok0 = ((int64_t)blockIdx.x * runs + wave / hs) * run_tok;
+    const int n = min(r.n, p.seqs.max_q);
+    const int64_t kv = n > 0 ? min((int64_t)r.kv, p.n_scores) : 0;  // tokens whose score changes
+    if (tok0 < kv) {
+        const int first = p.q_window > 0 && p.q_window < n ? n - p.q_window : 0;
+        const int rows = (n - first) * p.g;
+        const bool live = col < rows;
+        const int row = live ? col : rows - 1, qt = first + row / p.g;
+        const int see = !live ? 0 : p.causal ? max(r.kv - r.n + qt + 1, 0) : r.kv;
+        const int log_tpp = p.pool.log_tpp, in_page = (1 << log_tpp) - 1;
+        const int32_t *table = p.seqs.table + s * p.seqs.table_stride;
+        const int t0 = (int)(tok0 >> 4);
+        // lane i: the page of tile i; tiles past the end or outside the pool read page 0 and count nothing
+        const bool there = lane < p.blocks * NT && 16 * (int64_t)(t0 + lane) < r.kv;
+        uint32_t page = there ? (uint32_t)table[(t0 + lane) >> log_tpp] : 0xffffffffu;
+        const uint32_t have = (uint32_t)__builtin_amdgcn_ballot_w64(page < p.pool.n_pages);
+        if (page >= p.pool.n_pages) page = 0;
+        struct Keys {
+            uint32_t kc[NT][NS], m[NT];
+        } K[2];
+        auto load = [&](Keys &k, int b, int h) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const unsigned char *tile = p.pool.base + (int64_t)(uint32_t)__builtin_amdgcn_readlane(page, NT * b + i) * p.pool.page_bytes +
+                                            (int64_t)((h << log_tpp) + ((t0 + NT * b + i) & in_page)) * TB;
+                if constexpr (D == 128) {
+                    const u4 a = *(const u4 *)(tile + k_at);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) k.kc[i][e] = a[e];
+                } else {
+                    const u2 a = *(const u2 *)(tile + k_at);
+                    k.kc[i][0] = a[0], k.kc[i][1] = a[1];
+                }
+                k.m[i] = *(const uint32_t *)(tile + 16 * D + (lane & (MT - 1)) * 4);
+            }
+        };
+        const int blocks = (int)min((int64_t)p.blocks, (kv - tok0 + NT * 16 - 1) / (NT * 16)), last = blocks * nh - 1;
+        // head k's operand: [NS][64 lanes] of 16 bytes, then [NG + 2][16 rows]: sums, factor, -lse
+        unsigned char *qs = smem + wave * p.head_lds * paged_query_bytes(D, NG);
+        u4 qw[kImpHeads][NS];
+        float lse[kImpHeads];
+#pragma unroll
+        for (int k = 0; k < kImpHeads; ++k) {  // all at once: the last head's again where there are fewer
+            const int64_t t = r.begin + qt;
+            const int head = (h0 + min(k, nh - 1) * hs) * p.g + row % p.g;
+            load_row<D>(qw[k], p.q + t * p.q_t + head * p.q_h);
+            lse[k] = p.lse[t * p.Hq + head];
+        }
+        load(K[0], 0, h0);
+        load(K[1], min(1, last) / nh, h0 + min(1, last) % nh * hs);
+#pragma unroll
+        for (int k = 0; k < kImpHeads; ++k) {
+            if (k >= nh) break;
+            Query<D, NG> Q;
+            make_query<D, NG>(Q, qw[k], p.q_bf16, p.scale_log2);
+            unsigned char *at = qs + k * paged_query_bytes(D, NG);
+#pragma unroll
+            for (int st = 0; st < NS; ++st) *(h8 *)(at + (st * 64 + lane) * 16) = Q.op[st];
+            float *f = (float *)(at + NS * 1024);
+            if (grp == 0) {
+#pragma unroll
+                for (int g = 0; g < NG; ++g) f[g * 16 + col] = Q.sum[g];
+                f[NG * 16 + col] = Q.kx;
+                f[(NG + 1) * 16 + col] = live ? lse[k] * -1.4426950408889634f : -INFINITY;
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+        float sum[NT * 4];
+#pragma unroll
+        for (int i = 0; i < NT * 4; ++i) sum[i] = 0.f;
+        uint32_t *meta = smeta[wave];
+        int b = 0, k = 0;     // the pair that is next
+        auto consume = [&](Keys &keys) {
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < NT; ++i) meta[i * MT + (lane & (MT - 1))] = keys.m[i];
+            __builtin_amdgcn_wave_barrier();
+            const unsigned char *at = qs + k * paged_query_bytes(D, NG);
+            const float *f = (const float *)(at + NS * 1024);
+            Query<D, NG> Q;
+#pragma unroll
+            for (int st = 0; st < NS; ++st) Q.op[st] = *(const h8 *)(at + (st * 64 + lane) * 16);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) Q.sum[g] = f[g * 16 + col];
+            Q.kx = f[NG * 16 + col];
+            const float bias = f[(NG + 1) * 16 + col];
+            const int64_t tok = tok0 + b * (NT * 16);
+            const uint32_t mine = have >> (NT * b) & ALL;
+            const bool clean = mine == ALL && __builtin_amdgcn_ballot_w64(tok + NT * 16 <= see || !live) == ~0ull;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const f4 x = tile_scores<D, NG>(Q, keys.kc[i], meta + i * MT);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], Q.kx, bias));
+                    if (!clean) pr = tok + 16 * i + 4 * grp + e < see && (mine >> i & 1) ? pr : 0.f;
+                    sum[4 * i + e] += pr;
+                }
+                __builtin_amdgcn_sched_barrier(0);  // one tile's meta in registers at a time
+            }
+            if (++k < nh) return;
+            k = 0;
+            // over the 16 rows: each step halves what a lane holds; lane col ends with its NT / 4 sums of the quad's
+#pragma unroll
+            for (int d = 8, c = NT * 2; d > 0; d >>= 1, c >>= 1)
+#pragma unroll
+                for (int i = 0; i < c; ++i) {
+                    float x = sum[i], y = sum[i + c];
+                    asm("" : "+v"(x), "+v"(y));  // or a choice of values becomes one of indexes, 16 selects long
+                    sum[i] = (col & d ? y : x) + __shfl_xor(col & d ? x : y, d);
+                }
+#pragma unroll
+            for (int i = 0; i < NT / 4; ++i) {
+                const int v = NT / 4 * col + i;  // tile v / 4, token 4 grp + v % 4 of it
+                sums[wave][b * (NT * 16) + 16 * (v >> 2) + 4 * grp + (v & 3)] = sum[i];
+            }
+#pragma unroll
+            for (int i = 0; i < NT * 4; ++i) sum[i] = 0.f;
+            ++b;
+        };
+        int lb = min(2, last) / nh, lk = min(2, last) % nh;  // the pair that is loaded next
+        auto ahead = [&](Keys &keys) {
+            load(keys, lb, h0 + lk * hs);
+            if (lb * nh + lk < last && ++lk == nh) lk = 0, ++lb;
+        };
+        int i = 0;
+        for (; i < last; i += 2) {
+            consume(K[0]);
+            ahead(K[0]);
+            consume(K[1]);
+            ahead(K[1]);
+        }
+        if (i == last) consume(K[0]);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < runs * run_tok; i += kThreads) {
+        const int64_t j = (int64_t)blockIdx.x * runs * run_tok + i;
+        if (j >= p.n_scores) break;
+        const int run = i / run_tok, in = i - run * run_tok;
+        const float *old = p.scores + s * p.score_stride + j;
+        float *out = p.out + s * p.out_stride + j;
+        if (j < kv) {
+            float v = 0.f;
+            for (int q = 0; q < hs; ++q) v += sums[run * hs + q][in];
             *out = __builtin_fmaf(*old, p.decay, v / (float)p.Hq);
         } else if (out != old) {
             *out = *old;
@@ -853,6 +1027,29 @@ hipError_t paged_importance_launch(const PagedImportanceParams &p0, hipStream_t 
     if (window * p.g > kFewWindowRows) return paged_importance_tile_launch(p, st);
     p.head_split = p.pool.heads >= 4 ? 4 : p.pool.heads >= 2 ? 2 : 1;
     const int64_t tokens = kImpTiles * 16 * (kWaves / p.head_split);
+    p.head_lds = (p.pool.heads + p.head_split - 1) / p.head_split;
+    // Runs a wave of a decode step: as many as leave three workgroups a compute unit, what fits there.
+    // Fewer than two do not pay for the operands' way through LDS (two sequences of 12000 tokens and 8
+    // heads: 9.8 us in the kernel below, 11.1 here).
+    const int64_t groups = (p.n_scores + tokens - 1) / tokens * p.seqs.n_seqs;
+    p.blocks = (int)std::min<int64_t>(kImpBlocks, (groups + 384) / 768);
+    if (window * p.g <= kRows && p.head_lds <= kImpHeads && p.blocks >= 2) {
+        const dim3 grid((unsigned)((p.n_scores + tokens * p.blocks - 1) / (tokens * p.blocks)), p.seqs.n_seqs);
+        auto go = [&](auto kern) {
+            const int lds = kWaves * p.head_lds * paged_query_bytes(p.D, p.ng);
+            if (lds > 48 * 1024) (void)hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+            kern<<<grid, dim3(kThreads), lds, st>>>(p);
+        };
+        if (p.D == 128) {
+            if (p.ng == 4) go(paged_importance_step_kernel<128, 4>);
+            else if (p.ng == 2) go(paged_importance_step_kernel<128, 2>);
+            else go(paged_importance_step_kernel<128, 1>);
+        } else {
+            if (p.ng == 2) go(paged_importance_step_kernel<64, 2>);
+            else go(paged_importance_step_kernel<64, 1>);
+        }
+        return hipGetLastError();
+    }
     const dim3 grid((unsigned)((p.n_scores + tokens - 1) / tokens), p.seqs.n_seqs), block(kThreads);
     if (p.D == 128) {
         if (p.ng == 4) paged_importance_kernel<128, 4><<<grid, block, 0, st>>>(p);

@@ -817,9 +817,9 @@ __global__ __launch_bounds__(256, 2) void paged_importance_tile_kernel(const Pag
     for (int d = 16; d > 0; d >>= 1)
 #pragma unroll
         for (int i = 0; i < d; ++i) {
-            const bool up = col & d;
-            const float mine = up ? v[i + d] : v[i], other = up ? v[i] : v[i + d];
-            v[i] = mine + __shfl_xor(other, d);
+            float a = v[i], b = v[i + d];
+            asm("" : "+v"(a), "+v"(b));  // or a choice of values becomes one of indexes, 32 selects long
+            v[i] = (col & d ? b : a) + __shfl_xor(col & d ? a : b, d);
         }
     sums[wave][32 * (col >> 4) + 8 * ((col >> 2) & 3) + 4 * hi + (col & 3)] = v[0];
     __syncthreads();

@@ -42,6 +42,34 @@ def test_rows_do_not_feel_what_they_do_not_see(Hq, kv, m, D, G, P):
             assert torch.equal(a[~nan], b[~nan])
 
 
+def _check_importance(w, x, lse, N, win, causal):
+    import akv
+    kv, q = w.kv, w.q
+    scores = torch.rand(len(kv), N + 3, device="cuda")[:, 1:N + 1]
+    old = scores.double().cpu().numpy()
+    out = torch.full((len(kv), N), -5.0, device="cuda")
+    akv.paged_importance(x, lse, w.pool, w.batch, scores, decay=0.75, q_window=win, causal=causal, out=out)
+    for s, (n, m) in enumerate(zip(kv, q)):
+        got = out[s].double().cpu().numpy()
+        at = min(n, N) if m else 0
+        assert np.array_equal(got[at:], old[s, at:])
+        if not at:
+            continue
+        first = max(0, m - win) if win else 0
+        r = slice(w.starts[s] + first, w.starts[s + 1])
+        seen = np.arange(n - m + first, n) + 1 if causal else np.full(m - first, n)
+        kp, _ = w.ref.parts(0, w.table[s], np.arange(n))
+        e, d = ref.importance(x[r].double().cpu().numpy(), kp, w.D ** -0.5, seen, lse[r].double().cpu().numpy())
+        # keys as two float16 add up to them to 2^-22, which the bound's 64 roundings of 2^-24 hold
+        exp = 0.75 * old[s, :at] + e[:at]
+        assert (np.abs(got[:at] - exp) <= d[:at] + 2.0 ** -22 * (np.abs(exp) + old[s, :at])).all()
+    again = torch.full((len(kv), N), 3.0, device="cuda")
+    akv.paged_importance(x, lse, w.pool, w.batch, scores, decay=0.75, q_window=win, causal=causal, out=again)
+    assert torch.equal(out, again)
+    akv.paged_importance(x, lse, w.pool, w.batch, scores, decay=0.75, q_window=win, causal=causal)
+    assert torch.equal(out, scores)
+
+
 @pytest.mark.parametrize("D,G,P", FORMS)
 @pytest.mark.parametrize("Hq,H,kv,q,win", [
     (8, 2, [200, 70, 5], [40, 1, 5], 0), (3, 3, [1, 300, 0, 131], [1, 260, 0, 129], 0), (16, 2, [500, 65], [30, 17], 20),
@@ -56,29 +84,38 @@ def test_importance_of_chunks(Hq, H, kv, q, win, D, G, P):
     for dt, causal in (("fp16", True), ("bf16", False), ("bf16", True)):
         x, lse = _check_attention(w, Hq, dt, causal)
         for N in (max(kv) + 7, max(kv) // 2):
-            scores = torch.rand(len(kv), N + 3, device="cuda")[:, 1:N + 1]
-            old = scores.double().cpu().numpy()
-            out = torch.full((len(kv), N), -5.0, device="cuda")
-            akv.paged_importance(x, lse, w.pool, w.batch, scores, decay=0.75, q_window=win, causal=causal, out=out)
-            for s, (n, m) in enumerate(zip(kv, q)):
-                got = out[s].double().cpu().numpy()
-                at = min(n, N) if m else 0
-                assert np.array_equal(got[at:], old[s, at:])
-                if not at:
-                    continue
-                first = max(0, m - win) if win else 0
-                r = slice(w.starts[s] + first, w.starts[s + 1])
-                seen = np.arange(n - m + first, n) + 1 if causal else np.full(m - first, n)
-                kp, _ = w.ref.parts(0, w.table[s], np.arange(n))
-                e, d = ref.importance(x[r].double().cpu().numpy(), kp, D ** -0.5, seen, lse[r].double().cpu().numpy())
-                # keys as two float16 add up to them to 2^-22, which the bound's 64 roundings of 2^-24 hold
-                exp = 0.75 * old[s, :at] + e[:at]
-                assert (np.abs(got[:at] - exp) <= d[:at] + 2.0 ** -22 * (np.abs(exp) + old[s, :at])).all()
-            again = torch.full((len(kv), N), 3.0, device="cuda")
-            akv.paged_importance(x, lse, w.pool, w.batch, scores, decay=0.75, q_window=win, causal=causal, out=again)
-            assert torch.equal(out, again)
-            akv.paged_importance(x, lse, w.pool, w.batch, scores, decay=0.75, q_window=win, causal=causal)
-            assert torch.equal(out, scores)
+            _check_importance(w, x, lse, N, win, causal)
+
+
+@pytest.mark.parametrize("D,G,P", [FORMS[0], FORMS[1], FORMS[2], FORMS[4]])
+@pytest.mark.parametrize("Hq,H", [(4, 1), (6, 2), (9, 3), (8, 4), (10, 5), (16, 8), (24, 12)])
+def test_importance_of_a_large_step(Hq, H, D, G, P):
+    """Few rows of calls large enough for several runs a wave: scores far wider than the sequences,
+    all splits of the heads over waves, two to four runs."""
+    announce(f"paged importance of a large step Hq={Hq} H={H} D={D} G={G} P={P}")
+    w = World(D, G, P, H, [1100, 0, 65, 257], [2, 0, 5, 1])
+    w.fill()
+    tokens = 64 * (4 if H == 1 else 2 if H < 4 else 1)
+    for runs, dt, win, causal in ((2, "fp16", 0, True), (3, "bf16", 1, True), (4, "fp16", 3, False)):
+        x, lse = _check_attention(w, Hq, dt, causal)
+        _check_importance(w, x, lse, 768 * runs // 4 * tokens - 5, win, causal)
+
+
+def test_importance_of_many_short_sequences():
+    """700 sequences of up to 200 tokens, idle and empty ones among them; pages outside the pool."""
+    import akv
+    announce("paged importance, 700 sequences")
+    rng = np.random.default_rng(2)
+    kv = rng.integers(0, 200, 700).tolist()
+    q = [0 if i % 7 == 3 else min(n, 1 + i % 3) for i, n in enumerate(kv)]
+    w = World(64, 32, 16, 5, kv, q)
+    w.fill()
+    x, lse = _check_attention(w, 5, "fp16", True)
+    _check_importance(w, x, lse, 203, 0, True)
+    before = akv.paged_importance(x, lse, w.pool, w.batch, torch.zeros(700, 203, device="cuda"))
+    w.batch.page_table[:, 1] = 10 ** 6
+    got = akv.paged_importance(x, lse, w.pool, w.batch, torch.zeros(700, 203, device="cuda"))
+    assert not bool(got[:, 16:32].any()) and torch.equal(got[:, :16], before[:, :16]) and torch.equal(got[:, 32:], before[:, 32:])
 
 
 def test_importance_of_chunks_over_odd_pages():
