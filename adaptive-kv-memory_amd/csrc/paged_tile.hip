@@ -357,7 +357,7 @@ __device__ __forceinline__ int tile_query(h8 (&op)[D / 16], const u4 (&w)[D / 16
 
 }  // namespace
 
-template <int D, int NG, int W, bool TWO>
+template <int D, int NG, int W, bool TWO, bool PTWO>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_tile_kernel(const PagedAttnParams p) {
     constexpr int R = 32 * W, NB = D / 32, TB = paged_tile_bytes(D, NG), EROW = D + 4;
     constexpr int KT = (TWO ? 2 : 1) * kStep * 2 * D, BUF = KT + kStep * 2 * D;
@@ -547,14 +547,39 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
                             pr[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[tile >> 1][8 * (tile & 1) + i], kx, bias));
-                        pop[tile] = (h8){(_Float16)pr[0], (_Float16)pr[1], (_Float16)pr[2], (_Float16)pr[3],
-                                         (_Float16)pr[4], (_Float16)pr[5], (_Float16)pr[6], (_Float16)pr[7]};
+                        if constexpr (PTWO)
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) sc[tile >> 1][8 * (tile & 1) + i] = pr[i];
+                        else
+                            pop[tile] = (h8){(_Float16)pr[0], (_Float16)pr[1], (_Float16)pr[2], (_Float16)pr[3],
+                                             (_Float16)pr[4], (_Float16)pr[5], (_Float16)pr[6], (_Float16)pr[7]};
                         l += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
                     }
                 };
                 auto outputs = [&](const unsigned char *buf) {
-                    products<4 * NB>([&](int i) { return *(const h8 *)(buf + KT + (i * 64 + lane) * 16); },
-                                     [&](int i, h8 a) { acc[i % NB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pop[i / NB], acc[i % NB], 0, 0, 0); });
+                    auto read = [&](int i) { return *(const h8 *)(buf + KT + (i * 64 + lane) * 16); };
+                    if constexpr (PTWO) {  // p waits in the scores' registers; an operand's second product
+                                           // comes behind the next one's first, or it would wait for its own
+                        h8 ph[4], pl[4], was;
+                        products<4 * NB>(read, [&](int i, h8 a) {
+                            const int t4 = i / NB;
+                            if (i % NB == 0)
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) {
+                                    const float x = sc[t4 >> 1][8 * (t4 & 1) + j];
+                                    ph[t4][j] = (_Float16)x;
+                                    pl[t4][j] = (_Float16)(x - (float)ph[t4][j]);
+                                }
+                            acc[i % NB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[t4], acc[i % NB], 0, 0, 0);
+                            if (i > 0) acc[(i - 1) % NB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(was, pl[(i - 1) / NB], acc[(i - 1) % NB], 0, 0, 0);
+                            was = a;
+                        });
+                        acc[NB - 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(was, pl[3], acc[NB - 1], 0, 0, 0);
+                    } else {
+                        products<4 * NB>(read, [&](int i, h8 a) {
+                            acc[i % NB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pop[i / NB], acc[i % NB], 0, 0, 0);
+                        });
+                    }
                 };
 
                 post();
@@ -840,12 +865,12 @@ constexpr int kTileGroups = 256;  // one workgroup a compute unit
 constexpr int64_t kTileSums = 8192;               // scan_tiles' sums at the start of the workspace
 static_assert((64 * kTileWaves + 1) * 8 <= kTileSums, "the sums fit");
 
-template <int D, int NG, bool TWO>
+template <int D, int NG, bool TWO, bool PTWO>
 hipError_t tile_go_as(const PagedAttnParams &p, hipStream_t st) {
     constexpr int W = kTileWaves;
     constexpr int LDS = 2 * (TWO ? 3 : 2) * kStep * 2 * D + (2 * 16 + 4 * 16 * NG) * 4;  // two buffers, what `hide` writes of each, V meta
     static_assert((64 * W + 1 + W) * 8 <= LDS, "the sums fit the buffers");
-    auto kern = paged_tile_kernel<D, NG, W, TWO>;
+    auto kern = paged_tile_kernel<D, NG, W, TWO, PTWO>;
     if (LDS > 48 * 1024) (void)hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
     kern<<<dim3(p.tile_groups), dim3(64 * W), LDS, st>>>(p);
     hipError_t e = hipGetLastError();
@@ -856,7 +881,8 @@ hipError_t tile_go_as(const PagedAttnParams &p, hipStream_t st) {
 }
 template <int D, int NG>
 hipError_t tile_go(const PagedAttnParams &p, hipStream_t st) {
-    return p.lse ? tile_go_as<D, NG, true>(p, st) : tile_go_as<D, NG, false>(p, st);
+    if (!p.q_bf16) return tile_go_as<D, NG, true, true>(p, st);
+    return p.lse ? tile_go_as<D, NG, true, false>(p, st) : tile_go_as<D, NG, false, false>(p, st);
 }
 }  // namespace
 
