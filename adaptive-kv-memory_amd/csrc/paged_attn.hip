@@ -1,14 +1,13 @@
 // Attention over the paged 4-bit cache, its merge, and the importance of cached tokens.
 //
 // The mathematics.  A key is c s + z with whole codes c and one float16 (s, z) per token and
-// channel group, so q.k = sum over groups of s (q.c) + z (sum of q): the matrix cores take the
-// codes themselves, and scale and zero enter once per score in float32.  A code in the low
-// bits of a float16 is the subnormal c 2^-24, or 16 c 2^-24 one nibble higher, exact in the
-// MFMA; the operand for the query takes the 1/16, its rows are scaled to a maximum in
-// [2^13, 2^14), and the factor 2^24 leaves with the softmax scale.  Scores are thus exact to
-// float32 rounding, whatever the cache's widths.  Values: o = sum of p (c s + z) is the product
-// of the codes with p s plus sum of p z, one more MFMA row per channel group; p and p s enter as two
-// float16 each.  Softmax state: running maximum and sum per row in float32.
+// channel group, so q.k = sum over groups of s (q.(c - 7)) + (z + 7 s) (sum of q): the matrix cores
+// take the codes themselves, and scale and zero enter once per score in float32.  The query's
+// rows are scaled to a maximum in [2^13, 2^14), which leaves with the softmax scale.  Scores are
+// thus exact to float32 rounding, whatever the cache's widths.  Values: o = sum of p (c s + z) is the
+// product of the codes with p s plus sum of p z, one more MFMA row per channel group; p and p s enter
+// as two float16 each, for bfloat16 outputs as one.  Softmax state: running maximum and sum per row in
+// float32.
 #include <algorithm>
 #include <type_traits>
 
@@ -35,9 +34,14 @@ __device__ __forceinline__ float xsum(float x) {
     x += __shfl_xor(x, 16);
     return x + __shfl_xor(x, 32);
 }
-__device__ __forceinline__ h8 code_operand(uint32_t w) {
+// Codes enter as c - 7: around zero the sums stay of the size of their result, and zeros are those of
+// such codes, z + 7 s.  (The MFMA cuts terms off below its largest, always downwards, and holds
+// subnormals at their exponent: codes of one sign left float16 outputs of 60000 tokens 6e-4 of
+// their norm off, subnormal ones the log-sums 1.5e-6.)
+constexpr int kMid = 7;
+__device__ __forceinline__ h8 code_operand(const Nibbles &nb, uint32_t w) {
     const uint32_t v = w >> 8;
-    return __builtin_bit_cast(h8, (u4){w & 0x000F000Fu, w & 0x00F000F0u, v & 0x000F000Fu, v & 0x00F000F0u});
+    return __builtin_bit_cast(h8, (u4){as_u32(nb.low<kMid>(w)), as_u32(nb.high<kMid>(w)), as_u32(nb.low<kMid>(v)), as_u32(nb.high<kMid>(v))});
 }
 __device__ __forceinline__ float lo_f(uint32_t w) { return (float)as_h2(w)[0]; }
 __device__ __forceinline__ float hi_f(uint32_t w) { return (float)as_h2(w)[1]; }
@@ -46,7 +50,7 @@ __device__ __forceinline__ float hi_f(uint32_t w) { return (float)as_h2(w)[1]; }
 template <int D, int NG>
 struct Query {
     h8 op[D / 32];
-    float sum[NG];  // of the group's channels, times 2^-24
+    float sum[NG];  // of the group's channels
     float kx;       // score -> log2 domain
 };
 
@@ -57,8 +61,7 @@ __device__ __forceinline__ void load_row(u4 (&w)[D / 32], const unsigned char *r
     for (int g = 0; g < D / 32; ++g) w[g] = *(const u4 *)(row + (32 * g + 8 * grp) * 2);
 }
 
-// The row's maximum goes to [2^13, 2^14); channels that meet a code in the high nibble of its byte
-// are held divided by 16.
+// The row's maximum goes to [2^13, 2^14).
 template <int D, int NG>
 __device__ __forceinline__ void make_query(Query<D, NG> &Q, const u4 (&w)[D / 32], bool bf16, float scale_log2) {
     constexpr int NS = D / 32;
@@ -80,7 +83,7 @@ __device__ __forceinline__ void make_query(Query<D, NG> &Q, const u4 (&w)[D / 32
         for (int g = 0; g < NS; ++g) {
             float y[8];
 #pragma unroll
-            for (int n = 0; n < 8; ++n) y[n] = __builtin_ldexpf(x[g][n], (n & 1 ? 10 : 14) - ex);
+            for (int n = 0; n < 8; ++n) y[n] = __builtin_ldexpf(x[g][n], 14 - ex);
             Q.op[g] = (h8){(_Float16)y[0], (_Float16)y[4], (_Float16)y[1], (_Float16)y[5],
                            (_Float16)y[2], (_Float16)y[6], (_Float16)y[3], (_Float16)y[7]};
         }
@@ -97,7 +100,6 @@ __device__ __forceinline__ void make_query(Query<D, NG> &Q, const u4 (&w)[D / 32
         ex = max(top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 14, -16);
         const int e1 = min(14 - ex, 15);
         const _Float16 a = (_Float16)__builtin_ldexpf(1.0f, e1), c = (_Float16)__builtin_ldexpf(1.0f, 14 - ex - e1);
-        const _Float16 d = (_Float16)__builtin_ldexpf(1.0f, 10 - ex - e1);
 #pragma unroll
         for (int g = 0; g < NS; ++g) {
             u4 y;
@@ -105,46 +107,52 @@ __device__ __forceinline__ void make_query(Query<D, NG> &Q, const u4 (&w)[D / 32
             for (int n = 0; n < 4; ++n) {  // channels n and n + 4
                 const uint32_t at = (n & 1) ? 0x07060302u : 0x05040100u;
                 const h2 v = as_h2(__builtin_amdgcn_perm((uint32_t)w[g][2 + (n >> 1)], (uint32_t)w[g][n >> 1], at));
-                y[n] = as_u32(v * (h2){a, a} * (n & 1 ? (h2){d, d} : (h2){c, c}));
+                y[n] = as_u32(v * (h2){a, a} * (h2){c, c});
             }
             Q.op[g] = __builtin_bit_cast(h8, y);
         }
     }
-    const h8 ones = {1, 1, 16, 16, 1, 1, 16, 16};
+    const h8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
         f4 c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int st = 0; st < NS / NG; ++st) c = mfma_k32(ones, Q.op[g * (NS / NG) + st], c);
-        Q.sum[g] = c[0] * 0x1p-24f;
+        Q.sum[g] = c[0];
     }
-    Q.kx = __builtin_ldexpf(scale_log2, ex + 10);
+    Q.kx = __builtin_ldexpf(scale_log2, ex - 14);
 }
 
-// Scores (times 2^-24 of the scaled query) of tokens 4 grp + e of a tile for row col.  `meta`:
-// the tile's K meta in LDS.
+// K meta dword d of a tile for tile_scores: float32 scales, then float32 zeros of the centred codes.
+template <int NG>
+__device__ __forceinline__ void put_k_meta(float *meta, int d, uint32_t w) {
+    const float s = lo_f(w);
+    meta[d] = s;
+    meta[16 * NG + d] = __builtin_fmaf(s, (float)kMid, hi_f(w));
+}
+// Scores (of the scaled query) of tokens 4 grp + e of a tile for row col.  `meta`:
+// what put_k_meta left of the tile.
 template <int D, int NG>
-__device__ __forceinline__ f4 tile_scores(const Query<D, NG> &Q, const uint32_t (&kc)[D / 32], const uint32_t *meta) {
+__device__ __forceinline__ f4 tile_scores(const Query<D, NG> &Q, const Nibbles &nb, const uint32_t (&kc)[D / 32], const float *meta) {
     constexpr int NS = D / 32;
     const int grp = (threadIdx.x >> 4) & 3;
-    uint32_t m[4 * NG];
+    float m[4 * NG], z[4 * NG];
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
-        const u4 w = ((const u4 *)meta)[grp * NG + i];
+        const f4 w = ((const f4 *)meta)[grp * NG + i], y = ((const f4 *)meta)[4 * NG + grp * NG + i];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) m[4 * i + e] = w[e];
+        for (int e = 0; e < 4; ++e) m[4 * i + e] = w[e], z[4 * i + e] = y[e];
     }
     f4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
         f4 c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int st = 0; st < NS / NG; ++st) c = mfma_k32(code_operand(kc[g * (NS / NG) + st]), Q.op[g * (NS / NG) + st], c);
+        for (int st = 0; st < NS / NG; ++st) c = mfma_k32(code_operand(nb, kc[g * (NS / NG) + st]), Q.op[g * (NS / NG) + st], c);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const uint32_t w = m[e * NG + g];
-            s[e] = __builtin_fmaf(lo_f(w), c[e], s[e]);
-            s[e] = __builtin_fmaf(hi_f(w), Q.sum[g], s[e]);
+            s[e] = __builtin_fmaf(m[e * NG + g], c[e], s[e]);
+            s[e] = __builtin_fmaf(z[e * NG + g], Q.sum[g], s[e]);
         }
     }
     return s;
@@ -227,11 +235,11 @@ __device__ __forceinline__ void write_row(const PagedAttnParams &p, const SeqRow
 }  // namespace
 
 // Single tokens and a few drafted ones.  Bound by the cache's bytes and, nearly as much, by issue:
-// 270 vector instructions and 17 MFMAs for 32 tokens of a head (340 and 26 where p is two
+// 300 vector instructions and 17 MFMAs for 32 tokens of a head (400 and 27 where p is two
 // float16), two waves a SIMD.  24 sequences of 33 to 65536 tokens, 32 heads over 8, bfloat16 (299
-// MB): 57.5 us, 5.2 TB/s, and 5 us of merge; 20 rows of nine sequences of 1001 to 9001 tokens,
-// float16: 18 us and 5.6 us; one row of 517 tokens, whose time
-// is the chain of loads from lengths to tiles: 6.2 us and 3.4 us.
+// MB): 61 us, 4.9 TB/s, and 5 us of merge; 20 rows of nine sequences of 1001 to 9001 tokens,
+// float16: 21 us and 5.6 us; one row of 517 tokens, whose time
+// is the chain of loads from lengths to tiles: 6.6 us and 3.4 us.
 //
 // The units of all sequences, heads and chunks form one list, cut into equal runs, one a wave:
 // every wave has the same work whatever the lengths.  A run that covers an item (all units of
@@ -250,8 +258,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
     const int col = lane & 15, grp = lane >> 4;
     const int k_at = (4 * col + grp) * (D / 8);  // K codes of token col, quarter grp
     float *entries = (float *)smem;
-    uint32_t *meta = (uint32_t *)(smem + 2 * kWaves * p.rows * EROW * 4) + wave * 2 * 32 * NG;
+    uint32_t *meta = (uint32_t *)(smem + 2 * kWaves * p.rows * EROW * 4) + wave * 2 * 48 * NG;
     if (lane < 2) e_flags[2 * wave + lane] = 0;
+    Nibbles nb;
+    nb.init();
 
     const int per = (p.seqs.n_seqs + kThreads - 1) / kThreads;
     scan_seqs(p, sc, per);
@@ -379,15 +389,22 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                uint32_t *m = meta + i * 32 * NG;
-                if constexpr (MW == 2) *(u2 *)(m + 2 * lane) = (u2){u.m[i][0], u.m[i][1]};
-                else m[lane & (32 * NG - 1)] = u.m[i][0];
+                // K scales and zeros as float32, then the V half as it is
+                uint32_t *m = meta + i * 48 * NG;
+#pragma unroll
+                for (int q = 0; q < MW; ++q) {
+                    const int d = (lane & (32 * NG / MW - 1)) * MW + q;
+                    const uint32_t w = u.m[i][q];
+                    const float ks = lo_f(w), kz = __builtin_fmaf(ks, (float)kMid, hi_f(w));
+                    m[16 * NG + d] = d < 16 * NG ? __builtin_bit_cast(uint32_t, kz) : w;
+                    if (d < 16 * NG) m[d] = __builtin_bit_cast(uint32_t, ks);
+                }
             }
             __builtin_amdgcn_wave_barrier();
             f4 sc[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                sc[i] = tile_scores<D, NG>(Q, u.kc[i], meta + i * 32 * NG) * Q.kx;
+                sc[i] = tile_scores<D, NG>(Q, nb, u.kc[i], (const float *)meta + i * 48 * NG) * Q.kx;
                 if constexpr (!clean)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -427,7 +444,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
                 u4 pw, rw;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const u2 sv = *(const u2 *)(meta + i * 32 * NG + 16 * NG + (grp * NG + g) * 2);
+                    const u2 sv = *(const u2 *)(meta + i * 48 * NG + 32 * NG + (grp * NG + g) * 2);
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         const h2 sc2 = as_h2(sv[q]), t2 = ph[2 * i + q] * sc2;
@@ -444,20 +461,39 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         const uint32_t v = u.vc[q >> 1][(q & 1) * (NB / 4) + h4];
-                        a[q] = (n >= 2 ? v >> 8 : v) & (n & 1 ? 0x00F000F0u : 0x000F000Fu);
+                        const uint32_t x = n >= 2 ? v >> 8 : v;
+                        if constexpr (TWO) a[q] = as_u32(n & 1 ? nb.high<kMid>(x) : nb.low<kMid>(x));
+                        else a[q] = x & (n & 1 ? 0x00F000F0u : 0x000F000Fu);  // subnormals: c 2^-24, 16 c 2^-24
                     }
                     acc[b] = mfma_k32(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, pw), acc[b]);
                     if constexpr (TWO) acc[b] = mfma_k32(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, rw), acc[b]);
                 }
             }
-            u4 za = {0u, 0u, 0u, 0u};
+            // row g of the operand: the tokens' zeros of group g (of the centred codes: two float16)
+            u4 za = {0u, 0u, 0u, 0u}, zl = {0u, 0u, 0u, 0u};
             if (col < NG) {
-                const u2 a = *(const u2 *)(meta + 24 * NG + (grp * NG + col) * 2);
-                const u2 b = *(const u2 *)(meta + 32 * NG + 24 * NG + (grp * NG + col) * 2);
-                za = (u4){a[0], a[1], b[0], b[1]};
+                const uint32_t *at = meta + 32 * NG + (grp * NG + col) * 2;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const u2 zw = *(const u2 *)(at + i * 48 * NG + 8 * NG), sw = *(const u2 *)(at + i * 48 * NG);
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        za[2 * i + q] = zw[q];
+                        if constexpr (TWO) {
+                            const float x = __builtin_fmaf(lo_f(sw[q]), (float)kMid, lo_f(zw[q])), y = __builtin_fmaf(hi_f(sw[q]), (float)kMid, hi_f(zw[q]));
+                            const h2 h = {(_Float16)x, (_Float16)y};
+                            za[2 * i + q] = as_u32(h);
+                            zl[2 * i + q] = as_u32((h2){(_Float16)(x - (float)h[0]), (_Float16)(y - (float)h[1])});
+                        }
+                    }
+                }
             }
-            accz = mfma_k32(__builtin_bit_cast(h8, za), __builtin_bit_cast(h8, (u4){as_u32(ph[0]), as_u32(ph[1]), as_u32(ph[2]), as_u32(ph[3])}), accz);
-            if constexpr (TWO) accz = mfma_k32(__builtin_bit_cast(h8, za), __builtin_bit_cast(h8, (u4){as_u32(pl[0]), as_u32(pl[1]), as_u32(pl[2]), as_u32(pl[3])}), accz);
+            const h8 p_hi = __builtin_bit_cast(h8, (u4){as_u32(ph[0]), as_u32(ph[1]), as_u32(ph[2]), as_u32(ph[3])});
+            accz = mfma_k32(__builtin_bit_cast(h8, za), p_hi, accz);
+            if constexpr (TWO) {
+                accz = mfma_k32(__builtin_bit_cast(h8, zl), p_hi, accz);
+                accz = mfma_k32(__builtin_bit_cast(h8, za), __builtin_bit_cast(h8, (u4){as_u32(pl[0]), as_u32(pl[1]), as_u32(pl[2]), as_u32(pl[3])}), accz);
+            }
         };
 
         auto consume = [&](const Query<D, NG> &Q, Unit &u, int j) {
@@ -482,7 +518,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
         }
         if (j < jn) consume(Q, U[0], j);
 
-        // the segment's state in true units: 2^24 of the codes (2^20 where they lay a nibble higher), zeros
+        // the segment's state in true units (of subnormal codes 2^24, or 2^20 where they lay a nibble higher)
         l = xsum(l);
         float z[NG];
 #pragma unroll
@@ -498,8 +534,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
             float o[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                o[2 * i] = __builtin_fmaf(acc[2 * g][i], 0x1p24f, z[g * NG / NS]);
-                o[2 * i + 1] = __builtin_fmaf(acc[2 * g + 1][i], 0x1p20f, z[g * NG / NS]);
+                o[2 * i] = __builtin_fmaf(acc[2 * g][i], TWO ? 1.f : 0x1p24f, z[g * NG / NS]);
+                o[2 * i + 1] = __builtin_fmaf(acc[2 * g + 1][i], TWO ? 1.f : 0x1p20f, z[g * NG / NS]);
             }
             const int ch = 32 * g + 8 * grp;
             if (col < rows) {
@@ -662,15 +698,14 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnPa
 // split over the waves of a workgroup, at most four ways), the next head's keys in flight; the
 // sums over rows stay in registers, lane by lane of a row, until the end, and are joined in a
 // fixed order.  Bound by latency and issue (360 vector instructions for 16 rows and 64 tokens of a
-// head), the K half of the cache behind them: one row of eight sequences of 1000 to 31744 tokens,
-// 12 heads over 2: 11.5 us, 2.7 for the bytes; 32 rows of two sequences of 8191 to 16384 tokens, 32
-// heads over 8: 33 us.  (Queries of the next rows in flight, or three waves a SIMD without the
+// head), the K half of the cache behind them: one row of two sequences of 12000 tokens, 32 heads over
+// 8: 10.4 us; 32 rows of two sequences of 8191 to 16384 tokens: 32 us.  (Queries of the next rows in flight, or three waves a SIMD without the
 // second buffer, were no faster: 34 and 41 us.)
 template <int D, int NG>
 __global__ __launch_bounds__(kThreads, 2) void paged_importance_kernel(const PagedImportanceParams p) {
     constexpr int NS = D / 32, TB = paged_tile_bytes(D, NG), NT = kImpTiles, MT = 16 * NG;
     constexpr uint32_t ALL = (1u << NT) - 1;
-    __shared__ __align__(16) uint32_t smeta[kWaves][NT * MT];
+    __shared__ __align__(16) float smeta[kWaves][NT * 2 * MT];
     __shared__ float sums[kWaves][NT * 16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
@@ -686,7 +721,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_importance_kernel(const Pag
     float sum[NT * 4];
 #pragma unroll
     for (int i = 0; i < NT * 4; ++i) sum[i] = 0.f;
-    uint32_t *meta = smeta[wave];
+    float *meta = smeta[wave];
+    Nibbles nb;
+    nb.init();
     if (tok0 < kv) {
         const int log_tpp = p.pool.log_tpp, in_page = (1 << log_tpp) - 1;
         const int32_t *table = p.seqs.table + s * p.seqs.table_stride;
@@ -718,7 +755,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_importance_kernel(const Pag
         auto consume = [&](Keys &k, int h) {
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int i = 0; i < NT; ++i) meta[i * MT + (lane & (MT - 1))] = k.m[i];
+            for (int i = 0; i < NT; ++i) put_k_meta<NG>(meta + i * 2 * MT, lane & (MT - 1), k.m[i]);
             __builtin_amdgcn_wave_barrier();
             for (int row0 = 0; row0 < rows; row0 += kRows) {
                 const bool live = row0 + col < rows;
@@ -736,7 +773,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_importance_kernel(const Pag
                 const bool clean = have == ALL && __builtin_amdgcn_ballot_w64(tok0 + NT * 16 <= see) == ~0ull;
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
-                    const f4 x = tile_scores<D, NG>(Q, k.kc[i], meta + i * MT);
+                    const f4 x = tile_scores<D, NG>(Q, nb, k.kc[i], meta + i * 2 * MT);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], Q.kx, bias));
@@ -793,14 +830,13 @@ __global__ __launch_bounds__(kThreads, 2) void paged_importance_kernel(const Pag
 // The importance of a large decode step: at most 16 rows a head, few heads.  As above, but a wave makes
 // its heads' query operands once, in LDS, and takes p.blocks runs of 64 tokens, whose pages it looks up
 // at once, the next (run, head)'s keys in flight.  Bound by issue and memory, nearly even: one row of 24
-// sequences of 16000 tokens, 32 heads over 8 (246 MB of keys): 62 us, 4.0 TB/s, where the kernel above
-// takes 103; of 16 of 31744, 8 over 2: 29 against 42.  Lengths far apart keep less of the card
-// busy (eight of 1000 to 31744: 12.4 against 11.6).
+// sequences of 16000 tokens, 32 heads over 8 (246 MB of keys): 69 us, 3.6 TB/s, where the kernel above
+// took 103.  Lengths far apart keep less of the card busy (eight of 1000 to 31744: 13.0 against 12).
 template <int D, int NG>
 __global__ __launch_bounds__(kThreads, 2) void paged_importance_step_kernel(const PagedImportanceParams p) {
     constexpr int NS = D / 32, TB = paged_tile_bytes(D, NG), NT = kImpTiles, MT = 16 * NG;
     constexpr uint32_t ALL = (1u << NT) - 1;
-    __shared__ __align__(16) uint32_t smeta[kWaves][NT * MT];
+    __shared__ __align__(16) float smeta[kWaves][NT * 2 * MT];
     __shared__ float sums[kWaves][kImpBlocks * NT * 16];
     extern __shared__ __align__(16) unsigned char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -879,12 +915,14 @@ __global__ __launch_bounds__(kThreads, 2) void paged_importance_step_kernel(cons
         float sum[NT * 4];
 #pragma unroll
         for (int i = 0; i < NT * 4; ++i) sum[i] = 0.f;
-        uint32_t *meta = smeta[wave];
+        float *meta = smeta[wave];
+        Nibbles nb;
+        nb.init();
         int b = 0, k = 0;     // the pair that is next
         auto consume = [&](Keys &keys) {
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int i = 0; i < NT; ++i) meta[i * MT + (lane & (MT - 1))] = keys.m[i];
+            for (int i = 0; i < NT; ++i) put_k_meta<NG>(meta + i * 2 * MT, lane & (MT - 1), keys.m[i]);
             __builtin_amdgcn_wave_barrier();
             const unsigned char *at = qs + k * paged_query_bytes(D, NG);
             const float *f = (const float *)(at + NS * 1024);
@@ -900,7 +938,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_importance_step_kernel(cons
             const bool clean = mine == ALL && __builtin_amdgcn_ballot_w64(tok + NT * 16 <= see || !live) == ~0ull;
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
-                const f4 x = tile_scores<D, NG>(Q, keys.kc[i], meta + i * MT);
+                const f4 x = tile_scores<D, NG>(Q, nb, keys.kc[i], meta + i * 2 * MT);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], Q.kx, bias));
@@ -961,7 +999,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_importance_step_kernel(cons
 }
 
 namespace {
-int attn_lds(const PagedAttnParams &p) { return 2 * kWaves * p.rows * (p.D + 4) * 4 + kWaves * 2 * 128 * p.ng; }
+int attn_lds(const PagedAttnParams &p) { return 2 * kWaves * p.rows * (p.D + 4) * 4 + kWaves * 2 * 192 * p.ng; }
 constexpr int64_t kSumsBytes = 2048;  // Scan::pre at the start of the workspace
 static_assert((kThreads + 1) * 4 <= kSumsBytes, "the sums fit");
 }  // namespace

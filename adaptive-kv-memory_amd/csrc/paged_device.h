@@ -9,6 +9,26 @@ namespace {
 
 constexpr float kMinMax = -0x1p126f;  // a finite start of the running maximum: a row that sees nothing stays at p = 0
 
+// Masks of the two nibbles of a byte in both halves of a dword, in registers (so that mask and
+// exponent are one v_and_or_b32), and a pair of codes less MID as float16: under the exponent of
+// 1024 the low nibble reads as 1024 + c, under that of 64 the high one as 64 + c.
+struct Nibbles {
+    uint32_t lo, hi;
+    __device__ __forceinline__ void init() {
+        lo = 0x000F000Fu;
+        hi = 0x00F000F0u;
+        asm volatile("" : "+v"(lo), "+v"(hi));
+    }
+    template <int MID = 0>
+    __device__ __forceinline__ h2 low(uint32_t w) const {
+        return as_h2((w & lo) | 0x64006400u) - (h2){(_Float16)(1024.f + MID), (_Float16)(1024.f + MID)};
+    }
+    template <int MID = 0>
+    __device__ __forceinline__ h2 high(uint32_t w) const {
+        return as_h2((w & hi) | 0x54005400u) - (h2){(_Float16)(64.f + MID), (_Float16)(64.f + MID)};
+    }
+};
+
 // 1 / sum of a row's p; 0 for a row that sees nothing (and NaN stays).
 __device__ __forceinline__ float row_inverse(float l) { return l > 0.0f || l != l ? 1.0f / l : 0.0f; }
 // log of the sum of exp, from the maximum (log2 domain) and the sum of p times 2^bias.

@@ -5,11 +5,12 @@
 // cached head, each wave 32 of them as the columns of 32x32x16 MFMAs, and walks the cache in
 // steps of 64 tokens, two buffers in LDS: while the MFMAs read one step, the next step's tiles
 // are in flight to registers, one wave a tile and side, and are then dequantized into the
-// other buffer, once for all rows.  Keys and values become float16 c s + z, p is rounded to
-// float16 too (a float16 output is off by about 3e-4 of its norm, where its own rounding is
-// 2e-4); scores, running maximum and sum are float32.  Where the rows' log-sums are asked for,
-// which are float32, keys enter as two float16 that add up to them (TWO: 1.63 ms where one
-// takes 1.29, eight chunks of 512 tokens on 64 heads over 8 after 8k).
+// other buffer, once for all rows.  Keys and values become float16 c s + z and p is rounded to
+// float16, which bfloat16 outputs do not feel (1.75e-3 of the norm, 1.68e-3 their own rounding).
+// For float16 outputs keys and p (PTWO) are two float16 that add up to them (2.8e-4, 2.0e-4 their
+// own; with one of each 3.5e-4 to 5e-4), keys also (TWO) where the rows' log-sums are asked for,
+// which are float32.  Scores, running maximum and sum are float32.  Eight chunks of 512 tokens on 64
+// heads over 8 after 8k: bfloat16 1.28 ms, with log-sums 1.57, float16 2.1.
 //   K  [64 tokens][D / 8 chunks] of 16 bytes, chunk c at place c ^ turn(token) of its row;
 //   V  the PV operand: [tile][32 channels][lane] of 16 bytes, tokens 4 hi + 0..3, 8 + 4 hi + 0..3;
 //      row 16 b + r of its MFMA is channel 2 r + b of the 32.
@@ -104,23 +105,6 @@ __device__ __forceinline__ int64_t tile_share(const PagedAttnParams &p, int64_t 
 // in all three.
 __device__ __forceinline__ int turn(int token) { return (token & 1) << 2 | (token & 2) | (token >> 2 & 1); }
 
-// Masks of the two nibbles of a byte in both halves of a dword, in registers (so that mask and
-// exponent are one v_and_or_b32), and a pair of codes as float16: under the exponent of 1024
-// the low nibble reads as 1024 + c, under that of 64 the high one as 64 + c.
-struct Nibbles {
-    uint32_t lo, hi;
-    __device__ __forceinline__ void init() {
-        lo = 0x000F000Fu;
-        hi = 0x00F000F0u;
-        asm volatile("" : "+v"(lo), "+v"(hi));
-    }
-    __device__ __forceinline__ h2 low(uint32_t w) const {
-        return as_h2((w & lo) | 0x64006400u) - (h2){(_Float16)1024.f, (_Float16)1024.f};
-    }
-    __device__ __forceinline__ h2 high(uint32_t w) const {
-        return as_h2((w & hi) | 0x54005400u) - (h2){(_Float16)64.f, (_Float16)64.f};
-    }
-};
 // The four pairs of a dword of codes (nibbles n and n + 4 of it) as c s + z.
 __device__ __forceinline__ void dequant8(const Nibbles &nb, uint32_t w, h2 s, h2 z, uint32_t *o) {
     const uint32_t v = w >> 8;

@@ -380,3 +380,39 @@ def test_pages_past_32_bits_of_bytes():
         res.append([o, l, o1, l1, imp, *akv.paged_read(pool, batch)])
     assert all(torch.equal(a, b) for a, b in zip(*res))
     assert torch.equal(big.data[:, shift:], w.pool.data) and not bool(big.data[:, :shift:997].any())
+
+
+@pytest.mark.parametrize("kv,n,H,g,D,G", [(60000, 1, 2, 2, 128, 64), (30000, 4, 1, 7, 128, 128), (20000, 2, 2, 1, 64, 32), (120, 2, 4, 4, 128, 128),
+                                          (50, 1, 1, 2, 128, 128), (85, 1, 1, 1, 128, 32), (20000, 80, 1, 1, 128, 32), (400, 100, 2, 3, 64, 64)])
+def test_precision(kv, n, H, g, D, G):
+    """How far outputs and log-sums are off, by the norm.  Rounding to float16 alone leaves at most
+    2^-10 / sqrt(12) = 0.58 2^-11 of it, and the kernel's own part must stay below 0.47 2^-11 (then both
+    are below 0.75 2^-11 together); bfloat16 likewise with 2^-8.  Log-sums are float32: sums and
+    scores of up to 64 in steps of 2^-19 of log2 leave 2^-20 of theirs."""
+    import akv
+    announce(f"paged attention, precision at kv={kv} rows={n} H={H} g={g} D={D} G={G}")
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(kv)
+    pages = -(-kv // 16)
+    pool = akv.PagedPool.empty(1, pages, H, D, 16, G)
+    table = torch.randperm(pages, generator=gen, device="cuda").to(torch.int32).view(1, -1)
+    one = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    whole = akv.PagedBatch(table, one(kv), one(0, kv), kv, kv)
+    k, v = torch.randn(2, kv, H, D, generator=gen, device="cuda")
+    k[..., 3] *= 10.0
+    akv.paged_append(pool, whole, k, v)
+    k, v = (x.double().repeat_interleave(g, 1) for x in akv.paged_read(pool, whole, 0, torch.float32))
+    batch = akv.PagedBatch(table, one(kv), one(0, n), n, n)
+    see = torch.ones(n, kv, dtype=torch.bool, device="cuda").tril(kv - n)
+    for dt, half in ((torch.float16, 2.0 ** -11), (torch.bfloat16, 2.0 ** -8)):
+        q = torch.randn(n, H * g, D, generator=gen, device="cuda").to(dt)
+        x = torch.stack([(q[:, h].double() @ k[:, h].T) * D ** -0.5 for h in range(H * g)])
+        x = x.masked_fill(~see, -torch.inf)
+        el = torch.logsumexp(x, -1)
+        eo = torch.stack([torch.exp(x[h] - el[h, :, None]) @ v[:, h] for h in range(H * g)], 1)
+        for want_lse in (True, False):
+            o = akv.paged_attention(q, pool, batch, return_lse=want_lse)
+            if want_lse:
+                o, lse = o
+                assert float((lse.double() - el.T).norm() / el.norm()) < 2.0 ** -20
+            assert float((o.double() - eo).norm() / eo.norm()) < 0.75 * half
