@@ -432,7 +432,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
             l += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
             // float16 outputs: p, and p s below, as two float16 that add up to it: one alone would cost
             // them half a step (measured 3.5e-4 of the output's norm; 2.1e-4 is its own rounding).
-            // Beside bfloat16's own 1.7e-3 one is as good.
+            // Beside bfloat16's own 1.7e-3 one is as good, and so are the codes as they are.
             h2 ph[4], pl[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -1048,7 +1048,11 @@ hipError_t paged_attn_launch(const PagedAttnParams &p0, hipStream_t st) {
             else go(paged_decode_kernel<64, 1, TWO>);
         }
     };
-    if (p.q_bf16) by_form(std::false_type{});
+    // bfloat16 outputs take the shorter form while tables hold up to 128k tokens: its values' codes are
+    // of one sign, and what the matrix cores cut off grows with the context (errors of 1.78e-3, 2.2e-3
+    // and 2.8e-3 of the norm at 60000, 250000 and a million tokens, 1.7e-3 of it bfloat16's own; the
+    // longer form stays there).
+    if (p.q_bf16 && ((int64_t)p.seqs.width << (p.pool.log_tpp + 4)) <= 131072) by_form(std::false_type{});
     else by_form(std::true_type{});
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;

@@ -383,12 +383,13 @@ def test_pages_past_32_bits_of_bytes():
 
 
 @pytest.mark.parametrize("kv,n,H,g,D,G", [(60000, 1, 2, 2, 128, 64), (30000, 4, 1, 7, 128, 128), (20000, 2, 2, 1, 64, 32), (120, 2, 4, 4, 128, 128),
-                                          (50, 1, 1, 2, 128, 128), (85, 1, 1, 1, 128, 32), (20000, 80, 1, 1, 128, 32), (400, 100, 2, 3, 64, 64)])
+                                          (50, 1, 1, 2, 128, 128), (85, 1, 1, 1, 128, 32), (20000, 80, 1, 1, 128, 32), (400, 100, 2, 3, 64, 64), (700001, 1, 1, 4, 128, 32)])
 def test_precision(kv, n, H, g, D, G):
     """How far outputs and log-sums are off, by the norm.  Rounding to float16 alone leaves at most
     2^-10 / sqrt(12) = 0.58 2^-11 of it, and the kernel's own part must stay below 0.47 2^-11 (then both
-    are below 0.75 2^-11 together); bfloat16 likewise with 2^-8.  Log-sums are float32: sums and
-    scores of up to 64 in steps of 2^-19 of log2 leave 2^-20 of theirs."""
+    are below 0.75 2^-11 together); bfloat16 likewise with 2^-8, its own part below 0.15 2^-8 (0.6
+    together).  Log-sums are float32: sums and scores of up to 64 in steps of 2^-19 of log2 leave
+    2^-20 of theirs."""
     import akv
     announce(f"paged attention, precision at kv={kv} rows={n} H={H} g={g} D={D} G={G}")
     gen = torch.Generator(device="cuda")
@@ -415,4 +416,4 @@ def test_precision(kv, n, H, g, D, G):
             if want_lse:
                 o, lse = o
                 assert float((lse.double() - el.T).norm() / el.norm()) < 2.0 ** -20
-            assert float((o.double() - eo).norm() / eo.norm()) < 0.75 * half
+            assert float((o.double() - eo).norm() / eo.norm()) < (0.75 if dt == torch.float16 else 0.6) * half
