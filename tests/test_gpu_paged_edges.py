@@ -417,3 +417,38 @@ def test_precision(kv, n, H, g, D, G):
                 o, lse = o
                 assert float((lse.double() - el.T).norm() / el.norm()) < 2.0 ** -20
             assert float((o.double() - eo).norm() / eo.norm()) < (0.75 if dt == torch.float16 else 0.6) * half
+
+
+@pytest.mark.parametrize("D,G,P", FORMS)
+@pytest.mark.parametrize("size", [1e-6, 3e-3, 3e4])
+def test_attention_over_values_of_any_size(size, D, G, P):
+    """Caches of values at the clamp, of float16's smallest, and of groups of one value (scale 0)."""
+    import akv
+    announce(f"paged attention D={D} G={G} over values of {size}")
+    w = World(D, G, P, 2, [200, 90, 300], [3, 1, 90])
+    rng = np.random.default_rng(7)
+    for s, n in enumerate(w.kv):
+        k, v = rng.standard_normal((2, n, 2, D)) * size
+        k[:, 0, :G] = k[:, 0, :1]           # one value: scale 0
+        v[5::7, 1, D - G:] = 0.0
+        if size > 1:
+            v[3::5, 0, 1], v[4::5, 0, 2] = 1e9, -1e9    # clamped: a range of 122880
+            k[2::3, 1, 7] = 61440.0
+        w.ref.write(0, w.table[s], np.arange(n), k, v)
+    w.pool.data.copy_(torch.from_numpy(w.ref.data))
+    scale = D ** -0.5 / size
+    for dt in ("fp16", "bf16"):
+        q = _x((w.T, 8, D), 3, dt)
+        half = torch.finfo(q.dtype).eps / 2
+        for want in (True, False):
+            out = akv.paged_attention(q, w.pool, w.batch, sm_scale=scale, return_lse=want)
+            out, lse = out if want else (out, None)
+            for s, (n, m) in enumerate(zip(w.kv, w.q)):
+                kp, vp = w.ref.parts(0, w.table[s], np.arange(n))
+                r = w.rows(s)
+                eo, el, bo, bl = ref.attention(q[r].double().cpu().numpy(), kp, vp, scale, np.arange(n - m, n) + 1, half,
+                                               rounded=not want and m * 4 > 64)
+                # float16's smallest step, for values and outputs below its normal range
+                assert (np.abs(out[r].double().cpu().numpy() - eo) <= bo + 2.0 ** -24).all()
+                if want:
+                    assert (np.abs(lse[r].double().cpu().numpy() - el) <= bl).all()
