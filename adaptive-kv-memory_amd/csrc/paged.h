@@ -64,6 +64,7 @@ struct PagedAttnParams {
     int groups, tile_groups;   // workgroups of the two kernels
     int few_rows;              // the tile kernel takes sequences of more rows
     int rows;                  // most rows of an item
+    int whole;                 // > 0: every item counts this many units and is a workgroup's
 };
 
 struct PagedImportanceParams {

@@ -173,7 +173,7 @@ __device__ __forceinline__ SeqWork seq_work(const PagedAttnParams &p, const SeqR
     w.rows = min(r.n, p.seqs.max_q) * p.g;
     w.chunks = w.rows <= kFewRows ? (w.rows + kRows - 1) / kRows : 0;  // more rows are paged_tile_kernel's
     w.units = max(1, (r.kv + (kUnitTok - 1)) / kUnitTok);
-    w.cost = w.units + kSetup;
+    w.cost = p.whole ? p.whole : w.units + kSetup;
     return w;
 }
 __device__ __forceinline__ int seq_total(const PagedAttnParams &p, const SeqWork &w) { return w.chunks * w.cost * p.pool.heads; }
@@ -266,8 +266,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
     const int per = (p.seqs.n_seqs + kThreads - 1) / kThreads;
     scan_seqs(p, sc, per);
     const int total = __builtin_amdgcn_readfirstlane(sc.pre[kThreads]);
-    const int share = share_of(total, p.groups);
-    if (blockIdx.x == 0) {  // for the merge
+    const int share = p.whole ? p.whole / kWaves : share_of(total, p.groups);
+    if (blockIdx.x == 0 && !p.whole) {  // for the merge
         p.sums[threadIdx.x] = sc.pre[threadIdx.x];
         if (threadIdx.x == 0) p.sums[kThreads] = total;
     }
@@ -1017,6 +1017,16 @@ int64_t paged_attn_plan(PagedAttnParams *p) {
     p->groups = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxGroups, (most + kWaves - 1) / kWaves));
     // where every sequence has the most rows there is none of few, and if there is the tiles take it
     if (r > kFewRows && p->seqs.n_tokens == (int64_t)p->seqs.n_seqs * p->seqs.max_q) p->groups = 0;
+    // Short contexts and few of them: an item a workgroup, whatever its length, and nothing to merge
+    // (the workspace is not used).  Against runs of equal work, us for 128, 256, 384 and 512 tokens: one
+    // sequence of 8 heads: 10.1, 11.7, 13.3, 14.7 and 12.1, 12.1, 12.3, 12.5; for 512, 1024 and 2048, 32
+    // sequences, which fill the card: 15.6, 22.1, 34.0 and 19.4, 25.1, 34.3.
+    const int64_t items = (int64_t)p->seqs.n_seqs * p->pool.heads * few_chunks(*p);
+    if (r <= kFewRows && items <= kMaxGroups && units <= (items >= kMaxGroups / 2 ? 32 : 8)) {
+        p->whole = (int)((units + kSetup + kWaves - 1) / kWaves * kWaves);
+        p->groups = (int)std::max<int64_t>(1, items);
+        return kSumsBytes;
+    }
     const int64_t own = p->groups ? kSumsBytes + (int64_t)p->groups * 2 * p->rows * (p->D + 4) * 4 : 0;
     p->tile_part = p->part + own / 4;
     return own + paged_tile_plan(p);
@@ -1030,8 +1040,10 @@ hipError_t paged_attn_launch(const PagedAttnParams &p0, hipStream_t st) {
         const hipError_t e = paged_tile_launch(p, st);
         if (e != hipSuccess || !p.groups) return e;
     }
-    p.sums = (int *)p.part;
-    p.part += kSumsBytes / 4;
+    if (!p.whole) {
+        p.sums = (int *)p.part;
+        p.part += kSumsBytes / 4;
+    }
     const size_t lds = attn_lds(p);
     auto go = [&](auto kern) {
         if (lds > 48 * 1024) (void)hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -1055,7 +1067,7 @@ hipError_t paged_attn_launch(const PagedAttnParams &p0, hipStream_t st) {
     if (p.q_bf16 && ((int64_t)p.seqs.width << (p.pool.log_tpp + 4)) <= 131072) by_form(std::false_type{});
     else by_form(std::true_type{});
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    if (e != hipSuccess || p.whole) return e;
     const dim3 grid(p.pool.heads * few_chunks(p), p.seqs.n_seqs);
     if (p.D == 128) paged_merge_kernel<128><<<grid, dim3(kThreads), 0, st>>>(p);
     else paged_merge_kernel<64><<<grid, dim3(kThreads), 0, st>>>(p);

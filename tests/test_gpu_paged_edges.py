@@ -452,3 +452,18 @@ def test_attention_over_values_of_any_size(size, D, G, P):
                 assert (np.abs(out[r].double().cpu().numpy() - eo) <= bo + 2.0 ** -24).all()
                 if want:
                     assert (np.abs(lse[r].double().cpu().numpy() - el) <= bl).all()
+
+
+@pytest.mark.parametrize("Hq,H,kv,q", [(4, 2, [256, 1, 0, 130], [1, 1, 0, 1]), (8, 1, [64, 33], [8, 5]), (2, 1, [1], [1]), (12, 4, [17, 240, 90], [16, 3, 1]),
+                                       (4, 4, [1000] + [37 * i % 1024 for i in range(69)], [2] + [i % 2 for i in range(69)])])
+def test_attention_of_short_contexts(Hq, H, kv, q):
+    """An item a workgroup: fewer units than waves, sequences far shorter than the longest, idle ones,
+    chunks of 16 rows beside single ones, and many sequences of up to a thousand tokens."""
+    announce(f"paged attention of short contexts Hq={Hq} H={H} kv={kv[:4]} rows={q[:4]}")
+    for D, G in ((128, 32), (64, 64)):
+        q = [min(m, n) for m, n in zip(q, kv)]
+        w = World(D, G, 16, H, kv, q, spare=1)
+        w.fill()
+        for dt in ("fp16", "bf16"):
+            _check_attention(w, Hq, dt, True)
+            _check_attention(w, Hq, dt, False)
