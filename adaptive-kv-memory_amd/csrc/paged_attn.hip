@@ -6,8 +6,9 @@
 // rows are scaled to a maximum in [2^13, 2^14), which leaves with the softmax scale.  Scores are
 // thus exact to float32 rounding, whatever the cache's widths.  Values: o = sum of p (c s + z) is the
 // product of the codes with p s plus sum of p z, one more MFMA row per channel group; p and p s enter
-// as two float16 each, for bfloat16 outputs as one.  Softmax state: running maximum and sum per row in
-// float32.
+// as two float16 each, for bfloat16 outputs as one.  Both lie high in float16's range (kFewBias), so
+// that light tokens keep their part beside one that has nearly all of a row's weight.  Softmax
+// state: running maximum and sum per row in float32.
 #include <algorithm>
 #include <type_traits>
 
@@ -24,6 +25,13 @@ constexpr int kImpBlocks = 4;         // most runs of a wave in a decode step's
 constexpr int kImpHeads = 3;          // most heads of a wave there
 // LDS of one head's query operand of 16 rows, its groups' sums, factor and log-sum.
 __host__ __device__ constexpr int paged_query_bytes(int D, int ng) { return 32 * D + 64 * (ng + 2); }
+// The few-rows kernel holds p times 2^14, in (0, 2^14], and V scales over a power of two that they stay
+// below (at kHighExp below twice it: the append's largest is 2^13): p times a scale keeps 11 bits down
+// to 2^-28 of the largest, and something down to 2^-38.  (With p in (0, 4] and scales as they are, a
+// token of 0.999 of the weight and a value near 0 took 2e-3 to 1e-1 of an output with it, by the size
+// of the values and the length of a wave's run.)
+constexpr float kFewBias = 14.0f;
+constexpr int kLowExp = -12, kHighExp = 12;  // of that power, which goes in steps of 2^4: 2^12 and 7 2^12 are float16
 constexpr int kMaxGroups = 512;       // two workgroups a compute unit: what registers allow at head_dim 128
 
 __device__ __forceinline__ float xmax(float x) {
@@ -229,7 +237,7 @@ __device__ __forceinline__ void write_row(const PagedAttnParams &p, const SeqRow
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = to_pair(p.q_bf16, o[2 * i] * inv, o[2 * i + 1] * inv);
     *(u4 *)((unsigned char *)p.out + ((t * p.Hq + head) * p.D + ch) * 2) = w;
-    if (p.lse && ch == 0) p.lse[t * p.Hq + head] = row_lse(m, l, 2.0f);  // p is held times 4
+    if (p.lse && ch == 0) p.lse[t * p.Hq + head] = row_lse(m, l, kFewBias);
 }
 
 }  // namespace
@@ -361,6 +369,13 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
         f4 acc[NB], accz = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int b = 0; b < NB; ++b) acc[b] = (f4){0.f, 0.f, 0.f, 0.f};
+        // V scales enter over 2^vexp, which they stay below, and acc holds sums over it: raised like the
+        // running maximum, in steps of 2^4, so that caches of one kind of values raise it once
+        typedef uint16_t s2 __attribute__((ext_vector_type(2)));
+        constexpr uint64_t kScaleLanes = NG == 1 ? 0x00ff000000ff0000u : 0x0000ffff00000000u;  // whose meta is V scales
+        int vexp = kLowExp;
+        h2 down = {1.0f, 1.0f};  // 2^-vexp in those lanes
+        if (kScaleLanes >> lane & 1) down = (h2){(_Float16)0x1p12f, (_Float16)0x1p12f};
 
         auto work = [&](const Query<D, NG> &Q, Unit &u, int j, auto is_clean) {
             constexpr bool clean = decltype(is_clean)::value;
@@ -389,14 +404,14 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                // K scales and zeros as float32, then the V half as it is
+                // K scales and zeros as float32, then V scales over 2^vexp and V zeros as they are
                 uint32_t *m = meta + i * 48 * NG;
 #pragma unroll
                 for (int q = 0; q < MW; ++q) {
                     const int d = (lane & (32 * NG / MW - 1)) * MW + q;
                     const uint32_t w = u.m[i][q];
                     const float ks = lo_f(w), kz = __builtin_fmaf(ks, (float)kMid, hi_f(w));
-                    m[16 * NG + d] = d < 16 * NG ? __builtin_bit_cast(uint32_t, kz) : w;
+                    m[16 * NG + d] = d < 16 * NG ? __builtin_bit_cast(uint32_t, kz) : as_u32(as_h2(w) * down);
                     if (d < 16 * NG) m[d] = __builtin_bit_cast(uint32_t, ks);
                 }
             }
@@ -415,24 +430,54 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
             float t = sc[0][0];
 #pragma unroll
             for (int e = 1; e < 8; ++e) t = __builtin_fmaxf(t, sc[e >> 2][e & 3]);
-            if (__builtin_amdgcn_ballot_w64(t > mx)) {
-                const float mn = __builtin_fmaxf(mx, xmax(t));
+            s2 most = __builtin_elementwise_max(__builtin_bit_cast(s2, u.m[0][0]), __builtin_bit_cast(s2, u.m[1][0]));
+            if constexpr (MW == 2)
+                most = __builtin_elementwise_max(most, __builtin_elementwise_max(__builtin_bit_cast(s2, u.m[0][MW - 1]), __builtin_bit_cast(s2, u.m[1][MW - 1])));
+            const uint16_t below = (uint16_t)((vexp < kHighExp ? (vexp + 15) << 10 : 0x7c00) - 1);  // the largest float16 below 2^vexp
+            const uint64_t over = kScaleLanes & __builtin_amdgcn_ballot_w64(
+                __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(most, (s2){below, below})) != 0);
+            if (__builtin_amdgcn_ballot_w64(t + (kFewBias - mx) > kFewBias) | over) {
+                float to_new = 1.0f;  // from the old power to the new one
+                if (over) {
+                    s2 fin = {0, 0};  // the scales, without those that are not finite
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int q = 0; q < MW; ++q)
+                            fin = __builtin_elementwise_max(fin, __builtin_bit_cast(s2, u.m[i][q] & ~not_finite(u.m[i][q]) & 0x7fff7fffu));
+                    const int top = max(fin[0], fin[1]), was = vexp;
+                    while (vexp < kHighExp && __builtin_amdgcn_ballot_w64(top >= (vexp + 15) << 10) & kScaleLanes) vexp += 4;
+                    if (vexp != was) {
+                        to_new = __builtin_ldexpf(1.0f, was - vexp);
+                        const _Float16 x = (_Float16)__builtin_ldexpf(1.0f, -vexp);
+                        if (kScaleLanes >> lane & 1) {
+                            down = (h2){x, x};
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                                for (int q = 0; q < MW; ++q)
+                                    meta[i * 48 * NG + 16 * NG + (lane & (32 * NG / MW - 1)) * MW + q] = as_u32(as_h2(u.m[i][q]) * down);
+                        }
+                        __builtin_amdgcn_wave_barrier();
+                    }
+                }
+                const float most_t = xmax(t);
+                const float mn = most_t > mx ? running_max(most_t, kFewBias) : mx;
                 const float alpha = __builtin_amdgcn_exp2f(mx - mn);
                 l *= alpha;
 #pragma unroll
-                for (int b = 0; b < NB; ++b) acc[b] *= alpha;
+                for (int b = 0; b < NB; ++b) acc[b] *= alpha * to_new;
                 accz *= alpha;
                 mx = mn;
             }
-            // p in (0, 4]: p s stays in float16 for every scale that the append writes
-            const float bias = 2.0f - mx;
+            const float bias = kFewBias - mx;
             float pr[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) pr[e] = __builtin_amdgcn_exp2f(sc[e >> 2][e & 3] + bias);
             l += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
             // float16 outputs: p, and p s below, as two float16 that add up to it: one alone would cost
             // them half a step (measured 3.5e-4 of the output's norm; 2.1e-4 is its own rounding).
-            // Beside bfloat16's own 1.7e-3 one is as good, and so are the codes as they are.
+            // Beside bfloat16's own 1.7e-3 one is as good (2^-12 of each weight, an eighth of its half step).
             h2 ph[4], pl[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -462,14 +507,13 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
                     for (int q = 0; q < 4; ++q) {
                         const uint32_t v = u.vc[q >> 1][(q & 1) * (NB / 4) + h4];
                         const uint32_t x = n >= 2 ? v >> 8 : v;
-                        if constexpr (TWO) a[q] = as_u32(n & 1 ? nb.high<kMid>(x) : nb.low<kMid>(x));
-                        else a[q] = x & (n & 1 ? 0x00F000F0u : 0x000F000Fu);  // subnormals: c 2^-24, 16 c 2^-24
+                        a[q] = as_u32(n & 1 ? nb.high<kMid>(x) : nb.low<kMid>(x));
                     }
                     acc[b] = mfma_k32(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, pw), acc[b]);
                     if constexpr (TWO) acc[b] = mfma_k32(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, rw), acc[b]);
                 }
             }
-            // row g of the operand: the tokens' zeros of group g (of the centred codes: two float16)
+            // row g of the operand: the tokens' zeros of group g, z + 7 s (two float16, or one as p is)
             u4 za = {0u, 0u, 0u, 0u}, zl = {0u, 0u, 0u, 0u};
             if (col < NG) {
                 const uint32_t *at = meta + 32 * NG + (grp * NG + col) * 2;
@@ -478,12 +522,15 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
                     const u2 zw = *(const u2 *)(at + i * 48 * NG + 8 * NG), sw = *(const u2 *)(at + i * 48 * NG);
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
-                        za[2 * i + q] = zw[q];
                         if constexpr (TWO) {
-                            const float x = __builtin_fmaf(lo_f(sw[q]), (float)kMid, lo_f(zw[q])), y = __builtin_fmaf(hi_f(sw[q]), (float)kMid, hi_f(zw[q]));
+                            const float mid = __builtin_ldexpf((float)kMid, vexp);
+                            const float x = __builtin_fmaf(lo_f(sw[q]), mid, lo_f(zw[q])), y = __builtin_fmaf(hi_f(sw[q]), mid, hi_f(zw[q]));
                             const h2 h = {(_Float16)x, (_Float16)y};
                             za[2 * i + q] = as_u32(h);
                             zl[2 * i + q] = as_u32((h2){(_Float16)(x - (float)h[0]), (_Float16)(y - (float)h[1])});
+                        } else {
+                            const _Float16 mid = (_Float16)__builtin_ldexpf((float)kMid, vexp);
+                            za[2 * i + q] = as_u32(__builtin_elementwise_fma(as_h2(sw[q]), (h2){mid, mid}, as_h2(zw[q])));
                         }
                     }
                 }
@@ -518,7 +565,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
         }
         if (j < jn) consume(Q, U[0], j);
 
-        // the segment's state in true units (of subnormal codes 2^24, or 2^20 where they lay a nibble higher)
+        // the segment's state in true units
+        const float scale = __builtin_ldexpf(1.0f, vexp);
         l = xsum(l);
         float z[NG];
 #pragma unroll
@@ -534,8 +582,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
             float o[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                o[2 * i] = __builtin_fmaf(acc[2 * g][i], TWO ? 1.f : 0x1p24f, z[g * NG / NS]);
-                o[2 * i + 1] = __builtin_fmaf(acc[2 * g + 1][i], TWO ? 1.f : 0x1p20f, z[g * NG / NS]);
+                o[2 * i] = __builtin_fmaf(acc[2 * g][i], scale, z[g * NG / NS]);
+                o[2 * i + 1] = __builtin_fmaf(acc[2 * g + 1][i], scale, z[g * NG / NS]);
             }
             const int ch = 32 * g + 8 * grp;
             if (col < rows) {
@@ -1060,11 +1108,7 @@ hipError_t paged_attn_launch(const PagedAttnParams &p0, hipStream_t st) {
             else go(paged_decode_kernel<64, 1, TWO>);
         }
     };
-    // bfloat16 outputs take the shorter form while tables hold up to 128k tokens: its values' codes are
-    // of one sign, and what the matrix cores cut off grows with the context (errors of 1.78e-3, 2.2e-3
-    // and 2.8e-3 of the norm at 60000, 250000 and a million tokens, 1.7e-3 of it bfloat16's own; the
-    // longer form stays there).
-    if (p.q_bf16 && ((int64_t)p.seqs.width << (p.pool.log_tpp + 4)) <= 131072) by_form(std::false_type{});
+    if (p.q_bf16) by_form(std::false_type{});
     else by_form(std::true_type{});
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.whole) return e;
