@@ -462,7 +462,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
                     }
                 }
                 const float most_t = xmax(t);
-                const float mn = most_t > mx ? running_max(most_t, kFewBias) : mx;
+                const float mn = most_t > mx ? running_max(most_t, 1.0f, kFewBias) : mx;
                 const float alpha = __builtin_amdgcn_exp2f(mx - mn);
                 l *= alpha;
 #pragma unroll

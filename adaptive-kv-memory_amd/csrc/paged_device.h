@@ -29,11 +29,12 @@ struct Nibbles {
     }
 };
 
-// The running maximum of a row whose largest score is `top`, p being 2^(score + (bias - maximum)): the
-// next float above it where that exponent rounds to more than the bias, which scores past 2^23 let it,
-// so that p never leaves float16.
-__device__ __forceinline__ float running_max(float top, float bias) {
-    return top + (bias - top) > bias ? __builtin_fmaf(__builtin_fabsf(top), 0x1.8p-24f, top) : top;
+// The running maximum of a row whose largest score is top * kx, p being 2^(score * kx + (bias - maximum)):
+// the next float above it where that exponent rounds to more than the bias, which scores past 2^23 let
+// it, so that p never leaves float16.
+__device__ __forceinline__ float running_max(float top, float kx, float bias) {
+    const float m = top * kx;
+    return __builtin_fmaf(top, kx, bias - m) > bias ? __builtin_fmaf(__builtin_fabsf(m), 0x1.8p-24f, m) : m;
 }
 // 1 / sum of a row's p; 0 for a row that sees nothing (and NaN stays).
 __device__ __forceinline__ float row_inverse(float l) { return l > 0.0f || l != l ? 1.0f / l : 0.0f; }

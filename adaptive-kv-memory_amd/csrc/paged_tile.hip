@@ -5,12 +5,16 @@
 // cached head, each wave 32 of them as the columns of 32x32x16 MFMAs, and walks the cache in
 // steps of 64 tokens, two buffers in LDS: while the MFMAs read one step, the next step's tiles
 // are in flight to registers, one wave a tile and side, and are then dequantized into the
-// other buffer, once for all rows.  Keys and values become float16 c s + z and p is rounded to
-// float16, which bfloat16 outputs do not feel (1.75e-3 of the norm, 1.68e-3 their own rounding).
-// For float16 outputs keys and p (PTWO) are two float16 that add up to them (2.8e-4, 2.0e-4 their
-// own; with one of each 3.5e-4 to 5e-4), keys also (TWO) where the rows' log-sums are asked for,
-// which are float32.  Scores, running maximum and sum are float32.  Eight chunks of 512 tokens on 64
-// heads over 8 after 8k: bfloat16 1.28 ms, with log-sums 1.57, float16 2.1.
+// other buffer, once for all rows.  Scores, running maximum and sum are float32; values become
+// float16 c s + z.  What else is rounded to float16 goes by the output, whose own rounding leaves 1.68e-3
+// (bfloat16) and 2.0e-4 (float16) of its norm:
+//   bfloat16  keys and p: 1.75e-3 to 1.95e-3 together; a rounded key moves its score by up to 2^-12 of it
+//   float16   nothing: keys and p (PTWO) are two float16 that add up to them: 2.8e-4 (with one of
+//             each 3.5e-4 to 5e-4)
+// Where the rows' log-sums are asked for, which are float32, keys are two float16 (TWO) for bfloat16 too.
+// Two always would make the outputs of both calls the same and cost a quarter of the time (three chunks
+// of 65 to 512 tokens on 64 heads after 2k to 32k: 715 us, with two 905).  Eight chunks of 512 tokens on
+// 64 heads over 8 after 8k: bfloat16 1.28 ms, with log-sums 1.57, float16 2.1.
 //   K  [64 tokens][D / 8 chunks] of 16 bytes, chunk c at place c ^ turn(token) of its row;
 //   V  the PV operand: [tile][32 channels][lane] of 16 bytes, tokens 4 hi + 0..3, 8 + 4 hi + 0..3;
 //      row 16 b + r of its MFMA is channel 2 r + b of the 32.
@@ -34,8 +38,11 @@ namespace {
 constexpr int kStep = 64;               // tokens a step: a tile for each wave of a group
 constexpr int kTileWaves = 8;
 constexpr int kSetupTok = 2 * kStep;    // what an entry's start counts
-constexpr float kLag = 8.0f;            // log2 units the running maximum may lag behind
-constexpr float kPBias = 7.0f;          // p is held times 2^7
+// p is held times 2^13, and the running maximum may lag behind by two log2 units: p in (0, 2^15] keeps 11
+// bits down to 2^-27 of the largest weight and something down to 2^-38.  (With 2^7 and a lag of eight, bfloat16
+// outputs were 3.6e-3 of the norm off where 65535 tokens share 1e-4 of the weight.)
+constexpr float kLag = 2.0f;
+constexpr float kPBias = 13.0f;
 
 typedef float f16v __attribute__((ext_vector_type(16)));
 
@@ -515,9 +522,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
                     float top = sc[0][0];
 #pragma unroll
                     for (int i = 1; i < 32; ++i) top = __builtin_fmaxf(top, sc[i >> 4][i & 15]);
-                    top *= kx;
-                    if (__builtin_amdgcn_ballot_w64(top > mx + kLag)) {
-                        const float mn = __builtin_fmaxf(mx, __builtin_fmaxf(top, __shfl_xor(top, 32)));
+                    if (__builtin_amdgcn_ballot_w64(__builtin_fmaf(top, kx, kPBias - mx) > kPBias + kLag)) {
+                        top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+                        const float mn = top * kx > mx ? running_max(top, kx, kPBias) : mx;
                         const float alpha = __builtin_amdgcn_exp2f(mx - mn);
                         l *= alpha;
 #pragma unroll
