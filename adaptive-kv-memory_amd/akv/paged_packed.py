@@ -140,23 +140,26 @@ class PagedBatch:
         self._workspace: dict = {}  # bytes an attention call needs, by the sizes they depend on
 
 
-def _rows(x: torch.Tensor, name: str, T: int, H: int, D: int) -> torch.Tensor:
-    """(T, H, D) with consecutive channels and rows on 16 bytes; copied if it is not."""
+def _rows(x: torch.Tensor, name: str, T: int, H: int, D: int) -> Tuple[torch.Tensor, int, int]:
+    """(T, H, D) with consecutive channels and rows on 16 bytes, copied if it is not, and the byte
+    strides of tokens and heads (those of a dimension of size 1 say nothing, to contiguous() either)."""
     if x.shape != (T, H, D):
         raise ValueError(f"{name} must be ({T}, {H}, {D}), got {tuple(x.shape)}")
     e = x.element_size()
-    st = x.stride()
-    if st[2] != 1 or (st[0] * e | st[1] * e | x.data_ptr()) & 15:
-        x = nat.dev_contig(x)
-    return x
+    st, sh, sc = x.stride()
+    if T <= 1:
+        st = H * D
+    if H <= 1:
+        sh = D
+    if sc != 1 or (st * e | sh * e | x.data_ptr()) & 15:
+        x, st, sh = nat.dev_contig(x), H * D, D
+    return x, st * e, sh * e
 
 
-def _rows_args(pool: PagedPool, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, layer: int) -> bytes:
-    e = k.element_size()
-    kt, kh, _ = k.stride()
-    vt, vh, _ = v.stride()
+def _rows_args(pool: PagedPool, batch: PagedBatch, k: tuple, v: tuple, layer: int) -> bytes:
+    (k, kt, kh), (v, vt, vh) = k, v
     return _ROWS.pack(nat.ABI_VERSION, layer, nat.dtype_code(k.dtype), 0, pool._c, batch._c, k.data_ptr(), v.data_ptr(),
-                      kt * e, kh * e, vt * e, vh * e)
+                      kt, kh, vt, vh)
 
 
 def paged_append(pool: PagedPool, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, layer: int = 0) -> None:
@@ -181,11 +184,13 @@ def paged_read(pool: PagedPool, batch: PagedBatch, layer: int = 0,
     _check_device(pool, batch.page_table)
     nat.dtype_code(dtype)
     k, v = torch.empty(2, batch.n_tokens, pool.heads, pool.head_dim, dtype=dtype, device=pool.data.device).unbind(0)
-    _call(pool._index, "paged_read", nat.load().akv_paged_read, _rows_args(pool, batch, k, v, layer))
+    sh = pool.head_dim * k.element_size()
+    st = pool.heads * sh
+    _call(pool._index, "paged_read", nat.load().akv_paged_read, _rows_args(pool, batch, (k, st, sh), (v, st, sh), layer))
     return k, v
 
 
-def _queries(q: torch.Tensor, pool: PagedPool, batch: PagedBatch) -> torch.Tensor:
+def _queries(q: torch.Tensor, pool: PagedPool, batch: PagedBatch) -> Tuple[torch.Tensor, int, int]:
     _check_device(pool, q, batch.page_table)
     if q.dtype not in _QUERY:
         raise TypeError("paged attention takes float16 or bfloat16 queries")
@@ -201,14 +206,13 @@ def paged_attention(q: torch.Tensor, pool: PagedPool, batch: PagedBatch, layer: 
     Query head h reads cached head h // (Hq // heads).  With ``causal``, row i of a sequence's
     m rows sees its first kv_len - m + 1 + i tokens, else all of them; a row that sees none is 0.
     ``return_lse`` adds log(sum(exp(sm_scale q.k))) (n_tokens, Hq) float32, -inf for such rows."""
-    q = _queries(q, pool, batch)
+    q, qt, qh = _queries(q, pool, batch)
     T, Hq, D = q.shape
     lib = nat.load()
     out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
     lse = torch.empty(T, Hq, dtype=torch.float32, device=q.device) if return_lse else None
-    qt, qh, _ = q.stride()
     head = (nat.ABI_VERSION, layer, Hq, nat.dtype_code(q.dtype), int(causal),
-            nat.default_sm_scale(D) if sm_scale is None else float(sm_scale), pool._c, batch._c, q.data_ptr(), qt * 2, qh * 2,
+            nat.default_sm_scale(D) if sm_scale is None else float(sm_scale), pool._c, batch._c, q.data_ptr(), qt, qh,
             out.data_ptr(), 0 if lse is None else lse.data_ptr())
     key = (D, pool.group_size, pool.heads, pool.page_size, Hq)
     need = batch._workspace.get(key)
@@ -231,7 +235,7 @@ def paged_importance(q: torch.Tensor, lse: torch.Tensor, pool: PagedPool, batch:
 
     q and lse are those of ``paged_attention``; ``q_window`` > 0 counts a sequence's last rows
     only.  Written in place, or to ``out``; returns what was written."""
-    q = _queries(q, pool, batch)
+    q, qt, qh = _queries(q, pool, batch)
     T, Hq, D = q.shape
     dst = scores if out is None else out
     _check_device(pool, lse, scores, dst)
@@ -244,10 +248,9 @@ def paged_importance(q: torch.Tensor, lse: torch.Tensor, pool: PagedPool, batch:
             raise ValueError("a sequence's scores must be consecutive")
     if not lse.is_contiguous():
         lse = lse.contiguous()
-    qt, qh, _ = q.stride()
     args = _IMPORTANCE.pack(nat.ABI_VERSION, layer, Hq, nat.dtype_code(q.dtype), int(causal), int(q_window),
                             nat.default_sm_scale(D) if sm_scale is None else float(sm_scale), float(decay), pool._c,
-                            batch._c, q.data_ptr(), qt * 2, qh * 2, lse.data_ptr(), scores.data_ptr(), dst.data_ptr(),
+                            batch._c, q.data_ptr(), qt, qh, lse.data_ptr(), scores.data_ptr(), dst.data_ptr(),
                             scores.shape[1], scores.stride(0), dst.stride(0))
     _call(pool._index, "paged_importance", nat.load().akv_paged_importance, args)
     return dst

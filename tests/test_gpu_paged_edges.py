@@ -467,3 +467,24 @@ def test_attention_of_short_contexts(Hq, H, kv, q):
         for dt in ("fp16", "bf16"):
             _check_attention(w, Hq, dt, True)
             _check_attention(w, Hq, dt, False)
+
+
+@pytest.mark.parametrize("T,H", [(1, 2), (1, 1), (3, 1), (3, 2)])
+def test_rows_of_a_padded_projection(T, H):
+    """Keys, values and queries sliced from rows whose stride is no multiple of 16 bytes: one token too."""
+    import akv
+    announce(f"paged calls on {T} rows of {H} heads, 8 bytes beside the alignment")
+    w = World(128, 32, 16, H, [40], [T])
+    w.fill()
+    D, g = 128, 2
+    wide = _x((T + 1, (2 + g) * H * D + 4), 3)[1:]
+    k, v, q = (t.unflatten(1, (-1, D)) for t in (wide[:, :H * D], wide[:, H * D:2 * H * D], wide[:, 2 * H * D:(2 + g) * H * D]))
+    akv.paged_append(w.pool, w.batch, k, v)
+    w.ref.write(0, w.table[0], np.arange(40 - T, 40), k.double().cpu().numpy(), v.double().cpu().numpy())
+    w.same_pool()
+    plain = torch.empty(T, g * H, D, dtype=q.dtype, device="cuda").copy_(q)
+    out, lse = akv.paged_attention(q, w.pool, w.batch, return_lse=True)
+    want, wl = akv.paged_attention(plain, w.pool, w.batch, return_lse=True)
+    assert torch.equal(out, want) and torch.equal(lse, wl)
+    zero = torch.zeros(1, 40, device="cuda")
+    assert torch.equal(akv.paged_importance(q, lse, w.pool, w.batch, zero.clone()), akv.paged_importance(plain, lse, w.pool, w.batch, zero.clone()))

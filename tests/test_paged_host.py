@@ -246,3 +246,21 @@ def test_host_tensors_are_refused():
         akv.PagedPool(torch.zeros(1, 2, 3, 4, 5, dtype=torch.uint8), 128)
     with pytest.raises(NotImplementedError):
         akv.PagedPool.empty(1, 4, 2, 128, page_size=40)
+
+
+def test_strides_of_single_rows_say_nothing():
+    """One token, or one head, of a tensor whose rows are padded: what stride its size-1 dimensions
+    have does not matter, whether the rows are copied or not."""
+    from akv.paged_packed import _rows
+    buf = torch.randn(5, 1028)
+    for T, H, x in ((1, 8, buf[:, :1024].unflatten(1, (8, 128))[2:3]), (3, 8, buf[:, :1024].unflatten(1, (8, 128))[1:4]),
+                    (5, 1, buf[:, :128].unflatten(1, (1, 128))), (1, 1, buf[3:4, 4:132].unflatten(1, (1, 128))),
+                    (1, 1, buf[3:4, 1:129].unflatten(1, (1, 128))), (0, 8, buf[:0, :1024].unflatten(1, (8, 128))),
+                    (1, 2, buf.t()[:256, 2:3].t().unflatten(1, (2, 128)))):
+        for dt in (torch.float16, torch.float32):
+            y = torch.empty_strided(x.shape, x.stride(), dtype=dt).copy_(x)
+            z, st, sh = _rows(y, "x", T, H, 128)
+            e = z.element_size()
+            assert st % 16 == 0 and sh % 16 == 0 and z.data_ptr() % 16 == 0
+            got = torch.as_strided(z, (T, H, 128), (st // e, sh // e, 1))
+            assert torch.equal(got, y)
