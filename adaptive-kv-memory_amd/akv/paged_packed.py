@@ -116,8 +116,8 @@ class PagedBatch:
     ``page_table[s, j // page_size]``.  kv_lens (S,) int32: cached tokens, those of this call
     among them.  q_starts (S + 1,) int32: sequence s owns rows ``q_starts[s]`` to
     ``q_starts[s + 1]`` of the call's (n_tokens, heads, head_dim) tensors; they are its newest
-    tokens.  n_tokens: the rows; max_q: no sequence has more of them.  What calls return for rows
-    that are no sequence's (those of a padded batch) is not defined.
+    tokens.  n_tokens: the rows; max_q: no sequence has more of them.  Rows that are no sequence's
+    (those of a padded batch) are read as 0; what the attention returns for them is not defined.
 
     The tensors are kept, not copied (other integer types and orders are): what they hold when
     the work runs counts.  n_tokens and max_q are fixed."""

@@ -474,7 +474,7 @@ constexpr int64_t kManyRows = 8192;
 template <template <int, int, int> class K>
 hipError_t rows_launch(const PagedRowsParams &p, hipStream_t s) {
     const int64_t rows = p.seqs.n_tokens * p.pool.heads;
-    if (rows == 0 || p.seqs.n_seqs == 0) return hipSuccess;
+    if (rows == 0) return hipSuccess;  // (rows of no sequence are read as 0)
     if (rows >= (int64_t)1 << 31) return hipErrorInvalidConfiguration;
     const bool many = rows >= kManyRows;
     const int64_t wave_rows = (256 / p.D) * (many ? 4 : 1);

@@ -483,7 +483,7 @@ typedef struct akv_paged_rows_args {
  * both, and reads back as NaN. */
 int akv_paged_append(const akv_paged_rows_args *args, void *stream);
 /* The values of the call's rows as the cache holds them (code * scale + zero, rounded to
- * dtype) into k and v; rows without a slot become 0. */
+ * dtype) into k and v; rows without a slot, and those that are no sequence's, become 0. */
 int akv_paged_read(const akv_paged_rows_args *args, void *stream);
 
 typedef struct akv_paged_attn_args {

@@ -488,3 +488,30 @@ def test_rows_of_a_padded_projection(T, H):
     assert torch.equal(out, want) and torch.equal(lse, wl)
     zero = torch.zeros(1, 40, device="cuda")
     assert torch.equal(akv.paged_importance(q, lse, w.pool, w.batch, zero.clone()), akv.paged_importance(plain, lse, w.pool, w.batch, zero.clone()))
+
+
+@pytest.mark.parametrize("D,n", [(128, 5), (64, 3001)])
+def test_read_of_padded_batches(D, n):
+    """Rows of a read that are no sequence's, or that no sequence has a slot for, are 0: behind the last
+    sequence, and where there is none."""
+    import akv
+    announce(f"paged read of {n} rows, D={D}, padded")
+    w = World(D, 32, 16, 3, [40, 9], [2, 1])
+    w.fill()
+    b = w.batch
+    want = akv.paged_read(w.pool, b)
+    junk = [torch.full((n, 3, D), 7.0, dtype=torch.float16, device="cuda") for _ in range(2)]  # what the allocator may hand out
+    del junk
+    got = akv.paged_read(w.pool, akv.PagedBatch(b.page_table, b.kv_lens, b.q_starts, n, 2))
+    for x, y in zip(got, want):
+        assert torch.equal(x[:3], y) and not bool(x[3:].any())
+    junk = [torch.full((n, 3, D), 7.0, dtype=torch.float16, device="cuda") for _ in range(2)]
+    del junk
+    none = akv.PagedBatch(b.page_table[:0], b.kv_lens[:0], b.q_starts[:1], n, 2)
+    assert not any(bool(x.any()) for x in akv.paged_read(w.pool, none))
+    akv.paged_append(w.pool, none, *want_rows(n, D))
+    w.same_pool()
+
+
+def want_rows(n, D):
+    return _x((n, 3, D), 1), _x((n, 3, D), 2)
