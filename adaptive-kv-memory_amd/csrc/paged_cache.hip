@@ -103,8 +103,8 @@ __device__ __forceinline__ Slot slot_of(const PagedRowsParams &p, int t, bool li
     const int s = seq_of(p.seqs, t, live);
     if (s < 0) return at;
     const SeqRows r = seq_rows(p.seqs, s, log_page);
-    const int64_t pos = (int64_t)r.kv - r.n + (t - r.begin);
-    if (t < r.begin || t >= r.begin + r.n || pos < 0) return at;
+    const int64_t pos = (int64_t)p.seqs.kv_lens[s] - r.n + (t - r.begin);
+    if (t < r.begin || t >= r.begin + r.n || pos < 0 || pos >> log_page >= p.seqs.width) return at;
     const uint32_t page = (uint32_t)p.seqs.table[s * p.seqs.table_stride + (pos >> log_page)];
     if (page >= p.pool.n_pages) return at;
     at.page = p.pool.base + page * p.pool.page_bytes + (int64_t)((int)(pos >> 4) & ((1 << p.pool.log_tpp) - 1)) * tile_bytes;

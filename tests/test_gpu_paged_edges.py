@@ -515,3 +515,22 @@ def test_read_of_padded_batches(D, n):
 
 def want_rows(n, D):
     return _x((n, 3, D), 1), _x((n, 3, D), 2)
+
+
+def test_rows_past_the_table_have_no_slot():
+    """A sequence that outgrew its table: the rows whose place lies past its end are not written over the
+    tokens that are there, and are read as 0; those before it keep theirs."""
+    import akv
+    announce("paged append and read past the table's end")
+    w = World(128, 32, 16, 2, [32, 32, 32], [4, 4, 4], spare=0)
+    w.fill()
+    table = w.batch.page_table[:, :2].contiguous()
+    lens = torch.tensor([36, 34, 10 ** 9], dtype=torch.int32, device="cuda")  # places 32.., 30.., far away
+    batch = akv.PagedBatch(table, lens, w.batch.q_starts, 12, 4)
+    k, v = _x((12, 2, 128), 1), _x((12, 2, 128), 2)
+    akv.paged_append(w.pool, batch, k, v)
+    w.ref.write(0, w.table[1], [30, 31], *(x[4:6].double().cpu().numpy() for x in (k, v)))
+    w.same_pool()
+    for got, e in zip(akv.paged_read(w.pool, batch, dtype=torch.float32), w.ref.read(0, w.table[1], [30, 31])):
+        assert not bool(got[:4].any()) and not bool(got[6:].any())
+        assert (np.abs(got[4:6].double().cpu().numpy() - e) <= np.abs(e) * 2.0 ** -24 + 2.0 ** -25).all()
