@@ -113,13 +113,17 @@ hipError_t paged_importance_launch(const PagedImportanceParams &p, hipStream_t s
 hipError_t paged_importance_tile_launch(const PagedImportanceParams &p, hipStream_t s);
 
 #ifdef __HIPCC__
-// Rows [begin, begin + n) of sequence s in the call's tensors, and its cached tokens.
+// Rows [begin, begin + n) of sequence s in the call's tensors, its cached tokens that have a slot, and
+// the first row's place (of a sequence that outgrew its table they are not kv's last ones).
 struct SeqRows {
-    int begin, n, kv;
+    int begin, n, kv, at;
+    // Tokens that row i sees.
+    __device__ __forceinline__ int sees(int causal, int i) const { return causal ? min(max(at + i + 1, 0), kv) : kv; }
 };
 // The same of a sequence that is one for the whole wave, in scalar registers.
 __device__ __forceinline__ SeqRows wave_uniform(const SeqRows &r) {
-    return {__builtin_amdgcn_readfirstlane(r.begin), __builtin_amdgcn_readfirstlane(r.n), __builtin_amdgcn_readfirstlane(r.kv)};
+    return {__builtin_amdgcn_readfirstlane(r.begin), __builtin_amdgcn_readfirstlane(r.n), __builtin_amdgcn_readfirstlane(r.kv),
+            __builtin_amdgcn_readfirstlane(r.at)};
 }
 __device__ __forceinline__ SeqRows seq_rows(const PagedSeqs &q, int s, int log_page) {
     const int64_t lim = q.n_tokens;
@@ -127,9 +131,8 @@ __device__ __forceinline__ SeqRows seq_rows(const PagedSeqs &q, int s, int log_p
     a = a < 0 ? 0 : a > lim ? lim : a;
     b = b < a ? a : b > lim ? lim : b;
     const int64_t cap = (int64_t)q.width << log_page;
-    int64_t kv = q.kv_lens[s];
-    kv = kv < 0 ? 0 : kv > cap ? cap : kv;
-    return {(int)a, (int)(b - a), (int)kv};
+    const int64_t len = q.kv_lens[s] < 0 ? 0 : q.kv_lens[s];
+    return {(int)a, (int)(b - a), (int)(len > cap ? cap : len), (int)(len - (b - a))};
 }
 #endif
 

@@ -191,10 +191,10 @@ __device__ __forceinline__ int seq_total(const PagedAttnParams &p, const SeqWork
 struct Scan {
     int pre[257];
     int wave_sum[kWaves];
-    int begin[kThreads], n[kThreads], kv[kThreads];
+    int begin[kThreads], n[kThreads], kv[kThreads], at[kThreads];
 };
 __device__ __forceinline__ SeqRows scanned_rows(const PagedAttnParams &p, const Scan &sc, int s) {
-    return p.seqs.n_seqs <= kThreads ? SeqRows{sc.begin[s], sc.n[s], sc.kv[s]} : seq_rows(p.seqs, s, p.pool.log_tpp + 4);
+    return p.seqs.n_seqs <= kThreads ? SeqRows{sc.begin[s], sc.n[s], sc.kv[s], sc.at[s]} : seq_rows(p.seqs, s, p.pool.log_tpp + 4);
 }
 __device__ __forceinline__ void scan_seqs(const PagedAttnParams &p, Scan &sc, int per) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
@@ -204,7 +204,7 @@ __device__ __forceinline__ void scan_seqs(const PagedAttnParams &p, Scan &sc, in
         if (s < p.seqs.n_seqs) {
             const SeqRows r = seq_rows(p.seqs, s, p.pool.log_tpp + 4);
             mine += seq_total(p, seq_work(p, r));
-            if (per == 1) sc.begin[t] = r.begin, sc.n[t] = r.n, sc.kv[t] = r.kv;
+            if (per == 1) sc.begin[t] = r.begin, sc.n[t] = r.n, sc.kv[t] = r.kv, sc.at[t] = r.at;
         }
     }
     int inc = mine;
@@ -312,10 +312,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const PagedAt
         const int row = row0 + min(col, rows - 1);
         const int qt = row / p.g;
         const int kv = w.r.kv;
-        const int old = kv - w.r.n + 1;  // cached tokens the call's first row sees
-        const int see = p.causal ? max(old + qt, 0) : kv;
-        const int see_all = p.causal ? max(old + row0 / p.g, 0) : kv;
-        const int see_any = p.causal ? max(old + (row0 + rows - 1) / p.g, 0) : kv;
+        const int see = w.r.sees(p.causal, qt);
+        const int see_all = w.r.sees(p.causal, row0 / p.g);
+        const int see_any = w.r.sees(p.causal, (row0 + rows - 1) / p.g);
         u4 qw[NS];
         load_row<D>(qw, p.q + (w.r.begin + qt) * p.q_t + (h * p.g + row % p.g) * p.q_h);
 
@@ -817,7 +816,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_importance_kernel(const Pag
                 Query<D, NG> Q;
                 make_query<D, NG>(Q, qw, p.q_bf16, p.scale_log2);
                 const float bias = live ? -lse2 : -INFINITY;
-                const int see = p.causal ? max(r.kv - r.n + qt + 1, 0) : r.kv;
+                const int see = r.sees(p.causal, qt);
                 const bool clean = have == ALL && __builtin_amdgcn_ballot_w64(tok0 + NT * 16 <= see) == ~0ull;
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
@@ -901,7 +900,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_importance_step_kernel(cons
         const int rows = (n - first) * p.g;
         const bool live = col < rows;
         const int row = live ? col : rows - 1, qt = first + row / p.g;
-        const int see = !live ? 0 : p.causal ? max(r.kv - r.n + qt + 1, 0) : r.kv;
+        const int see = live ? r.sees(p.causal, qt) : 0;
         const int log_tpp = p.pool.log_tpp, in_page = (1 << log_tpp) - 1;
         const int32_t *table = p.seqs.table + s * p.seqs.table_stride;
         const int t0 = (int)(tok0 >> 4);

@@ -103,7 +103,7 @@ __device__ __forceinline__ Slot slot_of(const PagedRowsParams &p, int t, bool li
     const int s = seq_of(p.seqs, t, live);
     if (s < 0) return at;
     const SeqRows r = seq_rows(p.seqs, s, log_page);
-    const int64_t pos = (int64_t)p.seqs.kv_lens[s] - r.n + (t - r.begin);
+    const int64_t pos = (int64_t)r.at + (t - r.begin);
     if (t < r.begin || t >= r.begin + r.n || pos < 0 || pos >> log_page >= p.seqs.width) return at;
     const uint32_t page = (uint32_t)p.seqs.table[s * p.seqs.table_stride + (pos >> log_page)];
     if (page >= p.pool.n_pages) return at;

@@ -60,14 +60,14 @@ __device__ __forceinline__ TileSeq tile_seq(const PagedAttnParams &p, int s, boo
     if (uniform) q.r = wave_uniform(q.r);
     q.rows = min(q.r.n, p.seqs.max_q) * p.g;
     q.tiles = q.rows > p.few_rows ? (q.rows + R - 1) / R : 0;
-    const int64_t old = max(q.r.kv - q.r.n, 0);
+    const int64_t old = min(max(q.r.at, 0), q.r.kv);
     q.a = (int64_t)p.g * ((p.causal ? old : q.r.kv) + kSetupTok) + R;
     q.b = p.causal ? R : 0;
     return q;
 }
 // Tokens that row `row` sees.
 __device__ __forceinline__ int sees(const PagedAttnParams &p, const TileSeq &q, int row) {
-    return p.causal ? max(q.r.kv - q.r.n + row / p.g + 1, 0) : q.r.kv;
+    return q.r.sees(p.causal, row / p.g);
 }
 template <int R>
 __device__ __forceinline__ int steps_of(const PagedAttnParams &p, const TileSeq &q, int t) {
@@ -785,7 +785,7 @@ __global__ __launch_bounds__(256, 2) void paged_importance_tile_kernel(const Pag
             const unsigned char *buf = smem + (h & 1) * BUF;
             const bool live = row0 + 32 * wave + col < rows;
             const int row = min(row0 + 32 * wave + col, rows - 1);
-            const int see = live ? (p.causal ? r.kv - r.n + first + row / p.g + 1 : r.kv) : 0;
+            const int see = live ? r.sees(p.causal, first + row / p.g) : 0;
             h8 op[D / 16];
             const float kx = __builtin_ldexpf(p.scale_log2, tile_query<D>(op, w, p.q_bf16));
             float bias = lse * -1.4426950408889634f;

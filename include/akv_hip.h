@@ -452,9 +452,8 @@ typedef struct akv_paged_pool {
  * j % page_size of page page_table[s][j / page_size]; its q_starts[s + 1] - q_starts[s] newest
  * ones are this call's, rows q_starts[s].. of the call's (n_tokens, heads, D) tensors.  The
  * arrays are device memory (4-byte aligned) and are read when the work runs, so a captured
- * call follows them.  q_starts ascends from 0.  Tokens past the table's end have no slot: they are
- * not written, and to the attention and the importance a length past it counts as the end.  Slots
- * on pages outside the pool are not written and hold no token. */
+ * call follows them.  q_starts ascends from 0.  Tokens past the table's end have no slot, and slots
+ * on pages outside the pool hold no token: neither is written, or seen by a row. */
 typedef struct akv_paged_batch {
     const int32_t *page_table; /* [n_seqs] rows of table_width entries, table_stride apart */
     const int32_t *kv_lens;    /* [n_seqs] */

@@ -534,3 +534,33 @@ def test_rows_past_the_table_have_no_slot():
     for got, e in zip(akv.paged_read(w.pool, batch, dtype=torch.float32), w.ref.read(0, w.table[1], [30, 31])):
         assert not bool(got[:4].any()) and not bool(got[6:].any())
         assert (np.abs(got[4:6].double().cpu().numpy() - e) <= np.abs(e) * 2.0 ** -24 + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("D,G", [(128, 32), (64, 64)])
+@pytest.mark.parametrize("Hq,n,lens", [(4, 4, [66, 64, 63, 70]), (4, 40, [66, 100, 64, 80]), (2, 200, [90, 200, 264, 300])])
+def test_rows_past_the_table_see_what_is_there(Hq, n, lens, D, G):
+    """The rows of a sequence that outgrew its table count from its length: each sees the tokens up to its
+    own, of those that have a slot; the importance likewise."""
+    import akv
+    announce(f"paged attention past the table's end, {n} rows, D={D}")
+    cap, H = 64, 2
+    w = World(D, G, 16, H, [cap] * 4, [n] * 4)
+    w.fill()
+    batch = akv.PagedBatch(w.batch.page_table[:, :cap // 16].contiguous(), torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                           w.batch.q_starts, 4 * n, n)
+    for dt in ("fp16", "bf16"):
+        q = _x((4 * n, Hq, D), 5, dt)
+        out, lse = akv.paged_attention(q, w.pool, batch, return_lse=True)
+        scores = torch.zeros(4, cap, device="cuda")
+        akv.paged_importance(q, lse, w.pool, batch, scores)
+        for s, m in enumerate(lens):
+            seen = np.clip(np.arange(m - n, m) + 1, 0, cap)
+            r = slice(s * n, s * n + n)
+            kp, vp = w.ref.parts(0, w.table[s], np.arange(cap))
+            x = q[r].double().cpu().numpy()
+            eo, el, bo, bl = ref.attention(x, kp, vp, D ** -0.5, seen, torch.finfo(q.dtype).eps / 2)
+            ok = seen > 0
+            go, gl = out[r].double().cpu().numpy(), lse[r].double().cpu().numpy()
+            assert (np.abs(go - eo) <= bo).all() and (np.abs(gl[ok] - el[ok]) <= bl[ok]).all() and np.isneginf(gl[~ok]).all()
+            e, d = ref.importance(x, kp, D ** -0.5, seen, gl)
+            assert (np.abs(scores[s].double().cpu().numpy() - e) <= d + 2.0 ** -22 * e).all()
