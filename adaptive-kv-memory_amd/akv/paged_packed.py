@@ -516,7 +516,8 @@ class PackedPagedCache:
         the device, below its length), in every layer, and gives the rest of its pages back.
 
         The tokens move to fresh pages: a shared page stays as it is for those who share it.
-        Where the free pages do not hold all sequences at once, they move in turns."""
+        Where the free pages do not hold all sequences at once, they move in turns.  The positions are
+        looked at before anything moves, which waits for the device."""
         counts = [int(t.shape[0]) for t in keep]
         nat.require_device(*keep)
         for t in keep:
@@ -524,7 +525,13 @@ class PackedPagedCache:
                 raise ValueError("keep holds a one-dimensional integer tensor for each sequence")
         _check_device(self.pool, *keep)
         book = self._book
-        for group in book.plan_compaction(seqs, counts):
+        groups = book.plan_compaction(seqs, counts)
+        if any(counts):
+            n, c = self._upload([book.lens[s] for s in seqs], counts)
+            at, end = torch.cat(list(keep)), n.repeat_interleave(c, output_size=sum(counts))
+            if bool(((at < 0) | (at >= end)).any()):
+                raise ValueError("keep names a position that is not one of its sequence's tokens")
+        for group in groups:
             lens = [book.lens[seqs[i]] for i in group]
             moved = [book.replace(seqs[i], counts[i]) for i in group]
             try:

@@ -269,3 +269,34 @@ def test_empty_calls():
     akv.copy_pages(pool, z(0), z(0))
     akv.compact_pages(pool, z(0, 1), z(0, 1), z(0, 4), z(0))
     akv.compact_pages(pool, z(2, 1), z(2, 1), z(2, 0), z(2))
+
+
+def test_compaction_refuses_positions_that_are_no_tokens():
+    """A position at or behind a sequence's length would move a stale slot into it, a negative one none at
+    all: refused before anything moves, whatever the lists' types, and however the turns fall."""
+    import akv
+    announce("compaction, positions out of range")
+    cache = akv.PackedPagedCache(2, 1, 64, page_size=16, max_pages=10, group_size=32)
+    t = Twin(cache, 2, 32)
+    s = [cache.add_sequence() for _ in range(3)]
+    for x in s:
+        t.add(x)
+    t.step(s, [40, 20, 0], 2, 1, torch.float16)
+    free = cache.num_free_pages
+    one = lambda *x, dtype=torch.int64: torch.tensor(x, dtype=dtype, device="cuda")  # noqa: E731
+    good = one(0, 5, 39), one(19, dtype=torch.int32), one()
+    for i, bad in ((0, one(1, 40)), (0, one(-1, 3, dtype=torch.int32)), (1, one(20, dtype=torch.int32)), (1, one(2 ** 32 + 1)),
+                   (0, one(47)), (1, one(0, 10 ** 9, dtype=torch.int32))):
+        keep = list(good)
+        keep[i] = bad
+        with pytest.raises(ValueError, match="position"):
+            cache.compact(s, keep)
+        assert cache.num_free_pages == free
+        for x in s:
+            t.same(x)
+    cache.compact(s, good)
+    for x, k in zip(s, good):
+        if t.kv[x][0] is not None:
+            t.kv[x] = [[y[k.cpu().numpy()] for y in kv] for kv in t.kv[x]]
+        t.same(x)
+    cache.compact([], [])
