@@ -67,7 +67,7 @@ def _int32(name: str, t: torch.Tensor, dims: int) -> torch.Tensor:
     if t.dim() != dims or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be an int32 tensor of {dims} dimension{'s' if dims > 1 else ''}")
     if t.dtype != torch.int32:
-        t = t.to(torch.int32)
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)  # what is out of range stays so
     plain = t.numel() == 0 or (t.stride(-1) == 1 and (dims == 1 or t.shape[0] == 1 or t.stride(0) >= t.shape[1]))
     return t if plain else t.contiguous()
 

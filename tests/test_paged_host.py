@@ -264,3 +264,12 @@ def test_strides_of_single_rows_say_nothing():
             assert st % 16 == 0 and sh % 16 == 0 and z.data_ptr() % 16 == 0
             got = torch.as_strided(z, (T, H, 128), (st // e, sh // e, 1))
             assert torch.equal(got, y)
+
+
+def test_entries_past_32_bits_stay_out_of_range():
+    """64-bit tables and lists: what does not fit 32 bits must not come out as a page or position that is there."""
+    from akv.paged_packed import _int32
+    t = torch.tensor([3, -1, 2 ** 32 + 1, -2 ** 33, 2 ** 31, 2 ** 62])
+    got = _int32("keep", t, 1)
+    assert got.dtype == torch.int32 and got.tolist() == [3, -1, 2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 2 ** 31 - 1]
+    assert _int32("table", t.view(2, 3), 2).tolist() == [[3, -1, 2 ** 31 - 1], [-2 ** 31, 2 ** 31 - 1, 2 ** 31 - 1]]
