@@ -179,3 +179,31 @@ def test_scores_of_any_size(n, size):
             worst = float(((out.double() - mean).abs() - torch.finfo(dt).eps * mean.abs()).max())
             assert worst <= 2.0 ** -11
             assert bool(((lse - math.log(kv - 1)).abs() < 1e-4).all())
+
+
+@pytest.mark.parametrize("D,G", [(128, 32), (64, 64)])
+@pytest.mark.parametrize("size", [1e-2, 1e-3, 1e-4, 1e-6])
+def test_small_values(size, D, G):
+    """Flat weights over small values, few rows and chunks: the limits follow the outputs' size (and
+    float16's smallest step), so that zeros in their place would not pass."""
+    import akv
+    H, g = 2, 4
+    gen = torch.Generator(device="cuda").manual_seed(D)
+    one = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    for kv, n in ((90, 1), (2000, 3), (300, 90)):
+        announce(f"paged attention D={D} G={G} kv={kv} rows={n}, values of {size}")
+        pool, table, whole = _pool(kv, H, D, G, gen)
+        k, v = torch.randn(2, kv, H, D, generator=gen, device="cuda")
+        akv.paged_append(pool, whole, k, v * size)
+        k, v = (x.double() for x in akv.paged_read(pool, whole, 0, torch.float32))
+        batch = akv.PagedBatch(table, one(kv), one(0, n), n, n)
+        see = torch.ones(n, kv, dtype=torch.bool, device="cuda").tril(kv - n)
+        for dt in (torch.float16, torch.bfloat16):
+            q = torch.randn(n, H * g, D, generator=gen, device="cuda").to(dt)
+            eo = _exact(q, k, v, g, see)[0]
+            for lse in (True, False):
+                out = akv.paged_attention(q, pool, batch, return_lse=lse)
+                _check(out[0] if lse else out, eo, f"{dt}, kv {kv}, log-sums {lse}")
+            if dt == torch.bfloat16 or size > 1e-6:
+                with pytest.raises(AssertionError):
+                    _check(torch.zeros_like(q), eo, "zeros")
