@@ -1,6 +1,8 @@
 // The paged 4-bit cache's data movement: append (quantize into slots), read (values out of
 // slots), copies of whole pages and the compaction of sequences to the tokens that stay.
 // All of it is bound by memory; the tile layout is written out in akv_hip.h.
+#include <algorithm>
+
 #include "akv_common.h"
 #include "paged.h"
 
@@ -467,16 +469,24 @@ __global__ __launch_bounds__(256) void paged_compact_kernel(const PagedCompactPa
 
 namespace {
 
-// Rows of the smallest call whose waves take four sets each (fewer rows leave compute units
-// idle: 384 rows, a decode step of 48 sequences, are appended and read in 6.7 us at one set and 10.8 at four).
-constexpr int64_t kManyRows = 8192;
+// Whether a call's waves take four sets of rows each: fewer waves, which have their loads in flight
+// together, but leave compute units idle, and look up a slot for each of the `span` tokens in them.  By
+// the waves of one set that the call has.  Append of one set a wave against four, us: head_dim 128, 8
+// heads (one token): 8192, 12288, 16384 and 65536 rows 5.5, 7.0, 8.4, 22.1 and 6.5, 7.2, 7.5, 17.4; one
+// head (eight): 32768, 49152, 65536 rows 11.1, 15.3, 19.8 and 12.3, 15.8, 19.4; head_dim 64, 8 heads (two):
+// 24576, 32768, 49152 rows 5.8, 6.9, 9.5 and 6.7, 7.0, 8.2; 2 heads (eight): 65536, 131072 rows 10.9, 20.0
+// and 11.9, 19.9.  The read crosses at the same sizes.
+bool four_sets(int64_t rows, int64_t wave_rows, int64_t heads) {
+    const int64_t span = std::max<int64_t>(1, 4 * wave_rows / heads);
+    return rows >= 3072 * (1 + span) * wave_rows;
+}
 
 template <template <int, int, int> class K>
 hipError_t rows_launch(const PagedRowsParams &p, hipStream_t s) {
     const int64_t rows = p.seqs.n_tokens * p.pool.heads;
     if (rows == 0) return hipSuccess;  // (rows of no sequence are read as 0)
     if (rows >= (int64_t)1 << 31) return hipErrorInvalidConfiguration;
-    const bool many = rows >= kManyRows;
+    const bool many = four_sets(rows, 256 / p.D, p.pool.heads);
     const int64_t wave_rows = (256 / p.D) * (many ? 4 : 1);
     const unsigned blocks = (unsigned)((rows + 4 * wave_rows - 1) / (4 * wave_rows));
     auto go = [&](auto one, auto four) {

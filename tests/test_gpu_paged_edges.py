@@ -564,3 +564,37 @@ def test_rows_past_the_table_see_what_is_there(Hq, n, lens, D, G):
             assert (np.abs(go - eo) <= bo).all() and (np.abs(gl[ok] - el[ok]) <= bl[ok]).all() and np.isneginf(gl[~ok]).all()
             e, d = ref.importance(x, kp, D ** -0.5, seen, gl)
             assert (np.abs(scores[s].double().cpu().numpy() - e) <= d + 2.0 ** -22 * e).all()
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("D,G,P,H,T", [(128, 32, 16, 8, 1700), (128, 64, 32, 3, 7001), (64, 32, 64, 8, 5003), (128, 128, 16, 1, 60001), (64, 64, 16, 16, 2500)])
+def test_large_prompts_like_their_parts(D, G, P, H, T, dt):
+    """Calls whose waves take several sets of rows each write and read the bytes that small calls do."""
+    import akv
+    announce(f"paged append and read of {T} tokens at once and in parts, D={D} G={G} P={P} H={H} {dt}")
+    q = [T // 2 + 3, 0, T - T // 2 - 8, 5]
+    past = [0, 7, 21, 3]
+    kv = [a + b for a, b in zip(q, past)]
+    pages = [-(-n // P) for n in kv]
+    up = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    ids = torch.randperm(sum(pages) + 2, device="cuda").to(torch.int32)
+    table = torch.full((4, max(pages)), -1, dtype=torch.int32, device="cuda")
+    for s, c in enumerate(pages):
+        table[s, :c] = ids[sum(pages[:s]):sum(pages[:s]) + c]
+    starts = np.concatenate([[0], np.cumsum(q)]).tolist()
+    k, v = _x((T, H, D), 1, dt), _x((T, H, D), 2, dt)
+    k[T // 3, 0, 5] = float("nan")
+    one, parts = (akv.PagedPool.empty(1, sum(pages) + 2, H, D, P, G) for _ in range(2))
+    whole = akv.PagedBatch(table, up(kv), up(starts), T, max(q))
+    akv.paged_append(one, whole, k, v)
+    got = akv.paged_read(one, whole, dtype=DT[dt])
+    step = max(1, 4000 // H)
+    for s in range(4):
+        for a in range(0, q[s], step):
+            n = min(step, q[s] - a)
+            r = slice(starts[s] + a, starts[s] + a + n)
+            some = akv.PagedBatch(table[s:s + 1], up([past[s] + a + n]), up([0, n]), n, n)
+            akv.paged_append(parts, some, k[r], v[r])
+            for x, y in zip(got, akv.paged_read(parts, some, dtype=DT[dt])):
+                assert torch.equal(x[r].view(torch.uint8), y.view(torch.uint8))
+    assert torch.equal(one.data, parts.data)
