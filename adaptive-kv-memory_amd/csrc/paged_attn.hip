@@ -1065,9 +1065,11 @@ int64_t paged_attn_plan(PagedAttnParams *p) {
     // where every sequence has the most rows there is none of few, and if there is the tiles take it
     if (r > kFewRows && p->seqs.n_tokens == (int64_t)p->seqs.n_seqs * p->seqs.max_q) p->groups = 0;
     // Short contexts and few of them: an item a workgroup, whatever its length, and nothing to merge
-    // (the workspace is not used).  Against runs of equal work, us for 128, 256, 384 and 512 tokens: one
-    // sequence of 8 heads: 10.1, 11.7, 13.3, 14.7 and 12.1, 12.1, 12.3, 12.5; for 512, 1024 and 2048, 32
-    // sequences, which fill the card: 15.6, 22.1, 34.0 and 19.4, 25.1, 34.3.
+    // (the workspace is not used).  Against runs of equal work, us for 128, 256, 384 and 512 tokens,
+    // bfloat16: 2 to 64 items: 9.5, 11.1, 12.7, 14.0 and 11.8, 11.8, 11.9, 12.1 (64: 13.7); 128 items: 9.7, 11.3,
+    // 12.9, 14.3 and 12.2, 13.5, 13.8, 15.6.  For 512, 1024 and 2048 tokens of 256 items, which fill the
+    // card: 14.7, 21.3, 32.4 and 17.7, 23.7, 31.9; 512 items: 19.2, 27.4, 41.8 and 24.7, 32.6, 47.7.  float16 is
+    // 5% slower on both sides.  The lengths are on the device: the table's width stands for them.
     const int64_t items = (int64_t)p->seqs.n_seqs * p->pool.heads * few_chunks(*p);
     if (r <= kFewRows && items <= kMaxGroups && units <= (items >= kMaxGroups / 2 ? 32 : 8)) {
         p->whole = (int)((units + kSetup + kWaves - 1) / kWaves * kWaves);
