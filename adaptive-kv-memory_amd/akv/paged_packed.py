@@ -207,11 +207,9 @@ def paged_attention(q: torch.Tensor, pool: PagedPool, batch: PagedBatch, layer: 
     m rows sees its first kv_len - m + 1 + i tokens, else all of them; a row that sees none is 0.
     ``return_lse`` adds log(sum(exp(sm_scale q.k))) (n_tokens, Hq) float32, -inf for such rows.
 
-    Sums and log-sums are float32.  For bfloat16 outputs the weights are rounded to float16 (an eighth
-    of the output's own half step), and in chunks of more than 64 rows a cached head the values, and
-    the keys unless log-sums are asked for: such a chunk's outputs differ with ``return_lse``, by less
-    than bfloat16's own rounding where scores are of a few units (a key's is 2^-12 of its score); for
-    float16 outputs the chunks' values alone are."""
+    Scores, sums and log-sums are float32.  For bfloat16 outputs the weights are rounded to float16
+    (an eighth of the output's own half step), and so are the values in chunks of more than 64 rows a
+    cached head, for float16 outputs too."""
     q, qt, qh = _queries(q, pool, batch)
     T, Hq, D = q.shape
     lib = nat.load()

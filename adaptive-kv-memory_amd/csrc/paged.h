@@ -13,9 +13,9 @@ constexpr int kUnitTok = 32;   // tokens a wave of the attention takes at a time
 constexpr int kRows = 16;      // query rows (tokens x heads of a group) that a wave takes
 // Sequences of more rows a cached head go to the tile kernel: a chunk of 16 rows costs a compute
 // unit 0.7 us for 64 tokens, a tile of up to 256 rows 2 us.  Chunks against a tile, us, 48, 64 and 80
-// rows: 16 sequences of 8192 tokens and 8 heads, bfloat16: 124, 146, 168 against 120, 117, 119, with
-// log-sums 117, 140, 167 against 152, 148, 151; float16: 129, 165, 199 against 164, 164, 172; one of
-// 32768: 43, 50, 57 against 66, 67, 70 and 48, 56, 65 against 78, 79, 83.
+// rows: 16 sequences of 8192 tokens and 8 heads, bfloat16: 120, 143, 168 against 152, 148, 151;
+// float16: 129, 165, 199 against 164, 164, 172; one of 32768: 43, 50, 57 against 76, 76, 79 and
+// 48, 56, 65 against 78, 79, 83.
 constexpr int kFewRows = 64;
 // The same for the importance, by the rows that a call's sequences may have.  16 rows a wave
 // against 128 a workgroup, us: two sequences of 12000 tokens and 8 heads, 128, 256 and 2048 rows: 40,

@@ -5,16 +5,13 @@
 // cached head, each wave 32 of them as the columns of 32x32x16 MFMAs, and walks the cache in
 // steps of 64 tokens, two buffers in LDS: while the MFMAs read one step, the next step's tiles
 // are in flight to registers, one wave a tile and side, and are then dequantized into the
-// other buffer, once for all rows.  Scores, running maximum and sum are float32; values become
-// float16 c s + z.  What else is rounded to float16 goes by the output, whose own rounding leaves 1.68e-3
-// (bfloat16) and 2.0e-4 (float16) of its norm:
-//   bfloat16  keys and p: 1.75e-3 to 1.95e-3 together; a rounded key moves its score by up to 2^-12 of it
-//   float16   nothing: keys and p (PTWO) are two float16 that add up to them: 2.8e-4 (with one of
-//             each 3.5e-4 to 5e-4)
-// Where the rows' log-sums are asked for, which are float32, keys are two float16 (TWO) for bfloat16 too.
-// Two always would make the outputs of both calls the same and cost a quarter of the time (three chunks
-// of 65 to 512 tokens on 64 heads after 2k to 32k: 715 us, with two 905).  Eight chunks of 512 tokens on
-// 64 heads over 8 after 8k: bfloat16 1.28 ms, with log-sums 1.57, float16 2.1.
+// other buffer, once for all rows.  Scores, running maximum and sum are float32.  Keys are two float16
+// that add up to c s + z, so that scores are exact to float32 sums; values are one float16, and p is one
+// for bfloat16 outputs, two (PTWO) for float16.  The outputs' own rounding leaves 1.68e-3 (bfloat16) and
+// 2.0e-4 (float16) of their norm, all together 1.70e-3 and 2.8e-4.  (Keys as one float16 took three
+// chunks of 65 to 512 tokens on 64 heads after 2k to 32k from 900 to 710 us, but with a channel ten times
+// the others bfloat16 outputs were 2.0e-3 off, and not those of a call that asks for log-sums.)
+// Eight chunks of 512 tokens on 64 heads over 8 after 8k: bfloat16 1.57 ms, float16 2.1.
 //   K  [64 tokens][D / 8 chunks] of 16 bytes, chunk c at place c ^ turn(token) of its row;
 //   V  the PV operand: [tile][32 channels][lane] of 16 bytes, tokens 4 hi + 0..3, 8 + 4 hi + 0..3;
 //      row 16 b + r of its MFMA is channel 2 r + b of the 32.
@@ -112,16 +109,8 @@ __device__ __forceinline__ int64_t tile_share(const PagedAttnParams &p, int64_t 
 // in all three.
 __device__ __forceinline__ int turn(int token) { return (token & 1) << 2 | (token & 2) | (token >> 2 & 1); }
 
-// The four pairs of a dword of codes (nibbles n and n + 4 of it) as c s + z.
-__device__ __forceinline__ void dequant8(const Nibbles &nb, uint32_t w, h2 s, h2 z, uint32_t *o) {
-    const uint32_t v = w >> 8;
-    o[0] = as_u32(__builtin_elementwise_fma(nb.low(w), s, z));
-    o[1] = as_u32(__builtin_elementwise_fma(nb.high(w), s, z));
-    o[2] = as_u32(__builtin_elementwise_fma(nb.low(v), s, z));
-    o[3] = as_u32(__builtin_elementwise_fma(nb.high(v), s, z));
-}
-
-// The same as two float16 that add up to c s + z (to 2^-22 of it).
+// The four pairs of a dword of codes (nibbles n and n + 4 of it) as two float16 that add up to c s + z
+// (to 2^-22 of it).
 __device__ __forceinline__ void dequant8_two(const Nibbles &nb, uint32_t w, h2 s, h2 z, uint32_t *o, uint32_t *lo) {
     const uint32_t v = w >> 8;
     const h2 c[4] = {nb.low(w), nb.high(w), nb.low(v), nb.high(v)};
@@ -169,7 +158,7 @@ struct Words<1> {
     __device__ __forceinline__ uint32_t operator[](int) const { return v; }
 };
 
-template <int D, int NG, bool TWO>
+template <int D, int NG>
 struct KLoad {
     Words<D / 32> c;
     Words<NG> m;
@@ -185,11 +174,10 @@ struct KLoad {
             const uint32_t w = m[g * NG / (D / 32)];
             const h2 s = as_h2((w & 0xffffu) | (w << 16)), z = as_h2((w >> 16) | (w & 0xffff0000u));
             uint32_t o[4], r[4];
-            if constexpr (TWO) dequant8_two(nb, c[g], s, z, o, r);
-            else dequant8(nb, c[g], s, z, o);
+            dequant8_two(nb, c[g], s, z, o, r);
             u4 *d = (u4 *)(kt + tok * (2 * D) + (((4 * g + i) ^ turn(tok)) << 4));
             *d = (u4){o[0], o[1], o[2], o[3]};
-            if constexpr (TWO) d[kStep * 2 * D / 16] = (u4){r[0], r[1], r[2], r[3]};
+            d[kStep * 2 * D / 16] = (u4){r[0], r[1], r[2], r[3]};
         }
     }
 };
@@ -348,10 +336,10 @@ __device__ __forceinline__ int tile_query(h8 (&op)[D / 16], const u4 (&w)[D / 16
 
 }  // namespace
 
-template <int D, int NG, int W, bool TWO, bool PTWO>
+template <int D, int NG, int W, bool PTWO>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_tile_kernel(const PagedAttnParams p) {
     constexpr int R = 32 * W, NB = D / 32, TB = paged_tile_bytes(D, NG), EROW = D + 4;
-    constexpr int KT = (TWO ? 2 : 1) * kStep * 2 * D, BUF = KT + kStep * 2 * D;
+    constexpr int KT = 2 * kStep * 2 * D, BUF = KT + kStep * 2 * D;
     extern __shared__ __align__(16) unsigned char smem[];
     int64_t *pre = (int64_t *)smem, *wave_sum = pre + 64 * W + 1;  // before the first step only
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -444,7 +432,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
                     page_hi = (uint32_t)(at >> 32);
                 };
                 pages(f0);
-                std::conditional_t<late, VLoad<D, NG>, KLoad<D, NG, TWO>> raw;
+                std::conditional_t<late, VLoad<D, NG>, KLoad<D, NG>> raw;
                 Nibbles nb;
                 nb.init();
                 int nv = 0;         // tokens of the wave's tile of the step that was loaded last
@@ -499,13 +487,12 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
                 auto scores = [&](const unsigned char *buf) {  // operand: (chunk pair, half of K, 32 tokens)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) sc[i >> 4][i & 15] = 0.0f;
-                    constexpr int PARTS = TWO ? 2 : 1;
-                    products<PARTS * 2 * (D / 16)>(
+                    products<4 * (D / 16)>(
                         [&](int i) {
-                            const int st = i / (2 * PARTS), part = i / 2 % PARTS, b = i & 1;
+                            const int st = i / 4, part = i / 2 % 2, b = i & 1;
                             return *(const h8 *)(buf + part * (kStep * 2 * D) + (32 * b + col) * (2 * D) + (((2 * st + hi) ^ turn(col)) << 4));
                         },
-                        [&](int i, h8 a) { sc[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qop[i / (2 * PARTS)], sc[i & 1], 0, 0, 0); });
+                        [&](int i, h8 a) { sc[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qop[i / 4], sc[i & 1], 0, 0, 0); });
                 };
                 auto softmax = [&](int step, uint32_t here) {
                     if (kStep * (step + 1) > see_all || here != 15u) {
@@ -763,7 +750,7 @@ __global__ __launch_bounds__(256, 2) void paged_importance_tile_kernel(const Pag
         const unsigned char *tile = p.pool.base + (uint64_t)(uint32_t)__builtin_amdgcn_readlane(id, wave) * p.pool.page_bytes +
                                     (uint32_t)((mine & ((1 << log_tpp) - 1)) * TB);
         const int64_t head_bytes = (int64_t)TB << log_tpp;
-        KLoad<D, NG, true> raw;
+        KLoad<D, NG> raw;
         Nibbles nb;
         nb.init();
         u4 w[D / 16];  // the next rows' queries and log-sums, in flight
@@ -856,12 +843,12 @@ constexpr int kTileGroups = 256;  // one workgroup a compute unit
 constexpr int64_t kTileSums = 8192;               // scan_tiles' sums at the start of the workspace
 static_assert((64 * kTileWaves + 1) * 8 <= kTileSums, "the sums fit");
 
-template <int D, int NG, bool TWO, bool PTWO>
+template <int D, int NG, bool PTWO>
 hipError_t tile_go_as(const PagedAttnParams &p, hipStream_t st) {
     constexpr int W = kTileWaves;
-    constexpr int LDS = 2 * (TWO ? 3 : 2) * kStep * 2 * D + (2 * 16 + 4 * 16 * NG) * 4;  // two buffers, what `hide` writes of each, V meta
+    constexpr int LDS = 2 * 3 * kStep * 2 * D + (2 * 16 + 4 * 16 * NG) * 4;  // two buffers, what `hide` writes of each, V meta
     static_assert((64 * W + 1 + W) * 8 <= LDS, "the sums fit the buffers");
-    auto kern = paged_tile_kernel<D, NG, W, TWO, PTWO>;
+    auto kern = paged_tile_kernel<D, NG, W, PTWO>;
     if (LDS > 48 * 1024) (void)hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
     kern<<<dim3(p.tile_groups), dim3(64 * W), LDS, st>>>(p);
     hipError_t e = hipGetLastError();
@@ -872,8 +859,7 @@ hipError_t tile_go_as(const PagedAttnParams &p, hipStream_t st) {
 }
 template <int D, int NG>
 hipError_t tile_go(const PagedAttnParams &p, hipStream_t st) {
-    if (!p.q_bf16) return tile_go_as<D, NG, true, true>(p, st);
-    return p.lse ? tile_go_as<D, NG, true, false>(p, st) : tile_go_as<D, NG, false, false>(p, st);
+    return p.q_bf16 ? tile_go_as<D, NG, false>(p, st) : tile_go_as<D, NG, true>(p, st);
 }
 }  // namespace
 

@@ -54,14 +54,13 @@ def _exact(q, k, v, g, see):
     return torch.stack(out, 1), torch.stack(lse, 1), torch.stack(rest, 1)
 
 
-def _check(got, exact, what, keys=0.0):
+def _check(got, exact, what):
     """Rounding to the output's type alone leaves 0.58 of half a step (of float16 below its normal
     range: of half its smallest, 2^-25), and the kernel's own part stays below 0.47 of it for float16
-    and 0.15 for bfloat16: 0.75 and 0.6 together.  ``keys``: the sink's score, where the keys of a chunk
-    are rounded to float16: 2^-12 of it is what all the others' weight together may be off by."""
+    and 0.15 for bfloat16: 0.75 and 0.6 together."""
     half, share = (2.0 ** -11, 0.75) if got.dtype == torch.float16 else (2.0 ** -8, 0.6)
     err = got.double() - exact
-    limit = (share * half + 2.0 ** -12 * keys) * float(exact.norm())
+    limit = share * half * float(exact.norm())
     if got.dtype == torch.float16:
         limit += share * 2.0 ** -25 * float((exact.abs() < 2.0 ** -14).sum()) ** 0.5
     assert float(err.norm()) <= limit, f"{what}: error {float(err.norm() / exact.norm()):.2e} of the norm, {float(err.norm()) / limit:.2f} of the limit"
@@ -90,10 +89,7 @@ def test_one_sequence(kv, n, H, g, D, G):
                 out, lse = akv.paged_attention(q, pool, batch, return_lse=True)
                 _check(out, eo, f"{dt}, sink {weight}, values {size}, {share}")
                 assert float((lse.double() - el).norm() / el.norm()) < 2.0 ** -20
-                one_key = dt == torch.bfloat16 and n * g > 64
-                score = LIFT * float(k[kv // 3, :, 0].max()) * D ** -0.5
-                _check(akv.paged_attention(q, pool, batch), eo, f"{dt}, sink {weight}, values {size}, {share}, without log-sums",
-                       score if one_key else 0.0)
+                assert torch.equal(out, akv.paged_attention(q, pool, batch))
 
 
 @pytest.mark.parametrize("D,G", [(128, 32), (64, 64)])
@@ -207,3 +203,30 @@ def test_small_values(size, D, G):
             if dt == torch.bfloat16 or size > 1e-6:
                 with pytest.raises(AssertionError):
                     _check(torch.zeros_like(q), eo, "zeros")
+
+
+@pytest.mark.parametrize("kv,n,H,g,D,G", [(8192, 65, 1, 8, 128, 32), (20000, 300, 1, 1, 128, 64), (4000, 90, 2, 2, 64, 32), (3000, 100, 1, 1, 128, 128)])
+def test_chunks_with_channels_that_stand_out(kv, n, H, g, D, G):
+    """Chunks over keys with a channel ten times the others: outputs are the same with and without log-sums,
+    and for bfloat16 no more than 3% farther from 64 bits than rounding alone leaves them."""
+    import akv
+    announce(f"paged attention of a chunk, kv={kv} rows={n} D={D} G={G}, a channel ten times the others")
+    gen = torch.Generator(device="cuda").manual_seed(kv)
+    pool, table, whole = _pool(kv, H, D, G, gen)
+    k, v = torch.randn(2, kv, H, D, generator=gen, device="cuda")
+    k[..., 3] *= 10.0
+    akv.paged_append(pool, whole, k, v)
+    k, v = (x.double() for x in akv.paged_read(pool, whole, 0, torch.float32))
+    one = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    batch = akv.PagedBatch(table, one(kv), one(0, n), n, n)
+    see = torch.ones(n, kv, dtype=torch.bool, device="cuda").tril(kv - n)
+    for dt in (torch.float16, torch.bfloat16):
+        q = torch.randn(n, H * g, D, generator=gen, device="cuda").to(dt)
+        eo = _exact(q, k, v, g, see)[0]
+        out = akv.paged_attention(q, pool, batch)
+        assert torch.equal(out, akv.paged_attention(q, pool, batch, return_lse=True)[0])
+        _check(out, eo, str(dt))
+        if dt == torch.bfloat16:
+            # p and the values in float16 leave 2^-12 / sqrt(3) = 1.4e-4 each, 2.0e-4 together: beside
+            # bfloat16's 1.65e-3 and more, the root of both squares is 0.8% above it
+            assert float((out.double() - eo).norm()) <= 1.03 * float((eo.to(dt).double() - eo).norm())
