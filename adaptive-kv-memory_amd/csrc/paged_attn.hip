@@ -242,12 +242,12 @@ __device__ __forceinline__ void write_row(const PagedAttnParams &p, const SeqRow
 
 }  // namespace
 
-// Single tokens and a few drafted ones.  Bound by the cache's bytes and, nearly as much, by issue:
-// 300 vector instructions and 17 MFMAs for 32 tokens of a head (400 and 27 where p is two
+// Single tokens and a few drafted ones.  Bound by issue and, nearly as much, by the cache's bytes:
+// 325 vector instructions and 17 MFMAs for 32 tokens of a head (415 and 27 where p is two
 // float16), two waves a SIMD.  24 sequences of 33 to 65536 tokens, 32 heads over 8, bfloat16 (299
-// MB): 61 us, 4.9 TB/s, and 5 us of merge; 20 rows of nine sequences of 1001 to 9001 tokens,
-// float16: 21 us and 5.6 us; one row of 517 tokens, whose time
-// is the chain of loads from lengths to tiles: 6.6 us and 3.4 us.
+// MB): 73 us, 4.1 TB/s, and 5 us of merge; 20 rows of nine sequences of 1001 to 9001 tokens,
+// float16: 22.5 us and 5.2 us; one row of 517 tokens, whose time
+// is the chain of loads from lengths to tiles: 7.4 us and 3.4 us.
 //
 // The units of all sequences, heads and chunks form one list, cut into equal runs, one a wave:
 // every wave has the same work whatever the lengths.  A run that covers an item (all units of

@@ -404,8 +404,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
                 for (int i = 0; i < 16; ++i) acc[b][i] = 0.0f;
 
             // Waves 0-3 stage K, waves 4-7 V, a tile each, and run half a step behind: one group's
-            // products meet the other's softmax and staging on each SIMD (0.80 ms without the
-            // offset, 0.74 with it, chunks of 65 to 512 tokens on 64 heads after 2k to 32k).
+            // products meet the other's softmax and staging on each SIMD (keys as one float16, chunks of
+            // 65 to 512 tokens on 64 heads after 2k to 32k: 0.80 ms without the offset, 0.74 with it).
             // Slots between barriers, t a step:
             //   2 t      K group's products (t), V group's softmax (t - 1)
             //   2 t + 1  K group's softmax (t), V group's products (t)
