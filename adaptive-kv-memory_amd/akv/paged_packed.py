@@ -238,7 +238,7 @@ def paged_importance(q: torch.Tensor, lse: torch.Tensor, pool: PagedPool, batch:
     tokens of every sequence that has rows in the batch (its first N, where it has more).
 
     q and lse are those of ``paged_attention``; ``q_window`` > 0 counts a sequence's last rows
-    only.  Written in place, or to ``out``; returns what was written."""
+    only.  Written in place, or to ``out``, which does not overlap scores; returns what was written."""
     q, qt, qh = _queries(q, pool, batch)
     T, Hq, D = q.shape
     dst = scores if out is None else out

@@ -1103,6 +1103,17 @@ int akv_paged_attn(const akv_paged_attn_args *a, void *stream) {
     return ok();
 }
 
+// Whether n_rows rows of n floats at a and at b, sa and sb floats apart, overlap other than as the same rows.
+static bool rows_clash(const float *a, int64_t sa, const float *b, int64_t sb, int64_t n, int64_t n_rows) {
+    if (n_rows == 1) sa = sb = n;
+    if (a == b && sa == sb) return false;
+    const int64_t d = (int64_t)((intptr_t)b - (intptr_t)a), f = sizeof(float);
+    if (d >= ((n_rows - 1) * sa + n) * f || -d >= ((n_rows - 1) * sb + n) * f) return false;
+    if (sa != sb) return true;
+    const int64_t s = sa * f, in = (d % s + s) % s;  // where b's rows begin between two of a's
+    return in < n * f || s - in < n * f;
+}
+
 int akv_paged_importance(const akv_paged_importance_args *a, void *stream) {
     if (!a) return fail(AKV_E_INVALID, "args is NULL");
     akv::PagedImportanceParams p{};
@@ -1116,7 +1127,10 @@ int akv_paged_importance(const akv_paged_importance_args *a, void *stream) {
         return fail(AKV_E_SHAPE, "bad score rows");
     if (a->batch.n_seqs == 0 || a->n_scores == 0) return ok();
     if (!a->scores || !a->out || (a->batch.n_tokens > 0 && !a->lse)) return fail(AKV_E_INVALID, "scores, out and lse are required");
-    if (!aligned4(a->scores) || !aligned4(a->out) || !aligned4(a->lse)) return fail(AKV_E_ALIGN, "float32 rows must be 4-byte aligned");
+    if (!aligned4(a->scores) || !aligned4(a->out)) return fail(AKV_E_ALIGN, "float32 rows must be 4-byte aligned");
+    if (rows_clash(a->scores, a->score_stride, a->out, a->out_stride, a->n_scores, a->batch.n_seqs))
+        return fail(AKV_E_SHAPE, "out must be scores or not overlap it");
+    if (!aligned4(a->lse)) return fail(AKV_E_ALIGN, "lse must be 4-byte aligned");
     p.D = a->pool.D; p.ng = a->pool.D / a->pool.group_size;
     p.Hq = a->Hq; p.g = a->Hq / a->pool.heads;
     p.q_bf16 = a->q_dtype == AKV_DT_BF16; p.causal = a->causal != 0; p.q_window = a->q_window;

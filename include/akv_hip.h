@@ -523,7 +523,7 @@ typedef struct akv_paged_importance_args {
     int64_t q_t, q_h;
     const float *lse;      /* (n_tokens, Hq) of akv_paged_attn */
     const float *scores;   /* [n_seqs] rows of n_scores, score_stride apart */
-    float *out;            /* likewise, out_stride apart; may be scores */
+    float *out;            /* likewise, out_stride apart; scores itself, or no part of it */
     int64_t n_scores, score_stride, out_stride;
 } akv_paged_importance_args;
 

@@ -273,3 +273,23 @@ def test_entries_past_32_bits_stay_out_of_range():
     got = _int32("keep", t, 1)
     assert got.dtype == torch.int32 and got.tolist() == [3, -1, 2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 2 ** 31 - 1]
     assert _int32("table", t.view(2, 3), 2).tolist() == [[3, -1, 2 ** 31 - 1], [-2 ** 31, 2 ** 31 - 1, 2 ** 31 - 1]]
+
+
+@pytest.mark.parametrize("scores,out,n,ss,so,S,clash", [
+    (0, 0, 10, 10, 10, 3, False), (0, 30, 10, 10, 10, 3, False), (30, 0, 10, 10, 10, 3, False),
+    (0, 10, 10, 20, 20, 3, False), (10, 0, 10, 20, 20, 3, False),                                # columns of one buffer
+    (0, 1, 10, 20, 20, 3, True), (9, 0, 10, 20, 20, 3, True), (0, 11, 10, 20, 20, 3, True),      # shifted
+    (0, 10, 10, 10, 10, 3, True), (0, 20, 10, 20, 20, 3, True), (0, 60, 10, 20, 20, 3, False),   # rows on
+    (0, 0, 10, 10, 12, 3, True), (0, 0, 10, 10, 12, 1, False),                                   # one row: strides say nothing
+    (0, 5, 10, 10, 10, 1, True), (5, 0, 10, 10, 10, 1, True), (0, 10, 10, 1, 1, 1, False),
+])
+def test_importance_refuses_scores_that_overlap_its_output(scores, out, n, ss, so, S, clash):
+    """out may be scores or lie apart from it, also as columns of one buffer; other views are refused.
+    (lse off its alignment is refused behind that: no call here is launched.)"""
+    from akv import _native as nat
+    lib = nat.load()
+    at = 1 << 20
+    a = nat.PagedImportanceArgs(abi_version=nat.ABI_VERSION, layer=0, pool=_pool(nat), batch=_batch(nat, n_seqs=S), Hq=4, q_dtype=0,
+                                causal=1, sm_scale=0.1, q=4096, q_t=1024, q_h=256, q_window=0, decay=0.9, lse=4097,
+                                scores=at + 4 * scores, out=at + 4 * out, n_scores=n, score_stride=ss, out_stride=so)
+    assert lib.akv_paged_importance(ctypes.byref(a), None) == (nat.AKV_E_SHAPE if clash else nat.AKV_E_ALIGN), lib.akv_last_error()
