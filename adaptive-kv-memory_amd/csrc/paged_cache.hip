@@ -478,7 +478,7 @@ namespace {
 // and 11.9, 19.9.  The read crosses at the same sizes.
 bool four_sets(int64_t rows, int64_t wave_rows, int64_t heads) {
     const int64_t span = std::max<int64_t>(1, 4 * wave_rows / heads);
-    return rows >= 3072 * (1 + span) * wave_rows;
+    return rows >= 3000 * (1 + span) * wave_rows;
 }
 
 template <template <int, int, int> class K>
