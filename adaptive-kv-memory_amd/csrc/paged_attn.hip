@@ -27,7 +27,7 @@ constexpr int kImpHeads = 3;          // most heads of a wave there
 __host__ __device__ constexpr int paged_query_bytes(int D, int ng) { return 32 * D + 64 * (ng + 2); }
 // The few-rows kernel holds p times 2^14, in (0, 2^14], and V scales over a power of two that they stay
 // below (at kHighExp below twice it: the append's largest is 2^13): p times a scale keeps 11 bits down
-// to 2^-28 of the largest, and something down to 2^-38.  (With p in (0, 4] and scales as they are, a
+// to 2^-28 of the largest, and something down to 2^-38 (less by what scales lie below 2^-12).  (With p in (0, 4] and scales as they are, a
 // token of 0.999 of the weight and a value near 0 took 2e-3 to 1e-1 of an output with it, by the size
 // of the values and the length of a wave's run.)
 constexpr float kFewBias = 14.0f;
