@@ -388,8 +388,8 @@ def run(st):
         if c["kind"] == "importance":
             return akv.latent_importance(st["q"], st["q_rope"], st["lse"], st["pages"], st["batch"], st["scores"], st["scale"],
                                          decay=0.9, q_window=c["q_window"], out=st["out"])
-        keep, n_keep, scores = akv.evict_select(st["scores"], st["kv_lens"], c["budget"], protect_first=c["first"],
-                                                protect_last=c["last"])
+        keep, n_keep, scores = akv.evict_select(st["scores"], st["kv_lens"], c["budget"], protect_initial=c["first"],
+                                                protect_recent=c["last"])
         akv.compact_pages(st["pages"], st["table"], st["to"], keep, n_keep)
         return keep, n_keep, scores, st["pool"][:, st["first"]:]
     if c["kind"] == "attend":
