@@ -11,12 +11,23 @@ from .drop_in import AKVCache, AKVLayer, _PRESETS, recommend_preset, select_demo
 from .fused_attention import fused_int4_decode_attention, mixed_precision_decode_attention
 from .importance import ImportanceConfig, ImportanceScorer, ScoringStrategy
 from .packed_layout import PackedKVArena, PackedKVConfig, PagedKVCache
+from .paged_latent import (
+    LatentWeights,
+    PagedLatentCache,
+    PagedLatentPool,
+    latent_append,
+    latent_attention,
+    latent_importance,
+    latent_prefill,
+    latent_read,
+)
 from .paged_packed import (
     PackedPagedCache,
     PagedBatch,
     PagedPool,
     compact_pages,
     copy_pages,
+    evict_select,
     paged_append,
     paged_attention,
     paged_importance,
@@ -46,6 +57,8 @@ __all__ = [
     "fused_decode_attention", "fused_quantize_evict",
     "HAS_TRITON", "fused_importance_update", "fused_mixed_precision_attention", "fused_quantized_attention",
     "PackedPagedCache", "PagedBatch", "PagedPool", "compact_pages", "copy_pages", "paged_append", "paged_attention",
-    "paged_importance", "paged_read",
+    "paged_importance", "paged_read", "evict_select",
+    "LatentWeights", "PagedLatentCache", "PagedLatentPool", "latent_append", "latent_attention", "latent_importance",
+    "latent_prefill", "latent_read",
     "WarmTier", "decode_attention", "dequantize", "prefill_attention", "quantize_kv",
 ]

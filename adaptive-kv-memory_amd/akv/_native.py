@@ -193,6 +193,70 @@ class PagedCompactArgs(ctypes.Structure):
     ]
 
 
+class LatentPool(ctypes.Structure):
+    _fields_ = [
+        ("data", _vp), ("n_pages", _i64), ("num_layers", _i32), ("latent_dim", _i32), ("rope_dim", _i32),
+        ("page_size", _i32),
+    ]
+
+
+class LatentRowsArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _i32), ("layer", _i32), ("dtype", _i32), ("_pad0", _i32),
+        ("pool", LatentPool), ("batch", PagedBatch),
+        ("latent", _vp), ("rope", _vp), ("latent_t", _i64), ("rope_t", _i64),
+    ]
+
+
+class LatentAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _i32), ("layer", _i32), ("H", _i32), ("q_dtype", _i32), ("causal", _i32),
+        ("sm_scale", ctypes.c_float),
+        ("pool", LatentPool), ("batch", PagedBatch),
+        ("q", _vp), ("q_rope", _vp), ("q_t", _i64), ("q_h", _i64), ("q_rope_t", _i64), ("q_rope_h", _i64),
+        ("out", _vp), ("lse", _vp), ("workspace", _vp), ("workspace_bytes", _i64),
+    ]
+
+
+class LatentPrefillArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _i32), ("layer", _i32), ("H", _i32), ("q_dtype", _i32), ("causal", _i32),
+        ("sm_scale", ctypes.c_float),
+        ("pool", LatentPool), ("batch", PagedBatch),
+        ("w", _vp), ("w_scale", _vp), ("q", _vp), ("q_t", _i64), ("q_h", _i64), ("out", _vp),
+        ("workspace", _vp), ("workspace_bytes", _i64),
+    ]
+
+
+class LatentImportanceArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _i32), ("layer", _i32), ("H", _i32), ("q_dtype", _i32), ("causal", _i32), ("q_window", _i32),
+        ("sm_scale", ctypes.c_float), ("decay", ctypes.c_float),
+        ("pool", LatentPool), ("batch", PagedBatch),
+        ("q", _vp), ("q_rope", _vp), ("q_t", _i64), ("q_h", _i64), ("q_rope_t", _i64), ("q_rope_h", _i64),
+        ("lse", _vp), ("scores", _vp), ("out", _vp),
+        ("n_scores", _i64), ("score_stride", _i64), ("out_stride", _i64),
+    ]
+
+
+class LatentCompactArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _i32), ("n_seqs", _i32), ("pool", LatentPool),
+        ("src_table", _vp), ("dst_table", _vp), ("src_stride", _i64), ("dst_stride", _i64),
+        ("src_width", _i32), ("dst_width", _i32), ("keep", _vp), ("n_keep", _vp),
+        ("keep_stride", _i64), ("max_keep", _i64),
+    ]
+
+
+class EvictArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _i32), ("n_seqs", _i32),
+        ("scores", _vp), ("n_scores", _i64), ("score_stride", _i64), ("lens", _vp), ("budgets", _vp), ("budget", _i64),
+        ("protect_initial", _i32), ("protect_recent", _i32), ("keep", _vp), ("n_keep", _vp), ("kept", _vp),
+        ("keep_stride", _i64), ("max_keep", _i64), ("kept_stride", _i64),
+    ]
+
+
 EXPORTS = (
     "akv_abi_version", "akv_last_error", "akv_struct_size",
     "akv_decode_workspace_bytes", "akv_decode_counter_bytes", "akv_decode_attn", "akv_decode_attn_noalloc",
@@ -205,9 +269,13 @@ EXPORTS = (
     "akv_timeline_words", "akv_timeline_fetch", "akv_timeline_clear",
     "akv_paged_append", "akv_paged_read", "akv_paged_attn_workspace_bytes", "akv_paged_attn",
     "akv_paged_importance", "akv_paged_copy", "akv_paged_compact",
+    "akv_latent_append", "akv_latent_read", "akv_latent_attn_workspace_bytes", "akv_latent_attn",
+    "akv_latent_prefill_workspace_bytes", "akv_latent_prefill", "akv_latent_importance", "akv_latent_copy",
+    "akv_latent_compact", "akv_evict_select",
 )
 STRUCTS = (WarmDesc, DecodeArgs, QuantArgs, DequantArgs, ImportanceArgs, PrefillArgs, RowsJob, KiviSide,
-           PagedPool, PagedBatch, PagedRowsArgs, PagedAttnArgs, PagedImportanceArgs, PagedCompactArgs)
+           PagedPool, PagedBatch, PagedRowsArgs, PagedAttnArgs, PagedImportanceArgs, PagedCompactArgs,
+           LatentPool, LatentRowsArgs, LatentAttnArgs, LatentPrefillArgs, LatentImportanceArgs, LatentCompactArgs, EvictArgs)
 
 _lib: Optional[ctypes.CDLL] = None
 
@@ -275,13 +343,17 @@ def load() -> ctypes.CDLL:
     lib.akv_timeline_clear.restype = ctypes.c_int
     lib.akv_timeline_clear.argtypes = [_vp]
     # their structs as addresses: callers pack them as bytes or fill the mirrors
-    for name in ("akv_paged_append", "akv_paged_read", "akv_paged_attn", "akv_paged_importance", "akv_paged_compact"):
+    for name in ("akv_paged_append", "akv_paged_read", "akv_paged_attn", "akv_paged_importance", "akv_paged_compact",
+                 "akv_latent_append", "akv_latent_read", "akv_latent_attn", "akv_latent_prefill", "akv_latent_importance",
+                 "akv_latent_compact", "akv_evict_select"):
         getattr(lib, name).restype = ctypes.c_int
         getattr(lib, name).argtypes = [_vp, _vp]
-    lib.akv_paged_attn_workspace_bytes.restype = _i64
-    lib.akv_paged_attn_workspace_bytes.argtypes = [_vp]
-    lib.akv_paged_copy.restype = ctypes.c_int
-    lib.akv_paged_copy.argtypes = [_vp, _vp, _vp, _i64, _vp]
+    for name in ("akv_paged_attn_workspace_bytes", "akv_latent_attn_workspace_bytes", "akv_latent_prefill_workspace_bytes"):
+        getattr(lib, name).restype = _i64
+        getattr(lib, name).argtypes = [_vp]
+    for name in ("akv_paged_copy", "akv_latent_copy"):
+        getattr(lib, name).restype = ctypes.c_int
+        getattr(lib, name).argtypes = [_vp, _vp, _vp, _i64, _vp]
     if lib.akv_abi_version() != ABI_VERSION:
         raise RuntimeError(f"{LIB_PATH} has ABI {lib.akv_abi_version()}, expected {ABI_VERSION}")
     for i, st in enumerate(STRUCTS):

@@ -13,6 +13,7 @@ when the work runs, so a call captured into a graph follows what is in them at e
   paged_importance  the running importance of the cached tokens
   copy_pages        pages duplicated in every layer
   compact_pages     sequences reduced to the tokens that stay, in every layer
+  evict_select      which tokens stay, by the attention that they gathered
 
 ``PackedPagedCache`` keeps the books: page allocation, forks that share pages and copy them
 when one side writes, compaction.  Everything runs in libakv_hip.so; there is no CPU path and
@@ -38,8 +39,9 @@ _ROWS = struct.Struct(f"@4i{_POOL}s{_BATCH}s6q")
 _ATTN = struct.Struct(f"@5if{_POOL}s{_BATCH}s7q")
 _IMPORTANCE = struct.Struct(f"@6i2f{_POOL}s{_BATCH}s9q")
 _COMPACT = struct.Struct(f"@2i{_POOL}s4q2i4q")
+_EVICT = struct.Struct("@2i6q2i6q")
 for _s, _c in ((_ROWS, nat.PagedRowsArgs), (_ATTN, nat.PagedAttnArgs), (_IMPORTANCE, nat.PagedImportanceArgs),
-               (_COMPACT, nat.PagedCompactArgs)):
+               (_COMPACT, nat.PagedCompactArgs), (_EVICT, nat.EvictArgs)):
     assert _s.size == ctypes.sizeof(_c), _c
 
 
@@ -92,8 +94,10 @@ class PagedPool:
         self._index = data.get_device()
         self._c = bytes(nat.PagedPool(data.data_ptr(), self.num_pages, self.num_layers, self.heads, head_dim,
                                       self.page_size, group_size, 0))
+        lib = nat.load()
+        self._copy, self._compact, self._compact_args = lib.akv_paged_copy, lib.akv_paged_compact, _COMPACT
         # every refusal of a pool's shape is the library's
-        nat.check(nat.load().akv_paged_copy(self._c, None, None, 0, None), "PagedPool")
+        nat.check(self._copy(self._c, None, None, 0, None), "PagedPool")
 
     @classmethod
     def empty(cls, num_layers: int, num_pages: int, heads: int, head_dim: int, page_size: int = 16,
@@ -260,20 +264,20 @@ def paged_importance(q: torch.Tensor, lse: torch.Tensor, pool: PagedPool, batch:
     return dst
 
 
-def copy_pages(pool: PagedPool, src: torch.Tensor, dst: torch.Tensor) -> None:
-    """Page dst[i] of every layer becomes a copy of page src[i].  int32 tensors on the pool's
-    device; no page may be written twice, or both read and written."""
+def copy_pages(pool, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Page dst[i] of every layer becomes a copy of page src[i].  ``pool`` is a PagedPool or a
+    PagedLatentPool; int32 tensors on its device; no page may be written twice, or both read and written."""
     _check_device(pool, src, dst)
     src, dst = _int32("src", src, 1), _int32("dst", dst, 1)
     if src.shape != dst.shape:
         raise ValueError("src and dst must be of one length")
-    _call(pool._index, "copy_pages", nat.load().akv_paged_copy, pool._c, src.data_ptr(), dst.data_ptr(), src.shape[0])
+    _call(pool._index, "copy_pages", pool._copy, pool._c, src.data_ptr(), dst.data_ptr(), src.shape[0])
 
 
-def compact_pages(pool: PagedPool, src_table: torch.Tensor, dst_table: torch.Tensor, keep: torch.Tensor,
+def compact_pages(pool, src_table: torch.Tensor, dst_table: torch.Tensor, keep: torch.Tensor,
                   n_keep: torch.Tensor) -> None:
     """Token j of sequence s on ``dst_table`` (S, W') becomes token ``keep[s, j]`` on
-    ``src_table`` (S, W), j < n_keep[s], in every layer.
+    ``src_table`` (S, W), j < n_keep[s], in every layer of a PagedPool or a PagedLatentPool.
 
     keep (S, K) and n_keep (S,) int32.  No slot that is read may be written, except tokens that
     stay where they are.  Slots behind the last token keep what they hold."""
@@ -283,10 +287,52 @@ def compact_pages(pool: PagedPool, src_table: torch.Tensor, dst_table: torch.Ten
     S = n_keep.shape[0]
     if src_table.shape[0] != S or dst_table.shape[0] != S or keep.shape[0] != S:
         raise ValueError(f"{S} sequences take {S} rows of src_table, dst_table and keep")
-    args = _COMPACT.pack(nat.ABI_VERSION, S, pool._c, src_table.data_ptr(), dst_table.data_ptr(), src_table.stride(0),
+    args = pool._compact_args.pack(nat.ABI_VERSION, S, pool._c, src_table.data_ptr(), dst_table.data_ptr(), src_table.stride(0),
                          dst_table.stride(0), src_table.shape[1], dst_table.shape[1], keep.data_ptr(), n_keep.data_ptr(),
                          keep.stride(0), keep.shape[1])
-    _call(pool._index, "compact_pages", nat.load().akv_paged_compact, args)
+    _call(pool._index, "compact_pages", pool._compact, args)
+
+
+def evict_select(scores: torch.Tensor, lens: torch.Tensor, budget: Union[int, torch.Tensor], protect_initial: int = 4,
+                 protect_recent: int = 16, max_keep: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Which tokens stay where each sequence is held to a budget, by the attention they gathered.
+
+    scores (S, N) float32, a sequence's consecutive: accumulated weights, as ``paged_importance`` and
+    ``latent_importance`` keep them; lens (S,) int32, at most N.  ``budget`` is a number of tokens, or (S,) int32 on the
+    device with ``max_keep`` the most it may say (N where that is not given).  The first ``protect_initial`` and
+    last ``protect_recent`` tokens stay before all others (where the budget does not hold those, the later ones), then those of the
+    highest score, NaN above all; of equal ones the lowest position leaves first.
+
+    Returns keep (S, K) int32, ascending positions, n_keep (S,) int32, as ``compact_pages`` takes them, and
+    the scores of the tokens that stay at their new positions, (S, N) float32; all three are 0 behind the last."""
+    nat.require_device(scores, lens)
+    if scores.dtype != torch.float32 or scores.dim() != 2:
+        raise ValueError("scores must be a (sequences, tokens) float32 tensor")
+    S, N = scores.shape
+    dev = scores.get_device()
+    lens = _int32("lens", lens, 1)
+    each = isinstance(budget, torch.Tensor)
+    if each:
+        nat.require_device(budget)
+        budget = _int32("budget", budget, 1)
+    K = min(N, N if max_keep is None else index(max_keep)) if each else min(N, index(budget), N if max_keep is None else index(max_keep))
+    for name, t in (("lens", lens),) + ((("budget", budget),) if each else ()):
+        if t.shape[0] != S:
+            raise ValueError(f"{S} sequences take {S} entries of {name}")
+        if t.get_device() != dev:
+            raise ValueError(f"{name} on {t.device} beside scores on {scores.device}")
+    if K < 0:
+        raise ValueError("a budget must be at least 0")
+    if N > 1 and scores.stride(1) != 1 or (S > 1 and scores.stride(0) < N):
+        scores = scores.contiguous()
+    out = torch.empty(S * (K + 1 + N), dtype=torch.int32, device=scores.device)
+    keep, n_keep, kept = out.split([S * K, S, S * N])
+    kept = kept.view(torch.float32)
+    args = _EVICT.pack(nat.ABI_VERSION, S, scores.data_ptr(), N, scores.stride(0), lens.data_ptr(),
+                       budget.data_ptr() if each else 0, 0 if each else min(index(budget), N), index(protect_initial), index(protect_recent),
+                       keep.data_ptr(), n_keep.data_ptr(), kept.data_ptr(), K, K, N)
+    _call(dev, "evict_select", nat.load().akv_evict_select, args)
+    return keep.view(S, K), n_keep, kept.view(S, N)
 
 
 class PageLedger:
@@ -427,21 +473,13 @@ class PageLedger:
         self.pages[seq], self.lens[seq] = old, length
 
 
-class PackedPagedCache:
-    """Sequences of one model in a pool of 4-bit pages, shared by all its layers.
+class _PagedCache:
+    """The books of sequences in a pool's pages: what ``PackedPagedCache`` and
+    ``PagedLatentCache`` share."""
 
-    A step: ``batch = cache.extend(seqs, counts)`` makes room (and copies the shared pages that
-    will be written), then per layer ``append`` and ``attention``.  ``fork`` shares a sequence's
-    pages; ``compact`` keeps chosen tokens; ``crop`` drops the last ones; ``remove`` frees.
-    Calls that raise leave the cache as it was (a compaction in turns, the turns that are done).
-    Work goes to the current stream."""
-
-    def __init__(self, num_layers: int, num_heads: int, head_dim: int, page_size: int = 16, max_pages: int = 4096,
-                 group_size: int = 32, device="cuda"):
-        if torch.device(device).type != "cuda":
-            raise RuntimeError("PackedPagedCache lives on the GPU (device 'cuda')")
-        self.pool = PagedPool.empty(num_layers, max_pages, num_heads, head_dim, page_size, group_size, device)
-        self._book = PageLedger(max_pages, page_size)
+    def __init__(self, pool, max_pages: int):
+        self.pool = pool
+        self._book = PageLedger(max_pages, pool.page_size)
 
     # ---- sequences
     def add_sequence(self) -> int:
@@ -497,23 +535,6 @@ class PackedPagedCache:
             raise
         return batch
 
-    # ---- a layer's work
-    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, batch: PagedBatch) -> None:
-        paged_append(self.pool, batch, k, v, layer)
-
-    def attention(self, layer: int, q: torch.Tensor, batch: PagedBatch, sm_scale: Optional[float] = None,
-                  causal: bool = True, return_lse: bool = False):
-        return paged_attention(q, self.pool, batch, layer, sm_scale, causal, return_lse)
-
-    def importance(self, layer: int, q: torch.Tensor, lse: torch.Tensor, batch: PagedBatch, scores: torch.Tensor,
-                   decay: float = 0.9, q_window: int = 0, sm_scale: Optional[float] = None, causal: bool = True) -> torch.Tensor:
-        return paged_importance(q, lse, self.pool, batch, scores, layer, decay, q_window, sm_scale, causal)
-
-    def get_kv(self, layer: int, seq: int, dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
-        """A sequence's keys and values (heads, length, head_dim) as the cache holds them."""
-        k, v = paged_read(self.pool, self._batch([seq], [self.get_seq_length(seq)]), layer, dtype)
-        return k.transpose(0, 1), v.transpose(0, 1)
-
     # ---- compaction
     def compact(self, seqs: Sequence[int], keep: Sequence[torch.Tensor]) -> None:
         """Sequence ``seqs[i]`` keeps the tokens at positions ``keep[i]`` (ascending integers on
@@ -535,6 +556,12 @@ class PackedPagedCache:
             at, end = torch.cat(list(keep)), n.repeat_interleave(c, output_size=sum(counts))
             if bool(((at < 0) | (at >= end)).any()):
                 raise ValueError("keep names a position that is not one of its sequence's tokens")
+        self._move(seqs, counts, groups, lambda group: torch.nn.utils.rnn.pad_sequence(
+            [keep[i].to(torch.int32) for i in group], batch_first=True))
+
+    def _move(self, seqs: Sequence[int], counts: Sequence[int], groups, rows) -> None:
+        """The compaction of the groups of ``plan_compaction``; rows(group): the positions that stay."""
+        book = self._book
         for group in groups:
             lens = [book.lens[seqs[i]] for i in group]
             moved = [book.replace(seqs[i], counts[i]) for i in group]
@@ -542,11 +569,67 @@ class PackedPagedCache:
                 old, wo = self._table([a for a, _ in moved])
                 new, wn = self._table([b for _, b in moved])
                 t_old, t_new, n = self._upload(old, new, [counts[i] for i in group])
-                rows = torch.nn.utils.rnn.pad_sequence([keep[i].to(torch.int32) for i in group], batch_first=True)
-                compact_pages(self.pool, t_old.view(len(group), wo), t_new.view(len(group), wn), rows, n)
+                compact_pages(self.pool, t_old.view(len(group), wo), t_new.view(len(group), wn), rows(group), n)
             except BaseException:
                 for i, (a, _), n in zip(group, moved, lens):
                     book.undo_replace(seqs[i], a, n)
                 raise
             for a, _ in moved:
                 book._drop(a)
+
+    def evict(self, seqs: Sequence[int], scores: torch.Tensor, budget: int, protect_initial: int = 4,
+              protect_recent: int = 16) -> torch.Tensor:
+        """Hold each sequence to ``budget`` tokens: those past it that gathered the least attention leave,
+        in every layer, by ``evict_select``'s rule.  scores (len(seqs), N) float32, N at least the longest
+        sequence's length: the running importance of their tokens.  Returns it for the tokens that stay, at
+        their new positions and 0 behind them.
+
+        Nothing waits for the device.  Tokens move as in ``compact``; sequences within the budget stay as they are."""
+        book = self._book
+        book._known(seqs)
+        budget, lens = index(budget), [book.lens[s] for s in seqs]
+        if budget < 0:
+            raise ValueError("a budget must be at least 0")
+        if scores.dim() != 2 or scores.shape[0] != len(seqs) or scores.shape[1] < max(lens, default=0):
+            raise ValueError(f"scores must be ({len(seqs)}, {max(lens, default=0)} or more)")
+        _check_device(self.pool, scores)
+        over = [i for i, n in enumerate(lens) if n > budget]
+        groups = book.plan_compaction([seqs[i] for i in over], [budget] * len(over))
+        keep, _, kept = evict_select(scores, self._upload(lens)[0], budget, protect_initial, protect_recent)
+        self._move([seqs[i] for i in over], [budget] * len(over), groups,
+                   lambda group: keep[self._upload([over[i] for i in group])[0].long()])
+        return kept
+
+
+class PackedPagedCache(_PagedCache):
+    """Sequences of one model in a pool of 4-bit pages, shared by all its layers.
+
+    A step: ``batch = cache.extend(seqs, counts)`` makes room (and copies the shared pages that
+    will be written), then per layer ``append`` and ``attention``.  ``fork`` shares a sequence's
+    pages; ``compact`` keeps chosen tokens, ``evict`` those that gathered the most attention;
+    ``crop`` drops the last ones; ``remove`` frees.
+    Calls that raise leave the cache as it was (a compaction in turns, the turns that are done).
+    Work goes to the current stream."""
+
+    def __init__(self, num_layers: int, num_heads: int, head_dim: int, page_size: int = 16, max_pages: int = 4096,
+                 group_size: int = 32, device="cuda"):
+        if torch.device(device).type != "cuda":
+            raise RuntimeError("PackedPagedCache lives on the GPU (device 'cuda')")
+        super().__init__(PagedPool.empty(num_layers, max_pages, num_heads, head_dim, page_size, group_size, device), max_pages)
+
+    # ---- a layer's work
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, batch: PagedBatch) -> None:
+        paged_append(self.pool, batch, k, v, layer)
+
+    def attention(self, layer: int, q: torch.Tensor, batch: PagedBatch, sm_scale: Optional[float] = None,
+                  causal: bool = True, return_lse: bool = False):
+        return paged_attention(q, self.pool, batch, layer, sm_scale, causal, return_lse)
+
+    def importance(self, layer: int, q: torch.Tensor, lse: torch.Tensor, batch: PagedBatch, scores: torch.Tensor,
+                   decay: float = 0.9, q_window: int = 0, sm_scale: Optional[float] = None, causal: bool = True) -> torch.Tensor:
+        return paged_importance(q, lse, self.pool, batch, scores, layer, decay, q_window, sm_scale, causal)
+
+    def get_kv(self, layer: int, seq: int, dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
+        """A sequence's keys and values (heads, length, head_dim) as the cache holds them."""
+        k, v = paged_read(self.pool, self._batch([seq], [self.get_seq_length(seq)]), layer, dtype)
+        return k.transpose(0, 1), v.transpose(0, 1)

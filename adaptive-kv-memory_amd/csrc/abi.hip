@@ -12,6 +12,7 @@
 #include "prefill.h"
 #include "misc.h"
 #include "paged.h"
+#include "latent.h"
 #include "quant.h"
 #include "rows.h"
 
@@ -320,6 +321,13 @@ int64_t akv_struct_size(int32_t which) {
         case 11: return (int64_t)sizeof(akv_paged_attn_args);
         case 12: return (int64_t)sizeof(akv_paged_importance_args);
         case 13: return (int64_t)sizeof(akv_paged_compact_args);
+        case 14: return (int64_t)sizeof(akv_latent_pool);
+        case 15: return (int64_t)sizeof(akv_latent_rows_args);
+        case 16: return (int64_t)sizeof(akv_latent_attn_args);
+        case 17: return (int64_t)sizeof(akv_latent_prefill_args);
+        case 18: return (int64_t)sizeof(akv_latent_importance_args);
+        case 19: return (int64_t)sizeof(akv_latent_compact_args);
+        case 20: return (int64_t)sizeof(akv_evict_args);
         default: return -1;
     }
 }
@@ -804,16 +812,16 @@ int akv_stream_read(const void *data, int64_t bytes, uint32_t *sink, void *strea
     return ok();
 }
 
-int akv_select_demote(const float *scores, int64_t rows, int64_t len, int64_t n_demote, int32_t protect_first,
-                      int32_t protect_last, int64_t *out, void *stream) {
+int akv_select_demote(const float *scores, int64_t rows, int64_t len, int64_t n_demote, int32_t protect_initial,
+                      int32_t protect_recent, int64_t *out, void *stream) {
     if (rows < 0 || len < 0 || n_demote < 0) return fail(AKV_E_SHAPE, "negative size");
     if (n_demote > len) return fail(AKV_E_SHAPE, "n_demote (%lld) > len (%lld)", (long long)n_demote, (long long)len);
-    if (protect_first < 0 || protect_last < 0) return fail(AKV_E_SHAPE, "negative protection");
+    if (protect_initial < 0 || protect_recent < 0) return fail(AKV_E_SHAPE, "negative protection");
     if (rows == 0 || n_demote == 0) return ok();
     if (!scores || !out) return fail(AKV_E_INVALID, "scores and out are required");
     if (!aligned16(scores) || !aligned16(out)) return fail(AKV_E_ALIGN, "scores/out must be 16-byte aligned");
     if (len >= ((int64_t)1 << 31)) return fail(AKV_E_SHAPE, "len too large");
-    hipError_t e = akv::select_launch(scores, rows, len, n_demote, protect_first, protect_last, out, (hipStream_t)stream);
+    hipError_t e = akv::select_launch(scores, rows, len, n_demote, protect_initial, protect_recent, out, (hipStream_t)stream);
     if (e != hipSuccess) return hip_fail(e, "select launch");
     return ok();
 }
@@ -943,26 +951,38 @@ static int64_t paged_page_bytes(const akv_paged_pool &p) {
 
 static bool aligned4(const void *p) { return ((uintptr_t)p & 3u) == 0; }
 
-// The pool and batch of a call as the kernels see them.
-static int paged_views(int32_t abi, int32_t layer, const akv_paged_pool &p, const akv_paged_batch &b, akv::PagedView *v,
-                       akv::PagedSeqs *s) {
-    if (abi != AKV_ABI_VERSION) return fail(AKV_E_ABI, "ABI mismatch");
-    const int rc = check_paged_pool(p);
-    if (rc != AKV_OK) return rc;
-    if (layer < 0 || layer >= p.num_layers) return fail(AKV_E_SHAPE, "layer %d of %d", layer, p.num_layers);
+// The batch of a call over pages of page_size tokens as the kernels see it.
+static int paged_seqs(int32_t layer, int32_t layers, int32_t page_size, const akv_paged_batch &b, akv::PagedSeqs *s) {
+    if (layer < 0 || layer >= layers) return fail(AKV_E_SHAPE, "layer %d of %d", layer, layers);
     if (b.n_seqs < 0 || b.n_seqs > 65535) return fail(AKV_E_SHAPE, "0 to 65535 sequences");
     if (b.table_width < 0 || (b.n_seqs > 1 && b.table_stride < b.table_width)) return fail(AKV_E_SHAPE, "bad page table");
     if (b.n_tokens < 0 || b.n_tokens >= ((int64_t)1 << 31) || b.max_q < 0) return fail(AKV_E_SHAPE, "bad row counts");
-    if ((int64_t)b.table_width * p.page_size >= ((int64_t)1 << 31)) return fail(AKV_E_SHAPE, "sequences of 2^31 tokens or more");
+    if ((int64_t)b.table_width * page_size >= ((int64_t)1 << 31)) return fail(AKV_E_SHAPE, "sequences of 2^31 tokens or more");
     if (b.n_seqs > 0 && (!b.kv_lens || !b.q_starts || (b.table_width > 0 && !b.page_table)))
         return fail(AKV_E_INVALID, "null pointer in the batch");
     if (!aligned4(b.page_table) || !aligned4(b.kv_lens) || !aligned4(b.q_starts))
         return fail(AKV_E_ALIGN, "the batch's arrays must be 4-byte aligned");
-    int log_tpp = 0;
-    while ((16 << log_tpp) < p.page_size) ++log_tpp;
-    const int64_t page = paged_page_bytes(p);
-    *v = akv::PagedView{(unsigned char *)p.data + layer * p.n_pages * page, page, (uint32_t)p.n_pages, p.heads, log_tpp};
     *s = akv::PagedSeqs{b.page_table, b.kv_lens, b.q_starts, b.table_stride, b.n_tokens, b.n_seqs, b.table_width, b.max_q};
+    return AKV_OK;
+}
+
+static int log2_of(int x) {
+    int n = 0;
+    while ((1 << n) < x) ++n;
+    return n;
+}
+
+// The pool and batch of a call as the kernels see them.
+static int paged_views(int32_t abi, int32_t layer, const akv_paged_pool &p, const akv_paged_batch &b, akv::PagedView *v,
+                       akv::PagedSeqs *s) {
+    if (abi != AKV_ABI_VERSION) return fail(AKV_E_ABI, "ABI mismatch");
+    int rc = check_paged_pool(p);
+    if (rc != AKV_OK) return rc;
+    rc = paged_seqs(layer, p.num_layers, p.page_size, b, s);
+    if (rc != AKV_OK) return rc;
+    const int64_t page = paged_page_bytes(p);
+    *v = akv::PagedView{(unsigned char *)p.data + layer * p.n_pages * page, page, (uint32_t)p.n_pages, p.heads,
+                        log2_of(p.page_size / 16)};
     return AKV_OK;
 }
 
@@ -1140,6 +1160,256 @@ int akv_paged_importance(const akv_paged_importance_args *a, void *stream) {
     p.n_scores = a->n_scores; p.score_stride = a->score_stride; p.out_stride = a->out_stride;
     hipError_t e = akv::paged_importance_launch(p, (hipStream_t)stream);
     if (e != hipSuccess) return hip_fail(e, "paged importance launch");
+    return ok();
+}
+
+// ------------------------------------------------------------------ paged latent cache
+
+static int check_latent_pool(const akv_latent_pool &p) {
+    if (p.latent_dim != 256 && p.latent_dim != 512) return fail(AKV_E_UNSUPPORTED, "latent_dim 256 or 512, got %d", p.latent_dim);
+    if (p.rope_dim != akv::kLatentRope) return fail(AKV_E_UNSUPPORTED, "rope_dim %d, got %d", akv::kLatentRope, p.rope_dim);
+    if (p.page_size < 16 || p.page_size > 256 || !pow2(p.page_size))
+        return fail(AKV_E_UNSUPPORTED, "page_size a power of two from 16 to 256, got %d", p.page_size);
+    if (p.num_layers < 1 || p.num_layers > 65535 || p.n_pages < 0 || p.n_pages >= ((int64_t)1 << 31))
+        return fail(AKV_E_SHAPE, "bad pool sizes");
+    if (p.n_pages > 0 && !p.data) return fail(AKV_E_INVALID, "the pool's data is NULL");
+    if (!aligned16(p.data)) return fail(AKV_E_ALIGN, "the pool must be 16-byte aligned");
+    return AKV_OK;
+}
+
+static akv::LatentView latent_view(const akv_latent_pool &p, int32_t layer) {
+    const int row = 2 * (p.latent_dim + p.rope_dim);
+    const int64_t page = (int64_t)p.page_size * row;
+    return {(unsigned char *)p.data + layer * p.n_pages * page, page, (uint32_t)p.n_pages, log2_of(p.page_size), row};
+}
+
+static int latent_views(int32_t abi, int32_t layer, const akv_latent_pool &p, const akv_paged_batch &b, akv::LatentView *v,
+                        akv::PagedSeqs *s) {
+    if (abi != AKV_ABI_VERSION) return fail(AKV_E_ABI, "ABI mismatch");
+    int rc = check_latent_pool(p);
+    if (rc != AKV_OK) return rc;
+    rc = paged_seqs(layer, p.num_layers, p.page_size, b, s);
+    if (rc != AKV_OK) return rc;
+    *v = latent_view(p, layer);
+    return AKV_OK;
+}
+
+static int latent_rows_params(const akv_latent_rows_args *a, akv::LatentRowsParams *p) {
+    if (!a) return fail(AKV_E_INVALID, "args is NULL");
+    const int rc = latent_views(a->abi_version, a->layer, a->pool, a->batch, &p->pool, &p->seqs);
+    if (rc != AKV_OK) return rc;
+    if (a->dtype < 0 || a->dtype > 2) return fail(AKV_E_DTYPE, "float16, bfloat16 or float32 rows");
+    if (a->batch.n_tokens > 0 && (!a->latent || !a->rope)) return fail(AKV_E_INVALID, "latent and rope are required");
+    if (!aligned16(a->latent) || !aligned16(a->rope) || ((a->latent_t | a->rope_t) & 15))
+        return fail(AKV_E_ALIGN, "rows must be 16-byte aligned");
+    p->Dc = a->pool.latent_dim; p->dt = a->dtype;
+    p->latent = (unsigned char *)a->latent; p->rope = (unsigned char *)a->rope;
+    p->latent_t = a->latent_t; p->rope_t = a->rope_t;
+    return AKV_OK;
+}
+
+int akv_latent_append(const akv_latent_rows_args *a, void *stream) {
+    akv::LatentRowsParams p{};
+    const int rc = latent_rows_params(a, &p);
+    if (rc != AKV_OK) return rc;
+    hipError_t e = akv::latent_append_launch(p, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "latent append launch");
+    return ok();
+}
+
+int akv_latent_read(const akv_latent_rows_args *a, void *stream) {
+    akv::LatentRowsParams p{};
+    const int rc = latent_rows_params(a, &p);
+    if (rc != AKV_OK) return rc;
+    hipError_t e = akv::latent_read_launch(p, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "latent read launch");
+    return ok();
+}
+
+// Shared by both forms of the attention and the importance.
+static int check_latent_queries(int32_t H, int32_t dt, float sm_scale, const akv_paged_batch &b, const void *q, const void *qr,
+                                int64_t strides) {
+    if (dt != AKV_DT_F16 && dt != AKV_DT_BF16) return fail(AKV_E_DTYPE, "float16 or bfloat16 queries");
+    if (H < 1 || H > 65535) return fail(AKV_E_SHAPE, "%d query heads", H);
+    if (!(sm_scale > 0.0f) || !std::isfinite(sm_scale)) return fail(AKV_E_INVALID, "sm_scale must be positive");
+    if (b.n_tokens > 0 && (!q || !qr)) return fail(AKV_E_INVALID, "queries are required");
+    if (!aligned16(q) || !aligned16(qr) || (strides & 15)) return fail(AKV_E_ALIGN, "query rows must be 16-byte aligned");
+    if ((int64_t)b.max_q * H >= ((int64_t)1 << 27)) return fail(AKV_E_SHAPE, "too many rows a sequence");
+    return AKV_OK;
+}
+
+static int latent_attn_params(const akv_latent_attn_args *a, akv::LatentAttnParams *p, int64_t *bytes) {
+    if (!a) return fail(AKV_E_INVALID, "args is NULL");
+    int rc = latent_views(a->abi_version, a->layer, a->pool, a->batch, &p->pool, &p->seqs);
+    if (rc != AKV_OK) return rc;
+    rc = check_latent_queries(a->H, a->q_dtype, a->sm_scale, a->batch, a->q, a->q_rope, a->q_t | a->q_h | a->q_rope_t | a->q_rope_h);
+    if (rc != AKV_OK) return rc;
+    // units of 64 tokens of a tile of at least 16 rows are counted in 31 bits
+    const double cap = (double)a->batch.table_width * a->pool.page_size, rows = (double)a->batch.max_q * a->H;
+    if ((cap / 64 + 4) * (rows / 16 + 1) * a->batch.n_seqs >= 0x1p30) return fail(AKV_E_SHAPE, "too much for one call");
+    p->Dc = a->pool.latent_dim; p->H = a->H;
+    p->q_bf16 = a->q_dtype == AKV_DT_BF16; p->causal = a->causal != 0;
+    p->scale_log2 = a->sm_scale * 1.4426950408889634f;
+    p->q = (const unsigned char *)a->q; p->qr = (const unsigned char *)a->q_rope;
+    p->q_t = a->q_t; p->q_h = a->q_h; p->qr_t = a->q_rope_t; p->qr_h = a->q_rope_h;
+    p->out = a->out; p->lse = a->lse; p->sums = (int *)a->workspace;
+    *bytes = akv::latent_attn_plan(p);
+    return AKV_OK;
+}
+
+int64_t akv_latent_attn_workspace_bytes(const akv_latent_attn_args *a) {
+    akv::LatentAttnParams p{};
+    int64_t bytes;
+    return latent_attn_params(a, &p, &bytes) == AKV_OK ? bytes : -1;
+}
+
+int akv_latent_attn(const akv_latent_attn_args *a, void *stream) {
+    akv::LatentAttnParams p{};
+    int64_t bytes;
+    const int rc = latent_attn_params(a, &p, &bytes);
+    if (rc != AKV_OK) return rc;
+    if (a->batch.n_tokens == 0) return ok();
+    if (!a->out) return fail(AKV_E_INVALID, "out is required");
+    if (!aligned16(a->out) || !aligned4(a->lse)) return fail(AKV_E_ALIGN, "out must be 16-byte aligned");
+    if (!a->workspace || a->workspace_bytes < bytes) return fail(AKV_E_WORKSPACE, "workspace of %lld bytes needed", (long long)bytes);
+    if (!aligned16(a->workspace)) return fail(AKV_E_ALIGN, "workspace must be 16-byte aligned");
+    hipError_t e = akv::latent_attn_launch(p, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "latent attention launch");
+    return ok();
+}
+
+static int latent_prefill_params(const akv_latent_prefill_args *a, akv::LatentPrefillParams *p, int64_t *bytes) {
+    if (!a) return fail(AKV_E_INVALID, "args is NULL");
+    int rc = latent_views(a->abi_version, a->layer, a->pool, a->batch, &p->pool, &p->seqs);
+    if (rc != AKV_OK) return rc;
+    rc = check_latent_queries(a->H, a->q_dtype, a->sm_scale, a->batch, a->q, a->q, a->q_t | a->q_h);
+    if (rc != AKV_OK) return rc;
+    if (!a->w || !a->w_scale) return fail(AKV_E_INVALID, "weights are required");
+    if (!aligned16(a->w) || !aligned16(a->w_scale)) return fail(AKV_E_ALIGN, "weights must be 16-byte aligned");
+    p->Dc = a->pool.latent_dim; p->H = a->H;
+    p->q_bf16 = a->q_dtype == AKV_DT_BF16; p->causal = a->causal != 0;
+    p->scale_log2 = a->sm_scale * 1.4426950408889634f;
+    p->q = (const unsigned char *)a->q; p->q_t = a->q_t; p->q_h = a->q_h;
+    p->w = (const unsigned char *)a->w; p->w_scale = a->w_scale;
+    p->out = a->out; p->sums = (int64_t *)a->workspace;
+    *bytes = akv::latent_prefill_plan(p);
+    return AKV_OK;
+}
+
+int64_t akv_latent_prefill_workspace_bytes(const akv_latent_prefill_args *a) {
+    akv::LatentPrefillParams p{};
+    int64_t bytes;
+    return latent_prefill_params(a, &p, &bytes) == AKV_OK ? bytes : -1;
+}
+
+int akv_latent_prefill(const akv_latent_prefill_args *a, void *stream) {
+    akv::LatentPrefillParams p{};
+    int64_t bytes;
+    const int rc = latent_prefill_params(a, &p, &bytes);
+    if (rc != AKV_OK) return rc;
+    if (a->batch.n_tokens == 0) return ok();
+    if (!a->out) return fail(AKV_E_INVALID, "out is required");
+    if (!aligned16(a->out)) return fail(AKV_E_ALIGN, "out must be 16-byte aligned");
+    if (!a->workspace || a->workspace_bytes < bytes) return fail(AKV_E_WORKSPACE, "workspace of %lld bytes needed", (long long)bytes);
+    if (!aligned16(a->workspace)) return fail(AKV_E_ALIGN, "workspace must be 16-byte aligned");
+    hipError_t e = akv::latent_prefill_launch(p, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "latent prefill launch");
+    return ok();
+}
+
+int akv_latent_importance(const akv_latent_importance_args *a, void *stream) {
+    if (!a) return fail(AKV_E_INVALID, "args is NULL");
+    akv::LatentImportanceParams p{};
+    int rc = latent_views(a->abi_version, a->layer, a->pool, a->batch, &p.pool, &p.seqs);
+    if (rc != AKV_OK) return rc;
+    rc = check_latent_queries(a->H, a->q_dtype, a->sm_scale, a->batch, a->q, a->q_rope, a->q_t | a->q_h | a->q_rope_t | a->q_rope_h);
+    if (rc != AKV_OK) return rc;
+    if (a->q_window < 0) return fail(AKV_E_SHAPE, "q_window must be >= 0");
+    if (a->n_scores < 0 || a->n_scores >= ((int64_t)1 << 31) ||
+        (a->batch.n_seqs > 1 && (a->score_stride < a->n_scores || a->out_stride < a->n_scores)))
+        return fail(AKV_E_SHAPE, "bad score rows");
+    if (a->batch.n_seqs == 0 || a->n_scores == 0) return ok();
+    if (!a->scores || !a->out || (a->batch.n_tokens > 0 && !a->lse)) return fail(AKV_E_INVALID, "scores, out and lse are required");
+    if (!aligned4(a->scores) || !aligned4(a->out)) return fail(AKV_E_ALIGN, "float32 rows must be 4-byte aligned");
+    if (rows_clash(a->scores, a->score_stride, a->out, a->out_stride, a->n_scores, a->batch.n_seqs))
+        return fail(AKV_E_SHAPE, "out must be scores or not overlap it");
+    if (!aligned4(a->lse)) return fail(AKV_E_ALIGN, "lse must be 4-byte aligned");
+    p.Dc = a->pool.latent_dim; p.H = a->H;
+    p.q_bf16 = a->q_dtype == AKV_DT_BF16; p.causal = a->causal != 0; p.q_window = a->q_window;
+    p.scale_log2 = a->sm_scale * 1.4426950408889634f; p.decay = a->decay;
+    p.q = (const unsigned char *)a->q; p.qr = (const unsigned char *)a->q_rope;
+    p.q_t = a->q_t; p.q_h = a->q_h; p.qr_t = a->q_rope_t; p.qr_h = a->q_rope_h;
+    p.lse = a->lse; p.scores = a->scores; p.out = a->out;
+    p.n_scores = a->n_scores; p.score_stride = a->score_stride; p.out_stride = a->out_stride;
+    hipError_t e = akv::latent_importance_launch(p, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "latent importance launch");
+    return ok();
+}
+
+int akv_latent_copy(const akv_latent_pool *pool, const int32_t *src, const int32_t *dst, int64_t n, void *stream) {
+    if (!pool) return fail(AKV_E_INVALID, "pool is NULL");
+    const int rc = check_latent_pool(*pool);
+    if (rc != AKV_OK) return rc;
+    if (n < 0 || n > pool->n_pages) return fail(AKV_E_SHAPE, "%lld pairs in a pool of %lld pages", (long long)n, (long long)pool->n_pages);
+    if (n > 0 && (!src || !dst)) return fail(AKV_E_INVALID, "src and dst are required");
+    if (!aligned4(src) || !aligned4(dst)) return fail(AKV_E_ALIGN, "src and dst must be 4-byte aligned");
+    const akv::PagedCopyParams p{(unsigned char *)pool->data, latent_view(*pool, 0).page_bytes, pool->n_pages, n, pool->num_layers, src, dst};
+    hipError_t e = akv::paged_copy_launch(p, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "latent copy launch");
+    return ok();
+}
+
+int akv_latent_compact(const akv_latent_compact_args *a, void *stream) {
+    if (!a) return fail(AKV_E_INVALID, "args is NULL");
+    if (a->abi_version != AKV_ABI_VERSION) return fail(AKV_E_ABI, "ABI mismatch");
+    const int rc = check_latent_pool(a->pool);
+    if (rc != AKV_OK) return rc;
+    if (a->n_seqs < 0 || a->n_seqs > 65535) return fail(AKV_E_SHAPE, "0 to 65535 sequences");
+    if (a->src_width < 0 || a->dst_width < 0 || a->max_keep < 0 || a->max_keep >= ((int64_t)1 << 31) ||
+        (a->n_seqs > 1 && (a->src_stride < a->src_width || a->dst_stride < a->dst_width || a->keep_stride < a->max_keep)))
+        return fail(AKV_E_SHAPE, "bad tables");
+    if ((int64_t)a->src_width * a->pool.page_size >= ((int64_t)1 << 31) ||
+        (int64_t)a->dst_width * a->pool.page_size >= ((int64_t)1 << 31))
+        return fail(AKV_E_SHAPE, "sequences of 2^31 tokens or more");
+    if (a->n_seqs > 0 && a->max_keep > 0 &&
+        (!a->keep || !a->n_keep || (a->src_width > 0 && !a->src_table) || (a->dst_width > 0 && !a->dst_table)))
+        return fail(AKV_E_INVALID, "null pointer");
+    if (!aligned4(a->src_table) || !aligned4(a->dst_table) || !aligned4(a->keep) || !aligned4(a->n_keep))
+        return fail(AKV_E_ALIGN, "tables and lists must be 4-byte aligned");
+    akv::LatentCompactParams p{};
+    p.pool = latent_view(a->pool, 0);
+    p.layer_bytes = p.pool.page_bytes * a->pool.n_pages;
+    p.layers = a->pool.num_layers; p.n_seqs = a->n_seqs;
+    p.src_table = a->src_table; p.dst_table = a->dst_table;
+    p.src_stride = a->src_stride; p.dst_stride = a->dst_stride;
+    p.src_width = a->src_width; p.dst_width = a->dst_width;
+    p.keep = a->keep; p.n_keep = a->n_keep; p.keep_stride = a->keep_stride; p.max_keep = a->max_keep;
+    hipError_t e = akv::latent_compact_launch(p, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "latent compact launch");
+    return ok();
+}
+
+int akv_evict_select(const akv_evict_args *a, void *stream) {
+    if (!a) return fail(AKV_E_INVALID, "args is NULL");
+    if (a->abi_version != AKV_ABI_VERSION) return fail(AKV_E_ABI, "ABI mismatch");
+    if (a->n_seqs < 0 || a->n_seqs > 65535) return fail(AKV_E_SHAPE, "0 to 65535 sequences");
+    if (a->n_scores < 0 || a->n_scores >= ((int64_t)1 << 31) || a->max_keep < 0 || a->max_keep >= ((int64_t)1 << 31) ||
+        (a->n_seqs > 1 && (a->score_stride < a->n_scores || a->keep_stride < a->max_keep || (a->kept && a->kept_stride < a->n_scores))))
+        return fail(AKV_E_SHAPE, "bad rows of scores or positions");
+    if (a->protect_initial < 0 || a->protect_recent < 0) return fail(AKV_E_SHAPE, "protect_initial and protect_recent must be >= 0");
+    if (!a->budgets && a->budget < 0) return fail(AKV_E_SHAPE, "a budget must be >= 0");
+    if (a->n_seqs == 0) return ok();
+    if (!a->lens || !a->n_keep || (a->n_scores > 0 && !a->scores) || (a->max_keep > 0 && !a->keep)) return fail(AKV_E_INVALID, "null pointer");
+    if (!aligned4(a->scores) || !aligned4(a->lens) || !aligned4(a->budgets) || !aligned4(a->keep) || !aligned4(a->n_keep) || !aligned4(a->kept))
+        return fail(AKV_E_ALIGN, "arrays must be 4-byte aligned");
+    if (a->kept && a->n_scores > 0) {
+        const float *e0 = a->scores + (a->n_seqs - 1) * a->score_stride + a->n_scores, *e1 = a->kept + (a->n_seqs - 1) * a->kept_stride + a->n_scores;
+        if (a->kept < e0 && a->scores < e1) return fail(AKV_E_SHAPE, "kept must not overlap scores");
+    }
+    const akv::EvictParams p{a->scores, a->n_scores, a->score_stride, a->lens, a->budgets, a->budget, a->n_seqs, a->protect_initial,
+                             a->protect_recent, a->keep, a->n_keep, a->kept, a->keep_stride, a->max_keep, a->kept_stride};
+    hipError_t e = akv::evict_launch(p, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "evict launch");
     return ok();
 }
 

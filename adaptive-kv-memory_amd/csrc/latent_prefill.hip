@@ -1,0 +1,536 @@
+// Attention over the paged latent cache in its expanded form, for chunks of a prompt.
+//
+// The mathematics.  Head h's keys are k = [W_k,h c | r] and its values v = W_v,h c of a cached row
+// (latent c, rotated key r).  A row and token cost 2 (Dn + Dr + Dv) operations a head once they are
+// made, against 2 (2 Dc + Dr) where the latent itself is key and value; making them costs 2 Dc (Dn + Dv) a
+// token and head, which some 170 query tokens outweigh.  Two kernels: the expansion is a matrix product
+// whose left side stays in LDS for all heads, the attention streams its results.  Keys and values are
+// float16 over a power of two for each channel (which goes to the queries and the outputs, so that small weights
+// keep their bits), query rows float16 scaled by a power of two, p one float16; scores, sums and the softmax
+// state are float32.
+#include <algorithm>
+#include <type_traits>
+
+#include "akv_common.h"
+#include "latent.h"
+#include "latent_device.h"
+
+namespace akv {
+namespace {
+
+constexpr int kD = kLatentHead;       // channels of a head's own keys, and of its values
+constexpr int kThreads = 256;         // of the scan, the expansion and the merge
+constexpr int kExpandTok = 128;       // tokens of a workgroup of the expansion
+constexpr int kStep = 64;             // tokens of a step of the attention
+constexpr int kSetupTok = 2 * kStep;  // what an item's start counts
+constexpr int kGroups = 256;
+
+}  // namespace
+
+// Expansion.  A workgroup holds 128 cached rows' latents in LDS and makes the 128 key and 128 value channels
+// of one head after another; a wave makes 64 of them for all 128 tokens, its weights coming straight from
+// memory in operand order.
+template <int DC>
+__global__ __launch_bounds__(kThreads, 1) void latent_expand_kernel(const LatentPrefillParams p) {
+    constexpr int LROW = 2 * DC, KS = DC / 32, TILES = kExpandTok / 16;
+    constexpr int PIECES = 16 * LROW / 1024;  // KiB of a tile's latents
+    extern __shared__ __align__(1024) unsigned char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, grp = lane >> 4;
+    const int s = blockIdx.y;
+    const SeqRows r = wave_uniform(seq_rows(p.seqs, s, p.pool.log_page));
+    const int tok0 = blockIdx.x * kExpandTok;
+    if (r.n == 0 || tok0 >= r.kv) return;
+    Pages pages{p.seqs.table + s * p.seqs.table_stride, p.seqs.width, 0, 0};
+    pages.fill(tok0 >> p.pool.log_page);
+    // chunk c of row t lies at c ^ (t & 7)
+#pragma unroll
+    for (int i = 0; i < TILES / 4; ++i) {
+        const int tile = wave + 4 * i;
+        const Tile at = tile_at(p.pool, pages, tok0 + 16 * tile, r.kv);
+        const u4 rsrc = wave_rsrc(at.at, at.rows * p.pool.row_bytes);
+#pragma unroll
+        for (int n = 0; n < PIECES; ++n) {
+            const int c = 64 * n + lane, row = c / (LROW / 16), in = c % (LROW / 16);
+            dma_kib(rsrc, __builtin_amdgcn_readfirstlane(lds_addr(smem) + tile * 16 * LROW + n * 1024),
+                    row * p.pool.row_bytes + ((in ^ (row & 7)) << 4));
+        }
+    }
+    wait_vm<0>();
+    __syncthreads();
+    const uint32_t at = lds_addr(smem) + col * LROW;
+    const int h0 = blockIdx.z * p.tile_heads, h1 = min(p.heads, h0 + p.tile_heads);
+    for (int h = h0; h < h1; ++h) {
+        const int head = p.head0 + h;
+        const u4 *w = (const u4 *)p.w + ((int64_t)head * KS * 16 + wave * 4) * 64 + lane;
+        f4 acc[TILES][4];
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) acc[t][b] = (f4){0.f, 0.f, 0.f, 0.f};
+        u4 W[2][4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) W[0][b] = w[b * 64];
+#pragma unroll 1
+        for (int k = 0; k < KS; k += 2)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int next = min(k + u + 1, KS - 1);
+#pragma unroll
+                for (int b = 0; b < 4; ++b) W[u ^ 1][b] = w[(next * 16 + b) * 64];
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) {
+                    const h8 c = __builtin_bit_cast(h8, *lds_ptr<u4>(at + t * 16 * LROW + (((4 * (k + u) + grp) ^ (col & 7)) << 4)));
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) acc[t][b] = mfma_k32(__builtin_bit_cast(h8, W[u][b]), c, acc[t][b]);
+                }
+            }
+        // a lane has 16 consecutive channels of token col of every tile
+        unsigned char *to = (wave < 2 ? p.keys : p.values) +
+                            (((int64_t)h * p.cap + s * p.seq_cap + tok0 + col) * kD + 64 * (wave & 1) + 16 * grp) * 2;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            if (tok0 + 16 * t + col >= p.seq_cap) continue;
+            u4 o[2];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                f4 v = acc[t][b];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = v[e] != v[e] ? v[e] : __builtin_amdgcn_fmed3f(v[e], -65504.0f, 65504.0f);
+                o[b >> 1][2 * (b & 1)] = as_u32((h2){(_Float16)v[0], (_Float16)v[1]});
+                o[b >> 1][2 * (b & 1) + 1] = as_u32((h2){(_Float16)v[2], (_Float16)v[3]});
+            }
+            ((u4 *)(to + (int64_t)t * 16 * kD * 2))[0] = o[0];
+            ((u4 *)(to + (int64_t)t * 16 * kD * 2))[1] = o[1];
+        }
+    }
+}
+
+namespace {
+
+// The work of a sequence: tile t of a head's rows costs a + b t tokens.
+struct TileWork {
+    SeqRows r;
+    int rows, tiles;
+    int64_t a, b;
+    __device__ __forceinline__ int64_t cost(int t) const { return a + b * t; }
+    __device__ __forceinline__ int64_t before(int64_t t) const { return a * t + b * (t * (t - 1) / 2); }
+};
+template <int R>
+__device__ __forceinline__ TileWork tile_work(const LatentPrefillParams &p, const SeqRows &r) {
+    TileWork w;
+    w.r = r;
+    w.rows = min(r.n, p.seqs.max_q);
+    w.tiles = (w.rows + R - 1) / R;
+    const int64_t old = min(max(r.at, 0), r.kv);
+    w.a = (p.causal ? old + R : r.kv) + kSetupTok;
+    w.b = p.causal ? R : 0;
+    return w;
+}
+// Steps of tile t, and how many of them lie before cost c of it.
+template <int R>
+__device__ __forceinline__ int steps_of(const LatentPrefillParams &p, const TileWork &w, int t) {
+    return (w.r.sees(p.causal, min((t + 1) * R, w.rows) - 1) + kStep - 1) / kStep;
+}
+__device__ __forceinline__ int steps_before(int64_t c, int64_t cost, int steps) {
+    if (c >= cost) return steps;
+    const int64_t x = (c - kSetupTok + kStep - 1) / kStep;
+    return (int)(x < 0 ? 0 : x > steps ? steps : x);
+}
+struct TileScan {
+    int64_t pre[kThreads + 1], wave_sum[kThreads / 64];
+};
+template <int R>
+__device__ __forceinline__ void scan_tiles(const LatentPrefillParams &p, TileScan &sc) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, per = (p.seqs.n_seqs + kThreads - 1) / kThreads;
+    int64_t mine = 0, inc = 0;
+    if (t < kThreads) {
+        for (int i = 0; i < per; ++i) {
+            const int s = t * per + i;
+            if (s < p.seqs.n_seqs) {
+                const TileWork w = tile_work<R>(p, seq_rows(p.seqs, s, p.pool.log_page));
+                mine += w.before(w.tiles) * p.heads;
+            }
+        }
+        inc = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int64_t o = __shfl_up(inc, d);
+            if (lane >= d) inc += o;
+        }
+        if (lane == 63) sc.wave_sum[wave] = inc;
+    }
+    __syncthreads();
+    if (t < kThreads) {
+        int64_t before = 0;
+        for (int w = 0; w < wave; ++w) before += sc.wave_sum[w];
+        sc.pre[t] = before + inc - mine;
+        if (t == kThreads - 1) sc.pre[kThreads] = before + inc;
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+    return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
+}
+__device__ __forceinline__ int64_t share_of(int64_t total, int groups) { return max((total + groups - 1) / groups, (int64_t)(4 * kStep)); }
+
+// Row chunks of 16 bytes lie turned: eight rows read at one chunk, and the transposed reads of four rows
+// at two, fall on different banks.
+__device__ __forceinline__ int turn16(int row) { return (row & 3) << 1 | (row >> 2 & 1); }
+
+}  // namespace
+
+// Attention.  A workgroup of NW waves takes 32 NW query tokens of one head, each wave 32 of them, and
+// walks the keys and values in steps of 64 tokens, three buffers in LDS that buffer loads fill: the keys' own
+// channels, the shared rotated ones straight from the cache's rows, the values.  S^T = K Q^T leaves a lane with
+// its row's scores of the tokens that the second product's operand wants, so p stays in registers.
+template <int DC, int NW>
+__global__ __launch_bounds__(64 * NW, NW / 4) void latent_prefill_kernel(const LatentPrefillParams p) {
+    constexpr int R = 32 * NW, SLOTS = 3, KB = kStep * kD * 2, RB = kStep * kLatentRope * 2, SLOT = 2 * KB + RB;
+    constexpr int LOADS = SLOT / 1024 / NW, CB = kD / 16, NI = (kD + kLatentRope) / 32, ROWB = 2 * (DC + kLatentRope);
+    extern __shared__ __align__(1024) unsigned char smem[];
+    __shared__ TileScan sc;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, grp = lane >> 4;
+    const uint32_t ring = lds_addr(smem);
+    // keys and values: a piece is four rows; rotated keys: eight
+    const uint32_t kv_off[2] = {(uint32_t)((lane >> 4) * kD * 2 + ((col ^ turn16(grp)) << 4)),
+                                (uint32_t)((lane >> 4) * kD * 2 + ((col ^ turn16(grp + 4)) << 4))};
+    const uint32_t r_off = (lane >> 3) * ROWB + 2 * DC + (((lane & 7) ^ turn(lane >> 3)) << 4);
+    const uint32_t k_at = col * kD * 2;                                     // chunk c at c ^ turn16(col)
+    const uint32_t r_at = 2 * KB + col * kLatentRope * 2 + ((grp ^ turn(col)) << 4);
+    const int vrow = 4 * grp + (col >> 2);
+    const uint32_t v_at = KB + vrow * kD * 2 + 8 * (col & 1);
+
+    scan_tiles<R>(p, sc);
+    const int per = (p.seqs.n_seqs + kThreads - 1) / kThreads;
+    const int64_t total = uniform64(sc.pre[kThreads]);
+    const int64_t share = share_of(total, p.groups);
+    if (blockIdx.x == 0 && threadIdx.x < kThreads) {
+        p.sums[threadIdx.x] = sc.pre[threadIdx.x];
+        if (threadIdx.x == 0) p.sums[kThreads] = total;
+    }
+    int64_t x = min((int64_t)blockIdx.x * share, total);
+    const int64_t x_end = min(x + share, total);
+    if (x >= x_end) return;
+    int s, h = 0, tile = 0;
+    int64_t c0;  // where in the tile's cost the run stands
+    TileWork w;
+    {
+        int k = 0;
+        for (int i = 0; i < kThreads / 64; ++i) k += __builtin_popcountll(__builtin_amdgcn_ballot_w64(sc.pre[64 * i + lane] <= x));
+        s = (k - 1) * per;
+        int64_t off = x - uniform64(sc.pre[k - 1]);
+        for (;;) {
+            w = tile_work<R>(p, wave_uniform(seq_rows(p.seqs, s, p.pool.log_page)));
+            const int64_t n = w.before(w.tiles) * p.heads;
+            if (off < n) break;
+            off -= n;
+            ++s;
+        }
+        const int64_t one = w.before(w.tiles);
+        h = (int)(off / one);
+        off -= h * one;
+        while (off >= w.cost(tile)) off -= w.cost(tile++);
+        c0 = off;
+    }
+    while (x < x_end) {
+        const int64_t cost = w.cost(tile), c1 = min(cost, c0 + (x_end - x));
+        const int steps_all = steps_of<R>(p, w, tile);
+        const int j0 = steps_before(c0, cost, steps_all), j1 = steps_before(c1, cost, steps_all);
+        const bool starts = c0 <= kSetupTok, ends = c1 == cost;
+        x += c1 - c0;
+        if (j1 > j0 || (starts && ends)) {
+            const int row0 = tile * R, head = p.head0 + h;
+            const int mine = row0 + 32 * wave;
+            int see[2];
+            float kx[2];
+            h8 Q[2][NI];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int row = min(mine + 16 * r + col, w.rows - 1);
+                see[r] = w.r.sees(p.causal, row);
+                const unsigned char *q = p.q + (w.r.begin + row) * p.q_t + head * p.q_h + 16 * grp;
+                const f4 *ws = (const f4 *)(p.w_scale + (int64_t)head * 2 * kD + 8 * grp);  // of the keys' channels
+                u4 raw[NI];
+                f4 by[kD / 32][2];
+#pragma unroll
+                for (int i = 0; i < NI; ++i) raw[i] = *(const u4 *)(q + 64 * i);
+#pragma unroll
+                for (int i = 0; i < kD / 32; ++i) by[i][0] = ws[8 * i], by[i][1] = ws[8 * i + 1];
+                kx[r] = scaled_row(Q[r], [&](int i, int e) {
+                    const float v = query_value(raw[i], e, p.q_bf16);
+                    return i < kD / 32 ? v * by[i][e >> 2][e & 3] : v;
+                }, p.scale_log2);
+            }
+            const int see_all = w.r.sees(p.causal, min(mine, w.rows - 1));  // what all of the wave's rows see
+            const int kv = w.r.kv;
+            Pages pages{p.seqs.table + s * p.seqs.table_stride, p.seqs.width, 0, 0};
+            const int64_t base = ((int64_t)h * p.cap + s * p.seq_cap) * kD * 2;
+            uint32_t there = 0;  // bits 4 slot ..
+            auto load = [&](int j, int slot) {
+                const int k = j * kStep, end = j < j1 ? kv : 0;
+                const int left = max(0, min(end - k, kStep));
+                const u4 rk = wave_rsrc(p.keys + base + (int64_t)k * kD * 2, left * kD * 2);
+                const u4 rv = wave_rsrc(p.values + base + (int64_t)k * kD * 2, left * kD * 2);
+                const uint32_t lds = __builtin_amdgcn_readfirstlane(ring + slot * SLOT);
+#pragma unroll
+                for (int i = 0; i < 16 / NW; ++i) {
+                    const int n = wave * (16 / NW) + i;  // (parity of n: the lane's offset)
+                    dma_kib(rk, lds + n * 1024, kv_off[i & 1] + n * 1024);
+                    dma_kib(rv, lds + KB + n * 1024, kv_off[i & 1] + n * 1024);
+                }
+                uint32_t bits = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const Tile t = tile_at(p.pool, pages, k + 16 * i, end);
+                    bits |= (uint32_t)t.there << i;
+                    if (i == (wave * (8 / NW)) >> 1) {
+                        const u4 rr = wave_rsrc(t.at, t.rows * ROWB);
+#pragma unroll
+                        for (int e = 0; e < 8 / NW; ++e) {
+                            const int n = wave * (8 / NW) + e;
+                            dma_kib(rr, lds + 2 * KB + n * 1024, r_off + (n & 1) * 8 * ROWB);
+                        }
+                    }
+                }
+                there = (there & ~(15u << 4 * slot)) | bits << 4 * slot;
+            };
+            pages.fill((j0 * kStep) >> p.pool.log_page);
+#pragma unroll
+            for (int i = 0; i < SLOTS - 1; ++i) load(j0 + i, i);
+            float mx[2] = {kMinMax, kMinMax}, l[2] = {0.0f, 0.0f};
+            f4 acc[CB][2];
+#pragma unroll
+            for (int b = 0; b < CB; ++b) acc[b][0] = acc[b][1] = (f4){0.f, 0.f, 0.f, 0.f};
+            int slot = 0, ahead = SLOTS - 1;
+            for (int j = j0; j < j1; ++j) {
+                wait_vm<(SLOTS - 2) * LOADS>();
+                wait_lgkm0();
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                load(j + SLOTS - 1, ahead);
+                const uint32_t at = ring + slot * SLOT, first = j * kStep;
+                const uint32_t have = there >> 4 * slot & 15;
+                slot = slot + 1 == SLOTS ? 0 : slot + 1;
+                ahead = ahead + 1 == SLOTS ? 0 : ahead + 1;
+                f4 S[4][2] = {};
+#pragma unroll
+                for (int c = 0; c < NI; ++c)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t a = c < kD / 32 ? at + k_at + i * 16 * kD * 2 + (((4 * c + grp) ^ turn16(col & 7)) << 4)
+                                                       : at + (r_at ^ (64 * (c - kD / 32))) + i * 16 * kLatentRope * 2;
+                        const h8 k = __builtin_bit_cast(h8, *lds_ptr<u4>(a));
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) S[i][r] = mfma_k32(k, Q[r][c], S[i][r]);
+                    }
+                if (!((int)first + kStep <= see_all && have == 15))
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if ((int)first + 16 * i + 4 * grp + e >= see[r] || !(have >> i & 1)) S[i][r][e] = -INFINITY;
+                float top[2];
+                bool over = false;
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    top[r] = S[0][r][0];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) top[r] = __builtin_fmaxf(top[r], S[i >> 2][r][i & 3]);
+                    over |= __builtin_fmaf(top[r], kx[r], kBias - mx[r]) > kBias + kLagBy;
+                }
+                if (__builtin_amdgcn_ballot_w64(over)) {
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float most = qmax(top[r]);
+                        const float mn = __builtin_fmaf(most, kx[r], kBias - mx[r]) > kBias ? running_max(most, kx[r], kBias) : mx[r];
+                        const float alpha = __builtin_amdgcn_exp2f(mx[r] - mn);
+                        l[r] *= alpha;
+                        mx[r] = mn;
+#pragma unroll
+                        for (int b = 0; b < CB; ++b) acc[b][r] *= alpha;
+                    }
+                }
+                u4 P[2][2];  // of 32 tokens each
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float e[4];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) e[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i][r][q], kx[r], kBias - mx[r]));
+                        l[r] += (e[0] + e[1]) + (e[2] + e[3]);
+                        P[i >> 1][r][2 * (i & 1)] = as_u32((h2){(_Float16)e[0], (_Float16)e[1]});
+                        P[i >> 1][r][2 * (i & 1) + 1] = as_u32((h2){(_Float16)e[2], (_Float16)e[3]});
+                    }
+#pragma unroll
+                for (int b = 0; b < CB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t a = at + v_at + i * 32 * kD * 2 + (((2 * b + ((col & 3) >> 1)) ^ turn16(vrow & 7)) << 4);
+                        const u2 lo = read_transposed(a), hi = read_transposed(a + 16 * kD * 2);
+                        const h8 v = __builtin_bit_cast(h8, (u4){lo[0], lo[1], hi[0], hi[1]});
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) acc[b][r] = mfma_k32(v, __builtin_bit_cast(h8, P[i][r]), acc[b][r]);
+                    }
+            }
+            wait_vm<0>();
+            float *e = p.part + ((int64_t)blockIdx.x * 2 + starts) * (R * (kD + 2));
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                l[r] = qsum(l[r]);
+                const int row = mine + 16 * r + col;
+                if (starts && ends) {
+                    const float inv = row_inverse(l[r]);
+                    if (row < w.rows) {
+                        const f4 *vs = (const f4 *)(p.w_scale + ((int64_t)head * 2 + 1) * kD) + grp;
+                        unsigned char *out = (unsigned char *)p.out + ((int64_t)(w.r.begin + row) * p.H + head) * (2 * kD) + 8 * grp;
+#pragma unroll
+                        for (int b = 0; b < CB; ++b) {
+                            const f4 v = acc[b][r] * inv * vs[4 * b];
+                            *(u2 *)(out + 32 * b) = (u2){to_pair(p.q_bf16, v[0], v[1]), to_pair(p.q_bf16, v[2], v[3])};
+                        }
+                    }
+                } else {
+                    const int at = 2 * wave + r;
+#pragma unroll
+                    for (int b = 0; b < CB; ++b) *(f4 *)(e + (at * CB + b) * 256 + lane * 4) = acc[b][r];
+                    if (grp == 0) e[R * kD + 16 * at + col] = mx[r], e[R * kD + R + 16 * at + col] = l[r];
+                }
+            }
+            __syncthreads();
+        }
+        // the next item
+        c0 = 0;
+        if (x < x_end && ++tile == w.tiles) {
+            tile = 0;
+            if (++h == p.heads) {
+                h = 0;
+                do {
+                    w = tile_work<R>(p, wave_uniform(seq_rows(p.seqs, ++s, p.pool.log_page)));
+                } while (w.tiles == 0);
+            }
+        }
+    }
+}
+
+// Joins the partial states of items that several workgroups share: a wave takes 16 rows of one.
+template <int R>
+__global__ __launch_bounds__(kThreads) void latent_prefill_merge_kernel(const LatentPrefillParams p) {
+    constexpr int CB = kD / 16;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
+    const int s = blockIdx.z, h = blockIdx.y;
+    const int block = blockIdx.x * (kThreads / 64) + wave, tile = block / (R / 16), in = block % (R / 16);
+    const int per = (p.seqs.n_seqs + kThreads - 1) / kThreads;
+    const TileWork w = tile_work<R>(p, wave_uniform(seq_rows(p.seqs, s, p.pool.log_page)));
+    const int row = tile * R + 16 * in + col;
+    if (tile >= w.tiles || tile * R + 16 * in >= w.rows) return;
+    int64_t start = p.sums[s / per] + h * w.before(w.tiles) + w.before(tile);
+    for (int i = s / per * per; i < s; ++i) {
+        const TileWork b = tile_work<R>(p, wave_uniform(seq_rows(p.seqs, i, p.pool.log_page)));
+        start += b.before(b.tiles) * p.heads;
+    }
+    const int64_t share = share_of(p.sums[kThreads], p.groups), cost = w.cost(tile);
+    const int g0 = (int)(start / share), g1 = (int)((start + cost - 1) / share);
+    if (g0 == g1) return;
+    const int steps = steps_of<R>(p, w, tile);
+    // the runs that hold steps of it, and whether a run's entry is the one whose item starts there
+    auto part = [&](int g, int64_t &c0) {
+        c0 = max((int64_t)0, g * share - start);
+        const int64_t c1 = min(cost, (g + 1) * share - start);
+        return steps_before(c1, cost, steps) > steps_before(c0, cost, steps);
+    };
+    auto entry = [&](int g, int64_t c0) { return p.part + ((int64_t)g * 2 + (c0 <= kSetupTok)) * (R * (kD + 2)); };
+    float m = kMinMax;
+    int64_t c0;
+    int n = 0;
+    bool whole = false;
+    for (int g = g0; g <= g1; ++g)
+        if (part(g, c0)) {
+            m = __builtin_fmaxf(m, entry(g, c0)[R * kD + 16 * in + col]);
+            ++n;
+            whole = c0 <= kSetupTok && g == g1;
+        }
+    if (n == 1 && whole) return;  // one run held all of it and wrote the rows
+    float l = 0.0f;
+    f4 acc[CB] = {};
+    for (int g = g0; g <= g1; ++g)
+        if (part(g, c0)) {
+            const float *e = entry(g, c0);
+            const float a = __builtin_amdgcn_exp2f(e[R * kD + 16 * in + col] - m);
+            l += e[R * kD + R + 16 * in + col] * a;
+#pragma unroll
+            for (int b = 0; b < CB; ++b) acc[b] += *(const f4 *)(e + (in * CB + b) * 256 + lane * 4) * a;
+        }
+    if (row >= w.rows) return;
+    const float inv = row_inverse(l);
+    const f4 *vs = (const f4 *)(p.w_scale + ((int64_t)(p.head0 + h) * 2 + 1) * kD) + grp;
+    unsigned char *out = (unsigned char *)p.out + ((int64_t)(w.r.begin + row) * p.H + p.head0 + h) * (2 * kD) + 8 * grp;
+#pragma unroll
+    for (int b = 0; b < CB; ++b) {
+        const f4 v = acc[b] * inv * vs[4 * b];
+        *(u2 *)(out + 32 * b) = (u2){to_pair(p.q_bf16, v[0], v[1]), to_pair(p.q_bf16, v[2], v[3])};
+    }
+}
+
+namespace {
+constexpr int64_t kSumsBytes = 4096;
+static_assert((kThreads + 1) * 8 <= kSumsBytes, "the sums fit");
+constexpr int64_t kMostBytes = (int64_t)4 << 30;  // keys and values of a pass, where one head's are not more
+int64_t part_bytes(const LatentPrefillParams &p) { return (int64_t)p.groups * 2 * 32 * p.waves * (kD + 2) * 4; }
+}  // namespace
+
+int64_t latent_prefill_plan(LatentPrefillParams *p) {
+    p->seq_cap = (int64_t)p->seqs.width << p->pool.log_page;
+    p->cap = p->seq_cap * p->seqs.n_seqs;
+    const int64_t head = std::max<int64_t>(1, p->cap * 2 * kD * 2);
+    p->heads = (int)std::max<int64_t>(1, std::min<int64_t>(p->H, kMostBytes / head));
+    p->waves = p->seqs.max_q <= 128 ? 4 : 8;
+    p->groups = kGroups;
+    return kSumsBytes + part_bytes(*p) + p->heads * head;
+}
+
+hipError_t latent_prefill_launch(const LatentPrefillParams &p0, hipStream_t st) {
+    LatentPrefillParams p = p0;
+    if (p.seqs.n_seqs == 0 || p.seqs.max_q == 0) return hipSuccess;
+    unsigned char *at = (unsigned char *)p.sums + kSumsBytes;
+    p.part = (float *)at;
+    p.keys = at + part_bytes(p);
+    p.values = p.keys + p.heads * p.cap * kD * 2;
+    const int most = p.heads;
+    if (p.pool.n_pages == 0) p.seqs.width = 0;
+    auto of = [&](auto dc, auto nw) {
+        constexpr int DC = decltype(dc)::value, NW = decltype(nw)::value;
+        auto expand = latent_expand_kernel<DC>;
+        auto attend = latent_prefill_kernel<DC, NW>;
+        const int lds_e = kExpandTok * 2 * DC, lds_a = 3 * kStep * (4 * kD + 2 * kLatentRope);
+        (void)hipFuncSetAttribute((const void *)expand, hipFuncAttributeMaxDynamicSharedMemorySize, lds_e);
+        (void)hipFuncSetAttribute((const void *)attend, hipFuncAttributeMaxDynamicSharedMemorySize, lds_a);
+        for (p.head0 = 0; p.head0 < p.H; p.head0 += most) {
+            p.heads = std::min(most, p.H - p.head0);
+            const int64_t tiles = (((int64_t)p.seqs.width << p.pool.log_page) + kExpandTok - 1) / kExpandTok;
+            if (tiles) {
+                p.tile_heads = (int)std::max<int64_t>(1, std::min<int64_t>(8, p.heads * tiles * p.seqs.n_seqs / 1024));
+                const dim3 grid((unsigned)tiles, p.seqs.n_seqs, (p.heads + p.tile_heads - 1) / p.tile_heads);
+                expand<<<grid, dim3(kThreads), lds_e, st>>>(p);
+                const hipError_t e = hipGetLastError();
+                if (e != hipSuccess) return e;
+            }
+            attend<<<dim3(p.groups), dim3(64 * NW), lds_a, st>>>(p);
+            hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+            const int64_t blocks = ((int64_t)(p.seqs.max_q + 32 * NW - 1) / (32 * NW) * (2 * NW) + 3) / 4;
+            latent_prefill_merge_kernel<32 * NW><<<dim3((unsigned)blocks, p.heads, p.seqs.n_seqs), dim3(kThreads), 0, st>>>(p);
+            e = hipGetLastError();
+            if (e != hipSuccess) return e;
+        }
+        return hipSuccess;
+    };
+    auto by_rows = [&](auto dc) { return p.waves == 4 ? of(dc, std::integral_constant<int, 4>{}) : of(dc, std::integral_constant<int, 8>{}); };
+    return p.Dc == 512 ? by_rows(std::integral_constant<int, 512>{}) : by_rows(std::integral_constant<int, 256>{});
+}
+
+}  // namespace akv

@@ -5,6 +5,7 @@
 
 #include "akv_common.h"
 #include "paged.h"
+#include "paged_device.h"
 
 namespace akv {
 namespace {
@@ -75,22 +76,6 @@ __device__ __forceinline__ float over_group(float x, int log_lanes) {
     if (log_lanes >= 3) x = pick<MAX>(x, dpp<0x141>(x)); // quads of a half row (mirrored: a quad's lanes agree)
     if (log_lanes >= 4) x = pick<MAX>(x, dpp<0x140>(x));
     return x;
-}
-
-// Sequence of each lane's token t: the number of sequences that end at or before it.
-__device__ __forceinline__ int seq_of(const PagedSeqs &q, int t, bool live) {
-    const int lane = threadIdx.x & 63;
-    const int first = __builtin_amdgcn_readfirstlane(t);
-    const int last = __builtin_amdgcn_readlane(t, 63);
-    int n = 0;
-    for (int s0 = 0; s0 < q.n_seqs; s0 += 64) {
-        const int end = s0 + lane < q.n_seqs ? q.q_starts[s0 + lane + 1] : 0x7fffffff;
-        for (int tt = first; tt <= last; ++tt) {
-            const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(end <= tt));
-            if (tt == t) n += c;
-        }
-    }
-    return live && n < q.n_seqs ? n : -1;
 }
 
 // Where the rows of token t lie: the tile of head 0, the next head's distance, the token in it.

@@ -1,4 +1,4 @@
-// Device helpers shared by the attention kernels over the paged 4-bit cache.
+// Device helpers shared by the kernels over the paged caches.
 #pragma once
 
 #include "akv_common.h"
@@ -48,6 +48,22 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
 }
 __device__ __forceinline__ uint32_t to_pair(bool bf16, float a, float b) {
     return bf16 ? f32_to_bf16_rne(a) | ((uint32_t)f32_to_bf16_rne(b) << 16) : as_u32((h2){(_Float16)a, (_Float16)b});
+}
+
+// Sequence of each lane's token t: the number of sequences that end at or before it.
+__device__ __forceinline__ int seq_of(const PagedSeqs &q, int t, bool live) {
+    const int lane = threadIdx.x & 63;
+    const int first = __builtin_amdgcn_readfirstlane(t);
+    const int last = __builtin_amdgcn_readlane(t, 63);
+    int n = 0;
+    for (int s0 = 0; s0 < q.n_seqs; s0 += 64) {
+        const int end = s0 + lane < q.n_seqs ? q.q_starts[s0 + lane + 1] : 0x7fffffff;
+        for (int tt = first; tt <= last; ++tt) {
+            const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(end <= tt));
+            if (tt == t) n += c;
+        }
+    }
+    return live && n < q.n_seqs ? n : -1;
 }
 
 }  // namespace

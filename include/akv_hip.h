@@ -556,6 +556,149 @@ typedef struct akv_paged_compact_args {
  * tokens whose position or page is out of range are skipped. */
 int akv_paged_compact(const akv_paged_compact_args *args, void *stream);
 
+/* ------------------------------------------------------------ paged latent cache */
+
+/* A pool for models whose heads share one latent vector and one rotated key a token: data
+ * [num_layers][n_pages][page_size][latent_dim + rope_dim] float16.  Batches are those of the
+ * paged 4-bit cache.  A token that was given a value that is not finite is held as latents of
+ * 0 and a rotated key of NaN. */
+typedef struct akv_latent_pool {
+    void *data;            /* 16-byte aligned */
+    int64_t n_pages;
+    int32_t num_layers;
+    int32_t latent_dim;    /* 256 or 512 */
+    int32_t rope_dim;      /* 64 */
+    int32_t page_size;     /* a power of two, 16 to 256 */
+} akv_latent_pool;
+
+typedef struct akv_latent_rows_args {
+    int32_t abi_version;
+    int32_t layer;
+    int32_t dtype;         /* AKV_DT_* of latent and rope */
+    int32_t _pad0;
+    akv_latent_pool pool;
+    akv_paged_batch batch;
+    void *latent, *rope;   /* (n_tokens, latent_dim) and (n_tokens, rope_dim), channels contiguous */
+    int64_t latent_t, rope_t; /* byte strides of a token, multiples of 16 */
+} akv_latent_rows_args;
+
+/* The call's rows into their slots, clamped to +-61440 and rounded to float16. */
+int akv_latent_append(const akv_latent_rows_args *args, void *stream);
+/* The call's rows as the cache holds them, rounded to dtype; a token that was given a value
+ * that is not finite is NaN throughout.  Rows without a slot, and those that are no sequence's,
+ * become 0. */
+int akv_latent_read(const akv_latent_rows_args *args, void *stream);
+
+typedef struct akv_latent_attn_args {
+    int32_t abi_version;
+    int32_t layer;
+    int32_t H;             /* query heads */
+    int32_t q_dtype;       /* AKV_DT_F16 or AKV_DT_BF16 */
+    int32_t causal;        /* 1: row i of m sees tokens 0 .. kv_len - m + i; 0: every token */
+    float sm_scale;        /* > 0 */
+    akv_latent_pool pool;
+    akv_paged_batch batch;
+    const void *q, *q_rope; /* (n_tokens, H, latent_dim) and (n_tokens, H, rope_dim), channels contiguous */
+    int64_t q_t, q_h, q_rope_t, q_rope_h; /* byte strides of token and head, multiples of 16 */
+    void *out;             /* (n_tokens, H, latent_dim) contiguous, q dtype */
+    float *lse;            /* optional (n_tokens, H): log sum exp of the scaled scores */
+    void *workspace;       /* akv_latent_attn_workspace_bytes() bytes, no initial value needed */
+    int64_t workspace_bytes;
+} akv_latent_attn_args;
+
+/* Attention in its absorbed form: score = sm_scale (q . latent + q_rope . rope), the output the
+ * weighted sum of latents.  Rows that see no token: 0, and -inf in lse.  Calls that share a
+ * workspace must not overlap. */
+int64_t akv_latent_attn_workspace_bytes(const akv_latent_attn_args *args);
+int akv_latent_attn(const akv_latent_attn_args *args, void *stream);
+
+typedef struct akv_latent_prefill_args {
+    int32_t abi_version;
+    int32_t layer;
+    int32_t H;
+    int32_t q_dtype;       /* AKV_DT_F16 or AKV_DT_BF16 */
+    int32_t causal;
+    float sm_scale;
+    akv_latent_pool pool;
+    akv_paged_batch batch;
+    const void *w;         /* float16 [H][latent_dim / 32][16][64][8]: value j of lane l of block 4 a + b of step k
+                              is weight (channel 64 a + 16 (l % 16 / 4) + 4 b + l % 4, latent 32 k + 8 (l / 16) + j);
+                              channels 0..127 of a head are its keys', 128..255 its values' */
+    const float *w_scale;  /* [H][256]: what a channel is multiplied by (a key's in the queries, a value's in out) */
+    const void *q;         /* (n_tokens, H, 128 + rope_dim), channels contiguous */
+    int64_t q_t, q_h;      /* byte strides of token and head, multiples of 16 */
+    void *out;             /* (n_tokens, H, 128) contiguous, q dtype */
+    void *workspace;       /* akv_latent_prefill_workspace_bytes() bytes, no initial value needed */
+    int64_t workspace_bytes;
+} akv_latent_prefill_args;
+
+/* Attention in its expanded form: a head's keys are (W_k latent, rope) and its values W_v latent, made
+ * in the workspace as float16 (without w_scale, clamped to +-65504) and then attended to.  Rows that see no token: 0.
+ * Calls that share a workspace must not overlap. */
+int64_t akv_latent_prefill_workspace_bytes(const akv_latent_prefill_args *args);
+int akv_latent_prefill(const akv_latent_prefill_args *args, void *stream);
+
+typedef struct akv_latent_importance_args {
+    int32_t abi_version;
+    int32_t layer;
+    int32_t H;
+    int32_t q_dtype;       /* AKV_DT_F16 or AKV_DT_BF16 */
+    int32_t causal;
+    int32_t q_window;      /* > 0: only a sequence's last q_window rows count */
+    float sm_scale, decay;
+    akv_latent_pool pool;
+    akv_paged_batch batch;
+    const void *q, *q_rope;
+    int64_t q_t, q_h, q_rope_t, q_rope_h;
+    const float *lse;      /* (n_tokens, H) of akv_latent_attn */
+    const float *scores;   /* [n_seqs] rows of n_scores, score_stride apart */
+    float *out;            /* likewise, out_stride apart; scores itself, or no part of it */
+    int64_t n_scores, score_stride, out_stride;
+} akv_latent_importance_args;
+
+/* As akv_paged_importance, over the latent cache. */
+int akv_latent_importance(const akv_latent_importance_args *args, void *stream);
+
+/* As akv_paged_copy, over the latent cache. */
+int akv_latent_copy(const akv_latent_pool *pool, const int32_t *src, const int32_t *dst, int64_t n, void *stream);
+
+typedef struct akv_latent_compact_args {
+    int32_t abi_version;
+    int32_t n_seqs;
+    akv_latent_pool pool;
+    const int32_t *src_table, *dst_table; /* [n_seqs] rows */
+    int64_t src_stride, dst_stride;
+    int32_t src_width, dst_width;
+    const int32_t *keep;   /* [n_seqs] rows of max_keep positions, keep_stride apart */
+    const int32_t *n_keep; /* [n_seqs] */
+    int64_t keep_stride;
+    int64_t max_keep;
+} akv_latent_compact_args;
+
+/* As akv_paged_compact, over the latent cache. */
+int akv_latent_compact(const akv_latent_compact_args *args, void *stream);
+
+typedef struct akv_evict_args {
+    int32_t abi_version;
+    int32_t n_seqs;
+    const float *scores;   /* [n_seqs] rows of n_scores, score_stride apart */
+    int64_t n_scores, score_stride;
+    const int32_t *lens;   /* [n_seqs]: tokens of a sequence; past n_scores they count as n_scores */
+    const int32_t *budgets; /* [n_seqs], or NULL: `budget` for every sequence */
+    int64_t budget;
+    int32_t protect_initial, protect_recent;
+    int32_t *keep;         /* [n_seqs] rows of max_keep, keep_stride apart */
+    int32_t *n_keep;       /* [n_seqs] */
+    float *kept;           /* [n_seqs] rows of n_scores, kept_stride apart, or NULL; no part of scores */
+    int64_t keep_stride, max_keep, kept_stride;
+} akv_evict_args;
+
+/* Which tokens of a sequence stay: min(len, budget, max_keep) of them, the protected first and last
+ * ones before all others (where the budget does not hold those, the later ones), then those of the
+ * highest score, NaN above all; of equal ones the lowest position leaves first.  keep[s] lists them
+ * in ascending order, 0 behind them; kept[s] has their scores, 0 behind them. */
+int akv_evict_select(const akv_evict_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
