@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "akv_hip.h"
+#include "fastdiv.h"
 #include "paged.h"
 
 namespace akv {
@@ -39,7 +40,8 @@ struct LatentAttnParams {
     float *lse;
     int *sums;                 // the workspace: first units of the sequences, then partial states
     float *part;
-    int groups, row_tile;      // workgroups, rows of one
+    int groups, log_tile;      // workgroups, log2 of the rows of one
+    FastDiv by_heads, by_groups;
 };
 
 // The expanded form: keys and values of `heads` heads at a time are made from the latents, then attended to.

@@ -22,18 +22,15 @@ constexpr int kUnit = 64;             // tokens of a unit of work
 constexpr int kSetup = 2;             // units that an item's start counts
 constexpr int kGroups = 256;          // one workgroup a compute unit
 
-// A row's query operand: lane (row, quarter grp) holds channels 32 i + 8 grp .. of latent and rope.
+// A row's query: lane (row, quarter grp) holds channels 32 i + 8 grp .. of latent and rope.
 template <int DC>
 struct Row {
     static constexpr int NI = (DC + kLatentRope) / 32;
     u4 w[NI];
-    __device__ __forceinline__ void load(const unsigned char *q, const unsigned char *qr, int grp) {
+    __device__ __forceinline__ void load(const LatentAttnParams &p, int t, int h, int grp) {
+        const unsigned char *q = p.q + t * p.q_t + h * p.q_h + 16 * grp, *qr = p.qr + t * p.qr_t + h * p.qr_h + 16 * grp;
 #pragma unroll
-        for (int i = 0; i < NI; ++i)
-            w[i] = i < DC / 32 ? *(const u4 *)(q + 64 * i + 16 * grp) : *(const u4 *)(qr + 64 * (i - DC / 32) + 16 * grp);
-    }
-    __device__ __forceinline__ float make(h8 (&op)[NI], bool bf16, float scale_log2) const {
-        return scaled_row(op, [&](int i, int e) { return query_value(w[i], e, bf16); }, scale_log2);
+        for (int i = 0; i < NI; ++i) w[i] = i < DC / 32 ? *(const u4 *)(q + 64 * i) : *(const u4 *)(qr + 64 * (i - DC / 32));
     }
 };
 
@@ -46,25 +43,38 @@ __device__ __forceinline__ Work seq_work(const LatentAttnParams &p, const SeqRow
     Work w;
     w.r = r;
     w.rows = min(r.n, p.seqs.max_q) * p.H;
-    w.tiles = (w.rows + p.row_tile - 1) / p.row_tile;
+    w.tiles = (w.rows + (1 << p.log_tile) - 1) >> p.log_tile;
     w.cost = max(1, (r.kv + kUnit - 1) / kUnit) + kSetup;
     return w;
 }
 
+__device__ __forceinline__ int share_of(const LatentAttnParams &p, int total) {
+    return max(1, (int)fast_div((uint32_t)(total + p.groups - 1), p.by_groups));
+}
+
+// The sequences of a call in LDS: where their units lie (pre[i]: the first unit of sequence i * per,
+// pre[256] the total), and up to 256 sequences their rows.
 struct Scan {
     int pre[kThreads + 1];
-    int wave_sum[kWaves];
+    int wave_sum[kThreads / 64];
+    SeqRows rows[kThreads];
 };
-// pre[i]: the first unit of sequence i * per, pre[256] the total.  For workgroups of 256 threads or more.
-__device__ __forceinline__ void scan_seqs(const LatentAttnParams &p, Scan &sc, int per) {
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+__device__ __forceinline__ int seqs_per(const LatentAttnParams &p) { return p.seqs.n_seqs <= kThreads ? 1 : (p.seqs.n_seqs + kThreads - 1) / kThreads; }
+__device__ __forceinline__ SeqRows rows_of(const LatentAttnParams &p, const Scan &sc, int s) {
+    return wave_uniform(p.seqs.n_seqs <= kThreads ? sc.rows[s] : seq_rows(p.seqs, s, p.pool.log_page));
+}
+// For workgroups of 256 threads or more; the total.
+__device__ __forceinline__ int scan_seqs(const LatentAttnParams &p, Scan &sc) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, n = p.seqs.n_seqs, per = seqs_per(p);
     int mine = 0, inc = 0;
     if (t < kThreads) {
         for (int i = 0; i < per; ++i) {
             const int s = t * per + i;
-            if (s < p.seqs.n_seqs) {
-                const Work w = seq_work(p, seq_rows(p.seqs, s, p.pool.log_page));
+            if (s < n) {
+                const SeqRows r = seq_rows(p.seqs, s, p.pool.log_page);
+                const Work w = seq_work(p, r);
                 mine += w.tiles * w.cost;
+                if (per == 1) sc.rows[t] = r;
             }
         }
         inc = mine;
@@ -77,14 +87,18 @@ __device__ __forceinline__ void scan_seqs(const LatentAttnParams &p, Scan &sc, i
     }
     __syncthreads();
     if (t < kThreads) {
-        int before = 0;
-        for (int w = 0; w < wave; ++w) before += sc.wave_sum[w];
-        sc.pre[t] = before + inc - mine;
-        if (t == kThreads - 1) sc.pre[kThreads] = before + inc;
+#pragma unroll
+        for (int w = 0; w < kThreads / 64; ++w) inc += w < wave ? sc.wave_sum[w] : 0;
+        sc.pre[t] = inc - mine;
+        if (t == kThreads - 1) sc.pre[kThreads] = inc;
+        if (blockIdx.x == 0) {  // for the merge
+            p.sums[t] = inc - mine;
+            if (t == kThreads - 1) p.sums[kThreads] = inc;
+        }
     }
     __syncthreads();
+    return __builtin_amdgcn_readfirstlane(sc.pre[kThreads]);
 }
-__device__ __forceinline__ int share_of(int total, int groups) { return max(1, (total + groups - 1) / groups); }
 
 // A run of units as items: whole or partial (sequence, tile of rows).
 struct Run {
@@ -95,10 +109,8 @@ struct Item {
     int tile, j0, j1;
     bool starts, ends;
 };
-__device__ __forceinline__ Run run_of(const LatentAttnParams &p, Scan &sc) {
-    const int lane = threadIdx.x & 63, per = (p.seqs.n_seqs + kThreads - 1) / kThreads;
-    const int total = __builtin_amdgcn_readfirstlane(sc.pre[kThreads]);
-    const int share = share_of(total, p.groups);
+__device__ __forceinline__ Run run_of(const LatentAttnParams &p, const Scan &sc, int total) {
+    const int lane = threadIdx.x & 63, per = seqs_per(p), share = share_of(p, total);
     Run r{};
     r.x = (int)min((int64_t)blockIdx.x * share, (int64_t)total);
     r.x_end = min(r.x + share, total);
@@ -109,7 +121,7 @@ __device__ __forceinline__ Run run_of(const LatentAttnParams &p, Scan &sc) {
     r.s = (k - 1) * per;
     r.off = r.x - __builtin_amdgcn_readfirstlane(sc.pre[k - 1]);
     for (;;) {
-        r.w = seq_work(p, wave_uniform(seq_rows(p.seqs, r.s, p.pool.log_page)));
+        r.w = seq_work(p, rows_of(p, sc, r.s));
         const int n = r.w.tiles * r.w.cost;
         if (r.off < n) break;
         r.off -= n;
@@ -118,13 +130,13 @@ __device__ __forceinline__ Run run_of(const LatentAttnParams &p, Scan &sc) {
     return r;
 }
 // The next item's part of the run; false at the end.
-__device__ __forceinline__ bool next_item(const LatentAttnParams &p, Run &r, Item &it) {
+__device__ __forceinline__ bool next_item(const LatentAttnParams &p, const Scan &sc, Run &r, Item &it) {
     if (r.x >= r.x_end) return false;
     while (r.off == r.w.tiles * r.w.cost) {
         r.off = 0;
-        r.w = seq_work(p, wave_uniform(seq_rows(p.seqs, ++r.s, p.pool.log_page)));
+        r.w = seq_work(p, rows_of(p, sc, ++r.s));
     }
-    it.tile = r.off / r.w.cost;
+    it.tile = r.w.tiles == 1 ? 0 : __builtin_amdgcn_readfirstlane(r.off / r.w.cost);  // (divided by vector instructions)
     const int c0 = r.off - it.tile * r.w.cost, c1 = min(r.w.cost, c0 + (r.x_end - r.x));
     it.j0 = max(0, c0 - kSetup), it.j1 = max(0, c1 - kSetup);
     it.starts = it.j0 == 0, it.ends = c1 == r.w.cost;
@@ -139,59 +151,45 @@ template <int DC, int ROWS>
 __device__ __forceinline__ float *entry_of(const LatentAttnParams &p, int group, bool starts) {
     return p.part + ((int64_t)group * 2 + starts) * (ROWS * (DC + 2));
 }
-__device__ __forceinline__ void keep_sums(const LatentAttnParams &p, const Scan &sc) {  // for the merge
-    if (blockIdx.x == 0 && threadIdx.x <= kThreads) {
-        p.sums[threadIdx.x] = sc.pre[threadIdx.x];
-        if (threadIdx.x == 0) p.sums[kThreads] = sc.pre[kThreads];
-    }
-}
 
 }  // namespace
 
 // Up to 16 rows a sequence (a token's heads).  Bound by the cache's bytes.
 //
 // Each of the four waves takes 16 tokens at a time for all 16 rows, from two buffers of LDS of its own
-// that buffer loads fill; nothing is shared until the waves join at an item's end.
+// that buffer loads fill; nothing is shared until the waves join at an item's end.  What is run once for an item is
+// kept short: the code comes from memory too.
 template <int DC>
-__global__ __launch_bounds__(kThreads, 1) void latent_few_kernel(const LatentAttnParams p) {
+__global__ __launch_bounds__(kThreads, 2) void latent_few_kernel(const LatentAttnParams p) {
     using T = Rows16<DC>;
     constexpr int NI = Row<DC>::NI, NB = DC / 16, ROWB = T::ROWB, SLOTS = 2;
-    constexpr int STATE = NB * 1024 + 512;  // bytes of a wave's state on its way to another
-    static_assert(2 * STATE <= kWaves * SLOTS * T::BYTES, "the joins fit");
+    constexpr int OWN = NB / kWaves;  // blocks of channels that a wave joins and writes
+    static_assert(NB * 1024 <= SLOTS * T::BYTES, "a wave's sums fit its buffers");
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ Scan sc;
+    __shared__ float ms[kWaves][16], ls[kWaves][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
     const uint32_t ring = __builtin_amdgcn_readfirstlane(lds_addr(smem) + wave * SLOTS * T::BYTES);
-
-    uint32_t voff[T::PIECES];
-#pragma unroll
-    for (int i = 0; i < T::PIECES; ++i) voff[i] = T::offset(i, lane);
     const uint32_t k_at = col * ROWB + ((grp ^ turn(col)) << 4);
     const int vrow = 4 * grp + (col >> 2);
     const uint32_t v_at = vrow * ROWB + ((((col & 3) >> 1) ^ turn(vrow)) << 4) + 8 * (col & 1);
 
-    scan_seqs(p, sc, (p.seqs.n_seqs + kThreads - 1) / kThreads);
-    keep_sums(p, sc);
-    Run run = run_of(p, sc);
+    Run run = run_of(p, sc, scan_seqs(p, sc));
     Item it;
-    while (next_item(p, run, it)) {
+    while (next_item(p, sc, run, it)) {
         const Work &w = run.w;
-        const int row = min(col, w.rows - 1), qt = row / p.H, h = row - qt * p.H;
-        const int see = w.r.sees(p.causal, qt), see_all = w.r.sees(p.causal, 0), see_any = w.r.sees(p.causal, (w.rows - 1) / p.H);
+        const int row = min(col, w.rows - 1), qt = (int)fast_div(row, p.by_heads), h = row - qt * p.H;
+        const int see = w.r.sees(p.causal, qt), see_all = w.r.sees(p.causal, 0), see_any = w.r.sees(p.causal, (int)fast_div(w.rows - 1, p.by_heads));
         const int key0 = it.j0 * kUnit, key1 = min(it.j1 * kUnit, see_any);
-        const int steps = key1 > key0 ? (key1 - key0 + 16 * kWaves - 1) / (16 * kWaves) : 0;
-        Row<DC> raw;
-        raw.load(p.q + (w.r.begin + qt) * p.q_t + h * p.q_h, p.qr + (w.r.begin + qt) * p.qr_t + h * p.qr_h, grp);
+        const int steps = key1 > key0 ? (key1 - key0 + kUnit - 1) / kUnit : 0;
         Pages pages{p.seqs.table + run.s * p.seqs.table_stride, p.seqs.width, 0, 0};
         bool there[SLOTS] = {};
         auto load = [&](int t, int slot) {
-            const int k = key0 + (t * kWaves + wave) * 16;
+            const int k = key0 + t * kUnit + wave * 16;
             const Tile tile = tile_at(p.pool, pages, k, t < steps ? w.r.kv : 0);
             there[slot] = tile.there;
-            const u4 rsrc = wave_rsrc(tile.at, tile.rows * ROWB);
-#pragma unroll
-            for (int i = 0; i < T::PIECES; ++i) dma_kib(rsrc, ring + slot * T::BYTES + i * 1024, voff[i]);
+            load_tile<DC>(wave_rsrc(tile.at, tile.rows * ROWB), ring + slot * T::BYTES, lane);
         };
         if (steps) {
             pages.fill(key0 >> p.pool.log_page);
@@ -199,26 +197,34 @@ __global__ __launch_bounds__(kThreads, 1) void latent_few_kernel(const LatentAtt
             load(1, 1);
         }
         h8 Q[NI];
-        const float kx = raw.make(Q, p.q_bf16, p.scale_log2);
+        float kx;
+        {
+            Row<DC> raw;
+            raw.load(p, w.r.begin + qt, h, grp);
+            kx = query_operand(Q, raw.w, p.q_bf16, p.scale_log2);
+        }
         float mx = kMinMax, l = 0.0f;
         f4 acc[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) acc[b] = (f4){0.f, 0.f, 0.f, 0.f};
 
-        auto step = [&](int t, int slot) {
+#pragma unroll 1
+        for (int t = 0; t < steps; ++t) {
+            const int slot = t & 1;
             wait_vm<T::PIECES>();  // the next step's rows are still on their way
             const uint32_t at = ring + slot * T::BYTES;
-            const int first = key0 + (t * kWaves + wave) * 16;
+            const int first = key0 + t * kUnit + wave * 16;
+            const bool here = slot ? there[1] : there[0];
             f4 S2[2] = {};
             const uint32_t ka = at + k_at, kb = ka ^ 64;
 #pragma unroll
             for (int c = 0; c < NI; ++c)
                 S2[c & 1] = mfma_k32(__builtin_bit_cast(h8, *lds_ptr<u4>((c & 1 ? kb : ka) + (c >> 1) * 128)), Q[c], S2[c & 1]);
             f4 S = S2[0] + S2[1];
-            if (!(first + 16 <= see_all && there[slot]))
+            if (!(first + 16 <= see_all && here))
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (first + 4 * grp + e >= see || !there[slot]) S[e] = -INFINITY;
+                    if (first + 4 * grp + e >= see || !here) S[e] = -INFINITY;
             const float top = __builtin_fmaxf(__builtin_fmaxf(S[0], S[1]), __builtin_fmaxf(S[2], S[3]));
             if (__builtin_amdgcn_ballot_w64(__builtin_fmaf(top, kx, kBias - mx) > kBias + kLagBy)) {
                 const float most = qmax(top);
@@ -235,59 +241,63 @@ __global__ __launch_bounds__(kThreads, 1) void latent_few_kernel(const LatentAtt
             l += (e[0] + e[1]) + (e[2] + e[3]);
             const h4 P = {(_Float16)e[0], (_Float16)e[1], (_Float16)e[2], (_Float16)e[3]};  // 2^-12 of a weight
             const uint32_t va = at + v_at;
+            constexpr int AHEAD = 4;  // reads that are under way
+            u2 V[AHEAD];
+            auto value = [&](int b) { return read_transposed((va ^ (32 * (b & 3))) + (b >> 2) * 128); };
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-                acc[b] = mfma_k16(__builtin_bit_cast(h4, read_transposed((va ^ (32 * (b & 3))) + (b >> 2) * 128)), P, acc[b]);
+            for (int b = 0; b < AHEAD; ++b) V[b] = value(b);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                acc[b] = mfma_k16(__builtin_bit_cast(h4, V[b % AHEAD]), P, acc[b]);
+                if (b + AHEAD < NB) V[b % AHEAD] = value(b + AHEAD);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             wait_lgkm0();
             asm volatile("" ::: "memory");
-            load(t + SLOTS, slot);
-        };
-        for (int t = 0; t < steps; t += 2) {
-            step(t, 0);
-            if (t + 1 < steps) step(t + 1, 1);
+            // (one copy of the loads' code for both buffers)
+            const int k = key0 + (t + SLOTS) * kUnit + wave * 16;
+            const Tile tile = tile_at(p.pool, pages, k, t + SLOTS < steps ? w.r.kv : 0);
+            if (slot) there[1] = tile.there;
+            else there[0] = tile.there;
+            load_tile<DC>(wave_rsrc(tile.at, tile.rows * ROWB), __builtin_amdgcn_readfirstlane(at), lane);
         }
         wait_vm<0>();
 
+        // The waves' states meet in LDS, each wave then sums its share of the channels.
         l = qsum(l);
+        if (grp == 0) ms[wave][col] = mx, ls[wave][col] = l;
+        __syncthreads();
+        float mj = ms[0][col];
 #pragma unroll
-        for (int n = kWaves / 2; n >= 1; n >>= 1) {
-            __syncthreads();
-            unsigned char *place = smem + (wave & (n - 1)) * STATE;
-            float *ml = (float *)(place + NB * 1024);
-            if (wave >= n && wave < 2 * n) {
+        for (int i = 1; i < kWaves; ++i) mj = __builtin_fmaxf(mj, ms[i][col]);
+        l = 0.0f;
 #pragma unroll
-                for (int b = 0; b < NB; ++b) *(f4 *)(place + b * 1024 + lane * 16) = acc[b];
-                ml[lane] = mx, ml[64 + lane] = l;
-            }
-            __syncthreads();
-            if (wave < n) {
-                const float mo = ml[lane], lo = ml[64 + lane], mn = __builtin_fmaxf(mx, mo);
-                const float a = __builtin_amdgcn_exp2f(mx - mn), c = __builtin_amdgcn_exp2f(mo - mn);
-                l = l * a + lo * c;
-                mx = mn;
+        for (int i = 0; i < kWaves; ++i) l += ls[i][col] * __builtin_amdgcn_exp2f(ms[i][col] - mj);
+        const float alpha = __builtin_amdgcn_exp2f(mx - mj);
+        unsigned char *states = smem + wave * SLOTS * T::BYTES + lane * 16;
 #pragma unroll
-                for (int b = 0; b < NB; ++b) acc[b] = acc[b] * a + *(const f4 *)(place + b * 1024 + lane * 16) * c;
+        for (int b = 0; b < NB; ++b) *(f4 *)(states + b * 1024) = acc[b] * alpha;
+        __syncthreads();
+        const bool whole = it.starts && it.ends;
+        const float inv = row_inverse(l);
+        const int64_t o = (int64_t)(w.r.begin + qt) * p.H + h;
+        unsigned char *out = (unsigned char *)p.out + o * (2 * DC) + 8 * grp;
+        float *e = entry_of<DC, 16>(p, blockIdx.x, it.starts);
+#pragma unroll 2
+        for (int b = wave * OWN; b < (wave + 1) * OWN; ++b) {
+            f4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < kWaves; ++i) v += *(const f4 *)(smem + i * SLOTS * T::BYTES + b * 1024 + lane * 16);
+            if (whole) {
+                v *= inv;
+                if (col < w.rows) *(u2 *)(out + 32 * b) = (u2){out_pair(p.q_bf16, v[0], v[1]), out_pair(p.q_bf16, v[2], v[3])};
+            } else {
+                *(f4 *)(e + b * 256 + lane * 4) = v;
             }
         }
-        if (wave == 0) {
-            if (it.starts && it.ends) {
-                const float inv = row_inverse(l);
-                if (col < w.rows) {
-                    const int64_t o = (int64_t)(w.r.begin + qt) * p.H + h;
-                    unsigned char *out = (unsigned char *)p.out + o * (2 * DC) + 8 * grp;
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        const f4 v = acc[b] * inv;
-                        *(u2 *)(out + 32 * b) = (u2){to_pair(p.q_bf16, v[0], v[1]), to_pair(p.q_bf16, v[2], v[3])};
-                    }
-                    if (p.lse && grp == 0) p.lse[o] = row_lse(mx, l, kBias);
-                }
-            } else {
-                float *e = entry_of<DC, 16>(p, blockIdx.x, it.starts);
-#pragma unroll
-                for (int b = 0; b < NB; ++b) *(f4 *)(e + b * 256 + lane * 4) = acc[b];
-                if (grp == 0) e[16 * DC + col] = mx, e[16 * DC + 16 + col] = l;
-            }
+        if (wave == 0 && grp == 0) {
+            if (!whole) e[16 * DC + col] = mj, e[16 * DC + 16 + col] = l;
+            else if (p.lse && col < w.rows) p.lse[o] = row_lse(mj, l, kBias);
         }
         __syncthreads();
     }
@@ -295,81 +305,73 @@ __global__ __launch_bounds__(kThreads, 1) void latent_few_kernel(const LatentAtt
 
 // More rows: all heads of a token on one card, drafted tokens, chunks.
 //
-// A workgroup of NW waves takes 16 RB rows and walks the cache in steps of 32 tokens, whose rows lie in
-// LDS once for all waves.  For the scores a wave has 16 rows (and half of the tokens, where there are fewer row
-// blocks than waves), whose queries stay in registers; p goes through LDS, and for the second product a
-// wave has all rows and its share of the channels, so that the sums of 128 rows x 512 channels fit the
-// registers of eight waves and a value is read from LDS by one wave only.  One barrier a step: when it opens, p and
-// the factors of this step are there, the next step's rows are too, and the step before is read by all.
-template <int DC, int RB>
+// Two groups of four waves take 64 rows each and walk the cache in steps of 32 tokens, whose rows lie in
+// LDS once for all waves.  For the scores a wave has 16 rows, whose queries stay in registers, and all 32 tokens;
+// p goes through LDS, and for the second product a wave has its group's 64 rows and a quarter of the
+// channels.  While one group's waves make scores, the other's are at the second product, so that each SIMD
+// has a wave for the softmax and one for the matrix cores.  A barrier ends each such half step: when it opens,
+// what one group leaves in LDS for itself is there, and so are the rows that are needed next.  SPLIT: both groups
+// take the same 64 rows, and every other step each; they join at an item's end.  Else 128 rows.
+// Bound by what LDS delivers: 192 bytes of operands for each MFMA of the first product, 96 for the second.
+template <int DC>
 struct RowsForm {
-    static constexpr int NW = RB == 2 ? 4 : 8, KW = NW / RB, KS = 32, KT = 2 / KW;
-    static constexpr int ROWS = 16 * RB, CB = DC / 16 / NW, SLOTS = RB == 8 ? 3 : 4;
-    static constexpr int SLOT = 2 * Rows16<DC>::BYTES, PIECES = 2 * Rows16<DC>::PIECES, LOADS = (PIECES + NW - 1) / NW;
-    static constexpr int LDS = SLOTS * SLOT + 2 * RB * 1024;
+    static constexpr int KS = 32, CB = DC / 64, SLOTS = 4;
+    static constexpr int SLOT = 2 * Rows16<DC>::BYTES, PIECES = Rows16<DC>::PIECES, LOADS = (PIECES + 3) / 4;
+    static constexpr int LDS = SLOTS * SLOT + 8 * 1024;  // the rows, p of both groups
+    static_assert(4 * CB * 4 * 1024 <= SLOTS * SLOT, "a group's sums fit the buffers");
 };
-template <int DC, int RB>
-__global__ __launch_bounds__((RB == 2 ? 256 : 512), (RB == 2 ? 1 : 2)) void latent_rows_kernel(const LatentAttnParams p) {
-    using F = RowsForm<DC, RB>;
+template <int DC, bool SPLIT>
+__global__ __launch_bounds__(512, 2) void latent_rows_kernel(const LatentAttnParams p) {
+    using F = RowsForm<DC>;
     using T = Rows16<DC>;
-    constexpr int NI = Row<DC>::NI, ROWB = T::ROWB, ROWS = F::ROWS, NW = F::NW, KW = F::KW, KT = F::KT, CB = F::CB, SLOTS = F::SLOTS;
+    constexpr int NI = Row<DC>::NI, ROWB = T::ROWB, ROWS = SPLIT ? 64 : 128, CB = F::CB, SLOTS = F::SLOTS, RB = 4;
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ Scan sc;
-    __shared__ float alphas[2][ROWS], tops[2][2][ROWS];  // (tops: the waves that share rows; at the end the sums)
-    __shared__ int flags[2][8];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 15, grp = lane >> 4;
-    const int rbw = wave % RB, kw = wave / RB;
-    const uint32_t ring = lds_addr(smem), p_at = ring + SLOTS * F::SLOT;
+    __shared__ float alphas[2][64];
+    __shared__ __align__(16) int flags[2][4];
+    __shared__ int miss[SLOTS][2];               // whether a tile of 16 tokens has no page
+    __shared__ uint16_t offsets[T::PIECES][64];  // what a lane loads of a piece: in LDS, registers are scarce
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = wave >> 2, wg = wave & 3;
+    const uint32_t ring = lds_addr(smem), p_ring = ring + SLOTS * F::SLOT + group * 4096;
+    for (int i = wave; i < T::PIECES; i += 8) offsets[i][threadIdx.x & 63] = (uint16_t)T::offset(i, threadIdx.x & 63);
 
-    uint32_t voff[F::LOADS];  // pieces wave, wave + NW, ..: of the first tile of 16 rows, then the second
-#pragma unroll
-    for (int i = 0; i < F::LOADS; ++i) {
-        int n = wave + NW * i;
-        if (n >= F::PIECES) n -= NW;  // the last one again, so that all waves count alike
-        voff[i] = T::offset(n % T::PIECES, lane);
-    }
-    const uint32_t k_at = kw * T::BYTES + col * ROWB + ((grp ^ turn(col)) << 4);
-    const int vrow = 4 * grp + (col >> 2);
-    const uint32_t v_at = vrow * ROWB + ((((col & 3) >> 1) ^ turn(vrow)) << 4) + 8 * (col & 1);
-
-    scan_seqs(p, sc, (p.seqs.n_seqs + kThreads - 1) / kThreads);
-    keep_sums(p, sc);
-    Run run = run_of(p, sc);
+    Run run = run_of(p, sc, scan_seqs(p, sc));
     Item it;
-    while (next_item(p, run, it)) {
+    while (next_item(p, sc, run, it)) {
         const Work &w = run.w;
-        const int row0 = it.tile * ROWS, rows = min(ROWS, w.rows - row0);
-        const int row = row0 + min(16 * rbw + col, rows - 1), qt = row / p.H, h = row - qt * p.H;
-        const int see = w.r.sees(p.causal, qt), see_all = w.r.sees(p.causal, row0 / p.H);
-        const int see_any = w.r.sees(p.causal, (row0 + rows - 1) / p.H);
+        const int row0 = it.tile * ROWS, rows = min(ROWS, w.rows - row0), mine = (SPLIT ? 0 : 64 * group) + 16 * wg;  // the wave's first for the scores
+        const int see_all = w.r.sees(p.causal, (int)fast_div(row0, p.by_heads));
+        const int see_any = w.r.sees(p.causal, (int)fast_div(row0 + rows - 1, p.by_heads));
         const int key0 = it.j0 * kUnit, key1 = min(it.j1 * kUnit, see_any);
         const int steps = key1 > key0 ? (key1 - key0 + F::KS - 1) / F::KS : 0;
-        h8 Q[NI];
-        float kx;
-        {
-            Row<DC> raw;
-            raw.load(p.q + (w.r.begin + qt) * p.q_t + h * p.q_h, p.qr + (w.r.begin + qt) * p.qr_t + h * p.qr_h, grp);
-            kx = raw.make(Q, p.q_bf16, p.scale_log2);
-        }
+        const int halves = SPLIT ? steps + 1 : 2 * steps + 1;
         Pages pages{p.seqs.table + run.s * p.seqs.table_stride, p.seqs.width, 0, 0};
-        uint32_t there = 0;  // bits 2 slot ..
-        auto load = [&](int t, int slot) {
-            const int k = key0 + t * F::KS, kv = t < steps ? w.r.kv : 0;
-            const Tile a = tile_at(p.pool, pages, k, kv), b = tile_at(p.pool, pages, k + 16, kv);
-            there = (there & ~(3u << 2 * slot)) | ((uint32_t)a.there | (uint32_t)b.there << 1) << 2 * slot;
-            const u4 ra = wave_rsrc(a.at, a.rows * ROWB), rb = wave_rsrc(b.at, b.rows * ROWB);
+        auto load = [&](int t, int slot) {  // a group takes 16 of the 32 rows
+            const Tile tile = tile_at(p.pool, pages, key0 + t * F::KS + 16 * group, t < steps ? w.r.kv : 0);
+            const int ln = lane_again();
+            if (ln == 0) miss[slot][group] = !tile.there;
+            const u4 rsrc = wave_rsrc(tile.at, tile.rows * ROWB);
+            const uint32_t offs = lds_addr((const unsigned char *)offsets) + 2 * ln, to = ring + slot * F::SLOT + group * T::BYTES;
+            uint32_t off[F::LOADS];
+            // pieces wg, wg + 4, ..; the last one again where a wave has one less, so that all count alike
 #pragma unroll
-            for (int i = 0; i < F::LOADS; ++i) {
-                int n = wave + NW * i;
-                if (n >= F::PIECES) n -= NW;
-                dma_kib(n < T::PIECES ? ra : rb, __builtin_amdgcn_readfirstlane(ring + slot * F::SLOT + n * 1024), voff[i]);
-            }
+            for (int i = 0; i < F::LOADS; ++i) off[i] = *lds_ptr<uint16_t>(offs + (wg + 4 * i < T::PIECES ? wg + 4 * i : wg + 4 * i - 4) * 128);
+#pragma unroll
+            for (int i = 0; i < F::LOADS; ++i)
+                dma_kib(rsrc, __builtin_amdgcn_readfirstlane(to + (wg + 4 * i < T::PIECES ? wg + 4 * i : wg + 4 * i - 4) * 1024), off[i]);
         };
         if (steps) {
             pages.fill(key0 >> p.pool.log_page);
-#pragma unroll
-            for (int t = 0; t < SLOTS - 1; ++t) load(t, t);
+            load(0, 0);
+            load(1, 1);
+        }
+        h8 Q[NI];
+        float kx;
+        {
+            const int row = row0 + min(mine + (int)(threadIdx.x & 15), rows - 1), qt = (int)fast_div(row, p.by_heads), h = row - qt * p.H;
+            Row<DC> raw;
+            raw.load(p, w.r.begin + qt, h, (threadIdx.x >> 4) & 3);
+            kx = query_operand(Q, raw.w, p.q_bf16, p.scale_log2);
         }
         float mx = kMinMax, l = 0.0f;
         f4 acc[RB][CB];
@@ -377,149 +379,184 @@ __global__ __launch_bounds__((RB == 2 ? 256 : 512), (RB == 2 ? 1 : 2)) void late
         for (int r = 0; r < RB; ++r)
 #pragma unroll
             for (int b = 0; b < CB; ++b) acc[r][b] = (f4){0.f, 0.f, 0.f, 0.f};
-        wait_vm<(SLOTS - 2) * F::LOADS>();
+        wait_vm<F::LOADS>();
+        wait_lgkm0();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
 
-        int slot = 0, ahead = SLOTS - 1;
-        for (int t = 0; t < steps; ++t) {
-            const int buf = t & 1;
-            const uint32_t at = ring + slot * F::SLOT;
-            f4 S[2] = {};  // of two tiles, or of one in two parts
-            const uint32_t ka = at + k_at, kb = ka ^ 64;
+#pragma unroll 1
+        for (int i = 0; i < halves; ++i) {
+            const bool fetch = SPLIT || (i & 1);
+            if (fetch) load(SPLIT ? i + 2 : (i >> 1) + 2, (SPLIT ? i + 2 : (i >> 1) + 2) & (SLOTS - 1));
+            const int lane = lane_again(), col = lane & 15, grp = lane >> 4;
+            const bool scores = ((i ^ group) & 1) == 0;
+            const int t = SPLIT ? (scores ? i : i - 1) : ((scores ? i : i - 1) - group) >> 1;
+            if (t >= 0 && t < steps) {
+                const uint32_t at = ring + (t & (SLOTS - 1)) * F::SLOT, p_at = p_ring + lane * 16;
+                if (scores) {
+                    const uint32_t ka = at + col * ROWB + ((grp ^ turn(col)) << 4), kb = ka ^ 64;
+                    constexpr int READS = 2 * NI, AHEAD = 4;  // reads that are under way
+                    f4 S[2] = {};
+                    h8 K[AHEAD];
+                    auto key = [&](int n) {
+                        const int c = n >> 1;
+                        return __builtin_bit_cast(h8, *lds_ptr<u4>((c & 1 ? kb : ka) + (n & 1) * T::BYTES + (c >> 1) * 128));
+                    };
 #pragma unroll
-            for (int c = 0; c < NI; ++c)
+                    for (int n = 0; n < AHEAD; ++n) K[n] = key(n);
+                    const int gone = miss[t & (SLOTS - 1)][0] | miss[t & (SLOTS - 1)][1] << 1;
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int i = 0; i < KT; ++i) {
-                    const h8 k = __builtin_bit_cast(h8, *lds_ptr<u4>((c & 1 ? kb : ka) + i * T::BYTES + (c >> 1) * 128));
-                    f4 &x = S[KT == 2 ? i : c & 1];
-                    x = mfma_k32(k, Q[c], x);
+                    for (int n = 0; n < READS; ++n) {
+                        S[n & 1] = mfma_k32(K[n % AHEAD], Q[n >> 1], S[n & 1]);
+                        if (n + AHEAD < READS) K[n % AHEAD] = key(n + AHEAD);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    const int first = key0 + t * F::KS, lost = __builtin_amdgcn_readfirstlane(gone);
+                    if (first + F::KS > see_all || lost) {
+                        const int see = w.r.sees(p.causal, (int)fast_div(row0 + min(mine + col, rows - 1), p.by_heads));
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (first + 16 * k + 4 * grp + e >= see || (lost >> k & 1)) S[k][e] = -INFINITY;
+                    }
+                    float top = S[0][0];
+#pragma unroll
+                    for (int e = 1; e < 8; ++e) top = __builtin_fmaxf(top, S[e >> 2][e & 3]);
+                    float alpha = 1.0f;
+                    const bool over = __builtin_amdgcn_ballot_w64(__builtin_fmaf(top, kx, kBias - mx) > kBias + kLagBy) != 0;
+                    if (over) {
+                        top = qmax(top);
+                        const float mn = __builtin_fmaf(top, kx, kBias - mx) > kBias ? running_max(top, kx, kBias) : mx;
+                        alpha = __builtin_amdgcn_exp2f(mx - mn);
+                        l *= alpha;
+                        mx = mn;
+                        if (grp == 0) alphas[group][16 * wg + col] = alpha;
+                    } else if (grp == 0) {
+                        alphas[group][16 * wg + col] = 1.0f;
+                    }
+                    if (lane == 0) flags[group][wg] = over;
+                    u4 P;  // one float16 each: 2^-12 of a weight
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        float e[4];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) e[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[k][q], kx, kBias - mx));
+                        l += (e[0] + e[1]) + (e[2] + e[3]);
+                        P[2 * k] = as_u32((h2){(_Float16)e[0], (_Float16)e[1]});
+                        P[2 * k + 1] = as_u32((h2){(_Float16)e[2], (_Float16)e[3]});
+                    }
+                    *lds_mut<u4>(p_at + wg * 1024) = P;
+                } else {
+                    const int vrow = 4 * grp + (col >> 2);
+                    const uint32_t va = at + vrow * ROWB + ((((col & 3) >> 1) ^ turn(vrow)) << 4) + 8 * (col & 1);
+                    constexpr int AHEAD = 2;
+                    h8 V[AHEAD], P[RB];
+                    auto value = [&](int b) {
+                        const int c = wg * CB + b;
+                        const uint32_t x = (va ^ (32 * (c & 3))) + (c >> 2) * 128;
+                        const u2 lo = read_transposed(x), hi = read_transposed(x + T::BYTES);
+                        return __builtin_bit_cast(h8, (u4){lo[0], lo[1], hi[0], hi[1]});
+                    };
+                    const u4 f = *(const u4 *)flags[group];
+#pragma unroll
+                    for (int r = 0; r < RB; ++r) P[r] = __builtin_bit_cast(h8, *lds_ptr<u4>(p_at + r * 1024));
+#pragma unroll
+                    for (int b = 0; b < AHEAD; ++b) V[b] = value(b);
+                    if (__builtin_amdgcn_readfirstlane(f[0] | f[1] | f[2] | f[3])) {
+#pragma unroll
+                        for (int r = 0; r < RB; ++r) {
+                            const float a = alphas[group][16 * r + col];
+#pragma unroll
+                            for (int b = 0; b < CB; ++b) acc[r][b] *= a;
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int b = 0; b < CB; ++b) {
+#pragma unroll
+                        for (int r = 0; r < RB; ++r) acc[r][b] = mfma_k32(V[b % AHEAD], P[r], acc[r][b]);
+                        if (b + AHEAD < CB) V[b % AHEAD] = value(b + AHEAD);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
-            if constexpr (KT == 1) S[0] = S[0] + S[1];
-            const int first = key0 + t * F::KS + 16 * kw;
-            const uint32_t have = there >> (2 * slot + kw) & ((1u << KT) - 1);
-            if (!(first + 16 * KT <= see_all && have == (1u << KT) - 1))
-#pragma unroll
-                for (int i = 0; i < KT; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (first + 16 * i + 4 * grp + e >= see || !(have >> i & 1)) S[i][e] = -INFINITY;
-            float top = S[0][0];
-#pragma unroll
-            for (int i = 0; i < KT; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) top = __builtin_fmaxf(top, S[i][e]);
-            if constexpr (KW == 2) {  // the rows' other tokens
-                top = qmax(top);
-                if (grp == 0) tops[buf][kw][16 * rbw + col] = top;
-                wait_lgkm0();
-                __builtin_amdgcn_s_barrier();
-                asm volatile("" ::: "memory");
-                top = __builtin_fmaxf(top, tops[buf][kw ^ 1][16 * rbw + col]);
             }
-            float alpha = 1.0f;
-            const bool over = __builtin_amdgcn_ballot_w64(__builtin_fmaf(top, kx, kBias - mx) > kBias + kLagBy) != 0;
-            if (over) {
-                if constexpr (KW == 1) top = qmax(top);
-                const float mn = __builtin_fmaf(top, kx, kBias - mx) > kBias ? running_max(top, kx, kBias) : mx;
-                alpha = __builtin_amdgcn_exp2f(mx - mn);
-                l *= alpha;
-                mx = mn;
-            }
-            if (grp == 0) alphas[buf][16 * rbw + col] = alpha;
-            if (lane == 0) flags[buf][wave] = over;
-            u4 P;
-#pragma unroll
-            for (int i = 0; i < KT; ++i) {
-                float e[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) e[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i][q], kx, kBias - mx));
-                l += (e[0] + e[1]) + (e[2] + e[3]);
-                P[2 * i] = as_u32((h2){(_Float16)e[0], (_Float16)e[1]});
-                P[2 * i + 1] = as_u32((h2){(_Float16)e[2], (_Float16)e[3]});
-            }
-            unsigned char *pw = smem + SLOTS * F::SLOT + (buf * RB + rbw) * 1024 + lane * 16;
-            if constexpr (KT == 2) *(u4 *)pw = P;
-            else *(u2 *)(pw + 8 * kw) = (u2){P[0], P[1]};
-            wait_vm<(SLOTS - 3) * F::LOADS>();
+            if (fetch) wait_vm<F::LOADS>();
             wait_lgkm0();
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            load(t + SLOTS - 1, ahead);
-            int any = 0;
-#pragma unroll
-            for (int i = 0; i < NW; ++i) any |= flags[buf][i];
-            if (__builtin_amdgcn_readfirstlane(any)) {
-#pragma unroll
-                for (int r = 0; r < RB; ++r) {
-                    const float a = alphas[buf][16 * r + col];
-#pragma unroll
-                    for (int b = 0; b < CB; ++b) acc[r][b] *= a;
-                }
-            }
-            const uint32_t va = at + v_at;
-            h8 V[CB];
-#pragma unroll
-            for (int b = 0; b < CB; ++b) {
-                const int c = wave * CB + b;
-                const uint32_t x = (va ^ (32 * (c & 3))) + (c >> 2) * 128;
-                const u2 lo = read_transposed(x), hi = read_transposed(x + T::BYTES);
-                V[b] = __builtin_bit_cast(h8, (u4){lo[0], lo[1], hi[0], hi[1]});
-            }
-#pragma unroll
-            for (int r = 0; r < RB; ++r) {
-                const h8 pr = __builtin_bit_cast(h8, *lds_ptr<u4>(p_at + (buf * RB + r) * 1024 + lane * 16));
-#pragma unroll
-                for (int b = 0; b < CB; ++b) acc[r][b] = mfma_k32(V[b], pr, acc[r][b]);
-            }
-            slot = slot + 1 == SLOTS ? 0 : slot + 1;
-            ahead = ahead + 1 == SLOTS ? 0 : ahead + 1;
         }
         wait_vm<0>();
-        __syncthreads();
+        const int lane = lane_again(), col = lane & 15, grp = lane >> 4;
         l = qsum(l);
-        if (grp == 0) tops[0][kw][16 * rbw + col] = l, tops[1][kw][16 * rbw + col] = mx;
+        // the rows' sums and maxima for all waves: in the p of the groups
+        float *const sums = (float *)(smem + SLOTS * F::SLOT + group * 4096);
+        if (grp == 0) sums[16 * wg + col] = l, sums[64 + 16 * wg + col] = mx;
         __syncthreads();
-        const bool all = it.starts && it.ends;
-        float *e = entry_of<DC, ROWS>(p, blockIdx.x, it.starts);
+        if constexpr (SPLIT) {
+            if (group == 1)
 #pragma unroll
-        for (int r = 0; r < RB; ++r) {
-            float lr = tops[0][0][16 * r + col];
-            if constexpr (KW == 2) lr += tops[0][1][16 * r + col];
-            const float mr = tops[1][0][16 * r + col];
-            if (all) {
-                const int at = row0 + 16 * r + col;
-                if (at < w.rows) {
-                    const float inv = row_inverse(lr);
-                    const int t = at / p.H;
-                    const int64_t o = (int64_t)(w.r.begin + t) * p.H + (at - t * p.H);
-                    unsigned char *out = (unsigned char *)p.out + o * (2 * DC) + wave * CB * 32 + 8 * grp;
+                for (int r = 0; r < RB; ++r)
+#pragma unroll
+                    for (int b = 0; b < CB; ++b) *(f4 *)(smem + ((wg * RB + r) * CB + b) * 1024 + lane * 16) = acc[r][b];
+            __syncthreads();
+        }
+        if (!SPLIT || group == 0) {
+            const bool all = it.starts && it.ends;
+            const int base = SPLIT ? 0 : 64 * group;
+            float *e = entry_of<DC, ROWS>(p, blockIdx.x, it.starts);
+#pragma unroll
+            for (int r = 0; r < RB; ++r) {
+                float lr = sums[16 * r + col], mr = sums[64 + 16 * r + col];
+                if constexpr (SPLIT) {
+                    const float lo = sums[1024 + 16 * r + col], mo = sums[1024 + 64 + 16 * r + col];
+                    const float mn = __builtin_fmaxf(mr, mo), x = __builtin_amdgcn_exp2f(mr - mn), y = __builtin_amdgcn_exp2f(mo - mn);
+                    lr = lr * x + lo * y;
+                    mr = mn;
 #pragma unroll
                     for (int b = 0; b < CB; ++b) {
-                        const f4 v = acc[r][b] * inv;
-                        *(u2 *)(out + 32 * b) = (u2){to_pair(p.q_bf16, v[0], v[1]), to_pair(p.q_bf16, v[2], v[3])};
-                    }
-                    if (p.lse && wave == 0 && grp == 0) p.lse[o] = row_lse(mr, lr, kBias);
-                }
-            } else {
+                        const f4 o = *(const f4 *)(smem + ((wg * RB + r) * CB + b) * 1024 + lane * 16);
 #pragma unroll
-                for (int b = 0; b < CB; ++b) *(f4 *)(e + (r * (DC / 16) + wave * CB + b) * 256 + lane * 4) = acc[r][b];
-                if (wave == 0 && grp == 0) e[ROWS * DC + 16 * r + col] = mr, e[ROWS * DC + ROWS + 16 * r + col] = lr;
+                        for (int q = 0; q < 4; ++q) acc[r][b][q] = __builtin_fmaf(o[q], y, acc[r][b][q] * x);
+                    }
+                }
+                if (all) {
+                    const int at = row0 + base + 16 * r + col;
+                    if (at < w.rows) {
+                        const float inv = row_inverse(lr);
+                        const int t = (int)fast_div(at, p.by_heads);
+                        const int64_t o = (int64_t)(w.r.begin + t) * p.H + (at - t * p.H);
+                        unsigned char *out = (unsigned char *)p.out + o * (2 * DC) + wg * CB * 32 + 8 * grp;
+#pragma unroll
+                        for (int b = 0; b < CB; ++b) {
+                            const f4 v = acc[r][b] * inv;
+                            *(u2 *)(out + 32 * b) = (u2){out_pair(p.q_bf16, v[0], v[1]), out_pair(p.q_bf16, v[2], v[3])};
+                        }
+                        if (p.lse && wg == 0 && grp == 0) p.lse[o] = row_lse(mr, lr, kBias);
+                    }
+                } else {
+#pragma unroll
+                    for (int b = 0; b < CB; ++b) *(f4 *)(e + ((base / 16 + r) * (DC / 16) + wg * CB + b) * 256 + lane * 4) = acc[r][b];
+                    if (wg == 0 && grp == 0) e[ROWS * DC + base + 16 * r + col] = mr, e[ROWS * DC + ROWS + base + 16 * r + col] = lr;
+                }
             }
         }
         __syncthreads();
     }
 }
 
-// Joins the partial states of items that several workgroups share: a wave takes four of the 16-channel
-// blocks of 16 rows.
+// Joins the partial states of items that several workgroups share: a workgroup takes two of the
+// 16-channel blocks of 16 rows, each of its waves every fourth state.
 template <int DC, int ROWS>
 __global__ __launch_bounds__(kThreads) void latent_merge_kernel(const LatentAttnParams p) {
-    constexpr int NB = DC / 16, PER = 4, SPLIT = NB / (PER * kWaves);
+    constexpr int NB = DC / 16, PER = 2, SPLIT = NB / PER;
+    __shared__ __align__(16) f4 sums[kWaves][PER][64];
+    __shared__ float ms[kWaves][16], ls[kWaves][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
-    const int s = blockIdx.y, part = blockIdx.x % SPLIT, block = blockIdx.x / SPLIT;
+    const int s = blockIdx.y, b0 = blockIdx.x % SPLIT * PER, block = blockIdx.x / SPLIT;
     const int tile = block / (ROWS / 16), r = block % (ROWS / 16);
-    const int per = (p.seqs.n_seqs + kThreads - 1) / kThreads;
+    const int per = seqs_per(p);
     const Work w = seq_work(p, wave_uniform(seq_rows(p.seqs, s, p.pool.log_page)));
     const int row0 = tile * ROWS + 16 * r;
     if (tile >= w.tiles || row0 >= w.rows) return;
@@ -528,37 +565,49 @@ __global__ __launch_bounds__(kThreads) void latent_merge_kernel(const LatentAttn
         const Work b = seq_work(p, wave_uniform(seq_rows(p.seqs, i, p.pool.log_page)));
         start += b.tiles * b.cost;
     }
-    const int share = share_of(p.sums[kThreads], p.groups);
+    const int share = share_of(p, p.sums[kThreads]);
     // the runs that hold units of the item (its first kSetup are none)
     const int g0 = (start + kSetup) / share, g1 = (start + w.cost - 1) / share;
     if (g0 == g1) return;
     float m = kMinMax;
-    for (int g = g0; g <= g1; ++g) m = __builtin_fmaxf(m, entry_of<DC, ROWS>(p, g, g == g0)[ROWS * DC + 16 * r + col]);
+    for (int g = g0 + wave + kWaves * grp; g <= g1; g += 4 * kWaves)
+        m = __builtin_fmaxf(m, entry_of<DC, ROWS>(p, g, g == g0)[ROWS * DC + 16 * r + col]);
+    m = qmax(m);
     float l = 0.0f;
     f4 acc[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) acc[i] = (f4){0.f, 0.f, 0.f, 0.f};
-    const int b0 = (part * kWaves + wave) * PER;
-#pragma unroll 2
-    for (int g = g0; g <= g1; ++g) {
+#pragma unroll 4
+    for (int g = g0 + wave; g <= g1; g += kWaves) {
         const float *e = entry_of<DC, ROWS>(p, g, g == g0);
         const float a = __builtin_amdgcn_exp2f(e[ROWS * DC + 16 * r + col] - m);
         l += e[ROWS * DC + ROWS + 16 * r + col] * a;
 #pragma unroll
         for (int i = 0; i < PER; ++i) acc[i] += *(const f4 *)(e + (r * NB + b0 + i) * 256 + lane * 4) * a;
     }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sums[wave][i][lane] = acc[i];
+    if (grp == 0) ms[wave][col] = m, ls[wave][col] = l;
+    __syncthreads();
+    if (wave >= PER) return;
+    float mx = ms[0][col];
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) mx = __builtin_fmaxf(mx, ms[i][col]);
+    f4 o = {0.f, 0.f, 0.f, 0.f};
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        const float a = __builtin_amdgcn_exp2f(ms[i][col] - mx);
+        l += ls[i][col] * a;
+        o += sums[i][wave][lane] * a;
+    }
     const int row = row0 + col;
     if (row >= w.rows) return;
-    const int qt = row / p.H, h = row - qt * p.H;
-    const int64_t o = (int64_t)(w.r.begin + qt) * p.H + h;
-    const float inv = row_inverse(l);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const f4 v = acc[i] * inv;
-        *(u2 *)((unsigned char *)p.out + o * (2 * DC) + 32 * (b0 + i) + 8 * grp) =
-            (u2){to_pair(p.q_bf16, v[0], v[1]), to_pair(p.q_bf16, v[2], v[3])};
-    }
-    if (p.lse && grp == 0 && b0 == 0) p.lse[o] = row_lse(m, l, kBias);
+    const int qt = (int)fast_div(row, p.by_heads), h = row - qt * p.H;
+    const int64_t at = (int64_t)(w.r.begin + qt) * p.H + h;
+    o *= row_inverse(l);
+    *(u2 *)((unsigned char *)p.out + at * (2 * DC) + 32 * (b0 + wave) + 8 * grp) = (u2){out_pair(p.q_bf16, o[0], o[1]), out_pair(p.q_bf16, o[2], o[3])};
+    if (p.lse && grp == 0 && b0 + wave == 0) p.lse[at] = row_lse(mx, l, kBias);
 }
 
 // The importance: sum over rows and heads of 2^(s - lse), for 32 tokens a wave, whose rows stay in
@@ -616,21 +665,24 @@ __global__ __launch_bounds__(kThreads, 1) void latent_importance_kernel(const La
             see_in = row < rows ? r.sees(p.causal, qt) : 0;
         };
         auto stage = [&](int buf) {
-            float top = 0.0f;
+            int ex = 14;
+            float x = 1.0f;
+            if (p.q_bf16) {
+                const us2 pair = largest(w);
+                uint32_t top = max(pair[0], pair[1]);
 #pragma unroll
-            for (int j = 0; j < MINE; ++j)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top = __builtin_fmaxf(top, __builtin_fabsf(query_value(w[j], e, p.q_bf16)));
-#pragma unroll
-            for (int d = 1; d < 16; d <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, d));
-            const int ex = row_exponent(top);
+                for (int d = 1; d < 16; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+                ex = row_exponent(top);
+                x = __builtin_ldexpf(1.0f, 14 - ex);
+            }
 #pragma unroll
             for (int j = 0; j < MINE; ++j) {
                 const int c = sl + 16 * j;
-                h8 v;
+                u4 v = w[j];
+                if (p.q_bf16)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = (_Float16)__builtin_ldexpf(query_value(w[j], e, p.q_bf16), 14 - ex);
-                if (c < CH) op[buf][(c >> 2) * 64 + (c & 3) * 16 + sr] = __builtin_bit_cast(u4, v);
+                    for (int e = 0; e < 4; ++e) v[e] = scaled_pair(w[j][e], x);
+                if (c < CH) op[buf][(c >> 2) * 64 + (c & 3) * 16 + sr] = v;
             }
             if (sl == 0) {
                 kxs[buf][sr] = row_factor(p.scale_log2, ex);
@@ -685,11 +737,13 @@ static_assert((kThreads + 1) * 4 <= kSumsBytes, "the sums fit");
 
 int64_t latent_attn_plan(LatentAttnParams *p) {
     const int64_t rows = (int64_t)p->seqs.max_q * p->H;
-    p->row_tile = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    p->log_tile = rows <= 16 ? 4 : rows <= 64 ? 6 : 7;
     const int64_t units = (((int64_t)p->seqs.width << p->pool.log_page) + kUnit - 1) / kUnit + 1 + kSetup;
-    const int64_t tiles = (rows + p->row_tile - 1) / p->row_tile;
+    const int64_t tiles = (rows + (1 << p->log_tile) - 1) >> p->log_tile;
     p->groups = (int)std::max<int64_t>(1, std::min<int64_t>(kGroups, units * tiles * p->seqs.n_seqs));
-    return kSumsBytes + (int64_t)p->groups * 2 * p->row_tile * (p->Dc + 2) * 4;
+    p->by_heads = make_fast_div((uint32_t)p->H);
+    p->by_groups = make_fast_div((uint32_t)p->groups);
+    return kSumsBytes + ((int64_t)p->groups * 2 * (p->Dc + 2) * 4 << p->log_tile);
 }
 
 hipError_t latent_attn_launch(const LatentAttnParams &p0, hipStream_t st) {
@@ -702,22 +756,17 @@ hipError_t latent_attn_launch(const LatentAttnParams &p0, hipStream_t st) {
         kern<<<dim3(p.groups), dim3(threads), lds, st>>>(p);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess || p.groups == 1) return e;
-        const int64_t tiles = ((int64_t)p.seqs.max_q * p.H + p.row_tile - 1) / p.row_tile;
-        const dim3 grid((unsigned)(tiles * (p.row_tile / 16) * (p.Dc / 256)), p.seqs.n_seqs);
+        const int64_t tiles = ((int64_t)p.seqs.max_q * p.H + (1 << p.log_tile) - 1) >> p.log_tile;
+        const dim3 grid((unsigned)((tiles << (p.log_tile - 4)) * (p.Dc / 32)), p.seqs.n_seqs);
         merge<<<grid, dim3(kThreads), 0, st>>>(p);
         return hipGetLastError();
     };
     auto of = [&](auto dc) {
         constexpr int DC = decltype(dc)::value;
-        auto rows = [&](auto rb) {
-            constexpr int RB = decltype(rb)::value;
-            using F = RowsForm<DC, RB>;
-            return go(latent_rows_kernel<DC, RB>, latent_merge_kernel<DC, F::ROWS>, 64 * F::NW, F::LDS);
-        };
-        if (p.row_tile == 16) return go(latent_few_kernel<DC>, latent_merge_kernel<DC, 16>, kThreads, 2 * kWaves * Rows16<DC>::BYTES);
-        if (p.row_tile == 32) return rows(std::integral_constant<int, 2>{});
-        if (p.row_tile == 64) return rows(std::integral_constant<int, 4>{});
-        return rows(std::integral_constant<int, 8>{});
+        using F = RowsForm<DC>;
+        if (p.log_tile == 4) return go(latent_few_kernel<DC>, latent_merge_kernel<DC, 16>, kThreads, 2 * kWaves * Rows16<DC>::BYTES);
+        if (p.log_tile == 6) return go(latent_rows_kernel<DC, true>, latent_merge_kernel<DC, 64>, 512, F::LDS);
+        return go(latent_rows_kernel<DC, false>, latent_merge_kernel<DC, 128>, 512, F::LDS);
     };
     return p.Dc == 512 ? of(std::integral_constant<int, 512>{}) : of(std::integral_constant<int, 256>{});
 }

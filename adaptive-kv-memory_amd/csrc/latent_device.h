@@ -1,6 +1,8 @@
 // Device helpers shared by the kernels over the paged latent cache.
 #pragma once
 
+#include <type_traits>
+
 #include "akv_common.h"
 #include "latent.h"
 #include "paged_device.h"
@@ -27,12 +29,12 @@ __device__ __forceinline__ float qsum(float x) {
 // transposed reads of four rows at two chunks, fall on different banks.
 __device__ __forceinline__ int turn(int row) { return (row & 2) << 1 | (row & 4) >> 1; }
 
-// 1 KiB: 16 bytes of each lane, from buffer offset voff, to LDS [lds, lds + 1024).
-__device__ __forceinline__ void dma_kib(u4 rsrc, uint32_t lds, uint32_t voff) {
+// 1 KiB: 16 bytes of each lane, from buffer offset voff + soff, to LDS [lds, lds + 1024).
+__device__ __forceinline__ void dma_kib(u4 rsrc, uint32_t lds, uint32_t voff, uint32_t soff = 0) {
     uint32_t m0;
     asm volatile("s_mov_b32 %[m0], m0\n\ts_mov_b32 m0, %[lds]\n\ts_nop 3\n\t"
-                 "buffer_load_dwordx4 %[v], %[r], 0 offen lds\n\ts_mov_b32 m0, %[m0]"
-                 : [m0] "=&s"(m0) : [lds] "s"(lds), [r] "s"(rsrc), [v] "v"(voff) : "memory");
+                 "buffer_load_dwordx4 %[v], %[r], %[s] offen lds\n\ts_mov_b32 m0, %[m0]"
+                 : [m0] "=&s"(m0) : [lds] "s"(lds), [r] "s"(rsrc), [v] "v"(voff), [s] "s"(soff) : "memory");
 }
 // A buffer of `bytes` at `at`, which are one for the whole wave.
 __device__ __forceinline__ u4 wave_rsrc(const unsigned char *at, int bytes) {
@@ -40,6 +42,18 @@ __device__ __forceinline__ u4 wave_rsrc(const unsigned char *at, int bytes) {
 #pragma unroll
     for (int i = 0; i < 3; ++i) r[i] = (uint32_t)__builtin_amdgcn_readfirstlane((int)r[i]);
     return r;
+}
+
+// The lane's number, computed where it is asked for: what follows from it is not kept in registers over a
+// loop that has none left (a register that is spilled costs a wait for all loads in flight).
+__device__ __forceinline__ int lane_again() {
+    int x;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
+    return x;
+}
+template <typename T>
+__device__ __forceinline__ __attribute__((address_space(3))) T *lds_mut(uint32_t a) {
+    return (__attribute__((address_space(3))) T *)(size_t)a;
 }
 
 typedef short s4v __attribute__((ext_vector_type(4)));
@@ -58,13 +72,29 @@ struct Rows16 {
     }
 };
 
+// A tile of 16 rows to LDS: a loop, whose code is a tenth of its instructions.
+template <int DC>
+__device__ __forceinline__ void load_tile(u4 rsrc, uint32_t lds, int lane) {
+    using T = Rows16<DC>;
+    constexpr int CH = T::ROWB / 16;
+    int row = lane / CH, at = lane - row * CH;  // of the lane's chunk
+#pragma unroll 1
+    for (int i = 0; i < T::PIECES; ++i) {
+        dma_kib(rsrc, lds + i * 1024, row * T::ROWB + ((at ^ turn(row)) << 4));
+        at += 64;
+        if (at >= CH) at -= CH, ++row;
+        if (CH < 64 && at >= CH) at -= CH, ++row;
+    }
+}
+
 // Where the tiles of a sequence lie, 64 pages of its table in a wave's lanes.
 struct Pages {
     const int32_t *table;
     int width, first, ids;
     __device__ __forceinline__ void fill(int page) {
-        first = page;
-        ids = page + (int)(threadIdx.x & 63) < width ? table[page + (threadIdx.x & 63)] : -1;
+        first = __builtin_amdgcn_readfirstlane(page);
+        const int at = page + lane_again();
+        ids = at < width ? table[at] : -1;
         asm volatile("" : "+v"(ids));  // waited for here
     }
     __device__ __forceinline__ uint32_t at(int page) {
@@ -81,6 +111,7 @@ struct Tile {
     bool there;
 };
 __device__ __forceinline__ Tile tile_at(const LatentView &v, Pages &pages, int k, int kv) {
+    k = __builtin_amdgcn_readfirstlane(k), kv = __builtin_amdgcn_readfirstlane(kv);
     uint32_t page = k < kv ? pages.at(k >> v.log_page) : ~0u;
     Tile t;
     t.there = page < v.n_pages;
@@ -90,27 +121,55 @@ __device__ __forceinline__ Tile tile_at(const LatentView &v, Pages &pages, int k
     return t;
 }
 
-// Eight values of a query row as float.
-__device__ __forceinline__ float query_value(u4 w, int e, bool bf16) {
-    const uint32_t v = w[e >> 1];
-    return bf16 ? __builtin_bit_cast(float, e & 1 ? v & 0xffff0000u : v << 16) : (float)as_h2(v)[e & 1];
+// Two outputs, rounded to the nearest.
+__device__ __forceinline__ uint32_t out_pair(bool bf16, float a, float b) {
+    typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+    return bf16 ? __builtin_bit_cast(uint32_t, (bf2){(__bf16)a, (__bf16)b}) : as_u32((h2){(_Float16)a, (_Float16)b});
 }
-// A row enters times 2^(14 - exponent), its largest then in [2^13, 2^14) (less where that is below
-// 2^-60), and its scores times the factor are in the log2 domain.
-__device__ __forceinline__ int row_exponent(float top) { return top > 0.0f ? max(__builtin_amdgcn_frexp_expf(top), -60) : 14; }
+
+// A query row as the operand of the first product, N pieces of eight channels a lane.  float16 enters as it
+// is.  bfloat16 enters as float16 times 2^(14 - exponent), its largest then in [2^13, 2^14) (less where that
+// is below 2^-60), which its scores' factor takes back.  Returns the factor that turns scores to the log2 domain.
+__device__ __forceinline__ int row_exponent(uint32_t top_bf16) {  // of the largest's bits without its sign
+    const float top = __builtin_bit_cast(float, top_bf16 << 16);
+    return top > 0.0f ? max(__builtin_amdgcn_frexp_expf(top), -60) : 14;
+}
 __device__ __forceinline__ float row_factor(float scale_log2, int ex) { return __builtin_fmaxf(__builtin_ldexpf(scale_log2, ex - 14), 0x1p-126f); }
-template <int N, typename Value>
-__device__ __forceinline__ float scaled_row(h8 (&op)[N], Value value, float scale_log2) {
-    float top = 0.0f;
+typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+template <int N>
+__device__ __forceinline__ us2 largest(const u4 (&w)[N]) {
+    us2 top = {0, 0};
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = __builtin_fmaxf(top, __builtin_fabsf(value(i, e)));
-    const int ex = row_exponent(qmax(top));
+        for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(us2, (uint32_t)w[i][e] & 0x7fff7fffu));
+    return top;
+}
+// Two bfloat16 times x as float16.
+__device__ __forceinline__ uint32_t scaled_pair(uint32_t w, float x) {
+    const float lo = __builtin_fmaf(__builtin_bit_cast(float, w << 16), x, -0.0f), hi = __builtin_fmaf(__builtin_bit_cast(float, w & 0xffff0000u), x, -0.0f);
+    return as_u32((h2){(_Float16)lo, (_Float16)hi});
+}
+template <int N>
+__device__ __forceinline__ float query_operand(h8 (&op)[N], const u4 (&w)[N], int bf16, float scale_log2) {
+    if (!bf16) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+        for (int i = 0; i < N; ++i) op[i] = __builtin_bit_cast(h8, w[i]);
+        return __builtin_fmaxf(scale_log2, 0x1p-126f);
+    }
+    const us2 t = largest(w);
+    uint32_t top = max(t[0], t[1]);
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+    const int ex = row_exponent(top);
+    const float x = __builtin_ldexpf(1.0f, 14 - ex);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) op[i][e] = (_Float16)__builtin_ldexpf(value(i, e), 14 - ex);
+    for (int i = 0; i < N; ++i) {
+        u4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = scaled_pair(w[i][e], x);
+        op[i] = __builtin_bit_cast(h8, o);
+    }
     return row_factor(scale_log2, ex);
 }
 

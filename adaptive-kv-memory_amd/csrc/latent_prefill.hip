@@ -174,6 +174,31 @@ __device__ __forceinline__ int64_t uniform64(int64_t x) {
 }
 __device__ __forceinline__ int64_t share_of(int64_t total, int groups) { return max((total + groups - 1) / groups, (int64_t)(4 * kStep)); }
 
+// Value e of eight of a query row as float.
+template <bool BF16>
+__device__ __forceinline__ float query_value(u4 w, int e) {
+    const uint32_t v = w[e >> 1];
+    return BF16 ? __builtin_bit_cast(float, e & 1 ? v & 0xffff0000u : v << 16) : (float)as_h2(v)[e & 1];
+}
+// value(i, e) times a power of two that takes the row's largest to [2^13, 2^14) as float16; returns what
+// turns its scores to the log2 domain.
+template <int N, typename Value>
+__device__ __forceinline__ float scaled_row(h8 (&op)[N], Value value, float scale_log2) {
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = __builtin_fmaxf(top, __builtin_fabsf(value(i, e)));
+    top = qmax(top);
+    const int ex = top > 0.0f ? max(__builtin_amdgcn_frexp_expf(top), -60) : 14;
+    const float x = __builtin_ldexpf(1.0f, 14 - ex);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) op[i][e] = (_Float16)__builtin_fmaf(value(i, e), x, -0.0f);
+    return row_factor(scale_log2, ex);
+}
+
 // Row chunks of 16 bytes lie turned: eight rows read at one chunk, and the transposed reads of four rows
 // at two, fall on different banks.
 __device__ __forceinline__ int turn16(int row) { return (row & 3) << 1 | (row >> 2 & 1); }
@@ -258,10 +283,14 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void latent_prefill_kernel(const L
                 for (int i = 0; i < NI; ++i) raw[i] = *(const u4 *)(q + 64 * i);
 #pragma unroll
                 for (int i = 0; i < kD / 32; ++i) by[i][0] = ws[8 * i], by[i][1] = ws[8 * i + 1];
-                kx[r] = scaled_row(Q[r], [&](int i, int e) {
-                    const float v = query_value(raw[i], e, p.q_bf16);
-                    return i < kD / 32 ? v * by[i][e >> 2][e & 3] : v;
-                }, p.scale_log2);
+                auto make = [&](auto is_bf16) {
+                    kx[r] = scaled_row(Q[r], [&](int i, int e) {
+                        const float v = query_value<decltype(is_bf16)::value>(raw[i], e);
+                        return i < kD / 32 ? v * by[i][e >> 2][e & 3] : v;
+                    }, p.scale_log2);
+                };
+                if (p.q_bf16) make(std::true_type{});
+                else make(std::false_type{});
             }
             const int see_all = w.r.sees(p.causal, min(mine, w.rows - 1));  // what all of the wave's rows see
             const int kv = w.r.kv;
@@ -391,7 +420,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void latent_prefill_kernel(const L
 #pragma unroll
                         for (int b = 0; b < CB; ++b) {
                             const f4 v = acc[b][r] * inv * vs[4 * b];
-                            *(u2 *)(out + 32 * b) = (u2){to_pair(p.q_bf16, v[0], v[1]), to_pair(p.q_bf16, v[2], v[3])};
+                            *(u2 *)(out + 32 * b) = (u2){out_pair(p.q_bf16, v[0], v[1]), out_pair(p.q_bf16, v[2], v[3])};
                         }
                     }
                 } else {
@@ -472,7 +501,7 @@ __global__ __launch_bounds__(kThreads) void latent_prefill_merge_kernel(const La
 #pragma unroll
     for (int b = 0; b < CB; ++b) {
         const f4 v = acc[b] * inv * vs[4 * b];
-        *(u2 *)(out + 32 * b) = (u2){to_pair(p.q_bf16, v[0], v[1]), to_pair(p.q_bf16, v[2], v[3])};
+        *(u2 *)(out + 32 * b) = (u2){out_pair(p.q_bf16, v[0], v[1]), out_pair(p.q_bf16, v[2], v[3])};
     }
 }
 
