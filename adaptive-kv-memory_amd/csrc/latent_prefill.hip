@@ -27,81 +27,167 @@ constexpr int kGroups = 256;
 
 }  // namespace
 
+namespace {
+
+struct TileScan {
+    int64_t pre[kThreads + 1], wave_sum[kThreads / 64];
+};
+// What lies before each thread's sequences, of(s) for sequence s.
+template <typename Of>
+__device__ __forceinline__ void scan_sequences(int n_seqs, TileScan &sc, Of of) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, per = (n_seqs + kThreads - 1) / kThreads;
+    int64_t mine = 0, inc = 0;
+    if (t < kThreads) {
+        for (int i = 0; i < per; ++i)
+            if (t * per + i < n_seqs) mine += of(t * per + i);
+        inc = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int64_t o = __shfl_up(inc, d);
+            if (lane >= d) inc += o;
+        }
+        if (lane == 63) sc.wave_sum[wave] = inc;
+    }
+    __syncthreads();
+    if (t < kThreads) {
+        int64_t before = 0;
+        for (int w = 0; w < wave; ++w) before += sc.wave_sum[w];
+        sc.pre[t] = before + inc - mine;
+        if (t == kThreads - 1) sc.pre[kThreads] = before + inc;
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+    return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
+}
+// The first sequence of the thread whose sequences hold x, and how much of x lies in them; returns how many
+// sequences a thread has.
+__device__ __forceinline__ int seq_of_first(const TileScan &sc, int64_t x, int n_seqs, int &s, int64_t &off) {
+    const int per = (n_seqs + kThreads - 1) / kThreads;
+    int k = 0;
+    for (int i = 0; i < kThreads / 64; ++i) k += __builtin_popcountll(__builtin_amdgcn_ballot_w64(sc.pre[64 * i + (threadIdx.x & 63)] <= x));
+    s = (k - 1) * per;
+    off = x - uniform64(sc.pre[k - 1]);
+    return per;
+}
+
+}  // namespace
+
 // Expansion.  A workgroup holds 128 cached rows' latents in LDS and makes the 128 key and 128 value channels
-// of one head after another; a wave makes 64 of them for all 128 tokens, its weights coming straight from
-// memory in operand order.
+// of one head after another; a wave makes 64 of them for all 128 tokens.  Its weights come straight from
+// memory in operand order, a stream of 16-byte loads that runs half a head ahead and on over the heads.
+// All workgroups are at the same heads at about the same time, so that a chiplet's L2 reads them once.
 template <int DC>
 __global__ __launch_bounds__(kThreads, 1) void latent_expand_kernel(const LatentPrefillParams p) {
-    constexpr int LROW = 2 * DC, KS = DC / 32, TILES = kExpandTok / 16;
+    constexpr int LROW = 2 * DC, KS = DC / 32, TILES = kExpandTok / 16, RING = KS / 2;
     constexpr int PIECES = 16 * LROW / 1024;  // KiB of a tile's latents
     extern __shared__ __align__(1024) unsigned char smem[];
+    __shared__ TileScan sc;
+    // float16 results that overflow become the largest
+    __builtin_amdgcn_s_setreg(1 | 23 << 6, 1);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
-    const int s = blockIdx.y;
-    const SeqRows r = wave_uniform(seq_rows(p.seqs, s, p.pool.log_page));
-    const int tok0 = blockIdx.x * kExpandTok;
-    if (r.n == 0 || tok0 >= r.kv) return;
-    Pages pages{p.seqs.table + s * p.seqs.table_stride, p.seqs.width, 0, 0};
-    pages.fill(tok0 >> p.pool.log_page);
-    // chunk c of row t lies at c ^ (t & 7)
-#pragma unroll
-    for (int i = 0; i < TILES / 4; ++i) {
-        const int tile = wave + 4 * i;
-        const Tile at = tile_at(p.pool, pages, tok0 + 16 * tile, r.kv);
-        const u4 rsrc = wave_rsrc(at.at, at.rows * p.pool.row_bytes);
-#pragma unroll
-        for (int n = 0; n < PIECES; ++n) {
-            const int c = 64 * n + lane, row = c / (LROW / 16), in = c % (LROW / 16);
-            dma_kib(rsrc, __builtin_amdgcn_readfirstlane(lds_addr(smem) + tile * 16 * LROW + n * 1024),
-                    row * p.pool.row_bytes + ((in ^ (row & 7)) << 4));
-        }
+    auto tiles_of = [&](int s) {
+        const SeqRows r = seq_rows(p.seqs, s, p.pool.log_page);
+        return r.n == 0 ? 0 : (r.kv + kExpandTok - 1) / kExpandTok;
+    };
+    scan_sequences(p.seqs.n_seqs, sc, tiles_of);
+    const int tiles = __builtin_amdgcn_readfirstlane((int)sc.pre[kThreads]);
+    if (tiles == 0) return;
+    // The heads in blocks, as many as make the longest workgroup shortest.  A tile of latents costs about
+    // as much as two heads.
+    int blocks = 1;
+    float least = INFINITY;
+    for (int n = lane + 1; n <= p.heads; n += 64) {
+        const float cost = (float)(((int64_t)tiles * n + (int)gridDim.x - 1) / (int)gridDim.x) * (2 + (p.heads + n - 1) / n);
+        if (cost < least) least = cost, blocks = n;
     }
-    wait_vm<0>();
-    __syncthreads();
-    const uint32_t at = lds_addr(smem) + col * LROW;
-    const int h0 = blockIdx.z * p.tile_heads, h1 = min(p.heads, h0 + p.tile_heads);
-    for (int h = h0; h < h1; ++h) {
-        const int head = p.head0 + h;
-        const u4 *w = (const u4 *)p.w + ((int64_t)head * KS * 16 + wave * 4) * 64 + lane;
-        f4 acc[TILES][4];
 #pragma unroll
-        for (int t = 0; t < TILES; ++t)
+    for (int d = 1; d < 64; d <<= 1) {
+        const float cost = __shfl_xor(least, d);
+        const int n = __shfl_xor(blocks, d);
+        if (cost < least || (cost == least && n < blocks)) least = cost, blocks = n;
+    }
+    blocks = __builtin_amdgcn_readfirstlane(blocks);
+    const int each = (p.heads + blocks - 1) / blocks;
+    for (int64_t item = blockIdx.x; item < (int64_t)tiles * blocks; item += gridDim.x) {
+        const int block = (int)(item / tiles), tile = (int)(item - (int64_t)block * tiles);
+        const int h0 = block * each, h1 = min(p.heads, h0 + each);
+        if (h0 >= h1) break;
+        int s, tok0;
+        {
+            int64_t off;
+            const int per = seq_of_first(sc, tile, p.seqs.n_seqs, s, off);
+            for (int i = 0; i < per; ++i) {
+                const int n = tiles_of(s);
+                if (off < n) break;
+                off -= n, ++s;
+            }
+            s = __builtin_amdgcn_readfirstlane(s), tok0 = __builtin_amdgcn_readfirstlane((int)off * kExpandTok);
+        }
+        const SeqRows r = wave_uniform(seq_rows(p.seqs, s, p.pool.log_page));
+        const u4 *w = (const u4 *)p.w + ((int64_t)(p.head0 + h0) * KS * 16 + wave * 4) * 64 + lane;
+        const int last = (h1 - h0) * KS - 1;  // step of the stream: the heads lie one after the other
+        u4 W[RING][4];
 #pragma unroll
-            for (int b = 0; b < 4; ++b) acc[t][b] = (f4){0.f, 0.f, 0.f, 0.f};
-        u4 W[2][4];
+        for (int u = 0; u < RING - 1; ++u)
 #pragma unroll
-        for (int b = 0; b < 4; ++b) W[0][b] = w[b * 64];
+            for (int b = 0; b < 4; ++b) W[u][b] = w[(u * 16 + b) * 64];
+        Pages pages{p.seqs.table + s * p.seqs.table_stride, p.seqs.width, 0, 0};
+        pages.fill(tok0 >> p.pool.log_page);
+        __syncthreads();  // the tile before is read
+        // chunk c of row t lies at c ^ (t & 7)
 #pragma unroll 1
-        for (int k = 0; k < KS; k += 2)
+        for (int i = 0; i < TILES / 4; ++i) {
+            const int t = wave + 4 * i;
+            const Tile at = tile_at(p.pool, pages, tok0 + 16 * t, r.kv);
+            const u4 rsrc = wave_rsrc(at.at, at.rows * p.pool.row_bytes);
+#pragma unroll 1
+            for (int n = 0; n < PIECES; ++n) {
+                const int c = 64 * n + lane, row = c / (LROW / 16), in = c % (LROW / 16);
+                dma_kib(rsrc, __builtin_amdgcn_readfirstlane(lds_addr(smem) + t * 16 * LROW + n * 1024),
+                        row * p.pool.row_bytes + ((in ^ (row & 7)) << 4));
+            }
+        }
+        wait_vm<0>();
+        __syncthreads();
+        const uint32_t at = lds_addr(smem) + col * LROW;
+        for (int h = h0; h < h1; ++h) {
+            f4 acc[TILES][4];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int next = min(k + u + 1, KS - 1);
+            for (int t = 0; t < TILES; ++t)
 #pragma unroll
-                for (int b = 0; b < 4; ++b) W[u ^ 1][b] = w[(next * 16 + b) * 64];
+                for (int b = 0; b < 4; ++b) acc[t][b] = (f4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int k = 0; k < KS; k += RING)
 #pragma unroll
-                for (int t = 0; t < TILES; ++t) {
-                    const h8 c = __builtin_bit_cast(h8, *lds_ptr<u4>(at + t * 16 * LROW + (((4 * (k + u) + grp) ^ (col & 7)) << 4)));
+                for (int u = 0; u < RING; ++u) {
+                    const int64_t next = min((h - h0) * KS + k + u + RING - 1, last);
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) acc[t][b] = mfma_k32(__builtin_bit_cast(h8, W[u][b]), c, acc[t][b]);
+                    for (int b = 0; b < 4; ++b) W[(u + RING - 1) % RING][b] = w[(next * 16 + b) * 64];
+#pragma unroll
+                    for (int t = 0; t < TILES; ++t) {
+                        const h8 c = __builtin_bit_cast(h8, *lds_ptr<u4>(at + t * 16 * LROW + (((4 * (k + u) + grp) ^ (col & 7)) << 4)));
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) acc[t][b] = mfma_k32(__builtin_bit_cast(h8, W[u][b]), c, acc[t][b]);
+                    }
                 }
+            // a lane has 16 consecutive channels of token col of every tile
+            unsigned char *to = (wave < 2 ? p.keys : p.values) +
+                                (((int64_t)h * p.cap + s * p.seq_cap + tok0 + col) * kD + 64 * (wave & 1) + 16 * grp) * 2;
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+                if (tok0 + 16 * t + col >= p.seq_cap) continue;
+                u4 o[2];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const f4 v = acc[t][b];
+                    o[b >> 1][2 * (b & 1)] = as_u32((h2){(_Float16)v[0], (_Float16)v[1]});
+                    o[b >> 1][2 * (b & 1) + 1] = as_u32((h2){(_Float16)v[2], (_Float16)v[3]});
+                }
+                ((u4 *)(to + (int64_t)t * 16 * kD * 2))[0] = o[0];
+                ((u4 *)(to + (int64_t)t * 16 * kD * 2))[1] = o[1];
             }
-        // a lane has 16 consecutive channels of token col of every tile
-        unsigned char *to = (wave < 2 ? p.keys : p.values) +
-                            (((int64_t)h * p.cap + s * p.seq_cap + tok0 + col) * kD + 64 * (wave & 1) + 16 * grp) * 2;
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-            if (tok0 + 16 * t + col >= p.seq_cap) continue;
-            u4 o[2];
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                f4 v = acc[t][b];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = v[e] != v[e] ? v[e] : __builtin_amdgcn_fmed3f(v[e], -65504.0f, 65504.0f);
-                o[b >> 1][2 * (b & 1)] = as_u32((h2){(_Float16)v[0], (_Float16)v[1]});
-                o[b >> 1][2 * (b & 1) + 1] = as_u32((h2){(_Float16)v[2], (_Float16)v[3]});
-            }
-            ((u4 *)(to + (int64_t)t * 16 * kD * 2))[0] = o[0];
-            ((u4 *)(to + (int64_t)t * 16 * kD * 2))[1] = o[1];
         }
     }
 }
@@ -137,40 +223,12 @@ __device__ __forceinline__ int steps_before(int64_t c, int64_t cost, int steps) 
     const int64_t x = (c - kSetupTok + kStep - 1) / kStep;
     return (int)(x < 0 ? 0 : x > steps ? steps : x);
 }
-struct TileScan {
-    int64_t pre[kThreads + 1], wave_sum[kThreads / 64];
-};
 template <int R>
 __device__ __forceinline__ void scan_tiles(const LatentPrefillParams &p, TileScan &sc) {
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, per = (p.seqs.n_seqs + kThreads - 1) / kThreads;
-    int64_t mine = 0, inc = 0;
-    if (t < kThreads) {
-        for (int i = 0; i < per; ++i) {
-            const int s = t * per + i;
-            if (s < p.seqs.n_seqs) {
-                const TileWork w = tile_work<R>(p, seq_rows(p.seqs, s, p.pool.log_page));
-                mine += w.before(w.tiles) * p.heads;
-            }
-        }
-        inc = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int64_t o = __shfl_up(inc, d);
-            if (lane >= d) inc += o;
-        }
-        if (lane == 63) sc.wave_sum[wave] = inc;
-    }
-    __syncthreads();
-    if (t < kThreads) {
-        int64_t before = 0;
-        for (int w = 0; w < wave; ++w) before += sc.wave_sum[w];
-        sc.pre[t] = before + inc - mine;
-        if (t == kThreads - 1) sc.pre[kThreads] = before + inc;
-    }
-    __syncthreads();
-}
-__device__ __forceinline__ int64_t uniform64(int64_t x) {
-    return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
+    scan_sequences(p.seqs.n_seqs, sc, [&](int s) {
+        const TileWork w = tile_work<R>(p, seq_rows(p.seqs, s, p.pool.log_page));
+        return w.before(w.tiles) * p.heads;
+    });
 }
 __device__ __forceinline__ int64_t share_of(int64_t total, int groups) { return max((total + groups - 1) / groups, (int64_t)(4 * kStep)); }
 
@@ -228,7 +286,6 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void latent_prefill_kernel(const L
     const uint32_t v_at = KB + vrow * kD * 2 + 8 * (col & 1);
 
     scan_tiles<R>(p, sc);
-    const int per = (p.seqs.n_seqs + kThreads - 1) / kThreads;
     const int64_t total = uniform64(sc.pre[kThreads]);
     const int64_t share = share_of(total, p.groups);
     if (blockIdx.x == 0 && threadIdx.x < kThreads) {
@@ -242,10 +299,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void latent_prefill_kernel(const L
     int64_t c0;  // where in the tile's cost the run stands
     TileWork w;
     {
-        int k = 0;
-        for (int i = 0; i < kThreads / 64; ++i) k += __builtin_popcountll(__builtin_amdgcn_ballot_w64(sc.pre[64 * i + lane] <= x));
-        s = (k - 1) * per;
-        int64_t off = x - uniform64(sc.pre[k - 1]);
+        int64_t off;
+        seq_of_first(sc, x, p.seqs.n_seqs, s, off);
         for (;;) {
             w = tile_work<R>(p, wave_uniform(seq_rows(p.seqs, s, p.pool.log_page)));
             const int64_t n = w.before(w.tiles) * p.heads;
@@ -540,16 +595,11 @@ hipError_t latent_prefill_launch(const LatentPrefillParams &p0, hipStream_t st) 
         (void)hipFuncSetAttribute((const void *)attend, hipFuncAttributeMaxDynamicSharedMemorySize, lds_a);
         for (p.head0 = 0; p.head0 < p.H; p.head0 += most) {
             p.heads = std::min(most, p.H - p.head0);
-            const int64_t tiles = (((int64_t)p.seqs.width << p.pool.log_page) + kExpandTok - 1) / kExpandTok;
-            if (tiles) {
-                p.tile_heads = (int)std::max<int64_t>(1, std::min<int64_t>(8, p.heads * tiles * p.seqs.n_seqs / 1024));
-                const dim3 grid((unsigned)tiles, p.seqs.n_seqs, (p.heads + p.tile_heads - 1) / p.tile_heads);
-                expand<<<grid, dim3(kThreads), lds_e, st>>>(p);
-                const hipError_t e = hipGetLastError();
-                if (e != hipSuccess) return e;
-            }
-            attend<<<dim3(p.groups), dim3(64 * NW), lds_a, st>>>(p);
+            expand<<<dim3(p.groups), dim3(kThreads), lds_e, st>>>(p);
             hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+            attend<<<dim3(p.groups), dim3(64 * NW), lds_a, st>>>(p);
+            e = hipGetLastError();
             if (e != hipSuccess) return e;
             const int64_t blocks = ((int64_t)(p.seqs.max_q + 32 * NW - 1) / (32 * NW) * (2 * NW) + 3) / 4;
             latent_prefill_merge_kernel<32 * NW><<<dim3((unsigned)blocks, p.heads, p.seqs.n_seqs), dim3(kThreads), 0, st>>>(p);
