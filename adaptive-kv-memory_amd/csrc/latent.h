@@ -60,7 +60,7 @@ struct LatentPrefillParams {
     unsigned char *keys, *values;  // [heads][cap] rows of kLatentHead float16
     int64_t cap, seq_cap;      // rows of a head, and of a sequence in it
     int head0, heads;          // those of this pass
-    int groups, waves;         // workgroups, and the attention's waves of one
+    int groups, rows;          // workgroups, and the attention's query tokens of one
 };
 
 struct LatentImportanceParams {

@@ -20,6 +20,7 @@ namespace {
 
 constexpr int kD = kLatentHead;       // channels of a head's own keys, and of its values
 constexpr int kThreads = 256;         // of the scan, the expansion and the merge
+constexpr int kAttendThreads = 512;
 constexpr int kExpandTok = 128;       // tokens of a workgroup of the expansion
 constexpr int kStep = 64;             // tokens of a step of the attention
 constexpr int kSetupTok = 2 * kStep;  // what an item's start counts
@@ -136,7 +137,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_expand_kernel(const Latent
         Pages pages{p.seqs.table + s * p.seqs.table_stride, p.seqs.width, 0, 0};
         pages.fill(tok0 >> p.pool.log_page);
         __syncthreads();  // the tile before is read
-        // chunk c of row t lies at c ^ (t & 7)
+        // chunk c of row t lies at c ^ t % 16, so that the sixteen chunks that a read takes at once differ
 #pragma unroll 1
         for (int i = 0; i < TILES / 4; ++i) {
             const int t = wave + 4 * i;
@@ -146,7 +147,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_expand_kernel(const Latent
             for (int n = 0; n < PIECES; ++n) {
                 const int c = 64 * n + lane, row = c / (LROW / 16), in = c % (LROW / 16);
                 dma_kib(rsrc, __builtin_amdgcn_readfirstlane(lds_addr(smem) + t * 16 * LROW + n * 1024),
-                        row * p.pool.row_bytes + ((in ^ (row & 7)) << 4));
+                        row * p.pool.row_bytes + ((in ^ (row & 15)) << 4));
             }
         }
         wait_vm<0>();
@@ -167,7 +168,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_expand_kernel(const Latent
                     for (int b = 0; b < 4; ++b) W[(u + RING - 1) % RING][b] = w[(next * 16 + b) * 64];
 #pragma unroll
                     for (int t = 0; t < TILES; ++t) {
-                        const h8 c = __builtin_bit_cast(h8, *lds_ptr<u4>(at + t * 16 * LROW + (((4 * (k + u) + grp) ^ (col & 7)) << 4)));
+                        const h8 c = __builtin_bit_cast(h8, *lds_ptr<u4>(at + t * 16 * LROW + (((4 * (k + u) + grp) ^ col) << 4)));
 #pragma unroll
                         for (int b = 0; b < 4; ++b) acc[t][b] = mfma_k32(__builtin_bit_cast(h8, W[u][b]), c, acc[t][b]);
                     }
@@ -257,33 +258,45 @@ __device__ __forceinline__ float scaled_row(h8 (&op)[N], Value value, float scal
     return row_factor(scale_log2, ex);
 }
 
-// Row chunks of 16 bytes lie turned: eight rows read at one chunk, and the transposed reads of four rows
-// at two, fall on different banks.
-__device__ __forceinline__ int turn16(int row) { return (row & 3) << 1 | (row >> 2 & 1); }
+// 64 pages of a sequence's table in a wave's lanes, and which of them are pages of the pool.
+struct StepPages {
+    int first, ids;
+    uint64_t valid;
+    __device__ __forceinline__ void fill(const LatentPrefillParams &p, int s, int page) {
+        first = __builtin_amdgcn_readfirstlane(page);
+        const int at = page + lane_again();
+        ids = at < p.seqs.width ? p.seqs.table[s * p.seqs.table_stride + at] : -1;
+        valid = __builtin_amdgcn_ballot_w64((uint32_t)ids < p.pool.n_pages);  // waited for here
+    }
+};
 
 }  // namespace
 
-// Attention.  A workgroup of NW waves takes 32 NW query tokens of one head, each wave 32 of them, and
-// walks the keys and values in steps of 64 tokens, three buffers in LDS that buffer loads fill: the keys' own
-// channels, the shared rotated ones straight from the cache's rows, the values.  S^T = K Q^T leaves a lane with
-// its row's scores of the tokens that the second product's operand wants, so p stays in registers.
-template <int DC, int NW>
-__global__ __launch_bounds__(64 * NW, NW / 4) void latent_prefill_kernel(const LatentPrefillParams p) {
-    constexpr int R = 32 * NW, SLOTS = 3, KB = kStep * kD * 2, RB = kStep * kLatentRope * 2, SLOT = 2 * KB + RB;
-    constexpr int LOADS = SLOT / 1024 / NW, CB = kD / 16, NI = (kD + kLatentRope) / 32, ROWB = 2 * (DC + kLatentRope);
+// Attention.  A workgroup of eight waves takes 128 RB query tokens of one head, each wave 16 RB of them, and
+// walks the keys and values in steps of 64 tokens.  Buffer loads fill two rings of three steps in LDS: the keys'
+// own channels with the shared rotated ones, straight from the cache's rows, and the values.
+// S^T = K Q^T leaves a lane with its row's scores of the tokens that the second product's operand wants, so p
+// stays in registers.  A SIMD has two waves, which take turns: while one multiplies (the values of its last step,
+// then the keys of the next) the other turns scores into p.  The second four waves do so by standing at one barrier
+// more before their first step.
+template <int DC, int RB>
+__global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const LatentPrefillParams p) {
+    constexpr int NW = kAttendThreads / 64, R = 16 * RB * NW, SLOTS = 3, VB = kStep * kD * 2, KB = VB + kStep * kLatentRope * 2;
+    constexpr int LOADS = (KB + VB) / 1024 / NW, CB = kD / 16, NI = (kD + kLatentRope) / 32, ROWB = 2 * (DC + kLatentRope);
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ TileScan sc;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 15, grp = lane >> 4;
+    const int col = lane & 15, grp = lane >> 4, second = wave / (NW / 2);
     const uint32_t ring = lds_addr(smem);
-    // keys and values: a piece is four rows; rotated keys: eight
-    const uint32_t kv_off[2] = {(uint32_t)((lane >> 4) * kD * 2 + ((col ^ turn16(grp)) << 4)),
-                                (uint32_t)((lane >> 4) * kD * 2 + ((col ^ turn16(grp + 4)) << 4))};
-    const uint32_t r_off = (lane >> 3) * ROWB + 2 * DC + (((lane & 7) ^ turn(lane >> 3)) << 4);
-    const uint32_t k_at = col * kD * 2;                                     // chunk c at c ^ turn16(col)
-    const uint32_t r_at = 2 * KB + col * kLatentRope * 2 + ((grp ^ turn(col)) << 4);
+    // Rows' 16-byte chunks lie turned so that the sixteen slots of 256 bytes that a read takes at once differ:
+    // chunk c of a row of keys at c ^ row % 16, of rotated keys at c ^ row / 2 % 8, of values at
+    // c ^ 2 (row % 8).  A load of 1 KiB brings four rows of keys or values, eight of rotated keys.
+    const uint32_t k_off = grp * kD * 2 + ((col ^ grp) << 4), v_off = grp * kD * 2 + ((col ^ 2 * grp) << 4);
+    const uint32_t r_off = (lane >> 3) * ROWB + 2 * DC + (((lane & 7) ^ grp) << 4);
+    const uint32_t k_at = col * kD * 2 + ((grp ^ col) << 4);
+    const uint32_t r_at = VB + col * kLatentRope * 2 + ((grp ^ col >> 1) << 4);
     const int vrow = 4 * grp + (col >> 2);
-    const uint32_t v_at = KB + vrow * kD * 2 + 8 * (col & 1);
+    const uint32_t v_at = vrow * kD * 2 + (((col & 3) >> 1 ^ 2 * (vrow & 7)) << 4) + 8 * (col & 1);
 
     scan_tiles<R>(p, sc);
     const int64_t total = uniform64(sc.pre[kThreads]);
@@ -322,12 +335,12 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void latent_prefill_kernel(const L
         x += c1 - c0;
         if (j1 > j0 || (starts && ends)) {
             const int row0 = tile * R, head = p.head0 + h;
-            const int mine = row0 + 32 * wave;
-            int see[2];
-            float kx[2];
-            h8 Q[2][NI];
+            const int mine = row0 + 16 * RB * wave;
+            int see[RB];
+            float kx[RB];
+            h8 Q[RB][NI];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+            for (int r = 0; r < RB; ++r) {
                 const int row = min(mine + 16 * r + col, w.rows - 1);
                 see[r] = w.r.sees(p.causal, row);
                 const unsigned char *q = p.q + (w.r.begin + row) * p.q_t + head * p.q_h + 16 * grp;
@@ -349,86 +362,143 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void latent_prefill_kernel(const L
             }
             const int see_all = w.r.sees(p.causal, min(mine, w.rows - 1));  // what all of the wave's rows see
             const int kv = w.r.kv;
-            Pages pages{p.seqs.table + s * p.seqs.table_stride, p.seqs.width, 0, 0};
+            const int lp = p.pool.log_page;
+            StepPages pages;
             const int64_t base = ((int64_t)h * p.cap + s * p.seq_cap) * kD * 2;
             uint32_t there = 0;  // bits 4 slot ..
-            auto load = [&](int j, int slot) {
-                const int k = j * kStep, end = j < j1 ? kv : 0;
-                const int left = max(0, min(end - k, kStep));
-                const u4 rk = wave_rsrc(p.keys + base + (int64_t)k * kD * 2, left * kD * 2);
-                const u4 rv = wave_rsrc(p.values + base + (int64_t)k * kD * 2, left * kD * 2);
-                const uint32_t lds = __builtin_amdgcn_readfirstlane(ring + slot * SLOT);
+            auto load = [&](int j, int k_slot, int v_slot) {  // the keys of step j and the values of the one before
+                const int k = j * kStep, end = j < j1 ? kv : 0, before = k - kStep, v_end = j <= j1 ? kv : 0;
+                const u4 rk = wave_rsrc(p.keys + base + (int64_t)k * kD * 2, max(0, min(end - k, kStep)) * kD * 2);
+                const uint32_t to_k = __builtin_amdgcn_readfirstlane(ring + k_slot * KB);
 #pragma unroll
-                for (int i = 0; i < 16 / NW; ++i) {
-                    const int n = wave * (16 / NW) + i;  // (parity of n: the lane's offset)
-                    dma_kib(rk, lds + n * 1024, kv_off[i & 1] + n * 1024);
-                    dma_kib(rv, lds + KB + n * 1024, kv_off[i & 1] + n * 1024);
+                for (int i = 0; i < 2; ++i) {
+                    const int n = 2 * wave + i;
+                    dma_kib(rk, to_k + n * 1024, (k_off ^ (n & 3) << 6) + n * 1024);
                 }
-                uint32_t bits = 0;
+                const int page = k >> lp;
+                if (page + (48 >> lp) - pages.first >= 64) pages.fill(p, s, page);
+                const uint64_t valid = pages.valid >> (page - pages.first);
+                const uint32_t bits = (uint32_t)(valid & 1) | (uint32_t)(valid >> (16 >> lp) & 1) << 1 |
+                                      (uint32_t)(valid >> (32 >> lp) & 1) << 2 | (uint32_t)(valid >> (48 >> lp) & 1) << 3;
+                // the rotated keys of this wave's eight tokens
+                const int tok = k + 8 * wave, in = (tok >> lp) - pages.first;
+                const int rows = pages.valid >> in & 1 ? max(0, min(end - tok, 8)) : 0;
+                const unsigned char *rows_at = p.pool.base + (int64_t)__builtin_amdgcn_readlane(pages.ids, in) * p.pool.page_bytes +
+                                               (int64_t)(tok & ((1 << lp) - 1)) * ROWB;
+                dma_kib(wave_rsrc(rows_at, rows * ROWB), to_k + VB + wave * 1024, r_off ^ (wave & 1) << 6);
+                there = (there & ~(15u << 4 * k_slot)) | bits << 4 * k_slot;
+                if (j > j0) {
+                    const u4 rv = wave_rsrc(p.values + base + (int64_t)before * kD * 2, max(0, min(v_end - before, kStep)) * kD * 2);
+                    const uint32_t to_v = __builtin_amdgcn_readfirstlane(ring + SLOTS * KB + v_slot * VB);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const Tile t = tile_at(p.pool, pages, k + 16 * i, end);
-                    bits |= (uint32_t)t.there << i;
-                    if (i == (wave * (8 / NW)) >> 1) {
-                        const u4 rr = wave_rsrc(t.at, t.rows * ROWB);
-#pragma unroll
-                        for (int e = 0; e < 8 / NW; ++e) {
-                            const int n = wave * (8 / NW) + e;
-                            dma_kib(rr, lds + 2 * KB + n * 1024, r_off + (n & 1) * 8 * ROWB);
-                        }
+                    for (int i = 0; i < 2; ++i) {
+                        const int n = 2 * wave + i;
+                        dma_kib(rv, to_v + n * 1024, (v_off ^ (n & 1) << 7) + n * 1024);
                     }
                 }
-                there = (there & ~(15u << 4 * slot)) | bits << 4 * slot;
             };
-            pages.fill((j0 * kStep) >> p.pool.log_page);
+            auto after = [](int slot) { return slot + 1 == SLOTS ? 0 : slot + 1; };
+            float mx[RB], l[RB];
+            f4 acc[CB][RB];
+            u4 P[2][RB];  // of 32 tokens each
 #pragma unroll
-            for (int i = 0; i < SLOTS - 1; ++i) load(j0 + i, i);
-            float mx[2] = {kMinMax, kMinMax}, l[2] = {0.0f, 0.0f};
-            f4 acc[CB][2];
+            for (int r = 0; r < RB; ++r) {
+                mx[r] = kMinMax, l[r] = 0.0f;
 #pragma unroll
-            for (int b = 0; b < CB; ++b) acc[b][0] = acc[b][1] = (f4){0.f, 0.f, 0.f, 0.f};
-            int slot = 0, ahead = SLOTS - 1;
-            for (int j = j0; j < j1; ++j) {
-                wait_vm<(SLOTS - 2) * LOADS>();
+                for (int b = 0; b < CB; ++b) acc[b][r] = (f4){0.f, 0.f, 0.f, 0.f};
+                P[0][r] = P[1][r] = (u4){0, 0, 0, 0};
+            }
+            constexpr int V_AHEAD = 6, K_AHEAD = 8;  // reads that are under way
+            auto value = [&](uint32_t va, int n) {
+                const uint32_t a = (va ^ (n % CB) << 5) + n / CB * 32 * kD * 2;
+                const u2 lo = read_transposed(a), hi = read_transposed(a + 16 * kD * 2);
+                return __builtin_bit_cast(h8, (u4){lo[0], lo[1], hi[0], hi[1]});
+            };
+            // p times the values; then(m) in the steps that read no more of them
+            auto add_values = [&](uint32_t va, auto then) {
+                constexpr int READS = 2 * CB;
+                h8 V[V_AHEAD];
+#pragma unroll
+                for (int n = 0; n < V_AHEAD; ++n) V[n] = value(va, n);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int n = 0; n < READS; ++n) {
+#pragma unroll
+                    for (int r = 0; r < RB; ++r) acc[n % CB][r] = mfma_k32(V[n % V_AHEAD], __builtin_bit_cast(h8, P[n / CB][r]), acc[n % CB][r]);
+                    if (n + V_AHEAD < READS) V[n % V_AHEAD] = value(va, n + V_AHEAD);
+                    else then(n + V_AHEAD - READS);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+            const uint32_t values = ring + SLOTS * KB + v_at;
+            auto meet = [&]() {
                 wait_lgkm0();
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
-                load(j + SLOTS - 1, ahead);
-                const uint32_t at = ring + slot * SLOT, first = j * kStep;
+            };
+            pages.fill(p, s, (j0 * kStep) >> lp);
+            load(j0, 0, 0);
+            load(j0 + 1, 1, 0);
+            wait_vm<LOADS>();
+            int slot = 0;  // of step j, for keys and for values
+            if (second) {
+                meet();
+                load(j0 + 2, 2, 1);
+            }
+            for (int j = j0; j < j1; ++j) {
+                wait_vm<LOADS>();
+                meet();
+                const int next = after(slot), last = after(next);
+                const uint32_t ka = ring + slot * KB + k_at, ra = ring + slot * KB + r_at;
+                auto key = [&](int n) {
+                    const int c = n >> 2, i = n & 3;
+                    return __builtin_bit_cast(h8, *lds_ptr<u4>(c < kD / 32 ? (ka ^ c << 6) + i * 16 * kD * 2
+                                                                          : (ra ^ (c - kD / 32) << 6) + i * 16 * kLatentRope * 2));
+                };
+                h8 K[K_AHEAD];
+                auto read_keys = [&](int from, int to) {
+#pragma unroll
+                    for (int n = from; n < to; ++n) K[n] = key(n);
+                };
+                if (j > j0) add_values(values + last * VB, [&](int m) { read_keys(m * K_AHEAD / V_AHEAD, (m + 1) * K_AHEAD / V_AHEAD); });
+                else read_keys(0, K_AHEAD);
+                __builtin_amdgcn_sched_barrier(0);
+                f4 S[4][RB] = {};
+#pragma unroll
+                for (int n = 0; n < 4 * NI; ++n) {
+#pragma unroll
+                    for (int r = 0; r < RB; ++r) S[n & 3][r] = mfma_k32(K[n % K_AHEAD], Q[r][n >> 2], S[n & 3][r]);
+                    if (n + K_AHEAD < 4 * NI) K[n % K_AHEAD] = key(n + K_AHEAD);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                const int first = j * kStep;
                 const uint32_t have = there >> 4 * slot & 15;
-                slot = slot + 1 == SLOTS ? 0 : slot + 1;
-                ahead = ahead + 1 == SLOTS ? 0 : ahead + 1;
-                f4 S[4][2] = {};
-#pragma unroll
-                for (int c = 0; c < NI; ++c)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t a = c < kD / 32 ? at + k_at + i * 16 * kD * 2 + (((4 * c + grp) ^ turn16(col & 7)) << 4)
-                                                       : at + (r_at ^ (64 * (c - kD / 32))) + i * 16 * kLatentRope * 2;
-                        const h8 k = __builtin_bit_cast(h8, *lds_ptr<u4>(a));
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) S[i][r] = mfma_k32(k, Q[r][c], S[i][r]);
-                    }
-                if (!((int)first + kStep <= see_all && have == 15))
+                meet();
+                if (second) load(j + 3, slot, last);
+                else load(j + 2, last, next);
+                if (!(first + kStep <= see_all && have == 15)) {
+                    int at0 = first + 4 * grp;
+                    asm volatile("" : "+v"(at0));  // (nothing of this is computed where nothing is masked)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
-                        for (int r = 0; r < 2; ++r)
+                        for (int r = 0; r < RB; ++r)
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
-                                if ((int)first + 16 * i + 4 * grp + e >= see[r] || !(have >> i & 1)) S[i][r][e] = -INFINITY;
-                float top[2];
+                                if (at0 + 16 * i + e >= see[r] || !(have >> i & 1)) S[i][r][e] = -INFINITY;
+                }
+                float top[RB];
                 bool over = false;
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
+                for (int r = 0; r < RB; ++r) {
                     top[r] = S[0][r][0];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) top[r] = __builtin_fmaxf(top[r], S[i >> 2][r][i & 3]);
+                    for (int i = 1; i < 16; ++i) top[r] = __builtin_fmaxf(top[r], S[i >> 2][r][i & 3]);
                     over |= __builtin_fmaf(top[r], kx[r], kBias - mx[r]) > kBias + kLagBy;
                 }
                 if (__builtin_amdgcn_ballot_w64(over)) {
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
+                    for (int r = 0; r < RB; ++r) {
                         const float most = qmax(top[r]);
                         const float mn = __builtin_fmaf(most, kx[r], kBias - mx[r]) > kBias ? running_max(most, kx[r], kBias) : mx[r];
                         const float alpha = __builtin_amdgcn_exp2f(mx[r] - mn);
@@ -438,9 +508,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void latent_prefill_kernel(const L
                         for (int b = 0; b < CB; ++b) acc[b][r] *= alpha;
                     }
                 }
-                u4 P[2][2];  // of 32 tokens each
 #pragma unroll
-                for (int r = 0; r < 2; ++r)
+                for (int r = 0; r < RB; ++r)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         float e[4];
@@ -450,21 +519,15 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void latent_prefill_kernel(const L
                         P[i >> 1][r][2 * (i & 1)] = as_u32((h2){(_Float16)e[0], (_Float16)e[1]});
                         P[i >> 1][r][2 * (i & 1) + 1] = as_u32((h2){(_Float16)e[2], (_Float16)e[3]});
                     }
-#pragma unroll
-                for (int b = 0; b < CB; ++b)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t a = at + v_at + i * 32 * kD * 2 + (((2 * b + ((col & 3) >> 1)) ^ turn16(vrow & 7)) << 4);
-                        const u2 lo = read_transposed(a), hi = read_transposed(a + 16 * kD * 2);
-                        const h8 v = __builtin_bit_cast(h8, (u4){lo[0], lo[1], hi[0], hi[1]});
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) acc[b][r] = mfma_k32(v, __builtin_bit_cast(h8, P[i][r]), acc[b][r]);
-                    }
+                slot = next;
             }
             wait_vm<0>();
+            meet();
+            if (j1 > j0) add_values(values + (slot == 0 ? SLOTS - 1 : slot - 1) * VB, [](int) {});
+            if (!second) meet();
             float *e = p.part + ((int64_t)blockIdx.x * 2 + starts) * (R * (kD + 2));
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+            for (int r = 0; r < RB; ++r) {
                 l[r] = qsum(l[r]);
                 const int row = mine + 16 * r + col;
                 if (starts && ends) {
@@ -479,7 +542,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void latent_prefill_kernel(const L
                         }
                     }
                 } else {
-                    const int at = 2 * wave + r;
+                    const int at = RB * wave + r;
 #pragma unroll
                     for (int b = 0; b < CB; ++b) *(f4 *)(e + (at * CB + b) * 256 + lane * 4) = acc[b][r];
                     if (grp == 0) e[R * kD + 16 * at + col] = mx[r], e[R * kD + R + 16 * at + col] = l[r];
@@ -518,7 +581,14 @@ __global__ __launch_bounds__(kThreads) void latent_prefill_merge_kernel(const La
         start += b.before(b.tiles) * p.heads;
     }
     const int64_t share = share_of(p.sums[kThreads], p.groups), cost = w.cost(tile);
-    const int g0 = (int)(start / share), g1 = (int)((start + cost - 1) / share);
+    // start / share and (start + cost - 1) / share: below 2^8, so that the product errs by less than one
+    const float one = 1.0f / (float)share;
+    auto run_of = [&](int64_t at) {
+        int g = (int)((float)at * one);
+        g -= g * share > at;
+        return g + ((g + 1) * share <= at);
+    };
+    const int g0 = run_of(start), g1 = run_of(start + cost - 1);
     if (g0 == g1) return;
     const int steps = steps_of<R>(p, w, tile);
     // the runs that hold steps of it, and whether a run's entry is the one whose item starts there
@@ -528,27 +598,27 @@ __global__ __launch_bounds__(kThreads) void latent_prefill_merge_kernel(const La
         return steps_before(c1, cost, steps) > steps_before(c0, cost, steps);
     };
     auto entry = [&](int g, int64_t c0) { return p.part + ((int64_t)g * 2 + (c0 <= kSetupTok)) * (R * (kD + 2)); };
-    float m = kMinMax;
-    int64_t c0;
+    float m = kMinMax, l = 0.0f;
+    f4 acc[CB] = {};
     int n = 0;
     bool whole = false;
-    for (int g = g0; g <= g1; ++g)
-        if (part(g, c0)) {
-            m = __builtin_fmaxf(m, entry(g, c0)[R * kD + 16 * in + col]);
-            ++n;
-            whole = c0 <= kSetupTok && g == g1;
-        }
-    if (n == 1 && whole) return;  // one run held all of it and wrote the rows
-    float l = 0.0f;
-    f4 acc[CB] = {};
-    for (int g = g0; g <= g1; ++g)
-        if (part(g, c0)) {
-            const float *e = entry(g, c0);
-            const float a = __builtin_amdgcn_exp2f(e[R * kD + 16 * in + col] - m);
-            l += e[R * kD + R + 16 * in + col] * a;
+    for (int g = g0; g <= g1; ++g) {
+        int64_t c0;
+        if (!part(g, c0)) continue;
+        ++n;
+        whole = c0 <= kSetupTok && g == g1;
+        if (whole && n == 1) return;  // one run held all of it and wrote the rows
+        const float *e = entry(g, c0);
+        const float m_e = e[R * kD + 16 * in + col], l_e = e[R * kD + R + 16 * in + col];
+        f4 a_e[CB];
 #pragma unroll
-            for (int b = 0; b < CB; ++b) acc[b] += *(const f4 *)(e + (in * CB + b) * 256 + lane * 4) * a;
-        }
+        for (int b = 0; b < CB; ++b) a_e[b] = *(const f4 *)(e + (in * CB + b) * 256 + lane * 4);
+        const float most = __builtin_fmaxf(m, m_e), old = __builtin_amdgcn_exp2f(m - most), add = __builtin_amdgcn_exp2f(m_e - most);
+        m = most;
+        l = l * old + l_e * add;
+#pragma unroll
+        for (int b = 0; b < CB; ++b) acc[b] = acc[b] * old + a_e[b] * add;
+    }
     if (row >= w.rows) return;
     const float inv = row_inverse(l);
     const f4 *vs = (const f4 *)(p.w_scale + ((int64_t)(p.head0 + h) * 2 + 1) * kD) + grp;
@@ -564,7 +634,7 @@ namespace {
 constexpr int64_t kSumsBytes = 4096;
 static_assert((kThreads + 1) * 8 <= kSumsBytes, "the sums fit");
 constexpr int64_t kMostBytes = (int64_t)4 << 30;  // keys and values of a pass, where one head's are not more
-int64_t part_bytes(const LatentPrefillParams &p) { return (int64_t)p.groups * 2 * 32 * p.waves * (kD + 2) * 4; }
+int64_t part_bytes(const LatentPrefillParams &p) { return (int64_t)p.groups * 2 * p.rows * (kD + 2) * 4; }
 }  // namespace
 
 int64_t latent_prefill_plan(LatentPrefillParams *p) {
@@ -572,7 +642,7 @@ int64_t latent_prefill_plan(LatentPrefillParams *p) {
     p->cap = p->seq_cap * p->seqs.n_seqs;
     const int64_t head = std::max<int64_t>(1, p->cap * 2 * kD * 2);
     p->heads = (int)std::max<int64_t>(1, std::min<int64_t>(p->H, kMostBytes / head));
-    p->waves = p->seqs.max_q <= 128 ? 4 : 8;
+    p->rows = p->seqs.max_q <= 128 ? 128 : 256;
     p->groups = kGroups;
     return kSumsBytes + part_bytes(*p) + p->heads * head;
 }
@@ -586,10 +656,10 @@ hipError_t latent_prefill_launch(const LatentPrefillParams &p0, hipStream_t st) 
     p.values = p.keys + p.heads * p.cap * kD * 2;
     const int most = p.heads;
     if (p.pool.n_pages == 0) p.seqs.width = 0;
-    auto of = [&](auto dc, auto nw) {
-        constexpr int DC = decltype(dc)::value, NW = decltype(nw)::value;
+    auto of = [&](auto dc, auto rb) {
+        constexpr int DC = decltype(dc)::value, RB = decltype(rb)::value, R = 128 * RB;
         auto expand = latent_expand_kernel<DC>;
-        auto attend = latent_prefill_kernel<DC, NW>;
+        auto attend = latent_prefill_kernel<DC, RB>;
         const int lds_e = kExpandTok * 2 * DC, lds_a = 3 * kStep * (4 * kD + 2 * kLatentRope);
         (void)hipFuncSetAttribute((const void *)expand, hipFuncAttributeMaxDynamicSharedMemorySize, lds_e);
         (void)hipFuncSetAttribute((const void *)attend, hipFuncAttributeMaxDynamicSharedMemorySize, lds_a);
@@ -598,17 +668,17 @@ hipError_t latent_prefill_launch(const LatentPrefillParams &p0, hipStream_t st) 
             expand<<<dim3(p.groups), dim3(kThreads), lds_e, st>>>(p);
             hipError_t e = hipGetLastError();
             if (e != hipSuccess) return e;
-            attend<<<dim3(p.groups), dim3(64 * NW), lds_a, st>>>(p);
+            attend<<<dim3(p.groups), dim3(kAttendThreads), lds_a, st>>>(p);
             e = hipGetLastError();
             if (e != hipSuccess) return e;
-            const int64_t blocks = ((int64_t)(p.seqs.max_q + 32 * NW - 1) / (32 * NW) * (2 * NW) + 3) / 4;
-            latent_prefill_merge_kernel<32 * NW><<<dim3((unsigned)blocks, p.heads, p.seqs.n_seqs), dim3(kThreads), 0, st>>>(p);
+            const int64_t blocks = ((int64_t)p.seqs.max_q + R - 1) / R * (R / 64);
+            latent_prefill_merge_kernel<R><<<dim3((unsigned)blocks, p.heads, p.seqs.n_seqs), dim3(kThreads), 0, st>>>(p);
             e = hipGetLastError();
             if (e != hipSuccess) return e;
         }
         return hipSuccess;
     };
-    auto by_rows = [&](auto dc) { return p.waves == 4 ? of(dc, std::integral_constant<int, 4>{}) : of(dc, std::integral_constant<int, 8>{}); };
+    auto by_rows = [&](auto dc) { return p.rows == 128 ? of(dc, std::integral_constant<int, 1>{}) : of(dc, std::integral_constant<int, 2>{}); };
     return p.Dc == 512 ? by_rows(std::integral_constant<int, 512>{}) : by_rows(std::integral_constant<int, 256>{});
 }
 
