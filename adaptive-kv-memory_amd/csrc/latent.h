@@ -73,6 +73,7 @@ struct LatentImportanceParams {
     const float *lse, *scores;
     float *out;
     int64_t n_scores, score_stride, out_stride;
+    FastDiv by_heads;
 };
 
 struct LatentCompactParams {

@@ -611,14 +611,17 @@ __global__ __launch_bounds__(kThreads) void latent_merge_kernel(const LatentAttn
 }
 
 // The importance: sum over rows and heads of 2^(s - lse), for 32 tokens a wave, whose rows stay in
-// registers while 16 query rows at a time go through LDS as the other operand.
-template <int DC>
-__global__ __launch_bounds__(kThreads, 1) void latent_importance_kernel(const LatentImportanceParams p) {
+// registers while 16 G query rows at a time go through LDS as the other operand.  G waves of a SIMD have the
+// same tokens, and each of them every G-th 16 of the rows.
+template <int DC, int G>
+__global__ __launch_bounds__(kThreads * G, G) void latent_importance_kernel(const LatentImportanceParams p) {
     constexpr int NI = Row<DC>::NI, W = DC + kLatentRope, CH = W / 8, ROWB = 2 * W;
-    __shared__ __align__(16) u4 op[2][NI * 64];
-    __shared__ float kxs[2][16], ls[2][16];
-    __shared__ int sees[2][16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
+    extern __shared__ __align__(16) unsigned char smem[];
+    u4 (*op)[G][NI * 64] = (u4 (*)[G][NI * 64])smem;
+    __shared__ float kxs[2][16 * G], ls[2][16 * G], joined[G][kWaves][32];
+    __shared__ int sees[2][16 * G];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6 & 3, group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    const int col = lane & 15, grp = lane >> 4;
     const int s = blockIdx.y;
     const SeqRows r = wave_uniform(seq_rows(p.seqs, s, p.pool.log_page));
     const int n = min(r.n, p.seqs.max_q), win = p.q_window > 0 ? min(p.q_window, n) : n;
@@ -626,24 +629,16 @@ __global__ __launch_bounds__(kThreads, 1) void latent_importance_kernel(const La
     const int64_t lim = min((int64_t)r.kv, p.n_scores);
     const bool live = n > 0 && block0 < lim;
     const int64_t tok0 = block0 + wave * 32;
-    h8 K[2][NI];
-    bool have[2] = {false, false};
-    if (live) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int64_t t = tok0 + 16 * i;
-            uint32_t page = ~0u;
-            if (t < lim) page = (uint32_t)p.seqs.table[s * p.seqs.table_stride + (t >> p.pool.log_page)];
-            have[i] = page < p.pool.n_pages;
-            const unsigned char *at = p.pool.base + (int64_t)(have[i] ? page : 0) * p.pool.page_bytes +
-                                      (have[i] ? (t & ((1 << p.pool.log_page) - 1)) : 0) * ROWB + col * ROWB + 16 * grp;
-#pragma unroll
-            for (int c = 0; c < NI; ++c) K[i][c] = p.pool.n_pages ? *(const h8 *)(at + 64 * c) : (h8){};
-        }
-    }
+    // the token whose score this lane writes
+    const int64_t mine = tok0 + 4 * (col & 4) + 4 * grp + (col & 3);
+    const bool writes = group == 0 && col < 8 && mine < p.n_scores;
+    float *out = p.out + s * p.out_stride;
+    const float *old = p.scores + s * p.score_stride;
     float sum[2][4] = {};
+    bool have[2] = {false, false};
+    float before = 0.0f;
     if (live) {
-        const int rows = win * p.H, blocks = (rows + 15) / 16;
+        const int rows = win * p.H, blocks = (rows + 16 * G - 1) / (16 * G);
         // 16 lanes stage a row
         const int sr = threadIdx.x >> 4, sl = threadIdx.x & 15;
         constexpr int MINE = (CH + 15) / 16;
@@ -651,8 +646,8 @@ __global__ __launch_bounds__(kThreads, 1) void latent_importance_kernel(const La
         float lse_in = 0.0f;
         int see_in = 0;
         auto fetch = [&](int b) {
-            const int row = 16 * b + sr, i = min(row, rows - 1);
-            const int qt = n - win + i / p.H, h = i % p.H;
+            const int row = 16 * G * b + sr, i = min(row, rows - 1);
+            const int qt = n - win + (int)fast_div(i, p.by_heads), h = i - (int)fast_div(i, p.by_heads) * p.H;
             const int64_t t = r.begin + qt;
             const unsigned char *q = p.q + t * p.q_t + h * p.q_h, *qr = p.qr + t * p.qr_t + h * p.qr_h;
 #pragma unroll
@@ -664,6 +659,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_importance_kernel(const La
             lse_in = p.lse[t * p.H + h];
             see_in = row < rows ? r.sees(p.causal, qt) : 0;
         };
+        // chunk c of row sr lies at place sr ^ 4 (c % 4) of the sixteen of (c, any row): writes and reads fall on all banks
         auto stage = [&](int buf) {
             int ex = 14;
             float x = 1.0f;
@@ -682,7 +678,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_importance_kernel(const La
                 if (p.q_bf16)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[e] = scaled_pair(w[j][e], x);
-                if (c < CH) op[buf][(c >> 2) * 64 + (c & 3) * 16 + sr] = v;
+                if (c < CH) op[buf][sr >> 4][c * 16 + ((sr & 15) ^ 4 * (c & 3))] = v;
             }
             if (sl == 0) {
                 kxs[buf][sr] = row_factor(p.scale_log2, ex);
@@ -691,19 +687,41 @@ __global__ __launch_bounds__(kThreads, 1) void latent_importance_kernel(const La
             }
         };
         fetch(0);
+        h8 K[2][NI];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int64_t t = tok0 + 16 * i;
+            uint32_t page = ~0u;
+            if (t < lim) page = (uint32_t)p.seqs.table[s * p.seqs.table_stride + (t >> p.pool.log_page)];
+            have[i] = page < p.pool.n_pages;
+            const unsigned char *at = p.pool.base + (int64_t)(have[i] ? page : 0) * p.pool.page_bytes +
+                                      (have[i] ? (t & ((1 << p.pool.log_page) - 1)) : 0) * ROWB + col * ROWB + 16 * grp;
+#pragma unroll
+            for (int c = 0; c < NI; ++c) K[i][c] = p.pool.n_pages ? *(const h8 *)(at + 64 * c) : (h8){};
+        }
+        if (writes) before = old[mine];
+        const int at = grp * 16 + (col ^ 4 * grp), line = 16 * group + col;
+#pragma unroll 1
         for (int b = 0; b < blocks; ++b) {
             stage(b & 1);
             __syncthreads();
             if (b + 1 < blocks) fetch(b + 1);
+            constexpr int AHEAD = 6;  // reads that are under way
+            const u4 *from = op[b & 1][group] + at;
             f4 S[2] = {};
+            u4 q[AHEAD];
+#pragma unroll
+            for (int c = 0; c < AHEAD; ++c) q[c] = from[c * 64];
+            const float kx = kxs[b & 1][line], lse = ls[b & 1][line];
+            const int see = sees[b & 1][line];
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int c = 0; c < NI; ++c) {
-                const h8 q = __builtin_bit_cast(h8, op[b & 1][c * 64 + lane]);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) S[i] = mfma_k32(K[i][c], q, S[i]);
+                for (int i = 0; i < 2; ++i) S[i] = mfma_k32(K[i][c], __builtin_bit_cast(h8, q[c % AHEAD]), S[i]);
+                if (c + AHEAD < NI) q[c % AHEAD] = from[(c + AHEAD) * 64];
+                __builtin_amdgcn_sched_barrier(0);
             }
-            const float kx = kxs[b & 1][col], lse = ls[b & 1][col];
-            const int see = sees[b & 1][col];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -712,22 +730,27 @@ __global__ __launch_bounds__(kThreads, 1) void latent_importance_kernel(const La
                     sum[i][e] += tok0 + 16 * i + 4 * grp + e < see ? v : 0.0f;
                 }
         }
-    }
-    float *out = p.out + s * p.out_stride;
-    const float *old = p.scores + s * p.score_stride;
+    } else if (writes) before = old[mine];
+    float v = 0.0f;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            float v = sum[i][e];
 #pragma unroll
-            for (int d = 1; d < 16; d <<= 1) v += __shfl_xor(v, d);
-            const int64_t j = tok0 + 16 * i + 4 * grp + e;
-            if (col == 0 && j < p.n_scores) {
-                if (n > 0 && j < lim) out[j] = __builtin_fmaf(old[j], p.decay, have[i] ? v / (float)p.H : 0.0f);
-                else if (out + j != old + j) out[j] = old[j];
-            }
+            for (int d = 1; d < 16; d <<= 1) sum[i][e] += __shfl_xor(sum[i][e], d);
+            v = col == 4 * i + e ? sum[i][e] : v;
         }
+    if (G > 1) {
+        if (col < 8) joined[group][wave][8 * grp + col] = v;
+        __syncthreads();
+        v = 0.0f;
+#pragma unroll
+        for (int g = 0; g < G; ++g) v += joined[g][wave][8 * grp + (col & 7)];
+    }
+    if (writes) {
+        if (n > 0 && mine < lim) out[mine] = __builtin_fmaf(before, p.decay, (col < 4 ? have[0] : have[1]) ? v / (float)p.H : 0.0f);
+        else if (out + mine != old + mine) out[mine] = before;
+    }
 }
 
 namespace {
@@ -775,8 +798,15 @@ hipError_t latent_importance_launch(const LatentImportanceParams &p0, hipStream_
     LatentImportanceParams p = p0;
     if (p.pool.n_pages == 0) p.seqs.width = 0;
     const dim3 grid((unsigned)((p.n_scores + kWaves * 32 - 1) / (kWaves * 32)), p.seqs.n_seqs);
-    if (p.Dc == 512) latent_importance_kernel<512><<<grid, dim3(kThreads), 0, st>>>(p);
-    else latent_importance_kernel<256><<<grid, dim3(kThreads), 0, st>>>(p);
+    p.by_heads = make_fast_div((uint32_t)p.H);
+    const int64_t rows = (int64_t)(p.q_window > 0 ? std::min(p.q_window, p.seqs.max_q) : p.seqs.max_q) * p.H;
+    auto go = [&](auto kernel, int groups) {
+        const int lds = 2 * groups * 16 * 2 * (p.Dc + kLatentRope);
+        (void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        kernel<<<grid, dim3(kThreads * groups), lds, st>>>(p);
+    };
+    if (p.Dc == 512) rows <= 16 ? go(latent_importance_kernel<512, 1>, 1) : go(latent_importance_kernel<512, 2>, 2);
+    else rows <= 16 ? go(latent_importance_kernel<256, 1>, 1) : go(latent_importance_kernel<256, 2>, 2);
     return hipGetLastError();
 }
 
