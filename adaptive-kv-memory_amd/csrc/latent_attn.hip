@@ -19,7 +19,7 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kUnit = 64;             // tokens of a unit of work
-constexpr int kSetup = 2;             // units that an item's start counts
+constexpr int kSetup = 5;             // units that an item's start counts
 constexpr int kGroups = 256;          // one workgroup a compute unit
 
 // A row's query: lane (row, quarter grp) holds channels 32 i + 8 grp .. of latent and rope.
@@ -386,7 +386,9 @@ __global__ __launch_bounds__(512, 2) void latent_rows_kernel(const LatentAttnPar
 
 #pragma unroll 1
         for (int i = 0; i < halves; ++i) {
-            const bool fetch = SPLIT || (i & 1);
+            // in a group's half step without scores, the shorter one; the second group's is a step later, and so is what
+            // it overwrites done with
+            const bool fetch = SPLIT || ((i ^ group) & 1);
             if (fetch) load(SPLIT ? i + 2 : (i >> 1) + 2, (SPLIT ? i + 2 : (i >> 1) + 2) & (SLOTS - 1));
             const int lane = lane_again(), col = lane & 15, grp = lane >> 4;
             const bool scores = ((i ^ group) & 1) == 0;
