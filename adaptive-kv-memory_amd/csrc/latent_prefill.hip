@@ -282,7 +282,7 @@ struct StepPages {
 template <int DC, int RB>
 __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const LatentPrefillParams p) {
     constexpr int NW = kAttendThreads / 64, R = 16 * RB * NW, SLOTS = 3, VB = kStep * kD * 2, KB = VB + kStep * kLatentRope * 2;
-    constexpr int LOADS = (KB + VB) / 1024 / NW, CB = kD / 16, NI = (kD + kLatentRope) / 32, ROWB = 2 * (DC + kLatentRope);
+    constexpr int K_LOADS = KB / 1024 / NW, V_LOADS = VB / 1024 / NW, CB = kD / 16, NI = (kD + kLatentRope) / 32, ROWB = 2 * (DC + kLatentRope);
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ TileScan sc;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -366,10 +366,10 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
             StepPages pages;
             const int64_t base = ((int64_t)h * p.cap + s * p.seq_cap) * kD * 2;
             uint32_t there = 0;  // bits 4 slot ..
-            auto load = [&](int j, int k_slot, int v_slot) {  // the keys of step j and the values of the one before
-                const int k = j * kStep, end = j < j1 ? kv : 0, before = k - kStep, v_end = j <= j1 ? kv : 0;
+            auto load_keys = [&](int j, int slot) {
+                const int k = j * kStep, end = j < j1 ? kv : 0;
                 const u4 rk = wave_rsrc(p.keys + base + (int64_t)k * kD * 2, max(0, min(end - k, kStep)) * kD * 2);
-                const uint32_t to_k = __builtin_amdgcn_readfirstlane(ring + k_slot * KB);
+                const uint32_t to_k = __builtin_amdgcn_readfirstlane(ring + slot * KB);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int n = 2 * wave + i;
@@ -386,15 +386,16 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
                 const unsigned char *rows_at = p.pool.base + (int64_t)__builtin_amdgcn_readlane(pages.ids, in) * p.pool.page_bytes +
                                                (int64_t)(tok & ((1 << lp) - 1)) * ROWB;
                 dma_kib(wave_rsrc(rows_at, rows * ROWB), to_k + VB + wave * 1024, r_off ^ (wave & 1) << 6);
-                there = (there & ~(15u << 4 * k_slot)) | bits << 4 * k_slot;
-                if (j > j0) {
-                    const u4 rv = wave_rsrc(p.values + base + (int64_t)before * kD * 2, max(0, min(v_end - before, kStep)) * kD * 2);
-                    const uint32_t to_v = __builtin_amdgcn_readfirstlane(ring + SLOTS * KB + v_slot * VB);
+                there = (there & ~(15u << 4 * slot)) | bits << 4 * slot;
+            };
+            auto load_values = [&](int j, int slot) {
+                const int k = j * kStep, end = j < j1 ? kv : 0;
+                const u4 rv = wave_rsrc(p.values + base + (int64_t)k * kD * 2, max(0, min(end - k, kStep)) * kD * 2);
+                const uint32_t to_v = __builtin_amdgcn_readfirstlane(ring + SLOTS * KB + slot * VB);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int n = 2 * wave + i;
-                        dma_kib(rv, to_v + n * 1024, (v_off ^ (n & 1) << 7) + n * 1024);
-                    }
+                for (int i = 0; i < 2; ++i) {
+                    const int n = 2 * wave + i;
+                    dma_kib(rv, to_v + n * 1024, (v_off ^ (n & 1) << 7) + n * 1024);
                 }
             };
             auto after = [](int slot) { return slot + 1 == SLOTS ? 0 : slot + 1; };
@@ -437,18 +438,22 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
                 asm volatile("" ::: "memory");
             };
             pages.fill(p, s, (j0 * kStep) >> lp);
-            load(j0, 0, 0);
-            load(j0 + 1, 1, 0);
-            wait_vm<LOADS>();
+            load_keys(j0, 0);
+            load_keys(j0 + 1, 1);
+            load_values(j0, 0);
+            wait_vm<K_LOADS + V_LOADS>();
             int slot = 0;  // of step j, for keys and for values
             if (second) {
                 meet();
-                load(j0 + 2, 2, 1);
+                load_keys(j0 + 2, 2);
             }
             for (int j = j0; j < j1; ++j) {
-                wait_vm<LOADS>();
+                // done then: this step's keys, the last one's values, and in the second waves, whose next barrier is the
+                // first ones', also the next keys and this step's values
+                wait_vm<K_LOADS>();
                 meet();
                 const int next = after(slot), last = after(next);
+                load_values(j + 1, next);
                 const uint32_t ka = ring + slot * KB + k_at, ra = ring + slot * KB + r_at;
                 auto key = [&](int n) {
                     const int c = n >> 2, i = n & 3;
@@ -474,8 +479,8 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
                 const int first = j * kStep;
                 const uint32_t have = there >> 4 * slot & 15;
                 meet();
-                if (second) load(j + 3, slot, last);
-                else load(j + 2, last, next);
+                if (second) load_keys(j + 3, slot);
+                else load_keys(j + 2, last);
                 if (!(first + kStep <= see_all && have == 15)) {
                     int at0 = first + 4 * grp;
                     asm volatile("" : "+v"(at0));  // (nothing of this is computed where nothing is masked)
