@@ -4,7 +4,7 @@
 // their upper 11 bits, then those of the bin that the budget's border falls into by the next 11, then by
 // the last 10: the border's exact value and how many of the tokens at it stay (of equal ones the lowest
 // positions leave).  A second look deals the places: ballots give a token's place in its wave, a scan over
-// the waves' counts the rest, so the list ascends.  Scores stay in registers between (up to 32 a thread; longer
+// the waves' counts the rest, so the list ascends.  Their orders stay in registers between (up to 32 a thread; longer
 // sequences are read once a look).
 #include <algorithm>
 #include <type_traits>
@@ -17,7 +17,7 @@ namespace {
 
 constexpr int kEvictThreads = 1024, kEvictWaves = 16;
 
-// Bits that order like the scores: NaN above all numbers (both signs alike), zeros alike.
+// Bits that order like the scores, above 0: NaN above all numbers (both signs alike), zeros alike.
 __device__ __forceinline__ uint32_t order_of(float x) {
     if (x != x) return 0xfffffffeu;
     const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.0f);
@@ -69,20 +69,19 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(const EvictParams 
     const uint32_t n = (uint32_t)n64, k = (uint32_t)(k64 < n64 ? k64 : n64);
     const uint32_t head = (uint32_t)min((int64_t)p.first, n64), tail = n - (uint32_t)min((int64_t)p.last, n64);
     const uint32_t chunks = max(1u, (n + R * kEvictThreads - 1) / (R * kEvictThreads));
-    float x[R];
+    uint32_t order[R];  // 0: no token; protected ones lie above every score
     auto fetch = [&](uint32_t c) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const uint32_t i = (c * R + r) * kEvictThreads + t;
-            x[r] = i < n ? scores[i] : 0.0f;
+            order[r] = i < n ? __builtin_bit_cast(uint32_t, scores[i]) : 0;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const uint32_t i = (c * R + r) * kEvictThreads + t;
+            order[r] = i >= n ? 0 : i < head || i >= tail ? 0xffffffffu : order_of(__builtin_bit_cast(float, order[r]));
         }
     };
-    // the order of a thread's token r of chunk c; protected ones lie above every score
-    auto key = [&](uint32_t c, int r) {
-        const uint32_t i = (c * R + r) * kEvictThreads + t;
-        return i < head || i >= tail ? 0xffffffffu : order_of(x[r]);
-    };
-    auto there = [&](uint32_t c, int r) { return (c * R + r) * kEvictThreads + t < n; };
     fetch(0);
 
     uint32_t border = 0, ties = 0, at_border = 0;  // the border's order, how many of those at it stay, how many there are
@@ -98,8 +97,8 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(const EvictParams 
                 if (chunks > 1) fetch(c);
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    const uint32_t o = key(c, r);
-                    const bool in = there(c, r) && (pass == 0 || o >> (shift + bits) == border >> (shift + bits));
+                    const uint32_t o = order[r];
+                    const bool in = pass == 0 ? o != 0 : o >> (shift + bits) == border >> (shift + bits);
                     const uint64_t who = __builtin_amdgcn_ballot_w64(in);
                     if (!who) continue;
                     const uint32_t bin = o >> shift & ((1u << bits) - 1);
@@ -157,21 +156,22 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(const EvictParams 
         uint64_t stays = 0;
         if (k == n) {
 #pragma unroll
-            for (int r = 0; r < R; ++r) stays |= (uint64_t)there(c, r) << r;
+            for (int r = 0; r < R; ++r) stays |= (uint64_t)(order[r] != 0) << r;
         } else {
-            const auto tie = deal([&](int r) { return there(c, r) && key(c, r) == border; }, ties_before);
+            const auto tie = deal([&](int r) { return order[r] == border; }, ties_before);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const uint32_t o = key(c, r);
-                stays |= (uint64_t)(there(c, r) && (o > border || (o == border && tie.at[r] >= leave))) << r;
+                const uint32_t o = order[r];
+                stays |= (uint64_t)(o > border || (o == border && tie.at[r] >= leave)) << r;
             }
         }
         const auto place = deal([&](int r) { return (stays >> r & 1) != 0; }, kept_before);
 #pragma unroll
         for (int r = 0; r < R; ++r)
             if (stays >> r & 1) {
-                keep[place.at[r]] = (int32_t)((c * R + r) * kEvictThreads + t);
-                if (kept) kept[place.at[r]] = x[r];
+                const uint32_t i = (c * R + r) * kEvictThreads + t;
+                keep[place.at[r]] = (int32_t)i;
+                if (kept) kept[place.at[r]] = scores[i];
             }
     }
     for (int64_t i = k + t; i < p.max_keep; i += kEvictThreads) keep[i] = 0;
