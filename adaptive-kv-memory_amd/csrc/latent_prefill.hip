@@ -188,6 +188,17 @@ __global__ __launch_bounds__(kThreads, 1) void latent_expand_kernel(const Latent
                 }
                 ((u4 *)(to + (int64_t)t * 16 * kD * 2))[0] = o[0];
                 ((u4 *)(to + (int64_t)t * 16 * kD * 2))[1] = o[1];
+                if (!p.rest || wave < 2) continue;
+                u4 rest[2];
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const h2 high = as_h2(o[b >> 1][2 * (b & 1) + e]);
+                        rest[b >> 1][2 * (b & 1) + e] = as_u32((h2){(_Float16)(acc[t][b][2 * e] - (float)high[0]), (_Float16)(acc[t][b][2 * e + 1] - (float)high[1])});
+                    }
+                ((u4 *)(to - p.values + p.rest + (int64_t)t * 16 * kD * 2))[0] = rest[0];
+                ((u4 *)(to - p.values + p.rest + (int64_t)t * 16 * kD * 2))[1] = rest[1];
             }
         }
     }
@@ -279,7 +290,12 @@ struct StepPages {
 // stays in registers.  A SIMD has two waves, which take turns: while one multiplies (the values of its last step,
 // then the keys of the next) the other turns scores into p.  The second four waves do so by standing at one barrier
 // more before their first step.
-template <int DC, int RB>
+//
+// TWO, for float16 outputs: p and the values enter their product as two float16 each, without the product of both
+// rests, or their roundings would be larger than the output's own (a chunk that sees a few hundred tokens is 2.6e-4 of
+// the norm off, 3.6e-4 with one each, where the output's rounding alone is 2.1e-4).  For bfloat16 outputs one is
+// enough.  2 chunks of up to 1024 tokens, 64 heads: 2.4 ms, and 1.65 with one each.
+template <int DC, int RB, bool TWO>
 __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const LatentPrefillParams p) {
     constexpr int NW = kAttendThreads / 64, R = 16 * RB * NW, SLOTS = 3, VB = kStep * kD * 2, KB = VB + kStep * kLatentRope * 2;
     constexpr int K_LOADS = KB / 1024 / NW, V_LOADS = VB / 1024 / NW, CB = kD / 16, NI = (kD + kLatentRope) / 32, ROWB = 2 * (DC + kLatentRope);
@@ -398,40 +414,61 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
                     dma_kib(rv, to_v + n * 1024, (v_off ^ (n & 1) << 7) + n * 1024);
                 }
             };
+            auto load_rest = [&](int j, int slot) {
+                const int k = j * kStep, end = j < j1 ? kv : 0;
+                const u4 rv = wave_rsrc(p.rest + base + (int64_t)k * kD * 2, max(0, min(end - k, kStep)) * kD * 2);
+                const uint32_t to = __builtin_amdgcn_readfirstlane(ring + SLOTS * (KB + VB) + slot * VB);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int n = 2 * wave + i;
+                    dma_kib(rv, to + n * 1024, (v_off ^ (n & 1) << 7) + n * 1024);
+                }
+            };
             auto after = [](int slot) { return slot + 1 == SLOTS ? 0 : slot + 1; };
             float mx[RB], l[RB];
             f4 acc[CB][RB];
-            u4 P[2][RB];  // of 32 tokens each
+            u4 P[2][RB], P_rest[2][RB];  // of 32 tokens each
 #pragma unroll
             for (int r = 0; r < RB; ++r) {
                 mx[r] = kMinMax, l[r] = 0.0f;
 #pragma unroll
                 for (int b = 0; b < CB; ++b) acc[b][r] = (f4){0.f, 0.f, 0.f, 0.f};
-                P[0][r] = P[1][r] = (u4){0, 0, 0, 0};
+                P[0][r] = P[1][r] = P_rest[0][r] = P_rest[1][r] = (u4){0, 0, 0, 0};
             }
-            constexpr int V_AHEAD = 6, K_AHEAD = 8;  // reads that are under way
+            constexpr int V_AHEAD = TWO ? 3 : 6, K_AHEAD = 8;  // reads that are under way
             auto value = [&](uint32_t va, int n) {
                 const uint32_t a = (va ^ (n % CB) << 5) + n / CB * 32 * kD * 2;
                 const u2 lo = read_transposed(a), hi = read_transposed(a + 16 * kD * 2);
                 return __builtin_bit_cast(h8, (u4){lo[0], lo[1], hi[0], hi[1]});
             };
             // p times the values; then(m) in the steps that read no more of them
-            auto add_values = [&](uint32_t va, auto then) {
+            auto add_values = [&](uint32_t va, uint32_t ra, auto then) {
                 constexpr int READS = 2 * CB;
-                h8 V[V_AHEAD];
+                h8 V[V_AHEAD], V_rest[V_AHEAD];
+                auto read = [&](int n) {
+                    V[n % V_AHEAD] = value(va, n);
+                    if (TWO) V_rest[n % V_AHEAD] = value(ra, n);
+                };
 #pragma unroll
-                for (int n = 0; n < V_AHEAD; ++n) V[n] = value(va, n);
+                for (int n = 0; n < V_AHEAD; ++n) read(n);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int n = 0; n < READS; ++n) {
+                    if (TWO)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int r = 0; r < RB; ++r)
+                                acc[n % CB][r] = mfma_k32(i ? V_rest[n % V_AHEAD] : V[n % V_AHEAD],
+                                                          __builtin_bit_cast(h8, i ? P[n / CB][r] : P_rest[n / CB][r]), acc[n % CB][r]);
 #pragma unroll
                     for (int r = 0; r < RB; ++r) acc[n % CB][r] = mfma_k32(V[n % V_AHEAD], __builtin_bit_cast(h8, P[n / CB][r]), acc[n % CB][r]);
-                    if (n + V_AHEAD < READS) V[n % V_AHEAD] = value(va, n + V_AHEAD);
+                    if (n + V_AHEAD < READS) read(n + V_AHEAD);
                     else then(n + V_AHEAD - READS);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             };
-            const uint32_t values = ring + SLOTS * KB + v_at;
+            const uint32_t values = ring + SLOTS * KB + v_at, rests = values + SLOTS * VB;
             auto meet = [&]() {
                 wait_lgkm0();
                 __builtin_amdgcn_s_barrier();
@@ -445,6 +482,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
             int slot = 0;  // of step j, for keys and for values
             if (second) {
                 meet();
+                if (TWO) load_rest(j0, 0);
                 load_keys(j0 + 2, 2);
             }
             for (int j = j0; j < j1; ++j) {
@@ -454,6 +492,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
                 meet();
                 const int next = after(slot), last = after(next);
                 load_values(j + 1, next);
+                if (TWO && !second) load_rest(j, j - j0 & 1);
                 const uint32_t ka = ring + slot * KB + k_at, ra = ring + slot * KB + r_at;
                 auto key = [&](int n) {
                     const int c = n >> 2, i = n & 3;
@@ -465,7 +504,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
 #pragma unroll
                     for (int n = from; n < to; ++n) K[n] = key(n);
                 };
-                if (j > j0) add_values(values + last * VB, [&](int m) { read_keys(m * K_AHEAD / V_AHEAD, (m + 1) * K_AHEAD / V_AHEAD); });
+                if (j > j0) add_values(values + last * VB, rests + (j - 1 - j0 & 1) * VB, [&](int m) { read_keys(m * K_AHEAD / V_AHEAD, (m + 1) * K_AHEAD / V_AHEAD); });
                 else read_keys(0, K_AHEAD);
                 __builtin_amdgcn_sched_barrier(0);
                 f4 S[4][RB] = {};
@@ -479,8 +518,12 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
                 const int first = j * kStep;
                 const uint32_t have = there >> 4 * slot & 15;
                 meet();
-                if (second) load_keys(j + 3, slot);
-                else load_keys(j + 2, last);
+                if (second) {
+                    if (TWO) load_rest(j + 1, j + 1 - j0 & 1);
+                    load_keys(j + 3, slot);
+                } else {
+                    load_keys(j + 2, last);
+                }
                 if (!(first + kStep <= see_all && have == 15)) {
                     int at0 = first + 4 * grp;
                     asm volatile("" : "+v"(at0));  // (nothing of this is computed where nothing is masked)
@@ -521,14 +564,18 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
 #pragma unroll
                         for (int q = 0; q < 4; ++q) e[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i][r][q], kx[r], kBias - mx[r]));
                         l[r] += (e[0] + e[1]) + (e[2] + e[3]);
-                        P[i >> 1][r][2 * (i & 1)] = as_u32((h2){(_Float16)e[0], (_Float16)e[1]});
-                        P[i >> 1][r][2 * (i & 1) + 1] = as_u32((h2){(_Float16)e[2], (_Float16)e[3]});
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            const h2 high = {(_Float16)e[2 * q], (_Float16)e[2 * q + 1]};
+                            P[i >> 1][r][2 * (i & 1) + q] = as_u32(high);
+                            if (TWO) P_rest[i >> 1][r][2 * (i & 1) + q] = as_u32((h2){(_Float16)(e[2 * q] - (float)high[0]), (_Float16)(e[2 * q + 1] - (float)high[1])});
+                        }
                     }
                 slot = next;
             }
             wait_vm<0>();
             meet();
-            if (j1 > j0) add_values(values + (slot == 0 ? SLOTS - 1 : slot - 1) * VB, [](int) {});
+            if (j1 > j0) add_values(values + (slot == 0 ? SLOTS - 1 : slot - 1) * VB, rests + (j1 - 1 - j0 & 1) * VB, [](int) {});
             if (!second) meet();
             float *e = p.part + ((int64_t)blockIdx.x * 2 + starts) * (R * (kD + 2));
 #pragma unroll
@@ -645,7 +692,7 @@ int64_t part_bytes(const LatentPrefillParams &p) { return (int64_t)p.groups * 2 
 int64_t latent_prefill_plan(LatentPrefillParams *p) {
     p->seq_cap = (int64_t)p->seqs.width << p->pool.log_page;
     p->cap = p->seq_cap * p->seqs.n_seqs;
-    const int64_t head = std::max<int64_t>(1, p->cap * 2 * kD * 2);
+    const int64_t head = std::max<int64_t>(1, p->cap * (p->q_bf16 ? 2 : 3) * kD * 2);
     p->heads = (int)std::max<int64_t>(1, std::min<int64_t>(p->H, kMostBytes / head));
     // 256 query tokens a workgroup where there are tiles of them for all, else 128 (attention and merge of 5
     // prompts of up to 777, 16 heads: 48 us as 256, 39 as 128; 2 chunks of up to 1024, 64 heads: 1.08 and 1.40 ms)
@@ -661,13 +708,15 @@ hipError_t latent_prefill_launch(const LatentPrefillParams &p0, hipStream_t st) 
     p.part = (float *)at;
     p.keys = at + part_bytes(p);
     p.values = p.keys + p.heads * p.cap * kD * 2;
+    p.rest = p.q_bf16 ? nullptr : p.values + p.heads * p.cap * kD * 2;
     const int most = p.heads;
     if (p.pool.n_pages == 0) p.seqs.width = 0;
-    auto of = [&](auto dc, auto rb) {
+    auto of = [&](auto dc, auto rb, auto two) {
         constexpr int DC = decltype(dc)::value, RB = decltype(rb)::value, R = 128 * RB;
+        constexpr bool TWO = decltype(two)::value;
         auto expand = latent_expand_kernel<DC>;
-        auto attend = latent_prefill_kernel<DC, RB>;
-        const int lds_e = kExpandTok * 2 * DC, lds_a = 3 * kStep * (4 * kD + 2 * kLatentRope);
+        auto attend = latent_prefill_kernel<DC, RB, TWO>;
+        const int lds_e = kExpandTok * 2 * DC, lds_a = kStep * (3 * (4 * kD + 2 * kLatentRope) + (TWO ? 4 * kD : 0));
         (void)hipFuncSetAttribute((const void *)expand, hipFuncAttributeMaxDynamicSharedMemorySize, lds_e);
         (void)hipFuncSetAttribute((const void *)attend, hipFuncAttributeMaxDynamicSharedMemorySize, lds_a);
         for (p.head0 = 0; p.head0 < p.H; p.head0 += most) {
@@ -685,7 +734,8 @@ hipError_t latent_prefill_launch(const LatentPrefillParams &p0, hipStream_t st) 
         }
         return hipSuccess;
     };
-    auto by_rows = [&](auto dc) { return p.rows == 128 ? of(dc, std::integral_constant<int, 1>{}) : of(dc, std::integral_constant<int, 2>{}); };
+    auto by_type = [&](auto dc, auto rb) { return p.q_bf16 ? of(dc, rb, std::false_type{}) : of(dc, rb, std::true_type{}); };
+    auto by_rows = [&](auto dc) { return p.rows == 128 ? by_type(dc, std::integral_constant<int, 1>{}) : by_type(dc, std::integral_constant<int, 2>{}); };
     return p.Dc == 512 ? by_rows(std::integral_constant<int, 512>{}) : by_rows(std::integral_constant<int, 256>{});
 }
 
