@@ -192,8 +192,8 @@ def latent_prefill(q: torch.Tensor, pool: PagedLatentPool, batch: PagedBatch, we
 
     ``sm_scale`` is by default one over the root of q's channels.  Rows see what they do in ``latent_attention``.
     Keys and values are float16, by channel over 16 times the power of two above its largest weight and clamped to +-65504
-    there; they are made for as many heads at a time as 4 GiB of workspace hold, and for
-    as many tokens of a sequence as its row of the page table has slots."""
+    there (values two float16 each for float16 queries); they are made for as many heads at a time as 4 GiB of workspace
+    hold, and for as many tokens of a sequence as its row of the page table has slots."""
     _check_device(pool, q, batch.page_table, weights.data)
     if q.dtype not in _QUERY:
         raise TypeError("latent attention takes float16 or bfloat16 queries")
@@ -206,8 +206,8 @@ def latent_prefill(q: torch.Tensor, pool: PagedLatentPool, batch: PagedBatch, we
     head = (nat.ABI_VERSION, layer, H, nat.dtype_code(q.dtype), int(causal),
             nat.default_sm_scale(D) if sm_scale is None else float(sm_scale), pool._c, batch._c, weights.data.data_ptr(),
             weights.scale.data_ptr(), q.data_ptr(), qt, qh, out.data_ptr())
-    need = _workspace(batch, ("prefill", pool.latent_dim, pool.page_size, H), lib.akv_latent_prefill_workspace_bytes, _PREFILL,
-                      head)
+    need = _workspace(batch, ("prefill", q.dtype, pool.latent_dim, pool.page_size, H), lib.akv_latent_prefill_workspace_bytes,
+                      _PREFILL, head)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
     _call(pool._index, "latent_prefill", lib.akv_latent_prefill,
           _PREFILL.pack(*head, 0, 0) if ws is None else _PREFILL.pack(*head, ws.data_ptr(), need))

@@ -330,6 +330,38 @@ def test_weights_of_any_size(size):
     assert bool((d <= b).all()), float((d / b).max())
 
 
+def test_prefill_types_share_a_batch():
+    """Float16 queries take more workspace than bfloat16 ones of the same sizes."""
+    import akv
+    announce("latent prefill, bfloat16 then float16 on one batch")
+    H = 5
+    w = World(512, 64, [300, 90], [40, 90])
+    w.fill()
+    wt = akv.LatentWeights(*(_randn(H, 128, 512, seed=s, scale=512 ** -0.5).cuda() for s in (1, 2)))
+    q = _randn(w.T, H, 192, seed=3, dt="bf16")
+    first = akv.latent_prefill(q.cuda(), w.pool, w.batch, wt)
+    after = akv.latent_prefill(q.half().cuda(), w.pool, w.batch, wt)
+    fresh = akv.PagedBatch(w.batch.page_table, w.batch.kv_lens, w.batch.q_starts, w.T, w.batch.max_q)
+    assert torch.equal(after, akv.latent_prefill(q.half().cuda(), w.pool, fresh, wt))
+    assert torch.equal(first, akv.latent_prefill(q.cuda(), w.pool, w.batch, wt))
+
+
+@pytest.mark.parametrize("Dc", [256, 512])
+def test_prefill_holds_what_float16_cannot(Dc):
+    """A value beyond 65504 times its channel's scale is held there: equal weights of 1 have the scale 32."""
+    import akv
+    announce(f"latent prefill, values beyond float16: Dc={Dc}")
+    w = World(Dc, 16, [1], [1])
+    page, row = w.slots(0, torch.arange(1))
+    w.data[0, page, row] = 61440.0
+    w.pool = akv.PagedLatentPool(w.data.cuda(), Dc)
+    ones = torch.ones(1, 128, Dc).cuda()
+    sign = torch.where(torch.arange(128) % 2 == 0, 1.0, -1.0).cuda()
+    out = akv.latent_prefill(torch.zeros(1, 1, 192, dtype=torch.bfloat16).cuda(), w.pool, w.batch,
+                             akv.LatentWeights(ones, ones * sign[None, :, None]))
+    assert torch.equal(out[0, 0], (65504.0 * 32.0 * sign).bfloat16())
+
+
 def test_prefill_in_passes_of_heads(monkeypatch):
     """A table so wide that the heads take more than one pass: as one pass with a narrow one."""
     import akv
