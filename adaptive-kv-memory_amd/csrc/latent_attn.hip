@@ -3,9 +3,9 @@
 //
 // The mathematics.  The heads' key matrices are in the queries already, so a cached row (latent c,
 // rotated key r) is the key of every head and its latent the value: s = q.c + q_r.r, o = sum of p c.
-// The rows of all heads and query tokens of a sequence thus share one stream of cached rows.  A query
-// row is scaled by a power of two to a maximum in [2^13, 2^14), which leaves with the softmax scale,
-// and enters as float16 whatever its type; scores are exact but for float32 sums.  p is one float16.
+// The rows of all heads and query tokens of a sequence thus share one stream of cached rows.  A float16 query
+// row enters as it is, a bfloat16 one as float16 after scaling by a power of two to a maximum in [2^13, 2^14),
+// which leaves with the softmax scale; scores are exact but for float32 sums.  p is one float16.
 // Softmax state: running maximum and sum per row in float32.
 #include <algorithm>
 #include <type_traits>
@@ -154,7 +154,10 @@ __device__ __forceinline__ float *entry_of(const LatentAttnParams &p, int group,
 
 }  // namespace
 
-// Up to 16 rows a sequence (a token's heads).  Bound by the cache's bytes.
+// Up to 16 rows a sequence (a token's heads).  Bound by the cache's bytes: 24 sequences of up to 65536 tokens
+// and 16 heads (269 MB) take 62 us, of which the memory's rate is 49 and the rest an item's chain of
+// lengths, pages, loads and its join, which is all of the 14 us of one sequence of 517.  (In the form for more rows:
+// 87 us.)
 //
 // Each of the four waves takes 16 tokens at a time for all 16 rows, from two buffers of LDS of its own
 // that buffer loads fill; nothing is shared until the waves join at an item's end.  What is run once for an item is
@@ -312,7 +315,10 @@ __global__ __launch_bounds__(kThreads, 2) void latent_few_kernel(const LatentAtt
 // has a wave for the softmax and one for the matrix cores.  A barrier ends each such half step: when it opens,
 // what one group leaves in LDS for itself is there, and so are the rows that are needed next.  SPLIT: both groups
 // take the same 64 rows, and every other step each; they join at an item's end.  Else 128 rows.
-// Bound by what LDS delivers: 192 bytes of operands for each MFMA of the first product, 96 for the second.
+// 40 sequences of up to 9001 tokens, 128 heads (41 GFLOP): 79 us, and 16 for the merge.  Neither MFMAs (busy 28% of
+// the cycles) nor LDS (24%, no conflicts) bound it but what a half step of 32 tokens does one after
+// the other: read, multiply, softmax, write p, meet.  Splitting 128 rows of so few sequences over all compute units costs
+// 67 MB of partial states written and read.
 template <int DC>
 struct RowsForm {
     static constexpr int KS = 32, CB = DC / 64, SLOTS = 4;
@@ -549,7 +555,8 @@ __global__ __launch_bounds__(512, 2) void latent_rows_kernel(const LatentAttnPar
 }
 
 // Joins the partial states of items that several workgroups share: a workgroup takes two of the
-// 16-channel blocks of 16 rows, each of its waves every fourth state.
+// 16-channel blocks of 16 rows, each of its waves every fourth state.  Bound by the states' bytes where they are
+// many (16 us for 128 rows of 40 sequences: 67 MB), else by its loads' chain (4.4 us for one of 517 tokens).
 template <int DC, int ROWS>
 __global__ __launch_bounds__(kThreads) void latent_merge_kernel(const LatentAttnParams p) {
     constexpr int NB = DC / 16, PER = 2, SPLIT = NB / PER;
@@ -615,6 +622,9 @@ __global__ __launch_bounds__(kThreads) void latent_merge_kernel(const LatentAttn
 // The importance: sum over rows and heads of 2^(s - lse), for 32 tokens a wave, whose rows stay in
 // registers while 16 G query rows at a time go through LDS as the other operand.  G waves of a SIMD have the
 // same tokens, and each of them every G-th 16 of the rows.
+// One query token of 16 heads is bound by the cache's bytes (8 sequences of up to 31744, 93 MB: 23 us, 4 TB/s;
+// with G = 2, which has half the tokens under way, 44).  2048 rows are not: 2 sequences of up to 16384 take 119 us, of
+// which the products alone would be 50, the queries' way from L2 through the registers into LDS the rest.
 template <int DC, int G>
 __global__ __launch_bounds__(kThreads * G, G) void latent_importance_kernel(const LatentImportanceParams p) {
     constexpr int NI = Row<DC>::NI, W = DC + kLatentRope, CH = W / 8, ROWB = 2 * W;
@@ -762,6 +772,8 @@ static_assert((kThreads + 1) * 4 <= kSumsBytes, "the sums fit");
 
 int64_t latent_attn_plan(LatentAttnParams *p) {
     const int64_t rows = (int64_t)p->seqs.max_q * p->H;
+    // tiles of 16 rows, 64 or 128: 40 sequences of up to 9001 tokens take 47 us as one of 16 and 63 as one of 64
+    // with 16 heads, 64 us as one of 64 and 70 as one of 128 with 32 heads, 66 and 73 with 64
     p->log_tile = rows <= 16 ? 4 : rows <= 64 ? 6 : 7;
     const int64_t units = (((int64_t)p->seqs.width << p->pool.log_page) + kUnit - 1) / kUnit + 1 + kSetup;
     const int64_t tiles = (rows + (1 << p->log_tile) - 1) >> p->log_tile;

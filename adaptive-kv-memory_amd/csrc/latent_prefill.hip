@@ -6,8 +6,8 @@
 // token and head, which some 170 query tokens outweigh.  Two kernels: the expansion is a matrix product
 // whose left side stays in LDS for all heads, the attention streams its results.  Keys and values are
 // float16 over a power of two for each channel (which goes to the queries and the outputs, so that small weights
-// keep their bits), query rows float16 scaled by a power of two, p one float16; scores, sums and the softmax
-// state are float32.
+// keep their bits), query rows float16 scaled by a power of two, p one float16 (for float16 outputs p and values are
+// two); scores, sums and the softmax state are float32.
 #include <algorithm>
 #include <type_traits>
 
@@ -26,9 +26,6 @@ constexpr int kStep = 64;             // tokens of a step of the attention
 constexpr int kSetupTok = 2 * kStep;  // what an item's start counts
 constexpr int kGroups = 256;
 
-}  // namespace
-
-namespace {
 
 struct TileScan {
     int64_t pre[kThreads + 1], wave_sum[kThreads / 64];
@@ -78,6 +75,9 @@ __device__ __forceinline__ int seq_of_first(const TileScan &sc, int64_t x, int n
 // of one head after another; a wave makes 64 of them for all 128 tokens.  Its weights come straight from
 // memory in operand order, a stream of 16-byte loads that runs half a head ahead and on over the heads.
 // All workgroups are at the same heads at about the same time, so that a chiplet's L2 reads them once.
+// Bound by the matrix cores at the clock that the card's power leaves them, and by the weights' way from L2: 64 heads and
+// 2 sequences of up to 17408 tokens (0.5 TFLOP, 1 GB written) take 510 to 580 us; 16 heads and 1396 tokens, a head a
+// workgroup, 20 us, most of it the first 128 KB of latents and 256 KB of weights of each.
 template <int DC>
 __global__ __launch_bounds__(kThreads, 1) void latent_expand_kernel(const LatentPrefillParams p) {
     constexpr int LROW = 2 * DC, KS = DC / 32, TILES = kExpandTok / 16, RING = KS / 2;
@@ -290,6 +290,9 @@ struct StepPages {
 // stays in registers.  A SIMD has two waves, which take turns: while one multiplies (the values of its last step,
 // then the keys of the next) the other turns scores into p.  The second four waves do so by standing at one barrier
 // more before their first step.
+// 2 chunks of up to 1024 tokens after up to 16384, 64 heads: 0.95 to 1.07 ms, 0.93 PFLOP/s with what the causal tiles'
+// corners waste, at 1.7 GHz: the card's power holds the clock, and fewer cycles (17.5 to 14.3 million of all chiplets)
+// gave little time.  5 prompts of up to 777 tokens, 16 heads: 28 us, most of it an item's start and end.
 //
 // TWO, for float16 outputs: p and the values enter their product as two float16 each, without the product of both
 // rests, or their roundings would be larger than the output's own (a chunk that sees a few hundred tokens is 2.6e-4 of
@@ -616,7 +619,8 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
     }
 }
 
-// Joins the partial states of items that several workgroups share: a wave takes 16 rows of one.
+// Joins the partial states of items that several workgroups share: a wave takes 16 rows of one.  Bound by the
+// states' bytes: 10 us for 5 prompts of up to 777 tokens, 16 heads.
 template <int R>
 __global__ __launch_bounds__(kThreads) void latent_prefill_merge_kernel(const LatentPrefillParams p) {
     constexpr int CB = kD / 16;
