@@ -314,6 +314,67 @@ def test_prefill_split_over_workgroups(H, kv, q, P):
     _check_prefill(w, H, "bf16")
 
 
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("Dc,P,H,kv,q,causal", [(512, 64, 128, [700, 40, 0], [300, 40, 0], True), (256, 16, 128, [333, 1], [332, 1], False),
+                                                (256, 32, 64, [1031], [1000], True)])
+def test_prefill_of_many_tiles(Dc, P, H, kv, q, causal, dt):
+    """Enough heads and tokens that workgroups take 256 query tokens each."""
+    announce(f"latent prefill, many tiles: H={H} kv={kv} q={q} Dc={Dc} P={P} {dt}")
+    w = World(Dc, P, kv, q)
+    w.fill()
+    _check_prefill(w, H, dt, causal=causal)
+    w.same_pool()
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+def test_prefill_of_many_tiles_with_missing_pages(dt):
+    import akv
+    announce(f"latent prefill, many tiles and pages outside the pool: {dt}")
+    H = 128
+    w = World(512, 16, [500, 40], [300, 40])
+    w.fill()
+    w.batch.page_table[0, 3] = w.batch.page_table[0, 20] = w.batch.page_table[1, 0] = -1
+    stay = [torch.ones(n, dtype=torch.bool) for n in w.kv]
+    stay[0][48:64] = stay[0][320:336] = stay[1][:16] = False
+    weights = [_randn(H, 128, 512, seed=s, dt=dt, scale=512 ** -0.5) for s in (1, 2)]
+    q = _randn(w.T, H, 192, seed=9, dt=dt)
+    got = akv.latent_prefill(q.cuda(), w.pool, w.batch, akv.LatentWeights(*(a.cuda() for a in weights))).double().cpu()
+    for s, i in ((0, 0), (0, 128), (0, 299), (1, 3), (1, 39)):
+        n, at = w.kv[s] - w.q[s] + 1 + i, slice(w.mine(s).start + i, w.mine(s).start + i + 1)
+        e, b = ref.prefill(q[at].double(), w.rows(s)[:n][stay[s][:n]], weights[0].double(), weights[1].double(), _scale(),
+                           torch.finfo(DT[dt]).eps / 2)
+        assert bool(((got[at] - e).abs() <= b).all()), (s, i)
+    assert not bool(got[w.mine(1)][:16].any())  # these see no token
+
+
+def test_prefill_of_many_tiles_captured():
+    """A captured call follows lengths and tables that change, as an eager one does."""
+    import akv
+    announce("latent prefill, many tiles, captured")
+    H = 128
+    w = World(256, 32, [300, 200], [200, 60])
+    w.fill()
+    wt = akv.LatentWeights(*(_randn(H, 128, 256, seed=s, scale=256 ** -0.5).cuda() for s in (1, 2)))
+    q = _randn(w.T, H, 192, seed=3, dt="bf16").cuda()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        akv.latent_prefill(q, w.pool, w.batch, wt)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = akv.latent_prefill(q, w.pool, w.batch, wt)
+    table = w.batch.page_table.clone()
+    for lens, hole in (([300, 200], None), ([260, 61], None), ([300, 200], (0, 2)), ([200, 0], None)):
+        w.batch.kv_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        w.batch.page_table.copy_(table)
+        if hole:
+            w.batch.page_table[hole] = -1
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, akv.latent_prefill(q, w.pool, w.batch, wt)), lens
+
+
 @pytest.mark.parametrize("size", [1e-6, 1e-3, 1e4])
 def test_weights_of_any_size(size):
     announce(f"latent prefill, weights times {size}")
