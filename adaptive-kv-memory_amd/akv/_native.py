@@ -236,6 +236,7 @@ class LatentImportanceArgs(ctypes.Structure):
         ("q", _vp), ("q_rope", _vp), ("q_t", _i64), ("q_h", _i64), ("q_rope_t", _i64), ("q_rope_h", _i64),
         ("lse", _vp), ("scores", _vp), ("out", _vp),
         ("n_scores", _i64), ("score_stride", _i64), ("out_stride", _i64),
+        ("workspace", _vp), ("workspace_bytes", _i64),
     ]
 
 
@@ -270,8 +271,8 @@ EXPORTS = (
     "akv_paged_append", "akv_paged_read", "akv_paged_attn_workspace_bytes", "akv_paged_attn",
     "akv_paged_importance", "akv_paged_copy", "akv_paged_compact",
     "akv_latent_append", "akv_latent_read", "akv_latent_attn_workspace_bytes", "akv_latent_attn",
-    "akv_latent_prefill_workspace_bytes", "akv_latent_prefill", "akv_latent_importance", "akv_latent_copy",
-    "akv_latent_compact", "akv_evict_select",
+    "akv_latent_prefill_workspace_bytes", "akv_latent_prefill", "akv_latent_importance_workspace_bytes", "akv_latent_importance",
+    "akv_latent_copy", "akv_latent_compact", "akv_evict_select",
 )
 STRUCTS = (WarmDesc, DecodeArgs, QuantArgs, DequantArgs, ImportanceArgs, PrefillArgs, RowsJob, KiviSide,
            PagedPool, PagedBatch, PagedRowsArgs, PagedAttnArgs, PagedImportanceArgs, PagedCompactArgs,
@@ -348,7 +349,8 @@ def load() -> ctypes.CDLL:
                  "akv_latent_compact", "akv_evict_select"):
         getattr(lib, name).restype = ctypes.c_int
         getattr(lib, name).argtypes = [_vp, _vp]
-    for name in ("akv_paged_attn_workspace_bytes", "akv_latent_attn_workspace_bytes", "akv_latent_prefill_workspace_bytes"):
+    for name in ("akv_paged_attn_workspace_bytes", "akv_latent_attn_workspace_bytes", "akv_latent_prefill_workspace_bytes",
+                 "akv_latent_importance_workspace_bytes"):
         getattr(lib, name).restype = _i64
         getattr(lib, name).argtypes = [_vp]
     for name in ("akv_paged_copy", "akv_latent_copy"):

@@ -31,7 +31,7 @@ _POOL, _BATCH = ctypes.sizeof(nat.LatentPool), ctypes.sizeof(nat.PagedBatch)
 _ROWS = struct.Struct(f"@4i{_POOL}s{_BATCH}s4q")
 _ATTN = struct.Struct(f"@5if{_POOL}s{_BATCH}s10q")
 _PREFILL = struct.Struct(f"@5if{_POOL}s{_BATCH}s8q")
-_IMPORTANCE = struct.Struct(f"@6i2f{_POOL}s{_BATCH}s12q")
+_IMPORTANCE = struct.Struct(f"@6i2f{_POOL}s{_BATCH}s14q")
 _COMPACT = struct.Struct(f"@2i{_POOL}s4q2i4q")
 for _s, _c in ((_ROWS, nat.LatentRowsArgs), (_ATTN, nat.LatentAttnArgs), (_PREFILL, nat.LatentPrefillArgs),
                (_IMPORTANCE, nat.LatentImportanceArgs), (_COMPACT, nat.LatentCompactArgs)):
@@ -235,10 +235,14 @@ def latent_importance(q: torch.Tensor, q_rope: torch.Tensor, lse: torch.Tensor, 
             raise ValueError("a sequence's scores must be consecutive")
     if not lse.is_contiguous():
         lse = lse.contiguous()
-    args = _IMPORTANCE.pack(nat.ABI_VERSION, layer, H, nat.dtype_code(q.dtype), int(causal), int(q_window), float(sm_scale),
-                            float(decay), pool._c, batch._c, q.data_ptr(), qr.data_ptr(), qt, qh, qrt, qrh, lse.data_ptr(),
-                            scores.data_ptr(), dst.data_ptr(), scores.shape[1], scores.stride(0), dst.stride(0))
-    _call(pool._index, "latent_importance", nat.load().akv_latent_importance, args)
+    lib = nat.load()
+    head = (nat.ABI_VERSION, layer, H, nat.dtype_code(q.dtype), int(causal), int(q_window), float(sm_scale), float(decay), pool._c,
+            batch._c, q.data_ptr(), qr.data_ptr(), qt, qh, qrt, qrh, lse.data_ptr(), scores.data_ptr(), dst.data_ptr(),
+            scores.shape[1], scores.stride(0), dst.stride(0))
+    need = _workspace(batch, ("importance", D, H, int(q_window)), lib.akv_latent_importance_workspace_bytes, _IMPORTANCE, head)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+    _call(pool._index, "latent_importance", lib.akv_latent_importance,
+          _IMPORTANCE.pack(*head, 0, 0) if ws is None else _IMPORTANCE.pack(*head, ws.data_ptr(), need))
     return dst
 
 

@@ -1244,9 +1244,9 @@ static int latent_attn_params(const akv_latent_attn_args *a, akv::LatentAttnPara
     if (rc != AKV_OK) return rc;
     rc = check_latent_queries(a->H, a->q_dtype, a->sm_scale, a->batch, a->q, a->q_rope, a->q_t | a->q_h | a->q_rope_t | a->q_rope_h);
     if (rc != AKV_OK) return rc;
-    // units of 64 tokens of a tile of at least 16 rows are counted in 31 bits
+    // units of 64 tokens of a tile of at least 16 rows, and a few for an item, are counted in 31 bits
     const double cap = (double)a->batch.table_width * a->pool.page_size, rows = (double)a->batch.max_q * a->H;
-    if ((cap / 64 + 4) * (rows / 16 + 1) * a->batch.n_seqs >= 0x1p30) return fail(AKV_E_SHAPE, "too much for one call");
+    if ((cap / 64 + 8) * (rows / 16 + 1) * a->batch.n_seqs >= 0x1p30) return fail(AKV_E_SHAPE, "too much for one call");
     p->Dc = a->pool.latent_dim; p->H = a->H;
     p->q_bf16 = a->q_dtype == AKV_DT_BF16; p->causal = a->causal != 0;
     p->scale_log2 = a->sm_scale * 1.4426950408889634f;
@@ -1317,14 +1317,36 @@ int akv_latent_prefill(const akv_latent_prefill_args *a, void *stream) {
     return ok();
 }
 
-int akv_latent_importance(const akv_latent_importance_args *a, void *stream) {
+static int latent_importance_params(const akv_latent_importance_args *a, akv::LatentImportanceParams *p, int64_t *bytes) {
     if (!a) return fail(AKV_E_INVALID, "args is NULL");
-    akv::LatentImportanceParams p{};
-    int rc = latent_views(a->abi_version, a->layer, a->pool, a->batch, &p.pool, &p.seqs);
+    int rc = latent_views(a->abi_version, a->layer, a->pool, a->batch, &p->pool, &p->seqs);
     if (rc != AKV_OK) return rc;
     rc = check_latent_queries(a->H, a->q_dtype, a->sm_scale, a->batch, a->q, a->q_rope, a->q_t | a->q_h | a->q_rope_t | a->q_rope_h);
     if (rc != AKV_OK) return rc;
     if (a->q_window < 0) return fail(AKV_E_SHAPE, "q_window must be >= 0");
+    p->Dc = a->pool.latent_dim; p->H = a->H;
+    p->q_bf16 = a->q_dtype == AKV_DT_BF16; p->causal = a->causal != 0; p->q_window = a->q_window;
+    p->scale_log2 = a->sm_scale * 1.4426950408889634f; p->decay = a->decay;
+    p->q = (const unsigned char *)a->q; p->qr = (const unsigned char *)a->q_rope;
+    p->q_t = a->q_t; p->q_h = a->q_h; p->qr_t = a->q_rope_t; p->qr_h = a->q_rope_h;
+    p->lse = a->lse; p->scores = a->scores; p->out = a->out;
+    p->n_scores = a->n_scores; p->score_stride = a->score_stride; p->out_stride = a->out_stride;
+    p->blocks = (unsigned char *)a->workspace;
+    *bytes = akv::latent_importance_plan(p);
+    return AKV_OK;
+}
+
+int64_t akv_latent_importance_workspace_bytes(const akv_latent_importance_args *a) {
+    akv::LatentImportanceParams p{};
+    int64_t bytes;
+    return latent_importance_params(a, &p, &bytes) == AKV_OK ? bytes : -1;
+}
+
+int akv_latent_importance(const akv_latent_importance_args *a, void *stream) {
+    akv::LatentImportanceParams p{};
+    int64_t bytes;
+    const int rc = latent_importance_params(a, &p, &bytes);
+    if (rc != AKV_OK) return rc;
     if (a->n_scores < 0 || a->n_scores >= ((int64_t)1 << 31) ||
         (a->batch.n_seqs > 1 && (a->score_stride < a->n_scores || a->out_stride < a->n_scores)))
         return fail(AKV_E_SHAPE, "bad score rows");
@@ -1334,13 +1356,9 @@ int akv_latent_importance(const akv_latent_importance_args *a, void *stream) {
     if (rows_clash(a->scores, a->score_stride, a->out, a->out_stride, a->n_scores, a->batch.n_seqs))
         return fail(AKV_E_SHAPE, "out must be scores or not overlap it");
     if (!aligned4(a->lse)) return fail(AKV_E_ALIGN, "lse must be 4-byte aligned");
-    p.Dc = a->pool.latent_dim; p.H = a->H;
-    p.q_bf16 = a->q_dtype == AKV_DT_BF16; p.causal = a->causal != 0; p.q_window = a->q_window;
-    p.scale_log2 = a->sm_scale * 1.4426950408889634f; p.decay = a->decay;
-    p.q = (const unsigned char *)a->q; p.qr = (const unsigned char *)a->q_rope;
-    p.q_t = a->q_t; p.q_h = a->q_h; p.qr_t = a->q_rope_t; p.qr_h = a->q_rope_h;
-    p.lse = a->lse; p.scores = a->scores; p.out = a->out;
-    p.n_scores = a->n_scores; p.score_stride = a->score_stride; p.out_stride = a->out_stride;
+    if (bytes > 0 && (!a->workspace || a->workspace_bytes < bytes))
+        return fail(AKV_E_WORKSPACE, "workspace of %lld bytes needed", (long long)bytes);
+    if (!aligned16(a->workspace)) return fail(AKV_E_ALIGN, "workspace must be 16-byte aligned");
     hipError_t e = akv::latent_importance_launch(p, (hipStream_t)stream);
     if (e != hipSuccess) return hip_fail(e, "latent importance launch");
     return ok();

@@ -75,6 +75,7 @@ struct LatentImportanceParams {
     float *out;
     int64_t n_scores, score_stride, out_stride;
     FastDiv by_heads;
+    unsigned char *blocks;     // the workspace, for more than 16 rows a sequence: query rows as operands
 };
 
 struct LatentCompactParams {
@@ -107,6 +108,7 @@ int64_t latent_attn_plan(LatentAttnParams *p);
 hipError_t latent_attn_launch(const LatentAttnParams &p, hipStream_t s);
 int64_t latent_prefill_plan(LatentPrefillParams *p);
 hipError_t latent_prefill_launch(const LatentPrefillParams &p, hipStream_t s);
+int64_t latent_importance_plan(LatentImportanceParams *p);
 hipError_t latent_importance_launch(const LatentImportanceParams &p, hipStream_t s);
 hipError_t evict_launch(const EvictParams &p, hipStream_t s);
 

@@ -620,19 +620,184 @@ __global__ __launch_bounds__(kThreads) void latent_merge_kernel(const LatentAttn
 }
 
 // The importance: sum over rows and heads of 2^(s - lse), for 32 tokens a wave, whose rows stay in
-// registers while 16 G query rows at a time go through LDS as the other operand.  G waves of a SIMD have the
-// same tokens, and each of them every G-th 16 of the rows.
-// One query token of 16 heads is bound by the cache's bytes (8 sequences of up to 31744, 93 MB: 23 us, 4 TB/s;
-// with G = 2, which has half the tokens under way, 44).  2048 rows are not: 2 sequences of up to 16384 take 119 us, of
-// which the products alone would be 50, the queries' way from L2 through the registers into LDS the rest.
-template <int DC, int G>
-__global__ __launch_bounds__(kThreads * G, G) void latent_importance_kernel(const LatentImportanceParams p) {
-    constexpr int NI = Row<DC>::NI, W = DC + kLatentRope, CH = W / 8, ROWB = 2 * W;
-    extern __shared__ __align__(16) unsigned char smem[];
-    u4 (*op)[G][NI * 64] = (u4 (*)[G][NI * 64])smem;
-    __shared__ float kxs[2][16 * G], ls[2][16 * G], joined[G][kWaves][32];
-    __shared__ int sees[2][16 * G];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6 & 3, group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+// registers while query rows go through LDS as the other operand.
+//
+// Up to 16 rows a sequence: bound by the cache's bytes (8 sequences of up to 31744 tokens, 16 heads, 93 MB: 23 us).
+template <int DC>
+__global__ __launch_bounds__(kThreads, 1) void latent_importance_few_kernel(const LatentImportanceParams p) {
+    constexpr int NI = Row<DC>::NI, W = DC + kLatentRope, CH = W / 8, ROWB = 2 * W, MINE = (CH + 15) / 16;
+    __shared__ __align__(16) u4 op[NI * 64];
+    __shared__ float kxs[16], ls[16];
+    __shared__ int sees[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
+    const int s = blockIdx.y;
+    const SeqRows r = wave_uniform(seq_rows(p.seqs, s, p.pool.log_page));
+    const int n = min(r.n, p.seqs.max_q), win = p.q_window > 0 ? min(p.q_window, n) : n;
+    const int64_t block0 = (int64_t)blockIdx.x * (kWaves * 32);
+    const int64_t lim = min((int64_t)r.kv, p.n_scores);
+    const bool live = n > 0 && block0 < lim;
+    const int64_t tok0 = block0 + wave * 32;
+    // the token whose score this lane writes
+    const int64_t mine = tok0 + 4 * (col & 4) + 4 * grp + (col & 3);
+    const bool writes = col < 8 && mine < p.n_scores;
+    float *out = p.out + s * p.out_stride;
+    const float *old = p.scores + s * p.score_stride;
+    float sum[2][4] = {};
+    bool have[2] = {false, false};
+    float before = 0.0f;
+    if (live) {
+        const int rows = win * p.H;
+        // 16 lanes stage a row
+        const int sr = threadIdx.x >> 4, sl = threadIdx.x & 15;
+        u4 w[MINE];
+        float lse_in = 0.0f;
+        int see_in = 0;
+        {
+            const int i = min(sr, rows - 1), qt = (int)fast_div(i, p.by_heads), h = i - qt * p.H;
+            const int64_t t = r.begin + n - win + qt;
+            const unsigned char *q = p.q + t * p.q_t + h * p.q_h, *qr = p.qr + t * p.qr_t + h * p.qr_h;
+#pragma unroll
+            for (int j = 0; j < MINE; ++j) {
+                const int c = sl + 16 * j;
+                w[j] = (u4){0, 0, 0, 0};
+                if (c < CH) w[j] = c < DC / 8 ? ((const u4 *)q)[c] : ((const u4 *)qr)[c - DC / 8];
+            }
+            lse_in = p.lse[t * p.H + h];
+            see_in = sr < rows ? r.sees(p.causal, n - win + qt) : 0;
+        }
+        h8 K[2][NI];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int64_t t = tok0 + 16 * i;
+            uint32_t page = ~0u;
+            if (t < lim) page = (uint32_t)p.seqs.table[s * p.seqs.table_stride + (t >> p.pool.log_page)];
+            have[i] = page < p.pool.n_pages;
+            const unsigned char *at = p.pool.base + (int64_t)(have[i] ? page : 0) * p.pool.page_bytes +
+                                      (have[i] ? (t & ((1 << p.pool.log_page) - 1)) : 0) * ROWB + col * ROWB + 16 * grp;
+#pragma unroll
+            for (int c = 0; c < NI; ++c) K[i][c] = p.pool.n_pages ? *(const h8 *)(at + 64 * c) : (h8){};
+        }
+        if (writes) before = old[mine];
+        int ex = 14;
+        if (p.q_bf16) {
+            const us2 pair = largest(w);
+            uint32_t top = max(pair[0], pair[1]);
+#pragma unroll
+            for (int d = 1; d < 16; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+            ex = row_exponent(top);
+            const float x = __builtin_ldexpf(1.0f, 14 - ex);
+#pragma unroll
+            for (int j = 0; j < MINE; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[j][e] = scaled_pair(w[j][e], x);
+        }
+        // chunk c of row sr lies at place sr ^ 4 (c % 4) of the sixteen of the chunk: writes and reads fall on all banks
+#pragma unroll
+        for (int j = 0; j < MINE; ++j) {
+            const int c = sl + 16 * j;
+            if (c < CH) op[c * 16 + (sr ^ 4 * (c & 3))] = w[j];
+        }
+        if (sl == 0) {
+            kxs[sr] = row_factor(p.scale_log2, ex);
+            ls[sr] = lse_in * 1.4426950408889634f;
+            sees[sr] = see_in;
+        }
+        __syncthreads();
+        f4 S[2] = {};
+#pragma unroll
+        for (int c = 0; c < NI; ++c) {
+            const h8 q = __builtin_bit_cast(h8, op[c * 64 + grp * 16 + (col ^ 4 * grp)]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) S[i] = mfma_k32(K[i][c], q, S[i]);
+        }
+        const float kx = kxs[col], lse = ls[col];
+        const int see = sees[col];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i][e], kx, -lse));
+                sum[i][e] = tok0 + 16 * i + 4 * grp + e < see ? v : 0.0f;
+            }
+    } else if (writes) before = old[mine];
+    float v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+#pragma unroll
+            for (int d = 1; d < 16; d <<= 1) sum[i][e] += __shfl_xor(sum[i][e], d);
+            v = col == 4 * i + e ? sum[i][e] : v;
+        }
+    if (writes) {
+        if (n > 0 && mine < lim) out[mine] = __builtin_fmaf(before, p.decay, (col < 4 ? have[0] : have[1]) ? v / (float)p.H : 0.0f);
+        else if (out + mine != old + mine) out[mine] = before;
+    }
+}
+
+// For more rows.  First every query row is made an operand once: blocks of 16 rows as the lanes read them, then
+// the rows' factors, log-sums and how many tokens they see.  They come in pairs, what lacks sees none.
+template <int DC>
+struct QueryBlock {
+    static constexpr int NI = Row<DC>::NI, BYTES = (NI + 1) * 1024;
+};
+__device__ __forceinline__ int64_t first_block(const LatentImportanceParams &p, const SeqRows &r, int s) {
+    return (p.q_window > 0 ? (int64_t)s * min(p.q_window, p.seqs.max_q) : (int64_t)r.begin) * p.H / 16 + 3 * s;
+}
+template <int DC>
+__global__ __launch_bounds__(kThreads) void latent_importance_queries_kernel(const LatentImportanceParams p) {
+    using B = QueryBlock<DC>;
+    constexpr int CH = (DC + kLatentRope) / 8, MINE = (CH + 15) / 16;
+    const int s = blockIdx.y, b = blockIdx.x, sr = threadIdx.x >> 4, sl = threadIdx.x & 15;
+    const SeqRows r = wave_uniform(seq_rows(p.seqs, s, p.pool.log_page));
+    const int n = min(r.n, p.seqs.max_q), win = p.q_window > 0 ? min(p.q_window, n) : n, rows = win * p.H;
+    if (16 * (b & ~1) >= rows) return;
+    const int row = 16 * b + sr, i = min(row, rows - 1), qt = (int)fast_div(i, p.by_heads), h = i - qt * p.H;
+    const int64_t t = r.begin + n - win + qt;
+    const unsigned char *q = p.q + t * p.q_t + h * p.q_h, *qr = p.qr + t * p.qr_t + h * p.qr_h;
+    u4 w[MINE];
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
+        const int c = sl + 16 * j;
+        w[j] = (u4){0, 0, 0, 0};
+        if (c < CH) w[j] = c < DC / 8 ? ((const u4 *)q)[c] : ((const u4 *)qr)[c - DC / 8];
+    }
+    int ex = 14;
+    if (p.q_bf16) {
+        const us2 pair = largest(w);
+        uint32_t top = max(pair[0], pair[1]);
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+        ex = row_exponent(top);
+        const float x = __builtin_ldexpf(1.0f, 14 - ex);
+#pragma unroll
+        for (int j = 0; j < MINE; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[j][e] = scaled_pair(w[j][e], x);
+    }
+    unsigned char *to = p.blocks + (first_block(p, r, s) + b) * B::BYTES;
+#pragma unroll
+    for (int j = 0; j < MINE; ++j)
+        if (const int c = sl + 16 * j; c < CH) ((u4 *)to)[c * 16 + sr] = w[j];
+    if (sl == 0) {
+        float *of = (float *)(to + B::NI * 1024);
+        of[sr] = row_factor(p.scale_log2, ex);
+        of[16 + sr] = p.lse[t * p.H + h] * 1.4426950408889634f;
+        ((int *)of)[32 + sr] = row < rows ? r.sees(p.causal, n - win + qt) : 0;
+    }
+}
+
+// Then a workgroup takes 128 tokens, two waves of a SIMD the same 32 and every other block; buffer loads
+// bring pairs of blocks three steps ahead.  2 sequences of up to 16384 tokens, 32 query tokens of 64 heads: 7 and 77 us,
+// of which the products alone, with nothing to load, are 50 (every workgroup making its own operands: 120).
+template <int DC>
+__global__ __launch_bounds__(2 * kThreads, 2) void latent_importance_rows_kernel(const LatentImportanceParams p) {
+    using B = QueryBlock<DC>;
+    constexpr int NI = B::NI, ROWB = 2 * (DC + kLatentRope), SLOTS = 4, SLOT = 2 * B::BYTES;
+    constexpr int PIECES = SLOT / 1024, LOADS = (PIECES + 7) / 8;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    __shared__ float joined[2][kWaves][32];
+    const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all & 3, group = all >> 2;
     const int col = lane & 15, grp = lane >> 4;
     const int s = blockIdx.y;
     const SeqRows r = wave_uniform(seq_rows(p.seqs, s, p.pool.log_page));
@@ -649,56 +814,8 @@ __global__ __launch_bounds__(kThreads * G, G) void latent_importance_kernel(cons
     float sum[2][4] = {};
     bool have[2] = {false, false};
     float before = 0.0f;
+    if (writes) before = old[mine];
     if (live) {
-        const int rows = win * p.H, blocks = (rows + 16 * G - 1) / (16 * G);
-        // 16 lanes stage a row
-        const int sr = threadIdx.x >> 4, sl = threadIdx.x & 15;
-        constexpr int MINE = (CH + 15) / 16;
-        u4 w[MINE];
-        float lse_in = 0.0f;
-        int see_in = 0;
-        auto fetch = [&](int b) {
-            const int row = 16 * G * b + sr, i = min(row, rows - 1);
-            const int qt = n - win + (int)fast_div(i, p.by_heads), h = i - (int)fast_div(i, p.by_heads) * p.H;
-            const int64_t t = r.begin + qt;
-            const unsigned char *q = p.q + t * p.q_t + h * p.q_h, *qr = p.qr + t * p.qr_t + h * p.qr_h;
-#pragma unroll
-            for (int j = 0; j < MINE; ++j) {
-                const int c = sl + 16 * j;
-                w[j] = (u4){0, 0, 0, 0};
-                if (c < CH) w[j] = c < DC / 8 ? ((const u4 *)q)[c] : ((const u4 *)qr)[c - DC / 8];
-            }
-            lse_in = p.lse[t * p.H + h];
-            see_in = row < rows ? r.sees(p.causal, qt) : 0;
-        };
-        // chunk c of row sr lies at place sr ^ 4 (c % 4) of the sixteen of (c, any row): writes and reads fall on all banks
-        auto stage = [&](int buf) {
-            int ex = 14;
-            float x = 1.0f;
-            if (p.q_bf16) {
-                const us2 pair = largest(w);
-                uint32_t top = max(pair[0], pair[1]);
-#pragma unroll
-                for (int d = 1; d < 16; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-                ex = row_exponent(top);
-                x = __builtin_ldexpf(1.0f, 14 - ex);
-            }
-#pragma unroll
-            for (int j = 0; j < MINE; ++j) {
-                const int c = sl + 16 * j;
-                u4 v = w[j];
-                if (p.q_bf16)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = scaled_pair(w[j][e], x);
-                if (c < CH) op[buf][sr >> 4][c * 16 + ((sr & 15) ^ 4 * (c & 3))] = v;
-            }
-            if (sl == 0) {
-                kxs[buf][sr] = row_factor(p.scale_log2, ex);
-                ls[buf][sr] = lse_in * 1.4426950408889634f;
-                sees[buf][sr] = see_in;
-            }
-        };
-        fetch(0);
         h8 K[2][NI];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -711,38 +828,59 @@ __global__ __launch_bounds__(kThreads * G, G) void latent_importance_kernel(cons
 #pragma unroll
             for (int c = 0; c < NI; ++c) K[i][c] = p.pool.n_pages ? *(const h8 *)(at + 64 * c) : (h8){};
         }
-        if (writes) before = old[mine];
-        const int at = grp * 16 + (col ^ 4 * grp), line = 16 * group + col;
-#pragma unroll 1
-        for (int b = 0; b < blocks; ++b) {
-            stage(b & 1);
-            __syncthreads();
-            if (b + 1 < blocks) fetch(b + 1);
-            constexpr int AHEAD = 6;  // reads that are under way
-            const u4 *from = op[b & 1][group] + at;
-            f4 S[2] = {};
-            u4 q[AHEAD];
+        const int steps = (win * p.H + 31) / 32;
+        const unsigned char *from = p.blocks + first_block(p, r, s) * B::BYTES;
+        const uint32_t ring = lds_addr(smem);
+        auto load = [&](int b) {
+            const u4 rsrc = wave_rsrc(from + (int64_t)b * SLOT, b < steps ? SLOT : 0);
 #pragma unroll
-            for (int c = 0; c < AHEAD; ++c) q[c] = from[c * 64];
-            const float kx = kxs[b & 1][line], lse = ls[b & 1][line];
-            const int see = sees[b & 1][line];
+            for (int i = 0; i < LOADS; ++i) {
+                // (the last one again where a wave has one less, so that all count alike)
+                const int k = all + 8 * i < PIECES ? all + 8 * i : all + 8 * i - 8;
+                dma_kib(rsrc, __builtin_amdgcn_readfirstlane(ring + (b & (SLOTS - 1)) * SLOT + k * 1024), lane * 16 + k * 1024);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int c = 0; c < NI; ++c) asm volatile("" : "+v"(K[i][c]));  // waited for here, not in the loop
+#pragma unroll
+        for (int b = 0; b < SLOTS - 1; ++b) load(b);
+#pragma unroll 1
+        for (int b = 0; b < steps; ++b) {
+            wait_vm<(SLOTS - 2) * LOADS>();
+            wait_lgkm0();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            load(b + SLOTS - 1);
+            constexpr int AHEAD = 6;  // reads that are under way
+            const uint32_t at = ring + (b & (SLOTS - 1)) * SLOT + group * B::BYTES, of = at + NI * 1024 + col * 4;
+            auto query = [&](int c) { return __builtin_bit_cast(h8, *lds_ptr<u4>(at + lane * 16 + c * 1024)); };
+            f4 S[2] = {};
+            h8 Q[AHEAD];
+#pragma unroll
+            for (int c = 0; c < AHEAD; ++c) Q[c] = query(c);
+            const float kx = *lds_ptr<float>(of), lse = *lds_ptr<float>(of + 64);
+            const int see = *lds_ptr<int>(of + 128);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int c = 0; c < NI; ++c) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) S[i] = mfma_k32(K[i][c], __builtin_bit_cast(h8, q[c % AHEAD]), S[i]);
-                if (c + AHEAD < NI) q[c % AHEAD] = from[(c + AHEAD) * 64];
+                for (int i = 0; i < 2; ++i) S[i] = mfma_k32(K[i][c], Q[c % AHEAD], S[i]);
+                if (c + AHEAD < NI) Q[c % AHEAD] = query(c + AHEAD);
                 __builtin_amdgcn_sched_barrier(0);
             }
+            const int left = (int)(see - tok0) - 4 * grp;  // of this lane's tokens, counted from its first
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i][e], kx, -lse));
-                    sum[i][e] += tok0 + 16 * i + 4 * grp + e < see ? v : 0.0f;
+                    sum[i][e] += 16 * i + e < left ? v : 0.0f;
                 }
         }
-    } else if (writes) before = old[mine];
+        wait_vm<0>();
+    }
     float v = 0.0f;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -752,17 +890,12 @@ __global__ __launch_bounds__(kThreads * G, G) void latent_importance_kernel(cons
             for (int d = 1; d < 16; d <<= 1) sum[i][e] += __shfl_xor(sum[i][e], d);
             v = col == 4 * i + e ? sum[i][e] : v;
         }
-    if (G > 1) {
-        if (col < 8) joined[group][wave][8 * grp + col] = v;
-        __syncthreads();
-        v = 0.0f;
-#pragma unroll
-        for (int g = 0; g < G; ++g) v += joined[g][wave][8 * grp + (col & 7)];
-    }
-    if (writes) {
-        if (n > 0 && mine < lim) out[mine] = __builtin_fmaf(before, p.decay, (col < 4 ? have[0] : have[1]) ? v / (float)p.H : 0.0f);
-        else if (out + mine != old + mine) out[mine] = before;
-    }
+    if (col < 8) joined[group][wave][8 * grp + col] = v;
+    __syncthreads();
+    if (!writes) return;
+    v = joined[0][wave][8 * grp + col] + joined[1][wave][8 * grp + col];
+    if (n > 0 && mine < lim) out[mine] = __builtin_fmaf(before, p.decay, (col < 4 ? have[0] : have[1]) ? v / (float)p.H : 0.0f);
+    else if (out + mine != old + mine) out[mine] = before;
 }
 
 namespace {
@@ -808,20 +941,38 @@ hipError_t latent_attn_launch(const LatentAttnParams &p0, hipStream_t st) {
     return p.Dc == 512 ? of(std::integral_constant<int, 512>{}) : of(std::integral_constant<int, 256>{});
 }
 
+static int64_t importance_rows(const LatentImportanceParams &p) {  // of a sequence, at most
+    return (int64_t)(p.q_window > 0 ? std::min(p.q_window, p.seqs.max_q) : p.seqs.max_q) * p.H;
+}
+int64_t latent_importance_plan(LatentImportanceParams *p) {
+    p->by_heads = make_fast_div((uint32_t)p->H);
+    if (importance_rows(*p) <= 16) return 0;
+    const int64_t rows = p->q_window > 0 ? p->seqs.n_seqs * importance_rows(*p) : p->seqs.n_tokens * p->H;
+    return (rows / 16 + 3 * (p->seqs.n_seqs + 1)) * (p->Dc == 512 ? QueryBlock<512>::BYTES : QueryBlock<256>::BYTES);
+}
+
 hipError_t latent_importance_launch(const LatentImportanceParams &p0, hipStream_t st) {
     LatentImportanceParams p = p0;
     if (p.pool.n_pages == 0) p.seqs.width = 0;
     const dim3 grid((unsigned)((p.n_scores + kWaves * 32 - 1) / (kWaves * 32)), p.seqs.n_seqs);
-    p.by_heads = make_fast_div((uint32_t)p.H);
-    const int64_t rows = (int64_t)(p.q_window > 0 ? std::min(p.q_window, p.seqs.max_q) : p.seqs.max_q) * p.H;
-    auto go = [&](auto kernel, int groups) {
-        const int lds = 2 * groups * 16 * 2 * (p.Dc + kLatentRope);
+    const int64_t rows = importance_rows(p);
+    auto of = [&](auto dc) {
+        constexpr int DC = decltype(dc)::value;
+        // (16 rows of 8 sequences of up to 31744 tokens: 23 us here, 5 + 46 below, which has half the tokens under way)
+        if (rows <= 16) {
+            latent_importance_few_kernel<DC><<<grid, dim3(kThreads), 0, st>>>(p);
+            return hipGetLastError();
+        }
+        latent_importance_queries_kernel<DC><<<dim3((unsigned)((rows + 31) / 32 * 2), p.seqs.n_seqs), dim3(kThreads), 0, st>>>(p);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        auto kernel = latent_importance_rows_kernel<DC>;
+        const int lds = 8 * QueryBlock<DC>::BYTES;
         (void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-        kernel<<<grid, dim3(kThreads * groups), lds, st>>>(p);
+        kernel<<<grid, dim3(2 * kThreads), lds, st>>>(p);
+        return hipGetLastError();
     };
-    if (p.Dc == 512) rows <= 16 ? go(latent_importance_kernel<512, 1>, 1) : go(latent_importance_kernel<512, 2>, 2);
-    else rows <= 16 ? go(latent_importance_kernel<256, 1>, 1) : go(latent_importance_kernel<256, 2>, 2);
-    return hipGetLastError();
+    return p.Dc == 512 ? of(std::integral_constant<int, 512>{}) : of(std::integral_constant<int, 256>{});
 }
 
 }  // namespace akv

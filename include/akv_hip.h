@@ -654,9 +654,12 @@ typedef struct akv_latent_importance_args {
     const float *scores;   /* [n_seqs] rows of n_scores, score_stride apart */
     float *out;            /* likewise, out_stride apart; scores itself, or no part of it */
     int64_t n_scores, score_stride, out_stride;
+    void *workspace;       /* akv_latent_importance_workspace_bytes (may be 0), 16-byte aligned */
+    int64_t workspace_bytes;
 } akv_latent_importance_args;
 
 /* As akv_paged_importance, over the latent cache. */
+int64_t akv_latent_importance_workspace_bytes(const akv_latent_importance_args *args);
 int akv_latent_importance(const akv_latent_importance_args *args, void *stream);
 
 /* As akv_paged_copy, over the latent cache. */

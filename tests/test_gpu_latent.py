@@ -440,6 +440,40 @@ def test_prefill_in_passes_of_heads(monkeypatch):
     assert float((got.float() - want.float()).abs().max()) <= 2.0 ** -10 * float(want.float().abs().max())
 
 
+def test_importance_of_many_rows_captured():
+    """A captured call, with a window and without, follows lengths, rows and tables that change."""
+    import akv
+    announce("latent importance, many rows, captured")
+    H, T = 9, 40
+    w = World(512, 16, [260, 90, 300], [20, 8, 12])
+    w.fill()
+    q, qr, _ = _queries(w, H, "bf16")
+    lse = akv.latent_attention(q, qr, w.pool, w.batch, _scale(), return_lse=True)[1]
+    table = w.batch.page_table.clone()
+    for window in (0, 5):
+        scores = torch.rand(3, 290, generator=torch.Generator().manual_seed(2)).cuda()
+        out = torch.empty_like(scores)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            akv.latent_importance(q, qr, lse, w.pool, w.batch, scores, _scale(), q_window=window, out=out)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            akv.latent_importance(q, qr, lse, w.pool, w.batch, scores, _scale(), q_window=window, out=out)
+        for lens, starts, hole in (([260, 90, 300], [0, 20, 28, 40], None), ([255, 8, 290], [0, 1, 21, 40], None),
+                                   ([0, 90, 128], [0, 0, 20, 23], (1, 2)), ([260, 90, 300], [0, 20, 28, 40], None)):
+            w.batch.kv_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+            w.batch.q_starts.copy_(torch.tensor(starts, dtype=torch.int32))
+            w.batch.page_table.copy_(table)
+            if hole:
+                w.batch.page_table[hole] = -1
+            out.fill_(-1.0)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, akv.latent_importance(q, qr, lse, w.pool, w.batch, scores, _scale(), q_window=window, out=torch.empty_like(out)))
+
+
 @pytest.mark.parametrize("Dc,P", FORMS)
 @pytest.mark.parametrize("H,kv,q,win", [(16, [517, 33], [1, 1], 0), (5, [130, 0, 64], [9, 0, 3], 4), (40, [300], [20], 0), (128, [200, 70], [1, 2], 1), (1, [31], [31], 0)])
 def test_importance(H, kv, q, win, Dc, P):

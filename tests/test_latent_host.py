@@ -72,6 +72,37 @@ def test_c_refusals(call):
         assert run(batch=dict(max_q=2 ** 20, n_tokens=2 ** 21, table_width=2 ** 16, table_stride=2 ** 16)) == (nat.AKV_E_SHAPE,)
 
 
+def test_c_importance_workspace():
+    """None for up to 16 rows a sequence, else blocks of 16 rows that hold every sequence's in pairs."""
+    from akv import _native as nat
+    lib = nat.load()
+
+    def args(H, T, max_q, S=2, window=0, Dc=512, **kw):
+        return nat.LatentImportanceArgs(abi_version=nat.ABI_VERSION, layer=0, pool=_pool(nat, latent_dim=Dc),
+                                        batch=_batch(nat, n_seqs=S, n_tokens=T, max_q=max_q), H=H, q_dtype=0, causal=1, sm_scale=0.1,
+                                        q=4096, q_t=4096, q_h=1024, q_rope=4096, q_rope_t=512, q_rope_h=128, lse=4096, q_window=window,
+                                        decay=0.9, scores=4096, out=4096, n_scores=10, score_stride=10, out_stride=10, **kw)
+
+    def need(*a, **kw):
+        return lib.akv_latent_importance_workspace_bytes(ctypes.byref(args(*a, **kw)))
+
+    assert need(16, 2, 1) == need(4, 8, 4) == need(4, 50, 30, window=4) == need(1, 16, 16) == 0
+    for H, T, q, window, Dc in ((17, 2, 1, 0, 512), (16, 3, 2, 0, 256), (3, 40, 33, 0, 512), (128, 64, 60, 7, 256), (1, 17, 17, 0, 512)):
+        block = 1024 * ((Dc + 64) // 32 + 1)
+        for lens in ((q, T - q), (T - q, q)):
+            at = 0
+            for s, n in enumerate(lens):  # a sequence's blocks lie before the next one's, the last one's inside
+                rows = min(n, window or n) * H
+                first = (s * min(window, q) if window else sum(lens[:s])) * H // 16 + 3 * s
+                assert first >= at
+                at = first + 2 * -(-rows // 32)
+            assert at * block <= need(H, T, q, window=window, Dc=Dc)
+    more = need(17, 2, 1)
+    for kw, want in ((dict(), nat.AKV_E_WORKSPACE), (dict(workspace=4096, workspace_bytes=more - 1), nat.AKV_E_WORKSPACE),
+                     (dict(workspace=4104, workspace_bytes=more), nat.AKV_E_ALIGN)):
+        assert lib.akv_latent_importance(ctypes.byref(args(17, 2, 1, **kw)), None) == want
+
+
 def test_c_refusals_of_moves():
     from akv import _native as nat
     lib = nat.load()
