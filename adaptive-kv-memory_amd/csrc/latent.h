@@ -58,7 +58,7 @@ struct LatentPrefillParams {
     int64_t *sums;             // the workspace: first costs of the sequences, partial states, keys, values
     float *part;
     unsigned char *keys, *values;  // [heads][cap] rows of kLatentHead float16
-    unsigned char *rest;       // what the values' float16 leave over, likewise; NULL for bfloat16 queries
+    int64_t rest;              // bytes from them to what their float16 leave over; 0 for bfloat16 queries: none
     int64_t cap, seq_cap;      // rows of a head, and of a sequence in it
     int head0, heads;          // those of this pass
     int groups, rows;          // workgroups, and the attention's query tokens of one

@@ -6,8 +6,8 @@
 // token and head, which some 170 query tokens outweigh.  Two kernels: the expansion is a matrix product
 // whose left side stays in LDS for all heads, the attention streams its results.  Keys and values are
 // float16 over a power of two for each channel (which goes to the queries and the outputs, so that small weights
-// keep their bits), query rows float16 scaled by a power of two, p one float16 (for float16 outputs p and values are
-// two); scores, sums and the softmax state are float32.
+// keep their bits), query rows float16 scaled by a power of two, p one float16; for float16 outputs keys, values and p are
+// two float16 each.  Scores, sums and the softmax state are float32.
 #include <algorithm>
 #include <type_traits>
 
@@ -22,10 +22,10 @@ constexpr int kD = kLatentHead;       // channels of a head's own keys, and of i
 constexpr int kThreads = 256;         // of the scan, the expansion and the merge
 constexpr int kAttendThreads = 512;
 constexpr int kExpandTok = 128;       // tokens of a workgroup of the expansion
-constexpr int kStep = 64;             // tokens of a step of the attention
-constexpr int kSetupTok = 2 * kStep;  // what an item's start counts
+constexpr int kSetupTok = 128;        // tokens that an item's start counts
 constexpr int kGroups = 256;
-
+// Tokens of a step of the attention: with two float16 each they are twice the bytes in LDS.
+__host__ __device__ constexpr int step_tokens(bool two) { return two ? 32 : 64; }
 
 struct TileScan {
     int64_t pre[kThreads + 1], wave_sum[kThreads / 64];
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_expand_kernel(const Latent
                 }
                 ((u4 *)(to + (int64_t)t * 16 * kD * 2))[0] = o[0];
                 ((u4 *)(to + (int64_t)t * 16 * kD * 2))[1] = o[1];
-                if (!p.rest || wave < 2) continue;
+                if (!p.rest) continue;
                 u4 rest[2];
 #pragma unroll
                 for (int b = 0; b < 4; ++b)
@@ -197,8 +197,8 @@ __global__ __launch_bounds__(kThreads, 1) void latent_expand_kernel(const Latent
                         const h2 high = as_h2(o[b >> 1][2 * (b & 1) + e]);
                         rest[b >> 1][2 * (b & 1) + e] = as_u32((h2){(_Float16)(acc[t][b][2 * e] - (float)high[0]), (_Float16)(acc[t][b][2 * e + 1] - (float)high[1])});
                     }
-                ((u4 *)(to - p.values + p.rest + (int64_t)t * 16 * kD * 2))[0] = rest[0];
-                ((u4 *)(to - p.values + p.rest + (int64_t)t * 16 * kD * 2))[1] = rest[1];
+                ((u4 *)(to + p.rest + (int64_t)t * 16 * kD * 2))[0] = rest[0];
+                ((u4 *)(to + p.rest + (int64_t)t * 16 * kD * 2))[1] = rest[1];
             }
         }
     }
@@ -226,13 +226,14 @@ __device__ __forceinline__ TileWork tile_work(const LatentPrefillParams &p, cons
     return w;
 }
 // Steps of tile t, and how many of them lie before cost c of it.
-template <int R>
+template <int R, int ST>
 __device__ __forceinline__ int steps_of(const LatentPrefillParams &p, const TileWork &w, int t) {
-    return (w.r.sees(p.causal, min((t + 1) * R, w.rows) - 1) + kStep - 1) / kStep;
+    return (w.r.sees(p.causal, min((t + 1) * R, w.rows) - 1) + ST - 1) / ST;
 }
+template <int ST>
 __device__ __forceinline__ int steps_before(int64_t c, int64_t cost, int steps) {
     if (c >= cost) return steps;
-    const int64_t x = (c - kSetupTok + kStep - 1) / kStep;
+    const int64_t x = (c - kSetupTok + ST - 1) / ST;
     return (int)(x < 0 ? 0 : x > steps ? steps : x);
 }
 template <int R>
@@ -242,7 +243,7 @@ __device__ __forceinline__ void scan_tiles(const LatentPrefillParams &p, TileSca
         return w.before(w.tiles) * p.heads;
     });
 }
-__device__ __forceinline__ int64_t share_of(int64_t total, int groups) { return max((total + groups - 1) / groups, (int64_t)(4 * kStep)); }
+__device__ __forceinline__ int64_t share_of(int64_t total, int groups) { return max((total + groups - 1) / groups, (int64_t)(2 * kSetupTok)); }
 
 // Value e of eight of a query row as float.
 template <bool BF16>
@@ -294,14 +295,19 @@ struct StepPages {
 // corners waste, at 1.7 GHz: the card's power holds the clock, and fewer cycles (17.5 to 14.3 million of all chiplets)
 // gave little time.  5 prompts of up to 777 tokens, 16 heads: 28 us, most of it an item's start and end.
 //
-// TWO, for float16 outputs: p and the values enter their product as two float16 each, without the product of both
-// rests, or their roundings would be larger than the output's own (a chunk that sees a few hundred tokens is 2.6e-4 of
-// the norm off, 3.6e-4 with one each, where the output's rounding alone is 2.1e-4).  For bfloat16 outputs one is
-// enough.  2 chunks of up to 1024 tokens, 64 heads: 2.4 ms, and 1.65 with one each.
+// TWO, for float16 outputs: keys, values and p enter their products as two float16 each (of p v without the product of
+// both rests), or their roundings would be larger than the output's own, 2.1e-4 of the norm.  One float16 for the keys
+// moves a score by 2^-12 of its size and more: with scores of standard deviation 1 and 4 outputs are 2.6e-4 and 4.4e-4 off,
+// single rows 1.9e-3; with two all are 2.1e-4, rows 2.7e-4.  For bfloat16 outputs, which round to 1.7e-3, one is
+// enough (1.68e-3 at deviation 1, 1.73e-3 at 4).  Steps have 32 tokens then, so that three slots fit LDS.  2 chunks of
+// up to 1024 tokens, 64 heads: 2.67 ms, 2.18 with one float16 for the keys, 1.51 with one for all.
 template <int DC, int RB, bool TWO>
 __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const LatentPrefillParams p) {
-    constexpr int NW = kAttendThreads / 64, R = 16 * RB * NW, SLOTS = 3, VB = kStep * kD * 2, KB = VB + kStep * kLatentRope * 2;
-    constexpr int K_LOADS = KB / 1024 / NW, V_LOADS = VB / 1024 / NW, CB = kD / 16, NI = (kD + kLatentRope) / 32, ROWB = 2 * (DC + kLatentRope);
+    constexpr int NW = kAttendThreads / 64, R = 16 * RB * NW, SLOTS = 3, ST = step_tokens(TWO), TT = ST / 16;
+    // a slot of keys: the heads' own channels, the rotated ones, the rest; of values: the values, the rest
+    constexpr int OWN = ST * kD * 2, ROPE = ST * kLatentRope * 2, KB = OWN + ROPE + (TWO ? OWN : 0), VB = OWN + (TWO ? OWN : 0);
+    constexpr int PIECES = OWN / 1024 / NW, V_LOADS = (TWO ? 2 : 1) * PIECES, K_LOADS = V_LOADS + 1;
+    constexpr int CB = kD / 16, NI = (kD + kLatentRope) / 32, ROWB = 2 * (DC + kLatentRope);
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ TileScan sc;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -313,7 +319,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
     const uint32_t k_off = grp * kD * 2 + ((col ^ grp) << 4), v_off = grp * kD * 2 + ((col ^ 2 * grp) << 4);
     const uint32_t r_off = (lane >> 3) * ROWB + 2 * DC + (((lane & 7) ^ grp) << 4);
     const uint32_t k_at = col * kD * 2 + ((grp ^ col) << 4);
-    const uint32_t r_at = VB + col * kLatentRope * 2 + ((grp ^ col >> 1) << 4);
+    const uint32_t r_at = OWN + col * kLatentRope * 2 + ((grp ^ col >> 1) << 4);
     const int vrow = 4 * grp + (col >> 2);
     const uint32_t v_at = vrow * kD * 2 + (((col & 3) >> 1 ^ 2 * (vrow & 7)) << 4) + 8 * (col & 1);
 
@@ -348,8 +354,8 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
     }
     while (x < x_end) {
         const int64_t cost = w.cost(tile), c1 = min(cost, c0 + (x_end - x));
-        const int steps_all = steps_of<R>(p, w, tile);
-        const int j0 = steps_before(c0, cost, steps_all), j1 = steps_before(c1, cost, steps_all);
+        const int steps_all = steps_of<R, ST>(p, w, tile);
+        const int j0 = steps_before<ST>(c0, cost, steps_all), j1 = steps_before<ST>(c1, cost, steps_all);
         const bool starts = c0 <= kSetupTok, ends = c1 == cost;
         x += c1 - c0;
         if (j1 > j0 || (starts && ends)) {
@@ -384,59 +390,51 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
             const int lp = p.pool.log_page;
             StepPages pages;
             const int64_t base = ((int64_t)h * p.cap + s * p.seq_cap) * kD * 2;
-            uint32_t there = 0;  // bits 4 slot ..
-            auto load_keys = [&](int j, int slot) {
-                const int k = j * kStep, end = j < j1 ? kv : 0;
-                const u4 rk = wave_rsrc(p.keys + base + (int64_t)k * kD * 2, max(0, min(end - k, kStep)) * kD * 2);
-                const uint32_t to_k = __builtin_amdgcn_readfirstlane(ring + slot * KB);
+            uint32_t there = 0;  // bits TT slot ..
+            auto load_own = [&](const unsigned char *from, int k, int end, uint32_t to, uint32_t off, int turns) {
+                const u4 rsrc = wave_rsrc(from + base + (int64_t)k * kD * 2, max(0, min(end - k, ST)) * kD * 2);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int n = 2 * wave + i;
-                    dma_kib(rk, to_k + n * 1024, (k_off ^ (n & 3) << 6) + n * 1024);
+                for (int i = 0; i < PIECES; ++i) {
+                    const int n = PIECES * wave + i;
+                    dma_kib(rsrc, to + n * 1024, (off ^ (turns == 4 ? (n & 3) << 6 : (n & 1) << 7)) + n * 1024);
                 }
+            };
+            auto load_keys = [&](int j, int slot) {
+                const int k = j * ST, end = j < j1 ? kv : 0;
+                const uint32_t to = __builtin_amdgcn_readfirstlane(ring + slot * KB);
+                load_own(p.keys, k, end, to, k_off, 4);
+                if (TWO) load_own(p.keys + p.rest, k, end, to + OWN + ROPE, k_off, 4);
                 const int page = k >> lp;
-                if (page + (48 >> lp) - pages.first >= 64) pages.fill(p, s, page);
+                if (page + ((ST - 16) >> lp) - pages.first >= 64) pages.fill(p, s, page);
                 const uint64_t valid = pages.valid >> (page - pages.first);
-                const uint32_t bits = (uint32_t)(valid & 1) | (uint32_t)(valid >> (16 >> lp) & 1) << 1 |
-                                      (uint32_t)(valid >> (32 >> lp) & 1) << 2 | (uint32_t)(valid >> (48 >> lp) & 1) << 3;
-                // the rotated keys of this wave's eight tokens
-                const int tok = k + 8 * wave, in = (tok >> lp) - pages.first;
+                uint32_t bits = 0;
+#pragma unroll
+                for (int i = 0; i < TT; ++i) bits |= (uint32_t)(valid >> (16 * i >> lp) & 1) << i;
+                // the rotated keys of eight tokens (of four waves the same as of the others where a step has 32)
+                const int eight = wave & (ST / 8 - 1), tok = k + 8 * eight, in = (tok >> lp) - pages.first;
                 const int rows = pages.valid >> in & 1 ? max(0, min(end - tok, 8)) : 0;
                 const unsigned char *rows_at = p.pool.base + (int64_t)__builtin_amdgcn_readlane(pages.ids, in) * p.pool.page_bytes +
                                                (int64_t)(tok & ((1 << lp) - 1)) * ROWB;
-                dma_kib(wave_rsrc(rows_at, rows * ROWB), to_k + VB + wave * 1024, r_off ^ (wave & 1) << 6);
-                there = (there & ~(15u << 4 * slot)) | bits << 4 * slot;
+                dma_kib(wave_rsrc(rows_at, rows * ROWB), to + OWN + eight * 1024, r_off ^ (eight & 1) << 6);
+                there = (there & ~(((1u << TT) - 1) << TT * slot)) | bits << TT * slot;
             };
             auto load_values = [&](int j, int slot) {
-                const int k = j * kStep, end = j < j1 ? kv : 0;
-                const u4 rv = wave_rsrc(p.values + base + (int64_t)k * kD * 2, max(0, min(end - k, kStep)) * kD * 2);
-                const uint32_t to_v = __builtin_amdgcn_readfirstlane(ring + SLOTS * KB + slot * VB);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int n = 2 * wave + i;
-                    dma_kib(rv, to_v + n * 1024, (v_off ^ (n & 1) << 7) + n * 1024);
-                }
-            };
-            auto load_rest = [&](int j, int slot) {
-                const int k = j * kStep, end = j < j1 ? kv : 0;
-                const u4 rv = wave_rsrc(p.rest + base + (int64_t)k * kD * 2, max(0, min(end - k, kStep)) * kD * 2);
-                const uint32_t to = __builtin_amdgcn_readfirstlane(ring + SLOTS * (KB + VB) + slot * VB);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int n = 2 * wave + i;
-                    dma_kib(rv, to + n * 1024, (v_off ^ (n & 1) << 7) + n * 1024);
-                }
+                const int k = j * ST, end = j < j1 ? kv : 0;
+                const uint32_t to = __builtin_amdgcn_readfirstlane(ring + SLOTS * KB + slot * VB);
+                load_own(p.values, k, end, to, v_off, 2);
+                if (TWO) load_own(p.values + p.rest, k, end, to + OWN, v_off, 2);
             };
             auto after = [](int slot) { return slot + 1 == SLOTS ? 0 : slot + 1; };
             float mx[RB], l[RB];
             f4 acc[CB][RB];
-            u4 P[2][RB], P_rest[2][RB];  // of 32 tokens each
+            u4 P[ST / 32][RB], P_rest[ST / 32][RB];  // of 32 tokens each
 #pragma unroll
             for (int r = 0; r < RB; ++r) {
                 mx[r] = kMinMax, l[r] = 0.0f;
 #pragma unroll
                 for (int b = 0; b < CB; ++b) acc[b][r] = (f4){0.f, 0.f, 0.f, 0.f};
-                P[0][r] = P[1][r] = P_rest[0][r] = P_rest[1][r] = (u4){0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < ST / 32; ++i) P[i][r] = P_rest[i][r] = (u4){0, 0, 0, 0};
             }
             constexpr int V_AHEAD = TWO ? 3 : 6, K_AHEAD = 8;  // reads that are under way
             auto value = [&](uint32_t va, int n) {
@@ -445,12 +443,12 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
                 return __builtin_bit_cast(h8, (u4){lo[0], lo[1], hi[0], hi[1]});
             };
             // p times the values; then(m) in the steps that read no more of them
-            auto add_values = [&](uint32_t va, uint32_t ra, auto then) {
-                constexpr int READS = 2 * CB;
+            auto add_values = [&](uint32_t va, auto then) {
+                constexpr int READS = ST / 32 * CB;
                 h8 V[V_AHEAD], V_rest[V_AHEAD];
                 auto read = [&](int n) {
                     V[n % V_AHEAD] = value(va, n);
-                    if (TWO) V_rest[n % V_AHEAD] = value(ra, n);
+                    if (TWO) V_rest[n % V_AHEAD] = value(va + OWN, n);
                 };
 #pragma unroll
                 for (int n = 0; n < V_AHEAD; ++n) read(n);
@@ -471,13 +469,13 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
                     __builtin_amdgcn_sched_barrier(0);
                 }
             };
-            const uint32_t values = ring + SLOTS * KB + v_at, rests = values + SLOTS * VB;
+            const uint32_t values = ring + SLOTS * KB + v_at;
             auto meet = [&]() {
                 wait_lgkm0();
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
             };
-            pages.fill(p, s, (j0 * kStep) >> lp);
+            pages.fill(p, s, (j0 * ST) >> lp);
             load_keys(j0, 0);
             load_keys(j0 + 1, 1);
             load_values(j0, 0);
@@ -485,7 +483,6 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
             int slot = 0;  // of step j, for keys and for values
             if (second) {
                 meet();
-                if (TWO) load_rest(j0, 0);
                 load_keys(j0 + 2, 2);
             }
             for (int j = j0; j < j1; ++j) {
@@ -495,43 +492,43 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
                 meet();
                 const int next = after(slot), last = after(next);
                 load_values(j + 1, next);
-                if (TWO && !second) load_rest(j, j - j0 & 1);
                 const uint32_t ka = ring + slot * KB + k_at, ra = ring + slot * KB + r_at;
                 auto key = [&](int n) {
-                    const int c = n >> 2, i = n & 3;
+                    const int c = n / TT, i = n % TT;
                     return __builtin_bit_cast(h8, *lds_ptr<u4>(c < kD / 32 ? (ka ^ c << 6) + i * 16 * kD * 2
-                                                                          : (ra ^ (c - kD / 32) << 6) + i * 16 * kLatentRope * 2));
+                                                               : c < NI    ? (ra ^ (c - kD / 32) << 6) + i * 16 * kLatentRope * 2
+                                                                           : (ka ^ (c - NI) << 6) + OWN + ROPE + i * 16 * kD * 2));
                 };
                 h8 K[K_AHEAD];
                 auto read_keys = [&](int from, int to) {
 #pragma unroll
                     for (int n = from; n < to; ++n) K[n] = key(n);
                 };
-                if (j > j0) add_values(values + last * VB, rests + (j - 1 - j0 & 1) * VB, [&](int m) { read_keys(m * K_AHEAD / V_AHEAD, (m + 1) * K_AHEAD / V_AHEAD); });
+                if (j > j0) add_values(values + last * VB, [&](int m) { read_keys(m * K_AHEAD / V_AHEAD, (m + 1) * K_AHEAD / V_AHEAD); });
                 else read_keys(0, K_AHEAD);
                 __builtin_amdgcn_sched_barrier(0);
-                f4 S[4][RB] = {};
+                f4 S[TT][RB] = {};
+                constexpr int READS = TT * (NI + (TWO ? kD / 32 : 0));  // the rest meets the same queries
 #pragma unroll
-                for (int n = 0; n < 4 * NI; ++n) {
+                for (int n = 0; n < READS; ++n) {
 #pragma unroll
-                    for (int r = 0; r < RB; ++r) S[n & 3][r] = mfma_k32(K[n % K_AHEAD], Q[r][n >> 2], S[n & 3][r]);
-                    if (n + K_AHEAD < 4 * NI) K[n % K_AHEAD] = key(n + K_AHEAD);
+                    for (int r = 0; r < RB; ++r) S[n % TT][r] = mfma_k32(K[n % K_AHEAD], Q[r][n / TT % NI], S[n % TT][r]);
+                    if (n + K_AHEAD < READS) K[n % K_AHEAD] = key(n + K_AHEAD);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                const int first = j * kStep;
-                const uint32_t have = there >> 4 * slot & 15;
+                const int first = j * ST;
+                const uint32_t have = there >> TT * slot & ((1u << TT) - 1);
                 meet();
                 if (second) {
-                    if (TWO) load_rest(j + 1, j + 1 - j0 & 1);
                     load_keys(j + 3, slot);
                 } else {
                     load_keys(j + 2, last);
                 }
-                if (!(first + kStep <= see_all && have == 15)) {
+                if (!(first + ST <= see_all && have == (1u << TT) - 1)) {
                     int at0 = first + 4 * grp;
                     asm volatile("" : "+v"(at0));  // (nothing of this is computed where nothing is masked)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                    for (int i = 0; i < TT; ++i)
 #pragma unroll
                         for (int r = 0; r < RB; ++r)
 #pragma unroll
@@ -544,7 +541,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
                 for (int r = 0; r < RB; ++r) {
                     top[r] = S[0][r][0];
 #pragma unroll
-                    for (int i = 1; i < 16; ++i) top[r] = __builtin_fmaxf(top[r], S[i >> 2][r][i & 3]);
+                    for (int i = 1; i < 4 * TT; ++i) top[r] = __builtin_fmaxf(top[r], S[i >> 2][r][i & 3]);
                     over |= __builtin_fmaf(top[r], kx[r], kBias - mx[r]) > kBias + kLagBy;
                 }
                 if (__builtin_amdgcn_ballot_w64(over)) {
@@ -562,7 +559,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
 #pragma unroll
                 for (int r = 0; r < RB; ++r)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < TT; ++i) {
                         float e[4];
 #pragma unroll
                         for (int q = 0; q < 4; ++q) e[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i][r][q], kx[r], kBias - mx[r]));
@@ -578,7 +575,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
             }
             wait_vm<0>();
             meet();
-            if (j1 > j0) add_values(values + (slot == 0 ? SLOTS - 1 : slot - 1) * VB, rests + (j1 - 1 - j0 & 1) * VB, [](int) {});
+            if (j1 > j0) add_values(values + (slot == 0 ? SLOTS - 1 : slot - 1) * VB, [](int) {});
             if (!second) meet();
             float *e = p.part + ((int64_t)blockIdx.x * 2 + starts) * (R * (kD + 2));
 #pragma unroll
@@ -621,7 +618,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void latent_prefill_kernel(const
 
 // Joins the partial states of items that several workgroups share: a wave takes 16 rows of one.  Bound by the
 // states' bytes: 10 us for 5 prompts of up to 777 tokens, 16 heads.
-template <int R>
+template <int R, int ST>
 __global__ __launch_bounds__(kThreads) void latent_prefill_merge_kernel(const LatentPrefillParams p) {
     constexpr int CB = kD / 16;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
@@ -646,12 +643,12 @@ __global__ __launch_bounds__(kThreads) void latent_prefill_merge_kernel(const La
     };
     const int g0 = run_of(start), g1 = run_of(start + cost - 1);
     if (g0 == g1) return;
-    const int steps = steps_of<R>(p, w, tile);
+    const int steps = steps_of<R, ST>(p, w, tile);
     // the runs that hold steps of it, and whether a run's entry is the one whose item starts there
     auto part = [&](int g, int64_t &c0) {
         c0 = max((int64_t)0, g * share - start);
         const int64_t c1 = min(cost, (g + 1) * share - start);
-        return steps_before(c1, cost, steps) > steps_before(c0, cost, steps);
+        return steps_before<ST>(c1, cost, steps) > steps_before<ST>(c0, cost, steps);
     };
     auto entry = [&](int g, int64_t c0) { return p.part + ((int64_t)g * 2 + (c0 <= kSetupTok)) * (R * (kD + 2)); };
     float m = kMinMax, l = 0.0f;
@@ -696,7 +693,7 @@ int64_t part_bytes(const LatentPrefillParams &p) { return (int64_t)p.groups * 2 
 int64_t latent_prefill_plan(LatentPrefillParams *p) {
     p->seq_cap = (int64_t)p->seqs.width << p->pool.log_page;
     p->cap = p->seq_cap * p->seqs.n_seqs;
-    const int64_t head = std::max<int64_t>(1, p->cap * (p->q_bf16 ? 2 : 3) * kD * 2);
+    const int64_t head = std::max<int64_t>(1, p->cap * (p->q_bf16 ? 2 : 4) * kD * 2);
     p->heads = (int)std::max<int64_t>(1, std::min<int64_t>(p->H, kMostBytes / head));
     // 256 query tokens a workgroup where there are tiles of them for all, else 128 (attention and merge of 5
     // prompts of up to 777, 16 heads: 48 us as 256, 39 as 128; 2 chunks of up to 1024, 64 heads: 1.08 and 1.40 ms)
@@ -712,15 +709,16 @@ hipError_t latent_prefill_launch(const LatentPrefillParams &p0, hipStream_t st) 
     p.part = (float *)at;
     p.keys = at + part_bytes(p);
     p.values = p.keys + p.heads * p.cap * kD * 2;
-    p.rest = p.q_bf16 ? nullptr : p.values + p.heads * p.cap * kD * 2;
+    p.rest = p.q_bf16 ? 0 : p.heads * p.cap * 2 * kD * 2;
     const int most = p.heads;
     if (p.pool.n_pages == 0) p.seqs.width = 0;
     auto of = [&](auto dc, auto rb, auto two) {
         constexpr int DC = decltype(dc)::value, RB = decltype(rb)::value, R = 128 * RB;
         constexpr bool TWO = decltype(two)::value;
+        constexpr int ST = step_tokens(TWO);
         auto expand = latent_expand_kernel<DC>;
         auto attend = latent_prefill_kernel<DC, RB, TWO>;
-        const int lds_e = kExpandTok * 2 * DC, lds_a = kStep * (3 * (4 * kD + 2 * kLatentRope) + (TWO ? 4 * kD : 0));
+        const int lds_e = kExpandTok * 2 * DC, lds_a = 3 * ST * ((TWO ? 8 : 4) * kD + 2 * kLatentRope);
         (void)hipFuncSetAttribute((const void *)expand, hipFuncAttributeMaxDynamicSharedMemorySize, lds_e);
         (void)hipFuncSetAttribute((const void *)attend, hipFuncAttributeMaxDynamicSharedMemorySize, lds_a);
         for (p.head0 = 0; p.head0 < p.H; p.head0 += most) {
@@ -732,7 +730,7 @@ hipError_t latent_prefill_launch(const LatentPrefillParams &p0, hipStream_t st) 
             e = hipGetLastError();
             if (e != hipSuccess) return e;
             const int64_t blocks = ((int64_t)p.seqs.max_q + R - 1) / R * (R / 64);
-            latent_prefill_merge_kernel<R><<<dim3((unsigned)blocks, p.heads, p.seqs.n_seqs), dim3(kThreads), 0, st>>>(p);
+            latent_prefill_merge_kernel<R, ST><<<dim3((unsigned)blocks, p.heads, p.seqs.n_seqs), dim3(kThreads), 0, st>>>(p);
             e = hipGetLastError();
             if (e != hipSuccess) return e;
         }
