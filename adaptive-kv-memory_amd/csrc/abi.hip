@@ -1252,7 +1252,7 @@ static int latent_attn_params(const akv_latent_attn_args *a, akv::LatentAttnPara
     p->scale_log2 = a->sm_scale * 1.4426950408889634f;
     p->q = (const unsigned char *)a->q; p->qr = (const unsigned char *)a->q_rope;
     p->q_t = a->q_t; p->q_h = a->q_h; p->qr_t = a->q_rope_t; p->qr_h = a->q_rope_h;
-    p->out = a->out; p->lse = a->lse; p->sums = (int *)a->workspace;
+    p->out = a->out; p->lse = a->lse; p->joins = (akv::LatentJoin *)a->workspace;
     *bytes = akv::latent_attn_plan(p);
     return AKV_OK;
 }

@@ -29,6 +29,12 @@ struct LatentRowsParams {
     int64_t latent_t, rope_t;
 };
 
+// What the merge joins where a run begins inside an item: rows [row0, rows) of a sequence's, in the runs g0 to g1.
+struct LatentJoin {
+    int begin, rows, row0;
+    uint16_t g0, g1;
+};
+
 struct LatentAttnParams {
     LatentView pool;
     PagedSeqs seqs;
@@ -38,7 +44,7 @@ struct LatentAttnParams {
     int64_t q_t, q_h, qr_t, qr_h;
     void *out;
     float *lse;
-    int *sums;                 // the workspace: first units of the sequences, then partial states
+    LatentJoin *joins;         // the workspace: one of every run, then partial states
     float *part;
     int groups, log_tile;      // workgroups, log2 of the rows of one
     FastDiv by_heads, by_groups;

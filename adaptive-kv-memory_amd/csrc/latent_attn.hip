@@ -91,10 +91,6 @@ __device__ __forceinline__ int scan_seqs(const LatentAttnParams &p, Scan &sc) {
         for (int w = 0; w < kThreads / 64; ++w) inc += w < wave ? sc.wave_sum[w] : 0;
         sc.pre[t] = inc - mine;
         if (t == kThreads - 1) sc.pre[kThreads] = inc;
-        if (blockIdx.x == 0) {  // for the merge
-            p.sums[t] = inc - mine;
-            if (t == kThreads - 1) p.sums[kThreads] = inc;
-        }
     }
     __syncthreads();
     return __builtin_amdgcn_readfirstlane(sc.pre[kThreads]);
@@ -128,6 +124,19 @@ __device__ __forceinline__ Run run_of(const LatentAttnParams &p, const Scan &sc,
         ++r.s;
     }
     return r;
+}
+// The item that the run's first unit lies in, for the merge, where the run before it holds units of it too
+// (an item's first kSetup are none).
+__device__ __forceinline__ void note_join(const LatentAttnParams &p, const Run &r, int total) {
+    if (threadIdx.x != 0) return;
+    const int g = blockIdx.x, share = share_of(p, total);
+    LatentJoin j{};
+    if (r.x < r.x_end) {
+        const int tile = r.off / r.w.cost, start = r.x - (r.off - tile * r.w.cost);
+        const int g0 = (start + kSetup) / share, g1 = (start + r.w.cost - 1) / share;
+        if (g0 < g) j = LatentJoin{r.w.r.begin, r.w.rows, tile << p.log_tile, (uint16_t)g0, (uint16_t)g1};
+    }
+    p.joins[g] = j;
 }
 // The next item's part of the run; false at the end.
 __device__ __forceinline__ bool next_item(const LatentAttnParams &p, const Scan &sc, Run &r, Item &it) {
@@ -178,7 +187,9 @@ __global__ __launch_bounds__(kThreads, 2) void latent_few_kernel(const LatentAtt
     const int vrow = 4 * grp + (col >> 2);
     const uint32_t v_at = vrow * ROWB + ((((col & 3) >> 1) ^ turn(vrow)) << 4) + 8 * (col & 1);
 
-    Run run = run_of(p, sc, scan_seqs(p, sc));
+    const int total = scan_seqs(p, sc);
+    Run run = run_of(p, sc, total);
+    note_join(p, run, total);
     Item it;
     while (next_item(p, sc, run, it)) {
         const Work &w = run.w;
@@ -341,7 +352,9 @@ __global__ __launch_bounds__(512, 2) void latent_rows_kernel(const LatentAttnPar
     const uint32_t ring = lds_addr(smem), p_ring = ring + SLOTS * F::SLOT + group * 4096;
     for (int i = wave; i < T::PIECES; i += 8) offsets[i][threadIdx.x & 63] = (uint16_t)T::offset(i, threadIdx.x & 63);
 
-    Run run = run_of(p, sc, scan_seqs(p, sc));
+    const int total = scan_seqs(p, sc);
+    Run run = run_of(p, sc, total);
+    note_join(p, run, total);
     Item it;
     while (next_item(p, sc, run, it)) {
         const Work &w = run.w;
@@ -554,69 +567,64 @@ __global__ __launch_bounds__(512, 2) void latent_rows_kernel(const LatentAttnPar
     }
 }
 
-// Joins the partial states of items that several workgroups share: a workgroup takes two of the
-// 16-channel blocks of 16 rows, each of its waves every fourth state.  Bound by the states' bytes where they are
-// many (16 us for 128 rows of 40 sequences: 67 MB), else by its loads' chain (4.4 us for one of 517 tokens).
+// Joins the partial states of items that several workgroups share.  Every run but the first that begins inside an item
+// has workgroups here, and the runs of an item divide its parts, two 16-channel blocks of 16 rows each: there are at most
+// 255 such runs, whatever sequences and rows a call has.  Each of a workgroup's waves takes every fourth state.
+// Bound by the states' bytes where they are many (16 us for 128 rows of 40 sequences: 67 MB), else by its loads'
+// chain (4.4 us for one of 517 tokens).
 template <int DC, int ROWS>
 __global__ __launch_bounds__(kThreads) void latent_merge_kernel(const LatentAttnParams p) {
-    constexpr int NB = DC / 16, PER = 2, SPLIT = NB / PER;
+    constexpr int NB = DC / 16, PER = 2, SPLIT = NB / PER, PARTS = ROWS / 16 * SPLIT;
     __shared__ __align__(16) f4 sums[kWaves][PER][64];
     __shared__ float ms[kWaves][16], ls[kWaves][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
-    const int s = blockIdx.y, b0 = blockIdx.x % SPLIT * PER, block = blockIdx.x / SPLIT;
-    const int tile = block / (ROWS / 16), r = block % (ROWS / 16);
-    const int per = seqs_per(p);
-    const Work w = seq_work(p, wave_uniform(seq_rows(p.seqs, s, p.pool.log_page)));
-    const int row0 = tile * ROWS + 16 * r;
-    if (tile >= w.tiles || row0 >= w.rows) return;
-    int start = p.sums[s / per] + tile * w.cost;
-    for (int i = s / per * per; i < s; ++i) {
-        const Work b = seq_work(p, wave_uniform(seq_rows(p.seqs, i, p.pool.log_page)));
-        start += b.tiles * b.cost;
-    }
-    const int share = share_of(p, p.sums[kThreads]);
-    // the runs that hold units of the item (its first kSetup are none)
-    const int g0 = (start + kSetup) / share, g1 = (start + w.cost - 1) / share;
-    if (g0 == g1) return;
-    float m = kMinMax;
-    for (int g = g0 + wave + kWaves * grp; g <= g1; g += 4 * kWaves)
-        m = __builtin_fmaxf(m, entry_of<DC, ROWS>(p, g, g == g0)[ROWS * DC + 16 * r + col]);
-    m = qmax(m);
-    float l = 0.0f;
-    f4 acc[PER];
+    const LatentJoin j = p.joins[blockIdx.y + 1];
+    const int g0 = j.g0, g1 = j.g1, nth = (int)blockIdx.y - g0;
+    for (int part = nth * (int)gridDim.x + (int)blockIdx.x; part < PARTS; part += (g1 - g0) * (int)gridDim.x) {
+        const int r = part / SPLIT, b0 = part % SPLIT * PER;
+        if (j.row0 + 16 * r >= j.rows) return;  // (also where there is no item: rows 0)
+        float m = kMinMax;
+        for (int g = g0 + wave + kWaves * grp; g <= g1; g += 4 * kWaves)
+            m = __builtin_fmaxf(m, entry_of<DC, ROWS>(p, g, g == g0)[ROWS * DC + 16 * r + col]);
+        m = qmax(m);
+        float l = 0.0f;
+        f4 acc[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = (f4){0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < PER; ++i) acc[i] = (f4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int g = g0 + wave; g <= g1; g += kWaves) {
-        const float *e = entry_of<DC, ROWS>(p, g, g == g0);
-        const float a = __builtin_amdgcn_exp2f(e[ROWS * DC + 16 * r + col] - m);
-        l += e[ROWS * DC + ROWS + 16 * r + col] * a;
+        for (int g = g0 + wave; g <= g1; g += kWaves) {
+            const float *e = entry_of<DC, ROWS>(p, g, g == g0);
+            const float a = __builtin_amdgcn_exp2f(e[ROWS * DC + 16 * r + col] - m);
+            l += e[ROWS * DC + ROWS + 16 * r + col] * a;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) acc[i] += *(const f4 *)(e + (r * NB + b0 + i) * 256 + lane * 4) * a;
+            for (int i = 0; i < PER; ++i) acc[i] += *(const f4 *)(e + (r * NB + b0 + i) * 256 + lane * 4) * a;
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) sums[wave][i][lane] = acc[i];
+        if (grp == 0) ms[wave][col] = m, ls[wave][col] = l;
+        __syncthreads();
+        const int row = j.row0 + 16 * r + col;
+        if (wave < PER && row < j.rows) {
+            float mx = ms[0][col];
+#pragma unroll
+            for (int i = 1; i < kWaves; ++i) mx = __builtin_fmaxf(mx, ms[i][col]);
+            f4 o = {0.f, 0.f, 0.f, 0.f};
+            l = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kWaves; ++i) {
+                const float a = __builtin_amdgcn_exp2f(ms[i][col] - mx);
+                l += ls[i][col] * a;
+                o += sums[i][wave][lane] * a;
+            }
+            const int qt = (int)fast_div(row, p.by_heads), h = row - qt * p.H;
+            const int64_t at = (int64_t)(j.begin + qt) * p.H + h;
+            o *= row_inverse(l);
+            *(u2 *)((unsigned char *)p.out + at * (2 * DC) + 32 * (b0 + wave) + 8 * grp) =
+                (u2){out_pair(p.q_bf16, o[0], o[1]), out_pair(p.q_bf16, o[2], o[3])};
+            if (p.lse && grp == 0 && b0 + wave == 0) p.lse[at] = row_lse(mx, l, kBias);
+        }
+        __syncthreads();
     }
-#pragma unroll
-    for (int i = 0; i < PER; ++i) sums[wave][i][lane] = acc[i];
-    if (grp == 0) ms[wave][col] = m, ls[wave][col] = l;
-    __syncthreads();
-    if (wave >= PER) return;
-    float mx = ms[0][col];
-#pragma unroll
-    for (int i = 1; i < kWaves; ++i) mx = __builtin_fmaxf(mx, ms[i][col]);
-    f4 o = {0.f, 0.f, 0.f, 0.f};
-    l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-        const float a = __builtin_amdgcn_exp2f(ms[i][col] - mx);
-        l += ls[i][col] * a;
-        o += sums[i][wave][lane] * a;
-    }
-    const int row = row0 + col;
-    if (row >= w.rows) return;
-    const int qt = (int)fast_div(row, p.by_heads), h = row - qt * p.H;
-    const int64_t at = (int64_t)(w.r.begin + qt) * p.H + h;
-    o *= row_inverse(l);
-    *(u2 *)((unsigned char *)p.out + at * (2 * DC) + 32 * (b0 + wave) + 8 * grp) = (u2){out_pair(p.q_bf16, o[0], o[1]), out_pair(p.q_bf16, o[2], o[3])};
-    if (p.lse && grp == 0 && b0 + wave == 0) p.lse[at] = row_lse(mx, l, kBias);
 }
 
 // The importance: sum over rows and heads of 2^(s - lse), for 32 tokens a wave, whose rows stay in
@@ -899,8 +907,7 @@ __global__ __launch_bounds__(2 * kThreads, 2) void latent_importance_rows_kernel
 }
 
 namespace {
-constexpr int64_t kSumsBytes = 2048;
-static_assert((kThreads + 1) * 4 <= kSumsBytes, "the sums fit");
+constexpr int64_t kJoinBytes = kGroups * (int64_t)sizeof(LatentJoin);
 }  // namespace
 
 int64_t latent_attn_plan(LatentAttnParams *p) {
@@ -913,22 +920,21 @@ int64_t latent_attn_plan(LatentAttnParams *p) {
     p->groups = (int)std::max<int64_t>(1, std::min<int64_t>(kGroups, units * tiles * p->seqs.n_seqs));
     p->by_heads = make_fast_div((uint32_t)p->H);
     p->by_groups = make_fast_div((uint32_t)p->groups);
-    return kSumsBytes + ((int64_t)p->groups * 2 * (p->Dc + 2) * 4 << p->log_tile);
+    return kJoinBytes + ((int64_t)p->groups * 2 * (p->Dc + 2) * 4 << p->log_tile);
 }
 
 hipError_t latent_attn_launch(const LatentAttnParams &p0, hipStream_t st) {
     LatentAttnParams p = p0;
     if (p.seqs.n_seqs == 0 || p.seqs.max_q == 0) return hipSuccess;
     if (p.pool.n_pages == 0) p.seqs.width = 0;
-    p.part = (float *)((unsigned char *)p.sums + kSumsBytes);
+    p.part = (float *)((unsigned char *)p.joins + kJoinBytes);
     auto go = [&](auto kern, auto merge, int threads, int lds) {
         (void)hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         kern<<<dim3(p.groups), dim3(threads), lds, st>>>(p);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess || p.groups == 1) return e;
-        const int64_t tiles = ((int64_t)p.seqs.max_q * p.H + (1 << p.log_tile) - 1) >> p.log_tile;
-        const dim3 grid((unsigned)((tiles << (p.log_tile - 4)) * (p.Dc / 32)), p.seqs.n_seqs);
-        merge<<<grid, dim3(kThreads), 0, st>>>(p);
+        const int parts = (p.Dc / 32) << (p.log_tile - 4);
+        merge<<<dim3(std::min(32, parts / 2), p.groups - 1), dim3(kThreads), 0, st>>>(p);
         return hipGetLastError();
     };
     auto of = [&](auto dc) {
