@@ -1244,9 +1244,6 @@ static int latent_attn_params(const akv_latent_attn_args *a, akv::LatentAttnPara
     if (rc != AKV_OK) return rc;
     rc = check_latent_queries(a->H, a->q_dtype, a->sm_scale, a->batch, a->q, a->q_rope, a->q_t | a->q_h | a->q_rope_t | a->q_rope_h);
     if (rc != AKV_OK) return rc;
-    // units of 64 tokens of a tile of at least 16 rows, and a few for an item, are counted in 31 bits
-    const double cap = (double)a->batch.table_width * a->pool.page_size, rows = (double)a->batch.max_q * a->H;
-    if ((cap / 64 + 8) * (rows / 16 + 1) * a->batch.n_seqs >= 0x1p30) return fail(AKV_E_SHAPE, "too much for one call");
     p->Dc = a->pool.latent_dim; p->H = a->H;
     p->q_bf16 = a->q_dtype == AKV_DT_BF16; p->causal = a->causal != 0;
     p->scale_log2 = a->sm_scale * 1.4426950408889634f;
@@ -1254,6 +1251,9 @@ static int latent_attn_params(const akv_latent_attn_args *a, akv::LatentAttnPara
     p->q_t = a->q_t; p->q_h = a->q_h; p->qr_t = a->q_rope_t; p->qr_h = a->q_rope_h;
     p->out = a->out; p->lse = a->lse; p->joins = (akv::LatentJoin *)a->workspace;
     *bytes = akv::latent_attn_plan(p);
+    // units of 64 tokens of a tile of rows, and a few for an item, are counted in 31 bits
+    const double cap = (double)a->batch.table_width * a->pool.page_size, rows = (double)a->batch.max_q * a->H;
+    if ((cap / 64 + 8) * (rows / (1 << p->log_tile) + 1) * a->batch.n_seqs >= 0x1p30) return fail(AKV_E_SHAPE, "too much for one call");
     return AKV_OK;
 }
 

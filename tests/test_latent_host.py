@@ -72,6 +72,24 @@ def test_c_refusals(call):
         assert run(batch=dict(max_q=2 ** 20, n_tokens=2 ** 21, table_width=2 ** 16, table_stride=2 ** 16)) == (nat.AKV_E_SHAPE,)
 
 
+def test_c_attention_counts_units_of_its_tiles():
+    """A wide table and a chunk in a batch: refused where the units of the tiles that the call takes pass 2^30, not before."""
+    from akv import _native as nat
+    lib = nat.load()
+
+    def need(S, q, H, tokens):
+        a = nat.LatentAttnArgs(abi_version=nat.ABI_VERSION, layer=0, pool=_pool(nat, page_size=64), H=H, q_dtype=1, causal=1, sm_scale=0.1,
+                               batch=_batch(nat, n_seqs=S, n_tokens=S * q, max_q=q, table_width=tokens // 64, table_stride=tokens // 64),
+                               q=4096, q_t=4096, q_h=1024, q_rope=4096, q_rope_t=512, q_rope_h=128, out=4096)
+        return lib.akv_latent_attn_workspace_bytes(ctypes.byref(a))
+    # units (with eight for an item) times tiles of 128, 64 and 16 rows times sequences
+    for S, q, H, tokens, tile in ((256, 512, 128, 131072, 128), (4096, 1, 64, 2 ** 22, 64), (8000, 1, 16, 2 ** 22, 16), (1, 2 ** 19, 128, 65536, 128)):
+        units = (tokens // 64 + 8) * (q * H // tile + 1) * S
+        assert (need(S, q, H, tokens) > 0) == (units < 2 ** 30), (S, q, H, tokens)
+        more = 2 * 2 ** 30 // units + 1
+        assert need(min(65535, S * more), q, H, tokens) == -1
+
+
 def test_c_importance_workspace():
     """None for up to 16 rows a sequence, else blocks of 16 rows that hold every sequence's in pairs."""
     from akv import _native as nat
