@@ -1177,6 +1177,9 @@ static int check_latent_pool(const akv_latent_pool &p) {
     return AKV_OK;
 }
 
+// Rows that a launch of eight lanes a row holds: 2^32 work items and more wrap.
+constexpr int64_t kMostMoved = ((int64_t)1 << 29) - 32;
+
 static akv::LatentView latent_view(const akv_latent_pool &p, int32_t layer) {
     const int row = 2 * (p.latent_dim + p.rope_dim);
     const int64_t page = (int64_t)p.page_size * row;
@@ -1199,6 +1202,7 @@ static int latent_rows_params(const akv_latent_rows_args *a, akv::LatentRowsPara
     const int rc = latent_views(a->abi_version, a->layer, a->pool, a->batch, &p->pool, &p->seqs);
     if (rc != AKV_OK) return rc;
     if (a->dtype < 0 || a->dtype > 2) return fail(AKV_E_DTYPE, "float16, bfloat16 or float32 rows");
+    if (a->batch.n_tokens > kMostMoved) return fail(AKV_E_SHAPE, "more than %lld rows in a call", (long long)kMostMoved);
     if (a->batch.n_tokens > 0 && (!a->latent || !a->rope)) return fail(AKV_E_INVALID, "latent and rope are required");
     if (!aligned16(a->latent) || !aligned16(a->rope) || ((a->latent_t | a->rope_t) & 15))
         return fail(AKV_E_ALIGN, "rows must be 16-byte aligned");
@@ -1347,7 +1351,7 @@ int akv_latent_importance(const akv_latent_importance_args *a, void *stream) {
     int64_t bytes;
     const int rc = latent_importance_params(a, &p, &bytes);
     if (rc != AKV_OK) return rc;
-    if (a->n_scores < 0 || a->n_scores >= ((int64_t)1 << 31) ||
+    if (a->n_scores < 0 || a->n_scores > kMostMoved ||
         (a->batch.n_seqs > 1 && (a->score_stride < a->n_scores || a->out_stride < a->n_scores)))
         return fail(AKV_E_SHAPE, "bad score rows");
     if (a->batch.n_seqs == 0 || a->n_scores == 0) return ok();
@@ -1383,7 +1387,7 @@ int akv_latent_compact(const akv_latent_compact_args *a, void *stream) {
     const int rc = check_latent_pool(a->pool);
     if (rc != AKV_OK) return rc;
     if (a->n_seqs < 0 || a->n_seqs > 65535) return fail(AKV_E_SHAPE, "0 to 65535 sequences");
-    if (a->src_width < 0 || a->dst_width < 0 || a->max_keep < 0 || a->max_keep >= ((int64_t)1 << 31) ||
+    if (a->src_width < 0 || a->dst_width < 0 || a->max_keep < 0 || a->max_keep > kMostMoved ||
         (a->n_seqs > 1 && (a->src_stride < a->src_width || a->dst_stride < a->dst_width || a->keep_stride < a->max_keep)))
         return fail(AKV_E_SHAPE, "bad tables");
     if ((int64_t)a->src_width * a->pool.page_size >= ((int64_t)1 << 31) ||

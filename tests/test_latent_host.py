@@ -143,6 +143,25 @@ def test_c_refusals_of_moves():
     assert lib.akv_latent_compact(None, None) == nat.AKV_E_INVALID
 
 
+def test_c_refusals_of_launches_that_wrap():
+    """2^32 work items are none to the runtime: rows, scores and positions that would take as many are refused."""
+    from akv import _native as nat
+    lib = nat.load()
+    for n in (2 ** 29 - 31, 2 ** 29, 2 ** 30, 2 ** 31 - 1):
+        a = nat.LatentRowsArgs(abi_version=nat.ABI_VERSION, layer=0, dtype=0, pool=_pool(nat), batch=_batch(nat, n_tokens=n, max_q=1),
+                               latent=4096, rope=4096, latent_t=0, rope_t=0)
+        assert lib.akv_latent_append(ctypes.byref(a), None) == lib.akv_latent_read(ctypes.byref(a), None) == nat.AKV_E_SHAPE
+        c = nat.LatentCompactArgs(abi_version=nat.ABI_VERSION, n_seqs=1, pool=_pool(nat), src_table=4096, dst_table=4096, src_stride=4,
+                                  dst_stride=4, src_width=4, dst_width=4, keep=4096, n_keep=4096, keep_stride=n, max_keep=n)
+        assert lib.akv_latent_compact(ctypes.byref(c), None) == nat.AKV_E_SHAPE
+        for H in (4, 40):
+            i = nat.LatentImportanceArgs(abi_version=nat.ABI_VERSION, layer=0, pool=_pool(nat), batch=_batch(nat, n_seqs=1, n_tokens=1, max_q=1),
+                                         H=H, q_dtype=0, causal=1, sm_scale=0.1, q=4096, q_t=4096, q_h=1024, q_rope=4096, q_rope_t=512,
+                                         q_rope_h=128, lse=4096, q_window=0, decay=0.9, scores=4096, out=4096, n_scores=n, score_stride=n,
+                                         out_stride=n)
+            assert lib.akv_latent_importance(ctypes.byref(i), None) == nat.AKV_E_SHAPE
+
+
 def test_c_refusals_of_evictions():
     from akv import _native as nat
     lib = nat.load()
