@@ -506,8 +506,13 @@ class _PagedCache:
 
     # ---- batches
     def _upload(self, *rows: List[int]) -> List[torch.Tensor]:
-        """Lists of integers as int32 tensors on the device, with one copy."""
-        flat = torch.tensor([x for r in rows for x in r], dtype=torch.int32).to(self.pool.data.device)
+        """Lists of integers as int32 tensors on the device, with one copy that the host does not wait for: pinned
+        memory, which torch's allocator holds until the copy has ended."""
+        device = self.pool.data.device
+        pinned = device.type == "cuda"
+        if pinned and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a cache's books cannot be captured: each replay would upload what they said at the capture")
+        flat = torch.tensor([x for r in rows for x in r], dtype=torch.int32, pin_memory=pinned).to(device, non_blocking=True)
         return list(flat.split([len(r) for r in rows]))
 
     def _table(self, page_lists) -> Tuple[List[int], int]:
