@@ -589,7 +589,10 @@ class _PagedCache:
         sequence's length: the running importance of their tokens.  Returns it for the tokens that stay, at
         their new positions and 0 behind them.
 
-        Nothing waits for the device.  Tokens move as in ``compact``; sequences within the budget stay as they are."""
+        Nothing waits for the device.  Tokens move as in ``compact``, to fresh pages, in turns where need be; sequences
+        within the budget stay as they are.  So a full pool is not relieved: it raises, and changes nothing, where the
+        free pages do not hold one sequence's budget (``ceil(budget / page_size)``) at a time.  Keep as many free, or evict
+        before ``extend`` finds none."""
         book = self._book
         book._known(seqs)
         budget, lens = index(budget), [book.lens[s] for s in seqs]

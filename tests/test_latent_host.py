@@ -291,3 +291,20 @@ def test_eviction_in_turns_and_refusals(monkeypatch):
     with pytest.raises(RuntimeError, match="launch"):
         c.evict(seqs, scores, 16)
     assert [list(c._book.pages[s]) for s in seqs] == before and c.num_free_pages == free and [c.get_seq_length(s) for s in seqs] == lens
+
+
+def test_eviction_needs_a_budget_of_free_pages(monkeypatch):
+    """What stays moves to fresh pages: with none, or one too few, it raises and nothing changes; with as many as one
+    sequence's budget takes, all sequences move in turns."""
+    lens = [64, 48, 64]                                       # 4 + 3 + 4 pages
+    for free in range(4):
+        pp, c, seqs, moved = _cache(monkeypatch, lens, pages=11 + free)
+        monkeypatch.setattr(pp, "evict_select", lambda s, n, b, f, l: (torch.arange(b, dtype=torch.int32).expand(3, b), None, s))
+        before = [list(c._book.pages[s]) for s in seqs]
+        if free < 3:
+            with pytest.raises(RuntimeError, match="exhausted"):
+                c.evict(seqs, torch.zeros(3, 64), 40)         # 3 pages
+            assert [list(c._book.pages[s]) for s in seqs] == before and c.num_free_pages == free and not moved
+        else:
+            c.evict(seqs, torch.zeros(3, 64), 40)
+            assert len(moved) == 3 and [c.get_seq_length(s) for s in seqs] == [40, 40, 40] and c.num_free_pages == 14 - 9
