@@ -51,7 +51,9 @@ def limits(want, dtype):
     """Rounding the outputs leaves `own` of their norm, and at most half a step of any row's.  What comes before it
     may add a quarter of that in quadrature (1.03 in all): for float16 5.1e-5, where 300 tokens and one float16 for keys,
     values or p add 1.2e-4 and more, and float32 sums some 1e-5; for bfloat16 4.1e-4, where one float16 for all three and scores of
-    standard deviation 1 add 2.3e-4.  A row's part of what comes before may be larger than the whole's: a quarter of a
+    standard deviation 1 add 2.3e-4.  In quadrature means over many outputs: with errors r of the rounding and d before it,
+    |r + d|^2 has a cross term 2 r.d that differs from 0 by 2 |r| |d| / sqrt(N), for 256 outputs and d = 0.15 r 2% of |r|^2 at one
+    standard deviation, for 25600 0.2%; so the norm is a whole call's.  A row's part of what comes before may be larger than the whole's: a quarter of a
     half step is granted."""
     own = off(want.to(dtype).double(), want)[0]
     return 1.03 * own, 1.25 * torch.finfo(dtype).eps / 2
