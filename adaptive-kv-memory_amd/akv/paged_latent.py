@@ -143,7 +143,8 @@ def latent_attention(q: torch.Tensor, q_rope: torch.Tensor, pool: PagedLatentPoo
     ``sm_scale`` is that of the heads' own keys (their channels are not the latent's).  With ``causal``, row i of a
     sequence's m rows sees its first kv_len - m + 1 + i tokens, else all of them; a row that sees none is 0.
     ``return_lse`` adds the log-sums of exp(scores) (n_tokens, H) float32, -inf for such rows.  Scores, sums and
-    log-sums are float32; the weights are rounded to float16."""
+    log-sums are float32; the weights are rounded to float16 (in float16 calls of up to 16 rows a sequence, a token's heads
+    each one, to two)."""
     q, qt, qh, qr, qrt, qrh = _queries(q, q_rope, pool, batch)
     T, H, D = q.shape
     lib = nat.load()
@@ -192,8 +193,8 @@ def latent_prefill(q: torch.Tensor, pool: PagedLatentPool, batch: PagedBatch, we
 
     ``sm_scale`` is by default one over the root of q's channels.  Rows see what they do in ``latent_attention``.
     Keys and values are float16, by channel over 16 times the power of two above its largest weight and clamped to +-65504
-    there, and so are the weights of the sums; for float16 queries all three are two float16 each.  Keys and values are made
-    for as many heads at a time as 4 GiB of workspace hold, and for as many tokens of a sequence as its row of the page table
+    there, and so are the weights of the sums; for float16 queries all three are two float16 each, and a key or value is
+    held within twice that.  Keys and values are made for as many heads at a time as 4 GiB of workspace hold, and for as many tokens of a sequence as its row of the page table
     has slots."""
     _check_device(pool, q, batch.page_table, weights.data)
     if q.dtype not in _QUERY:

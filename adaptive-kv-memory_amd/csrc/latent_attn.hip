@@ -5,7 +5,8 @@
 // rotated key r) is the key of every head and its latent the value: s = q.c + q_r.r, o = sum of p c.
 // The rows of all heads and query tokens of a sequence thus share one stream of cached rows.  A float16 query
 // row enters as it is, a bfloat16 one as float16 after scaling by a power of two to a maximum in [2^13, 2^14),
-// which leaves with the softmax scale; scores are exact but for float32 sums.  p is one float16.
+// which leaves with the softmax scale; scores are exact but for float32 sums and, in bfloat16 rows, values below 2^-28
+// of the row's largest.  p is one float16, for float16 outputs of up to 16 rows a sequence two.
 // Softmax state: running maximum and sum per row in float32.
 #include <algorithm>
 #include <type_traits>
@@ -168,10 +169,13 @@ __device__ __forceinline__ float *entry_of(const LatentAttnParams &p, int group,
 // lengths, pages, loads and its join, which is all of the 14 us of one sequence of 517.  (In the form for more rows:
 // 87 us.)
 //
+// TWO, for float16 outputs: p is two float16, which memory hides (71.5 us against 71 for the sequences above): one leaves
+// outputs up to 2.4e-4 of their norm off, where their own rounding is 2.1e-4.
+//
 // Each of the four waves takes 16 tokens at a time for all 16 rows, from two buffers of LDS of its own
 // that buffer loads fill; nothing is shared until the waves join at an item's end.  What is run once for an item is
 // kept short: the code comes from memory too.
-template <int DC>
+template <int DC, bool TWO>
 __global__ __launch_bounds__(kThreads, 2) void latent_few_kernel(const LatentAttnParams p) {
     using T = Rows16<DC>;
     constexpr int NI = Row<DC>::NI, NB = DC / 16, ROWB = T::ROWB, SLOTS = 2;
@@ -253,7 +257,11 @@ __global__ __launch_bounds__(kThreads, 2) void latent_few_kernel(const LatentAtt
 #pragma unroll
             for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], kx, kBias - mx));
             l += (e[0] + e[1]) + (e[2] + e[3]);
-            const h4 P = {(_Float16)e[0], (_Float16)e[1], (_Float16)e[2], (_Float16)e[3]};  // 2^-12 of a weight
+            const h4 P = {(_Float16)e[0], (_Float16)e[1], (_Float16)e[2], (_Float16)e[3]};
+            h4 rest;
+            if constexpr (TWO)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) rest[i] = (_Float16)(e[i] - (float)P[i]);
             const uint32_t va = at + v_at;
             constexpr int AHEAD = 4;  // reads that are under way
             u2 V[AHEAD];
@@ -262,6 +270,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_few_kernel(const LatentAtt
             for (int b = 0; b < AHEAD; ++b) V[b] = value(b);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
+                if constexpr (TWO) acc[b] = mfma_k16(__builtin_bit_cast(h4, V[b % AHEAD]), rest, acc[b]);
                 acc[b] = mfma_k16(__builtin_bit_cast(h4, V[b % AHEAD]), P, acc[b]);
                 if (b + AHEAD < NB) V[b % AHEAD] = value(b + AHEAD);
                 __builtin_amdgcn_sched_barrier(0);
@@ -458,7 +467,9 @@ __global__ __launch_bounds__(512, 2) void latent_rows_kernel(const LatentAttnPar
                         alphas[group][16 * wg + col] = 1.0f;
                     }
                     if (lane == 0) flags[group][wg] = over;
-                    u4 P;  // one float16 each: 2^-12 of a weight
+                    // One float16 each, for float16 outputs too: 2.3e-4 of the norm off where the output's own rounding is
+                    // 2.1e-4; the rest would be 8 KB more, and LDS is full.
+                    u4 P;
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         float e[4];
@@ -940,7 +951,9 @@ hipError_t latent_attn_launch(const LatentAttnParams &p0, hipStream_t st) {
     auto of = [&](auto dc) {
         constexpr int DC = decltype(dc)::value;
         using F = RowsForm<DC>;
-        if (p.log_tile == 4) return go(latent_few_kernel<DC>, latent_merge_kernel<DC, 16>, kThreads, 2 * kWaves * Rows16<DC>::BYTES);
+        const int few = 2 * kWaves * Rows16<DC>::BYTES;
+        if (p.log_tile == 4 && p.q_bf16) return go(latent_few_kernel<DC, false>, latent_merge_kernel<DC, 16>, kThreads, few);
+        if (p.log_tile == 4) return go(latent_few_kernel<DC, true>, latent_merge_kernel<DC, 16>, kThreads, few);
         if (p.log_tile == 6) return go(latent_rows_kernel<DC, true>, latent_merge_kernel<DC, 64>, 512, F::LDS);
         return go(latent_rows_kernel<DC, false>, latent_merge_kernel<DC, 128>, 512, F::LDS);
     };

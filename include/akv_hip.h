@@ -633,8 +633,8 @@ typedef struct akv_latent_prefill_args {
 } akv_latent_prefill_args;
 
 /* Attention in its expanded form: a head's keys are (W_k latent, rope) and its values W_v latent, made
- * in the workspace as float16 (without w_scale, clamped to +-65504; for float16 queries as two float16 each) and then
- * attended to.  Rows that see no token: 0.
+ * in the workspace as float16 (without w_scale, clamped to +-65504; for float16 queries as two float16 each, each
+ * clamped) and then attended to.  Rows that see no token: 0.
  * Calls that share a workspace must not overlap. */
 int64_t akv_latent_prefill_workspace_bytes(const akv_latent_prefill_args *args);
 int akv_latent_prefill(const akv_latent_prefill_args *args, void *stream);

@@ -1,4 +1,4 @@
-"""The expanded form's precision by norms: the output's own rounding and little beside it, whole and
+"""The latent attention's precision by norms: the output's own rounding and little beside it, whole and
 row by row."""
 import pytest
 import torch
@@ -6,7 +6,7 @@ import torch
 import latent_norms as ln
 import latent_ref as ref
 from gpu_util import announce
-from test_gpu_latent import DT, World, _randn, _scale
+from test_gpu_latent import DT, World, _queries, _randn, _scale
 
 pytestmark = pytest.mark.gpu
 
@@ -51,6 +51,22 @@ def test_bfloat16(H, kv, m, Dc, P):
     w = World(Dc, P, [kv], [m])
     w.fill()
     _check(w, H, "bf16", 1.0, torch.arange(H)[:: max(1, H // 5)])
+
+
+@pytest.mark.parametrize("H,kv,m,Dc,P", [(16, 300, 1, 512, 64), (8, 300, 2, 256, 16), (16, 4000, 1, 512, 16), (1, 700, 16, 512, 64)])
+def test_absorbed_float16_of_few_rows(H, kv, m, Dc, P):
+    """p as two float16: the output's own rounding alone, as the plain formula has it."""
+    import akv
+    announce(f"latent attention precision, float16: H={H} kv={kv} m={m} Dc={Dc}")
+    S = 12
+    w = World(Dc, P, [kv + i for i in range(S)], [m] * S)
+    w.fill()
+    q, qr, x = _queries(w, H, "fp16")
+    out = akv.latent_attention(q, qr, w.pool, w.batch, _scale()).double().cpu()
+    want = torch.cat([ref.attention(x[w.mine(s), :, :Dc], x[w.mine(s), :, Dc:], w.rows(s), _scale(), 0.0)[0] for s in range(S)])
+    got, most = ln.off(out, want), ln.limits(want, torch.float16)
+    print(f"off by {got[0]:.3e} (limit {most[0]:.3e}), rows {got[1]:.3e} ({most[1]:.3e})", flush=True)
+    assert got[0] <= most[0] and got[1] <= most[1]
 
 
 def _ragged(n, most, seed):
