@@ -143,8 +143,7 @@ def latent_attention(q: torch.Tensor, q_rope: torch.Tensor, pool: PagedLatentPoo
     ``sm_scale`` is that of the heads' own keys (their channels are not the latent's).  With ``causal``, row i of a
     sequence's m rows sees its first kv_len - m + 1 + i tokens, else all of them; a row that sees none is 0.
     ``return_lse`` adds the log-sums of exp(scores) (n_tokens, H) float32, -inf for such rows.  Scores, sums and
-    log-sums are float32; the weights are rounded to float16 (in float16 calls of up to 16 rows a sequence, a token's heads
-    each one, to two)."""
+    log-sums are float32; the weights are rounded to float16, for float16 queries to 14 bits or more."""
     q, qt, qh, qr, qrt, qrh = _queries(q, q_rope, pool, batch)
     T, H, D = q.shape
     lib = nat.load()

@@ -6,7 +6,7 @@
 // The rows of all heads and query tokens of a sequence thus share one stream of cached rows.  A float16 query
 // row enters as it is, a bfloat16 one as float16 after scaling by a power of two to a maximum in [2^13, 2^14),
 // which leaves with the softmax scale; scores are exact but for float32 sums and, in bfloat16 rows, values below 2^-28
-// of the row's largest.  p is one float16, for float16 outputs of up to 16 rows a sequence two.
+// of the row's largest.  p is one float16 for bfloat16 outputs (an eighth of their own half step), two for float16.
 // Softmax state: running maximum and sum per row in float32.
 #include <algorithm>
 #include <type_traits>
@@ -54,18 +54,21 @@ __device__ __forceinline__ int share_of(const LatentAttnParams &p, int total) {
 }
 
 // The sequences of a call in LDS: where their units lie (pre[i]: the first unit of sequence i * per,
-// pre[256] the total), and up to 256 sequences their rows.
+// pre[256] the total), and up to KEPT sequences their rows (256 or none).
+template <int KEPT>
 struct Scan {
     int pre[kThreads + 1];
     int wave_sum[kThreads / 64];
-    SeqRows rows[kThreads];
+    SeqRows rows[KEPT ? KEPT : 1];
 };
 __device__ __forceinline__ int seqs_per(const LatentAttnParams &p) { return p.seqs.n_seqs <= kThreads ? 1 : (p.seqs.n_seqs + kThreads - 1) / kThreads; }
-__device__ __forceinline__ SeqRows rows_of(const LatentAttnParams &p, const Scan &sc, int s) {
-    return wave_uniform(p.seqs.n_seqs <= kThreads ? sc.rows[s] : seq_rows(p.seqs, s, p.pool.log_page));
+template <int KEPT>
+__device__ __forceinline__ SeqRows rows_of(const LatentAttnParams &p, const Scan<KEPT> &sc, int s) {
+    return wave_uniform(p.seqs.n_seqs <= KEPT ? sc.rows[s] : seq_rows(p.seqs, s, p.pool.log_page));
 }
 // For workgroups of 256 threads or more; the total.
-__device__ __forceinline__ int scan_seqs(const LatentAttnParams &p, Scan &sc) {
+template <int KEPT>
+__device__ __forceinline__ int scan_seqs(const LatentAttnParams &p, Scan<KEPT> &sc) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, n = p.seqs.n_seqs, per = seqs_per(p);
     int mine = 0, inc = 0;
     if (t < kThreads) {
@@ -75,7 +78,7 @@ __device__ __forceinline__ int scan_seqs(const LatentAttnParams &p, Scan &sc) {
                 const SeqRows r = seq_rows(p.seqs, s, p.pool.log_page);
                 const Work w = seq_work(p, r);
                 mine += w.tiles * w.cost;
-                if (per == 1) sc.rows[t] = r;
+                if (KEPT && per == 1) sc.rows[t] = r;
             }
         }
         inc = mine;
@@ -106,7 +109,8 @@ struct Item {
     int tile, j0, j1;
     bool starts, ends;
 };
-__device__ __forceinline__ Run run_of(const LatentAttnParams &p, const Scan &sc, int total) {
+template <int KEPT>
+__device__ __forceinline__ Run run_of(const LatentAttnParams &p, const Scan<KEPT> &sc, int total) {
     const int lane = threadIdx.x & 63, per = seqs_per(p), share = share_of(p, total);
     Run r{};
     r.x = (int)min((int64_t)blockIdx.x * share, (int64_t)total);
@@ -140,7 +144,8 @@ __device__ __forceinline__ void note_join(const LatentAttnParams &p, const Run &
     p.joins[g] = j;
 }
 // The next item's part of the run; false at the end.
-__device__ __forceinline__ bool next_item(const LatentAttnParams &p, const Scan &sc, Run &r, Item &it) {
+template <int KEPT>
+__device__ __forceinline__ bool next_item(const LatentAttnParams &p, const Scan<KEPT> &sc, Run &r, Item &it) {
     if (r.x >= r.x_end) return false;
     while (r.off == r.w.tiles * r.w.cost) {
         r.off = 0;
@@ -182,7 +187,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_few_kernel(const LatentAtt
     constexpr int OWN = NB / kWaves;  // blocks of channels that a wave joins and writes
     static_assert(NB * 1024 <= SLOTS * T::BYTES, "a wave's sums fit its buffers");
     extern __shared__ __align__(1024) unsigned char smem[];
-    __shared__ Scan sc;
+    __shared__ Scan<kThreads> sc;
     __shared__ float ms[kWaves][16], ls[kWaves][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
@@ -335,6 +340,10 @@ __global__ __launch_bounds__(kThreads, 2) void latent_few_kernel(const LatentAtt
 // has a wave for the softmax and one for the matrix cores.  A barrier ends each such half step: when it opens,
 // what one group leaves in LDS for itself is there, and so are the rows that are needed next.  SPLIT: both groups
 // take the same 64 rows, and every other step each; they join at an item's end.  Else 128 rows.
+// TWO, for float16 outputs: what p's float16 leave over follows as bytes, five bits of exponent and two of mantissa (the
+// upper halves of float16; 4 KB, where LDS has no 8 left), and the values are read again for it.  p is then off by
+// 2^-14 of itself, and outputs by their own rounding, 2.05e-4 of the norm (2.4e-4 with one float16), for 79 us
+// instead of 67 (9 sequences of up to 16385 tokens, 1 to 5 query tokens of 64 heads).
 // 40 sequences of up to 9001 tokens, 128 heads (41 GFLOP): 79 us, and 16 for the merge.  Neither MFMAs (busy 28% of
 // the cycles) nor LDS (24%, no conflicts) bound it but what a half step of 32 tokens does one after
 // the other: read, multiply, softmax, write p, meet.  Splitting 128 rows of so few sequences over all compute units costs
@@ -343,22 +352,22 @@ template <int DC>
 struct RowsForm {
     static constexpr int KS = 32, CB = DC / 64, SLOTS = 4;
     static constexpr int SLOT = 2 * Rows16<DC>::BYTES, PIECES = Rows16<DC>::PIECES, LOADS = (PIECES + 3) / 4;
-    static constexpr int LDS = SLOTS * SLOT + 8 * 1024;  // the rows, p of both groups
+    static constexpr int LDS = SLOTS * SLOT + 8 * 1024, LDS_TWO = LDS + 4 * 1024;  // the rows, p of both groups, its rest
     static_assert(4 * CB * 4 * 1024 <= SLOTS * SLOT, "a group's sums fit the buffers");
 };
-template <int DC, bool SPLIT>
+template <int DC, bool SPLIT, bool TWO>
 __global__ __launch_bounds__(512, 2) void latent_rows_kernel(const LatentAttnParams p) {
     using F = RowsForm<DC>;
     using T = Rows16<DC>;
     constexpr int NI = Row<DC>::NI, ROWB = T::ROWB, ROWS = SPLIT ? 64 : 128, CB = F::CB, SLOTS = F::SLOTS, RB = 4;
     extern __shared__ __align__(1024) unsigned char smem[];
-    __shared__ Scan sc;
+    __shared__ Scan<TWO ? 0 : kThreads> sc;
     __shared__ float alphas[2][64];
     __shared__ __align__(16) int flags[2][4];
     __shared__ int miss[SLOTS][2];               // whether a tile of 16 tokens has no page
     __shared__ uint16_t offsets[T::PIECES][64];  // what a lane loads of a piece: in LDS, registers are scarce
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = wave >> 2, wg = wave & 3;
-    const uint32_t ring = lds_addr(smem), p_ring = ring + SLOTS * F::SLOT + group * 4096;
+    const uint32_t ring = lds_addr(smem), p_ring = ring + SLOTS * F::SLOT + group * 4096, rest_ring = ring + F::LDS + group * 2048;
     for (int i = wave; i < T::PIECES; i += 8) offsets[i][threadIdx.x & 63] = (uint16_t)T::offset(i, threadIdx.x & 63);
 
     const int total = scan_seqs(p, sc);
@@ -467,18 +476,27 @@ __global__ __launch_bounds__(512, 2) void latent_rows_kernel(const LatentAttnPar
                         alphas[group][16 * wg + col] = 1.0f;
                     }
                     if (lane == 0) flags[group][wg] = over;
-                    // One float16 each, for float16 outputs too: 2.3e-4 of the norm off where the output's own rounding is
-                    // 2.1e-4; the rest would be 8 KB more, and LDS is full.
                     u4 P;
+                    u2 rest;
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         float e[4];
 #pragma unroll
                         for (int q = 0; q < 4; ++q) e[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[k][q], kx, kBias - mx));
                         l += (e[0] + e[1]) + (e[2] + e[3]);
-                        P[2 * k] = as_u32((h2){(_Float16)e[0], (_Float16)e[1]});
-                        P[2 * k + 1] = as_u32((h2){(_Float16)e[2], (_Float16)e[3]});
+                        int bytes = 0;
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            const h2 high = {(_Float16)e[2 * q], (_Float16)e[2 * q + 1]};
+                            P[2 * k + q] = as_u32(high);
+                            if constexpr (TWO) {
+                                const float x = e[2 * q] - (float)high[0], y = e[2 * q + 1] - (float)high[1];
+                                bytes = q ? __builtin_amdgcn_cvt_pk_bf8_f32(x, y, bytes, true) : __builtin_amdgcn_cvt_pk_bf8_f32(x, y, bytes, false);
+                            }
+                        }
+                        rest[k] = (uint32_t)bytes;
                     }
+                    if constexpr (TWO) *lds_mut<u2>(rest_ring + lane * 8 + wg * 512) = rest;
                     *lds_mut<u4>(p_at + wg * 1024) = P;
                 } else {
                     const int vrow = 4 * grp + (col >> 2);
@@ -505,11 +523,20 @@ __global__ __launch_bounds__(512, 2) void latent_rows_kernel(const LatentAttnPar
                         }
                     }
                     __builtin_amdgcn_sched_barrier(0);
+                    constexpr int READS = (TWO ? 2 : 1) * CB;  // the rest of p meets the same values
 #pragma unroll
-                    for (int b = 0; b < CB; ++b) {
+                    for (int n = 0; n < READS; ++n) {
+                        const int b = n % CB;
+                        if (n == CB)
 #pragma unroll
-                        for (int r = 0; r < RB; ++r) acc[r][b] = mfma_k32(V[b % AHEAD], P[r], acc[r][b]);
-                        if (b + AHEAD < CB) V[b % AHEAD] = value(b + AHEAD);
+                            for (int r = 0; r < RB; ++r) {  // the upper bytes of float16
+                                const u2 w = *lds_ptr<u2>(rest_ring + lane * 8 + r * 512);
+                                P[r] = __builtin_bit_cast(h8, (u4){__builtin_amdgcn_perm(w[0], w[0], 0x010c000cu), __builtin_amdgcn_perm(w[0], w[0], 0x030c020cu),
+                                                                   __builtin_amdgcn_perm(w[1], w[1], 0x010c000cu), __builtin_amdgcn_perm(w[1], w[1], 0x030c020cu)});
+                            }
+#pragma unroll
+                        for (int r = 0; r < RB; ++r) acc[r][b] = mfma_k32(V[n % AHEAD], P[r], acc[r][b]);
+                        if (n + AHEAD < READS) V[n % AHEAD] = value((n + AHEAD) % CB);
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
@@ -954,8 +981,12 @@ hipError_t latent_attn_launch(const LatentAttnParams &p0, hipStream_t st) {
         const int few = 2 * kWaves * Rows16<DC>::BYTES;
         if (p.log_tile == 4 && p.q_bf16) return go(latent_few_kernel<DC, false>, latent_merge_kernel<DC, 16>, kThreads, few);
         if (p.log_tile == 4) return go(latent_few_kernel<DC, true>, latent_merge_kernel<DC, 16>, kThreads, few);
-        if (p.log_tile == 6) return go(latent_rows_kernel<DC, true>, latent_merge_kernel<DC, 64>, 512, F::LDS);
-        return go(latent_rows_kernel<DC, false>, latent_merge_kernel<DC, 128>, 512, F::LDS);
+        if (p.q_bf16) {
+            if (p.log_tile == 6) return go(latent_rows_kernel<DC, true, false>, latent_merge_kernel<DC, 64>, 512, F::LDS);
+            return go(latent_rows_kernel<DC, false, false>, latent_merge_kernel<DC, 128>, 512, F::LDS);
+        }
+        if (p.log_tile == 6) return go(latent_rows_kernel<DC, true, true>, latent_merge_kernel<DC, 64>, 512, F::LDS_TWO);
+        return go(latent_rows_kernel<DC, false, true>, latent_merge_kernel<DC, 128>, 512, F::LDS_TWO);
     };
     return p.Dc == 512 ? of(std::integral_constant<int, 512>{}) : of(std::integral_constant<int, 256>{});
 }

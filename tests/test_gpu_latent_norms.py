@@ -53,8 +53,10 @@ def test_bfloat16(H, kv, m, Dc, P):
     _check(w, H, "bf16", 1.0, torch.arange(H)[:: max(1, H // 5)])
 
 
-@pytest.mark.parametrize("H,kv,m,Dc,P", [(16, 300, 1, 512, 64), (8, 300, 2, 256, 16), (16, 4000, 1, 512, 16), (1, 700, 16, 512, 64)])
-def test_absorbed_float16_of_few_rows(H, kv, m, Dc, P):
+@pytest.mark.parametrize("H,kv,m,Dc,P", [(16, 300, 1, 512, 64), (8, 300, 2, 256, 16), (16, 4000, 1, 512, 16), (1, 700, 16, 512, 64),
+                                         (40, 300, 1, 512, 64), (64, 4000, 1, 512, 16), (32, 900, 2, 256, 32), (128, 300, 1, 512, 32),
+                                         (128, 3000, 1, 256, 16), (16, 500, 40, 512, 64)])
+def test_absorbed_float16(H, kv, m, Dc, P):
     """p as two float16: the output's own rounding alone, as the plain formula has it."""
     import akv
     announce(f"latent attention precision, float16: H={H} kv={kv} m={m} Dc={Dc}")
