@@ -170,11 +170,11 @@ __device__ __forceinline__ float *entry_of(const LatentAttnParams &p, int group,
 }  // namespace
 
 // Up to 16 rows a sequence (a token's heads).  Bound by the cache's bytes: 24 sequences of up to 65536 tokens
-// and 16 heads (269 MB) take 62 us, of which the memory's rate is 49 and the rest an item's chain of
-// lengths, pages, loads and its join, which is all of the 14 us of one sequence of 517.  (In the form for more rows:
+// and 16 heads (269 MB) take 60 us, of which the memory's rate is 49 and the rest an item's chain of
+// lengths, pages, loads and its join, which is all of the 13 us of one sequence of 517.  (In the form for more rows:
 // 87 us.)
 //
-// TWO, for float16 outputs: p is two float16, which memory hides (71.5 us against 71 for the sequences above): one leaves
+// TWO, for float16 outputs: p is two float16, which memory hides (calls of 71.5 against 71 us for the sequences above): one leaves
 // outputs up to 2.4e-4 of their norm off, where their own rounding is 2.1e-4.
 //
 // Each of the four waves takes 16 tokens at a time for all 16 rows, from two buffers of LDS of its own
@@ -344,7 +344,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_few_kernel(const LatentAtt
 // upper halves of float16; 4 KB, where LDS has no 8 left), and the values are read again for it.  p is then off by
 // 2^-14 of itself, and outputs by their own rounding, 2.05e-4 of the norm (2.4e-4 with one float16), for 79 us
 // instead of 67 (9 sequences of up to 16385 tokens, 1 to 5 query tokens of 64 heads).
-// 40 sequences of up to 9001 tokens, 128 heads (41 GFLOP): 79 us, and 16 for the merge.  Neither MFMAs (busy 28% of
+// 40 sequences of up to 9001 tokens, 128 heads (41 GFLOP), bfloat16: 72 us, and 22 for the merge.  Neither MFMAs (busy 28% of
 // the cycles) nor LDS (24%, no conflicts) bound it but what a half step of 32 tokens does one after
 // the other: read, multiply, softmax, write p, meet.  Splitting 128 rows of so few sequences over all compute units costs
 // 67 MB of partial states written and read.
@@ -608,8 +608,8 @@ __global__ __launch_bounds__(512, 2) void latent_rows_kernel(const LatentAttnPar
 // Joins the partial states of items that several workgroups share.  Every run but the first that begins inside an item
 // has workgroups here, and the runs of an item divide its parts, two 16-channel blocks of 16 rows each: there are at most
 // 255 such runs, whatever sequences and rows a call has.  Each of a workgroup's waves takes every fourth state.
-// Bound by the states' bytes where they are many (16 us for 128 rows of 40 sequences: 67 MB), else by its loads'
-// chain (4.4 us for one of 517 tokens).
+// Bound by the states' bytes where they are many (22 us for 128 rows of 40 sequences: 67 MB), else by its loads'
+// chain (4.0 us for one of 517 tokens).
 template <int DC, int ROWS>
 __global__ __launch_bounds__(kThreads) void latent_merge_kernel(const LatentAttnParams p) {
     constexpr int NB = DC / 16, PER = 2, SPLIT = NB / PER, PARTS = ROWS / 16 * SPLIT;
