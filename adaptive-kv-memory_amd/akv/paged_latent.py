@@ -192,9 +192,9 @@ def latent_prefill(q: torch.Tensor, pool: PagedLatentPool, batch: PagedBatch, we
 
     ``sm_scale`` is by default one over the root of q's channels.  Rows see what they do in ``latent_attention``.
     Keys and values are float16, by channel over 16 times the power of two above its largest weight and clamped to +-65504
-    there, and so are the weights of the sums; for float16 queries all three are two float16 each, and a key or value is
-    held within twice that.  Keys and values are made for as many heads at a time as 4 GiB of workspace hold, and for as many tokens of a sequence as its row of the page table
-    has slots."""
+    there; the attention weights are float16 too.  For float16 queries all of them are two float16 each (and the clamp is twice
+    as wide).  Keys and values are made for as many heads at a time as 4 GiB of workspace hold, and for as many tokens of a
+    sequence as its row of the page table has slots."""
     _check_device(pool, q, batch.page_table, weights.data)
     if q.dtype not in _QUERY:
         raise TypeError("latent attention takes float16 or bfloat16 queries")
